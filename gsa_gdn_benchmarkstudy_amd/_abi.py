@@ -45,9 +45,27 @@ EXPORTS = (
     "gsa_selected_attn", "gsa_selected_attn_workspace_bytes", "gsa_masked_attn", "gsa_masked_attn_workspace_bytes",
     "gsa_dense_attn_split_bytes", "gsa_layer_attn", "gsa_layer_workspace_bytes",
     "gsa_rope_qk",
+    "gsa_rms_norm", "gsa_rms_norm_fp8", "gsa_rms_norm_backward", "gsa_rms_norm_backward_workspace_bytes",
+    "gsa_delta_step", "gsa_delta_rule", "gsa_delta_rule_backward", "gsa_delta_rule_workspace_bytes",
+    "gsa_delta_rule_saved_bytes",
 )
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+
+
+
+class DeltaArgs(ctypes.Structure):
+    """gsa_delta_args of include/gsa_hip.h."""
+
+    _fields_ = ([(n, _vp) for n in ("q", "k", "v", "g", "beta")]
+                + [(f"{n}_{s}", _i64) for n in ("q", "k", "v", "g", "beta") for s in ("sb", "st", "sh")]
+                + [("cu_seqlens", _vp)]
+                + [(n, _i32) for n in ("cu_bytes", "B", "T", "N", "Hk", "Hv", "d", "dtype", "beta_dtype")]
+                + [("scale", _f32), ("state_in", _vp), ("o", _vp), ("state_out", _vp), ("ws", _vp),
+                   ("ws_bytes", ctypes.c_size_t), ("saved", _vp), ("saved_bytes", ctypes.c_size_t), ("dout", _vp)]
+                + [(n, _i64) for n in ("do_sb", "do_st", "do_sh")]
+                + [(n, _vp) for n in ("dstate_out", "dq", "dk", "dv", "dg", "dbeta", "dstate_in")])
+
 
 _PROTOS = {
     "gsa_abi_version": ([], _i32),
@@ -105,6 +123,17 @@ _PROTOS = {
     "gsa_proj_pack": ([_vp, _i64, _vp, _i32, _i32, _i32, _vp, _vp, _vp], _i32),
     "gsa_proj_fused": ([_vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64,
                         _vp, _i64, _vp, _i64, _vp, _vp, _i32, _vp], _i32),
+    "gsa_rms_norm": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _f32, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp], _i32),
+    "gsa_rms_norm_fp8": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _f32, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp], _i32),
+    "gsa_rms_norm_backward_workspace_bytes": ([_i64, _i32], ctypes.c_size_t),
+    "gsa_rms_norm_backward": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _i32,
+                               _vp, _vp, _vp, ctypes.c_size_t, _vp], _i32),
+    "gsa_delta_step": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32,
+                        _vp, _i32, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp], _i32),
+    "gsa_delta_rule_workspace_bytes": ([_i32] * 7, ctypes.c_size_t),
+    "gsa_delta_rule_saved_bytes": ([_i32] * 6, ctypes.c_size_t),
+    "gsa_delta_rule": ([ctypes.POINTER(DeltaArgs), _vp], _i32),
+    "gsa_delta_rule_backward": ([ctypes.POINTER(DeltaArgs), _vp], _i32),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -865,3 +894,160 @@ def layer_attn(proj, offsets, bias32, idx_scale: float, cos, sin, halves, H: int
                             T * H * d, H * d, ws.data_ptr(), need, _stream(proj) if stream is None else stream)
     _check(st, "gsa_layer_attn")
     return out, k_rows
+
+
+# ---------------------------------------------------------------------------
+# RMS norm with the residual's addition
+# ---------------------------------------------------------------------------
+
+def _on(dev: torch.device, *ts: Optional[torch.Tensor]) -> None:
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}: one call takes one device")
+
+
+def _norm_rows(ts, D: int):
+    """The tensors (equal shapes [..., D], or None) as rows of D: (inner, [(tensor, s0, s1)]).
+    Strided ones are read in place where their leading dimensions make rows in groups of
+    shape[-2] (heads of a projection); others are copied."""
+    flat, inner = [], 1
+    for t in ts:
+        if t is not None and not t.is_contiguous():
+            inner = t.shape[-2] if t.dim() >= 2 else 1
+    for t in ts:
+        if t is None:
+            flat.append((None, 0, 0))
+            continue
+        if not t.is_contiguous():
+            try:
+                if t.stride(-1) != 1:
+                    raise RuntimeError
+                v = t.view(-1, inner, D)
+                flat.append((t, v.stride(0), v.stride(1)))
+                continue
+            except RuntimeError:
+                t = t.contiguous()
+        flat.append((t, inner * D, D))
+    return inner, flat
+
+
+def rms_norm(x, w, res=None, eps: float = 1e-6, want_rstd: bool = False):
+    """gsa_rms_norm: (y, h, rstd), h None without a residual, rstd None unless wanted."""
+    lib = load()
+    D = x.shape[-1]
+    rows = x.numel() // D
+    inner, ((x, x0, x1), (res, r0, r1)) = _norm_rows((x, res), D)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    h = torch.empty_like(y) if res is not None else None
+    rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if want_rstd else None
+    st = lib.gsa_rms_norm(_ptr(x), x0, x1, _ptr(res), r0, r1, _ptr(w), float(eps), rows, inner, D, dtype_code(x.dtype),
+                          _ptr(y), _ptr(h), _ptr(rstd), _stream(x))
+    _check(st, "gsa_rms_norm")
+    return y, h, rstd
+
+
+def rms_norm_fp8(x, w, res=None, eps: float = 1e-6):
+    """gsa_rms_norm_fp8: (y e4m3, scale fp32 [...], h or None)."""
+    lib = load()
+    D = x.shape[-1]
+    inner, ((x, x0, x1), (res, r0, r1)) = _norm_rows((x, res), D)
+    y = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if res is not None else None
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    st = lib.gsa_rms_norm_fp8(_ptr(x), x0, x1, _ptr(res), r0, r1, _ptr(w), float(eps), scale.numel(), inner, D,
+                              dtype_code(x.dtype), _ptr(y), _ptr(scale), _ptr(h), _stream(x))
+    _check(st, "gsa_rms_norm_fp8")
+    return y, scale, h
+
+
+def rms_norm_backward(h, dy, dh, w, rstd):
+    """gsa_rms_norm_backward: (dx, dw)."""
+    lib = load()
+    D = h.shape[-1]
+    rows = h.numel() // D
+    inner, ((h, h0, h1), (dy, y0, y1), (dh, d0, d1)) = _norm_rows((h, dy, dh), D)
+    dx = torch.empty(h.shape, device=h.device, dtype=h.dtype)
+    dw = torch.empty(D, device=h.device, dtype=h.dtype)
+    n = lib.gsa_rms_norm_backward_workspace_bytes(rows, D)
+    ws = torch.empty(n, device=h.device, dtype=torch.uint8)
+    st = lib.gsa_rms_norm_backward(_ptr(h), h0, h1, _ptr(dy), y0, y1, _ptr(dh), d0, d1, _ptr(w), _ptr(rstd), rows, inner, D,
+                                   dtype_code(h.dtype), _ptr(dx), _ptr(dw), _ptr(ws), n, _stream(h))
+    _check(st, "gsa_rms_norm_backward")
+    return dx, dw
+
+
+# ---------------------------------------------------------------------------
+# The gated delta rule
+# ---------------------------------------------------------------------------
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """t [..., heads, 128] with 16-byte aligned head rows: itself, or a copy."""
+    grp = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % grp == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def delta_step(q, k, v, g, beta, state, idx, scale: float) -> torch.Tensor:
+    """gsa_delta_step: o [N,Hv,128]; `state` is updated in place."""
+    lib = load()
+    N, Hv, d = v.shape
+    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    o = torch.empty(N, Hv, d, device=v.device, dtype=v.dtype)
+    st = lib.gsa_delta_step(_ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
+                            v.stride(1), _ptr(g), g.stride(0), g.stride(1), _ptr(beta), beta.stride(0), beta.stride(1),
+                            dtype_code(beta.dtype), _ptr(idx), 0 if idx is None else idx.element_size(), _ptr(state),
+                            state.stride(0), state.stride(1), N, state.shape[0], q.shape[1], Hv, d, float(scale),
+                            dtype_code(q.dtype), _ptr(o), _stream(v))
+    _check(st, "gsa_delta_step")
+    return o
+
+
+def _delta_args(q, k, v, g, beta, state_in, cu, scale: float) -> DeltaArgs:
+    B, T, Hv, d = v.shape
+    a = DeltaArgs(cu_seqlens=_ptr(cu), cu_bytes=0 if cu is None else cu.element_size(), B=B, T=T,
+                  N=B if cu is None else cu.numel() - 1, Hk=q.shape[2], Hv=Hv, d=d, dtype=dtype_code(q.dtype),
+                  beta_dtype=dtype_code(beta.dtype), scale=float(scale), state_in=_ptr(state_in))
+    for n, t in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta)):
+        setattr(a, n, _ptr(t))
+        for s, i in (("sb", 0), ("st", 1), ("sh", 2)):
+            setattr(a, f"{n}_{s}", t.stride(i))
+    return a
+
+
+def delta_rule(q, k, v, g, beta, state_in, cu, scale: float, want_state: bool, want_saved: bool):
+    """gsa_delta_rule: (o, state_out or None, saved or None).  q, k, v as _heads gives them."""
+    lib = load()
+    B, T, Hv, d = v.shape
+    a = _delta_args(q, k, v, g, beta, state_in, cu, scale)
+    sizes = (B, T, a.N, int(cu is not None), Hv, a.dtype)
+    # rows outside every packed sequence stay 0
+    o = (torch.empty if cu is None else torch.zeros)(B, T, Hv, d, device=v.device, dtype=v.dtype)
+    state = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_state else None
+    a.ws_bytes = lib.gsa_delta_rule_workspace_bytes(*sizes, 0)
+    ws = torch.empty(a.ws_bytes, device=v.device, dtype=torch.uint8)
+    saved = None
+    if want_saved:
+        a.saved_bytes = lib.gsa_delta_rule_saved_bytes(*sizes)
+        saved = torch.empty(a.saved_bytes, device=v.device, dtype=torch.uint8)
+    a.o, a.state_out, a.ws, a.saved = _ptr(o), _ptr(state), _ptr(ws), _ptr(saved)
+    _check(lib.gsa_delta_rule(ctypes.byref(a), _stream(v)), "gsa_delta_rule")
+    return o, state, saved
+
+
+def delta_rule_backward(q, k, v, g, beta, cu, scale: float, saved, dout, dstate, want_dstate: bool):
+    """gsa_delta_rule_backward: (dq, dk, dv, dg, dbeta, dstate_in or None)."""
+    lib = load()
+    B, T, Hv, d = v.shape
+    a = _delta_args(q, k, v, g, beta, None, cu, scale)
+    new = torch.empty if cu is None else torch.zeros
+    dq, dk, dv, dg, db = (new(t.shape, device=v.device, dtype=t.dtype) for t in (q, k, v, g, beta))
+    ds = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_dstate else None
+    a.ws_bytes = lib.gsa_delta_rule_workspace_bytes(B, T, a.N, int(cu is not None), Hv, a.dtype, 1)
+    ws = torch.empty(a.ws_bytes, device=v.device, dtype=torch.uint8)
+    a.ws, a.saved, a.saved_bytes = _ptr(ws), _ptr(saved), saved.numel()
+    a.dout, a.do_sb, a.do_st, a.do_sh = _ptr(dout), dout.stride(0), dout.stride(1), dout.stride(2)
+    a.dstate_out, a.dstate_in = _ptr(dstate), _ptr(ds)
+    a.dq, a.dk, a.dv, a.dg, a.dbeta = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dg), _ptr(db)
+    _check(lib.gsa_delta_rule_backward(ctypes.byref(a), _stream(v)), "gsa_delta_rule_backward")
+    return dq, dk, dv, dg, db, ds

@@ -25,7 +25,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libgsa_hip.so")
 ARCH = "gfx950"
 
 HIP_SOURCES = ("indexer.hip", "topk_select.hip", "sparse_attn.hip", "dense_attn.hip", "dense_attn_f32.hip",
-               "selected_attn.hip", "proj_fused.hip")
+               "selected_attn.hip", "proj_fused.hip", "rms_norm.hip", "delta_step.hip", "delta_rule.hip")
 CXX_SOURCES = ("abi.cpp", "layer.cpp")
 
 # Packed fp32 VALU forms are disabled in device code: the compiler would

@@ -1,0 +1,171 @@
+"""The gated delta rule on MI355X: the linear-attention mixer of the study's second half.
+
+``gated_delta_rule`` runs whole sequences (training, prefill) and is differentiable;
+``gated_delta_step`` runs one token of each sequence of a serving batch on the states that
+the former leaves.  The recurrence is the one of the reference's
+``recurrent_gated_delta_rule_ref`` (benchmark_models.ipynb:187)::
+
+    S_t = exp(g_t) S_{t-1} + k_t beta_t (v_t - exp(g_t) S_{t-1}^T k_t)^T
+    o_t = scale * S_t^T q_t                                  S [128, 128]: [k element, v element]
+
+q and k are taken as they are: normalise them before (``add_rms_norm`` with a weight of
+d**-0.5 gives them unit length).  There is no CPU or eager fallback.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _abi
+from .roctx import range_pop as _range_pop, range_push as _range_push
+
+D_HEAD = 128
+
+
+def _check(lead, q, k, v, g, beta) -> None:
+    """The checks that both entry points share; lead: the dimensions before the heads."""
+    n = len(lead)
+    if q.dim() != n + 2 or k.shape != q.shape or v.dim() != n + 2 or v.shape[:n] != q.shape[:n]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: expected [{', '.join(lead)}, heads, {D_HEAD}]")
+    if q.shape[-1] != D_HEAD or v.shape[-1] != D_HEAD:
+        raise ValueError(f"head dims {q.shape[-1]} and {v.shape[-1]}: the kernels take {D_HEAD}")
+    Hk, Hv = q.shape[n], v.shape[n]
+    if Hk < 1 or Hv < 1 or Hv % Hk:
+        raise ValueError(f"{Hv} v heads are not a multiple of {Hk} q/k heads")
+    if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
+        raise ValueError(f"g {tuple(g.shape)}, beta {tuple(beta.shape)}: expected {tuple(v.shape[:-1])}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise ValueError(f"q, k, v must share a dtype: got {q.dtype}, {k.dtype}, {v.dtype}")
+    _abi.dtype_code(q.dtype)
+    if g.dtype != torch.float32:
+        raise TypeError(f"g is {g.dtype}: log decays are float32")
+    if beta.dtype not in (torch.float32, q.dtype):
+        raise TypeError(f"beta is {beta.dtype}: expected float32 or {q.dtype}")
+
+
+def _device(first: torch.Tensor, *others: Optional[torch.Tensor]):
+    """Checks that all tensors are on one GPU and makes it the current one."""
+    _abi._need_cuda(first, *others)
+    _abi._on(first.device, *others)
+    return torch.cuda.device(first.device)
+
+
+class _Rule(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, cu, scale, want_state, want_saved):
+        q, k, v = _abi._heads(q), _abi._heads(k), _abi._heads(v)
+        o, final, saved = _abi.delta_rule(q, k, v, g, beta, state, cu, scale, want_state, want_saved)
+        ctx.set_materialize_grads(False)
+        ctx.scale, ctx.has_state = scale, state is not None
+        if want_saved:
+            ctx.save_for_backward(q, k, v, g, beta, cu, saved)
+        return o, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, dfinal):
+        q, k, v, g, beta, cu, saved = ctx.saved_tensors
+        _range_push("gsa_hip/delta_rule_backward")
+        try:
+            do = torch.zeros_like(v, memory_format=torch.contiguous_format) if do is None else _abi._heads(do)
+            if dfinal is not None:
+                dfinal = dfinal.contiguous()
+                if dfinal.data_ptr() % 16:
+                    dfinal = dfinal.clone()
+            grads = _abi.delta_rule_backward(q, k, v, g, beta, cu, ctx.scale, saved, do, dfinal, ctx.has_state)
+        finally:
+            _range_pop()
+        return (*grads, None, None, None, None)
+
+
+def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                     scale: Optional[float] = None, initial_state: Optional[torch.Tensor] = None,
+                     output_final_state: bool = False,
+                     cu_seqlens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(o [B,T,Hv,128], final state [N,Hv,128,128] fp32 or None) of the gated delta rule.
+
+    q, k [B,T,Hk,128] and v [B,T,Hv,128] in bf16 or fp32; v head h goes with q/k head
+    h // (Hv // Hk).  g [B,T,Hv] fp32, the log of the decay (at most 0; below -128, down to
+    -inf, it is a reset); beta [B,T,Hv] in fp32 or q's dtype.  Strided views with contiguous
+    head rows are read in place.  scale: 128**-0.5 unless given.  initial_state
+    [N,Hv,128,128] fp32: zeros unless given.
+
+    cu_seqlens (int32 or int64 [N+1], on the device, ascending from 0): B is 1 and N sequences
+    are packed in T, each with its own state; empty ones are allowed.  Rows of o and of the
+    gradients outside every sequence are 0.
+
+    Differentiable in q, k, v, g, beta and initial_state (once); the gradients are the same
+    bits on every run.  A forward that needs gradients keeps 1.5 KiB (bf16; fp32: 2.5 KiB) a
+    token and v head.
+    """
+    _check(("B", "T"), q, k, v, g, beta)
+    B, T, Hv, d = v.shape
+    if cu_seqlens is not None:
+        if B != 1:
+            raise ValueError(f"packed sequences come in one row: B is {B}")
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise ValueError("cu_seqlens: int32 or int64 [N + 1]")
+        cu_seqlens = cu_seqlens.contiguous()
+    N = B if cu_seqlens is None else cu_seqlens.numel() - 1
+    if initial_state is not None:
+        if tuple(initial_state.shape) != (N, Hv, d, d) or initial_state.dtype != torch.float32:
+            raise ValueError(f"initial_state {tuple(initial_state.shape)} {initial_state.dtype}: expected fp32 {(N, Hv, d, d)}")
+    scale = d ** -0.5 if scale is None else float(scale)
+    with _device(q, k, v, g, beta, initial_state, cu_seqlens):
+        if B * T == 0:
+            o = v.new_zeros(v.shape)
+            if not output_final_state:
+                return o, None
+            return o, v.new_zeros(N, Hv, d, d, dtype=torch.float32) if initial_state is None else initial_state.clone()
+        if initial_state is not None:
+            initial_state = initial_state.contiguous()
+            if initial_state.data_ptr() % 16:
+                initial_state = initial_state.clone()
+        grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
+        _range_push("gsa_hip/delta_rule")
+        try:
+            return _Rule.apply(q, k, v, g, beta, initial_state, cu_seqlens, scale, bool(output_final_state), grad)
+        finally:
+            _range_pop()
+
+
+def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                     state: torch.Tensor, state_indices: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """One token of each row of a serving batch: o [N,Hv,128]; ``state`` is updated in place.
+
+    q, k [N,Hk,128], v [N,Hv,128], g, beta [N,Hv] as in ``gated_delta_rule``.  state
+    [slots,Hv,128,128] fp32, each matrix contiguous.  state_indices (int32 or int64 [N], on
+    the device): the state of each row; row n has state n without it.  A row whose index is
+    outside [0, slots) is padding: its output is 0 and no state changes.  Rows with the same
+    index are consecutive tokens of one sequence, in the batch's order.
+
+    Forward only: it raises where a gradient would be needed.
+    """
+    _check(("N",), q, k, v, g, beta)
+    N, Hv, d = v.shape
+    if state.dim() != 4 or tuple(state.shape[1:]) != (Hv, d, d) or state.dtype != torch.float32:
+        raise ValueError(f"state {tuple(state.shape)} {state.dtype}: expected fp32 [slots, {Hv}, {d}, {d}]")
+    if state.stride()[2:] != (d, 1) or state.stride(0) % 4 or state.stride(1) % 4 or state.data_ptr() % 16:
+        raise ValueError("state is updated in place: its matrices must be contiguous and 16-byte aligned")
+    if state.shape[0] > 1 and state.stride(0) < d * d or Hv > 1 and state.stride(1) < d * d:
+        raise ValueError("state is updated in place: its matrices overlap")
+    if state_indices is not None:
+        if tuple(state_indices.shape) != (N,) or state_indices.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"state_indices: int32 or int64 [{N}]")
+        state_indices = state_indices.contiguous()
+    elif N > state.shape[0]:
+        raise ValueError(f"{N} rows, {state.shape[0]} states")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
+        raise RuntimeError("gated_delta_step is forward only: call it under torch.no_grad()")
+    with _device(q, k, v, g, beta, state, state_indices):
+        if N == 0 or state.shape[0] == 0:
+            return v.new_zeros(v.shape)
+        _range_push("gsa_hip/delta_step")
+        try:
+            return _abi.delta_step(q, k, v, g, beta, state, state_indices, d ** -0.5 if scale is None else scale)
+        finally:
+            _range_pop()

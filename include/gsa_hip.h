@@ -512,6 +512,96 @@ int gsa_proj_fused(const void* x, int64_t x_st, int B, int T, int D, int H, int 
                    void* q, int64_t q_st, void* og, int64_t og_st,
                    void* k_out, void* vt, int ldv, void* stream);
 
+/*
+ * RMS norm with the residual's addition (no counterpart in the reference's kernels; its
+ * layers take a normed input).  Row r of [rows, D]:
+ *   h = round(x + res) (x itself when res is NULL),  y = h * (mean h^2 + eps)^-1/2 * w
+ * Row r of an input lies at base + (r / inner) * s0 + (r % inner) * s1 elements (rows a
+ * multiple of inner), so heads of a strided projection are read in place; y, h and dx are
+ * contiguous [rows, D], w [D].  1 <= D <= 32768; any alignment of elements (16-byte rows
+ * are read and written whole).
+ *   gsa_rms_norm:          y, h (with res), and (nullable) rstd fp32 [rows] for the backward
+ *   gsa_rms_norm_fp8:      y in e4m3, y = round(y / scale), scale fp32 [rows] = max |y| / 448
+ *                          (1 for a row of zeros)
+ *   gsa_rms_norm_backward: dx = dh + rstd (dy w - n mean(dy w n)), n = h rstd (the gradient of
+ *                          x and of res; dh nullable), dw [D] = sum over rows of dy n; the same
+ *                          bits on every run.  ws: gsa_rms_norm_backward_workspace_bytes
+ */
+int gsa_rms_norm(const void* x, int64_t x_s0, int64_t x_s1, const void* res, int64_t r_s0, int64_t r_s1,
+                 const void* w, float eps, int64_t rows, int inner, int D, int dtype,
+                 void* y, void* h, float* rstd, void* stream);
+int gsa_rms_norm_fp8(const void* x, int64_t x_s0, int64_t x_s1, const void* res, int64_t r_s0, int64_t r_s1,
+                     const void* w, float eps, int64_t rows, int inner, int D, int dtype,
+                     void* y, float* scale, void* h, void* stream);
+size_t gsa_rms_norm_backward_workspace_bytes(int64_t rows, int D);
+int gsa_rms_norm_backward(const void* h, int64_t h_s0, int64_t h_s1, const void* dy, int64_t dy_s0, int64_t dy_s1,
+                          const void* dh, int64_t dh_s0, int64_t dh_s1, const void* w, const float* rstd,
+                          int64_t rows, int inner, int D, int dtype, void* dx, void* dw,
+                          void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * The gated delta rule (the recurrence of the reference's recurrent_gated_delta_rule_ref,
+ * benchmark_models.ipynb:187), states S [128,128] fp32 ([k element][v element]):
+ *   S_t = e^g_t S_{t-1} + k_t beta_t (v_t - e^g_t S_{t-1}^T k_t)^T,   o_t = scale S_t^T q_t
+ *
+ * gsa_delta_step: one token of each row of a serving batch, its state updated in place.
+ * q, k [N,Hk,128], v [N,Hv,128], g fp32 and beta [N,Hv] (strides of rows and heads, elements
+ * contiguous); v head h reads q/k head h / (Hv / Hk).  state [slots,Hv,128,128] fp32, each
+ * matrix contiguous, strides multiples of 4.  state_idx (nullable: row n has state n; int32 or
+ * int64 by idx_bytes): row n's state; one outside [0, slots) is padding: output 0, no state
+ * changes.  Rows with the same state are consecutive tokens of it, in the batch's order.
+ * o [N,Hv,128] contiguous.
+ */
+int gsa_delta_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int64_t k_sn, int64_t k_sh,
+                   const void* v, int64_t v_sn, int64_t v_sh, const float* g, int64_t g_sn, int64_t g_sh,
+                   const void* beta, int64_t b_sn, int64_t b_sh, int beta_dtype,
+                   const void* state_idx, int idx_bytes, float* state, int64_t s_sn, int64_t s_sh,
+                   int N, int slots, int Hk, int Hv, int d, float scale, int dtype, void* o, void* stream);
+
+/*
+ * gsa_delta_rule: whole sequences, in chunks on the matrix cores.  B rows of T tokens
+ * (N == B), or N sequences packed in the T tokens of one row (B == 1): cu_seqlens, N + 1
+ * ascending offsets on the device (int32 or int64 by cu_bytes); empty sequences are allowed,
+ * offsets are held within [0, T], and rows outside every sequence are not written.
+ * q, k [B,T,Hk,128], v [B,T,Hv,128] in dtype, g fp32 and beta (beta_dtype) [B,T,Hv]; strides
+ * of batch, token and head in elements, those of q, k, v (and dout) keeping 16-byte
+ * alignment.  g below -128 (down to -inf) acts as -128, whose e^g is 0.
+ * state_in, state_out (nullable) fp32 [N,Hv,128,128]; o [B,T,Hv,128] contiguous.
+ * ws: gsa_delta_rule_workspace_bytes(..., backward).  saved (nullable in the forward):
+ * gsa_delta_rule_saved_bytes, the states and deltas that gsa_delta_rule_backward reads.
+ *
+ * gsa_delta_rule_backward: the inputs above with `saved` of their forward, dout [B,T,Hv,128],
+ * dstate_out (nullable: 0) -> dq, dk, dv, dg (fp32), dbeta (beta_dtype) contiguous, and
+ * dstate_in (nullable).  The same bits on every run.
+ */
+typedef struct gsa_delta_args {
+  const void *q, *k, *v;
+  const float* g;
+  const void* beta;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh, beta_sb, beta_st, beta_sh;
+  const void* cu_seqlens;
+  int cu_bytes, B, T, N, Hk, Hv, d, dtype, beta_dtype;
+  float scale;
+  const float* state_in;
+  void* o;
+  float* state_out;
+  void* ws;
+  size_t ws_bytes;
+  void* saved;
+  size_t saved_bytes;
+  const void* dout;
+  int64_t do_sb, do_st, do_sh;
+  const float* dstate_out;
+  void *dq, *dk, *dv;
+  float* dg;
+  void* dbeta;
+  float* dstate_in;
+} gsa_delta_args;
+size_t gsa_delta_rule_workspace_bytes(int B, int T, int N, int packed, int Hv, int dtype, int backward);
+size_t gsa_delta_rule_saved_bytes(int B, int T, int N, int packed, int Hv, int dtype);
+int gsa_delta_rule(const gsa_delta_args* args, void* stream);
+int gsa_delta_rule_backward(const gsa_delta_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
