@@ -130,8 +130,8 @@ _PROTOS = {
                                _vp, _vp, _vp, ctypes.c_size_t, _vp], _i32),
     "gsa_delta_step": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32,
                         _vp, _i32, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp], _i32),
-    "gsa_delta_rule_workspace_bytes": ([_i32] * 7, ctypes.c_size_t),
-    "gsa_delta_rule_saved_bytes": ([_i32] * 6, ctypes.c_size_t),
+    "gsa_delta_rule_workspace_bytes": ([_i32] * 8, ctypes.c_size_t),
+    "gsa_delta_rule_saved_bytes": ([_i32] * 7, ctypes.c_size_t),
     "gsa_delta_rule": ([ctypes.POINTER(DeltaArgs), _vp], _i32),
     "gsa_delta_rule_backward": ([ctypes.POINTER(DeltaArgs), _vp], _i32),
 }
@@ -981,9 +981,10 @@ def rms_norm_backward(h, dy, dh, w, rstd):
 # ---------------------------------------------------------------------------
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
-    """t [..., heads, 128] with 16-byte aligned head rows: itself, or a copy."""
+    """t [B,T,heads,128] with 16-byte aligned head rows and tokens less than 32 MiB apart: itself, or a copy."""
     grp = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % grp == 0 for s in t.stride()[:-1]):
+    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % grp == 0 for s in t.stride()[:-1])
+            and t.stride(1) * t.element_size() < 1 << 25):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -1020,7 +1021,7 @@ def delta_rule(q, k, v, g, beta, state_in, cu, scale: float, want_state: bool, w
     lib = load()
     B, T, Hv, d = v.shape
     a = _delta_args(q, k, v, g, beta, state_in, cu, scale)
-    sizes = (B, T, a.N, int(cu is not None), Hv, a.dtype)
+    sizes = (B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
     # rows outside every packed sequence stay 0
     o = (torch.empty if cu is None else torch.zeros)(B, T, Hv, d, device=v.device, dtype=v.dtype)
     state = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_state else None
@@ -1043,7 +1044,7 @@ def delta_rule_backward(q, k, v, g, beta, cu, scale: float, saved, dout, dstate,
     new = torch.empty if cu is None else torch.zeros
     dq, dk, dv, dg, db = (new(t.shape, device=v.device, dtype=t.dtype) for t in (q, k, v, g, beta))
     ds = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_dstate else None
-    a.ws_bytes = lib.gsa_delta_rule_workspace_bytes(B, T, a.N, int(cu is not None), Hv, a.dtype, 1)
+    a.ws_bytes = lib.gsa_delta_rule_workspace_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype, 1)
     ws = torch.empty(a.ws_bytes, device=v.device, dtype=torch.uint8)
     a.ws, a.saved, a.saved_bytes = _ptr(ws), _ptr(saved), saved.numel()
     a.dout, a.do_sb, a.do_st, a.do_sh = _ptr(dout), dout.stride(0), dout.stride(1), dout.stride(2)

@@ -35,6 +35,8 @@ constexpr int kHead = 128;
 // product to product in its own registers.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int tile_row(int t, int m) { return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
+// tile_row(t, 4 g + r) = 8 g + tile_at(t, r): a lane's part and one the compiler knows.
+constexpr int tile_at(int t, int r) { return 32 * (t >> 1) + 4 * (t & 1) + r; }
 
 template <int N> struct Parts { bf16x8 p[N]; };
 
@@ -100,33 +102,33 @@ struct Rows { const void* p; int64_t sb, st, sh; };         // [B, T, heads, ...
 // needed).  Offsets are held within [0, T]: whatever cu says, nothing outside is touched.
 struct Seqs {
   const void* cu;
-  int cu64, N, T, slots;
+  int cu64, N, T;
   __device__ int64_t at(int n) const {
     const int64_t x = cu64 ? static_cast<const int64_t*>(cu)[n] : static_cast<const int32_t*>(cu)[n];
     return x < 0 ? 0 : x > T ? T : x;
   }
 };
 struct Span { int n, b, t0, len, slot0; };                   // sequence n: tokens t0 .. t0 + len - 1 of row b
-template <int C> __device__ __forceinline__ Span span_of(const Seqs& s, int n) {
-  if (!s.cu) return Span{n, n, 0, s.T, n * ((s.T + C - 1) / C)};
-  const int64_t a = s.at(n), e = s.at(n + 1);
-  return Span{n, 0, (int)a, e > a ? (int)(e - a) : 0, (int)(a / C) + n};
+__device__ __forceinline__ Span span_of(const Seqs& s, int n, int ch) {       // slots of ch tokens
+  if (!s.cu) return Span{n, n, 0, s.T, n * ((s.T + ch - 1) / ch)};
+  const int a = __builtin_amdgcn_readfirstlane((int)s.at(n)), e = __builtin_amdgcn_readfirstlane((int)s.at(n + 1));
+  return Span{n, 0, a, e > a ? e - a : 0, a / ch + n};
 }
-// The sequence and chunk of a slot; c < 0: an empty slot.
-template <int C> __device__ __forceinline__ Span slot_of(const Seqs& s, int slot, int& c) {
+// The sequence of a slot, and which of its pieces it is; c < 0: an empty slot.
+__device__ __forceinline__ Span slot_of(const Seqs& s, int slot, int ch, int& c) {
   if (!s.cu) {
-    const int nc = (s.T + C - 1) / C, n = slot / nc;
+    const int nc = (s.T + ch - 1) / ch, n = slot / nc;
     c = slot - n * nc;
-    return span_of<C>(s, n);
+    return span_of(s, n, ch);
   }
   int lo = 0, hi = s.N - 1;                                  // the last n whose first slot is not behind
   while (lo < hi) {
     const int m = (lo + hi + 1) / 2;
-    if ((int)(s.at(m) / C) + m <= slot) lo = m; else hi = m - 1;
+    if (__builtin_amdgcn_readfirstlane((int)s.at(m)) / ch + m <= slot) lo = m; else hi = m - 1;
   }
-  const Span r = span_of<C>(s, lo);
+  const Span r = span_of(s, lo, ch);
   c = slot - r.slot0;
-  if (c < 0 || c >= (r.len + C - 1) / C) c = -1;
+  if (c < 0 || c >= (r.len + ch - 1) / ch) c = -1;
   return r;
 }
 
@@ -138,10 +140,19 @@ struct DeltaArgs {
   const float* state_in;      // [N, Hv, 128, 128], nullable
   void* o;                    // [B, T, Hv, 128]
   float* state_out;           // nullable
-  // a chunk's, [slots][Hv] each
-  float* tm;                  // [C][C]: Tm, rows i
-  float* pm;                  // [C][C]: P
-  float* gates;               // [5][C]: e^G, e^(G_C - G), beta, G (upper and lower part)
+  // A chunk's operands in the order in which the lanes of the scan take them, a 1 KiB unit an
+  // operand part: 64 lanes' 16 bytes.
+  char* tm;                   // [slots][Hv]: Tm (the backward pass: transposed)
+  char* pm;                   // [slots][Hv]: P (transposed)
+  float* gates;               // [slots][Hv] units: e^G, e^(G_C - G), beta [C] each
+  float* sums;                // [slots][Hv][2][C]: G (upper and lower part); the backward pass only
+  char *kt, *qt;              // [slots][Hk]: K^T, Q^T (the backward pass)
+  char *kr, *qr;              // [slots][Hk]: fp32 inputs: K, Q
+  // The scan cut into segments of seg chunks (0: sequences in one piece), [segments][Hv][128][128] each
+  int seg, segs;
+  float* move;                // a segment's product of transitions
+  float* add;                 // its state from a start of 0 (the first: from state_in)
+  float* init;                // the state before it (backward: the gradient behind it)
   // kept for the backward pass (nullable)
   float* s0;                  // [128][128]: the state before the chunk
   float* u;                   // [C][128]
@@ -174,7 +185,7 @@ template <typename T> __device__ __forceinline__ Parts<DeltaType<T>::kParts> ope
 }
 
 // ---------------------------------------------------------------------------
-// Tm and P of every chunk and v head.  256 threads.
+// The operands of every chunk and v head (with kBwd those of the backward scan): 256 threads.
 // ---------------------------------------------------------------------------
 // 16x16 tile a b of LDS matrices, summed over K (fp32 matrix instruction).
 __device__ __forceinline__ floatx4 tile_f32(const float* a, int lda, const float* b, int ldb, int K) {
@@ -190,135 +201,51 @@ __device__ __forceinline__ void tile_put(float* d, int ld, const floatx4& x, flo
   for (int r = 0; r < 4; ++r) d[(4 * (l >> 4) + r) * ld + (l & 15)] = x[r] * f;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
-  constexpr int C = DeltaType<T>::kChunk, MT = C / 16, LD = C + 4;
-  __shared__ float am[C][LD], xm[C][LD], ym[C][LD];
-  __shared__ float gh[C], gl[C], bt[C];
-  const int slot = blockIdx.x, h = blockIdx.y, hk = h / (a.Hv / a.Hk), tid = threadIdx.x, wave = tid >> 6, l = lane_id();
-  int c;
-  const Span sp = slot_of<C>(a.s, slot, c);
-  if (c < 0) return;
-  const int64_t t0 = (int64_t)c * C;
-  const int left = sp.len - (int)t0;                         // tokens of the chunk (more than C: C)
-  const int64_t at = (int64_t)slot * a.Hv + h;
+constexpr int kUnit = 1024;
+// A chunk's square matrices are lower triangular: of their (tile, step) operands the ones that
+// are not 0 everywhere, with rows of tokens t and steps of 32 summed over (transposed: the
+// steps from t's on).
+template <int C> struct Square {
+  static constexpr int kFrags = C == 64 ? 6 : 2;
+  static constexpr int at(int tile, int js, bool transposed) {
+    return C == 32 ? tile : transposed ? (tile < 2 ? 2 * tile + js : 2 + tile) : (tile < 2 ? tile : 2 * tile - 2 + js);
+  }
+  // its tile and step
+  __device__ static int2 of(int f, bool transposed) {
+    if (C == 32) return int2{f, 0};
+    if (transposed) return f < 4 ? int2{f >> 1, f & 1} : int2{f - 2, 1};
+    return f < 2 ? int2{f, 0} : int2{(f + 2) >> 1, f & 1};
+  }
+};
+// Units of a chunk's operands.  P enters the output alone in the forward pass: for bf16 outputs
+// two parts (2^-17 of it) do; the backward pass sums it into states.
+template <typename T, bool kBwd> struct Pack {
+  static constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts;
+  static constexpr int kPParts = kBwd || NP == 3 ? 3 : 2;
+  static constexpr int kT = Square<C>::kFrags * 3, kP = Square<C>::kFrags * kPParts;
+  static constexpr int kCols = 8 * (C / 32) * NP, kRows = (C / 16) * 4 * NP;
+};
 
-  if (wave == 0) {
-    const bool ok = l < C && l < left;
-    float g = 0.f, b = 0.f;
-    if (ok) {
-      g = *row_at<float>(a.g, sp, t0 + l, h);
-      b = a.beta_bf16 ? bf16lo(*row_at<uint16_t>(a.beta, sp, t0 + l, h)) : *row_at<float>(a.beta, sp, t0 + l, h);
-      // e^-128 is 0 in fp32: a lower g (down to -inf, a reset) gives the same, without inf - inf
-      if (g < -128.f) g = -128.f;
+// [C][ld] fp32 matrix in LDS -> its operands of kN parts in global memory.
+template <int C, int kN, bool kTransposed>
+__device__ __forceinline__ void pack_square(char* dst, const float* x, int ld, int tid) {
+  for (int u = tid; u < Square<C>::kFrags * 64; u += 256) {
+    const int l = u & 63, f = u >> 6;
+    const int2 w = Square<C>::of(f, kTransposed);
+    const int t = tile_row(w.x, l & 15), j = 32 * w.y + 8 * (l >> 4);
+    float y[8];
+    if constexpr (kTransposed) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = x[(j + e) * ld + t];
+    } else {
+      load8(x + t * ld + j, y);
     }
-    double G = g;                                            // differences of sums keep fp32's precision
+    const Parts<3> p = split3(y);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(G, o, 64);
-      if (l >= o) G += y;
-    }
-    const double Ge = __shfl(G, C - 1, 64);
-    const float hi = (float)G, lo = (float)(G - (double)hi);
-    if (l < C) {
-      gh[l] = hi;
-      gl[l] = lo;
-      bt[l] = b;
-      float* gates = a.gates + at * 5 * C;
-      gates[l] = expf((float)G);
-      gates[C + l] = expf((float)(Ge - G));
-      gates[2 * C + l] = b;
-      gates[3 * C + l] = hi;
-      gates[4 * C + l] = lo;
-    }
-  }
-  for (int i = tid; i < C * LD; i += 256) (&xm[0][0])[i] = 0.f;
-  __syncthreads();
-
-  // row tile mt of K K^T (into am) and of Q K^T (to pm)
-  for (int job = wave; job < 2 * MT; job += 4) {
-    const int mt = job % MT;
-    const bool qk = job >= MT;
-    Parts<DeltaType<T>::kParts> x[4];
-    {
-      const int t = 16 * mt + (l & 15);
-      const T* p = qk ? row_at<T>(a.q, sp, t0 + t, hk) : row_at<T>(a.k, sp, t0 + t, hk);
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) x[ks] = operand<T>(p + 32 * ks + 8 * (l >> 4), t < left);
-    }
-    for (int nt = 0; nt < MT; ++nt) {
-      const int j = 16 * nt + (l & 15);
-      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-      if (nt <= mt) {
-        const T* p = row_at<T>(a.k, sp, t0 + j, hk);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) mma(acc, x[ks], operand<T>(p + 32 * ks + 8 * (l >> 4), j < left));
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * mt + 4 * (l >> 4) + r;
-        const float d = expf((gh[i] - gh[j]) + (gl[i] - gl[j]));
-        if (qk) a.pm[(at * C + i) * C + j] = j <= i ? a.scale * acc[r] * d : 0.f;
-        else am[i][j] = j < i ? bt[i] * acc[r] * d : 0.f;
-      }
-    }
-  }
-  __syncthreads();
-
-  // (I + A)^-1: blocks of 16 by substitution, a lane a column; then pairs of blocks, and of pairs:
-  // the lower left of the inverse is -Y A21 X with X, Y the inverses above and below it.  (Doubling
-  // products of I - A would cancel: for equal keys its terms grow like binomials.)
-  if (wave < MT && l < 16) {
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float s = i == l ? 1.f : 0.f;
-#pragma unroll
-      for (int m = 0; m < i; ++m) s = __builtin_fmaf(-am[16 * wave + i][16 * wave + m], x[m], s);
-      x[i] = s;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) xm[16 * wave + i][16 * wave + l] = x[i];
-  }
-  __syncthreads();
-  if (wave < C / 32) {
-    const int p = 32 * wave;
-    tile_put(&ym[p][p], LD, tile_f32(&am[p + 16][p], LD, &xm[p][p], LD, 16), 1.f);
-  }
-  __syncthreads();
-  if (wave < C / 32) {
-    const int p = 32 * wave;
-    tile_put(&xm[p + 16][p], LD, tile_f32(&xm[p + 16][p + 16], LD, &ym[p][p], LD, 16), -1.f);
-  }
-  __syncthreads();
-  if constexpr (C == 64) {
-    const int i = 16 * (wave >> 1), j = 16 * (wave & 1);
-    tile_put(&ym[i][j], LD, tile_f32(&am[32 + i][0], LD, &xm[0][j], LD, 32), 1.f);
-    __syncthreads();
-    tile_put(&xm[32 + i][j], LD, tile_f32(&xm[32 + i][32], LD, &ym[0][j], LD, 32), -1.f);
-    __syncthreads();
-  }
-  for (int i = tid; i < C * C; i += 256) a.tm[at * C * C + i] = xm[i / C][i % C];
-}
-
-// ---------------------------------------------------------------------------
-// The state from chunk to chunk.  512 threads: a wave owns 16 columns of one head's state,
-// tile 2 ks + e of its registers the rows tile_row(2 ks + e, .).  A chunk's operands lie in LDS
-// in the order in which the lanes take them: [tile][step][part][lane] of 16 bytes.
-// ---------------------------------------------------------------------------
-// Rows of tokens (tile_row), summed over the 128 elements.
-template <typename T>
-__device__ __forceinline__ void stage_rows(bf16x8* dst, const Rows& x, const Span& sp, int64_t t0, int left, int h, int tid) {
-  constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts;
-  for (int u = tid; u < C * 16; u += 512) {
-    const int d8 = u & 15, t = u >> 4;
-    const int tile = 2 * (t >> 5) + ((t >> 2) & 1), m = 4 * ((t >> 3) & 3) + (t & 3);
-    const Parts<NP> p = operand<T>(row_at<T>(x, sp, t0 + t, h) + 8 * d8, t < left);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) dst[((tile * 4 + (d8 >> 2)) * NP + i) * 64 + 16 * (d8 & 3) + m] = p.p[i];
+    for (int n = 0; n < kN; ++n) *reinterpret_cast<bf16x8*>(dst + (f * kN + n) * kUnit + 16 * l) = p.p[n];
   }
 }
-// Rows of the 128 elements (tile_row), summed over tokens.
+// Rows of the 128 elements (tile_row), summed over tokens, to global memory or LDS.
 template <typename T>
 __device__ __forceinline__ void stage_cols(bf16x8* dst, const Rows& x, const Span& sp, int64_t t0, int left, int h, int tid,
                                            int threads) {
@@ -352,27 +279,16 @@ __device__ __forceinline__ void stage_cols(bf16x8* dst, const Rows& x, const Spa
     }
   }
 }
-// A [C][C] fp32 matrix, or its transpose: rows of tokens (tile_row), summed over tokens.
-template <int C, bool kTransposed>
-__device__ __forceinline__ void stage_square(bf16x8* dst, const float* x, int tid) {
-  constexpr int JS = C / 32;
-  for (int u = tid; u < C * C / 8; u += 512) {
-    int t, oct;
-    float y[8];
-    if constexpr (kTransposed) {
-      t = u % C;
-      oct = u / C;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = x[(8 * oct + e) * C + t];
-    } else {
-      oct = u % (C / 8);
-      t = u / (C / 8);
-      load8(x + t * C + 8 * oct, y);
-    }
+// Rows of tokens (tile_row), summed over the 128 elements.
+template <typename T>
+__device__ __forceinline__ void stage_rows(bf16x8* dst, const Rows& x, const Span& sp, int64_t t0, int left, int h, int tid) {
+  constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts;
+  for (int u = tid; u < C * 16; u += 256) {
+    const int d8 = u & 15, t = u >> 4;
     const int tile = 2 * (t >> 5) + ((t >> 2) & 1), m = 4 * ((t >> 3) & 3) + (t & 3);
-    const Parts<3> p = split3(y);
+    const Parts<NP> p = operand<T>(row_at<T>(x, sp, t0 + t, h) + 8 * d8, t < left);
 #pragma unroll
-    for (int n = 0; n < 3; ++n) dst[((tile * JS + (oct >> 2)) * 3 + n) * 64 + 16 * (oct & 3) + m] = p.p[n];
+    for (int i = 0; i < NP; ++i) dst[((tile * 4 + (d8 >> 2)) * NP + i) * 64 + 16 * (d8 & 3) + m] = p.p[i];
   }
 }
 template <int N> __device__ __forceinline__ Parts<N> staged(const bf16x8* src, int frag, int l) {
@@ -382,229 +298,711 @@ template <int N> __device__ __forceinline__ Parts<N> staged(const bf16x8* src, i
   return r;
 }
 
-template <typename T> struct ScanLds {
-  static constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts, MT = C / 16, JS = C / 32;
-  static constexpr int kRows = MT * 4 * NP * 64, kCols = 8 * JS * NP * 64, kSquare = MT * JS * 3 * 64;
-  static constexpr int kGates = 0;                           // floats [3][C]
-  static constexpr size_t kFwd = 16 * (size_t)(2 * kRows + kCols + 2 * kSquare) + 3 * C * 4;
-  static constexpr size_t kBwd = 16 * (size_t)(kRows + 2 * kCols + 2 * kSquare) + 3 * C * 4;
-};
+template <typename T, bool kBwd>
+__global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
+  using K = Pack<T, kBwd>;
+  constexpr int C = K::C, NP = K::NP, MT = C / 16, LD = C + 4;
+  constexpr int kStage = K::kRows * kUnit, kX = C * LD * 4 > kStage ? C * LD * 4 : kStage;
+  __shared__ __align__(16) float am[C][LD], pm[C][LD];
+  __shared__ __align__(16) char xbuf[kX];                    // K's rows, then the inverse
+  __shared__ float gh[C], gl[C], bt[C];
+  float (*xm)[LD] = reinterpret_cast<float (*)[LD]>(xbuf);
+  bf16x8* sk = reinterpret_cast<bf16x8*>(xbuf);
+  const int slot = blockIdx.x, h = blockIdx.y, share = a.Hv / a.Hk, hk = h / share, tid = threadIdx.x, wave = tid >> 6, l = lane_id();
+  const int g4 = l >> 4, m = l & 15;
+  int c;
+  const Span sp = slot_of(a.s, slot, C, c);
+  if (c < 0) return;
+  const int64_t t0 = (int64_t)c * C;
+  const int left = sp.len - (int)t0;                         // tokens of the chunk (more than C: C)
+  const int64_t at = (int64_t)slot * a.Hv + h, atk = (int64_t)slot * a.Hk + hk;
 
-template <typename T>
-__global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
-  using L = ScanLds<T>;
-  constexpr int C = L::C, NP = L::NP, MT = L::MT, JS = L::JS;
-  extern __shared__ __align__(16) char lds[];
-  bf16x8* sk = reinterpret_cast<bf16x8*>(lds);
-  bf16x8* sq = sk + L::kRows;
-  bf16x8* skt = sq + L::kRows;
-  bf16x8* st = skt + L::kCols;
-  bf16x8* sp_ = st + L::kSquare;
-  float* gates = reinterpret_cast<float*>(sp_ + L::kSquare);
-  const int h = blockIdx.y, hk = h / (a.Hv / a.Hk), tid = threadIdx.x, l = lane_id(), g = l >> 4;
-  const int col = 16 * (tid >> 6) + (l & 15);
-  const Span sp = span_of<C>(a.s, blockIdx.x);
-  const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead;
-
-  floatx4 S[8];
+  stage_rows<T>(sk, a.k, sp, t0, left, hk, tid);
+  if (wave == 0) {
+    const bool ok = l < C && l < left;
+    float g = 0.f, b = 0.f;
+    if (ok) {
+      g = *row_at<float>(a.g, sp, t0 + l, h);
+      b = a.beta_bf16 ? bf16lo(*row_at<uint16_t>(a.beta, sp, t0 + l, h)) : *row_at<float>(a.beta, sp, t0 + l, h);
+      // e^-128 is 0 in fp32: a lower g (down to -inf, a reset) gives the same, without inf - inf
+      if (g < -128.f) g = -128.f;
+    }
+    double G = g;                                            // differences of sums keep fp32's precision
 #pragma unroll
-  for (int t = 0; t < 8; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) S[t][r] = a.state_in ? a.state_in[sn + tile_row(t, 4 * g + r) * kHead + col] : 0.f;
-
-  const int chunks = (sp.len + C - 1) / C;
-  for (int c = 0; c < chunks; ++c) {
-    const int64_t t0 = (int64_t)c * C, at = (int64_t)(sp.slot0 + c) * a.Hv + h;
-    const int left = sp.len - (int)t0;
-    float v[MT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = tile_row(mt, 4 * g + r);
-        v[mt][r] = t < left ? to_f32(row_at<T>(a.v, sp, t0 + t, h)[col]) : 0.f;
-      }
-    __syncthreads();
-    stage_rows<T>(sk, a.k, sp, t0, left, hk, tid);
-    stage_rows<T>(sq, a.q, sp, t0, left, hk, tid);
-    stage_cols<T>(skt, a.k, sp, t0, left, hk, tid, 512);
-    stage_square<C, false>(st, a.tm + at * C * C, tid);
-    stage_square<C, false>(sp_, a.pm + at * C * C, tid);
-    if (tid < 3 * C) gates[tid] = a.gates[at * 5 * C + tid];
-    if (a.s0)
-#pragma unroll
-      for (int t = 0; t < 8; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) a.s0[at * kHead * kHead + tile_row(t, 4 * g + r) * kHead + col] = S[t][r];
-    __syncthreads();
-
-    floatx4 X[MT], O[MT], U[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) X[mt] = O[mt] = U[mt] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const Parts<3> s = split_pair(S[2 * ks], S[2 * ks + 1]);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        mma(X[mt], staged<NP>(sk, mt * 4 + ks, l), s);
-        mma(O[mt], staged<NP>(sq, mt * 4 + ks, l), s);
+    for (int o = 1; o < 64; o <<= 1) {
+      const double y = __shfl_up(G, o, 64);
+      if (l >= o) G += y;
+    }
+    const double Ge = __shfl(G, C - 1, 64);
+    const float hi = (float)G, lo = (float)(G - (double)hi);
+    if (l < C) {
+      gh[l] = hi;
+      gl[l] = lo;
+      bt[l] = b;
+      float* gates = a.gates + at * (kUnit / 4);
+      gates[l] = expf((float)G);
+      gates[C + l] = expf((float)(Ge - G));
+      gates[2 * C + l] = b;
+      if (kBwd) {
+        a.sums[at * 2 * C + l] = hi;
+        a.sums[at * 2 * C + C + l] = lo;
       }
     }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = tile_row(mt, 4 * g + r);
-        X[mt][r] = gates[2 * C + t] * (v[mt][r] - gates[t] * X[mt][r]);      // R
-        O[mt][r] *= a.scale * gates[t];
-      }
-#pragma unroll
-    for (int js = 0; js < JS; ++js) {
-      const Parts<3> r = split_pair(X[2 * js], X[2 * js + 1]);
-#pragma unroll
-      for (int mt = 2 * js; mt < MT; ++mt) mma(U[mt], staged<3>(st, mt * JS + js, l), r);
-    }
-    const float whole = gates[C - 1];
-#pragma unroll
-    for (int t = 0; t < 8; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) S[t][r] *= whole;
-#pragma unroll
-    for (int js = 0; js < JS; ++js) {
-      const Parts<3> u = split_pair(U[2 * js], U[2 * js + 1]);
-#pragma unroll
-      for (int mt = 2 * js; mt < MT; ++mt) mma(O[mt], staged<3>(sp_, mt * JS + js, l), u);
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = U[2 * js + (e >> 2)][e & 3] * gates[C + 32 * js + 8 * g + e];
-      const Parts<3> ud = split3(x);
-#pragma unroll
-      for (int t = 0; t < 8; ++t) mma(S[t], staged<NP>(skt, t * JS + js, l), ud);
-    }
-    T* o = static_cast<T*>(a.o);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = tile_row(mt, 4 * g + r);
-        if (t < left) o[(((int64_t)sp.b * a.s.T + sp.t0 + t0 + t) * a.Hv + h) * kHead + col] = from_f32<T>(O[mt][r]);
-        if (a.u) a.u[(at * C + t) * kHead + col] = U[mt][r];
-      }
   }
-  if (a.state_out)
+  if (h % share == 0) {                                      // one of the heads that share q and k
+    stage_cols<T>(reinterpret_cast<bf16x8*>(a.kt + atk * K::kCols * kUnit), a.k, sp, t0, left, hk, tid, 256);
+    if (kBwd) stage_cols<T>(reinterpret_cast<bf16x8*>(a.qt + atk * K::kCols * kUnit), a.q, sp, t0, left, hk, tid, 256);
+    if constexpr (NP == 3) {
+      stage_rows<T>(reinterpret_cast<bf16x8*>(a.kr + atk * K::kRows * kUnit), a.k, sp, t0, left, hk, tid);
+      if (!kBwd) stage_rows<T>(reinterpret_cast<bf16x8*>(a.qr + atk * K::kRows * kUnit), a.q, sp, t0, left, hk, tid);
+    }
+  }
+  Parts<NP> xq[4];
+  const int mt = wave % MT;                                  // rows of this wave (C = 32: waves 2, 3 take Q K^T)
+  {
+    const int t = tile_row(mt, m);
+    const T* p = row_at<T>(a.q, sp, t0 + t, hk);
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
+    for (int ks = 0; ks < 4; ++ks) xq[ks] = operand<T>(p + 32 * ks + 8 * g4, t < left);
+  }
+  __syncthreads();
+
+  // row tile mt of K K^T (into am) and of Q K^T (into pm)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) a.state_out[sn + tile_row(t, 4 * g + r) * kHead + col] = S[t][r];
+  for (int nt = 0; nt < MT; ++nt) {
+    const int j = tile_row(nt, m);
+    floatx4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
+    if ((nt >> 1) <= (mt >> 1)) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const Parts<NP> kj = staged<NP>(sk, nt * 4 + ks, l);
+        if (C == 64 || wave < MT) mma(kk, staged<NP>(sk, mt * 4 + ks, l), kj);
+        if (C == 64 || wave >= MT) mma(qk, xq[ks], kj);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = tile_row(mt, 4 * g4 + r);
+      const float d = j <= i ? expf((gh[i] - gh[j]) + (gl[i] - gl[j])) : 0.f;
+      if (C == 64 || wave < MT) am[i][j] = j < i ? bt[i] * kk[r] * d : 0.f;
+      if (C == 64 || wave >= MT) pm[i][j] = j <= i ? a.scale * qk[r] * d : 0.f;
+    }
+  }
+  __syncthreads();
+  pack_square<C, K::kPParts, kBwd>(a.pm + at * K::kP * kUnit, &pm[0][0], LD, tid);
+  for (int i = tid; i < C * LD; i += 256) (&xm[0][0])[i] = 0.f;
+  __syncthreads();
+
+  // (I + A)^-1: blocks of 16 by substitution, a lane a column; then pairs of blocks, and of pairs:
+  // the lower left of the inverse is -Y A21 X with X, Y the inverses above and below it.  (Doubling
+  // products of I - A would cancel: for equal keys its terms grow like binomials.)
+  if (wave < MT && l < 16) {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == l ? 1.f : 0.f;
+#pragma unroll
+      for (int k = 0; k < i; ++k) s = __builtin_fmaf(-am[16 * wave + i][16 * wave + k], x[k], s);
+      x[i] = s;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) xm[16 * wave + i][16 * wave + l] = x[i];
+  }
+  float (*ym)[LD] = pm;
+  __syncthreads();
+  if (wave < C / 32) {
+    const int p = 32 * wave;
+    tile_put(&ym[p][p], LD, tile_f32(&am[p + 16][p], LD, &xm[p][p], LD, 16), 1.f);
+  }
+  __syncthreads();
+  if (wave < C / 32) {
+    const int p = 32 * wave;
+    tile_put(&xm[p + 16][p], LD, tile_f32(&xm[p + 16][p + 16], LD, &ym[p][p], LD, 16), -1.f);
+  }
+  __syncthreads();
+  if constexpr (C == 64) {
+    const int i = 16 * (wave >> 1), j = 16 * (wave & 1);
+    tile_put(&ym[i][j], LD, tile_f32(&am[32 + i][0], LD, &xm[0][j], LD, 32), 1.f);
+    __syncthreads();
+    tile_put(&xm[32 + i][j], LD, tile_f32(&xm[32 + i][32], LD, &ym[0][j], LD, 32), -1.f);
+    __syncthreads();
+  }
+  pack_square<C, 3, kBwd>(a.tm + at * K::kT * kUnit, &xm[0][0], LD, tid);
 }
 
-template <typename T>
-__global__ __launch_bounds__(512) void delta_scan_bwd_kernel(DeltaArgs a) {
-  using L = ScanLds<T>;
-  constexpr int C = L::C, NP = L::NP, MT = L::MT, JS = L::JS;
+// ---------------------------------------------------------------------------
+// The state from chunk to chunk.  256 threads: a wave owns 32 columns of one head's state in two
+// tiles of 16, tile 2 ks + e of its registers the rows tile_row(2 ks + e, .).  The chunk's
+// operands come to LDS by direct loads, each buffer refilled as soon as all four waves are
+// through with it; two blocks share a CU and cover each other's waits.
+// ---------------------------------------------------------------------------
+template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
+  const uint64_t x = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<const P*>((uint64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                                    (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// `units` KiB from src (16-byte aligned) to LDS, by four waves.
+__device__ __forceinline__ void fetch(const void* src, uint32_t lds, int units, int wave, int l) {
+  const char* p = uniform(static_cast<const char*>(src));
+  for (int i = wave; i < units; i += 4) load_lds16(p + (size_t)i * kUnit, 16u * l, lds + i * kUnit);
+}
+// The rows of a chunk (tile_row, summed over the 128 elements) straight from bf16 rows; rows behind
+// the sequence are its last one again (what they give is not used).
+template <int C>
+__device__ __forceinline__ void fetch_rows(const Rows& x, const Span& sp, int64_t t0, int left, int h, uint32_t lds, int wave, int l) {
+  const uint16_t* p = uniform(row_at<uint16_t>(x, sp, t0, h));
+#pragma unroll
+  for (int mt = 0; mt < C / 16; ++mt) {
+    const int t = min(tile_row(mt, l & 15), left - 1);
+    load_lds16(p, (uint32_t)(t * (int)x.st + 32 * wave + 8 * (l >> 4)) * 2u, lds + (mt * 4 + wave) * kUnit);
+  }
+}
+
+// A wave's own [C][32 columns] of a [tokens][128] matrix in LDS, 4 KiB in pieces of 16 bytes;
+// the piece's place turns with the token, so that a column's four groups of tokens meet
+// other banks.
+template <typename T> struct Slice {
+  static constexpr int C = DeltaType<T>::kChunk, kPieces = 2 * sizeof(T), kRow = 32 * sizeof(T);   // 4 or 8 pieces a row
+  __device__ static int turn(int t) { return sizeof(T) == 2 ? (t >> 3) & 3 : ((t >> 3) & 1) << 2; }
+  // byte offset of token 8 g, column 16 n + m; token 8 g + k lies k rows behind it (k % 32 < 8)
+  __device__ static int lane(int g, int n, int m) {
+    constexpr int kPer = 16 / sizeof(T);
+    const int col = 16 * n + m;
+    return 8 * g * kRow + (((col / kPer) ^ turn(8 * g)) << 4) + (col % kPer) * (int)sizeof(T);
+  }
+  __device__ static void fetch(const Rows& x, const Span& sp, int64_t t0, int left, int h, int wave, uint32_t lds, int l) {
+    const T* p = uniform(row_at<T>(x, sp, t0, h) + 32 * wave);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int u = 64 * i + l, t = u / kPieces, tt = min(t, left - 1);
+      load_lds16(p, (uint32_t)(tt * (int)x.st) * (uint32_t)sizeof(T) + (((u % kPieces) ^ turn(t)) << 4), lds + i * kUnit);
+    }
+  }
+  // out: the wave's columns of the chunk's first row, `stride` elements between rows
+  __device__ static void store(const char* lds, T* out, int64_t stride, int left, int l) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int u = 64 * i + l, t = u / kPieces;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(lds + 16 * u);
+      if (t < left) *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(out + t * stride) + (((u % kPieces) ^ turn(t)) << 4)) = x;
+    }
+  }
+};
+
+template <typename T> struct ScanLds {
+  using F = Pack<T, false>;
+  using B = Pack<T, true>;
+  // forward: K then K^T | Q | Tm | P | gates | V, then O
+  static constexpr int kKq = F::kRows > F::kCols ? F::kRows : F::kCols;
+  static constexpr size_t kFwd = (size_t)(kKq + F::kRows + F::kT + F::kP + 1 + 16) * kUnit;
+  static constexpr size_t kFwdState = (size_t)(kKq + F::kT + 1 + 16) * kUnit;
+  // backward: K then Q^T | K^T | Tm^T | P^T | gates
+  static constexpr size_t kBwd = (size_t)(kKq + B::kCols + B::kT + B::kP + 1) * kUnit;
+};
+
+// A [rows][128] fp32 matrix <-> the wave's tiles of it (rows tile_row, two tiles of 16 columns).  The
+// row is a uniform address, the lane's part the same for all of them.
+template <int kTiles>
+__device__ __forceinline__ void tiles_load(floatx4 (&S)[kTiles][2], const float* p, int wave, int l) {
+  const float* q = uniform(p) + 32 * wave;
+  const uint32_t off = 8 * (l >> 4) * kHead + (l & 15);
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[t][n][r] = (q + tile_at(t, r) * kHead + 16 * n)[off];
+}
+template <int kTiles>
+__device__ __forceinline__ void tiles_store(const floatx4 (&S)[kTiles][2], float* p, int wave, int l) {
+  float* q = const_cast<float*>(uniform(p)) + 32 * wave;
+  const uint32_t off = 8 * (l >> 4) * kHead + (l & 15);
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) (q + tile_at(t, r) * kHead + 16 * n)[off] = S[t][n][r];
+}
+
+// kOut: the outputs (and what the backward pass needs).  Otherwise only what a segment does to
+// the state: blockIdx.z 0 what it adds, 1 its product of transitions (V = 0 from the
+// identity).
+template <typename T, bool kOut>
+__global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
+  using K = Pack<T, false>;
+  constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32;
   extern __shared__ __align__(16) char lds[];
-  bf16x8* sk = reinterpret_cast<bf16x8*>(lds);
-  bf16x8* skt = sk + L::kRows;
-  bf16x8* sqt = skt + L::kCols;
-  bf16x8* st = sqt + L::kCols;
-  bf16x8* sp_ = st + L::kSquare;
-  float* gates = reinterpret_cast<float*>(sp_ + L::kSquare);
-  const int h = blockIdx.y, hk = h / (a.Hv / a.Hk), tid = threadIdx.x, l = lane_id(), g = l >> 4;
-  const int col = 16 * (tid >> 6) + (l & 15);
-  const Span sp = span_of<C>(a.s, blockIdx.x);
-  const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead;
+  char* bk = lds;
+  char* bt = bk + ScanLds<T>::kKq * kUnit;
+  char* bg = bt + K::kT * kUnit;
+  char* bv = bg + kUnit;
+  char* bq = bv + 16 * kUnit;
+  char* bp = bq + K::kRows * kUnit;
+  const int h = blockIdx.y, hk = h / (a.Hv / a.Hk), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
+  bv += wave * 4 * kUnit;
+  int piece = 0, c0 = 0, c1;
+  Span sp;
+  if (a.seg) {
+    sp = slot_of(a.s, blockIdx.x, C * a.seg, piece);
+    if (piece < 0) return;
+    c0 = piece * a.seg;
+  } else {
+    sp = span_of(a.s, blockIdx.x, C);
+  }
+  const int chunks = (sp.len + C - 1) / C;
+  const bool last = !a.seg || c0 + a.seg >= chunks;
+  c1 = last ? chunks : c0 + a.seg;
+  const bool ident = !kOut && blockIdx.z == 1;
+  if (!kOut && (last || (ident && piece == 0))) return;      // nobody asks for it
+  const int slot0 = a.s.cu ? span_of(a.s, sp.n, C).slot0 : sp.n * chunks;
+  const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)blockIdx.x * a.Hv + h) * kHead * kHead;
 
-  floatx4 S[8];                                              // dS
-#pragma unroll
-  for (int t = 0; t < 8; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) S[t][r] = a.dstate_out ? a.dstate_out[sn + tile_row(t, 4 * g + r) * kHead + col] : 0.f;
-
-  for (int c = (sp.len + C - 1) / C - 1; c >= 0; --c) {
-    const int64_t t0 = (int64_t)c * C, at = (int64_t)(sp.slot0 + c) * a.Hv + h;
-    const int left = sp.len - (int)t0;
-    float d[MT][4];                                          // dO
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = tile_row(mt, 4 * g + r);
-        d[mt][r] = t < left ? to_f32(row_at<T>(a.dout, sp, t0 + t, h)[col]) : 0.f;
-      }
-    __syncthreads();
-    stage_rows<T>(sk, a.k, sp, t0, left, hk, tid);
-    stage_cols<T>(skt, a.k, sp, t0, left, hk, tid, 512);
-    stage_cols<T>(sqt, a.q, sp, t0, left, hk, tid, 512);
-    stage_square<C, true>(st, a.tm + at * C * C, tid);
-    stage_square<C, true>(sp_, a.pm + at * C * C, tid);
-    if (tid < 3 * C) gates[tid] = a.gates[at * 5 * C + tid];
+  floatx4 S[8][2];
+  const float* from = piece == 0 ? (a.state_in ? a.state_in + sn : nullptr) : kOut ? a.init + gn : nullptr;
+  if (from) {
+    tiles_load(S, from, wave, l);
+  } else {
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) a.ds1[at * kHead * kHead + tile_row(t, 4 * g + r) * kHead + col] = S[t][r];
-    __syncthreads();
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          S[t][n][r] = ident && tile_row(t, 4 * g + r) == 32 * wave + 16 * n + (l & 15) ? 1.f : 0.f;
+  }
 
-    floatx4 X[MT], R[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) X[mt] = R[mt] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const Parts<3> s = split_pair(S[2 * ks], S[2 * ks + 1]);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) mma(X[mt], staged<NP>(sk, mt * 4 + ks, l), s);
-    }
+  auto fetch_k = [&](int64_t t0, int left, int64_t atk) {
+    if constexpr (NP == 1) fetch_rows<C>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
+    else fetch(a.kr + atk * K::kRows * kUnit, lds_addr(bk), K::kRows, wave, l);
+  };
+  auto fetch_q = [&](int64_t t0, int left, int64_t atk) {
+    if constexpr (NP == 1) fetch_rows<C>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
+    else fetch(a.qr + atk * K::kRows * kUnit, lds_addr(bq), K::kRows, wave, l);
+  };
+  const int slice[2] = {Slice<T>::lane(g, 0, l & 15), Slice<T>::lane(g, 1, l & 15)};
+  auto fetch_v = [&](int64_t t0, int left) {
+    if (!ident) Slice<T>::fetch(a.v, sp, t0, left, h, wave, lds_addr(bv), l);
+  };
+  if (c0 < c1) {
+    const int64_t t0 = (int64_t)c0 * C, at = (int64_t)(slot0 + c0) * a.Hv + h, atk = (int64_t)(slot0 + c0) * a.Hk + hk;
+    const int left = sp.len - (int)t0;
+    if (kOut) fetch_q(t0, left, atk);
+    fetch(a.tm + at * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
+    fetch_v(t0, left);
+    fetch_k(t0, left, atk);
+    if (kOut) fetch(a.pm + at * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
+    fetch(a.gates + at * (kUnit / 4), lds_addr(bg), 1, wave, l);
+  }
+  for (int c = c0; c < c1; ++c) {
+    const int64_t t0 = (int64_t)c * C, at = (int64_t)(slot0 + c) * a.Hv + h, atk = (int64_t)(slot0 + c) * a.Hk + hk;
+    const int left = sp.len - (int)t0;
+    const bool more = c + 1 < c1;
+    const int64_t t1 = t0 + C;
+    const int left1 = left - C;
+    wait_loads();
+    __syncthreads();
+    if (kOut && a.s0) tiles_store(S, a.s0 + at * kHead * kHead, wave, l);
+
+    const bf16x8* sk = reinterpret_cast<const bf16x8*>(bk);
+    const bf16x8* sq = reinterpret_cast<const bf16x8*>(bq);
+    const bf16x8* st = reinterpret_cast<const bf16x8*>(bt);
+    const bf16x8* spm = reinterpret_cast<const bf16x8*>(bp);
+    const float* gates = reinterpret_cast<const float*>(bg);
+    floatx4 X[MT][2], O[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) X[mt][r] *= gates[C + tile_row(mt, 4 * g + r)];
+      for (int n = 0; n < 2; ++n) X[mt][n] = O[mt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      Parts<3> s[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) s[n] = split_pair(S[2 * ks][n], S[2 * ks + 1][n]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const Parts<NP> k = staged<NP>(sk, mt * 4 + ks, l);
+        mma(X[mt][0], k, s[0]);
+        mma(X[mt][1], k, s[1]);
+      }
+      if constexpr (kOut) {
+        // for a bf16 output two parts of the state do (2^-17 of it)
+        constexpr int kS = NP == 1 ? 2 : 3;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const Parts<NP> q = staged<NP>(sq, mt * 4 + ks, l);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            Parts<kS> x;
+#pragma unroll
+            for (int i = 0; i < kS; ++i) x.p[i] = s[n].p[i];
+            mma(O[mt][n], q, x);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);                     // (later steps' operands are not read ahead into registers)
+    }
+    __syncthreads();                                         // K and Q are free
+    fetch(a.kt + atk * K::kCols * kUnit, lds_addr(bk), K::kCols, wave, l);
+    if (kOut && more) fetch_q(t1, left1, atk + a.Hk);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const floatx4 e = *reinterpret_cast<const floatx4*>(gates + 8 * g + tile_at(mt, 0));
+      const floatx4 b = *reinterpret_cast<const floatx4*>(gates + 2 * C + 8 * g + tile_at(mt, 0));
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = ident ? 0.f : to_f32(*reinterpret_cast<const T*>(bv + slice[n] + tile_at(mt, r) * Slice<T>::kRow));
+          X[mt][n][r] = 8 * g + tile_at(mt, r) < left ? b[r] * (v - e[r] * X[mt][n][r]) : 0.f;          // R
+          if (kOut) O[mt][n][r] *= a.scale * e[r];
+        }
+    }
+    floatx4 U[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) U[mt][0] = U[mt][1] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
-      const float x[8] = {d[2 * js][0], d[2 * js][1], d[2 * js][2], d[2 * js][3],
-                          d[2 * js + 1][0], d[2 * js + 1][1], d[2 * js + 1][2], d[2 * js + 1][3]};
-      const Parts<NP> p = parts_of<NP>(x);
+      Parts<3> r[2];
 #pragma unroll
-      for (int mt = 0; mt < 2 * js + 2; ++mt) mma(X[mt], staged<3>(sp_, mt * JS + js, l), p);    // dU
+      for (int n = 0; n < 2; ++n) r[n] = split_pair(X[2 * js][n], X[2 * js + 1][n]);
+#pragma unroll
+      for (int mt = 2 * js; mt < MT; ++mt) {
+        const Parts<3> x = staged<3>(st, Square<C>::at(mt, js, false), l);
+        mma(U[mt][0], x, r[0]);
+        mma(U[mt][1], x, r[1]);
+      }
     }
+    wait_loads();
+    __syncthreads();                                         // K^T is there; Tm and this wave's V are free
+    if (more) fetch(a.tm + (at + a.Hv) * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
+    if constexpr (kOut) {
 #pragma unroll
-    for (int js = 0; js < JS; ++js) {
-      const Parts<3> p = split_pair(X[2 * js], X[2 * js + 1]);
+      for (int js = 0; js < JS; ++js) {
+        Parts<K::kPParts> u[2];
 #pragma unroll
-      for (int mt = 0; mt < 2 * js + 2; ++mt) mma(R[mt], staged<3>(st, mt * JS + js, l), p);     // dR
+        for (int n = 0; n < 2; ++n) {
+          const Parts<3> p = split_pair(U[2 * js][n], U[2 * js + 1][n]);
+#pragma unroll
+          for (int i = 0; i < K::kPParts; ++i) u[n].p[i] = p.p[i];
+        }
+#pragma unroll
+        for (int mt = 2 * js; mt < MT; ++mt) {
+          const Parts<K::kPParts> x = staged<K::kPParts>(spm, Square<C>::at(mt, js, false), l);
+          mma(O[mt][0], x, u[0]);
+          mma(O[mt][1], x, u[1]);
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            *reinterpret_cast<T*>(bv + slice[n] + tile_at(mt, r) * Slice<T>::kRow) = from_f32<T>(O[mt][n][r]);
+      if (a.u) tiles_store(U, a.u + at * C * kHead, wave, l);
+      asm volatile("" ::: "memory");                         // (a wave's LDS accesses keep their order)
+      Slice<T>::store(bv, static_cast<T*>(a.o) + (((int64_t)sp.b * a.s.T + sp.t0 + t0) * a.Hv + h) * kHead + 32 * wave,
+                      (int64_t)a.Hv * kHead, left, l);
     }
-    T* dv = static_cast<T*>(a.dv);
+    if (more) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the wave has read its slice
+      fetch_v(t1, left1);
+    }
     const float whole = gates[C - 1];
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) S[t][r] *= whole;
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][n][r] *= whole;
+#pragma unroll
+    for (int js = 0; js < JS; ++js) {
+      Parts<3> u[2];
+      float d[8];
+      load8(gates + C + 32 * js + 8 * g, d);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = U[2 * js + (e >> 2)][n][e & 3] * d[e];
+        u[n] = split3(x);
+      }
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const Parts<NP> k = staged<NP>(sk, t * JS + js, l);
+        mma(S[t][0], k, u[0]);
+        mma(S[t][1], k, u[1]);
+      }
+    }
+    __syncthreads();                                         // all buffers but Q, Tm and V are free
+    if (more) {
+      fetch_k(t1, left1, atk + a.Hk);
+      if (kOut) fetch(a.pm + (at + a.Hv) * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
+      fetch(a.gates + (at + a.Hv) * (kUnit / 4), lds_addr(bg), 1, wave, l);
+    }
+  }
+  if (kOut ? last && a.state_out != nullptr : true)
+    tiles_store(S, kOut ? a.state_out + sn : (ident ? a.move : a.add) + gn, wave, l);
+}
+
+// kOut: dv, and the gradients of the states behind the chunks and of R that the last kernel reads.
+// Otherwise what a segment adds to the gradient of the state before it.
+template <typename T, bool kOut>
+__global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
+  using K = Pack<T, true>;
+  constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32;
+  extern __shared__ __align__(16) char lds[];
+  char* bk = lds;
+  char* bkt = bk + ScanLds<T>::kKq * kUnit;
+  char* bt = bkt + K::kCols * kUnit;
+  char* bp = bt + K::kT * kUnit;
+  char* bg = bp + K::kP * kUnit;
+  const int h = blockIdx.y, hk = h / (a.Hv / a.Hk), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
+  int piece = 0, c0 = 0;
+  Span sp;
+  if (a.seg) {
+    sp = slot_of(a.s, blockIdx.x, C * a.seg, piece);
+    if (piece < 0) return;
+    c0 = piece * a.seg;
+  } else {
+    sp = span_of(a.s, blockIdx.x, C);
+  }
+  const int chunks = (sp.len + C - 1) / C;
+  const bool last = !a.seg || c0 + a.seg >= chunks;
+  const int c1 = last ? chunks : c0 + a.seg;
+  if (!kOut && piece == 0) return;                           // nobody asks for it
+  const int slot0 = a.s.cu ? span_of(a.s, sp.n, C).slot0 : sp.n * chunks;
+  const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)blockIdx.x * a.Hv + h) * kHead * kHead;
+
+  floatx4 S[8][2];                                           // dS
+  const float* from = last ? (a.dstate_out ? a.dstate_out + sn : nullptr) : kOut ? a.init + gn : nullptr;
+  if (from) {
+    tiles_load(S, from, wave, l);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) S[t][0] = S[t][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  float d[MT][2][4];                                         // dO
+  auto load_do = [&](int64_t t0, int left) {
+    const T* p = uniform(row_at<T>(a.dout, sp, t0, h) + 32 * wave);
+    const uint32_t off = 8 * g * (uint32_t)a.dout.st + (l & 15);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = tile_row(mt, 4 * g + r);
-        const float beta = gates[2 * C + t];
-        a.dr[(at * C + t) * kHead + col] = R[mt][r];
-        if (t < left) dv[(((int64_t)sp.b * a.s.T + sp.t0 + t0 + t) * a.Hv + h) * kHead + col] = from_f32<T>(beta * R[mt][r]);
-        R[mt][r] *= -beta * gates[t];
-        d[mt][r] *= a.scale * gates[t];
-      }
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int js = 0; js < JS; ++js) {
-      const float x[8] = {d[2 * js][0], d[2 * js][1], d[2 * js][2], d[2 * js][3],
-                          d[2 * js + 1][0], d[2 * js + 1][1], d[2 * js + 1][2], d[2 * js + 1][3]};
-      const Parts<3> p = split3(x), r = split_pair(R[2 * js], R[2 * js + 1]);
+        for (int r = 0; r < 4; ++r)
+          d[mt][n][r] = 8 * g + tile_at(mt, r) < left ? to_f32((p + tile_at(mt, r) * a.dout.st + 16 * n)[off]) : 0.f;
+  };
+  auto fetch_k = [&](int64_t t0, int left, int64_t atk) {
+    if constexpr (NP == 1) fetch_rows<C>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
+    else fetch(a.kr + atk * K::kRows * kUnit, lds_addr(bk), K::kRows, wave, l);
+  };
+  if (c0 < c1) {
+    const int64_t t0 = (int64_t)(c1 - 1) * C, at = (int64_t)(slot0 + c1 - 1) * a.Hv + h, atk = (int64_t)(slot0 + c1 - 1) * a.Hk + hk;
+    load_do(t0, sp.len - (int)t0);
+    fetch_k(t0, sp.len - (int)t0, atk);
+    fetch(a.gates + at * (kUnit / 4), lds_addr(bg), 1, wave, l);
+    fetch(a.pm + at * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
+    fetch(a.tm + at * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
+    fetch(a.kt + atk * K::kCols * kUnit, lds_addr(bkt), K::kCols, wave, l);
+  }
+  for (int c = c1 - 1; c >= c0; --c) {
+    const int64_t t0 = (int64_t)c * C, at = (int64_t)(slot0 + c) * a.Hv + h, atk = (int64_t)(slot0 + c) * a.Hk + hk;
+    const int left = sp.len - (int)t0;
+    const bool more = c > c0;
+    wait_loads();
+    __syncthreads();
+    if (kOut) tiles_store(S, a.ds1 + at * kHead * kHead, wave, l);
+
+    const bf16x8* sk = reinterpret_cast<const bf16x8*>(bk);
+    const bf16x8* skt = reinterpret_cast<const bf16x8*>(bkt);
+    const bf16x8* st = reinterpret_cast<const bf16x8*>(bt);
+    const bf16x8* spm = reinterpret_cast<const bf16x8*>(bp);
+    const float* gates = reinterpret_cast<const float*>(bg);
+    floatx4 X[MT][2], R[MT][2];
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        mma(S[t], staged<NP>(sqt, t * JS + js, l), p);
-        mma(S[t], staged<NP>(skt, t * JS + js, l), r);
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) X[mt][n] = R[mt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      Parts<3> s[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) s[n] = split_pair(S[2 * ks][n], S[2 * ks + 1][n]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const Parts<NP> k = staged<NP>(sk, mt * 4 + ks, l);
+        mma(X[mt][0], k, s[0]);
+        mma(X[mt][1], k, s[1]);
       }
     }
-  }
-  if (a.dstate_in)
+    __syncthreads();                                         // K is free
+    fetch(a.qt + atk * K::kCols * kUnit, lds_addr(bk), K::kCols, wave, l);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const floatx4 e = *reinterpret_cast<const floatx4*>(gates + C + 8 * g + tile_at(mt, 0));
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) X[mt][n][r] = 8 * g + tile_at(mt, r) < left ? X[mt][n][r] * e[r] : 0.f;
+    }
+#pragma unroll
+    for (int js = 0; js < JS; ++js) {
+      Parts<NP> p[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float x[8] = {d[2 * js][n][0], d[2 * js][n][1], d[2 * js][n][2], d[2 * js][n][3],
+                            d[2 * js + 1][n][0], d[2 * js + 1][n][1], d[2 * js + 1][n][2], d[2 * js + 1][n][3]};
+        p[n] = parts_of<NP>(x);
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2 * js + 2; ++mt) {
+        const Parts<3> x = staged<3>(spm, Square<C>::at(mt, js, true), l);
+        mma(X[mt][0], x, p[0]);                              // dU
+        mma(X[mt][1], x, p[1]);
+      }
+    }
+#pragma unroll
+    for (int js = 0; js < JS; ++js) {
+      Parts<3> p[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) p[n] = split_pair(X[2 * js][n], X[2 * js + 1][n]);
+#pragma unroll
+      for (int mt = 0; mt < 2 * js + 2; ++mt) {
+        const Parts<3> x = staged<3>(st, Square<C>::at(mt, js, true), l);
+        mma(R[mt][0], x, p[0]);                              // dR
+        mma(R[mt][1], x, p[1]);
+      }
+    }
+    wait_loads();
+    __syncthreads();                                         // Q^T is there; Tm^T and P^T are free
+    if (more) {
+      fetch(a.pm + (at - a.Hv) * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
+      fetch(a.tm + (at - a.Hv) * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
+    }
+    const float whole = gates[C - 1];
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) a.dstate_in[sn + tile_row(t, 4 * g + r) * kHead + col] = S[t][r];
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][n][r] *= whole;
+    T* dv = kOut ? const_cast<T*>(uniform(static_cast<const T*>(a.dv) + (((int64_t)sp.b * a.s.T + sp.t0 + t0) * a.Hv + h) * kHead + 32 * wave)) : nullptr;
+    const uint32_t off = 8 * g * (uint32_t)(a.Hv * kHead) + (l & 15);
+    if (kOut) tiles_store(R, a.dr + at * C * kHead, wave, l);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const floatx4 e = *reinterpret_cast<const floatx4*>(gates + 8 * g + tile_at(mt, 0));
+      const floatx4 b = *reinterpret_cast<const floatx4*>(gates + 2 * C + 8 * g + tile_at(mt, 0));
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (kOut && 8 * g + tile_at(mt, r) < left)
+            (dv + tile_at(mt, r) * (int64_t)a.Hv * kHead + 16 * n)[off] = from_f32<T>(b[r] * R[mt][n][r]);
+          R[mt][n][r] *= -b[r] * e[r];
+          d[mt][n][r] *= a.scale * e[r];
+        }
+    }
+#pragma unroll
+    for (int js = 0; js < JS; ++js) {
+      Parts<3> p[2], q[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float x[8] = {d[2 * js][n][0], d[2 * js][n][1], d[2 * js][n][2], d[2 * js][n][3],
+                            d[2 * js + 1][n][0], d[2 * js + 1][n][1], d[2 * js + 1][n][2], d[2 * js + 1][n][3]};
+        p[n] = split3(x);
+        q[n] = split_pair(R[2 * js][n], R[2 * js + 1][n]);
+      }
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const Parts<NP> x = staged<NP>(sk, t * JS + js, l), y = staged<NP>(skt, t * JS + js, l);
+        mma(S[t][0], x, p[0]);
+        mma(S[t][1], x, p[1]);
+        mma(S[t][0], y, q[0]);
+        mma(S[t][1], y, q[1]);
+      }
+    }
+    if (more) load_do(t0 - C, left + C);
+    __syncthreads();                                         // all buffers but Tm^T and P^T are free
+    if (more) {
+      fetch_k(t0 - C, left + C, atk - a.Hk);
+      fetch(a.kt + (atk - a.Hk) * K::kCols * kUnit, lds_addr(bkt), K::kCols, wave, l);
+      fetch(a.gates + (at - a.Hv) * (kUnit / 4), lds_addr(bg), 1, wave, l);
+    }
+  }
+  if (kOut ? piece == 0 && a.dstate_in != nullptr : true) tiles_store(S, kOut ? a.dstate_in + sn : a.add + gn, wave, l);
+}
+
+// The states before the segments (kBwd: the gradients behind them) from what each adds and its
+// product of transitions: S <- move S + add (dS <- move^T dS + add), segment after segment.  512
+// threads and 16 columns a block: a wave owns the rows tile_row(wave, .), the state goes round
+// through LDS.
+template <bool kBwd>
+__global__ __launch_bounds__(512) void delta_join_kernel(DeltaArgs a, int chunk) {
+  __shared__ __align__(16) bf16x8 buf[2][4 * 3 * 64];
+  const int h = blockIdx.y, wave = threadIdx.x >> 6, l = lane_id(), g = l >> 4, m = l & 15, col = 16 * blockIdx.z + m;
+  const Span sp = span_of(a.s, blockIdx.x, chunk * a.seg);
+  const int pieces = (sp.len + chunk * a.seg - 1) / (chunk * a.seg);
+  if (pieces == 0) {                                         // no token: no segment to hand the state on
+    const float* from = kBwd ? a.dstate_out : a.state_in;
+    float* to = kBwd ? a.dstate_in : a.state_out;
+    if (to)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t o = (((int64_t)sp.n * a.Hv + h) * kHead + tile_row(wave, 4 * g + r)) * kHead + col;
+        to[o] = from ? from[o] : 0.f;
+      }
+  }
+  if (pieces < 2) return;
+  auto at = [&](int p) { return ((int64_t)(sp.slot0 + p) * a.Hv + h) * kHead * kHead; };
+  auto tile = [&](const float* x) {
+    floatx4 y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = x[tile_row(wave, 4 * g + r) * kHead + col];
+    return y;
+  };
+  float mv[4][8];
+  auto load_move = [&](int p) {                              // rows tile_row(wave, m) of move, or of its transpose
+    const float* x = a.move + at(p);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if constexpr (kBwd) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mv[ks][e] = x[(32 * ks + 8 * g + e) * kHead + tile_row(wave, m)];
+      } else {
+        load8(x + tile_row(wave, m) * kHead + 32 * ks + 8 * g, mv[ks]);
+      }
+    }
+  };
+  const int first = kBwd ? pieces - 1 : 0, step = kBwd ? -1 : 1;
+  floatx4 S = tile(a.add + at(first));                       // the first one's start is in it
+  if (pieces > 2) load_move(first + step);
+  for (int i = 1, p = first + step; i < pieces; ++i, p += step) {
+    float* init = a.init + at(p);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) init[tile_row(wave, 4 * g + r) * kHead + col] = S[r];
+    if (i + 1 == pieces) break;
+    const float x[8] = {S[0], S[1], S[2], S[3], 0.f, 0.f, 0.f, 0.f};
+    const Parts<3> s = split3(x);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      const u32x4 w = __builtin_bit_cast(u32x4, s.p[n]);
+      *reinterpret_cast<uint2*>(reinterpret_cast<char*>(&buf[i & 1][((wave >> 1) * 3 + n) * 64 + l]) + 8 * (wave & 1)) = uint2{w[0], w[1]};
+    }
+    S = tile(a.add + at(p));
+    Parts<3> k[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) k[ks] = split3(mv[ks]);
+    if (i + 2 < pieces) load_move(p + step);
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) mma(S, k[ks], staged<3>(buf[i & 1], ks, l));
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -652,7 +1050,7 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaArgs a) {
   float* cross = fs + C;                                     // [4]
   const int slot = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, l = lane_id(), g = l >> 4, m = l & 15;
   int c;
-  const Span sp = slot_of<C>(a.s, slot, c);
+  const Span sp = slot_of(a.s, slot, C, c);
   if (c < 0) return;
   const int64_t t0 = (int64_t)c * C;
   const int left = sp.len - (int)t0, share = a.Hv / a.Hk;
@@ -676,7 +1074,7 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaArgs a) {
       *reinterpret_cast<floatx4*>(su + t * LR + e) = *reinterpret_cast<const floatx4*>(a.u + (at * C + t) * kHead + e);
       *reinterpret_cast<floatx4*>(sr + t * LR + e) = *reinterpret_cast<const floatx4*>(a.dr + (at * C + t) * kHead + e);
     }
-    for (int i = tid; i < 5 * C; i += 256) gates[i] = a.gates[at * 5 * C + i];
+    for (int i = tid; i < 5 * C; i += 256) gates[i] = i < 3 * C ? a.gates[at * 256 + i] : a.sums[at * 2 * C + i - 3 * C];
     __syncthreads();
 
     // E, F, Q K^T, K K^T by tiles of tokens
@@ -907,19 +1305,56 @@ namespace {
 constexpr size_t kAlign = 256;
 inline size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
-struct DeltaSizes { int C; int64_t slots; size_t tm, gates, s0, u; };
-// Sizes of one call; slots 0: out of range.
-DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hv, int dtype) {
+// What one call lays out, from its sizes alone (so a backward pass finds what its forward kept).
+struct DeltaSizes {
+  int C, seg;                 // tokens of a chunk; chunks of a segment, 0: none
+  int64_t slots, segs;        // 0 slots: out of range
+  size_t tm, pm, gates, sums, kt, qt, kr, qr, states, s0, u;
+  size_t workspace(bool backward) const {
+    return backward ? tm + pm + gates + sums + kt + qt + kr + 2 * states + s0 + u : tm + pm + gates + kt + kr + qr + 3 * states;
+  }
+  size_t saved() const { return s0 + u + states; }
+};
+template <typename T, bool kBwd> void pack_sizes(DeltaSizes& z, size_t n, size_t nk) {
+  using K = gsa::Pack<T, kBwd>;
+  z.tm = n * K::kT * gsa::kUnit;
+  z.pm = n * K::kP * gsa::kUnit;
+  z.gates = n * gsa::kUnit;
+  z.kt = nk * K::kCols * gsa::kUnit;
+  if (kBwd) {
+    z.sums = up(n * 2 * K::C * 4);
+    z.qt = z.kt;
+  }
+  if (K::NP == 3) {
+    z.kr = nk * K::kRows * gsa::kUnit;
+    if (!kBwd) z.qr = z.kr;
+  }
+}
+DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtype, bool backward) {
   DeltaSizes z{};
   z.C = dtype == GSA_DTYPE_BF16 ? gsa::DeltaType<uint16_t>::kChunk : gsa::DeltaType<float>::kChunk;
-  if (B < 1 || T < 1 || N < 1 || Hv < 1 || !dtype_size(dtype)) return z;
-  z.slots = packed ? (int64_t)T / z.C + N : (int64_t)B * ((T + z.C - 1) / z.C);
-  if (z.slots > 0x7fffffff) z.slots = 0;
-  const size_t n = (size_t)z.slots * Hv;
-  z.tm = up(n * z.C * z.C * 4);
-  z.gates = up(n * 5 * z.C * 4);
-  z.s0 = up(n * 128 * 128 * 4);
-  z.u = up(n * z.C * 128 * 4);
+  if (B < 1 || T < 1 || N < 1 || Hk < 1 || Hv < Hk || Hv % Hk || !dtype_size(dtype)) return z;
+  const int64_t nc = (T + z.C - 1) / z.C;
+  z.slots = packed ? (int64_t)T / z.C + N : B * nc;
+  if (z.slots > 0x7fffffff) {
+    z.slots = 0;
+    return z;
+  }
+  // Segments of equal length where the sequences and heads alone would leave CUs without a block
+  if ((int64_t)N * Hv < 384) {
+    int64_t seg = (z.slots * Hv + 511) / 512;
+    if (seg < 4) seg = 4;
+    if (3 * seg <= nc) {
+      z.seg = (int)seg;
+      z.segs = packed ? (int64_t)T / (z.C * seg) + N : B * ((nc + seg - 1) / seg);
+    }
+  }
+  const size_t n = (size_t)z.slots * Hv, nk = (size_t)z.slots * Hk;
+  if (dtype == GSA_DTYPE_BF16) backward ? pack_sizes<uint16_t, true>(z, n, nk) : pack_sizes<uint16_t, false>(z, n, nk);
+  else backward ? pack_sizes<float, true>(z, n, nk) : pack_sizes<float, false>(z, n, nk);
+  z.states = (size_t)z.segs * Hv * 128 * 128 * 4;
+  z.s0 = n * 128 * 128 * 4;
+  z.u = n * z.C * 128 * 4;
   return z;
 }
 
@@ -935,25 +1370,39 @@ template <auto kKernel> int allow_lds(size_t bytes) {
   return GSA_OK;
 }
 
-template <typename T> int launch_forward(const gsa::DeltaArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(gsa::delta_chunk_kernel<T>, dim3(a.s.slots, a.Hv), dim3(256), 0, s, a);
+template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
+  using L = gsa::ScanLds<T>;
+  static_assert(2 * L::kFwd <= 160 * 1024, "two blocks a CU");
+  hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, false>), dim3(z.slots, a.Hv), dim3(256), 0, s, a);
   if (const int e = launch_status()) return e;
-  constexpr size_t lds = gsa::ScanLds<T>::kFwd;
-  static_assert(lds <= 160 * 1024);
-  if (const int e = allow_lds<gsa::delta_scan_kernel<T>>(lds)) return e;
-  hipLaunchKernelGGL(gsa::delta_scan_kernel<T>, dim3(a.s.N, a.Hv), dim3(512), lds, s, a);
+  if (a.seg) {
+    if (const int e = allow_lds<gsa::delta_scan_kernel<T, false>>(L::kFwdState)) return e;
+    hipLaunchKernelGGL((gsa::delta_scan_kernel<T, false>), dim3(z.segs, a.Hv, 2), dim3(256), L::kFwdState, s, a);
+    if (const int e = launch_status()) return e;
+    hipLaunchKernelGGL(gsa::delta_join_kernel<false>, dim3(a.s.N, a.Hv, 8), dim3(512), 0, s, a, z.C);
+    if (const int e = launch_status()) return e;
+  }
+  if (const int e = allow_lds<gsa::delta_scan_kernel<T, true>>(L::kFwd)) return e;
+  hipLaunchKernelGGL((gsa::delta_scan_kernel<T, true>), dim3(a.seg ? z.segs : a.s.N, a.Hv), dim3(256), L::kFwd, s, a);
   return launch_status();
 }
-template <typename T> int launch_backward(const gsa::DeltaArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(gsa::delta_chunk_kernel<T>, dim3(a.s.slots, a.Hv), dim3(256), 0, s, a);
-  if (const int e = launch_status()) return e;
+template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
   constexpr size_t lds = gsa::ScanLds<T>::kBwd, lds_grads = gsa::GradLds<T>::kBytes;
-  static_assert(lds <= 160 * 1024 && lds_grads <= 160 * 1024);
-  if (const int e = allow_lds<gsa::delta_scan_bwd_kernel<T>>(lds)) return e;
-  if (const int e = allow_lds<gsa::delta_grads_kernel<T>>(lds_grads)) return e;
-  hipLaunchKernelGGL(gsa::delta_scan_bwd_kernel<T>, dim3(a.s.N, a.Hv), dim3(512), lds, s, a);
+  static_assert(2 * lds <= 160 * 1024 && lds_grads <= 160 * 1024);
+  hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, true>), dim3(z.slots, a.Hv), dim3(256), 0, s, a);
   if (const int e = launch_status()) return e;
-  hipLaunchKernelGGL(gsa::delta_grads_kernel<T>, dim3(a.s.slots, a.Hk), dim3(256), lds_grads, s, a);
+  if (a.seg) {
+    if (const int e = allow_lds<gsa::delta_scan_bwd_kernel<T, false>>(lds)) return e;
+    hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, false>), dim3(z.segs, a.Hv), dim3(256), lds, s, a);
+    if (const int e = launch_status()) return e;
+    hipLaunchKernelGGL(gsa::delta_join_kernel<true>, dim3(a.s.N, a.Hv, 8), dim3(512), 0, s, a, z.C);
+    if (const int e = launch_status()) return e;
+  }
+  if (const int e = allow_lds<gsa::delta_scan_bwd_kernel<T, true>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, true>), dim3(a.seg ? z.segs : a.s.N, a.Hv), dim3(256), lds, s, a);
+  if (const int e = launch_status()) return e;
+  if (const int e = allow_lds<gsa::delta_grads_kernel<T>>(lds_grads)) return e;
+  hipLaunchKernelGGL(gsa::delta_grads_kernel<T>, dim3(z.slots, a.Hk), dim3(256), lds_grads, s, a);
   return launch_status();
 }
 
@@ -964,10 +1413,11 @@ int delta_args(const gsa_delta_args* x, bool backward, gsa::DeltaArgs& a, DeltaS
   if (x->B < 1 || x->T < 1 || x->N < 1 || x->Hk < 1 || x->Hv < x->Hk || x->Hv % x->Hk || x->Hv > 65535 || x->d != 128)
     return GSA_ERR_SHAPE;
   if (x->cu_seqlens ? x->B != 1 || (x->cu_bytes != 4 && x->cu_bytes != 8) : x->N != x->B) return GSA_ERR_SHAPE;
-  z = delta_sizes(x->B, x->T, x->N, x->cu_seqlens != nullptr, x->Hv, x->dtype);
-  if (!z.slots) return GSA_ERR_SHAPE;
-  const size_t need = 2 * z.tm + z.gates + (backward ? z.s0 + z.u : 0);
-  if (x->ws_bytes < need || (x->saved && x->saved_bytes < z.s0 + z.u)) return GSA_ERR_SHAPE;
+  z = delta_sizes(x->B, x->T, x->N, x->cu_seqlens != nullptr, x->Hk, x->Hv, x->dtype, backward);
+  if (!z.slots || x->ws_bytes < z.workspace(backward) || (x->saved && x->saved_bytes < z.saved())) return GSA_ERR_SHAPE;
+  // a chunk's rows are addressed by 32-bit offsets
+  for (int64_t st : {x->q_st, x->k_st, x->v_st, backward ? x->do_st : (int64_t)0})
+    if (st < 0 || st * 64 * dtype_size(x->dtype) >= (int64_t)1 << 31) return GSA_ERR_SHAPE;
   auto vec = [&](const void* p, int64_t sb, int64_t st, int64_t sh) {
     return vec_ok(p, sb, st, x->dtype) && sh % (x->dtype == GSA_DTYPE_BF16 ? 8 : 4) == 0;
   };
@@ -982,7 +1432,7 @@ int delta_args(const gsa_delta_args* x, bool backward, gsa::DeltaArgs& a, DeltaS
       !aligned(x->dbeta, dtype_size(x->beta_dtype)) || (x->cu_seqlens && !aligned(x->cu_seqlens, x->cu_bytes)))
     return GSA_ERR_ALIGN;
   a = gsa::DeltaArgs{};
-  a.s = {x->cu_seqlens, x->cu_bytes == 8, x->N, x->T, (int)z.slots};
+  a.s = {x->cu_seqlens, x->cu_bytes == 8, x->N, x->T};
   a.q = {x->q, x->q_sb, x->q_st, x->q_sh};
   a.k = {x->k, x->k_sb, x->k_st, x->k_sh};
   a.v = {x->v, x->v_sb, x->v_st, x->v_sh};
@@ -996,18 +1446,36 @@ int delta_args(const gsa_delta_args* x, bool backward, gsa::DeltaArgs& a, DeltaS
   a.o = x->o;
   a.state_out = x->state_out;
   char* w = static_cast<char*>(x->ws);
-  a.tm = reinterpret_cast<float*>(w);
-  a.pm = reinterpret_cast<float*>(w + z.tm);
-  a.gates = reinterpret_cast<float*>(w + 2 * z.tm);
+  auto take = [&](size_t n) {
+    char* p = w;
+    w += n;
+    return p;
+  };
+  a.tm = take(z.tm);
+  a.pm = take(z.pm);
+  a.gates = reinterpret_cast<float*>(take(z.gates));
+  a.sums = reinterpret_cast<float*>(take(z.sums));
+  a.kt = take(z.kt);
+  a.qt = take(z.qt);
+  a.kr = take(z.kr);
+  a.qr = take(z.qr);
+  a.seg = z.seg;
+  a.segs = (int)z.segs;
+  a.add = reinterpret_cast<float*>(take(z.states));
+  a.init = reinterpret_cast<float*>(take(z.states));
   if (x->saved) {
-    a.s0 = static_cast<float*>(x->saved);
-    a.u = reinterpret_cast<float*>(static_cast<char*>(x->saved) + z.s0);
+    char* p = static_cast<char*>(x->saved);
+    a.s0 = reinterpret_cast<float*>(p);
+    a.u = reinterpret_cast<float*>(p + z.s0);
+    a.move = reinterpret_cast<float*>(p + z.s0 + z.u);
+  } else {
+    a.move = reinterpret_cast<float*>(take(z.states));
   }
   if (backward) {
+    a.ds1 = reinterpret_cast<float*>(take(z.s0));
+    a.dr = reinterpret_cast<float*>(take(z.u));
     a.dout = {x->dout, x->do_sb, x->do_st, x->do_sh};
     a.dstate_out = x->dstate_out;
-    a.ds1 = reinterpret_cast<float*>(w + 2 * z.tm + z.gates);
-    a.dr = reinterpret_cast<float*>(w + 2 * z.tm + z.gates + z.s0);
     a.dq = x->dq;
     a.dk = x->dk;
     a.dv = x->dv;
@@ -1021,25 +1489,25 @@ int delta_args(const gsa_delta_args* x, bool backward, gsa::DeltaArgs& a, DeltaS
 }  // namespace
 }  // namespace gsa_host
 
-extern "C" size_t gsa_delta_rule_workspace_bytes(int B, int T, int N, int packed, int Hv, int dtype, int backward) {
-  const auto z = gsa_host::delta_sizes(B, T, N, packed, Hv, dtype);
-  return z.slots ? 2 * z.tm + z.gates + (backward ? z.s0 + z.u : 0) : 0;
+extern "C" size_t gsa_delta_rule_workspace_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype, int backward) {
+  const auto z = gsa_host::delta_sizes(B, T, N, packed, Hk, Hv, dtype, backward != 0);
+  return z.slots ? z.workspace(backward != 0) : 0;
 }
-extern "C" size_t gsa_delta_rule_saved_bytes(int B, int T, int N, int packed, int Hv, int dtype) {
-  const auto z = gsa_host::delta_sizes(B, T, N, packed, Hv, dtype);
-  return z.slots ? z.s0 + z.u : 0;
+extern "C" size_t gsa_delta_rule_saved_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype) {
+  const auto z = gsa_host::delta_sizes(B, T, N, packed, Hk, Hv, dtype, false);
+  return z.slots ? z.saved() : 0;
 }
 extern "C" int gsa_delta_rule(const gsa_delta_args* x, void* stream) {
   gsa::DeltaArgs a;
   gsa_host::DeltaSizes z;
   if (const int e = gsa_host::delta_args(x, false, a, z)) return e;
   const auto s = static_cast<hipStream_t>(stream);
-  return x->dtype == GSA_DTYPE_BF16 ? gsa_host::launch_forward<uint16_t>(a, s) : gsa_host::launch_forward<float>(a, s);
+  return x->dtype == GSA_DTYPE_BF16 ? gsa_host::launch_forward<uint16_t>(a, z, s) : gsa_host::launch_forward<float>(a, z, s);
 }
 extern "C" int gsa_delta_rule_backward(const gsa_delta_args* x, void* stream) {
   gsa::DeltaArgs a;
   gsa_host::DeltaSizes z;
   if (const int e = gsa_host::delta_args(x, true, a, z)) return e;
   const auto s = static_cast<hipStream_t>(stream);
-  return x->dtype == GSA_DTYPE_BF16 ? gsa_host::launch_backward<uint16_t>(a, s) : gsa_host::launch_backward<float>(a, s);
+  return x->dtype == GSA_DTYPE_BF16 ? gsa_host::launch_backward<uint16_t>(a, z, s) : gsa_host::launch_backward<float>(a, z, s);
 }

@@ -597,8 +597,8 @@ typedef struct gsa_delta_args {
   void* dbeta;
   float* dstate_in;
 } gsa_delta_args;
-size_t gsa_delta_rule_workspace_bytes(int B, int T, int N, int packed, int Hv, int dtype, int backward);
-size_t gsa_delta_rule_saved_bytes(int B, int T, int N, int packed, int Hv, int dtype);
+size_t gsa_delta_rule_workspace_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype, int backward);
+size_t gsa_delta_rule_saved_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype);
 int gsa_delta_rule(const gsa_delta_args* args, void* stream);
 int gsa_delta_rule_backward(const gsa_delta_args* args, void* stream);
 

@@ -142,8 +142,8 @@ def _rule_c(lib, backward=False, **kw):
         setattr(a, n, P)
     for n in ("q", "k", "v", "do"):
         a.__setattr__(n + "_sb", 25600), a.__setattr__(n + "_st", 256), a.__setattr__(n + "_sh", 128)
-    a.ws_bytes = lib.gsa_delta_rule_workspace_bytes(2, 100, 2, 0, 2, 1, int(backward))
-    a.saved_bytes = lib.gsa_delta_rule_saved_bytes(2, 100, 2, 0, 2, 1)
+    a.ws_bytes = lib.gsa_delta_rule_workspace_bytes(2, 100, 2, 0, 1, 2, 1, int(backward))
+    a.saved_bytes = lib.gsa_delta_rule_saved_bytes(2, 100, 2, 0, 1, 2, 1)
     for n, x in kw.items():
         setattr(a, n, x)
     return (lib.gsa_delta_rule_backward if backward else lib.gsa_delta_rule)(ctypes.byref(a), None)
@@ -167,11 +167,11 @@ def test_c_rule_refusals(lib):
 def test_c_rule_sizes(lib):
     for backward in (0, 1):
         f = lib.gsa_delta_rule_workspace_bytes
-        assert f(0, 5, 1, 0, 1, 1, backward) == f(1, 0, 1, 0, 1, 1, backward) == f(1, 5, 1, 0, 0, 1, backward) == 0
-        assert f(1, 5, 1, 0, 1, 7, backward) == 0
-        assert f(1, 64, 1, 0, 2, 1, backward) < f(1, 65, 1, 0, 2, 1, backward)
+        assert f(0, 5, 1, 0, 1, 1, 1, backward) == f(1, 0, 1, 0, 1, 1, 1, backward) == f(1, 5, 1, 0, 0, 0, 1, backward) == 0
+        assert f(1, 5, 1, 0, 1, 1, 7, backward) == f(1, 5, 1, 0, 2, 3, 1, backward) == 0
+        assert f(1, 64, 1, 0, 2, 2, 1, backward) < f(1, 65, 1, 0, 2, 2, 1, backward)
     # what a forward keeps: a state (64 KiB) and a chunk's deltas for each chunk (64 tokens, fp32: 32) and v head
-    assert lib.gsa_delta_rule_saved_bytes(1, 65, 1, 0, 2, 1) == 2 * 2 * (65536 + 64 * 512)
-    assert lib.gsa_delta_rule_saved_bytes(1, 65, 1, 0, 2, 0) == 3 * 2 * (65536 + 32 * 512)
+    assert lib.gsa_delta_rule_saved_bytes(1, 65, 1, 0, 2, 2, 1) == 2 * 2 * (65536 + 64 * 512)
+    assert lib.gsa_delta_rule_saved_bytes(1, 65, 1, 0, 2, 2, 0) == 3 * 2 * (65536 + 32 * 512)
     # packed sequences may each leave a chunk begun: one slot more for every one of them
-    assert lib.gsa_delta_rule_saved_bytes(1, 130, 5, 1, 1, 1) == (2 + 5) * (65536 + 64 * 512)
+    assert lib.gsa_delta_rule_saved_bytes(1, 130, 5, 1, 1, 1, 1) == (2 + 5) * (65536 + 64 * 512)

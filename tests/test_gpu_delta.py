@@ -149,6 +149,23 @@ def test_packed(dev, lens, lead, trail, idx, dtype):
         assert not t[0, outside.to(dev)].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,T,Hk,Hv,lens", [(1, 900, 1, 1, None), (2, 1537, 1, 2, None), (1, 2200, 1, 2, [900, 0, 1, 1000, 299])])
+def test_segments(dev, B, T, Hk, Hv, lens, dtype):
+    """Long sequences with few heads: cut into segments that are joined again (packed ones of several lengths)."""
+    print(f"segments {dtype} B={B} T={T} {lens}", flush=True)
+    x = _inputs(B, T, Hk, Hv, dtype, seed=T)
+    N = B if lens is None else len(lens)
+    gen = torch.Generator().manual_seed(14)
+    state = torch.randn(N, Hv, D, D, generator=gen)
+    grads = (torch.randn(B, T, Hv, D, generator=gen).to(dtype), torch.randn(N, Hv, D, D, generator=gen))
+    cu = None if lens is None else torch.tensor([0] + lens).cumsum(0)
+    spans = [(b, 0, T) for b in range(B)] if lens is None else [(0, int(cu[i]), int(cu[i + 1])) for i in range(N)]
+    got = _run(x, dev, state, cu=None if cu is None else cu.to(dev), grads=grads)
+    _compare(got, _oracle(x, spans, state, grads), T, Hv // Hk)
+    _check(_run(x, dev, cu=None if cu is None else cu.to(dev))[0], _oracle(x, spans)[0], T, 16, "o")
+
+
 def test_offsets_outside_the_tokens_touch_nothing(dev):
     """Offsets past T or descending: held within the tokens, other sequences are right."""
     x = _inputs(1, 100, 1, 1, torch.bfloat16, seed=3)
