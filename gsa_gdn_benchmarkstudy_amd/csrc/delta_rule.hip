@@ -1012,16 +1012,21 @@ __global__ __launch_bounds__(512) void delta_join_kernel(DeltaArgs a, int chunk)
 //   dbeta_i = dR_i . v_i - e^G_i k_i . (dR S0^T)_i - sum_j F_ij (k_i . k_j) D_ij
 //   dG: row sums less column sums of M = E P + B (K K^T), and the three products with S0 and
 //       dS1, row by row, times q or k; dg is the sum of dG from the token to the chunk's end.
-// 256 threads, a q/k head and the v heads that share it one after the other (so dq and dk need no
-// atomics).  Products with rows of the 128 elements are computed transposed: a wave owns 32
-// of them (two tiles), a lane 8 of one token.
+// 256 threads a chunk and v head.  First everything summed over the 128 elements of v, 32 at a
+// time through LDS; then the products summed over tokens.  Those with rows of the 128 elements of
+// k are computed transposed: a wave owns 32 of them (two tiles), a lane 8 of one token.  Where v
+// heads share a q/k head, each leaves its part of dq and dk in fp32 where its dS1 was, and
+// delta_shared_kernel adds them in the heads' order (no atomics).
 // ---------------------------------------------------------------------------
 template <typename T> struct GradLds {
-  static constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts, JS = C / 32;
-  static constexpr int kLdR = kHead + 4, kLdC = C + 4;
-  static constexpr int kCols = 8 * JS * NP * 64;             // 16-byte units
-  static constexpr int kFloats = 2 * C * kLdR + 3 * C * kLdC + 4 * 3 * C + 5 * C + 2 * C + 8;
-  static constexpr size_t kBytes = 16 * (size_t)(2 * kCols) + 4 * (size_t)kFloats + 8 * C;
+  static constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts, MT = C / 16, JS = C / 32, kLd = C + 4;
+  // what enters dq and dk alone: for bf16 two parts do (2^-17 of it)
+  static constexpr int kIn = NP == 1 ? 2 : 3;
+  static constexpr int kStage = MT * (NP + 3 + 3) * kUnit;   // dO, U, dR: 32 elements of every token
+  static constexpr int kKind = MT * JS * kIn * kUnit;        // a [C][C] operand
+  static constexpr int kLate = 3 * kKind + C * kLd * 4;
+  static constexpr int kBig = 2 * kStage > kLate ? 2 * kStage : kLate;
+  static constexpr size_t kBytes = kBig + 4 * (12 * C + 5 * C + C + MT * C + 4) + 8 * C;
 };
 
 __device__ __forceinline__ double wave_sum(double x) {
@@ -1031,166 +1036,157 @@ __device__ __forceinline__ double wave_sum(double x) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void delta_grads_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   using L = GradLds<T>;
-  constexpr int C = L::C, NP = L::NP, MT = C / 16, JS = L::JS, LR = L::kLdR, LC = L::kLdC;
+  using K = Pack<T, true>;
+  constexpr int C = L::C, NP = L::NP, MT = L::MT, JS = L::JS, kIn = L::kIn, LD = L::kLd;
+  constexpr int kTiles = MT * (MT + 1) / 2, kMine = (kTiles + 3) / 4;
   extern __shared__ __align__(16) char lds[];
-  bf16x8* skt = reinterpret_cast<bf16x8*>(lds);
-  bf16x8* sqt = skt + L::kCols;
-  double* dsum = reinterpret_cast<double*>(sqt + L::kCols);  // [C]
-  float* su = reinterpret_cast<float*>(dsum + C);            // U [C][LR]
-  float* sr = su + C * LR;                                   // dR
-  float* se = sr + C * LR;                                   // scale E D [C][LC]
-  float* sb = se + C * LC;                                   // B + B^T
-  float* sm = sb + C * LC;                                   // M
-  float* red = sm + C * LC;                                  // [4 waves][3][C]
+  bf16x8* stage = reinterpret_cast<bf16x8*>(lds);            // [2][dO | U | dR]
+  char* xe = lds;                                            // scale E D, then its transpose, then B + B^T
+  char* xt = xe + L::kKind;
+  char* xb = xt + L::kKind;
+  float* sm = reinterpret_cast<float*>(xb + L::kKind);       // M [C][LD]
+  float* red = reinterpret_cast<float*>(lds + L::kBig);      // [4 waves][3][C]
   float* gates = red + 12 * C;                               // [5][C]
-  float* db = gates + 5 * C;                                 // [C]: dR . v, then + sum of F (K K^T) D
-  float* fs = db + C;                                        // [C]
-  float* cross = fs + C;                                     // [4]
-  const int slot = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, l = lane_id(), g = l >> 4, m = l & 15;
+  float* db = gates + 5 * C;                                 // [C]: dR . v
+  float* fs = db + C;                                        // [MT][C]: sums of F (K K^T) D by tiles
+  float* cross = fs + MT * C;                                     // [4]
+  double* dsum = reinterpret_cast<double*>(cross + 4);       // [C]
+  const int slot = blockIdx.x, h = blockIdx.y, share = a.Hv / a.Hk, hk = h / share, tid = threadIdx.x, l = lane_id(), g = l >> 4;
+  const int m = l & 15, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int c;
   const Span sp = slot_of(a.s, slot, C, c);
   if (c < 0) return;
   const int64_t t0 = (int64_t)c * C;
-  const int left = sp.len - (int)t0, share = a.Hv / a.Hk;
+  const int left = sp.len - (int)t0;
   const int64_t tok = (int64_t)sp.b * a.s.T + sp.t0 + t0;    // row of [B * T]
+  const int64_t at = (int64_t)slot * a.Hv + h, atk = (int64_t)slot * a.Hk + hk;
 
-  stage_cols<T>(skt, a.k, sp, t0, left, hk, tid, 256);
-  stage_cols<T>(sqt, a.q, sp, t0, left, hk, tid, 256);
-
-  floatx4 dq[2][MT], dk[2][MT];                              // [128 elements: tile 2 wave + e][tokens]
+  {
+    // a thread's 8 elements of each 32: token tid / 4
+    const int st = tid >> 2, so = tid & 3;
+    const bool mine = st < C, there = mine && st < left;
+    const float* up = a.u + (at * C + st) * kHead + 8 * so;
+    const float* rp = a.dr + (at * C + st) * kHead + 8 * so;
+    const T* op = row_at<T>(a.dout, sp, t0 + st, h) + 8 * so;
+    const T* vp = row_at<T>(a.v, sp, t0 + st, h) + 8 * so;
+    float xu[8], xr[8], dot_v = 0.f;
+    u32x4 xo[sizeof(T) / 2], xv[sizeof(T) / 2];              // 8 elements as they are
+    auto load = [&](int ks) {
+      if (mine) {
+        load8(up + 32 * ks, xu);
+        load8(rp + 32 * ks, xr);
+      }
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        xo[i] = xv[i] = u32x4{0, 0, 0, 0};
+        if (there) {
+          xo[i] = reinterpret_cast<const u32x4*>(op + 32 * ks)[i];
+          xv[i] = reinterpret_cast<const u32x4*>(vp + 32 * ks)[i];
+        }
+      }
+    };
+    auto floats = [](const u32x4* x, float (&y)[8]) {
 #pragma unroll
-    for (int n = 0; n < MT; ++n) dq[e][n] = dk[e][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-
-  for (int hs = 0; hs < share; ++hs) {
-    const int h = hk * share + hs;
-    const int64_t at = (int64_t)slot * a.Hv + h;
-    __syncthreads();
-    for (int i = tid; i < C * kHead / 4; i += 256) {
-      const int t = i >> 5, e = 4 * (i & 31);
-      *reinterpret_cast<floatx4*>(su + t * LR + e) = *reinterpret_cast<const floatx4*>(a.u + (at * C + t) * kHead + e);
-      *reinterpret_cast<floatx4*>(sr + t * LR + e) = *reinterpret_cast<const floatx4*>(a.dr + (at * C + t) * kHead + e);
-    }
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = sizeof(T) == 2 ? x[0][i >> 1] : x[i >> 2][i & 3];
+        y[i] = sizeof(T) == 4 ? __uint_as_float(w) : i & 1 ? bf16hi(w) : bf16lo(w);
+      }
+    };
+    auto put = [&](int buf) {
+      if (!mine) return;
+      bf16x8* to = stage + buf * (L::kStage / 16) + 16 * so + (st & 15);
+      const int tile = st >> 4;
+      float fo[8], fv[8];
+      floats(xo, fo);
+      floats(xv, fv);
+      const Parts<NP> o = parts_of<NP>(fo);
+      const Parts<3> u = split3(xu), r = split3(xr);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) to[(tile * NP + i) * 64] = o.p[i];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) to[(MT * NP + tile * 3 + i) * 64] = u.p[i];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) to[(MT * (NP + 3) + tile * 3 + i) * 64] = r.p[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot_v = __builtin_fmaf(xr[i], fv[i], dot_v);
+    };
+    load(0);
     for (int i = tid; i < 5 * C; i += 256) gates[i] = i < 3 * C ? a.gates[at * 256 + i] : a.sums[at * 2 * C + i - 3 * C];
-    __syncthreads();
 
-    // E, F, Q K^T, K K^T by tiles of tokens
-    for (int mt = wave; mt < MT; mt += 4) {
-      const int i0 = 16 * mt + m;
-      Parts<NP> xo[4], xk[4], xq[4];
-      Parts<3> xr[4];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const int e = 32 * ks + 8 * g;
-        xo[ks] = operand<T>(row_at<T>(a.dout, sp, t0 + i0, h) + e, i0 < left);
-        xk[ks] = operand<T>(row_at<T>(a.k, sp, t0 + i0, hk) + e, i0 < left);
-        xq[ks] = operand<T>(row_at<T>(a.q, sp, t0 + i0, hk) + e, i0 < left);
-        float y[8];
-        load8(sr + i0 * LR + e, y);
-        xr[ks] = split3(y);
-      }
-      float f[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int nt = 0; nt < MT; ++nt) {
-        floatx4 E = {0.f, 0.f, 0.f, 0.f}, F = E, QK = E, KK = E;
-        const int j = 16 * nt + m;
-        if (nt <= mt) {
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const int e = 32 * ks + 8 * g;
-            float y[8];
-            load8(su + j * LR + e, y);
-            const Parts<3> u = split3(y);
-            const Parts<NP> kj = operand<T>(row_at<T>(a.k, sp, t0 + j, hk) + e, j < left);
-            mma(E, xo[ks], u);
-            mma(F, xr[ks], u);
-            mma(QK, xq[ks], kj);
-            mma(KK, xk[ks], kj);
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 16 * mt + 4 * g + r;
-          if (nt > mt) {
-            se[i * LC + j] = sm[i * LC + j] = 0.f;
-          } else {
-            const float d = j <= i ? expf((gates[3 * C + i] - gates[3 * C + j]) + (gates[4 * C + i] - gates[4 * C + j])) : 0.f;
-            const float ed = a.scale * E[r] * d, fd = j < i ? F[r] * d : 0.f, b = -gates[2 * C + i] * fd;
-            se[i * LC + j] = ed;
-            sm[i * LC + j] = j < i ? ed * QK[r] + b * KK[r] : 0.f;
-            f[r] += fd * KK[r];
-            if (j < i) {
-              sb[i * LC + j] = b;
-              sb[j * LC + i] = b;
-            } else if (j == i) {
-              sb[i * LC + i] = 0.f;
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        f[r] = row16_sum(f[r]);
-        if (m == 0) fs[16 * mt + 4 * g + r] = f[r];
-      }
-    }
-    // dR . v: 256 / C lanes a token
-    {
-      constexpr int kPer = 256 / C;
-      const int t = tid / kPer;
-      float x = 0.f;
-      if (t < left)
-        for (int e = tid % kPer; e < kHead; e += kPer)
-          x = __builtin_fmaf(sr[t * LR + e], to_f32(row_at<T>(a.v, sp, t0 + t, h)[e]), x);
-#pragma unroll
-      for (int o = 1; o < kPer; o <<= 1) x += __shfl_xor(x, o, 64);
-      if (tid % kPer == 0) db[t] = x;
-    }
-
-    // dO S0^T, dR S0^T, U dS1^T, transposed
-    floatx4 Z1[2][MT], Z2[2][MT], Z3[2][MT];
+    // dO S0^T, U dS1^T, dR S0^T (transposed), E and F by tiles of tokens
+    floatx4 Z1[2][MT], Z2[2][MT], Z3[2][MT], E[kMine], F[kMine];
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int n = 0; n < MT; ++n) Z1[e][n] = Z2[e][n] = Z3[e][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-    double dot = 0.;
 #pragma unroll
+    for (int i = 0; i < kMine; ++i) E[i] = F[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    double dot = 0.;
+    const float* s0p = uniform(a.s0 + at * kHead * kHead);
+    const float* s1p = uniform(a.ds1 + at * kHead * kHead);
+#pragma unroll 1
     for (int ks = 0; ks < 4; ++ks) {
-      Parts<3> s0[2], s1[2];
+      put(ks & 1);
+      float y[2][8], z[2][8];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int64_t o = at * kHead * kHead + tile_row(2 * wave + e, m) * kHead + 32 * ks + 8 * g;
-        float y[8], z[8];
-        load8(a.s0 + o, y);
-        load8(a.ds1 + o, z);
+        const uint32_t o = tile_row(2 * wave + e, m) * kHead + 32 * ks + 8 * g;
+        load8(s0p + o, y[e]);
+        load8(s1p + o, z[e]);
+      }
+      __syncthreads();
+      if (ks < 3) load(ks + 1);
+      const bf16x8* so_ = stage + (ks & 1) * (L::kStage / 16);
+      const bf16x8* su_ = so_ + MT * NP * 64;
+      const bf16x8* sr_ = su_ + MT * 3 * 64;
+      Parts<3> sx[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
         float x = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x = __builtin_fmaf(y[i], z[i], x);
+        for (int i = 0; i < 8; ++i) x = __builtin_fmaf(y[e][i], z[e][i], x);
         dot += x;
-        s0[e] = split3(y);
-        s1[e] = split3(z);
+        sx[e] = split3(y[e]);
       }
 #pragma unroll
       for (int n = 0; n < MT; ++n) {
-        const int t = 16 * n + m, e0 = 32 * ks + 8 * g;
-        const Parts<NP> o = operand<T>(row_at<T>(a.dout, sp, t0 + t, h) + e0, t < left);
-        float y[8];
-        load8(sr + t * LR + e0, y);
-        const Parts<3> r = split3(y);
-        load8(su + t * LR + e0, y);
-        const Parts<3> u = split3(y);
+        const Parts<NP> o = staged<NP>(so_, n, l);
+        const Parts<3> r = staged<3>(sr_, n, l);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          mma(Z1[e][n], s0[e], o);
-          mma(Z2[e][n], s1[e], u);
-          mma(Z3[e][n], s0[e], r);
+          mma(Z1[e][n], sx[e], o);
+          mma(Z3[e][n], sx[e], r);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);                     // (fewer operands in registers at a time)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) sx[e] = split3(z[e]);
+#pragma unroll
+      for (int n = 0; n < MT; ++n) {
+        const Parts<3> u = staged<3>(su_, n, l);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) mma(Z2[e][n], sx[e], u);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int t = wave + 4 * i;
+        if (t < kTiles) {
+          const int mt = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, nt = t - mt * (mt + 1) / 2;
+          const Parts<3> u = staged<3>(su_, nt, l);
+          mma(E[i], staged<NP>(so_, mt, l), u);
+          mma(F[i], staged<3>(sr_, mt, l), u);
         }
       }
     }
+    dot_v += __shfl_xor(dot_v, 1, 64);
+    dot_v += __shfl_xor(dot_v, 2, 64);
+    if (mine && so == 0) db[st] = dot_v;
     dot = wave_sum(dot);
     if (l == 0) cross[wave] = (float)dot;
+    floatx4 dq[2][MT], dk[2][MT];                            // [128 elements: tile 2 wave + e][tokens]
 #pragma unroll
     for (int n = 0; n < MT; ++n) {
       const int t = 16 * n + m;
@@ -1206,8 +1202,8 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaArgs a) {
         x1 = __builtin_fmaf(q[i], z1, x1);
         x2 = __builtin_fmaf(k[i], z2, x2);
         x3 = __builtin_fmaf(k[i], z3, x3);
-        dq[i >> 2][n][i & 3] += z1;
-        dk[i >> 2][n][i & 3] += z2 - beta * z3;
+        dq[i >> 2][n][i & 3] = z1;
+        dk[i >> 2][n][i & 3] = z2 - beta * z3;
       }
       x1 += __shfl_xor(x1, 16, 64); x1 += __shfl_xor(x1, 32, 64);
       x2 += __shfl_xor(x2, 16, 64); x2 += __shfl_xor(x2, 32, 64);
@@ -1218,59 +1214,135 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaArgs a) {
         red[(wave * 3 + 2) * C + t] = x3;
       }
     }
+    for (int i = tid; i < MT * C; i += 256) fs[i] = 0.f;
+    __syncthreads();                                         // the staged operands are read
+    for (int i = tid; i < L::kLate / 16; i += 256) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+    __syncthreads();
+
+    // Q K^T and K K^T of the wave's tiles; E and F become the operands of the products over tokens
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int t = wave + 4 * i;
+      if (t < kTiles) {
+        const int mt = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, nt = t - mt * (mt + 1) / 2;
+        const int ia = 16 * mt + m, j = 16 * nt + m;
+        const T* pq = row_at<T>(a.q, sp, t0 + ia, hk) + 8 * g;
+        const T* pk = row_at<T>(a.k, sp, t0 + ia, hk) + 8 * g;
+        const T* pj = row_at<T>(a.k, sp, t0 + j, hk) + 8 * g;
+        floatx4 QK = {0.f, 0.f, 0.f, 0.f}, KK = QK;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const Parts<NP> kj = operand<T>(pj + 32 * ks, j < left);
+          mma(QK, operand<T>(pq + 32 * ks, ia < left), kj);
+          mma(KK, operand<T>(pk + 32 * ks, ia < left), kj);
+        }
+        float ed[4], bb[4], f[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int ii = 16 * mt + 4 * g + r;
+          const float d = j <= ii ? expf((gates[3 * C + ii] - gates[3 * C + j]) + (gates[4 * C + ii] - gates[4 * C + j])) : 0.f;
+          const float fd = j < ii ? F[i][r] * d : 0.f;
+          ed[r] = a.scale * E[i][r] * d;
+          bb[r] = -gates[2 * C + ii] * fd;
+          f[r] = row16_sum(fd * KK[r]);
+          sm[ii * LD + j] = j < ii ? ed[r] * QK[r] + bb[r] * KK[r] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (m == 0) fs[nt * C + 16 * mt + 4 * g + r] = f[r];
+        // (row, summed over) = (i, j): elements apart; (j, i): 4 neighbours
+        const int ij = ((mt * JS + (j >> 5)) * kIn * 64 + 16 * ((j >> 3) & 3) + 4 * g) * 16 + 2 * (j & 7);
+        const int i0 = 16 * mt + 4 * g;
+        const int ji = ((nt * JS + (i0 >> 5)) * kIn * 64 + 16 * ((i0 >> 3) & 3) + m) * 16 + 2 * (i0 & 7);
+        __bf16 pe[kIn][4], pb[kIn][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = ed[r], y = bb[r];
+#pragma unroll
+          for (int n = 0; n < kIn; ++n) {
+            pe[n][r] = (__bf16)x;
+            pb[n][r] = (__bf16)y;
+            x -= (float)pe[n][r];
+            y -= (float)pb[n][r];
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kIn; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            *reinterpret_cast<uint16_t*>(xe + ij + n * kUnit + 16 * r) = __builtin_bit_cast(uint16_t, pe[n][r]);
+            if (j < i0 + r) *reinterpret_cast<uint16_t*>(xb + ij + n * kUnit + 16 * r) = __builtin_bit_cast(uint16_t, pb[n][r]);
+          }
+          uint32_t w[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[r] = __builtin_bit_cast(uint16_t, pe[n][r]);
+          *reinterpret_cast<uint2*>(xt + ji + n * kUnit) = uint2{w[0] | w[1] << 16, w[2] | w[3] << 16};
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (j < i0 + r) *reinterpret_cast<uint16_t*>(xb + ji + n * kUnit + 2 * r) = __builtin_bit_cast(uint16_t, pb[n][r]);
+        }
+      }
+    }
     __syncthreads();
 
     // the products with K and Q
+    const bf16x8* ktp = reinterpret_cast<const bf16x8*>(a.kt + atk * K::kCols * kUnit);
+    const bf16x8* qtp = reinterpret_cast<const bf16x8*>(a.qt + atk * K::kCols * kUnit);
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
       Parts<NP> kt[2], qt[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        kt[e] = staged<NP>(skt, (2 * wave + e) * JS + js, l);
-        qt[e] = staged<NP>(sqt, (2 * wave + e) * JS + js, l);
+        kt[e] = staged<NP>(ktp, (2 * wave + e) * JS + js, l);
+        qt[e] = staged<NP>(qtp, (2 * wave + e) * JS + js, l);
       }
 #pragma unroll
       for (int n = 0; n < MT; ++n) {
-        const int t = 16 * n + m, j0 = 32 * js + 8 * g;
-        float x[8], y[8], z[8];
-        load8(se + t * LC + j0, x);
-        load8(sb + t * LC + j0, y);
+        const Parts<kIn> b = staged<kIn>(reinterpret_cast<const bf16x8*>(xb), n * JS + js, l);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = se[(j0 + i) * LC + t];
-        const Parts<3> xe = split3(x), xb = split3(y), xt = split3(z);
+        for (int e = 0; e < 2; ++e) mma(dk[e][n], kt[e], b);
+        if (js <= n / 2) {
+          const Parts<kIn> x = staged<kIn>(reinterpret_cast<const bf16x8*>(xe), n * JS + js, l);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          mma(dq[e][n], kt[e], xe);
-          mma(dk[e][n], kt[e], xb);
-          mma(dk[e][n], qt[e], xt);
+          for (int e = 0; e < 2; ++e) mma(dq[e][n], kt[e], x);
+        }
+        if (js >= n / 2) {
+          const Parts<kIn> x = staged<kIn>(reinterpret_cast<const bf16x8*>(xt), n * JS + js, l);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) mma(dk[e][n], qt[e], x);
         }
       }
     }
     // dG in 64 bits: what cancels between the rows and columns of M has to cancel exactly
-    if (tid < C) {
+    if (mine) {
       double s = 0.;
-      for (int j = 0; j < C; ++j) s += (double)sm[tid * LC + j] - (double)sm[j * LC + tid];
-      double x1 = 0., x2 = 0., x3 = 0.;
-      for (int w = 0; w < 4; ++w) {
-        x1 += red[(w * 3 + 0) * C + tid];
-        x2 += red[(w * 3 + 1) * C + tid];
-        x3 += red[(w * 3 + 2) * C + tid];
+      for (int j = so; j < C; j += 4) s += (double)sm[st * LD + j] - (double)sm[j * LD + st];
+      s += __shfl_xor(s, 1, 64);
+      s += __shfl_xor(s, 2, 64);
+      if (so == 0) {
+        double x1 = 0., x2 = 0., x3 = 0.;
+        for (int w = 0; w < 4; ++w) {
+          x1 += red[(w * 3 + 0) * C + st];
+          x2 += red[(w * 3 + 1) * C + st];
+          x3 += red[(w * 3 + 2) * C + st];
+        }
+        const float beta = gates[2 * C + st];
+        if (st < left) {
+          float x = db[st] - (float)x3;
+          for (int n = 0; n < MT; ++n) x -= fs[n * C + st];
+          const int64_t o = (tok + st) * a.Hv + h;
+          if (a.beta_bf16) static_cast<uint16_t*>(a.dbeta)[o] = (uint16_t)f32_to_bf16_bits(x);
+          else static_cast<float*>(a.dbeta)[o] = x;
+        }
+        // at the end of the chunk: e^G_C <dS1, S0> and every x2
+        dsum[st] = s + x1 - x2 - beta * x3;
+        red[st] = (float)x2;
       }
-      const float beta = gates[2 * C + tid];
-      if (tid < left) {
-        const float x = db[tid] - (float)x3 - fs[tid];
-        const int64_t o = (tok + tid) * a.Hv + h;
-        if (a.beta_bf16) static_cast<uint16_t*>(a.dbeta)[o] = (uint16_t)f32_to_bf16_bits(x);
-        else static_cast<float*>(a.dbeta)[o] = x;
-      }
-      // at the end of the chunk: e^G_C <dS1, S0> and every x2
-      dsum[tid] = s + x1 - x2 - beta * x3;
-      red[tid] = (float)x2;
     }
     __syncthreads();
     if (wave == 0 && l < C) {
-      double x2 = red[l], s = dsum[l];
-      double all = x2;
+      const double x2 = red[l];
+      double s = dsum[l], all = x2;
 #pragma unroll
       for (int o = 1; o < C; o <<= 1) all += __shfl_xor(all, o, 64);
       if (l == C - 1) s += all + (double)gates[C - 1] * ((double)cross[0] + cross[1] + cross[2] + cross[3]);
@@ -1281,19 +1353,48 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaArgs a) {
       }
       if (l < left) a.dg[(tok + l) * a.Hv + h] = (float)s;
     }
-  }
-
 #pragma unroll
-  for (int n = 0; n < MT; ++n) {
-    const int t = 16 * n + m;
-    if (t < left) {
-      const int64_t o = ((tok + t) * a.Hk + hk) * kHead + 32 * wave + 8 * g;
+    for (int n = 0; n < MT; ++n) {
+      const int t = 16 * n + m;
       float x[8], y[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) { x[i] = dq[i >> 2][n][i & 3]; y[i] = dk[i >> 2][n][i & 3]; }
-      store8(static_cast<T*>(a.dq) + o, x);
-      store8(static_cast<T*>(a.dk) + o, y);
+      if (share > 1) {                                       // (every wave is through with dS1)
+        float* part = a.ds1 + at * kHead * kHead + t * kHead + 32 * wave + 8 * g;
+        store8(part, x);
+        store8(part + C * kHead, y);
+      } else if (t < left) {
+        const int64_t o = ((tok + t) * a.Hk + hk) * kHead + 32 * wave + 8 * g;
+        store8(static_cast<T*>(a.dq) + o, x);
+        store8(static_cast<T*>(a.dk) + o, y);
+      }
     }
+  }
+}
+
+// dq and dk of a q/k head from the parts of the v heads that share it.
+template <typename T>
+__global__ __launch_bounds__(256) void delta_shared_kernel(DeltaArgs a) {
+  constexpr int C = DeltaType<T>::kChunk;
+  const int slot = blockIdx.x, hk = blockIdx.y, share = a.Hv / a.Hk;
+  int c;
+  const Span sp = slot_of(a.s, slot, C, c);
+  if (c < 0) return;
+  const int left = sp.len - c * C;
+  const int64_t tok = (int64_t)sp.b * a.s.T + sp.t0 + (int64_t)c * C;
+  for (int u = threadIdx.x; u < 2 * C * 16; u += 256) {
+    const int t = (u >> 4) % C, e = 8 * (u & 15);
+    if (t >= left) continue;
+    const float* part = a.ds1 + ((int64_t)slot * a.Hv + hk * share) * kHead * kHead + (u >> 4) * kHead + e;
+    float x[8];
+    load8(part, x);
+    for (int i = 1; i < share; ++i) {
+      float y[8];
+      load8(part + (int64_t)i * kHead * kHead, y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] += y[k];
+    }
+    store8(static_cast<T*>((u >> 4) < C ? a.dq : a.dk) + ((tok + t) * a.Hk + hk) * kHead + e, x);
   }
 }
 
@@ -1388,7 +1489,7 @@ template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSiz
 }
 template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
   constexpr size_t lds = gsa::ScanLds<T>::kBwd, lds_grads = gsa::GradLds<T>::kBytes;
-  static_assert(2 * lds <= 160 * 1024 && lds_grads <= 160 * 1024);
+  static_assert(2 * lds <= 160 * 1024 && 2 * lds_grads <= 160 * 1024, "two blocks a CU");
   hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, true>), dim3(z.slots, a.Hv), dim3(256), 0, s, a);
   if (const int e = launch_status()) return e;
   if (a.seg) {
@@ -1402,7 +1503,11 @@ template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSi
   hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, true>), dim3(a.seg ? z.segs : a.s.N, a.Hv), dim3(256), lds, s, a);
   if (const int e = launch_status()) return e;
   if (const int e = allow_lds<gsa::delta_grads_kernel<T>>(lds_grads)) return e;
-  hipLaunchKernelGGL(gsa::delta_grads_kernel<T>, dim3(z.slots, a.Hk), dim3(256), lds_grads, s, a);
+  hipLaunchKernelGGL(gsa::delta_grads_kernel<T>, dim3(z.slots, a.Hv), dim3(256), lds_grads, s, a);
+  if (a.Hv > a.Hk) {
+    if (const int e = launch_status()) return e;
+    hipLaunchKernelGGL(gsa::delta_shared_kernel<T>, dim3(z.slots, a.Hk), dim3(256), 0, s, a);
+  }
   return launch_status();
 }
 
