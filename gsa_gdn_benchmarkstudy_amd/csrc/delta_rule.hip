@@ -80,6 +80,23 @@ __device__ __forceinline__ void mma(floatx4& acc, const Parts<NA>& a, const Part
         if (i + j == o) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
 }
 
+// acc[i][n] += a[i] b[n] for two columns of tiles: part by part over all of them, so that an
+// instruction does not wait for the one before it.
+template <int M, int NA, int NB>
+__device__ __forceinline__ void mma_grid(floatx4 (*acc)[2], const Parts<NA> (&a)[M], const Parts<NB> (&b)[2]) {
+#pragma unroll
+  for (int o = 2; o >= 0; --o)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        if (i + j == o)
+#pragma unroll
+          for (int t = 0; t < M; ++t)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t].p[i], b[n].p[j], acc[t][n], 0, 0, 0);
+}
+
 template <typename T> struct DeltaType;
 template <> struct DeltaType<uint16_t> { static constexpr int kParts = 1, kChunk = 64; };
 template <> struct DeltaType<float> { static constexpr int kParts = 3, kChunk = 32; };
@@ -146,8 +163,7 @@ struct DeltaArgs {
   char* pm;                   // [slots][Hv]: P (transposed)
   float* gates;               // [slots][Hv] units: e^G, e^(G_C - G), beta [C] each
   float* sums;                // [slots][Hv][2][C]: G (upper and lower part); the backward pass only
-  char *kt, *qt;              // [slots][Hk]: K^T, Q^T (the backward pass)
-  char *kr, *qr;              // [slots][Hk]: fp32 inputs: K, Q
+  char *kr, *qr;              // [slots][Hk]: K, Q (fp32 inputs; bf16 rows are read from where they are)
   // The scan cut into segments of seg chunks (0: sequences in one piece), [segments][Hv][128][128] each
   int seg, segs;
   float* move;                // a segment's product of transitions
@@ -223,7 +239,7 @@ template <typename T, bool kBwd> struct Pack {
   static constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts;
   static constexpr int kPParts = kBwd || NP == 3 ? 3 : 2;
   static constexpr int kT = Square<C>::kFrags * 3, kP = Square<C>::kFrags * kPParts;
-  static constexpr int kCols = 8 * (C / 32) * NP, kRows = (C / 16) * 4 * NP;
+  static constexpr int kRows = (C / 16) * 4 * NP;
 };
 
 // [C][ld] fp32 matrix in LDS -> its operands of kN parts in global memory.
@@ -245,41 +261,10 @@ __device__ __forceinline__ void pack_square(char* dst, const float* x, int ld, i
     for (int n = 0; n < kN; ++n) *reinterpret_cast<bf16x8*>(dst + (f * kN + n) * kUnit + 16 * l) = p.p[n];
   }
 }
-// Rows of the 128 elements (tile_row), summed over tokens, to global memory or LDS.
-template <typename T>
-__device__ __forceinline__ void stage_cols(bf16x8* dst, const Rows& x, const Span& sp, int64_t t0, int left, int h, int tid,
-                                           int threads) {
-  constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts, JS = C / 32;
-  for (int u = tid; u < C * 4; u += threads) {
-    const int d4 = u & 31, oct = u >> 5;
-    float v[4][8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int t = 8 * oct + e;
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
-      if (t < left) {
-        const T* p = row_at<T>(x, sp, t0 + t, h) + 4 * d4;
-        if constexpr (sizeof(T) == 2) {
-          const uint2 r = *reinterpret_cast<const uint2*>(p);
-          y[0] = bf16lo(r.x); y[1] = bf16hi(r.x); y[2] = bf16lo(r.y); y[3] = bf16hi(r.y);
-        } else {
-          const floatx4 r = *reinterpret_cast<const floatx4*>(p);
-          y[0] = r[0]; y[1] = r[1]; y[2] = r[2]; y[3] = r[3];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i][e] = y[i];
-    }
-    const int tile = 2 * (d4 >> 3) + (d4 & 1), m = 4 * ((d4 >> 1) & 3);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const Parts<NP> p = parts_of<NP>(v[i]);
-#pragma unroll
-      for (int n = 0; n < NP; ++n) dst[((tile * JS + (oct >> 2)) * NP + n) * 64 + 16 * (oct & 3) + m + i] = p.p[n];
-    }
-  }
-}
-// Rows of tokens (tile_row), summed over the 128 elements.
+// A chunk's rows of 128 elements: unit (tile, step of 32 elements, part), lane's place row_slot(g, m)
+// for row m's elements 8 g .. + 7.  The places turn with g, so that neither the lanes of an
+// operand with rows of tokens (rows_of) nor those of its transpose (cols_of) meet in a bank.
+__device__ __forceinline__ int row_slot(int g, int m) { return 16 * g + ((m + 4 * g) & 15); }
 template <typename T>
 __device__ __forceinline__ void stage_rows(bf16x8* dst, const Rows& x, const Span& sp, int64_t t0, int left, int h, int tid) {
   constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts;
@@ -288,13 +273,38 @@ __device__ __forceinline__ void stage_rows(bf16x8* dst, const Rows& x, const Spa
     const int tile = 2 * (t >> 5) + ((t >> 2) & 1), m = 4 * ((t >> 3) & 3) + (t & 3);
     const Parts<NP> p = operand<T>(row_at<T>(x, sp, t0 + t, h) + 8 * d8, t < left);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) dst[((tile * 4 + (d8 >> 2)) * NP + i) * 64 + 16 * (d8 & 3) + m] = p.p[i];
+    for (int i = 0; i < NP; ++i) dst[((tile * 4 + (d8 >> 2)) * NP + i) * 64 + row_slot(d8 & 3, m)] = p.p[i];
   }
 }
 template <int N> __device__ __forceinline__ Parts<N> staged(const bf16x8* src, int frag, int l) {
   Parts<N> r;
 #pragma unroll
   for (int i = 0; i < N; ++i) r.p[i] = src[(frag * N + i) * 64 + l];
+  return r;
+}
+// Rows of tokens (tile), elements 32 ks .. + 31; slot: the lane's row_slot.
+template <int N> __device__ __forceinline__ Parts<N> rows_of(const char* src, int tile, int ks, int slot) {
+  return staged<N>(reinterpret_cast<const bf16x8*>(src), tile * 4 + ks, slot);
+}
+// The transpose: rows of elements tile_row(t, .), tokens 32 js .. + 31 (ds_read_b64_tr_b16: of 16
+// lanes, lane i names row i / 4, elements 4 (i % 4) .. + 3 of 16, and gets element i of the four
+// rows).  place: the lane's cols_place.
+__device__ __forceinline__ int cols_place(int l) {
+  const int i = l & 15;
+  return 16 * row_slot(i & 3, 4 * (l >> 4) + (i >> 2));
+}
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+template <int N> __device__ __forceinline__ Parts<N> cols_of(const char* src, int t, int js, int place) {
+  Parts<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s16x4 x[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
+          src + (((2 * js + e) * 4 + (t >> 1)) * N + i) * 1024 + place + 8 * (t & 1)));
+    r.p[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
   return r;
 }
 
@@ -308,8 +318,8 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
   __shared__ float gh[C], gl[C], bt[C];
   float (*xm)[LD] = reinterpret_cast<float (*)[LD]>(xbuf);
   bf16x8* sk = reinterpret_cast<bf16x8*>(xbuf);
-  const int slot = blockIdx.x, h = blockIdx.y, share = a.Hv / a.Hk, hk = h / share, tid = threadIdx.x, wave = tid >> 6, l = lane_id();
-  const int g4 = l >> 4, m = l & 15;
+  const int slot = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, share = a.Hv / a.Hk, hk = h / share, tid = threadIdx.x, wave = tid >> 6, l = lane_id();
+  const int g4 = l >> 4, m = l & 15, rs = row_slot(g4, m);
   int c;
   const Span sp = slot_of(a.s, slot, C, c);
   if (c < 0) return;
@@ -349,12 +359,10 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
       }
     }
   }
-  if (h % share == 0) {                                      // one of the heads that share q and k
-    stage_cols<T>(reinterpret_cast<bf16x8*>(a.kt + atk * K::kCols * kUnit), a.k, sp, t0, left, hk, tid, 256);
-    if (kBwd) stage_cols<T>(reinterpret_cast<bf16x8*>(a.qt + atk * K::kCols * kUnit), a.q, sp, t0, left, hk, tid, 256);
-    if constexpr (NP == 3) {
+  if constexpr (NP == 3) {
+    if (h % share == 0) {                                    // one of the heads that share q and k
       stage_rows<T>(reinterpret_cast<bf16x8*>(a.kr + atk * K::kRows * kUnit), a.k, sp, t0, left, hk, tid);
-      if (!kBwd) stage_rows<T>(reinterpret_cast<bf16x8*>(a.qr + atk * K::kRows * kUnit), a.q, sp, t0, left, hk, tid);
+      stage_rows<T>(reinterpret_cast<bf16x8*>(a.qr + atk * K::kRows * kUnit), a.q, sp, t0, left, hk, tid);
     }
   }
   Parts<NP> xq[4];
@@ -375,8 +383,8 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
     if ((nt >> 1) <= (mt >> 1)) {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        const Parts<NP> kj = staged<NP>(sk, nt * 4 + ks, l);
-        if (C == 64 || wave < MT) mma(kk, staged<NP>(sk, mt * 4 + ks, l), kj);
+        const Parts<NP> kj = staged<NP>(sk, nt * 4 + ks, rs);
+        if (C == 64 || wave < MT) mma(kk, staged<NP>(sk, mt * 4 + ks, rs), kj);
         if (C == 64 || wave >= MT) mma(qk, xq[ks], kj);
       }
     }
@@ -455,7 +463,7 @@ __device__ __forceinline__ void fetch_rows(const Rows& x, const Span& sp, int64_
   const uint16_t* p = uniform(row_at<uint16_t>(x, sp, t0, h));
 #pragma unroll
   for (int mt = 0; mt < C / 16; ++mt) {
-    const int t = min(tile_row(mt, l & 15), left - 1);
+    const int t = min(tile_row(mt, (l - 4 * (l >> 4)) & 15), left - 1);      // (row_slot)
     load_lds16(p, (uint32_t)(t * (int)x.st + 32 * wave + 8 * (l >> 4)) * 2u, lds + (mt * 4 + wave) * kUnit);
   }
 }
@@ -494,12 +502,11 @@ template <typename T> struct Slice {
 template <typename T> struct ScanLds {
   using F = Pack<T, false>;
   using B = Pack<T, true>;
-  // forward: K then K^T | Q | Tm | P | gates | V, then O
-  static constexpr int kKq = F::kRows > F::kCols ? F::kRows : F::kCols;
-  static constexpr size_t kFwd = (size_t)(kKq + F::kRows + F::kT + F::kP + 1 + 16) * kUnit;
-  static constexpr size_t kFwdState = (size_t)(kKq + F::kT + 1 + 16) * kUnit;
-  // backward: K then Q^T | K^T | Tm^T | P^T | gates
-  static constexpr size_t kBwd = (size_t)(kKq + B::kCols + B::kT + B::kP + 1) * kUnit;
+  // forward: K | Tm | gates | V, then O | Q | P
+  static constexpr size_t kFwdState = (size_t)(F::kRows + F::kT + 1 + 16) * kUnit;
+  static constexpr size_t kFwd = kFwdState + (size_t)(F::kRows + F::kP) * kUnit;
+  // backward: K | Q | Tm^T | P^T | gates
+  static constexpr size_t kBwd = (size_t)(2 * B::kRows + B::kT + B::kP + 1) * kUnit;
 };
 
 // A [rows][128] fp32 matrix <-> the wave's tiles of it (rows tile_row, two tiles of 16 columns).  The
@@ -528,7 +535,7 @@ __device__ __forceinline__ void tiles_store(const floatx4 (&S)[kTiles][2], float
 }
 
 // kOut: the outputs (and what the backward pass needs).  Otherwise only what a segment does to
-// the state: blockIdx.z 0 what it adds, 1 its product of transitions (V = 0 from the
+// the state: blockIdx.y 0 what it adds, 1 its product of transitions (V = 0 from the
 // identity).
 template <typename T, bool kOut>
 __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
@@ -536,29 +543,29 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
   constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32;
   extern __shared__ __align__(16) char lds[];
   char* bk = lds;
-  char* bt = bk + ScanLds<T>::kKq * kUnit;
+  char* bt = bk + K::kRows * kUnit;
   char* bg = bt + K::kT * kUnit;
   char* bv = bg + kUnit;
   char* bq = bv + 16 * kUnit;
   char* bp = bq + K::kRows * kUnit;
-  const int h = blockIdx.y, hk = h / (a.Hv / a.Hk), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
+  const int piece_slot = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, hk = h / (a.Hv / a.Hk), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
   bv += wave * 4 * kUnit;
   int piece = 0, c0 = 0, c1;
   Span sp;
   if (a.seg) {
-    sp = slot_of(a.s, blockIdx.x, C * a.seg, piece);
+    sp = slot_of(a.s, piece_slot, C * a.seg, piece);
     if (piece < 0) return;
     c0 = piece * a.seg;
   } else {
-    sp = span_of(a.s, blockIdx.x, C);
+    sp = span_of(a.s, piece_slot, C);
   }
   const int chunks = (sp.len + C - 1) / C;
   const bool last = !a.seg || c0 + a.seg >= chunks;
   c1 = last ? chunks : c0 + a.seg;
-  const bool ident = !kOut && blockIdx.z == 1;
+  const bool ident = !kOut && blockIdx.y == 1;
   if (!kOut && (last || (ident && piece == 0))) return;      // nobody asks for it
   const int slot0 = a.s.cu ? span_of(a.s, sp.n, C).slot0 : sp.n * chunks;
-  const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)blockIdx.x * a.Hv + h) * kHead * kHead;
+  const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)piece_slot * a.Hv + h) * kHead * kHead;
 
   floatx4 S[8][2];
   const float* from = piece == 0 ? (a.state_in ? a.state_in + sn : nullptr) : kOut ? a.init + gn : nullptr;
@@ -582,6 +589,8 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
     if constexpr (NP == 1) fetch_rows<C>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
     else fetch(a.qr + atk * K::kRows * kUnit, lds_addr(bq), K::kRows, wave, l);
   };
+  constexpr int kSome = NP == 1 ? 4 : 2;
+  const int rs = row_slot(g, l & 15), place = cols_place(l);
   const int slice[2] = {Slice<T>::lane(g, 0, l & 15), Slice<T>::lane(g, 1, l & 15)};
   auto fetch_v = [&](int64_t t0, int left) {
     if (!ident) Slice<T>::fetch(a.v, sp, t0, left, h, wave, lds_addr(bv), l);
@@ -606,8 +615,6 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
     __syncthreads();
     if (kOut && a.s0) tiles_store(S, a.s0 + at * kHead * kHead, wave, l);
 
-    const bf16x8* sk = reinterpret_cast<const bf16x8*>(bk);
-    const bf16x8* sq = reinterpret_cast<const bf16x8*>(bq);
     const bf16x8* st = reinterpret_cast<const bf16x8*>(bt);
     const bf16x8* spm = reinterpret_cast<const bf16x8*>(bp);
     const float* gates = reinterpret_cast<const float*>(bg);
@@ -621,32 +628,28 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
       Parts<3> s[2];
 #pragma unroll
       for (int n = 0; n < 2; ++n) s[n] = split_pair(S[2 * ks][n], S[2 * ks + 1][n]);
+      Parts<NP> k[MT];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const Parts<NP> k = staged<NP>(sk, mt * 4 + ks, l);
-        mma(X[mt][0], k, s[0]);
-        mma(X[mt][1], k, s[1]);
-      }
+      for (int mt = 0; mt < MT; ++mt) k[mt] = rows_of<NP>(bk, mt, ks, rs);
+      mma_grid(X, k, s);
       if constexpr (kOut) {
         // for a bf16 output two parts of the state do (2^-17 of it)
         constexpr int kS = NP == 1 ? 2 : 3;
+        Parts<kS> x[2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const Parts<NP> q = staged<NP>(sq, mt * 4 + ks, l);
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            Parts<kS> x;
+          for (int i = 0; i < kS; ++i) x[n].p[i] = s[n].p[i];
 #pragma unroll
-            for (int i = 0; i < kS; ++i) x.p[i] = s[n].p[i];
-            mma(O[mt][n], q, x);
-          }
-        }
+        for (int mt = 0; mt < MT; ++mt) k[mt] = rows_of<NP>(bq, mt, ks, rs);
+        mma_grid(O, k, x);
       }
       __builtin_amdgcn_sched_barrier(0);                     // (later steps' operands are not read ahead into registers)
     }
-    __syncthreads();                                         // K and Q are free
-    fetch(a.kt + atk * K::kCols * kUnit, lds_addr(bk), K::kCols, wave, l);
-    if (kOut && more) fetch_q(t1, left1, atk + a.Hk);
+    if (kOut && more) {
+      __syncthreads();                                       // Q is free
+      fetch_q(t1, left1, atk + a.Hk);
+    }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const floatx4 e = *reinterpret_cast<const floatx4*>(gates + 8 * g + tile_at(mt, 0));
@@ -669,14 +672,12 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) r[n] = split_pair(X[2 * js][n], X[2 * js + 1][n]);
 #pragma unroll
-      for (int mt = 2 * js; mt < MT; ++mt) {
-        const Parts<3> x = staged<3>(st, Square<C>::at(mt, js, false), l);
-        mma(U[mt][0], x, r[0]);
-        mma(U[mt][1], x, r[1]);
+      for (int mt = 2 * js; mt < MT; mt += 2) {
+        const Parts<3> x[2] = {staged<3>(st, Square<C>::at(mt, js, false), l), staged<3>(st, Square<C>::at(mt + 1, js, false), l)};
+        mma_grid(U + mt, x, r);
       }
     }
-    wait_loads();
-    __syncthreads();                                         // K^T is there; Tm and this wave's V are free
+    __syncthreads();                                         // Tm is free
     if (more) fetch(a.tm + (at + a.Hv) * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
     if constexpr (kOut) {
 #pragma unroll
@@ -689,10 +690,10 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
           for (int i = 0; i < K::kPParts; ++i) u[n].p[i] = p.p[i];
         }
 #pragma unroll
-        for (int mt = 2 * js; mt < MT; ++mt) {
-          const Parts<K::kPParts> x = staged<K::kPParts>(spm, Square<C>::at(mt, js, false), l);
-          mma(O[mt][0], x, u[0]);
-          mma(O[mt][1], x, u[1]);
+        for (int mt = 2 * js; mt < MT; mt += 2) {
+          const Parts<K::kPParts> x[2] = {staged<K::kPParts>(spm, Square<C>::at(mt, js, false), l),
+                                          staged<K::kPParts>(spm, Square<C>::at(mt + 1, js, false), l)};
+          mma_grid(O + mt, x, u);
         }
       }
 #pragma unroll
@@ -731,10 +732,11 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
         u[n] = split3(x);
       }
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const Parts<NP> k = staged<NP>(sk, t * JS + js, l);
-        mma(S[t][0], k, u[0]);
-        mma(S[t][1], k, u[1]);
+      for (int t = 0; t < 8; t += kSome) {
+        Parts<NP> k[kSome];
+#pragma unroll
+        for (int i = 0; i < kSome; ++i) k[i] = cols_of<NP>(bk, t + i, js, place);
+        mma_grid(S + t, k, u);
       }
     }
     __syncthreads();                                         // all buffers but Q, Tm and V are free
@@ -756,26 +758,26 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
   constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32;
   extern __shared__ __align__(16) char lds[];
   char* bk = lds;
-  char* bkt = bk + ScanLds<T>::kKq * kUnit;
-  char* bt = bkt + K::kCols * kUnit;
+  char* bq = bk + K::kRows * kUnit;
+  char* bt = bq + K::kRows * kUnit;
   char* bp = bt + K::kT * kUnit;
   char* bg = bp + K::kP * kUnit;
-  const int h = blockIdx.y, hk = h / (a.Hv / a.Hk), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
+  const int piece_slot = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, hk = h / (a.Hv / a.Hk), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
   int piece = 0, c0 = 0;
   Span sp;
   if (a.seg) {
-    sp = slot_of(a.s, blockIdx.x, C * a.seg, piece);
+    sp = slot_of(a.s, piece_slot, C * a.seg, piece);
     if (piece < 0) return;
     c0 = piece * a.seg;
   } else {
-    sp = span_of(a.s, blockIdx.x, C);
+    sp = span_of(a.s, piece_slot, C);
   }
   const int chunks = (sp.len + C - 1) / C;
   const bool last = !a.seg || c0 + a.seg >= chunks;
   const int c1 = last ? chunks : c0 + a.seg;
   if (!kOut && piece == 0) return;                           // nobody asks for it
   const int slot0 = a.s.cu ? span_of(a.s, sp.n, C).slot0 : sp.n * chunks;
-  const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)blockIdx.x * a.Hv + h) * kHead * kHead;
+  const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)piece_slot * a.Hv + h) * kHead * kHead;
 
   floatx4 S[8][2];                                           // dS
   const float* from = last ? (a.dstate_out ? a.dstate_out + sn : nullptr) : kOut ? a.init + gn : nullptr;
@@ -801,6 +803,12 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
     if constexpr (NP == 1) fetch_rows<C>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
     else fetch(a.kr + atk * K::kRows * kUnit, lds_addr(bk), K::kRows, wave, l);
   };
+  auto fetch_q = [&](int64_t t0, int left, int64_t atk) {
+    if constexpr (NP == 1) fetch_rows<C>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
+    else fetch(a.qr + atk * K::kRows * kUnit, lds_addr(bq), K::kRows, wave, l);
+  };
+  constexpr int kSome = NP == 1 ? 4 : 2;
+  const int rs = row_slot(g, l & 15), place = cols_place(l);
   if (c0 < c1) {
     const int64_t t0 = (int64_t)(c1 - 1) * C, at = (int64_t)(slot0 + c1 - 1) * a.Hv + h, atk = (int64_t)(slot0 + c1 - 1) * a.Hk + hk;
     load_do(t0, sp.len - (int)t0);
@@ -808,7 +816,7 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
     fetch(a.gates + at * (kUnit / 4), lds_addr(bg), 1, wave, l);
     fetch(a.pm + at * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
     fetch(a.tm + at * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
-    fetch(a.kt + atk * K::kCols * kUnit, lds_addr(bkt), K::kCols, wave, l);
+    fetch_q(t0, sp.len - (int)t0, atk);
   }
   for (int c = c1 - 1; c >= c0; --c) {
     const int64_t t0 = (int64_t)c * C, at = (int64_t)(slot0 + c) * a.Hv + h, atk = (int64_t)(slot0 + c) * a.Hk + hk;
@@ -818,8 +826,6 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
     __syncthreads();
     if (kOut) tiles_store(S, a.ds1 + at * kHead * kHead, wave, l);
 
-    const bf16x8* sk = reinterpret_cast<const bf16x8*>(bk);
-    const bf16x8* skt = reinterpret_cast<const bf16x8*>(bkt);
     const bf16x8* st = reinterpret_cast<const bf16x8*>(bt);
     const bf16x8* spm = reinterpret_cast<const bf16x8*>(bp);
     const float* gates = reinterpret_cast<const float*>(bg);
@@ -833,15 +839,12 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
       Parts<3> s[2];
 #pragma unroll
       for (int n = 0; n < 2; ++n) s[n] = split_pair(S[2 * ks][n], S[2 * ks + 1][n]);
+      Parts<NP> k[MT];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const Parts<NP> k = staged<NP>(sk, mt * 4 + ks, l);
-        mma(X[mt][0], k, s[0]);
-        mma(X[mt][1], k, s[1]);
-      }
+      for (int mt = 0; mt < MT; ++mt) k[mt] = rows_of<NP>(bk, mt, ks, rs);
+      mma_grid(X, k, s);
+      __builtin_amdgcn_sched_barrier(0);                     // (later steps' operands are not read ahead into registers)
     }
-    __syncthreads();                                         // K is free
-    fetch(a.qt + atk * K::kCols * kUnit, lds_addr(bk), K::kCols, wave, l);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const floatx4 e = *reinterpret_cast<const floatx4*>(gates + C + 8 * g + tile_at(mt, 0));
@@ -860,10 +863,9 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
         p[n] = parts_of<NP>(x);
       }
 #pragma unroll
-      for (int mt = 0; mt < 2 * js + 2; ++mt) {
-        const Parts<3> x = staged<3>(spm, Square<C>::at(mt, js, true), l);
-        mma(X[mt][0], x, p[0]);                              // dU
-        mma(X[mt][1], x, p[1]);
+      for (int mt = 0; mt < 2 * js + 2; mt += 2) {           // dU
+        const Parts<3> x[2] = {staged<3>(spm, Square<C>::at(mt, js, true), l), staged<3>(spm, Square<C>::at(mt + 1, js, true), l)};
+        mma_grid(X + mt, x, p);
       }
     }
 #pragma unroll
@@ -872,14 +874,12 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) p[n] = split_pair(X[2 * js][n], X[2 * js + 1][n]);
 #pragma unroll
-      for (int mt = 0; mt < 2 * js + 2; ++mt) {
-        const Parts<3> x = staged<3>(st, Square<C>::at(mt, js, true), l);
-        mma(R[mt][0], x, p[0]);                              // dR
-        mma(R[mt][1], x, p[1]);
+      for (int mt = 0; mt < 2 * js + 2; mt += 2) {           // dR
+        const Parts<3> x[2] = {staged<3>(st, Square<C>::at(mt, js, true), l), staged<3>(st, Square<C>::at(mt + 1, js, true), l)};
+        mma_grid(R + mt, x, p);
       }
     }
-    wait_loads();
-    __syncthreads();                                         // Q^T is there; Tm^T and P^T are free
+    __syncthreads();                                         // Tm^T and P^T are free
     if (more) {
       fetch(a.pm + (at - a.Hv) * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
       fetch(a.tm + (at - a.Hv) * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
@@ -919,19 +919,21 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
         q[n] = split_pair(R[2 * js][n], R[2 * js + 1][n]);
       }
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const Parts<NP> x = staged<NP>(sk, t * JS + js, l), y = staged<NP>(skt, t * JS + js, l);
-        mma(S[t][0], x, p[0]);
-        mma(S[t][1], x, p[1]);
-        mma(S[t][0], y, q[0]);
-        mma(S[t][1], y, q[1]);
+      for (int t = 0; t < 8; t += kSome) {
+        Parts<NP> x[kSome];
+#pragma unroll
+        for (int i = 0; i < kSome; ++i) x[i] = cols_of<NP>(bq, t + i, js, place);
+        mma_grid(S + t, x, p);
+#pragma unroll
+        for (int i = 0; i < kSome; ++i) x[i] = cols_of<NP>(bk, t + i, js, place);
+        mma_grid(S + t, x, q);
       }
     }
     if (more) load_do(t0 - C, left + C);
     __syncthreads();                                         // all buffers but Tm^T and P^T are free
     if (more) {
       fetch_k(t0 - C, left + C, atk - a.Hk);
-      fetch(a.kt + (atk - a.Hk) * K::kCols * kUnit, lds_addr(bkt), K::kCols, wave, l);
+      fetch_q(t0 - C, left + C, atk - a.Hk);
       fetch(a.gates + (at - a.Hv) * (kUnit / 4), lds_addr(bg), 1, wave, l);
     }
   }
@@ -945,8 +947,8 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
 template <bool kBwd>
 __global__ __launch_bounds__(512) void delta_join_kernel(DeltaArgs a, int chunk) {
   __shared__ __align__(16) bf16x8 buf[2][4 * 3 * 64];
-  const int h = blockIdx.y, wave = threadIdx.x >> 6, l = lane_id(), g = l >> 4, m = l & 15, col = 16 * blockIdx.z + m;
-  const Span sp = span_of(a.s, blockIdx.x, chunk * a.seg);
+  const int h = blockIdx.y, wave = threadIdx.x >> 6, l = lane_id(), g = l >> 4, m = l & 15, col = 16 * blockIdx.x + m;
+  const Span sp = span_of(a.s, blockIdx.z, chunk * a.seg);
   const int pieces = (sp.len + chunk * a.seg - 1) / (chunk * a.seg);
   if (pieces == 0) {                                         // no token: no segment to hand the state on
     const float* from = kBwd ? a.dstate_out : a.state_in;
@@ -1023,9 +1025,11 @@ template <typename T> struct GradLds {
   // what enters dq and dk alone: for bf16 two parts do (2^-17 of it)
   static constexpr int kIn = NP == 1 ? 2 : 3;
   static constexpr int kStage = MT * (NP + 3 + 3) * kUnit;   // dO, U, dR: 32 elements of every token
+  static constexpr int kRows = MT * 4 * NP * kUnit;          // K, Q
   static constexpr int kKind = MT * JS * kIn * kUnit;        // a [C][C] operand
   static constexpr int kLate = 3 * kKind + C * kLd * 4;
-  static constexpr int kBig = 2 * kStage > kLate ? 2 * kStage : kLate;
+  static constexpr int kEarly = kStage + 2 * kRows;
+  static constexpr int kBig = kEarly > kLate ? kEarly : kLate;
   static constexpr size_t kBytes = kBig + 4 * (12 * C + 5 * C + C + MT * C + 4) + 8 * C;
 };
 
@@ -1038,11 +1042,12 @@ __device__ __forceinline__ double wave_sum(double x) {
 template <typename T>
 __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   using L = GradLds<T>;
-  using K = Pack<T, true>;
   constexpr int C = L::C, NP = L::NP, MT = L::MT, JS = L::JS, kIn = L::kIn, LD = L::kLd;
   constexpr int kTiles = MT * (MT + 1) / 2, kMine = (kTiles + 3) / 4;
   extern __shared__ __align__(16) char lds[];
-  bf16x8* stage = reinterpret_cast<bf16x8*>(lds);            // [2][dO | U | dR]
+  bf16x8* stage = reinterpret_cast<bf16x8*>(lds);            // dO | U | dR
+  char* bk = lds + L::kStage;
+  char* bq = bk + L::kRows;
   char* xe = lds;                                            // scale E D, then its transpose, then B + B^T
   char* xt = xe + L::kKind;
   char* xb = xt + L::kKind;
@@ -1053,7 +1058,7 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   float* fs = db + C;                                        // [MT][C]: sums of F (K K^T) D by tiles
   float* cross = fs + MT * C;                                     // [4]
   double* dsum = reinterpret_cast<double*>(cross + 4);       // [C]
-  const int slot = blockIdx.x, h = blockIdx.y, share = a.Hv / a.Hk, hk = h / share, tid = threadIdx.x, l = lane_id(), g = l >> 4;
+  const int slot = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, share = a.Hv / a.Hk, hk = h / share, tid = threadIdx.x, l = lane_id(), g = l >> 4;
   const int m = l & 15, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int c;
   const Span sp = slot_of(a.s, slot, C, c);
@@ -1063,6 +1068,13 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   const int64_t tok = (int64_t)sp.b * a.s.T + sp.t0 + t0;    // row of [B * T]
   const int64_t at = (int64_t)slot * a.Hv + h, atk = (int64_t)slot * a.Hk + hk;
 
+  if constexpr (NP == 1) {
+    fetch_rows<C>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
+    fetch_rows<C>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
+  } else {
+    fetch(a.kr + atk * L::kRows, lds_addr(bk), L::kRows / kUnit, wave, l);
+    fetch(a.qr + atk * L::kRows, lds_addr(bq), L::kRows / kUnit, wave, l);
+  }
   {
     // a thread's 8 elements of each 32: token tid / 4
     const int st = tid >> 2, so = tid & 3;
@@ -1094,9 +1106,9 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
         y[i] = sizeof(T) == 4 ? __uint_as_float(w) : i & 1 ? bf16hi(w) : bf16lo(w);
       }
     };
-    auto put = [&](int buf) {
+    auto put = [&]() {
       if (!mine) return;
-      bf16x8* to = stage + buf * (L::kStage / 16) + 16 * so + (st & 15);
+      bf16x8* to = stage + 16 * so + (st & 15);
       const int tile = st >> 4;
       float fo[8], fv[8];
       floats(xo, fo);
@@ -1128,7 +1140,6 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
     const float* s1p = uniform(a.ds1 + at * kHead * kHead);
 #pragma unroll 1
     for (int ks = 0; ks < 4; ++ks) {
-      put(ks & 1);
       float y[2][8], z[2][8];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -1136,9 +1147,11 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
         load8(s0p + o, y[e]);
         load8(s1p + o, z[e]);
       }
+      if (ks) __syncthreads();                               // the last elements' operands are read
+      put();
       __syncthreads();
       if (ks < 3) load(ks + 1);
-      const bf16x8* so_ = stage + (ks & 1) * (L::kStage / 16);
+      const bf16x8* so_ = stage;
       const bf16x8* su_ = so_ + MT * NP * 64;
       const bf16x8* sr_ = su_ + MT * 3 * 64;
       Parts<3> sx[2];
@@ -1215,27 +1228,48 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
       }
     }
     for (int i = tid; i < MT * C; i += 256) fs[i] = 0.f;
-    __syncthreads();                                         // the staged operands are read
+    wait_loads();
+    __syncthreads();                                         // K and Q are there
+    floatx4 QK[kMine], KK[kMine];
+    const int place = cols_place(l);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int t = wave + 4 * i;
+      QK[i] = KK[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+      if (t < kTiles) {
+        const int mt = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, nt = t - mt * (mt + 1) / 2;
+        // rows 16 mt + m of the tokens: where tile_row has them
+        auto natural = [&](const char* src, int tile, int ks) {
+          const int tk = 16 * tile + m, x = 2 * (tk >> 5) + ((tk >> 2) & 1), y = 4 * ((tk >> 3) & 3) + (tk & 3);
+          return staged<NP>(reinterpret_cast<const bf16x8*>(src), x * 4 + ks, row_slot(g, y));
+        };
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const Parts<NP> kj = natural(bk, nt, ks);
+          mma(QK[i], natural(bq, mt, ks), kj);
+          mma(KK[i], natural(bk, mt, ks), kj);
+        }
+      }
+    }
+    Parts<NP> kt[JS][2], qt[JS][2];                          // this wave's rows of K^T and Q^T
+#pragma unroll
+    for (int js = 0; js < JS; ++js)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        kt[js][e] = cols_of<NP>(bk, 2 * wave + e, js, place);
+        qt[js][e] = cols_of<NP>(bq, 2 * wave + e, js, place);
+      }
+    __syncthreads();                                         // all operands are read
     for (int i = tid; i < L::kLate / 16; i += 256) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
     __syncthreads();
 
-    // Q K^T and K K^T of the wave's tiles; E and F become the operands of the products over tokens
+    // E and F become the operands of the products over tokens
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int t = wave + 4 * i;
       if (t < kTiles) {
         const int mt = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, nt = t - mt * (mt + 1) / 2;
-        const int ia = 16 * mt + m, j = 16 * nt + m;
-        const T* pq = row_at<T>(a.q, sp, t0 + ia, hk) + 8 * g;
-        const T* pk = row_at<T>(a.k, sp, t0 + ia, hk) + 8 * g;
-        const T* pj = row_at<T>(a.k, sp, t0 + j, hk) + 8 * g;
-        floatx4 QK = {0.f, 0.f, 0.f, 0.f}, KK = QK;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const Parts<NP> kj = operand<T>(pj + 32 * ks, j < left);
-          mma(QK, operand<T>(pq + 32 * ks, ia < left), kj);
-          mma(KK, operand<T>(pk + 32 * ks, ia < left), kj);
-        }
+        const int j = 16 * nt + m;
         float ed[4], bb[4], f[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -1244,8 +1278,8 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
           const float fd = j < ii ? F[i][r] * d : 0.f;
           ed[r] = a.scale * E[i][r] * d;
           bb[r] = -gates[2 * C + ii] * fd;
-          f[r] = row16_sum(fd * KK[r]);
-          sm[ii * LD + j] = j < ii ? ed[r] * QK[r] + bb[r] * KK[r] : 0.f;
+          f[r] = row16_sum(fd * KK[i][r]);
+          sm[ii * LD + j] = j < ii ? ed[r] * QK[i][r] + bb[r] * KK[i][r] : 0.f;
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -1286,30 +1320,22 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
     __syncthreads();
 
     // the products with K and Q
-    const bf16x8* ktp = reinterpret_cast<const bf16x8*>(a.kt + atk * K::kCols * kUnit);
-    const bf16x8* qtp = reinterpret_cast<const bf16x8*>(a.qt + atk * K::kCols * kUnit);
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
-      Parts<NP> kt[2], qt[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        kt[e] = staged<NP>(ktp, (2 * wave + e) * JS + js, l);
-        qt[e] = staged<NP>(qtp, (2 * wave + e) * JS + js, l);
-      }
 #pragma unroll
       for (int n = 0; n < MT; ++n) {
         const Parts<kIn> b = staged<kIn>(reinterpret_cast<const bf16x8*>(xb), n * JS + js, l);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) mma(dk[e][n], kt[e], b);
+        for (int e = 0; e < 2; ++e) mma(dk[e][n], kt[js][e], b);
         if (js <= n / 2) {
           const Parts<kIn> x = staged<kIn>(reinterpret_cast<const bf16x8*>(xe), n * JS + js, l);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) mma(dq[e][n], kt[e], x);
+          for (int e = 0; e < 2; ++e) mma(dq[e][n], kt[js][e], x);
         }
         if (js >= n / 2) {
           const Parts<kIn> x = staged<kIn>(reinterpret_cast<const bf16x8*>(xt), n * JS + js, l);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) mma(dk[e][n], qt[e], x);
+          for (int e = 0; e < 2; ++e) mma(dk[e][n], qt[js][e], x);
         }
       }
     }
@@ -1376,7 +1402,7 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void delta_shared_kernel(DeltaArgs a) {
   constexpr int C = DeltaType<T>::kChunk;
-  const int slot = blockIdx.x, hk = blockIdx.y, share = a.Hv / a.Hk;
+  const int slot = blockIdx.x / a.Hk, hk = blockIdx.x % a.Hk, share = a.Hv / a.Hk;
   int c;
   const Span sp = slot_of(a.s, slot, C, c);
   if (c < 0) return;
@@ -1410,9 +1436,9 @@ inline size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 struct DeltaSizes {
   int C, seg;                 // tokens of a chunk; chunks of a segment, 0: none
   int64_t slots, segs;        // 0 slots: out of range
-  size_t tm, pm, gates, sums, kt, qt, kr, qr, states, s0, u;
+  size_t tm, pm, gates, sums, kr, states, s0, u;
   size_t workspace(bool backward) const {
-    return backward ? tm + pm + gates + sums + kt + qt + kr + 2 * states + s0 + u : tm + pm + gates + kt + kr + qr + 3 * states;
+    return tm + pm + gates + sums + 2 * kr + (backward ? 2 * states + s0 + u : 3 * states);
   }
   size_t saved() const { return s0 + u + states; }
 };
@@ -1421,15 +1447,8 @@ template <typename T, bool kBwd> void pack_sizes(DeltaSizes& z, size_t n, size_t
   z.tm = n * K::kT * gsa::kUnit;
   z.pm = n * K::kP * gsa::kUnit;
   z.gates = n * gsa::kUnit;
-  z.kt = nk * K::kCols * gsa::kUnit;
-  if (kBwd) {
-    z.sums = up(n * 2 * K::C * 4);
-    z.qt = z.kt;
-  }
-  if (K::NP == 3) {
-    z.kr = nk * K::kRows * gsa::kUnit;
-    if (!kBwd) z.qr = z.kr;
-  }
+  if (kBwd) z.sums = up(n * 2 * K::C * 4);
+  if (K::NP == 3) z.kr = nk * K::kRows * gsa::kUnit;
 }
 DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtype, bool backward) {
   DeltaSizes z{};
@@ -1437,7 +1456,7 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   if (B < 1 || T < 1 || N < 1 || Hk < 1 || Hv < Hk || Hv % Hk || !dtype_size(dtype)) return z;
   const int64_t nc = (T + z.C - 1) / z.C;
   z.slots = packed ? (int64_t)T / z.C + N : B * nc;
-  if (z.slots > 0x7fffffff) {
+  if (z.slots * Hv > 1 << 23 || (int64_t)N * Hv > 1 << 23) {    // a grid of 256 threads each
     z.slots = 0;
     return z;
   }
@@ -1474,39 +1493,39 @@ template <auto kKernel> int allow_lds(size_t bytes) {
 template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
   using L = gsa::ScanLds<T>;
   static_assert(2 * L::kFwd <= 160 * 1024, "two blocks a CU");
-  hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, false>), dim3(z.slots, a.Hv), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, false>), dim3(z.slots * a.Hv), dim3(256), 0, s, a);
   if (const int e = launch_status()) return e;
   if (a.seg) {
     if (const int e = allow_lds<gsa::delta_scan_kernel<T, false>>(L::kFwdState)) return e;
-    hipLaunchKernelGGL((gsa::delta_scan_kernel<T, false>), dim3(z.segs, a.Hv, 2), dim3(256), L::kFwdState, s, a);
+    hipLaunchKernelGGL((gsa::delta_scan_kernel<T, false>), dim3(z.segs * a.Hv, 2), dim3(256), L::kFwdState, s, a);
     if (const int e = launch_status()) return e;
-    hipLaunchKernelGGL(gsa::delta_join_kernel<false>, dim3(a.s.N, a.Hv, 8), dim3(512), 0, s, a, z.C);
+    hipLaunchKernelGGL(gsa::delta_join_kernel<false>, dim3(8, a.Hv, a.s.N), dim3(512), 0, s, a, z.C);
     if (const int e = launch_status()) return e;
   }
   if (const int e = allow_lds<gsa::delta_scan_kernel<T, true>>(L::kFwd)) return e;
-  hipLaunchKernelGGL((gsa::delta_scan_kernel<T, true>), dim3(a.seg ? z.segs : a.s.N, a.Hv), dim3(256), L::kFwd, s, a);
+  hipLaunchKernelGGL((gsa::delta_scan_kernel<T, true>), dim3((a.seg ? z.segs : a.s.N) * a.Hv), dim3(256), L::kFwd, s, a);
   return launch_status();
 }
 template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
   constexpr size_t lds = gsa::ScanLds<T>::kBwd, lds_grads = gsa::GradLds<T>::kBytes;
   static_assert(2 * lds <= 160 * 1024 && 2 * lds_grads <= 160 * 1024, "two blocks a CU");
-  hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, true>), dim3(z.slots, a.Hv), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, true>), dim3(z.slots * a.Hv), dim3(256), 0, s, a);
   if (const int e = launch_status()) return e;
   if (a.seg) {
     if (const int e = allow_lds<gsa::delta_scan_bwd_kernel<T, false>>(lds)) return e;
-    hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, false>), dim3(z.segs, a.Hv), dim3(256), lds, s, a);
+    hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, false>), dim3(z.segs * a.Hv), dim3(256), lds, s, a);
     if (const int e = launch_status()) return e;
-    hipLaunchKernelGGL(gsa::delta_join_kernel<true>, dim3(a.s.N, a.Hv, 8), dim3(512), 0, s, a, z.C);
+    hipLaunchKernelGGL(gsa::delta_join_kernel<true>, dim3(8, a.Hv, a.s.N), dim3(512), 0, s, a, z.C);
     if (const int e = launch_status()) return e;
   }
   if (const int e = allow_lds<gsa::delta_scan_bwd_kernel<T, true>>(lds)) return e;
-  hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, true>), dim3(a.seg ? z.segs : a.s.N, a.Hv), dim3(256), lds, s, a);
+  hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, true>), dim3((a.seg ? z.segs : a.s.N) * a.Hv), dim3(256), lds, s, a);
   if (const int e = launch_status()) return e;
   if (const int e = allow_lds<gsa::delta_grads_kernel<T>>(lds_grads)) return e;
-  hipLaunchKernelGGL(gsa::delta_grads_kernel<T>, dim3(z.slots, a.Hv), dim3(256), lds_grads, s, a);
+  hipLaunchKernelGGL(gsa::delta_grads_kernel<T>, dim3(z.slots * a.Hv), dim3(256), lds_grads, s, a);
   if (a.Hv > a.Hk) {
     if (const int e = launch_status()) return e;
-    hipLaunchKernelGGL(gsa::delta_shared_kernel<T>, dim3(z.slots, a.Hk), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(gsa::delta_shared_kernel<T>, dim3(z.slots * a.Hk), dim3(256), 0, s, a);
   }
   return launch_status();
 }
@@ -1560,10 +1579,8 @@ int delta_args(const gsa_delta_args* x, bool backward, gsa::DeltaArgs& a, DeltaS
   a.pm = take(z.pm);
   a.gates = reinterpret_cast<float*>(take(z.gates));
   a.sums = reinterpret_cast<float*>(take(z.sums));
-  a.kt = take(z.kt);
-  a.qt = take(z.qt);
   a.kr = take(z.kr);
-  a.qr = take(z.qr);
+  a.qr = take(z.kr);
   a.seg = z.seg;
   a.segs = (int)z.segs;
   a.add = reinterpret_cast<float*>(take(z.states));
