@@ -40,29 +40,27 @@ constexpr int tile_at(int t, int r) { return 32 * (t >> 1) + 4 * (t & 1) + r; }
 
 template <int N> struct Parts { bf16x8 p[N]; };
 
-__device__ __forceinline__ Parts<3> split3(const float (&x)[8]) {
-  Parts<3> r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const __bf16 a = (__bf16)x[i];
-    const float e = x[i] - (float)a;
-    const __bf16 b = (__bf16)e;
-    r.p[0][i] = a;
-    r.p[1][i] = b;
-    r.p[2][i] = (__bf16)(e - (float)b);
-  }
-  return r;
+// Rounded to bf16 by pairs (one v_cvt_pk_bf16_f32); what is left of them.
+__device__ __forceinline__ uint32_t take_part(float& x, float& y) {
+  const uint32_t p = pack_bf16(x, y);
+  x -= bf16lo(p);
+  y -= bf16hi(p);
+  return p;
 }
 template <int N> __device__ __forceinline__ Parts<N> parts_of(const float (&x)[8]) {
-  if constexpr (N == 3) {
-    return split3(x);
-  } else {
-    Parts<1> r;
+  u32x4 w[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.p[0][i] = (__bf16)x[i];
-    return r;
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int n = 0; n < N; ++n) w[n][i] = n + 1 < N ? take_part(a, b) : pack_bf16(a, b);
   }
+  Parts<N> r;
+#pragma unroll
+  for (int n = 0; n < N; ++n) r.p[n] = __builtin_bit_cast(bf16x8, w[n]);
+  return r;
 }
+__device__ __forceinline__ Parts<3> split3(const float (&x)[8]) { return parts_of<3>(x); }
 __device__ __forceinline__ Parts<3> split_pair(const floatx4& a, const floatx4& b) {
   const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   return split3(x);
@@ -351,7 +349,7 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
       bt[l] = b;
       float* gates = a.gates + at * (kUnit / 4);
       gates[l] = expf((float)G);
-      gates[C + l] = expf((float)(Ge - G));
+      gates[C + l] = ok ? expf((float)(Ge - G)) : 0.f;        // (nothing comes from behind the sequence)
       gates[2 * C + l] = b;
       if (kBwd) {
         a.sums[at * 2 * C + l] = hi;
@@ -446,8 +444,8 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
 // ---------------------------------------------------------------------------
 template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
   const uint64_t x = reinterpret_cast<uint64_t>(p);
-  return reinterpret_cast<const P*>((uint64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
-                                    (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+  const uint64_t y = (uint64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+  return (const P*)(__attribute__((address_space(1))) const P*)y;      // global memory, said so that accesses are not flat ones
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -659,7 +657,7 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float v = ident ? 0.f : to_f32(*reinterpret_cast<const T*>(bv + slice[n] + tile_at(mt, r) * Slice<T>::kRow));
-          X[mt][n][r] = 8 * g + tile_at(mt, r) < left ? b[r] * (v - e[r] * X[mt][n][r]) : 0.f;          // R
+          X[mt][n][r] = b[r] * (v - e[r] * X[mt][n][r]);     // R (behind the sequence beta is 0)
           if (kOut) O[mt][n][r] *= a.scale * e[r];
         }
     }
@@ -851,7 +849,7 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) X[mt][n][r] = 8 * g + tile_at(mt, r) < left ? X[mt][n][r] * e[r] : 0.f;
+        for (int r = 0; r < 4; ++r) X[mt][n][r] *= e[r];
     }
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
