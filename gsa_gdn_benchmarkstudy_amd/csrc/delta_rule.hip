@@ -78,10 +78,10 @@ __device__ __forceinline__ void mma(floatx4& acc, const Parts<NA>& a, const Part
         if (i + j == o) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
 }
 
-// acc[i][n] += a[i] b[n] for two columns of tiles: part by part over all of them, so that an
+// acc[i][n] += a[i] b[n] for NT columns of tiles: part by part over all of them, so that an
 // instruction does not wait for the one before it.
-template <int M, int NA, int NB>
-__device__ __forceinline__ void mma_grid(floatx4 (*acc)[2], const Parts<NA> (&a)[M], const Parts<NB> (&b)[2]) {
+template <int M, int NT, int NA, int NB>
+__device__ __forceinline__ void mma_grid(floatx4 (*acc)[NT], const Parts<NA> (&a)[M], const Parts<NB> (&b)[NT]) {
 #pragma unroll
   for (int o = 2; o >= 0; --o)
 #pragma unroll
@@ -92,7 +92,7 @@ __device__ __forceinline__ void mma_grid(floatx4 (*acc)[2], const Parts<NA> (&a)
 #pragma unroll
           for (int t = 0; t < M; ++t)
 #pragma unroll
-            for (int n = 0; n < 2; ++n) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t].p[i], b[n].p[j], acc[t][n], 0, 0, 0);
+            for (int n = 0; n < NT; ++n) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t].p[i], b[n].p[j], acc[t][n], 0, 0, 0);
 }
 
 template <typename T> struct DeltaType;
@@ -163,7 +163,7 @@ struct DeltaArgs {
   float* sums;                // [slots][Hv][2][C]: G (upper and lower part); the backward pass only
   char *kr, *qr;              // [slots][Hk]: K, Q (fp32 inputs; bf16 rows are read from where they are)
   // The scan cut into segments of seg chunks (0: sequences in one piece), [segments][Hv][128][128] each
-  int seg, segs;
+  int seg, units;             // units: heads of all sequences, or of all segments
   float* move;                // a segment's product of transitions
   float* add;                 // its state from a start of 0 (the first: from state_in)
   float* init;                // the state before it (backward: the gradient behind it)
@@ -311,8 +311,9 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
   using K = Pack<T, kBwd>;
   constexpr int C = K::C, NP = K::NP, MT = C / 16, LD = C + 4;
   constexpr int kStage = K::kRows * kUnit, kX = C * LD * 4 > kStage ? C * LD * 4 : kStage;
-  __shared__ __align__(16) float am[C][LD], pm[C][LD];
+  __shared__ __align__(16) float am[C][LD];                  // P, then A
   __shared__ __align__(16) char xbuf[kX];                    // K's rows, then the inverse
+  __shared__ __align__(16) float ybuf[C == 32 ? 16 * LD : 1];
   __shared__ float gh[C], gl[C], bt[C];
   float (*xm)[LD] = reinterpret_cast<float (*)[LD]>(xbuf);
   bf16x8* sk = reinterpret_cast<bf16x8*>(xbuf);
@@ -373,16 +374,18 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
   }
   __syncthreads();
 
-  // row tile mt of K K^T (into am) and of Q K^T (into pm)
+  // row tile mt of Q K^T (into am, packed as P) and of K K^T (into am behind it)
+  floatx4 kk[MT];
 #pragma unroll
   for (int nt = 0; nt < MT; ++nt) {
     const int j = tile_row(nt, m);
-    floatx4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
+    floatx4 qk = {0.f, 0.f, 0.f, 0.f};
+    kk[nt] = qk;
     if ((nt >> 1) <= (mt >> 1)) {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         const Parts<NP> kj = staged<NP>(sk, nt * 4 + ks, rs);
-        if (C == 64 || wave < MT) mma(kk, staged<NP>(sk, mt * 4 + ks, rs), kj);
+        if (C == 64 || wave < MT) mma(kk[nt], staged<NP>(sk, mt * 4 + ks, rs), kj);
         if (C == 64 || wave >= MT) mma(qk, xq[ks], kj);
       }
     }
@@ -390,13 +393,19 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
     for (int r = 0; r < 4; ++r) {
       const int i = tile_row(mt, 4 * g4 + r);
       const float d = j <= i ? expf((gh[i] - gh[j]) + (gl[i] - gl[j])) : 0.f;
-      if (C == 64 || wave < MT) am[i][j] = j < i ? bt[i] * kk[r] * d : 0.f;
-      if (C == 64 || wave >= MT) pm[i][j] = j <= i ? a.scale * qk[r] * d : 0.f;
+      if (C == 64 || wave >= MT) am[i][j] = a.scale * qk[r] * d;
+      kk[nt][r] = j < i ? bt[i] * kk[nt][r] * d : 0.f;
     }
   }
   __syncthreads();
-  pack_square<C, K::kPParts, kBwd>(a.pm + at * K::kP * kUnit, &pm[0][0], LD, tid);
+  pack_square<C, K::kPParts, kBwd>(a.pm + at * K::kP * kUnit, &am[0][0], LD, tid);
   for (int i = tid; i < C * LD; i += 256) (&xm[0][0])[i] = 0.f;
+  __syncthreads();
+  if (C == 64 || wave < MT)
+#pragma unroll
+    for (int nt = 0; nt < MT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) am[tile_row(mt, 4 * g4 + r)][tile_row(nt, m)] = kk[nt][r];
   __syncthreads();
 
   // (I + A)^-1: blocks of 16 by substitution, a lane a column; then pairs of blocks, and of pairs:
@@ -414,34 +423,52 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) xm[16 * wave + i][16 * wave + l] = x[i];
   }
-  float (*ym)[LD] = pm;
+  // products on the way: in the upper right of the inverse, which no operand takes (C = 32: beside it)
+  float* ym = C == 32 ? ybuf : &xm[0][32];
   __syncthreads();
   if (wave < C / 32) {
     const int p = 32 * wave;
-    tile_put(&ym[p][p], LD, tile_f32(&am[p + 16][p], LD, &xm[p][p], LD, 16), 1.f);
+    tile_put(ym + 16 * wave * LD, LD, tile_f32(&am[p + 16][p], LD, &xm[p][p], LD, 16), 1.f);
   }
   __syncthreads();
   if (wave < C / 32) {
     const int p = 32 * wave;
-    tile_put(&xm[p + 16][p], LD, tile_f32(&xm[p + 16][p + 16], LD, &ym[p][p], LD, 16), -1.f);
+    tile_put(&xm[p + 16][p], LD, tile_f32(&xm[p + 16][p + 16], LD, ym + 16 * wave * LD, LD, 16), -1.f);
   }
   __syncthreads();
   if constexpr (C == 64) {
     const int i = 16 * (wave >> 1), j = 16 * (wave & 1);
-    tile_put(&ym[i][j], LD, tile_f32(&am[32 + i][0], LD, &xm[0][j], LD, 32), 1.f);
+    tile_put(ym + i * LD + j, LD, tile_f32(&am[32 + i][0], LD, &xm[0][j], LD, 32), 1.f);
     __syncthreads();
-    tile_put(&xm[32 + i][j], LD, tile_f32(&xm[32 + i][32], LD, &ym[0][j], LD, 32), -1.f);
+    tile_put(&xm[32 + i][j], LD, tile_f32(&xm[32 + i][32], LD, ym + j, LD, 32), -1.f);
     __syncthreads();
   }
   pack_square<C, 3, kBwd>(a.tm + at * K::kT * kUnit, &xm[0][0], LD, tid);
 }
 
 // ---------------------------------------------------------------------------
-// The state from chunk to chunk.  256 threads: a wave owns 32 columns of one head's state in two
-// tiles of 16, tile 2 ks + e of its registers the rows tile_row(2 ks + e, .).  The chunk's
-// operands come to LDS by direct loads, each buffer refilled as soon as all four waves are
-// through with it; two blocks share a CU and cover each other's waits.
+// The state from chunk to chunk.  A wave owns 16 NT columns of one head's state in NT tiles of 16,
+// tile 2 ks + e of its registers the rows tile_row(2 ks + e, .); a block has W waves.  The chunk's
+// operands come to LDS by direct loads.  Three shapes (Shape), by how many heads and sequences
+// there are to fill the chip:
+//   <2, 4, one buffer>: a head a block; two blocks share a CU and cover each other's waits, each
+//     buffer is refilled as soon as all waves are through with it
+//   <1, 4> and <1, 2>, two buffers: 64 and 32 columns a block, one block a CU; the next
+//     chunk's operands are on their way during the whole of this one's products
 // ---------------------------------------------------------------------------
+// Blocks go to the 8 XCDs in turn, each with an L2 of its own: the kBlocks blocks of one head stand 8
+// apart, so that they share one.  The unit (head and sequence or segment) and block of a block
+// index; the grid has blocks_for(units) of them, some without a unit.
+template <int kBlocks> __device__ __forceinline__ int2 unit_of(int b) {
+  return kBlocks == 1 ? int2{b, 0} : int2{b / (8 * kBlocks) * 8 + b % 8, b / 8 % kBlocks};
+}
+constexpr int64_t blocks_for(int64_t units, int blocks) { return blocks == 1 ? units : (units + 7) / 8 * 8 * blocks; }
+
+template <int NT_, int W_, bool kDouble_> struct Shape {
+  static constexpr int NT = NT_, W = W_, kCols = 16 * NT_ * W_, kBlocks = kHead / kCols;     // columns of a block, blocks of a head
+  static constexpr bool kDouble = kDouble_;
+};
+
 template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
   const uint64_t x = reinterpret_cast<uint64_t>(p);
   const uint64_t y = (uint64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
@@ -449,85 +476,83 @@ template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// `units` KiB from src (16-byte aligned) to LDS, by four waves.
-__device__ __forceinline__ void fetch(const void* src, uint32_t lds, int units, int wave, int l) {
+// `units` KiB from src (16-byte aligned) to LDS, by W waves.
+template <int W> __device__ __forceinline__ void fetch(const void* src, uint32_t lds, int units, int wave, int l) {
   const char* p = uniform(static_cast<const char*>(src));
-  for (int i = wave; i < units; i += 4) load_lds16(p + (size_t)i * kUnit, 16u * l, lds + i * kUnit);
+  for (int i = wave; i < units; i += W) load_lds16(p + (size_t)i * kUnit, 16u * l, __builtin_amdgcn_readfirstlane(lds + i * kUnit));
 }
 // The rows of a chunk (tile_row, summed over the 128 elements) straight from bf16 rows; rows behind
 // the sequence are its last one again (what they give is not used).
-template <int C>
+template <int C, int W>
 __device__ __forceinline__ void fetch_rows(const Rows& x, const Span& sp, int64_t t0, int left, int h, uint32_t lds, int wave, int l) {
   const uint16_t* p = uniform(row_at<uint16_t>(x, sp, t0, h));
+  const int m = (l - 4 * (l >> 4)) & 15;                     // (row_slot)
 #pragma unroll
-  for (int mt = 0; mt < C / 16; ++mt) {
-    const int t = min(tile_row(mt, (l - 4 * (l >> 4)) & 15), left - 1);      // (row_slot)
-    load_lds16(p, (uint32_t)(t * (int)x.st + 32 * wave + 8 * (l >> 4)) * 2u, lds + (mt * 4 + wave) * kUnit);
+  for (int f = wave; f < C / 4; f += W) {
+    const int t = min(tile_row(f >> 2, m), left - 1);
+    load_lds16(p, (uint32_t)(t * (int)x.st + 32 * (f & 3) + 8 * (l >> 4)) * 2u, __builtin_amdgcn_readfirstlane(lds + f * kUnit));
   }
 }
 
-// A wave's own [C][32 columns] of a [tokens][128] matrix in LDS, 4 KiB in pieces of 16 bytes;
-// the piece's place turns with the token, so that a column's four groups of tokens meet
-// other banks.
-template <typename T> struct Slice {
-  static constexpr int C = DeltaType<T>::kChunk, kPieces = 2 * sizeof(T), kRow = 32 * sizeof(T);   // 4 or 8 pieces a row
-  __device__ static int turn(int t) { return sizeof(T) == 2 ? (t >> 3) & 3 : ((t >> 3) & 1) << 2; }
-  // byte offset of token 8 g, column 16 n + m; token 8 g + k lies k rows behind it (k % 32 < 8)
-  __device__ static int lane(int g, int n, int m) {
-    constexpr int kPer = 16 / sizeof(T);
-    const int col = 16 * n + m;
-    return 8 * g * kRow + (((col / kPer) ^ turn(8 * g)) << 4) + (col % kPer) * (int)sizeof(T);
-  }
-  __device__ static void fetch(const Rows& x, const Span& sp, int64_t t0, int left, int h, int wave, uint32_t lds, int l) {
-    const T* p = uniform(row_at<T>(x, sp, t0, h) + 32 * wave);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int u = 64 * i + l, t = u / kPieces, tt = min(t, left - 1);
-      load_lds16(p, (uint32_t)(tt * (int)x.st) * (uint32_t)sizeof(T) + (((u % kPieces) ^ turn(t)) << 4), lds + i * kUnit);
+// A wave's own [C][16 NT] of a [tokens][128] matrix in LDS: token 8 a + b in row b C / 8 + a, so that a
+// column's four groups of tokens lie side by side.
+template <typename T, int NT> struct Slice {
+  static constexpr int C = DeltaType<T>::kChunk, kRow = 16 * NT * sizeof(T), kPieces = kRow / 16, kBytes = C * kRow;
+  __device__ static int token(int row) { return row % (C / 8) * 8 + row / (C / 8); }
+  // bytes from the lane's place (token 8 g, column m) to token 8 g + tile_at(t, r), column 16 n + m
+  static constexpr int at(int t, int r, int n) { return ((4 * (t & 1) + r) * (C / 8) + 4 * (t >> 1)) * kRow + 16 * n * (int)sizeof(T); }
+  __device__ static int lane(int g, int m) { return g * kRow + m * (int)sizeof(T); }
+  // p: the wave's columns of the chunk's first row (uniform), `stride` elements between rows
+  __device__ static void fetch(const T* p, int64_t stride, int left, uint32_t lds, int l) {
+  #pragma unroll
+    for (int i = 0; i < kBytes / kUnit; ++i) {
+      const int u = 64 * i + l, t = min(token(u / kPieces), left - 1);
+      load_lds16(p, (uint32_t)(t * (int)stride) * (uint32_t)sizeof(T) + 16 * (u % kPieces), __builtin_amdgcn_readfirstlane(lds + i * kUnit));
     }
   }
-  // out: the wave's columns of the chunk's first row, `stride` elements between rows
   __device__ static void store(const char* lds, T* out, int64_t stride, int left, int l) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int u = 64 * i + l, t = u / kPieces;
+    for (int i = 0; i < kBytes / kUnit; ++i) {
+      const int u = 64 * i + l, t = token(u / kPieces);
       const u32x4 x = *reinterpret_cast<const u32x4*>(lds + 16 * u);
-      if (t < left) *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(out + t * stride) + (((u % kPieces) ^ turn(t)) << 4)) = x;
+      if (t < left) *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(out + t * stride) + 16 * (u % kPieces)) = x;
     }
   }
 };
 
-template <typename T> struct ScanLds {
+template <typename T, typename Sh> struct ScanLds {
   using F = Pack<T, false>;
   using B = Pack<T, true>;
-  // forward: K | Tm | gates | V, then O | Q | P
-  static constexpr size_t kFwdState = (size_t)(F::kRows + F::kT + 1 + 16) * kUnit;
-  static constexpr size_t kFwd = kFwdState + (size_t)(F::kRows + F::kP) * kUnit;
-  // backward: K | Q | Tm^T | P^T | gates
-  static constexpr size_t kBwd = (size_t)(2 * B::kRows + B::kT + B::kP + 1) * kUnit;
+  static constexpr int kSlices = Slice<T, Sh::NT>::kBytes * Sh::W;
+  // forward: K | Tm | gates | V, then O | Q | P (a pass for the state alone: without the last two)
+  static constexpr int kState = (F::kRows + F::kT + 1) * kUnit + kSlices, kOne = kState + (F::kRows + F::kP) * kUnit;
+  // backward: K | Q | Tm^T, then dv where it fits | P^T | gates | dv
+  static constexpr bool kDvInT = kSlices <= B::kT * kUnit;
+  static constexpr int kOneBwd = (2 * B::kRows + B::kT + B::kP + 1) * kUnit + (kDvInT ? 0 : kSlices);
+  static constexpr size_t kFwd = (size_t)kOne * (Sh::kDouble ? 2 : 1), kBwd = (size_t)kOneBwd * (Sh::kDouble ? 2 : 1);
 };
 
-// A [rows][128] fp32 matrix <-> the wave's tiles of it (rows tile_row, two tiles of 16 columns).  The
+// A [rows][128] fp32 matrix <-> the wave's tiles of it (rows tile_row, columns from col0).  The
 // row is a uniform address, the lane's part the same for all of them.
-template <int kTiles>
-__device__ __forceinline__ void tiles_load(floatx4 (&S)[kTiles][2], const float* p, int wave, int l) {
-  const float* q = uniform(p) + 32 * wave;
+template <int kTiles, int NT>
+__device__ __forceinline__ void tiles_load(floatx4 (&S)[kTiles][NT], const float* p, int col0, int l) {
+  const float* q = uniform(p) + col0;
   const uint32_t off = 8 * (l >> 4) * kHead + (l & 15);
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[t][n][r] = (q + tile_at(t, r) * kHead + 16 * n)[off];
 }
-template <int kTiles>
-__device__ __forceinline__ void tiles_store(const floatx4 (&S)[kTiles][2], float* p, int wave, int l) {
-  float* q = const_cast<float*>(uniform(p)) + 32 * wave;
+template <int kTiles, int NT>
+__device__ __forceinline__ void tiles_store(const floatx4 (&S)[kTiles][NT], float* p, int col0, int l) {
+  float* q = const_cast<float*>(uniform(p)) + col0;
   const uint32_t off = 8 * (l >> 4) * kHead + (l & 15);
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) (q + tile_at(t, r) * kHead + 16 * n)[off] = S[t][n][r];
 }
@@ -535,19 +560,28 @@ __device__ __forceinline__ void tiles_store(const floatx4 (&S)[kTiles][2], float
 // kOut: the outputs (and what the backward pass needs).  Otherwise only what a segment does to
 // the state: blockIdx.y 0 what it adds, 1 its product of transitions (V = 0 from the
 // identity).
-template <typename T, bool kOut>
-__global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
+template <typename T, bool kOut, typename Sh>
+__global__ __launch_bounds__(64 * Sh::W, 2) void delta_scan_kernel(DeltaArgs a) {
   using K = Pack<T, false>;
-  constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32;
+  using L = ScanLds<T, Sh>;
+  constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32, NT = Sh::NT, W = Sh::W;
+  using V = Slice<T, NT>;
   extern __shared__ __align__(16) char lds[];
-  char* bk = lds;
-  char* bt = bk + K::kRows * kUnit;
-  char* bg = bt + K::kT * kUnit;
-  char* bv = bg + kUnit;
-  char* bq = bv + 16 * kUnit;
-  char* bp = bq + K::kRows * kUnit;
-  const int piece_slot = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, hk = h / (a.Hv / a.Hk), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
-  bv += wave * 4 * kUnit;
+  int bk, bt, bg, bv, bq, bp;                                // this chunk's, bytes from lds
+  const uint32_t base = lds_addr(lds);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
+  auto buffers = [&](int which) {
+    bk = Sh::kDouble ? which * L::kOne : 0;
+    bt = bk + K::kRows * kUnit;
+    bg = bt + K::kT * kUnit;
+    bv = bg + kUnit + wave * V::kBytes;
+    bq = bg + kUnit + L::kSlices;
+    bp = bq + K::kRows * kUnit;
+  };
+  buffers(0);
+  const int2 unit = unit_of<Sh::kBlocks>(blockIdx.x);
+  const int piece_slot = unit.x / a.Hv, h = unit.x % a.Hv, hk = h / (a.Hv / a.Hk), col0 = unit.y * Sh::kCols + 16 * NT * wave;
+  if (unit.x >= a.units) return;
   int piece = 0, c0 = 0, c1;
   Span sp;
   if (a.seg) {
@@ -565,44 +599,45 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
   const int slot0 = a.s.cu ? span_of(a.s, sp.n, C).slot0 : sp.n * chunks;
   const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)piece_slot * a.Hv + h) * kHead * kHead;
 
-  floatx4 S[8][2];
+  floatx4 S[8][NT];
   const float* from = piece == 0 ? (a.state_in ? a.state_in + sn : nullptr) : kOut ? a.init + gn : nullptr;
   if (from) {
-    tiles_load(S, from, wave, l);
+    tiles_load(S, from, col0, l);
   } else {
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          S[t][n][r] = ident && tile_row(t, 4 * g + r) == 32 * wave + 16 * n + (l & 15) ? 1.f : 0.f;
+          S[t][n][r] = ident && tile_row(t, 4 * g + r) == col0 + 16 * n + (l & 15) ? 1.f : 0.f;
   }
 
   auto fetch_k = [&](int64_t t0, int left, int64_t atk) {
-    if constexpr (NP == 1) fetch_rows<C>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
-    else fetch(a.kr + atk * K::kRows * kUnit, lds_addr(bk), K::kRows, wave, l);
+    if constexpr (NP == 1) fetch_rows<C, W>(a.k, sp, t0, left, hk, base + bk, wave, l);
+    else fetch<W>(a.kr + atk * K::kRows * kUnit, base + bk, K::kRows, wave, l);
   };
   auto fetch_q = [&](int64_t t0, int left, int64_t atk) {
-    if constexpr (NP == 1) fetch_rows<C>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
-    else fetch(a.qr + atk * K::kRows * kUnit, lds_addr(bq), K::kRows, wave, l);
+    if constexpr (NP == 1) fetch_rows<C, W>(a.q, sp, t0, left, hk, base + bq, wave, l);
+    else fetch<W>(a.qr + atk * K::kRows * kUnit, base + bq, K::kRows, wave, l);
   };
   constexpr int kSome = NP == 1 ? 4 : 2;
   const int rs = row_slot(g, l & 15), place = cols_place(l);
-  const int slice[2] = {Slice<T>::lane(g, 0, l & 15), Slice<T>::lane(g, 1, l & 15)};
+  const int slice = V::lane(g, l & 15);
   auto fetch_v = [&](int64_t t0, int left) {
-    if (!ident) Slice<T>::fetch(a.v, sp, t0, left, h, wave, lds_addr(bv), l);
+    if (!ident) V::fetch(uniform(row_at<T>(a.v, sp, t0, h) + col0), a.v.st, left, base + bv, l);
   };
-  if (c0 < c1) {
-    const int64_t t0 = (int64_t)c0 * C, at = (int64_t)(slot0 + c0) * a.Hv + h, atk = (int64_t)(slot0 + c0) * a.Hk + hk;
+  auto fetch_all = [&](int c) {
+    const int64_t t0 = (int64_t)c * C, at = (int64_t)(slot0 + c) * a.Hv + h, atk = (int64_t)(slot0 + c) * a.Hk + hk;
     const int left = sp.len - (int)t0;
-    if (kOut) fetch_q(t0, left, atk);
-    fetch(a.tm + at * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
-    fetch_v(t0, left);
     fetch_k(t0, left, atk);
-    if (kOut) fetch(a.pm + at * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
-    fetch(a.gates + at * (kUnit / 4), lds_addr(bg), 1, wave, l);
-  }
+    fetch_v(t0, left);
+    fetch<W>(a.gates + at * (kUnit / 4), base + bg, 1, wave, l);
+    if (kOut) fetch_q(t0, left, atk);
+    fetch<W>(a.tm + at * K::kT * kUnit, base + bt, K::kT, wave, l);
+    if (kOut) fetch<W>(a.pm + at * K::kP * kUnit, base + bp, K::kP, wave, l);
+  };
+  if (c0 < c1) fetch_all(c0);
   for (int c = c0; c < c1; ++c) {
     const int64_t t0 = (int64_t)c * C, at = (int64_t)(slot0 + c) * a.Hv + h, atk = (int64_t)(slot0 + c) * a.Hk + hk;
     const int left = sp.len - (int)t0;
@@ -611,40 +646,54 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
     const int left1 = left - C;
     wait_loads();
     __syncthreads();
-    if (kOut && a.s0) tiles_store(S, a.s0 + at * kHead * kHead, wave, l);
+    if constexpr (Sh::kDouble) {
+      if (more) {
+        buffers((c - c0 + 1) & 1);
+        fetch_all(c + 1);
+      }
+      buffers((c - c0) & 1);
+    }
+    if (kOut && a.s0) tiles_store(S, a.s0 + at * kHead * kHead, col0, l);
 
-    const bf16x8* st = reinterpret_cast<const bf16x8*>(bt);
-    const bf16x8* spm = reinterpret_cast<const bf16x8*>(bp);
-    const float* gates = reinterpret_cast<const float*>(bg);
-    floatx4 X[MT][2], O[MT][2];
+    const bf16x8* st = reinterpret_cast<const bf16x8*>(lds + bt);
+    const bf16x8* spm = reinterpret_cast<const bf16x8*>(lds + bp);
+    const float* gates = reinterpret_cast<const float*>(lds + bg);
+    floatx4 X[MT][NT], O[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int n = 0; n < 2; ++n) X[mt][n] = O[mt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NT; ++n) X[mt][n] = O[mt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+    Parts<3> s[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n] = split_pair(S[0][n], S[1][n]);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      Parts<3> s[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) s[n] = split_pair(S[2 * ks][n], S[2 * ks + 1][n]);
       Parts<NP> k[MT];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) k[mt] = rows_of<NP>(bk, mt, ks, rs);
+      for (int mt = 0; mt < MT; ++mt) k[mt] = rows_of<NP>(lds + bk, mt, ks, rs);
+      Parts<3> next[NT];
+      if (ks < 3)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) next[n] = split_pair(S[2 * ks + 2][n], S[2 * ks + 3][n]);
       mma_grid(X, k, s);
       if constexpr (kOut) {
         // for a bf16 output two parts of the state do (2^-17 of it)
         constexpr int kS = NP == 1 ? 2 : 3;
-        Parts<kS> x[2];
+        Parts<kS> x[NT];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < kS; ++i) x[n].p[i] = s[n].p[i];
+        Parts<NP> q[MT];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) k[mt] = rows_of<NP>(bq, mt, ks, rs);
-        mma_grid(O, k, x);
+        for (int mt = 0; mt < MT; ++mt) q[mt] = rows_of<NP>(lds + bq, mt, ks, rs);
+        mma_grid(O, q, x);
       }
       __builtin_amdgcn_sched_barrier(0);                     // (later steps' operands are not read ahead into registers)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n] = next[n];
     }
-    if (kOut && more) {
+    if (kOut && more && !Sh::kDouble) {
       __syncthreads();                                       // Q is free
       fetch_q(t1, left1, atk + a.Hk);
     }
@@ -653,36 +702,38 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
       const floatx4 e = *reinterpret_cast<const floatx4*>(gates + 8 * g + tile_at(mt, 0));
       const floatx4 b = *reinterpret_cast<const floatx4*>(gates + 2 * C + 8 * g + tile_at(mt, 0));
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float v = ident ? 0.f : to_f32(*reinterpret_cast<const T*>(bv + slice[n] + tile_at(mt, r) * Slice<T>::kRow));
+          const float v = ident ? 0.f : to_f32(*reinterpret_cast<const T*>(lds + bv + slice + V::at(mt, r, n)));
           X[mt][n][r] = b[r] * (v - e[r] * X[mt][n][r]);     // R (behind the sequence beta is 0)
           if (kOut) O[mt][n][r] *= a.scale * e[r];
         }
     }
-    floatx4 U[MT][2];
+    floatx4 U[MT][NT];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) U[mt][0] = U[mt][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) U[mt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
-      Parts<3> r[2];
+      Parts<3> r[NT];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) r[n] = split_pair(X[2 * js][n], X[2 * js + 1][n]);
+      for (int n = 0; n < NT; ++n) r[n] = split_pair(X[2 * js][n], X[2 * js + 1][n]);
 #pragma unroll
       for (int mt = 2 * js; mt < MT; mt += 2) {
         const Parts<3> x[2] = {staged<3>(st, Square<C>::at(mt, js, false), l), staged<3>(st, Square<C>::at(mt + 1, js, false), l)};
         mma_grid(U + mt, x, r);
       }
     }
-    __syncthreads();                                         // Tm is free
-    if (more) fetch(a.tm + (at + a.Hv) * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
+    if (!Sh::kDouble) __syncthreads();                       // Tm is free
+    if (more && !Sh::kDouble) fetch<W>(a.tm + (at + a.Hv) * K::kT * kUnit, base + bt, K::kT, wave, l);
     if constexpr (kOut) {
 #pragma unroll
       for (int js = 0; js < JS; ++js) {
-        Parts<K::kPParts> u[2];
+        Parts<K::kPParts> u[NT];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < NT; ++n) {
           const Parts<3> p = split_pair(U[2 * js][n], U[2 * js + 1][n]);
 #pragma unroll
           for (int i = 0; i < K::kPParts; ++i) u[n].p[i] = p.p[i];
@@ -697,16 +748,16 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<T*>(bv + slice[n] + tile_at(mt, r) * Slice<T>::kRow) = from_f32<T>(O[mt][n][r]);
-      if (a.u) tiles_store(U, a.u + at * C * kHead, wave, l);
+            *reinterpret_cast<T*>(lds + bv + slice + V::at(mt, r, n)) = from_f32<T>(O[mt][n][r]);
+      if (a.u) tiles_store(U, a.u + at * C * kHead, col0, l);
       asm volatile("" ::: "memory");                         // (a wave's LDS accesses keep their order)
-      Slice<T>::store(bv, static_cast<T*>(a.o) + (((int64_t)sp.b * a.s.T + sp.t0 + t0) * a.Hv + h) * kHead + 32 * wave,
-                      (int64_t)a.Hv * kHead, left, l);
+      V::store(lds + bv, static_cast<T*>(a.o) + (((int64_t)sp.b * a.s.T + sp.t0 + t0) * a.Hv + h) * kHead + col0, (int64_t)a.Hv * kHead,
+               left, l);
     }
-    if (more) {
+    if (more && !Sh::kDouble) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the wave has read its slice
       fetch_v(t1, left1);
     }
@@ -714,16 +765,16 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[t][n][r] *= whole;
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
-      Parts<3> u[2];
+      Parts<3> u[NT];
       float d[8];
       load8(gates + C + 32 * js + 8 * g, d);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < NT; ++n) {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = U[2 * js + (e >> 2)][n][e & 3] * d[e];
@@ -733,34 +784,45 @@ __global__ __launch_bounds__(256, 2) void delta_scan_kernel(DeltaArgs a) {
       for (int t = 0; t < 8; t += kSome) {
         Parts<NP> k[kSome];
 #pragma unroll
-        for (int i = 0; i < kSome; ++i) k[i] = cols_of<NP>(bk, t + i, js, place);
+        for (int i = 0; i < kSome; ++i) k[i] = cols_of<NP>(lds + bk, t + i, js, place);
         mma_grid(S + t, k, u);
       }
     }
-    __syncthreads();                                         // all buffers but Q, Tm and V are free
-    if (more) {
+    if (!Sh::kDouble) __syncthreads();                       // all buffers but Q, Tm and V are free
+    if (more && !Sh::kDouble) {
       fetch_k(t1, left1, atk + a.Hk);
-      if (kOut) fetch(a.pm + (at + a.Hv) * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
-      fetch(a.gates + (at + a.Hv) * (kUnit / 4), lds_addr(bg), 1, wave, l);
+      if (kOut) fetch<W>(a.pm + (at + a.Hv) * K::kP * kUnit, base + bp, K::kP, wave, l);
+      fetch<W>(a.gates + (at + a.Hv) * (kUnit / 4), base + bg, 1, wave, l);
     }
   }
   if (kOut ? last && a.state_out != nullptr : true)
-    tiles_store(S, kOut ? a.state_out + sn : (ident ? a.move : a.add) + gn, wave, l);
+    tiles_store(S, kOut ? a.state_out + sn : (ident ? a.move : a.add) + gn, col0, l);
 }
 
 // kOut: dv, and the gradients of the states behind the chunks and of R that the last kernel reads.
 // Otherwise what a segment adds to the gradient of the state before it.
-template <typename T, bool kOut>
-__global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
+template <typename T, bool kOut, typename Sh>
+__global__ __launch_bounds__(64 * Sh::W, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
   using K = Pack<T, true>;
-  constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32;
+  using L = ScanLds<T, Sh>;
+  constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32, NT = Sh::NT, W = Sh::W;
   extern __shared__ __align__(16) char lds[];
-  char* bk = lds;
-  char* bq = bk + K::kRows * kUnit;
-  char* bt = bq + K::kRows * kUnit;
-  char* bp = bt + K::kT * kUnit;
-  char* bg = bp + K::kP * kUnit;
-  const int piece_slot = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, hk = h / (a.Hv / a.Hk), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
+  using V = Slice<T, NT>;
+  int bk, bq, bt, bp, bg, bv;                                // this chunk's, bytes from lds
+  const uint32_t base = lds_addr(lds);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4;
+  auto buffers = [&](int which) {
+    bk = Sh::kDouble ? which * L::kOneBwd : 0;
+    bq = bk + K::kRows * kUnit;
+    bt = bq + K::kRows * kUnit;
+    bp = bt + K::kT * kUnit;
+    bg = bp + K::kP * kUnit;
+    bv = (L::kDvInT ? bt : bg + kUnit) + wave * V::kBytes;
+  };
+  buffers(0);
+  const int2 unit = unit_of<Sh::kBlocks>(blockIdx.x);
+  const int piece_slot = unit.x / a.Hv, h = unit.x % a.Hv, hk = h / (a.Hv / a.Hk), col0 = unit.y * Sh::kCols + 16 * NT * wave;
+  if (unit.x >= a.units) return;
   int piece = 0, c0 = 0;
   Span sp;
   if (a.seg) {
@@ -777,44 +839,50 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
   const int slot0 = a.s.cu ? span_of(a.s, sp.n, C).slot0 : sp.n * chunks;
   const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)piece_slot * a.Hv + h) * kHead * kHead;
 
-  floatx4 S[8][2];                                           // dS
+  floatx4 S[8][NT];                                           // dS
   const float* from = last ? (a.dstate_out ? a.dstate_out + sn : nullptr) : kOut ? a.init + gn : nullptr;
   if (from) {
-    tiles_load(S, from, wave, l);
+    tiles_load(S, from, col0, l);
   } else {
 #pragma unroll
-    for (int t = 0; t < 8; ++t) S[t][0] = S[t][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) S[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  float d[MT][2][4];                                         // dO
+  T d[MT][NT][4];                                            // dO as it is (turned to fp32 where it is used)
   auto load_do = [&](int64_t t0, int left) {
-    const T* p = uniform(row_at<T>(a.dout, sp, t0, h) + 32 * wave);
+    const T* p = uniform(row_at<T>(a.dout, sp, t0, h) + col0);
     const uint32_t off = 8 * g * (uint32_t)a.dout.st + (l & 15);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          d[mt][n][r] = 8 * g + tile_at(mt, r) < left ? to_f32((p + tile_at(mt, r) * a.dout.st + 16 * n)[off]) : 0.f;
+          d[mt][n][r] = 8 * g + tile_at(mt, r) < left ? (p + tile_at(mt, r) * a.dout.st + 16 * n)[off] : T(0);
   };
   auto fetch_k = [&](int64_t t0, int left, int64_t atk) {
-    if constexpr (NP == 1) fetch_rows<C>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
-    else fetch(a.kr + atk * K::kRows * kUnit, lds_addr(bk), K::kRows, wave, l);
+    if constexpr (NP == 1) fetch_rows<C, W>(a.k, sp, t0, left, hk, base + bk, wave, l);
+    else fetch<W>(a.kr + atk * K::kRows * kUnit, base + bk, K::kRows, wave, l);
   };
   auto fetch_q = [&](int64_t t0, int left, int64_t atk) {
-    if constexpr (NP == 1) fetch_rows<C>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
-    else fetch(a.qr + atk * K::kRows * kUnit, lds_addr(bq), K::kRows, wave, l);
+    if constexpr (NP == 1) fetch_rows<C, W>(a.q, sp, t0, left, hk, base + bq, wave, l);
+    else fetch<W>(a.qr + atk * K::kRows * kUnit, base + bq, K::kRows, wave, l);
   };
   constexpr int kSome = NP == 1 ? 4 : 2;
-  const int rs = row_slot(g, l & 15), place = cols_place(l);
+  const int rs = row_slot(g, l & 15), place = cols_place(l), slice = V::lane(g, l & 15);
+  auto fetch_all = [&](int c) {
+    const int64_t t0 = (int64_t)c * C, at = (int64_t)(slot0 + c) * a.Hv + h, atk = (int64_t)(slot0 + c) * a.Hk + hk;
+    const int left = sp.len - (int)t0;
+    fetch_k(t0, left, atk);
+    fetch<W>(a.gates + at * (kUnit / 4), base + bg, 1, wave, l);
+    fetch<W>(a.pm + at * K::kP * kUnit, base + bp, K::kP, wave, l);
+    fetch<W>(a.tm + at * K::kT * kUnit, base + bt, K::kT, wave, l);
+    fetch_q(t0, left, atk);
+  };
   if (c0 < c1) {
-    const int64_t t0 = (int64_t)(c1 - 1) * C, at = (int64_t)(slot0 + c1 - 1) * a.Hv + h, atk = (int64_t)(slot0 + c1 - 1) * a.Hk + hk;
-    load_do(t0, sp.len - (int)t0);
-    fetch_k(t0, sp.len - (int)t0, atk);
-    fetch(a.gates + at * (kUnit / 4), lds_addr(bg), 1, wave, l);
-    fetch(a.pm + at * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
-    fetch(a.tm + at * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
-    fetch_q(t0, sp.len - (int)t0, atk);
+    load_do((int64_t)(c1 - 1) * C, sp.len - (c1 - 1) * C);
+    fetch_all(c1 - 1);
   }
   for (int c = c1 - 1; c >= c0; --c) {
     const int64_t t0 = (int64_t)c * C, at = (int64_t)(slot0 + c) * a.Hv + h, atk = (int64_t)(slot0 + c) * a.Hk + hk;
@@ -822,120 +890,142 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
     const bool more = c > c0;
     wait_loads();
     __syncthreads();
-    if (kOut) tiles_store(S, a.ds1 + at * kHead * kHead, wave, l);
+    if constexpr (Sh::kDouble) {
+      if (more) {
+        buffers((c1 - c) & 1);
+        fetch_all(c - 1);
+      }
+      buffers((c1 - 1 - c) & 1);
+    }
+    if (kOut) tiles_store(S, a.ds1 + at * kHead * kHead, col0, l);
 
-    const bf16x8* st = reinterpret_cast<const bf16x8*>(bt);
-    const bf16x8* spm = reinterpret_cast<const bf16x8*>(bp);
-    const float* gates = reinterpret_cast<const float*>(bg);
-    floatx4 X[MT][2], R[MT][2];
+    const bf16x8* st = reinterpret_cast<const bf16x8*>(lds + bt);
+    const bf16x8* spm = reinterpret_cast<const bf16x8*>(lds + bp);
+    const float* gates = reinterpret_cast<const float*>(lds + bg);
+    floatx4 X[MT][NT], R[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int n = 0; n < 2; ++n) X[mt][n] = R[mt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NT; ++n) X[mt][n] = R[mt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+    Parts<3> s[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n] = split_pair(S[0][n], S[1][n]);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      Parts<3> s[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) s[n] = split_pair(S[2 * ks][n], S[2 * ks + 1][n]);
       Parts<NP> k[MT];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) k[mt] = rows_of<NP>(bk, mt, ks, rs);
+      for (int mt = 0; mt < MT; ++mt) k[mt] = rows_of<NP>(lds + bk, mt, ks, rs);
+      Parts<3> next[NT];
+      if (ks < 3)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) next[n] = split_pair(S[2 * ks + 2][n], S[2 * ks + 3][n]);
       mma_grid(X, k, s);
       __builtin_amdgcn_sched_barrier(0);                     // (later steps' operands are not read ahead into registers)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n] = next[n];
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const floatx4 e = *reinterpret_cast<const floatx4*>(gates + C + 8 * g + tile_at(mt, 0));
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) X[mt][n][r] *= e[r];
     }
+    // dS <- e^G_C dS + Q^T (scale e^G dO), then dU <- dU + P^T dO: dO's registers are free behind it
+    const float whole = gates[C - 1];
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][n][r] *= whole;
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
-      Parts<NP> p[2];
+      Parts<NP> p[NT];
+      Parts<3> ps[NT];
+      float e[8];
+      load8(gates + 32 * js + 8 * g, e);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float x[8] = {d[2 * js][n][0], d[2 * js][n][1], d[2 * js][n][2], d[2 * js][n][3],
-                            d[2 * js + 1][n][0], d[2 * js + 1][n][1], d[2 * js + 1][n][2], d[2 * js + 1][n][3]};
+      for (int n = 0; n < NT; ++n) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(d[2 * js + (i >> 2)][n][i & 3]);
         p[n] = parts_of<NP>(x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= a.scale * e[i];
+        ps[n] = split3(x);
       }
 #pragma unroll
       for (int mt = 0; mt < 2 * js + 2; mt += 2) {           // dU
         const Parts<3> x[2] = {staged<3>(spm, Square<C>::at(mt, js, true), l), staged<3>(spm, Square<C>::at(mt + 1, js, true), l)};
         mma_grid(X + mt, x, p);
       }
+#pragma unroll
+      for (int t = 0; t < 8; t += kSome) {
+        Parts<NP> x[kSome];
+#pragma unroll
+        for (int i = 0; i < kSome; ++i) x[i] = cols_of<NP>(lds + bq, t + i, js, place);
+        mma_grid(S + t, x, ps);
+      }
+    }
+    load_do(more ? t0 - C : t0, more ? left + C : left);     // (no condition: it would be waited for here)
+    if (!Sh::kDouble) __syncthreads();                       // Q and P^T are free
+    if (more && !Sh::kDouble) {
+      fetch<W>(a.pm + (at - a.Hv) * K::kP * kUnit, base + bp, K::kP, wave, l);
+      fetch_q(t0 - C, left + C, atk - a.Hk);
     }
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
-      Parts<3> p[2];
+      Parts<3> p[NT];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) p[n] = split_pair(X[2 * js][n], X[2 * js + 1][n]);
+      for (int n = 0; n < NT; ++n) p[n] = split_pair(X[2 * js][n], X[2 * js + 1][n]);
 #pragma unroll
       for (int mt = 0; mt < 2 * js + 2; mt += 2) {           // dR
         const Parts<3> x[2] = {staged<3>(st, Square<C>::at(mt, js, true), l), staged<3>(st, Square<C>::at(mt + 1, js, true), l)};
         mma_grid(R + mt, x, p);
       }
     }
-    __syncthreads();                                         // Tm^T and P^T are free
-    if (more) {
-      fetch(a.pm + (at - a.Hv) * K::kP * kUnit, lds_addr(bp), K::kP, wave, l);
-      fetch(a.tm + (at - a.Hv) * K::kT * kUnit, lds_addr(bt), K::kT, wave, l);
-    }
-    const float whole = gates[C - 1];
-#pragma unroll
-    for (int t = 0; t < 8; ++t)
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[t][n][r] *= whole;
-    T* dv = kOut ? const_cast<T*>(uniform(static_cast<const T*>(a.dv) + (((int64_t)sp.b * a.s.T + sp.t0 + t0) * a.Hv + h) * kHead + 32 * wave)) : nullptr;
-    const uint32_t off = 8 * g * (uint32_t)(a.Hv * kHead) + (l & 15);
-    if (kOut) tiles_store(R, a.dr + at * C * kHead, wave, l);
+    __syncthreads();                                         // Tm^T is read by all: dv goes through its place
+    if (kOut) tiles_store(R, a.dr + at * C * kHead, col0, l);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const floatx4 e = *reinterpret_cast<const floatx4*>(gates + 8 * g + tile_at(mt, 0));
       const floatx4 b = *reinterpret_cast<const floatx4*>(gates + 2 * C + 8 * g + tile_at(mt, 0));
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if (kOut && 8 * g + tile_at(mt, r) < left)
-            (dv + tile_at(mt, r) * (int64_t)a.Hv * kHead + 16 * n)[off] = from_f32<T>(b[r] * R[mt][n][r]);
+          if (kOut) *reinterpret_cast<T*>(lds + bv + slice + V::at(mt, r, n)) = from_f32<T>(b[r] * R[mt][n][r]);
           R[mt][n][r] *= -b[r] * e[r];
-          d[mt][n][r] *= a.scale * e[r];
         }
+    }
+    if constexpr (kOut) {
+      asm volatile("" ::: "memory");                         // (a wave's LDS accesses keep their order)
+      V::store(lds + bv, static_cast<T*>(a.dv) + (((int64_t)sp.b * a.s.T + sp.t0 + t0) * a.Hv + h) * kHead + col0, (int64_t)a.Hv * kHead,
+               left, l);
     }
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
-      Parts<3> p[2], q[2];
+      Parts<3> q[NT];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float x[8] = {d[2 * js][n][0], d[2 * js][n][1], d[2 * js][n][2], d[2 * js][n][3],
-                            d[2 * js + 1][n][0], d[2 * js + 1][n][1], d[2 * js + 1][n][2], d[2 * js + 1][n][3]};
-        p[n] = split3(x);
-        q[n] = split_pair(R[2 * js][n], R[2 * js + 1][n]);
-      }
+      for (int n = 0; n < NT; ++n) q[n] = split_pair(R[2 * js][n], R[2 * js + 1][n]);
 #pragma unroll
       for (int t = 0; t < 8; t += kSome) {
         Parts<NP> x[kSome];
 #pragma unroll
-        for (int i = 0; i < kSome; ++i) x[i] = cols_of<NP>(bq, t + i, js, place);
-        mma_grid(S + t, x, p);
-#pragma unroll
-        for (int i = 0; i < kSome; ++i) x[i] = cols_of<NP>(bk, t + i, js, place);
+        for (int i = 0; i < kSome; ++i) x[i] = cols_of<NP>(lds + bk, t + i, js, place);
         mma_grid(S + t, x, q);
       }
     }
-    if (more) load_do(t0 - C, left + C);
-    __syncthreads();                                         // all buffers but Tm^T and P^T are free
-    if (more) {
+    if (!Sh::kDouble) __syncthreads();                       // K, the gates and dv's place are free
+    if (more && !Sh::kDouble) {
+      fetch<W>(a.tm + (at - a.Hv) * K::kT * kUnit, base + bt, K::kT, wave, l);
       fetch_k(t0 - C, left + C, atk - a.Hk);
-      fetch_q(t0 - C, left + C, atk - a.Hk);
-      fetch(a.gates + (at - a.Hv) * (kUnit / 4), lds_addr(bg), 1, wave, l);
+      fetch<W>(a.gates + (at - a.Hv) * (kUnit / 4), base + bg, 1, wave, l);
     }
   }
-  if (kOut ? piece == 0 && a.dstate_in != nullptr : true) tiles_store(S, kOut ? a.dstate_in + sn : a.add + gn, wave, l);
+  if (kOut ? piece == 0 && a.dstate_in != nullptr : true) tiles_store(S, kOut ? a.dstate_in + sn : a.add + gn, col0, l);
 }
 
 // The states before the segments (kBwd: the gradients behind them) from what each adds and its
@@ -944,9 +1034,12 @@ __global__ __launch_bounds__(256, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
 // through LDS.
 template <bool kBwd>
 __global__ __launch_bounds__(512) void delta_join_kernel(DeltaArgs a, int chunk) {
+  constexpr int kAhead = 3;                                  // segments whose loads are on their way
   __shared__ __align__(16) bf16x8 buf[2][4 * 3 * 64];
-  const int h = blockIdx.y, wave = threadIdx.x >> 6, l = lane_id(), g = l >> 4, m = l & 15, col = 16 * blockIdx.x + m;
-  const Span sp = span_of(a.s, blockIdx.z, chunk * a.seg);
+  const int2 unit = unit_of<8>(blockIdx.x);                  // a head of a sequence, 16 columns
+  if (unit.x >= a.s.N * a.Hv) return;
+  const int h = unit.x % a.Hv, wave = threadIdx.x >> 6, l = lane_id(), g = l >> 4, m = l & 15, col = 16 * unit.y + m;
+  const Span sp = span_of(a.s, unit.x / a.Hv, chunk * a.seg);
   const int pieces = (sp.len + chunk * a.seg - 1) / (chunk * a.seg);
   if (pieces == 0) {                                         // no token: no segment to hand the state on
     const float* from = kBwd ? a.dstate_out : a.state_in;
@@ -966,42 +1059,66 @@ __global__ __launch_bounds__(512) void delta_join_kernel(DeltaArgs a, int chunk)
     for (int r = 0; r < 4; ++r) y[r] = x[tile_row(wave, 4 * g + r) * kHead + col];
     return y;
   };
-  float mv[4][8];
-  auto load_move = [&](int p) {                              // rows tile_row(wave, m) of move, or of its transpose
-    const float* x = a.move + at(p);
+  const int first = kBwd ? pieces - 1 : 0, step = kBwd ? -1 : 1;
+  float mv[kAhead][4][8];                                    // rows tile_row(wave, m) of move, or of its transpose
+  floatx4 ad[kAhead];
+  // Loads run kAhead segments ahead, each array's into its own registers and under no condition: what
+  // is copied, or merged behind a branch, is waited for there.  Of the i-th segment (behind the last
+  // one that is asked for that one again):
+  auto where = [&](int i) { return at(first + max(min(i, pieces - 2), 1) * step); };
+  auto load_move = [&](int i, float (&to)[4][8]) {
+    const float* x = a.move + where(i);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       if constexpr (kBwd) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mv[ks][e] = x[(32 * ks + 8 * g + e) * kHead + tile_row(wave, m)];
+        for (int e = 0; e < 8; ++e) to[ks][e] = x[(32 * ks + 8 * g + e) * kHead + tile_row(wave, m)];
       } else {
-        load8(x + tile_row(wave, m) * kHead + 32 * ks + 8 * g, mv[ks]);
+        load8(x + tile_row(wave, m) * kHead + 32 * ks + 8 * g, to[ks]);
       }
     }
   };
-  const int first = kBwd ? pieces - 1 : 0, step = kBwd ? -1 : 1;
   floatx4 S = tile(a.add + at(first));                       // the first one's start is in it
-  if (pieces > 2) load_move(first + step);
-  for (int i = 1, p = first + step; i < pieces; ++i, p += step) {
-    float* init = a.init + at(p);
+  asm volatile("" : "+v"(S));                                // (arrived, before the loop knows of it)
+  auto keep = [&](int i) {
+    float* init = a.init + at(first + i * step);
 #pragma unroll
     for (int r = 0; r < 4; ++r) init[tile_row(wave, 4 * g + r) * kHead + col] = S[r];
-    if (i + 1 == pieces) break;
-    const float x[8] = {S[0], S[1], S[2], S[3], 0.f, 0.f, 0.f, 0.f};
-    const Parts<3> s = split3(x);
+  };
+  keep(1);
+  if (pieces == 2) return;
 #pragma unroll
-    for (int n = 0; n < 3; ++n) {
-      const u32x4 w = __builtin_bit_cast(u32x4, s.p[n]);
-      *reinterpret_cast<uint2*>(reinterpret_cast<char*>(&buf[i & 1][((wave >> 1) * 3 + n) * 64 + l]) + 8 * (wave & 1)) = uint2{w[0], w[1]};
+  for (int j = 0; j < kAhead; ++j) {
+    load_move(1 + j, mv[j]);
+    ad[j] = tile(a.add + where(1 + j));
+  }
+  for (int i0 = 1;; i0 += kAhead) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j;
+      const float x[8] = {S[0], S[1], S[2], S[3], 0.f, 0.f, 0.f, 0.f};
+      const Parts<3> s = split3(x);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) {
+        const u32x4 w = __builtin_bit_cast(u32x4, s.p[n]);
+        *reinterpret_cast<uint2*>(reinterpret_cast<char*>(&buf[i & 1][((wave >> 1) * 3 + n) * 64 + l]) + 8 * (wave & 1)) = uint2{w[0], w[1]};
+      }
+      Parts<3> k[4];
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) k[ks] = split3(mv[j][ks]);
+      load_move(i + kAhead, mv[j]);
+      __syncthreads();
+      floatx4 sum[4];
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        sum[ks] = floatx4{0.f, 0.f, 0.f, 0.f};
+        mma(sum[ks], k[ks], staged<3>(buf[i & 1], ks, l));
+      }
+      S = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ad[j];
+      ad[j] = tile(a.add + where(i + kAhead));
+      keep(i + 1);
+      if (i + 2 >= pieces) return;
     }
-    S = tile(a.add + at(p));
-    Parts<3> k[4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) k[ks] = split3(mv[ks]);
-    if (i + 2 < pieces) load_move(p + step);
-    __syncthreads();
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) mma(S, k[ks], staged<3>(buf[i & 1], ks, l));
   }
 }
 
@@ -1067,11 +1184,11 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   const int64_t at = (int64_t)slot * a.Hv + h, atk = (int64_t)slot * a.Hk + hk;
 
   if constexpr (NP == 1) {
-    fetch_rows<C>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
-    fetch_rows<C>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
+    fetch_rows<C, 4>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
+    fetch_rows<C, 4>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
   } else {
-    fetch(a.kr + atk * L::kRows, lds_addr(bk), L::kRows / kUnit, wave, l);
-    fetch(a.qr + atk * L::kRows, lds_addr(bq), L::kRows / kUnit, wave, l);
+    fetch<4>(a.kr + atk * L::kRows, lds_addr(bk), L::kRows / kUnit, wave, l);
+    fetch<4>(a.qr + atk * L::kRows, lds_addr(bq), L::kRows / kUnit, wave, l);
   }
   {
     // a thread's 8 elements of each 32: token tid / 4
@@ -1432,7 +1549,7 @@ inline size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
 // What one call lays out, from its sizes alone (so a backward pass finds what its forward kept).
 struct DeltaSizes {
-  int C, seg;                 // tokens of a chunk; chunks of a segment, 0: none
+  int C, seg, columns;        // tokens of a chunk; chunks of a segment, 0: none; columns of a scan's block
   int64_t slots, segs;        // 0 slots: out of range
   size_t tm, pm, gates, sums, kr, states, s0, u;
   size_t workspace(bool backward) const {
@@ -1458,14 +1575,20 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
     z.slots = 0;
     return z;
   }
-  // Segments of equal length where the sequences and heads alone would leave CUs without a block
-  if ((int64_t)N * Hv < 384) {
-    int64_t seg = (z.slots * Hv + 511) / 512;
+  // Which shape, and segments or not, in us a chunk of all heads (bf16 forward, 16384 tokens of 16 heads and
+  // alike): heads in one piece by 64 columns 6.5 while their blocks fit the chip, whole heads 9.3
+  // at one block a CU and 15 at two; segments cost 0.07 a head and chunk, both passes together.
+  // So segments for few heads (64 heads, T = 4096: 376 us against 415), and blocks of
+  // 64 columns up to 128 heads; packed sequences differ in length, and up to 384 the longest one's
+  // pace decides (23 of 12289 tokens, 16 heads: 244 against 271).
+  const int64_t heads = (int64_t)N * Hv;
+  z.columns = heads <= 32 ? 32 : heads <= (packed ? 384 : 128) ? 64 : 128;
+  const int64_t length = packed ? nc / N : nc;               // of one sequence
+  if (heads <= 88 && length >= 12) {
+    int64_t seg = (length * heads + 511) / 512;              // two blocks a CU
     if (seg < 4) seg = 4;
-    if (3 * seg <= nc) {
-      z.seg = (int)seg;
-      z.segs = packed ? (int64_t)T / (z.C * seg) + N : B * ((nc + seg - 1) / seg);
-    }
+    z.seg = (int)seg;
+    z.segs = packed ? (int64_t)T / (z.C * seg) + N : B * ((nc + seg - 1) / seg);
   }
   const size_t n = (size_t)z.slots * Hv, nk = (size_t)z.slots * Hk;
   if (dtype == GSA_DTYPE_BF16) backward ? pack_sizes<uint16_t, true>(z, n, nk) : pack_sizes<uint16_t, false>(z, n, nk);
@@ -1488,43 +1611,65 @@ template <auto kKernel> int allow_lds(size_t bytes) {
   return GSA_OK;
 }
 
-template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
-  using L = gsa::ScanLds<T>;
-  static_assert(2 * L::kFwd <= 160 * 1024, "two blocks a CU");
-  hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, false>), dim3(z.slots * a.Hv), dim3(256), 0, s, a);
-  if (const int e = launch_status()) return e;
-  if (a.seg) {
-    if (const int e = allow_lds<gsa::delta_scan_kernel<T, false>>(L::kFwdState)) return e;
-    hipLaunchKernelGGL((gsa::delta_scan_kernel<T, false>), dim3(z.segs * a.Hv, 2), dim3(256), L::kFwdState, s, a);
-    if (const int e = launch_status()) return e;
-    hipLaunchKernelGGL(gsa::delta_join_kernel<false>, dim3(8, a.Hv, a.s.N), dim3(512), 0, s, a, z.C);
-    if (const int e = launch_status()) return e;
-  }
-  if (const int e = allow_lds<gsa::delta_scan_kernel<T, true>>(L::kFwd)) return e;
-  hipLaunchKernelGGL((gsa::delta_scan_kernel<T, true>), dim3((a.seg ? z.segs : a.s.N) * a.Hv), dim3(256), L::kFwd, s, a);
+using Heads = gsa::Shape<2, 4, false>;
+using Columns64 = gsa::Shape<1, 4, true>;
+using Columns32 = gsa::Shape<1, 2, true>;
+
+template <typename T, bool kOut, typename Sh> int launch_scan(const gsa::DeltaArgs& a, int passes, hipStream_t s) {
+  using L = gsa::ScanLds<T, Sh>;
+  constexpr size_t lds = kOut ? L::kFwd : L::kState;
+  static_assert(lds * (Sh::kDouble ? 1 : 2) <= 160 * 1024);
+  if (const int e = allow_lds<gsa::delta_scan_kernel<T, kOut, Sh>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::delta_scan_kernel<T, kOut, Sh>), dim3(gsa::blocks_for(a.units, Sh::kBlocks), passes), dim3(64 * Sh::W), lds, s, a);
   return launch_status();
 }
-template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
-  constexpr size_t lds = gsa::ScanLds<T>::kBwd, lds_grads = gsa::GradLds<T>::kBytes;
-  static_assert(2 * lds <= 160 * 1024 && 2 * lds_grads <= 160 * 1024, "two blocks a CU");
-  hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, true>), dim3(z.slots * a.Hv), dim3(256), 0, s, a);
-  if (const int e = launch_status()) return e;
+template <typename T, bool kOut, typename Sh> int launch_scan_bwd(const gsa::DeltaArgs& a, hipStream_t s) {
+  constexpr size_t lds = gsa::ScanLds<T, Sh>::kBwd;
+  static_assert(lds * (Sh::kDouble ? 1 : 2) <= 160 * 1024);
+  if (const int e = allow_lds<gsa::delta_scan_bwd_kernel<T, kOut, Sh>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, kOut, Sh>), dim3(gsa::blocks_for(a.units, Sh::kBlocks)), dim3(64 * Sh::W), lds, s, a);
+  return launch_status();
+}
+template <typename T, bool kBwd> int launch_chunks(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
+  hipLaunchKernelGGL((gsa::delta_chunk_kernel<T, kBwd>), dim3(z.slots * a.Hv), dim3(256), 0, s, a);
+  return launch_status();
+}
+template <bool kBwd> int launch_join(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
+  hipLaunchKernelGGL(gsa::delta_join_kernel<kBwd>, dim3(gsa::blocks_for((int64_t)a.s.N * a.Hv, 8)), dim3(512), 0, s, a, z.C);
+  return launch_status();
+}
+template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
+  if (const int e = launch_chunks<T, false>(a, z, s)) return e;
   if (a.seg) {
-    if (const int e = allow_lds<gsa::delta_scan_bwd_kernel<T, false>>(lds)) return e;
-    hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, false>), dim3(z.segs * a.Hv), dim3(256), lds, s, a);
-    if (const int e = launch_status()) return e;
-    hipLaunchKernelGGL(gsa::delta_join_kernel<true>, dim3(8, a.Hv, a.s.N), dim3(512), 0, s, a, z.C);
-    if (const int e = launch_status()) return e;
+    if (const int e = launch_scan<T, false, Heads>(a, 2, s)) return e;
+    if (const int e = launch_join<false>(a, z, s)) return e;
+    return launch_scan<T, true, Heads>(a, 1, s);
   }
-  if (const int e = allow_lds<gsa::delta_scan_bwd_kernel<T, true>>(lds)) return e;
-  hipLaunchKernelGGL((gsa::delta_scan_bwd_kernel<T, true>), dim3((a.seg ? z.segs : a.s.N) * a.Hv), dim3(256), lds, s, a);
-  if (const int e = launch_status()) return e;
-  if (const int e = allow_lds<gsa::delta_grads_kernel<T>>(lds_grads)) return e;
-  hipLaunchKernelGGL(gsa::delta_grads_kernel<T>, dim3(z.slots * a.Hv), dim3(256), lds_grads, s, a);
-  if (a.Hv > a.Hk) {
-    if (const int e = launch_status()) return e;
-    hipLaunchKernelGGL(gsa::delta_shared_kernel<T>, dim3(z.slots * a.Hk), dim3(256), 0, s, a);
+  if (z.columns == 32) return launch_scan<T, true, Columns32>(a, 1, s);
+  if (z.columns == 64) return launch_scan<T, true, Columns64>(a, 1, s);
+  return launch_scan<T, true, Heads>(a, 1, s);
+}
+template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
+  if (const int e = launch_chunks<T, true>(a, z, s)) return e;
+  int e;
+  if (a.seg) {
+    if ((e = launch_scan_bwd<T, false, Heads>(a, s))) return e;
+    if ((e = launch_join<true>(a, z, s))) return e;
+    e = launch_scan_bwd<T, true, Heads>(a, s);
+  } else if (z.columns == 32) {
+    e = launch_scan_bwd<T, true, Columns32>(a, s);
+  } else if (z.columns == 64) {
+    e = launch_scan_bwd<T, true, Columns64>(a, s);
+  } else {
+    e = launch_scan_bwd<T, true, Heads>(a, s);
   }
+  if (e) return e;
+  constexpr size_t lds = gsa::GradLds<T>::kBytes;
+  static_assert(2 * lds <= 160 * 1024, "two blocks a CU");
+  if ((e = allow_lds<gsa::delta_grads_kernel<T>>(lds))) return e;
+  hipLaunchKernelGGL(gsa::delta_grads_kernel<T>, dim3(z.slots * a.Hv), dim3(256), lds, s, a);
+  if ((e = launch_status()) || a.Hv == a.Hk) return e;
+  hipLaunchKernelGGL(gsa::delta_shared_kernel<T>, dim3(z.slots * a.Hk), dim3(256), 0, s, a);
   return launch_status();
 }
 
@@ -1580,7 +1725,7 @@ int delta_args(const gsa_delta_args* x, bool backward, gsa::DeltaArgs& a, DeltaS
   a.kr = take(z.kr);
   a.qr = take(z.kr);
   a.seg = z.seg;
-  a.segs = (int)z.segs;
+  a.units = (int)((z.seg ? z.segs : x->N) * x->Hv);
   a.add = reinterpret_cast<float*>(take(z.states));
   a.init = reinterpret_cast<float*>(take(z.states));
   if (x->saved) {
