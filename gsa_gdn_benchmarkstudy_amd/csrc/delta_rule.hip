@@ -1141,9 +1141,10 @@ template <typename T> struct GradLds {
   static constexpr int kIn = NP == 1 ? 2 : 3;
   static constexpr int kStage = MT * (NP + 3 + 3) * kUnit;   // dO, U, dR: 32 elements of every token
   static constexpr int kRows = MT * 4 * NP * kUnit;          // K, Q
+  static constexpr int kStates = 4 * 2 * 4 * kUnit;          // 32 elements of the 32 rows of S0 and dS1 of each wave, then K, Q
   static constexpr int kKind = MT * JS * kIn * kUnit;        // a [C][C] operand
   static constexpr int kLate = 3 * kKind + C * kLd * 4;
-  static constexpr int kEarly = kStage + 2 * kRows;
+  static constexpr int kEarly = kStage + (2 * kRows > kStates ? 2 * kRows : kStates);
   static constexpr int kBig = kEarly > kLate ? kEarly : kLate;
   static constexpr size_t kBytes = kBig + 4 * (12 * C + 5 * C + C + MT * C + 4) + 8 * C;
 };
@@ -1183,13 +1184,31 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   const int64_t tok = (int64_t)sp.b * a.s.T + sp.t0 + t0;    // row of [B * T]
   const int64_t at = (int64_t)slot * a.Hv + h, atk = (int64_t)slot * a.Hk + hk;
 
-  if constexpr (NP == 1) {
-    fetch_rows<C, 4>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
-    fetch_rows<C, 4>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
-  } else {
-    fetch<4>(a.kr + atk * L::kRows, lds_addr(bk), L::kRows / kUnit, wave, l);
-    fetch<4>(a.qr + atk * L::kRows, lds_addr(bq), L::kRows / kUnit, wave, l);
-  }
+  auto fetch_kq = [&]() {
+    if constexpr (NP == 1) {
+      fetch_rows<C, 4>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
+      fetch_rows<C, 4>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
+    } else {
+      fetch<4>(a.kr + atk * L::kRows, lds_addr(bk), L::kRows / kUnit, wave, l);
+      fetch<4>(a.qr + atk * L::kRows, lds_addr(bq), L::kRows / kUnit, wave, l);
+    }
+  };
+  // The wave's rows of S0 and dS1, 32 elements each, by direct loads into a place of its own:
+  // piece p (16 bytes) of row r at p ^ turn(r), so that the 16 rows of an operand meet 16 banks.
+  const float* s0p = uniform(a.s0 + at * kHead * kHead + 32 * wave * kHead);
+  const float* s1p = uniform(a.ds1 + at * kHead * kHead + 32 * wave * kHead);
+  char* bs = bk + wave * 8 * kUnit;
+  auto turn = [](int r) { return (r >> 1 & 1) | (r >> 3 & 1) << 1 | (r >> 4 & 1) << 2; };
+  auto fetch_states = [&](int ks) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = 8 * u + (l >> 3);
+      const uint32_t o = 4 * (r * kHead + 32 * ks) + 16 * ((l & 7) ^ turn(r));
+      load_lds16(s0p, o, __builtin_amdgcn_readfirstlane(lds_addr(bs) + u * kUnit));
+      load_lds16(s1p, o, __builtin_amdgcn_readfirstlane(lds_addr(bs) + (4 + u) * kUnit));
+    }
+  };
+  fetch_states(0);
   {
     // a thread's 8 elements of each 32: token tid / 4
     const int st = tid >> 2, so = tid & 3;
@@ -1251,19 +1270,24 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
 #pragma unroll
     for (int i = 0; i < kMine; ++i) E[i] = F[i] = floatx4{0.f, 0.f, 0.f, 0.f};
     double dot = 0.;
-    const float* s0p = uniform(a.s0 + at * kHead * kHead);
-    const float* s1p = uniform(a.ds1 + at * kHead * kHead);
 #pragma unroll 1
     for (int ks = 0; ks < 4; ++ks) {
       float y[2][8], z[2][8];
+      wait_loads();
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const uint32_t o = tile_row(2 * wave + e, m) * kHead + 32 * ks + 8 * g;
-        load8(s0p + o, y[e]);
-        load8(s1p + o, z[e]);
+        const int r = 8 * (m >> 2) + 4 * e + (m & 3), o = 128 * r;
+        const floatx4* p = reinterpret_cast<const floatx4*>(bs + o);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const floatx4 u = p[(2 * g + i) ^ turn(r)], w = p[((2 * g + i) ^ turn(r)) + 4 * kUnit / 16];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) { y[e][4 * i + k] = u[k]; z[e][4 * i + k] = w[k]; }
+        }
       }
-      if (ks) __syncthreads();                               // the last elements' operands are read
+      __syncthreads();                                       // the last elements' operands are read
       put();
+      if (ks < 3) fetch_states(ks + 1); else fetch_kq();
       __syncthreads();
       if (ks < 3) load(ks + 1);
       const bf16x8* so_ = stage;
@@ -1585,8 +1609,11 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   z.columns = heads <= 32 ? 32 : heads <= (packed ? 384 : 128) ? 64 : 128;
   const int64_t length = packed ? nc / N : nc;               // of one sequence
   if (heads <= 88 && length >= 12) {
-    int64_t seg = (length * heads + 511) / 512;              // two blocks a CU
-    if (seg < 4) seg = 4;
+    // a block a CU (T = 16384 of 16 heads: 16 segments 358 us, 32 373); joining costs 2.4 us a segment and the two
+    // passes 17 us a chunk of one: more than sqrt(7 chunks) segments lose
+    int64_t pieces = 256 / heads;
+    while (pieces > 3 && pieces * pieces > 7 * length) --pieces;
+    const int64_t seg = std::max<int64_t>(4, (length + pieces - 1) / pieces);
     z.seg = (int)seg;
     z.segs = packed ? (int64_t)T / (z.C * seg) + N : B * ((nc + seg - 1) / seg);
   }
