@@ -10,6 +10,7 @@ missing library raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -898,7 +899,15 @@ def layer_attn(proj, offsets, bias32, idx_scale: float, cos, sin, halves, H: int
 
 # ---------------------------------------------------------------------------
 # RMS norm with the residual's addition
+#
+# The host's part of these calls is longer than a small one's kernel: the stream's handle is asked
+# for directly (0.1 us; through torch.cuda.current_stream 2), and tensors that need no
+# rearrangement go past what arranges them.
 # ---------------------------------------------------------------------------
+
+def _raw_stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
 
 def _on(dev: torch.device, *ts: Optional[torch.Tensor]) -> None:
     for t in ts:
@@ -910,10 +919,12 @@ def _norm_rows(ts, D: int):
     """The tensors (equal shapes [..., D], or None) as rows of D: (inner, [(tensor, s0, s1)]).
     Strided ones are read in place where their leading dimensions make rows in groups of
     shape[-2] (heads of a projection); others are copied."""
-    flat, inner = [], 1
     for t in ts:
         if t is not None and not t.is_contiguous():
-            inner = t.shape[-2] if t.dim() >= 2 else 1
+            break
+    else:
+        return 1, [(t, D, D) for t in ts]
+    flat, inner = [], t.shape[-2] if t.dim() >= 2 else 1
     for t in ts:
         if t is None:
             flat.append((None, 0, 0))
@@ -933,30 +944,32 @@ def _norm_rows(ts, D: int):
 
 def rms_norm(x, w, res=None, eps: float = 1e-6, want_rstd: bool = False):
     """gsa_rms_norm: (y, h, rstd), h None without a residual, rstd None unless wanted."""
-    lib = load()
     D = x.shape[-1]
     rows = x.numel() // D
     inner, ((x, x0, x1), (res, r0, r1)) = _norm_rows((x, res), D)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    h = torch.empty_like(y) if res is not None else None
-    rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if want_rstd else None
-    st = lib.gsa_rms_norm(_ptr(x), x0, x1, _ptr(res), r0, r1, _ptr(w), float(eps), rows, inner, D, dtype_code(x.dtype),
-                          _ptr(y), _ptr(h), _ptr(rstd), _stream(x))
-    _check(st, "gsa_rms_norm")
+    dev = x.device
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    h = torch.empty(x.shape, device=dev, dtype=x.dtype) if res is not None else None
+    rstd = torch.empty(rows, device=dev, dtype=torch.float32) if want_rstd else None
+    st = load().gsa_rms_norm(x.data_ptr(), x0, x1, _ptr(res), r0, r1, w.data_ptr(), eps, rows, inner, D, dtype_code(x.dtype),
+                             y.data_ptr(), _ptr(h), _ptr(rstd), _raw_stream(x))
+    if st:
+        _check(st, "gsa_rms_norm")
     return y, h, rstd
 
 
 def rms_norm_fp8(x, w, res=None, eps: float = 1e-6):
     """gsa_rms_norm_fp8: (y e4m3, scale fp32 [...], h or None)."""
-    lib = load()
     D = x.shape[-1]
     inner, ((x, x0, x1), (res, r0, r1)) = _norm_rows((x, res), D)
-    y = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
-    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if res is not None else None
-    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    st = lib.gsa_rms_norm_fp8(_ptr(x), x0, x1, _ptr(res), r0, r1, _ptr(w), float(eps), scale.numel(), inner, D,
-                              dtype_code(x.dtype), _ptr(y), _ptr(scale), _ptr(h), _stream(x))
-    _check(st, "gsa_rms_norm_fp8")
+    dev = x.device
+    y = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
+    h = torch.empty(x.shape, device=dev, dtype=x.dtype) if res is not None else None
+    scale = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
+    st = load().gsa_rms_norm_fp8(x.data_ptr(), x0, x1, _ptr(res), r0, r1, w.data_ptr(), eps, scale.numel(), inner, D,
+                                 dtype_code(x.dtype), y.data_ptr(), scale.data_ptr(), _ptr(h), _raw_stream(x))
+    if st:
+        _check(st, "gsa_rms_norm_fp8")
     return y, scale, h
 
 
@@ -966,13 +979,15 @@ def rms_norm_backward(h, dy, dh, w, rstd):
     D = h.shape[-1]
     rows = h.numel() // D
     inner, ((h, h0, h1), (dy, y0, y1), (dh, d0, d1)) = _norm_rows((h, dy, dh), D)
-    dx = torch.empty(h.shape, device=h.device, dtype=h.dtype)
-    dw = torch.empty(D, device=h.device, dtype=h.dtype)
+    dev, dt = h.device, h.dtype
+    dx = torch.empty(h.shape, device=dev, dtype=dt)
+    dw = torch.empty(D, device=dev, dtype=dt)
     n = lib.gsa_rms_norm_backward_workspace_bytes(rows, D)
-    ws = torch.empty(n, device=h.device, dtype=torch.uint8)
-    st = lib.gsa_rms_norm_backward(_ptr(h), h0, h1, _ptr(dy), y0, y1, _ptr(dh), d0, d1, _ptr(w), _ptr(rstd), rows, inner, D,
-                                   dtype_code(h.dtype), _ptr(dx), _ptr(dw), _ptr(ws), n, _stream(h))
-    _check(st, "gsa_rms_norm_backward")
+    ws = torch.empty(n, device=dev, dtype=torch.uint8)
+    st = lib.gsa_rms_norm_backward(h.data_ptr(), h0, h1, dy.data_ptr(), y0, y1, _ptr(dh), d0, d1, w.data_ptr(), rstd.data_ptr(),
+                                   rows, inner, D, dtype_code(dt), dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), n, _raw_stream(h))
+    if st:
+        _check(st, "gsa_rms_norm_backward")
     return dx, dw
 
 
@@ -982,73 +997,80 @@ def rms_norm_backward(h, dy, dh, w, rstd):
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """t [B,T,heads,128] with 16-byte aligned head rows and tokens less than 32 MiB apart: itself, or a copy."""
-    grp = 16 // t.element_size()
-    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % grp == 0 for s in t.stride()[:-1])
-            and t.stride(1) * t.element_size() < 1 << 25):
+    size = t.element_size()
+    b, s, h, e = t.stride()
+    if e == 1 and ((b | s | h) * size | t.data_ptr()) % 16 == 0 and s * size < 1 << 25:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def delta_step(q, k, v, g, beta, state, idx, scale: float) -> torch.Tensor:
     """gsa_delta_step: o [N,Hv,128]; `state` is updated in place."""
-    lib = load()
     N, Hv, d = v.shape
-    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    (qn, qh, qe), (kn, kh, ke), (vn, vh, ve) = q.stride(), k.stride(), v.stride()
+    if qe != 1 or ke != 1 or ve != 1:
+        return delta_step(q.contiguous(), k.contiguous(), v.contiguous(), g, beta, state, idx, scale)
     o = torch.empty(N, Hv, d, device=v.device, dtype=v.dtype)
-    st = lib.gsa_delta_step(_ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
-                            v.stride(1), _ptr(g), g.stride(0), g.stride(1), _ptr(beta), beta.stride(0), beta.stride(1),
-                            dtype_code(beta.dtype), _ptr(idx), 0 if idx is None else idx.element_size(), _ptr(state),
-                            state.stride(0), state.stride(1), N, state.shape[0], q.shape[1], Hv, d, float(scale),
-                            dtype_code(q.dtype), _ptr(o), _stream(v))
-    _check(st, "gsa_delta_step")
+    st = load().gsa_delta_step(q.data_ptr(), qn, qh, k.data_ptr(), kn, kh, v.data_ptr(), vn, vh, g.data_ptr(), *g.stride(),
+                               beta.data_ptr(), *beta.stride(), dtype_code(beta.dtype), _ptr(idx),
+                               0 if idx is None else idx.element_size(), state.data_ptr(), *state.stride()[:2], N,
+                               state.shape[0], q.shape[1], Hv, d, scale, dtype_code(q.dtype), o.data_ptr(), _raw_stream(v))
+    if st:
+        _check(st, "gsa_delta_step")
     return o
 
 
 def _delta_args(q, k, v, g, beta, state_in, cu, scale: float) -> DeltaArgs:
     B, T, Hv, d = v.shape
-    a = DeltaArgs(cu_seqlens=_ptr(cu), cu_bytes=0 if cu is None else cu.element_size(), B=B, T=T,
-                  N=B if cu is None else cu.numel() - 1, Hk=q.shape[2], Hv=Hv, d=d, dtype=dtype_code(q.dtype),
-                  beta_dtype=dtype_code(beta.dtype), scale=float(scale), state_in=_ptr(state_in))
-    for n, t in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta)):
-        setattr(a, n, _ptr(t))
-        for s, i in (("sb", 0), ("st", 1), ("sh", 2)):
-            setattr(a, f"{n}_{s}", t.stride(i))
-    return a
+    # in the order of the fields
+    return DeltaArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), *q.stride()[:3], *k.stride()[:3],
+                     *v.stride()[:3], *g.stride(), *beta.stride(), _ptr(cu), 0 if cu is None else cu.element_size(), B, T,
+                     B if cu is None else cu.numel() - 1, q.shape[2], Hv, d, dtype_code(q.dtype), dtype_code(beta.dtype), scale,
+                     _ptr(state_in))
+
+
+@functools.lru_cache(maxsize=256)
+def _delta_bytes(*sizes: int):
+    """Bytes of workspace forward and backward, and of what a forward keeps."""
+    lib = load()
+    return (lib.gsa_delta_rule_workspace_bytes(*sizes, 0), lib.gsa_delta_rule_workspace_bytes(*sizes, 1),
+            lib.gsa_delta_rule_saved_bytes(*sizes))
 
 
 def delta_rule(q, k, v, g, beta, state_in, cu, scale: float, want_state: bool, want_saved: bool):
     """gsa_delta_rule: (o, state_out or None, saved or None).  q, k, v as _heads gives them."""
-    lib = load()
     B, T, Hv, d = v.shape
     a = _delta_args(q, k, v, g, beta, state_in, cu, scale)
-    sizes = (B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
+    forward, _, keep = _delta_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
     # rows outside every packed sequence stay 0
     o = (torch.empty if cu is None else torch.zeros)(B, T, Hv, d, device=v.device, dtype=v.dtype)
     state = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_state else None
-    a.ws_bytes = lib.gsa_delta_rule_workspace_bytes(*sizes, 0)
-    ws = torch.empty(a.ws_bytes, device=v.device, dtype=torch.uint8)
+    ws = torch.empty(forward, device=v.device, dtype=torch.uint8)
+    a.o, a.state_out, a.ws, a.ws_bytes = o.data_ptr(), _ptr(state), ws.data_ptr(), forward
     saved = None
     if want_saved:
-        a.saved_bytes = lib.gsa_delta_rule_saved_bytes(*sizes)
-        saved = torch.empty(a.saved_bytes, device=v.device, dtype=torch.uint8)
-    a.o, a.state_out, a.ws, a.saved = _ptr(o), _ptr(state), _ptr(ws), _ptr(saved)
-    _check(lib.gsa_delta_rule(ctypes.byref(a), _stream(v)), "gsa_delta_rule")
+        saved = torch.empty(keep, device=v.device, dtype=torch.uint8)
+        a.saved, a.saved_bytes = saved.data_ptr(), keep
+    st = load().gsa_delta_rule(ctypes.byref(a), _raw_stream(v))
+    if st:
+        _check(st, "gsa_delta_rule")
     return o, state, saved
 
 
 def delta_rule_backward(q, k, v, g, beta, cu, scale: float, saved, dout, dstate, want_dstate: bool):
     """gsa_delta_rule_backward: (dq, dk, dv, dg, dbeta, dstate_in or None)."""
-    lib = load()
     B, T, Hv, d = v.shape
     a = _delta_args(q, k, v, g, beta, None, cu, scale)
     new = torch.empty if cu is None else torch.zeros
-    dq, dk, dv, dg, db = (new(t.shape, device=v.device, dtype=t.dtype) for t in (q, k, v, g, beta))
+    dq, dk, dv, dg, db = [new(t.shape, device=v.device, dtype=t.dtype) for t in (q, k, v, g, beta)]
     ds = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_dstate else None
-    a.ws_bytes = lib.gsa_delta_rule_workspace_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype, 1)
+    _, a.ws_bytes, a.saved_bytes = _delta_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
     ws = torch.empty(a.ws_bytes, device=v.device, dtype=torch.uint8)
-    a.ws, a.saved, a.saved_bytes = _ptr(ws), _ptr(saved), saved.numel()
-    a.dout, a.do_sb, a.do_st, a.do_sh = _ptr(dout), dout.stride(0), dout.stride(1), dout.stride(2)
+    a.ws, a.saved = ws.data_ptr(), saved.data_ptr()
+    a.dout, (a.do_sb, a.do_st, a.do_sh, _) = dout.data_ptr(), dout.stride()
     a.dstate_out, a.dstate_in = _ptr(dstate), _ptr(ds)
-    a.dq, a.dk, a.dv, a.dg, a.dbeta = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dg), _ptr(db)
-    _check(lib.gsa_delta_rule_backward(ctypes.byref(a), _stream(v)), "gsa_delta_rule_backward")
+    a.dq, a.dk, a.dv, a.dg, a.dbeta = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), db.data_ptr()
+    st = load().gsa_delta_rule_backward(ctypes.byref(a), _raw_stream(v))
+    if st:
+        _check(st, "gsa_delta_rule_backward")
     return dq, dk, dv, dg, db, ds

@@ -14,6 +14,7 @@ d**-0.5 gives them unit length).  There is no CPU or eager fallback.
 
 from __future__ import annotations
 
+import contextlib
 from typing import Optional, Tuple
 
 import torch
@@ -25,47 +26,73 @@ from .roctx import range_pop as _range_pop, range_push as _range_push
 D_HEAD = 128
 
 
-def _check(lead, q, k, v, g, beta) -> None:
-    """The checks that both entry points share; lead: the dimensions before the heads."""
-    n = len(lead)
-    if q.dim() != n + 2 or k.shape != q.shape or v.dim() != n + 2 or v.shape[:n] != q.shape[:n]:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: expected [{', '.join(lead)}, heads, {D_HEAD}]")
-    if q.shape[-1] != D_HEAD or v.shape[-1] != D_HEAD:
-        raise ValueError(f"head dims {q.shape[-1]} and {v.shape[-1]}: the kernels take {D_HEAD}")
-    Hk, Hv = q.shape[n], v.shape[n]
+def _check(n: int, q, k, v, g, beta) -> None:
+    """The checks that both entry points share; n: dimensions before the heads."""
+    qs, vs = q.shape, v.shape
+    if len(qs) != n + 2 or len(vs) != n + 2 or k.shape != qs or vs[:n] != qs[:n]:
+        raise ValueError(f"q {tuple(qs)}, k {tuple(k.shape)}, v {tuple(vs)}: expected [{'B, T' if n == 2 else 'N'}, heads, {D_HEAD}]")
+    if qs[-1] != D_HEAD or vs[-1] != D_HEAD:
+        raise ValueError(f"head dims {qs[-1]} and {vs[-1]}: the kernels take {D_HEAD}")
+    Hk, Hv = qs[n], vs[n]
     if Hk < 1 or Hv < 1 or Hv % Hk:
         raise ValueError(f"{Hv} v heads are not a multiple of {Hk} q/k heads")
-    if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
-        raise ValueError(f"g {tuple(g.shape)}, beta {tuple(beta.shape)}: expected {tuple(v.shape[:-1])}")
-    if not (q.dtype == k.dtype == v.dtype):
-        raise ValueError(f"q, k, v must share a dtype: got {q.dtype}, {k.dtype}, {v.dtype}")
-    _abi.dtype_code(q.dtype)
+    if g.shape != vs[:-1] or beta.shape != vs[:-1]:
+        raise ValueError(f"g {tuple(g.shape)}, beta {tuple(beta.shape)}: expected {tuple(vs[:-1])}")
+    dt = q.dtype
+    if k.dtype != dt or v.dtype != dt:
+        raise ValueError(f"q, k, v must share a dtype: got {dt}, {k.dtype}, {v.dtype}")
+    _abi.dtype_code(dt)
     if g.dtype != torch.float32:
         raise TypeError(f"g is {g.dtype}: log decays are float32")
-    if beta.dtype not in (torch.float32, q.dtype):
-        raise TypeError(f"beta is {beta.dtype}: expected float32 or {q.dtype}")
+    if beta.dtype != torch.float32 and beta.dtype != dt:
+        raise TypeError(f"beta is {beta.dtype}: expected float32 or {dt}")
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _device(first: torch.Tensor, *others: Optional[torch.Tensor]):
     """Checks that all tensors are on one GPU and makes it the current one."""
-    _abi._need_cuda(first, *others)
-    _abi._on(first.device, *others)
-    return torch.cuda.device(first.device)
+    at = first.get_device()                      # -1 on the CPU
+    for t in others:
+        if t is not None and t.get_device() != at:
+            _abi._need_cuda(first, *others)
+            _abi._on(first.device, *others)
+    if at < 0:
+        _abi._need_cuda(first)
+    return _HERE if torch.cuda.current_device() == at else torch.cuda.device(at)
+
+
+def _needs_grad(*ts: Optional[torch.Tensor]) -> bool:
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _once(backward):
+    """A backward pass that is differentiable once.  torch's once_differentiable costs 15 us: only
+    where a graph of the backward pass is being built is its error needed."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return staticmethod(run)
 
 
 class _Rule(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, cu, scale, want_state, want_saved):
+    def forward(ctx, q, k, v, g, beta, state, cu, scale, want_state):
         q, k, v = _abi._heads(q), _abi._heads(k), _abi._heads(v)
-        o, final, saved = _abi.delta_rule(q, k, v, g, beta, state, cu, scale, want_state, want_saved)
+        o, final, saved = _abi.delta_rule(q, k, v, g, beta, state, cu, scale, want_state, True)
         ctx.set_materialize_grads(False)
         ctx.scale, ctx.has_state = scale, state is not None
-        if want_saved:
-            ctx.save_for_backward(q, k, v, g, beta, cu, saved)
+        ctx.save_for_backward(q, k, v, g, beta, cu, saved)
         return o, final
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, do, dfinal):
         q, k, v, g, beta, cu, saved = ctx.saved_tensors
         _range_push("gsa_hip/delta_rule_backward")
@@ -78,7 +105,7 @@ class _Rule(torch.autograd.Function):
             grads = _abi.delta_rule_backward(q, k, v, g, beta, cu, ctx.scale, saved, do, dfinal, ctx.has_state)
         finally:
             _range_pop()
-        return (*grads, None, None, None, None)
+        return (*grads, None, None, None)
 
 
 def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -101,7 +128,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     bits on every run.  A forward that needs gradients keeps 1.5 KiB (bf16; fp32: 2.5 KiB) a
     token and v head.
     """
-    _check(("B", "T"), q, k, v, g, beta)
+    _check(2, q, k, v, g, beta)
     B, T, Hv, d = v.shape
     if cu_seqlens is not None:
         if B != 1:
@@ -124,10 +151,13 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
             initial_state = initial_state.contiguous()
             if initial_state.data_ptr() % 16:
                 initial_state = initial_state.clone()
-        grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
         _range_push("gsa_hip/delta_rule")
         try:
-            return _Rule.apply(q, k, v, g, beta, initial_state, cu_seqlens, scale, bool(output_final_state), grad)
+            if _needs_grad(q, k, v, g, beta, initial_state):
+                return _Rule.apply(q, k, v, g, beta, initial_state, cu_seqlens, scale, bool(output_final_state))
+            o, final, _ = _abi.delta_rule(_abi._heads(q), _abi._heads(k), _abi._heads(v), g, beta, initial_state, cu_seqlens,
+                                          scale, output_final_state, False)
+            return o, final
         finally:
             _range_pop()
 
@@ -145,13 +175,14 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
 
     Forward only: it raises where a gradient would be needed.
     """
-    _check(("N",), q, k, v, g, beta)
+    _check(1, q, k, v, g, beta)
     N, Hv, d = v.shape
     if state.dim() != 4 or tuple(state.shape[1:]) != (Hv, d, d) or state.dtype != torch.float32:
         raise ValueError(f"state {tuple(state.shape)} {state.dtype}: expected fp32 [slots, {Hv}, {d}, {d}]")
-    if state.stride()[2:] != (d, 1) or state.stride(0) % 4 or state.stride(1) % 4 or state.data_ptr() % 16:
+    s0, s1, s2, s3 = state.stride()
+    if s2 != d or s3 != 1 or (s0 | s1) % 4 or state.data_ptr() % 16:
         raise ValueError("state is updated in place: its matrices must be contiguous and 16-byte aligned")
-    if state.shape[0] > 1 and state.stride(0) < d * d or Hv > 1 and state.stride(1) < d * d:
+    if state.shape[0] > 1 and s0 < d * d or Hv > 1 and s1 < d * d:
         raise ValueError("state is updated in place: its matrices overlap")
     if state_indices is not None:
         if tuple(state_indices.shape) != (N,) or state_indices.dtype not in (torch.int32, torch.int64):
@@ -159,13 +190,13 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         state_indices = state_indices.contiguous()
     elif N > state.shape[0]:
         raise ValueError(f"{N} rows, {state.shape[0]} states")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
+    if _needs_grad(q, k, v, g, beta, state):
         raise RuntimeError("gated_delta_step is forward only: call it under torch.no_grad()")
     with _device(q, k, v, g, beta, state, state_indices):
         if N == 0 or state.shape[0] == 0:
             return v.new_zeros(v.shape)
         _range_push("gsa_hip/delta_step")
         try:
-            return _abi.delta_step(q, k, v, g, beta, state, state_indices, d ** -0.5 if scale is None else scale)
+            return _abi.delta_step(q, k, v, g, beta, state, state_indices, d ** -0.5 if scale is None else float(scale))
         finally:
             _range_pop()

@@ -14,25 +14,25 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _abi
-from .delta import _device
+from .delta import _device, _needs_grad, _once
 from .roctx import range_pop as _range_pop, range_push as _range_push
 
 MAX_D = 32768
 
 
 def _check(x, weight, residual) -> None:
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_D:
-        raise ValueError(f"x {tuple(x.shape)}: rows of 1 to {MAX_D} elements")
-    if tuple(weight.shape) != (x.shape[-1],):
-        raise ValueError(f"weight {tuple(weight.shape)} != {(x.shape[-1],)}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual {tuple(residual.shape)} != x {tuple(x.shape)}")
-    if weight.dtype != x.dtype or residual is not None and residual.dtype != x.dtype:
+    shape, dt = x.shape, x.dtype
+    if not shape or not 1 <= shape[-1] <= MAX_D:
+        raise ValueError(f"x {tuple(shape)}: rows of 1 to {MAX_D} elements")
+    if weight.shape != shape[-1:]:
+        raise ValueError(f"weight {tuple(weight.shape)} != {(shape[-1],)}")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual {tuple(residual.shape)} != x {tuple(shape)}")
+    if weight.dtype != dt or residual is not None and residual.dtype != dt:
         raise ValueError("x, weight and residual must share a dtype")
-    _abi.dtype_code(x.dtype)
+    _abi.dtype_code(dt)
 
 
 class _Norm(torch.autograd.Function):
@@ -45,8 +45,7 @@ class _Norm(torch.autograd.Function):
         ctx.save_for_backward(h if ctx.added else x, weight, rstd)
         return (y, h) if ctx.added else y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dh=None):
         h, weight, rstd = ctx.saved_tensors
         if dy is None:                           # only h was used
@@ -73,10 +72,10 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
             return h * weight, h
         _range_push("gsa_hip/rms_norm")
         try:
-            if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+            if _needs_grad(x, weight, residual):
                 out = _Norm.apply(x, weight, residual, float(eps))
                 return out if residual is not None else (out, x)
-            y, h, _ = _abi.rms_norm(x, weight.contiguous(), residual, eps)
+            y, h, _ = _abi.rms_norm(x, weight.contiguous(), residual, float(eps))
             return y, x if h is None else h
         finally:
             _range_pop()
@@ -88,7 +87,7 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
     y * scale[..., None] is the normed row; scale is the row's largest magnitude / 448 (1 for a
     row of zeros).  Forward only: it raises where a gradient would be needed."""
     _check(x, weight, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if _needs_grad(x, weight, residual):
         raise RuntimeError("add_rms_norm_fp8 is forward only: call it under torch.no_grad()")
     with _device(x, weight, residual):
         if x.numel() == 0:
@@ -96,7 +95,7 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
                     x if residual is None else x + residual)
         _range_push("gsa_hip/rms_norm_fp8")
         try:
-            y, scale, h = _abi.rms_norm_fp8(x, weight.contiguous(), residual, eps)
+            y, scale, h = _abi.rms_norm_fp8(x, weight.contiguous(), residual, float(eps))
             return y, scale, x if h is None else h
         finally:
             _range_pop()
