@@ -1639,6 +1639,7 @@ template <auto kKernel> int allow_lds(size_t bytes) {
 }
 
 using Heads = gsa::Shape<2, 4, false>;
+using HeadsAlone = gsa::Shape<1, 8, true>;
 using Columns64 = gsa::Shape<1, 4, true>;
 using Columns32 = gsa::Shape<1, 2, true>;
 
@@ -1670,11 +1671,11 @@ template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSiz
   if (a.seg) {
     if (const int e = launch_scan<T, false, Heads>(a, 2, s)) return e;
     if (const int e = launch_join<false>(a, z, s)) return e;
-    return launch_scan<T, true, Heads>(a, 1, s);
+    return a.units <= 256 ? launch_scan<T, true, HeadsAlone>(a, 1, s) : launch_scan<T, true, Heads>(a, 1, s);
   }
   if (z.columns == 32) return launch_scan<T, true, Columns32>(a, 1, s);
   if (z.columns == 64) return launch_scan<T, true, Columns64>(a, 1, s);
-  return launch_scan<T, true, Heads>(a, 1, s);
+  return a.units <= 256 ? launch_scan<T, true, HeadsAlone>(a, 1, s) : launch_scan<T, true, Heads>(a, 1, s);
 }
 template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
   if (const int e = launch_chunks<T, true>(a, z, s)) return e;
@@ -1682,13 +1683,13 @@ template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSi
   if (a.seg) {
     if ((e = launch_scan_bwd<T, false, Heads>(a, s))) return e;
     if ((e = launch_join<true>(a, z, s))) return e;
-    e = launch_scan_bwd<T, true, Heads>(a, s);
+    e = a.units <= 256 ? launch_scan_bwd<T, true, HeadsAlone>(a, s) : launch_scan_bwd<T, true, Heads>(a, s);
   } else if (z.columns == 32) {
     e = launch_scan_bwd<T, true, Columns32>(a, s);
   } else if (z.columns == 64) {
     e = launch_scan_bwd<T, true, Columns64>(a, s);
   } else {
-    e = launch_scan_bwd<T, true, Heads>(a, s);
+    e = a.units <= 256 ? launch_scan_bwd<T, true, HeadsAlone>(a, s) : launch_scan_bwd<T, true, Heads>(a, s);
   }
   if (e) return e;
   constexpr size_t lds = gsa::GradLds<T>::kBytes;
