@@ -464,9 +464,10 @@ template <int kBlocks> __device__ __forceinline__ int2 unit_of(int b) {
 }
 constexpr int64_t blocks_for(int64_t units, int blocks) { return blocks == 1 ? units : (units + 7) / 8 * 8 * blocks; }
 
-template <int NT_, int W_, bool kDouble_> struct Shape {
+template <int NT_, int W_, bool kDouble_, int kWaves_ = 2> struct Shape {
   static constexpr int NT = NT_, W = W_, kCols = 16 * NT_ * W_, kBlocks = kHead / kCols;     // columns of a block, blocks of a head
   static constexpr bool kDouble = kDouble_;
+  static constexpr int kWaves = kWaves_;                     // of a SIMD
 };
 
 template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
@@ -561,7 +562,7 @@ __device__ __forceinline__ void tiles_store(const floatx4 (&S)[kTiles][NT], floa
 // the state: blockIdx.y 0 what it adds, 1 its product of transitions (V = 0 from the
 // identity).
 template <typename T, bool kOut, typename Sh>
-__global__ __launch_bounds__(64 * Sh::W, 2) void delta_scan_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_kernel(DeltaArgs a) {
   using K = Pack<T, false>;
   using L = ScanLds<T, Sh>;
   constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32, NT = Sh::NT, W = Sh::W;
@@ -802,7 +803,7 @@ __global__ __launch_bounds__(64 * Sh::W, 2) void delta_scan_kernel(DeltaArgs a) 
 // kOut: dv, and the gradients of the states behind the chunks and of R that the last kernel reads.
 // Otherwise what a segment adds to the gradient of the state before it.
 template <typename T, bool kOut, typename Sh>
-__global__ __launch_bounds__(64 * Sh::W, 2) void delta_scan_bwd_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_bwd_kernel(DeltaArgs a) {
   using K = Pack<T, true>;
   using L = ScanLds<T, Sh>;
   constexpr int C = K::C, NP = K::NP, MT = C / 16, JS = C / 32, NT = Sh::NT, W = Sh::W;
@@ -1638,7 +1639,7 @@ template <auto kKernel> int allow_lds(size_t bytes) {
   return GSA_OK;
 }
 
-using Heads = gsa::Shape<2, 4, false>;
+using Heads = gsa::Shape<1, 8, false, 4>;
 using HeadsAlone = gsa::Shape<1, 8, true>;
 using Columns64 = gsa::Shape<1, 4, true>;
 using Columns32 = gsa::Shape<1, 2, true>;
