@@ -1032,14 +1032,19 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_bwd_kernel(
 // The states before the segments (kBwd: the gradients behind them) from what each adds and its
 // product of transitions: S <- move S + add (dS <- move^T dS + add), segment after segment.  512
 // threads and 16 columns a block: a wave owns the rows tile_row(wave, .), the state goes round
-// through LDS.
+// through LDS.  A wave's rows of move and add come by direct loads, two segments ahead, to places of
+// its own (loads to registers that far ahead were waited for at each turn of the loop).  1.9 us a
+// segment, most of it the parts of move's rows, which only 16 columns share.
+constexpr int kJoinWave = 9 * kUnit;                         // 8 of move, 1 of add
+constexpr size_t kJoinLds = 2 * 8 * kJoinWave + 12 * kUnit;
 template <bool kBwd>
 __global__ __launch_bounds__(512) void delta_join_kernel(DeltaArgs a, int chunk) {
-  constexpr int kAhead = 3;                                  // segments whose loads are on their way
-  __shared__ __align__(16) bf16x8 buf[2][4 * 3 * 64];
+  extern __shared__ __align__(16) char lds[];
+  bf16x8* buf = reinterpret_cast<bf16x8*>(lds + 2 * 8 * kJoinWave);          // the state's operands
   const int2 unit = unit_of<8>(blockIdx.x);                  // a head of a sequence, 16 columns
   if (unit.x >= a.s.N * a.Hv) return;
-  const int h = unit.x % a.Hv, wave = threadIdx.x >> 6, l = lane_id(), g = l >> 4, m = l & 15, col = 16 * unit.y + m;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l >> 4, m = l & 15;
+  const int h = unit.x % a.Hv, col = 16 * unit.y + m;
   const Span sp = span_of(a.s, unit.x / a.Hv, chunk * a.seg);
   const int pieces = (sp.len + chunk * a.seg - 1) / (chunk * a.seg);
   if (pieces == 0) {                                         // no token: no segment to hand the state on
@@ -1053,74 +1058,92 @@ __global__ __launch_bounds__(512) void delta_join_kernel(DeltaArgs a, int chunk)
       }
   }
   if (pieces < 2) return;
-  auto at = [&](int p) { return ((int64_t)(sp.slot0 + p) * a.Hv + h) * kHead * kHead; };
-  auto tile = [&](const float* x) {
-    floatx4 y;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] = x[tile_row(wave, 4 * g + r) * kHead + col];
-    return y;
-  };
   const int first = kBwd ? pieces - 1 : 0, step = kBwd ? -1 : 1;
-  float mv[kAhead][4][8];                                    // rows tile_row(wave, m) of move, or of its transpose
-  floatx4 ad[kAhead];
-  // Loads run kAhead segments ahead, each array's into its own registers and under no condition: what
-  // is copied, or merged behind a branch, is waited for there.  Of the i-th segment (behind the last
-  // one that is asked for that one again):
-  auto where = [&](int i) { return at(first + max(min(i, pieces - 2), 1) * step); };
-  auto load_move = [&](int i, float (&to)[4][8]) {
-    const float* x = a.move + where(i);
+  auto at = [&](int i) { return ((int64_t)(sp.slot0 + first + i * step) * a.Hv + h) * kHead * kHead; };   // the i-th segment's matrix
+  char* const mine = lds + wave * kJoinWave;
+  const uint32_t mine_lds = lds_addr(lds) + wave * kJoinWave;
+  // (behind the last segment that is asked for that one again: the waits count on all loads)
+  auto fetch = [&](int i) {
+    const int64_t o = at(max(min(i, pieces - 2), 1));
+    const float* mv = uniform(a.move + o);
+    const float* ad = uniform(a.add + o);
+    const uint32_t to = mine_lds + (i & 1) * 8 * kJoinWave;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      uint32_t off;
+      if constexpr (kBwd) {                                  // 16 columns, row 8 a + b at b 16 + a: so rows 8 apart lie side by side
+        off = 4 * ((8 * (l >> 2) + u) * kHead + tile_row(wave, 4 * (l & 3)));
+      } else {                                               // rows, two a unit; a piece's place turns with the row
+        const int r = 2 * u + (l >> 5);
+        off = 4 * tile_row(wave, r) * kHead + 16 * ((l & 31) ^ r);
+      }
+      load_lds16(mv, off, __builtin_amdgcn_readfirstlane(to + u * kUnit));
+    }
+    load_lds16(ad, 4 * (tile_row(wave, l >> 2) * kHead + 16 * unit.y + 4 * (l & 3)), __builtin_amdgcn_readfirstlane(to + 8 * kUnit));
+  };
+  floatx4 S;
+  auto keep = [&](int i) {                                   // 4 stores, no more and no fewer: the waits count them
+    const float* init = uniform(a.init + at(i));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t off = 4 * (tile_row(wave, 4 * g + r) * kHead + col);
+      const float x = S[r];
+      asm volatile("global_store_dword %0, %1, %2" ::"v"(off), "v"(x), "s"(init) : "memory");
+    }
+  };
+  {
+    const float* x = a.add + at(0);                          // the first one's start is in it
+#pragma unroll
+    for (int r = 0; r < 4; ++r) S[r] = x[tile_row(wave, 4 * g + r) * kHead + col];
+  }
+  if (pieces > 2) {
+    fetch(1);
+    fetch(2);
+  }
+  keep(1);
+  for (int i = 1; i + 1 < pieces; ++i) {
+    asm volatile("s_waitcnt vmcnt(13)" ::: "memory");        // all but the next segment's 9 loads and 4 stores
+    const char* p = mine + (i & 1) * 8 * kJoinWave;
+    Parts<3> k[4];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
+      float x[8];
       if constexpr (kBwd) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to[ks][e] = x[(32 * ks + 8 * g + e) * kHead + tile_row(wave, m)];
+        for (int e = 0; e < 8; ++e) x[e] = reinterpret_cast<const float*>(p)[(16 * e + 4 * ks + g) * 16 + m];
       } else {
-        load8(x + tile_row(wave, m) * kHead + 32 * ks + 8 * g, to[ks]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const floatx4 y = *reinterpret_cast<const floatx4*>(p + 512 * m + 16 * ((8 * ks + 2 * g + e) ^ m));
+#pragma unroll
+          for (int n = 0; n < 4; ++n) x[4 * e + n] = y[n];
+        }
       }
+      k[ks] = split3(x);
     }
-  };
-  floatx4 S = tile(a.add + at(first));                       // the first one's start is in it
-  asm volatile("" : "+v"(S));                                // (arrived, before the loop knows of it)
-  auto keep = [&](int i) {
-    float* init = a.init + at(first + i * step);
+    floatx4 ad;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) init[tile_row(wave, 4 * g + r) * kHead + col] = S[r];
-  };
-  keep(1);
-  if (pieces == 2) return;
+    for (int r = 0; r < 4; ++r) ad[r] = reinterpret_cast<const float*>(p + 8 * kUnit)[(4 * g + r) * 16 + m];
+    const float x[8] = {S[0], S[1], S[2], S[3], 0.f, 0.f, 0.f, 0.f};
+    const Parts<3> s = split3(x);
 #pragma unroll
-  for (int j = 0; j < kAhead; ++j) {
-    load_move(1 + j, mv[j]);
-    ad[j] = tile(a.add + where(1 + j));
-  }
-  for (int i0 = 1;; i0 += kAhead) {
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int i = i0 + j;
-      const float x[8] = {S[0], S[1], S[2], S[3], 0.f, 0.f, 0.f, 0.f};
-      const Parts<3> s = split3(x);
-#pragma unroll
-      for (int n = 0; n < 3; ++n) {
-        const u32x4 w = __builtin_bit_cast(u32x4, s.p[n]);
-        *reinterpret_cast<uint2*>(reinterpret_cast<char*>(&buf[i & 1][((wave >> 1) * 3 + n) * 64 + l]) + 8 * (wave & 1)) = uint2{w[0], w[1]};
-      }
-      Parts<3> k[4];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) k[ks] = split3(mv[j][ks]);
-      load_move(i + kAhead, mv[j]);
-      __syncthreads();
-      floatx4 sum[4];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        sum[ks] = floatx4{0.f, 0.f, 0.f, 0.f};
-        mma(sum[ks], k[ks], staged<3>(buf[i & 1], ks, l));
-      }
-      S = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ad[j];
-      ad[j] = tile(a.add + where(i + kAhead));
-      keep(i + 1);
-      if (i + 2 >= pieces) return;
+    for (int n = 0; n < 3; ++n) {
+      const u32x4 w = __builtin_bit_cast(u32x4, s.p[n]);
+      *reinterpret_cast<uint2*>(reinterpret_cast<char*>(&buf[((wave >> 1) * 3 + n) * 64 + l]) + 8 * (wave & 1)) = uint2{w[0], w[1]};
     }
+    __syncthreads();                                         // (this wave's reads are done as well)
+    fetch(i + 2);
+    floatx4 sum[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      sum[ks] = floatx4{0.f, 0.f, 0.f, 0.f};
+      mma(sum[ks], k[ks], staged<3>(buf, ks, l));
+    }
+    S = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ad;
+    keep(i + 1);
+    __syncthreads();                                         // the state's operands are read
   }
+  wait_loads();                                              // nothing on its way to LDS when the block ends
 }
 
 // ---------------------------------------------------------------------------
@@ -1610,10 +1633,10 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   z.columns = heads <= 32 ? 32 : heads <= (packed ? 384 : 128) ? 64 : 128;
   const int64_t length = packed ? nc / N : nc;               // of one sequence
   if (heads <= 88 && length >= 12) {
-    // a block a CU (T = 16384 of 16 heads: 16 segments 358 us, 32 373); joining costs 2.4 us a segment and the two
-    // passes 17 us a chunk of one: more than sqrt(7 chunks) segments lose
+    // a block a CU (T = 16384 of 16 heads: 16 segments 358 us, 32 373); joining costs 1.9 us a segment and the two
+    // passes 16 us a chunk of one: more than sqrt(8 chunks) segments lose
     int64_t pieces = 256 / heads;
-    while (pieces > 3 && pieces * pieces > 7 * length) --pieces;
+    while (pieces > 3 && pieces * pieces > 8 * length) --pieces;
     const int64_t seg = std::max<int64_t>(4, (length + pieces - 1) / pieces);
     z.seg = (int)seg;
     z.segs = packed ? (int64_t)T / (z.C * seg) + N : B * ((nc + seg - 1) / seg);
@@ -1664,7 +1687,8 @@ template <typename T, bool kBwd> int launch_chunks(const gsa::DeltaArgs& a, cons
   return launch_status();
 }
 template <bool kBwd> int launch_join(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
-  hipLaunchKernelGGL(gsa::delta_join_kernel<kBwd>, dim3(gsa::blocks_for((int64_t)a.s.N * a.Hv, 8)), dim3(512), 0, s, a, z.C);
+  if (const int e = allow_lds<gsa::delta_join_kernel<kBwd>>(gsa::kJoinLds)) return e;
+  hipLaunchKernelGGL(gsa::delta_join_kernel<kBwd>, dim3(gsa::blocks_for((int64_t)a.s.N * a.Hv, 8)), dim3(512), gsa::kJoinLds, s, a, z.C);
   return launch_status();
 }
 template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
