@@ -1042,8 +1042,7 @@ def delta_rule(q, k, v, g, beta, state_in, cu, scale: float, want_state: bool, w
     B, T, Hv, d = v.shape
     a = _delta_args(q, k, v, g, beta, state_in, cu, scale)
     forward, _, keep = _delta_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
-    # rows outside every packed sequence stay 0
-    o = (torch.empty if cu is None else torch.zeros)(B, T, Hv, d, device=v.device, dtype=v.dtype)
+    o = torch.empty(B, T, Hv, d, device=v.device, dtype=v.dtype)
     state = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_state else None
     ws = torch.empty(forward, device=v.device, dtype=torch.uint8)
     a.o, a.state_out, a.ws, a.ws_bytes = o.data_ptr(), _ptr(state), ws.data_ptr(), forward
@@ -1061,8 +1060,7 @@ def delta_rule_backward(q, k, v, g, beta, cu, scale: float, saved, dout, dstate,
     """gsa_delta_rule_backward: (dq, dk, dv, dg, dbeta, dstate_in or None)."""
     B, T, Hv, d = v.shape
     a = _delta_args(q, k, v, g, beta, None, cu, scale)
-    new = torch.empty if cu is None else torch.zeros
-    dq, dk, dv, dg, db = [new(t.shape, device=v.device, dtype=t.dtype) for t in (q, k, v, g, beta)]
+    dq, dk, dv, dg, db = [torch.empty(t.shape, device=v.device, dtype=t.dtype) for t in (q, k, v, g, beta)]
     ds = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_dstate else None
     _, a.ws_bytes, a.saved_bytes = _delta_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
     ws = torch.empty(a.ws_bytes, device=v.device, dtype=torch.uint8)

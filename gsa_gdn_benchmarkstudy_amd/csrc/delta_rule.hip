@@ -1587,6 +1587,34 @@ __global__ __launch_bounds__(256) void delta_shared_kernel(DeltaArgs a) {
   }
 }
 
+// Zeros to the rows of T that no packed sequence holds: before the first offset and behind the largest.
+// 256 threads; bytes: of a token's row in each array.
+struct Outside {
+  Seqs s;
+  char* p[5];
+  int64_t bytes[5];
+};
+__global__ __launch_bounds__(256) void delta_outside_kernel(Outside a) {
+  __shared__ int most[4];
+  int hi = 0;
+  for (int n = threadIdx.x; n <= a.s.N; n += 256) hi = max(hi, (int)a.s.at(n));
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) hi = max(hi, __shfl_xor(hi, o, 64));
+  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = hi;
+  __syncthreads();
+  hi = max(max(most[0], most[1]), max(most[2], most[3]));
+  const int64_t lo = a.s.at(0);
+  for (int i = 0; i < 5; ++i) {
+    if (!a.p[i]) continue;
+    auto clear = [&](int64_t from, int64_t to) {             // whole elements, 2 bytes at least
+      uint16_t* p = reinterpret_cast<uint16_t*>(a.p[i] + from * a.bytes[i]);
+      for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < (to - from) * a.bytes[i] / 2; k += (int64_t)gridDim.x * 256) p[k] = 0;
+    };
+    clear(0, lo);
+    clear(hi, a.s.T);
+  }
+}
+
 }  // namespace gsa
 
 namespace gsa_host {
@@ -1691,7 +1719,18 @@ template <bool kBwd> int launch_join(const gsa::DeltaArgs& a, const DeltaSizes& 
   hipLaunchKernelGGL(gsa::delta_join_kernel<kBwd>, dim3(gsa::blocks_for((int64_t)a.s.N * a.Hv, 8)), dim3(512), gsa::kJoinLds, s, a, z.C);
   return launch_status();
 }
+// Rows outside every packed sequence: o, or the gradients (two arrays of Hk heads, one of Hv, dg, dbeta).
+int launch_outside(const gsa::DeltaArgs& a, int dtype, bool backward, hipStream_t s) {
+  if (!a.s.cu) return GSA_OK;
+  const int64_t row = 128 * (int64_t)dtype_size(dtype), gate = a.beta_bf16 ? 2 : 4;
+  const gsa::Outside x = backward ? gsa::Outside{a.s, {(char*)a.dq, (char*)a.dk, (char*)a.dv, (char*)a.dg, (char*)a.dbeta},
+                                                 {a.Hk * row, a.Hk * row, a.Hv * row, a.Hv * (int64_t)4, a.Hv * gate}}
+                                  : gsa::Outside{a.s, {(char*)a.o}, {a.Hv * row}};
+  hipLaunchKernelGGL(gsa::delta_outside_kernel, dim3(256), dim3(256), 0, s, x);
+  return launch_status();
+}
 template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
+  if (const int e = launch_outside(a, sizeof(T) == 2 ? GSA_DTYPE_BF16 : GSA_DTYPE_F32, false, s)) return e;
   if (const int e = launch_chunks<T, false>(a, z, s)) return e;
   if (a.seg) {
     if (const int e = launch_scan<T, false, Heads>(a, 2, s)) return e;
@@ -1703,6 +1742,7 @@ template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSiz
   return a.units <= 256 ? launch_scan<T, true, HeadsAlone>(a, 1, s) : launch_scan<T, true, Heads>(a, 1, s);
 }
 template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
+  if (const int e = launch_outside(a, sizeof(T) == 2 ? GSA_DTYPE_BF16 : GSA_DTYPE_F32, true, s)) return e;
   if (const int e = launch_chunks<T, true>(a, z, s)) return e;
   int e;
   if (a.seg) {

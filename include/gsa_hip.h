@@ -562,7 +562,8 @@ int gsa_delta_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int
  * gsa_delta_rule: whole sequences, in chunks on the matrix cores.  B rows of T tokens
  * (N == B), or N sequences packed in the T tokens of one row (B == 1): cu_seqlens, N + 1
  * ascending offsets on the device (int32 or int64 by cu_bytes); empty sequences are allowed,
- * offsets are held within [0, T], and rows outside every sequence are not written.
+ * offsets are held within [0, T], and rows of o and of the gradients before the first and behind
+ * the last sequence are set to 0.
  * q, k [B,T,Hk,128], v [B,T,Hv,128] in dtype, g fp32 and beta (beta_dtype) [B,T,Hv]; strides
  * of batch, token and head in elements, those of q, k, v (and dout) keeping 16-byte
  * alignment.  g below -128 (down to -inf) acts as -128, whose e^g is 0.
