@@ -45,6 +45,39 @@ __device__ __forceinline__ void slot_load(const T* row, int e0, int D, float (&x
     }
   }
 }
+// The same as it is stored, and turned to fp32.
+template <typename T> struct RawSlot { u32x4 v[sizeof(T) / 2]; };
+template <bool kVec, typename T>
+__device__ __forceinline__ RawSlot<T> slot_raw(const T* row, int e0, int D) {
+  RawSlot<T> r;
+  if (kVec) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = e0 < D ? reinterpret_cast<const u32x4*>(row + e0)[i] : u32x4{0, 0, 0, 0};
+  } else {
+    float x[8];
+    slot_load<false>(row, e0, D, x);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.v[0][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.v[i >> 2][i & 3] = __float_as_uint(x[i]);
+    }
+  }
+  return r;
+}
+template <typename T> __device__ __forceinline__ void slot_floats(const RawSlot<T>& r, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t w = r.v[0][i >> 1];
+      x[i] = i & 1 ? bf16hi(w) : bf16lo(w);
+    } else {
+      const uint32_t w = r.v[i >> 2][i & 3];
+      x[i] = __uint_as_float(w);
+    }
+  }
+}
 template <bool kVec, typename T>
 __device__ __forceinline__ void slot_store(T* row, int e0, int D, const float (&x)[8]) {
   if (kVec) {
@@ -196,57 +229,81 @@ struct NormBwd {
 };
 
 // Each block walks over consecutive rows, its share of dw in registers; the block's rows at a
-// time are joined through LDS at its end.
+// time are joined through LDS at its end.  The next row's loads are on their way while a row is
+// summed (16384 rows of 2048 in bf16: 85 us without, 54 with, 268 MB: 5.0 TB/s).
 template <typename T, int kTpr, int kSlots, bool kVec>
 __global__ __launch_bounds__(norm_threads(kTpr)) void rms_norm_bwd_kernel(NormBwd a) {
   constexpr int kRows = norm_threads(kTpr) / kTpr;
+  constexpr bool kAhead = kTpr < 1024;           // (a block of 1024 has no registers for it, nor to keep w)
   __shared__ float red[2][norm_threads(kTpr) / 64];
   __shared__ float join[kRows > 1 ? kSlots * kTpr * 8 : 1];
   const int li = threadIdx.x % kTpr, sub = threadIdx.x / kTpr;
-  float w[kSlots][8], dw[kSlots][8];
+  RawSlot<T> w[kAhead ? kSlots : 1], hr[kSlots], yr[kSlots], zr[kSlots];
+  float dw[kSlots][8];
 #pragma unroll
   for (int s = 0; s < kSlots; ++s) {
-    slot_load<kVec>(static_cast<const T*>(a.w), 8 * (li + s * kTpr), a.D, w[s]);
+    if constexpr (kAhead) w[s] = slot_raw<kVec>(static_cast<const T*>(a.w), 8 * (li + s * kTpr), a.D);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[s][i] = 0.f;
   }
   const int64_t r0 = (int64_t)blockIdx.x * a.per * kRows + sub;
+  float rstd = 0.f;
+  auto load = [&](int64_t r) {                   // (past the last row that one again: no load under a condition)
+    r = r < a.rows ? r : a.rows - 1;
+    const T* hp = norm_row<T>(a.h, r, a.inner);
+    const T* yp = norm_row<T>(a.dy, r, a.inner);
+    const T* zp = norm_row<T>(a.dh.p ? a.dh : a.dy, r, a.inner);
+    rstd = a.rstd[r];
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      hr[s] = slot_raw<kVec>(hp, 8 * (li + s * kTpr), a.D);
+      yr[s] = slot_raw<kVec>(yp, 8 * (li + s * kTpr), a.D);
+      if (kAhead && a.dh.p) zr[s] = slot_raw<kVec>(zp, 8 * (li + s * kTpr), a.D);
+    }
+  };
+  if (kAhead) load(r0);
   for (int it = 0; it < a.per; ++it) {
     const int64_t r = r0 + (int64_t)it * kRows;
     if (r >= a.rows) break;                      // (all of a block of one row together)
-    const float rstd = a.rstd[r];
+    if (!kAhead) load(r);
+    const float rs = rstd;
     float h[kSlots][8], d[kSlots][8];
-    const T* hp = norm_row<T>(a.h, r, a.inner);
-    const T* dp = norm_row<T>(a.dy, r, a.inner);
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s) {
-      slot_load<kVec>(hp, 8 * (li + s * kTpr), a.D, h[s]);
-      slot_load<kVec>(dp, 8 * (li + s * kTpr), a.D, d[s]);
-    }
+    RawSlot<T> z[kAhead ? kSlots : 1];
     float c = 0.f;
 #pragma unroll
-    for (int s = 0; s < kSlots; ++s)
+    for (int s = 0; s < kSlots; ++s) {
+      float x[8];
+      slot_floats<T>(hr[s], h[s]);
+      slot_floats<T>(yr[s], d[s]);
+      if constexpr (kAhead) {
+        slot_floats<T>(w[s], x);
+        z[s] = zr[s];
+      } else {
+        slot_load<kVec>(static_cast<const T*>(a.w), 8 * (li + s * kTpr), a.D, x);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        h[s][i] *= rstd;
+        h[s][i] *= rs;
         dw[s][i] = __builtin_fmaf(d[s][i], h[s][i], dw[s][i]);
-        d[s][i] *= w[s][i];
+        d[s][i] *= x[i];
         c = __builtin_fmaf(d[s][i], h[s][i], c);
       }
+    }
+    if (kAhead) load(r + kRows);
     c = row_all<kTpr, false>(c, red[it & 1]) / (float)a.D;
     T* dx = static_cast<T*>(a.dx) + r * a.D;
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
-      const int e0 = 8 * (li + s * kTpr);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[s][i] = rstd * __builtin_fmaf(-h[s][i], c, d[s][i]);
+      for (int i = 0; i < 8; ++i) d[s][i] = rs * __builtin_fmaf(-h[s][i], c, d[s][i]);
       if (a.dh.p) {
-        float z[8];
-        slot_load<kVec>(norm_row<T>(a.dh, r, a.inner), e0, a.D, z);
+        float x[8];
+        if constexpr (kAhead) slot_floats<T>(z[s], x);
+        else slot_load<kVec>(norm_row<T>(a.dh, r, a.inner), 8 * (li + s * kTpr), a.D, x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[s][i] += z[i];
+        for (int i = 0; i < 8; ++i) d[s][i] += x[i];
       }
-      slot_store<kVec>(dx, e0, a.D, d[s]);
+      slot_store<kVec>(dx, 8 * (li + s * kTpr), a.D, d[s]);
     }
   }
   if constexpr (kRows > 1) {                     // sums in the order of the rows: the same on every run
@@ -279,19 +336,25 @@ __global__ __launch_bounds__(norm_threads(kTpr)) void rms_norm_bwd_kernel(NormBw
   }
 }
 
-// dw from the blocks' sums: 32 columns a block, 32 lanes' worth of parts side by side.
+// dw from the blocks' sums: 16 columns a block, 64 lanes' worth of parts side by side.
 template <typename T>
 __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* part, int blocks, int D, T* dw) {
-  __shared__ float s[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+  __shared__ float s[64][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, col = blockIdx.x * 16 + x;
   float v = 0.f;
-  if (col < D)
-    for (int b = y; b < blocks; b += 32) v += part[(int64_t)b * D + col];
-  s[y][threadIdx.x & 31] = v;
+  if (col < D) {
+#pragma unroll 8
+    for (int b = y; b < blocks; b += 64) v += part[(int64_t)b * D + col];
+  }
+  s[y][x] = v;
   __syncthreads();
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {             // the same order on every run
+    if (y < o) s[y][x] += s[y + o][x];
+    __syncthreads();
+  }
   if (y == 0 && col < D) {
-    v = 0.f;
-    for (int k = 0; k < 32; ++k) v += s[k][threadIdx.x];
+    v = s[0][x];
     if constexpr (sizeof(T) == 2) dw[col] = (T)f32_to_bf16_bits(v); else dw[col] = v;
   }
 }
@@ -303,25 +366,27 @@ namespace {
 
 constexpr int kNormMaxD = 32768;
 
-// Lanes and slots of a row of D.
+// Lanes and slots of a row of D, the same for any number of rows (so that a row's result does not
+// depend on them).  Rows of over 1024 take a block each: a wave with four slots was slower both
+// for one row of 2048 (4.0 us, by a block 2.4) and for 16384 (58 us, 53; backward 57, 54).
 struct NormShape { int tpr, slots; };
 NormShape norm_shape(int D) {
   if (D <= 128) return {16, 1};
   if (D <= 512) return {64, 1};
   if (D <= 1024) return {64, 2};
-  if (D <= 2048) return {64, 4};
+  if (D <= 2048) return {256, 1};
   if (D <= 4096) return {256, 2};
   if (D <= 8192) return {256, 4};
-  return {1024, 4};
+  return {1024, D <= 16384 ? 2 : 4};
 }
 
 template <typename F>
 int with_shape(const NormShape& s, F&& f) {
   if (s.tpr == 16) return f.template operator()<16, 1>();
-  if (s.tpr == 64) return s.slots == 1 ? f.template operator()<64, 1>()
-                        : s.slots == 2 ? f.template operator()<64, 2>() : f.template operator()<64, 4>();
-  if (s.tpr == 256) return s.slots == 2 ? f.template operator()<256, 2>() : f.template operator()<256, 4>();
-  return f.template operator()<1024, 4>();
+  if (s.tpr == 64) return s.slots == 1 ? f.template operator()<64, 1>() : f.template operator()<64, 2>();
+  if (s.tpr == 256) return s.slots == 1 ? f.template operator()<256, 1>()
+                         : s.slots == 2 ? f.template operator()<256, 2>() : f.template operator()<256, 4>();
+  return s.slots == 2 ? f.template operator()<1024, 2>() : f.template operator()<1024, 4>();
 }
 
 int norm_check(int64_t rows, int inner, int D, int dtype) {
@@ -385,7 +450,7 @@ int norm_backward(gsa::NormBwd a, void* dw, bool vec, hipStream_t stream) {
     return launch_status();
   });
   if (e) return e;
-  hipLaunchKernelGGL(gsa::rms_norm_dw_kernel<T>, dim3((a.D + 31) / 32), dim3(1024), 0, stream, a.part, blocks, a.D,
+  hipLaunchKernelGGL(gsa::rms_norm_dw_kernel<T>, dim3((a.D + 15) / 16), dim3(1024), 0, stream, a.part, blocks, a.D,
                      static_cast<T*>(dw));
   return launch_status();
 }
