@@ -447,14 +447,18 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// The state from chunk to chunk.  A wave owns 16 NT columns of one head's state in NT tiles of 16,
+// The state from chunk to chunk.  A wave owns 16 columns of one head's state in 8 tiles of 16,
 // tile 2 ks + e of its registers the rows tile_row(2 ks + e, .); a block has W waves.  The chunk's
 // operands come to LDS by direct loads.  Three shapes (Shape), by how many heads and sequences
 // there are to fill the chip:
-//   <2, 4, one buffer>: a head a block; two blocks share a CU and cover each other's waits, each
+//   <8, one buffer>: a head a block; two blocks share a CU and cover each other's waits, each
 //     buffer is refilled as soon as all waves are through with it
-//   <1, 4> and <1, 2>, two buffers: 64 and 32 columns a block, one block a CU; the next
-//     chunk's operands are on their way during the whole of this one's products
+//   <8, two buffers> and <4, two buffers>: a head and half a head a block, one block a CU; the
+//     next chunk's operands are on their way during the whole of this one's products
+// Bound by the issue of instructions, the matrix ones and the splits of fp32 into bf16 parts, which
+// do not overlap within a SIMD; a quarter of the cycles wait (loads of V and the barriers).  A
+// chunk of 64 takes 4.1 us by half heads, 5.9 by whole ones (8 on a full chip), 15 where two blocks
+// share a CU.
 // ---------------------------------------------------------------------------
 // Blocks go to the 8 XCDs in turn, each with an L2 of its own: the kBlocks blocks of one head stand 8
 // apart, so that they share one.  The unit (head and sequence or segment) and block of a block
@@ -464,10 +468,10 @@ template <int kBlocks> __device__ __forceinline__ int2 unit_of(int b) {
 }
 constexpr int64_t blocks_for(int64_t units, int blocks) { return blocks == 1 ? units : (units + 7) / 8 * 8 * blocks; }
 
-template <int NT_, int W_, bool kDouble_, int kWaves_ = 2> struct Shape {
-  static constexpr int NT = NT_, W = W_, kCols = 16 * NT_ * W_, kBlocks = kHead / kCols;     // columns of a block, blocks of a head
+template <int W_, bool kDouble_, int kWaves_ = 2> struct Shape {
+  static constexpr int NT = 1, W = W_, kCols = 16 * NT * W_, kBlocks = kHead / kCols;     // columns of a block, blocks of a head
   static constexpr bool kDouble = kDouble_;
-  static constexpr int kWaves = kWaves_;                     // of a SIMD
+  static constexpr int kWaves = kWaves_;                     // of a SIMD (a head by 4 waves of 2 tiles was slower)
 };
 
 template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
@@ -1651,18 +1655,19 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
     z.slots = 0;
     return z;
   }
-  // Which shape, and segments or not, in us a chunk of all heads (bf16 forward, 16384 tokens of 16 heads and
-  // alike): heads in one piece by 64 columns 6.5 while their blocks fit the chip, whole heads 9.3
-  // at one block a CU and 15 at two; segments cost 0.07 a head and chunk, both passes together.
-  // So segments for few heads (64 heads, T = 4096: 376 us against 415), and blocks of
-  // 64 columns up to 128 heads; packed sequences differ in length, and up to 384 the longest one's
-  // pace decides (23 of 12289 tokens, 16 heads: 244 against 271).
+  // Blocks of 64 columns while the longest of the pieces decides, whole heads when the chip is full.  Measured for the
+  // whole call, bf16, forward / forward and backward, us:
+  //   1024 tokens of 128 heads 109 / 486 by 64 columns, 134 / 544 by heads; of 160 heads 181 / 750 and 141 / 635
+  //   packed (sequences differ in length), 23 of 12289 tokens, 16 heads: 243 and 271; 7 of 6001: - / 632 and 751
   const int64_t heads = (int64_t)N * Hv;
-  z.columns = heads <= 32 ? 32 : heads <= (packed ? 384 : 128) ? 64 : 128;
+  z.columns = heads <= (packed ? 384 : 128) ? 64 : 128;
   const int64_t length = packed ? nc / N : nc;               // of one sequence
-  if (heads <= 88 && length >= 12) {
-    // a block a CU (T = 16384 of 16 heads: 16 segments 358 us, 32 373); joining costs 1.9 us a segment and the two
-    // passes 16 us a chunk of one: more than sqrt(8 chunks) segments lose
+  // Segments cost two passes over them and the join, and pay for few heads and long sequences:
+  //   16 heads of 512 tokens 46 / 143 in one piece, 60 / 175 by segments; 768: 62 / 187 and 64 / 185; 1024: 78 / 231 and 69 / 195
+  //   64 heads of 1024 tokens 88 / 312 and 100 / 330; 2048: 169 / 627 and 165 / 586; 80 heads of 4096: 377 / 1460 and 406 / 1418
+  if (heads <= 64 && length >= std::max<int64_t>(12, heads / 2 - 4)) {
+    // a block a CU, of at least 4 chunks (16384 tokens of 16 heads: 16 segments 358 us, 32 373); joining costs 1.9 us a
+    // segment and the two passes 16 us a chunk of one: more than sqrt(8 chunks) segments lose
     int64_t pieces = 256 / heads;
     while (pieces > 3 && pieces * pieces > 8 * length) --pieces;
     const int64_t seg = std::max<int64_t>(4, (length + pieces - 1) / pieces);
@@ -1690,10 +1695,9 @@ template <auto kKernel> int allow_lds(size_t bytes) {
   return GSA_OK;
 }
 
-using Heads = gsa::Shape<1, 8, false, 4>;
-using HeadsAlone = gsa::Shape<1, 8, true>;
-using Columns64 = gsa::Shape<1, 4, true>;
-using Columns32 = gsa::Shape<1, 2, true>;
+using Heads = gsa::Shape<8, false, 4>;
+using HeadsAlone = gsa::Shape<8, true>;
+using Columns64 = gsa::Shape<4, true>;
 
 template <typename T, bool kOut, typename Sh> int launch_scan(const gsa::DeltaArgs& a, int passes, hipStream_t s) {
   using L = gsa::ScanLds<T, Sh>;
@@ -1737,7 +1741,6 @@ template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSiz
     if (const int e = launch_join<false>(a, z, s)) return e;
     return a.units <= 256 ? launch_scan<T, true, HeadsAlone>(a, 1, s) : launch_scan<T, true, Heads>(a, 1, s);
   }
-  if (z.columns == 32) return launch_scan<T, true, Columns32>(a, 1, s);
   if (z.columns == 64) return launch_scan<T, true, Columns64>(a, 1, s);
   return a.units <= 256 ? launch_scan<T, true, HeadsAlone>(a, 1, s) : launch_scan<T, true, Heads>(a, 1, s);
 }
@@ -1749,8 +1752,6 @@ template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSi
     if ((e = launch_scan_bwd<T, false, Heads>(a, s))) return e;
     if ((e = launch_join<true>(a, z, s))) return e;
     e = a.units <= 256 ? launch_scan_bwd<T, true, HeadsAlone>(a, s) : launch_scan_bwd<T, true, Heads>(a, s);
-  } else if (z.columns == 32) {
-    e = launch_scan_bwd<T, true, Columns32>(a, s);
   } else if (z.columns == 64) {
     e = launch_scan_bwd<T, true, Columns64>(a, s);
   } else {
