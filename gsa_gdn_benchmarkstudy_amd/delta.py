@@ -19,6 +19,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version as _increment_version
 
 from . import _abi
 from .roctx import range_pop as _range_pop, range_push as _range_push
@@ -126,7 +127,11 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
 
     Differentiable in q, k, v, g, beta and initial_state (once); the gradients are the same
     bits on every run.  A forward that needs gradients keeps 1.5 KiB (bf16; fp32: 2.5 KiB) a
-    token and v head.
+    token and v head, and where it works by segments up to 0.25 KiB (0.5 KiB) more.
+
+    May be captured into a graph, forward and backward, after one call outside of it; as with any
+    backward pass no eager graph of the same leaves may live then (capture torch.autograd.grad, or
+    use leaves of the graph's own).
     """
     _check(2, q, k, v, g, beta)
     B, T, Hv, d = v.shape
@@ -171,7 +176,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     [slots,Hv,128,128] fp32, each matrix contiguous.  state_indices (int32 or int64 [N], on
     the device): the state of each row; row n has state n without it.  A row whose index is
     outside [0, slots) is padding: its output is 0 and no state changes.  Rows with the same
-    index are consecutive tokens of one sequence, in the batch's order.
+    index are consecutive tokens of one sequence, in the batch's order.  At most 65535 rows.
 
     Forward only: it raises where a gradient would be needed.
     """
@@ -182,8 +187,12 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     s0, s1, s2, s3 = state.stride()
     if s2 != d or s3 != 1 or (s0 | s1) % 4 or state.data_ptr() % 16:
         raise ValueError("state is updated in place: its matrices must be contiguous and 16-byte aligned")
-    if state.shape[0] > 1 and s0 < d * d or Hv > 1 and s1 < d * d:
-        raise ValueError("state is updated in place: its matrices overlap")
+    extent = d * d
+    for stride, n in sorted(((s0, state.shape[0]), (s1, Hv))):
+        if n > 1:
+            if stride < extent:
+                raise ValueError("state is updated in place: its matrices overlap")
+            extent += (n - 1) * stride
     if state_indices is not None:
         if tuple(state_indices.shape) != (N,) or state_indices.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"state_indices: int32 or int64 [{N}]")
@@ -197,6 +206,9 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
             return v.new_zeros(v.shape)
         _range_push("gsa_hip/delta_step")
         try:
-            return _abi.delta_step(q, k, v, g, beta, state, state_indices, d ** -0.5 if scale is None else float(scale))
+            o = _abi.delta_step(q, k, v, g, beta, state, state_indices, d ** -0.5 if scale is None else float(scale))
+            if not state.is_inference():
+                _increment_version(state)        # a graph that kept the old state must not use the new one
+            return o
         finally:
             _range_pop()

@@ -56,11 +56,20 @@ def _step(N=3, Hk=1, Hv=2, slots=4, **kw):
     (ValueError, dict(state=torch.zeros(4, 1, D, D))), (ValueError, dict(state=torch.zeros(4, 2, D, D, dtype=torch.bfloat16))),
     (ValueError, dict(state=torch.zeros(4, 2, D, D).transpose(2, 3))), (ValueError, dict(state=torch.zeros(1, 2, D, D).expand(4, 2, D, D))),
     (ValueError, dict(state=torch.zeros(4 * 2 * D * D + 1)[1:].view(4, 2, D, D))),
+    (ValueError, dict(state=torch.zeros(5 * D * D).as_strided((4, 2, D, D), (D * D, D * D, D, 1)))),
+    (ValueError, dict(state=torch.zeros(9 * D * D).as_strided((4, 2, D, D), (D * D, 3 * D * D, D, 1)))),
     (ValueError, dict(state_indices=torch.zeros(2, dtype=torch.int32))), (ValueError, dict(state_indices=torch.zeros(3))),
     (RuntimeError, dict(v=torch.zeros(3, 2, D, requires_grad=True))), (RuntimeError, {})])
 def test_step_refuses(error, kw):
     with pytest.raises(error):
         gated_delta_step(**_step(**kw))
+
+
+def test_step_takes_states_laid_out_by_head():
+    """A pool [Hv, slots] seen as [slots, Hv] passes the checks (and ends at the one for a GPU)."""
+    for pool in (torch.zeros(2, 4, D, D).transpose(0, 1), torch.zeros(4, 3, D, D)[:, :2], torch.zeros(1, 2, D, D).expand(1, 2, D, D)):
+        with pytest.raises(RuntimeError, match="GPU|cuda|CUDA|device"):
+            gated_delta_step(**_step(N=1, slots=pool.shape[0], state=pool))
 
 
 @pytest.mark.parametrize("op", [add_rms_norm, add_rms_norm_fp8])

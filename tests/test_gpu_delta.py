@@ -412,3 +412,212 @@ def test_prefill_then_decode(dev):
     ref = _oracle({n: t.cpu() for n, t in every.items()}, [(b, 0, T + new) for b in range(B)])
     _check(torch.cat(outs, 1), ref[0], T + new, 16, "o")
     _check(S, ref[1], T + new, 16, "state")
+
+
+# --------------------------------------------------------------------------- calls as programs make them
+
+def _leaves(x, dev):
+    return [x[n].to(dev).requires_grad_(True) for n in NAMES]
+
+
+def _train(leaf, do, cu=None):
+    o, S = gated_delta_rule(*leaf, output_final_state=True, cu_seqlens=cu)
+    return (o, S) + torch.autograd.grad([o, S], leaf, [do, torch.ones_like(S)])
+
+
+@pytest.mark.parametrize("T,Hk,Hv,offsets", [(130, 2, 2, None), (1500, 1, 2, None), (900, 2, 4, [0, 1, 64, 64, 700, 850])])
+def test_captured_training(dev, T, Hk, Hv, offsets):
+    """Forward and backward in a graph (in one piece, by segments, packed with rows outside), replayed
+    on new inputs with eager calls in between: the eager call's bits."""
+    leaf = _leaves(_inputs(1, T, Hk, Hv, torch.bfloat16, seed=81), dev)
+    do = torch.randn(1, T, Hv, D, device=dev, dtype=torch.bfloat16)
+    cu = None if offsets is None else torch.tensor(offsets, device=dev, dtype=torch.int32)
+    s = torch.cuda.Stream(device=dev)
+    s.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(s):
+        _train(leaf, do, cu)
+    torch.cuda.current_stream(dev).wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = _train(leaf, do, cu)
+    for i in range(4):
+        new = _inputs(1, T, Hk, Hv, torch.bfloat16, seed=90 + i)
+        with torch.no_grad():
+            for t, n in zip(leaf, NAMES):
+                t.copy_(new[n])
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, _train(_leaves(new, dev), do, cu)):
+            assert torch.equal(a, b)
+
+
+def test_two_graphs_at_once(dev):
+    """Two graphs with a memory pool each, replayed on two streams at the same time."""
+    graphs, outs, ins, want = [], [], [], []
+    with torch.no_grad():
+        for i in range(2):
+            x = {n: t.to(dev) for n, t in _inputs(1, 3000, 2, 4, torch.bfloat16, seed=100 + i).items()}
+            want.append(gated_delta_rule(*(x[n] for n in NAMES), output_final_state=True))
+            ins.append(x)
+        torch.cuda.synchronize()
+        for x in ins:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                outs.append(gated_delta_rule(*(x[n] for n in NAMES), output_final_state=True))
+        streams = [torch.cuda.Stream(device=dev) for _ in graphs]
+        for _ in range(3):
+            for o, S in outs:
+                o.zero_(), S.zero_()
+            torch.cuda.synchronize()
+            for s, graph in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    graph.replay()
+            torch.cuda.synchronize()
+            for (o, S), (o2, S2) in zip(outs, want):
+                assert torch.equal(o, o2) and torch.equal(S, S2)
+
+
+def test_two_threads(dev):
+    """Training calls from two threads, each on a stream of its own, at the same time."""
+    import threading
+
+    jobs, failed = [], []
+    for i in range(2):
+        x = _inputs(1, 700 + 900 * i, 1, 2, torch.bfloat16, seed=110 + i)
+        do = torch.randn(x["v"].shape, generator=torch.Generator().manual_seed(i)).to(dev, torch.bfloat16)
+        jobs.append((x, do, _train(_leaves(x, dev), do)))
+    torch.cuda.synchronize()
+
+    def work(x, do, want):
+        try:
+            s = torch.cuda.Stream(device=dev)
+            with torch.cuda.stream(s):
+                for _ in range(6):
+                    got = _train(_leaves(x, dev), do)
+                    s.synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
+def test_nothing_to_do(dev):
+    """No tokens, no sequences' tokens, no rows."""
+    z = dict(device=dev, dtype=torch.bfloat16)
+    S0 = torch.randn(2, 2, D, D, device=dev)
+    x = [torch.zeros(2, 0, 1, D, **z), torch.zeros(2, 0, 1, D, **z), torch.zeros(2, 0, 2, D, **z), torch.zeros(2, 0, 2, device=dev),
+         torch.zeros(2, 0, 2, device=dev)]
+    o, S = gated_delta_rule(*x, initial_state=S0, output_final_state=True)
+    assert o.shape == x[2].shape and torch.equal(S, S0) and S.data_ptr() != S0.data_ptr()
+    x = {n: t.to(dev) for n, t in _inputs(1, 70, 1, 2, torch.bfloat16, seed=5).items()}
+    cu = torch.zeros(3, device=dev, dtype=torch.int64)
+    leaf = [t.requires_grad_(True) for t in x.values()]
+    st = S0.clone().requires_grad_(True)
+    o, S = gated_delta_rule(*leaf, initial_state=st, output_final_state=True, cu_seqlens=cu)
+    assert not o.any() and torch.equal(S, S0)
+    d = torch.autograd.grad([o, S], leaf + [st], [torch.ones_like(o), S0])
+    assert not any(t.any() for t in d[:-1]) and torch.equal(d[-1], S0)
+    e = [torch.zeros(0, 1, D, **z), torch.zeros(0, 1, D, **z), torch.zeros(0, 2, D, **z), torch.zeros(0, 2, device=dev),
+         torch.zeros(0, 2, device=dev)]
+    keep = S0.clone()
+    assert gated_delta_step(*e, S0).shape == (0, 2, D) and torch.equal(S0, keep)
+
+
+def test_same_tensor_in_several_places(dev):
+    """q, k and v one leaf: its gradient is the sum of theirs."""
+    x = _inputs(1, 200, 2, 2, torch.float32, seed=120)
+    one = x["k"].to(dev)
+    g, b = x["g"].to(dev), x["beta"].to(dev)
+    do = torch.randn(1, 200, 2, D, device=dev)
+    leaf = one.clone().requires_grad_(True)
+    got, = torch.autograd.grad(gated_delta_rule(leaf, leaf, leaf, g, b)[0], leaf, do)
+    three = [one.clone().requires_grad_(True) for _ in range(3)]
+    parts = torch.autograd.grad(gated_delta_rule(*three, g, b)[0], three, do)
+    # three fp32 addends in another order: two roundings of at most their sum of magnitudes
+    tol = 2 * 2.0 ** -24 * sum(p.abs() for p in parts)
+    assert bool(((got - sum(parts)).abs() <= tol + 2.0 ** -24 * got.abs()).all())
+
+
+def test_tokens_far_apart(dev):
+    """Tokens 32 MiB and more apart (a view of a large buffer) are copied, not refused."""
+    x = _inputs(1, 3, 1, 1, torch.bfloat16, seed=130)
+    far = torch.empty(3 * (1 << 24), device=dev, dtype=torch.bfloat16).as_strided((1, 3, 1, D), (1, 1 << 24, D, 1))
+    far.copy_(x["k"])
+    y = {n: t.to(dev) for n, t in x.items()}
+    o, S = gated_delta_rule(y["q"], far, y["v"], y["g"], y["beta"], output_final_state=True)
+    o2, S2 = gated_delta_rule(*(y[n] for n in NAMES), output_final_state=True)
+    assert torch.equal(o, o2) and torch.equal(S, S2)
+
+
+def test_offsets_past_32_bits(dev):
+    """2**19 tokens of 16 heads: elements of the kept states, and bytes of every input, past 2**31.  The last
+    tokens' outputs and gradients are those of a call on them alone from the state before them; the first
+    tokens' gradients those of a call on the first 4096 (a decay of e^-0.1 a token leaves
+    e^-380 of what lies behind)."""
+    T, Hk, Hv, tail = (1 << 19) + 100, 8, 16, 612
+    gen = torch.Generator(device=dev).manual_seed(7)
+
+    def rn(*s):
+        return torch.randn(*s, generator=gen, device=dev, dtype=torch.bfloat16)
+
+    x = dict(q=rn(1, T, Hk, D), k=rn(1, T, Hk, D).mul_(D ** -0.5), v=rn(1, T, Hv, D))
+    x.update(g=torch.full((1, T, Hv), -0.1, device=dev), beta=torch.full((1, T, Hv), 0.5, device=dev))
+    do = rn(1, T, Hv, D)
+
+    def run(a, b, state=None):
+        leaf = [x[n][:, a:b].requires_grad_(True) if n in ("q", "k", "v") else x[n][:, a:b].clone().requires_grad_(True) for n in NAMES]
+        o, S = gated_delta_rule(*leaf, initial_state=state, output_final_state=True)
+        return o.detach(), S.detach(), torch.autograd.grad(o, leaf, do[:, a:b])
+
+    whole = run(0, T)
+    with torch.no_grad():
+        _, S = gated_delta_rule(*(x[n][:, :T - tail] for n in NAMES), output_final_state=True)
+    last = run(T - tail, T, S)
+    first = run(0, 4096)
+
+    def near(a, b, name):
+        # both sides err by fp32 roundings of sums that the decay keeps to some 10 tokens, and round to their type
+        scale = b.abs().max().float()
+        tol = 2 * torch.finfo(a.dtype).eps / 2 * b.float().abs() + 64 * (64 + 128) * 2.0 ** -24 * scale
+        assert bool(((a.float() - b.float()).abs() <= tol).all()), name
+
+    near(whole[0][:, -tail:], last[0], "o")
+    near(whole[1], last[1], "state")
+    for n, a, b, c in zip(NAMES, whole[2], last[2], first[2]):
+        near(a[:, -tail:], b, "d" + n + " at the end")
+        near(a[:, :256], c[:, :256], "d" + n + " at the start")
+
+
+def test_step_in_a_large_pool(dev):
+    """States more than 2**31 elements behind the first."""
+    slots, Hv = 8200, 16
+    pool = torch.zeros(slots, Hv, D, D, device=dev)
+    x = {n: t[0].to(dev) for n, t in _inputs(1, 3, 8, Hv, torch.bfloat16, seed=140).items()}
+    small = torch.randn(3, Hv, D, D, generator=torch.Generator().manual_seed(3)).to(dev)
+    at = torch.tensor([slots - 1, 0, 8195], device=dev)
+    pool[at] = small
+    o = gated_delta_step(*(x[n] for n in NAMES), pool, at)
+    o2 = gated_delta_step(*(x[n] for n in NAMES), small)
+    assert torch.equal(o, o2) and torch.equal(pool[at], small)
+    pool[at] = 0
+    assert not pool.any()
+
+
+def test_step_counts_as_a_change_of_the_state(dev):
+    """A graph that kept the state refuses its backward pass after a step has written to it."""
+    x = {n: t[:, 0].to(dev) for n, t in _inputs(1, 1, 1, 1, torch.bfloat16, seed=150).items()}
+    state = torch.randn(1, 1, D, D, device=dev)
+    w = torch.ones_like(state).requires_grad_(True)
+    y = (state * w).sum()
+    with torch.no_grad():
+        gated_delta_step(*(x[n] for n in NAMES), state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        gated_delta_step(*(x[n] for n in NAMES), torch.zeros(1, 1, D, D, device=dev))

@@ -181,3 +181,44 @@ def test_captured(dev):
         y, h = add_rms_norm(d[0], d[1], residual=d[2])
         for a, b in zip(got, (y, h) + torch.autograd.grad(y, d, dy)):
             assert torch.equal(a, b)
+
+
+def test_no_rows(dev):
+    x, w = torch.zeros(3, 0, 64, device=dev), torch.ones(64, device=dev)
+    y, h = add_rms_norm(x, w, residual=x)
+    assert y.shape == h.shape == x.shape
+    y, scale, h = add_rms_norm_fp8(x, w)
+    assert y.shape == x.shape and scale.shape == (3, 0) and y.dtype == torch.float8_e4m3fn
+
+
+def test_gradients_that_are_broadcast(dev):
+    """Gradients with strides of 0 (of a sum, of a mean over rows), and of a norm of a transposed x."""
+    x, _, w = _make((4, 6, 96), torch.float32, False, 21)
+    grads = []
+    for at in (dev, "cpu"):
+        a, b = x.to(at).requires_grad_(True), w.to(at).requires_grad_(True)
+        at_t = a.transpose(0, 1)
+        y = add_rms_norm(at_t, b, eps=EPS)[0] if at == dev else torch.nn.functional.rms_norm(at_t.double(), (96,), b.double(), EPS)
+        grads.append(torch.autograd.grad(y.sum() + y.mean(0).sum(), (a, b)))
+    for got, ref in zip(*grads):
+        # rows of 96 and 24 rows: sums of 96 and 24 fp32 terms, a few roundings each; ref itself rounds once to fp32
+        assert bool(((got.cpu() - ref).abs() <= (96 + 24 + 16) * 2.0 ** -24 * max(1.0, float(ref.abs().max()))).all())
+
+
+def test_two_streams(dev):
+    """Forward and backward on two streams at once, after the work that makes their inputs."""
+    x, res, w = (t.to(dev) for t in _make((6000, 1024), torch.bfloat16, True, 31))
+
+    def train():
+        leaf = [t.detach().clone().requires_grad_(True) for t in (x, w, res)]
+        y, h = add_rms_norm(leaf[0], leaf[1], residual=leaf[2])
+        return (y, h) + torch.autograd.grad([y, h], leaf, [x, res])
+
+    want, got, streams = train(), [], [torch.cuda.Stream(device=dev) for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(s):
+            got.append(train())
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
