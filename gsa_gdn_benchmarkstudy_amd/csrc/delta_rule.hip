@@ -493,8 +493,8 @@ __device__ __forceinline__ void fetch_rows(const Rows& x, const Span& sp, int64_
   const uint16_t* p = uniform(row_at<uint16_t>(x, sp, t0, h));
   const int m = (l - 4 * (l >> 4)) & 15;                     // (row_slot)
 #pragma unroll
-  for (int f = wave; f < C / 4; f += W) {
-    const int t = min(tile_row(f >> 2, m), left - 1);
+  for (int i = 0; i < C / 4 / W; ++i) {
+    const int f = wave + W * i, t = min(tile_row(f >> 2, m), left - 1);
     load_lds16(p, (uint32_t)(t * (int)x.st + 32 * (f & 3) + 8 * (l >> 4)) * 2u, __builtin_amdgcn_readfirstlane(lds + f * kUnit));
   }
 }
@@ -1212,10 +1212,17 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   const int64_t tok = (int64_t)sp.b * a.s.T + sp.t0 + t0;    // row of [B * T]
   const int64_t at = (int64_t)slot * a.Hv + h, atk = (int64_t)slot * a.Hk + hk;
 
+  // a lane whose offsets the compiler computes where they are used, instead of keeping (and spilling) them
+  auto here = [&]() {
+    int x = l;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
   auto fetch_kq = [&]() {
     if constexpr (NP == 1) {
-      fetch_rows<C, 4>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l);
-      fetch_rows<C, 4>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l);
+      const int l_ = here();
+      fetch_rows<C, 4>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l_);
+      fetch_rows<C, 4>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l_);
     } else {
       fetch<4>(a.kr + atk * L::kRows, lds_addr(bk), L::kRows / kUnit, wave, l);
       fetch<4>(a.qr + atk * L::kRows, lds_addr(bq), L::kRows / kUnit, wave, l);
@@ -1228,10 +1235,11 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   char* bs = bk + wave * 8 * kUnit;
   auto turn = [](int r) { return (r >> 1 & 1) | (r >> 3 & 1) << 1 | (r >> 4 & 1) << 2; };
   auto fetch_states = [&](int ks) {
+    const int l_ = here();
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int r = 8 * u + (l >> 3);
-      const uint32_t o = 4 * (r * kHead + 32 * ks) + 16 * ((l & 7) ^ turn(r));
+      const int r = 8 * u + (l_ >> 3);
+      const uint32_t o = 4 * (r * kHead + 32 * ks) + 16 * ((l_ & 7) ^ turn(r));
       load_lds16(s0p, o, __builtin_amdgcn_readfirstlane(lds_addr(bs) + u * kUnit));
       load_lds16(s1p, o, __builtin_amdgcn_readfirstlane(lds_addr(bs) + (4 + u) * kUnit));
     }
@@ -1240,25 +1248,29 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   {
     // a thread's 8 elements of each 32: token tid / 4
     const int st = tid >> 2, so = tid & 3;
-    const bool mine = st < C, there = mine && st < left;
-    const float* up = a.u + (at * C + st) * kHead + 8 * so;
-    const float* rp = a.dr + (at * C + st) * kHead + 8 * so;
-    const T* op = row_at<T>(a.dout, sp, t0 + st, h) + 8 * so;
-    const T* vp = row_at<T>(a.v, sp, t0 + st, h) + 8 * so;
-    float xu[8], xr[8], dot_v = 0.f;
-    u32x4 xo[sizeof(T) / 2], xv[sizeof(T) / 2];              // 8 elements as they are
+    const bool mine = 4 * C == 256 || st < C, there = st < left;
+    // uniform rows and one offset a thread (whole addresses were spilled, and what reads them back waits for every
+    // load in flight); rows that are not there: the last one
+    const char* up = reinterpret_cast<const char*>(uniform(a.u + at * C * kHead));
+    const char* rp = reinterpret_cast<const char*>(uniform(a.dr + at * C * kHead));
+    const char* op = reinterpret_cast<const char*>(uniform(row_at<T>(a.dout, sp, t0, h)));
+    const char* vp = reinterpret_cast<const char*>(uniform(row_at<T>(a.v, sp, t0, h)));
+    const int last = min(st, left - 1);
+    const uint32_t uo = 4 * (min(st, C - 1) * kHead + 8 * so);
+    const uint32_t oo = sizeof(T) * ((uint32_t)last * (uint32_t)a.dout.st + 8 * so);
+    const uint32_t vo = sizeof(T) * ((uint32_t)last * (uint32_t)a.v.st + 8 * so);
+    float dot_v = 0.f;
+    u32x4 xu[2], xr[2], xo[sizeof(T) / 2], xv[sizeof(T) / 2];   // 8 elements as they are
     auto load = [&](int ks) {
-      if (mine) {
-        load8(up + 32 * ks, xu);
-        load8(rp + 32 * ks, xr);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        xu[i] = *reinterpret_cast<const u32x4*>(up + 128 * ks + 16 * i + uo);
+        xr[i] = *reinterpret_cast<const u32x4*>(rp + 128 * ks + 16 * i + uo);
       }
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-        xo[i] = xv[i] = u32x4{0, 0, 0, 0};
-        if (there) {
-          xo[i] = reinterpret_cast<const u32x4*>(op + 32 * ks)[i];
-          xv[i] = reinterpret_cast<const u32x4*>(vp + 32 * ks)[i];
-        }
+        xo[i] = *reinterpret_cast<const u32x4*>(op + 32 * sizeof(T) * ks + 16 * i + oo);
+        xv[i] = *reinterpret_cast<const u32x4*>(vp + 32 * sizeof(T) * ks + 16 * i + vo);
       }
     };
     auto floats = [](const u32x4* x, float (&y)[8]) {
@@ -1272,11 +1284,17 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
       if (!mine) return;
       bf16x8* to = stage + 16 * so + (st & 15);
       const int tile = st >> 4;
-      float fo[8], fv[8];
+      float fo[8], fv[8], fu[8], fr[8];
       floats(xo, fo);
       floats(xv, fv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        fo[i] = there ? fo[i] : 0.f;
+        fu[i] = __uint_as_float(xu[i >> 2][i & 3]);
+        fr[i] = __uint_as_float(xr[i >> 2][i & 3]);
+      }
       const Parts<NP> o = parts_of<NP>(fo);
-      const Parts<3> u = split3(xu), r = split3(xr);
+      const Parts<3> u = split3(fu), r = split3(fr);
 #pragma unroll
       for (int i = 0; i < NP; ++i) to[(tile * NP + i) * 64] = o.p[i];
 #pragma unroll
@@ -1284,7 +1302,7 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
 #pragma unroll
       for (int i = 0; i < 3; ++i) to[(MT * (NP + 3) + tile * 3 + i) * 64] = r.p[i];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) dot_v = __builtin_fmaf(xr[i], fv[i], dot_v);
+      for (int i = 0; i < 8; ++i) dot_v = __builtin_fmaf(fr[i], fv[i], dot_v);
     };
     load(0);
     for (int i = tid; i < 5 * C; i += 256) gates[i] = i < 3 * C ? a.gates[at * 256 + i] : a.sums[at * 2 * C + i - 3 * C];
@@ -1317,7 +1335,6 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
       put();
       if (ks < 3) fetch_states(ks + 1); else fetch_kq();
       __syncthreads();
-      if (ks < 3) load(ks + 1);
       const bf16x8* so_ = stage;
       const bf16x8* su_ = so_ + MT * NP * 64;
       const bf16x8* sr_ = su_ + MT * 3 * 64;
@@ -1341,6 +1358,7 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
         }
       }
       __builtin_amdgcn_sched_barrier(0);                     // (fewer operands in registers at a time)
+      load(ks < 3 ? ks + 1 : 3);                             // (a load under a condition would be waited for at its end)
 #pragma unroll
       for (int e = 0; e < 2; ++e) sx[e] = split3(z[e]);
 #pragma unroll
@@ -1366,15 +1384,28 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
     if (mine && so == 0) db[st] = dot_v;
     dot = wave_sum(dot);
     if (l == 0) cross[wave] = (float)dot;
+    // rows 16 tile + m of the tokens: where tile_row has them
+    auto natural = [&](const char* src, int tile, int ks) {
+      const int tk = 16 * tile + m, x = 2 * (tk >> 5) + ((tk >> 2) & 1), y = 4 * ((tk >> 3) & 3) + (tk & 3);
+      return staged<NP>(reinterpret_cast<const bf16x8*>(src), x * 4 + ks, row_slot(g, y));
+    };
+    wait_loads();
+    __syncthreads();                                         // K and Q are there
     floatx4 dq[2][MT], dk[2][MT];                            // [128 elements: tile 2 wave + e][tokens]
 #pragma unroll
     for (int n = 0; n < MT; ++n) {
       const int t = 16 * n + m;
       const float e = gates[t], rest = gates[C + t], beta = gates[2 * C + t];
-      float q[8] = {0, 0, 0, 0, 0, 0, 0, 0}, k[8] = {0, 0, 0, 0, 0, 0, 0, 0}, x1 = 0.f, x2 = 0.f, x3 = 0.f;
-      if (t < left) {
-        load8(row_at<T>(a.q, sp, t0 + t, hk) + 32 * wave + 8 * g, q);
-        load8(row_at<T>(a.k, sp, t0 + t, hk) + 32 * wave + 8 * g, k);
+      float q[8], k[8], x1 = 0.f, x2 = 0.f, x3 = 0.f;
+      const Parts<NP> qp = natural(bq, n, wave), kp = natural(bk, n, wave);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        q[i] = k[i] = 0.f;
+#pragma unroll
+        for (int j = NP - 1; j >= 0; --j) {                  // (the parts' sum: exactly the element)
+          q[i] += (float)qp.p[j][i];
+          k[i] += (float)kp.p[j][i];
+        }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -1389,14 +1420,12 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
       x2 += __shfl_xor(x2, 16, 64); x2 += __shfl_xor(x2, 32, 64);
       x3 += __shfl_xor(x3, 16, 64); x3 += __shfl_xor(x3, 32, 64);
       if (g == 0) {
-        red[(wave * 3 + 0) * C + t] = x1;
-        red[(wave * 3 + 1) * C + t] = x2;
-        red[(wave * 3 + 2) * C + t] = x3;
+        red[(wave * 3 + 0) * C + t] = t < left ? x1 : 0.f;
+        red[(wave * 3 + 1) * C + t] = t < left ? x2 : 0.f;
+        red[(wave * 3 + 2) * C + t] = t < left ? x3 : 0.f;
       }
     }
     for (int i = tid; i < MT * C; i += 256) fs[i] = 0.f;
-    wait_loads();
-    __syncthreads();                                         // K and Q are there
     floatx4 QK[kMine], KK[kMine];
     const int place = cols_place(l);
 #pragma unroll
@@ -1405,11 +1434,6 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
       QK[i] = KK[i] = floatx4{0.f, 0.f, 0.f, 0.f};
       if (t < kTiles) {
         const int mt = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, nt = t - mt * (mt + 1) / 2;
-        // rows 16 mt + m of the tokens: where tile_row has them
-        auto natural = [&](const char* src, int tile, int ks) {
-          const int tk = 16 * tile + m, x = 2 * (tk >> 5) + ((tk >> 2) & 1), y = 4 * ((tk >> 3) & 3) + (tk & 3);
-          return staged<NP>(reinterpret_cast<const bf16x8*>(src), x * 4 + ks, row_slot(g, y));
-        };
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           const Parts<NP> kj = natural(bk, nt, ks);
