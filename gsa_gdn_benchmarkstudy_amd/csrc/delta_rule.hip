@@ -1162,6 +1162,10 @@ __global__ __launch_bounds__(512) void delta_join_kernel(DeltaArgs a, int chunk)
 // k are computed transposed: a wave owns 32 of them (two tiles), a lane 8 of one token.  Where v
 // heads share a q/k head, each leaves its part of dq and dk in fp32 where its dS1 was, and
 // delta_shared_kernel adds them in the heads' order (no atomics).
+// 4 x 4096 tokens of 16 heads in bf16: 337 us, 1.07 GB (3.2 TB/s).  Bound by issue: the splits and
+// products take three quarters of a block's cycles, at a clock that falls to 1.7 GHz under them; with
+// everything in the caches it would be 290.  (Slices of S0, dS1, U and dR laid out end to end: the
+// same.  512 threads, 128 registers: spills, 859 us.)
 // ---------------------------------------------------------------------------
 template <typename T> struct GradLds {
   static constexpr int C = DeltaType<T>::kChunk, NP = DeltaType<T>::kParts, MT = C / 16, JS = C / 32, kLd = C + 4;
@@ -1305,7 +1309,8 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
       for (int i = 0; i < 8; ++i) dot_v = __builtin_fmaf(fr[i], fv[i], dot_v);
     };
     load(0);
-    for (int i = tid; i < 5 * C; i += 256) gates[i] = i < 3 * C ? a.gates[at * 256 + i] : a.sums[at * 2 * C + i - 3 * C];
+    if (tid < 3 * C / 4) load_lds16(uniform(a.gates + at * 256), 16u * l, lds_addr(gates));
+    if (tid < 2 * C / 4) load_lds16(uniform(a.sums + at * 2 * C), 16u * l, lds_addr(gates + 3 * C));
 
     // dO S0^T, U dS1^T, dR S0^T (transposed), E and F by tiles of tokens
     floatx4 Z1[2][MT], Z2[2][MT], Z3[2][MT], E[kMine], F[kMine];
@@ -1451,8 +1456,12 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
         qt[js][e] = cols_of<NP>(bq, 2 * wave + e, js, place);
       }
     __syncthreads();                                         // all operands are read
-    for (int i = tid; i < L::kLate / 16; i += 256) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
-    __syncthreads();
+    // of the triangular operands' tiles beside the diagonal's, those that are read and 0 everywhere
+    if (tid < MT * kIn * 32) {
+      const int pair = tid >> 6, n = pair % kIn, t = 2 * (pair / kIn);
+      char* to = l < 32 ? xe + ((t * JS + t / 2) * kIn + n) * kUnit + 512 : xt + (((t + 1) * JS + t / 2) * kIn + n) * kUnit;
+      reinterpret_cast<u32x4*>(to)[l & 31] = u32x4{0, 0, 0, 0};
+    }
 
     // E and F become the operands of the products over tokens
 #pragma unroll
@@ -1496,7 +1505,7 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             *reinterpret_cast<uint16_t*>(xe + ij + n * kUnit + 16 * r) = __builtin_bit_cast(uint16_t, pe[n][r]);
-            if (j < i0 + r) *reinterpret_cast<uint16_t*>(xb + ij + n * kUnit + 16 * r) = __builtin_bit_cast(uint16_t, pb[n][r]);
+            if (j <= i0 + r) *reinterpret_cast<uint16_t*>(xb + ij + n * kUnit + 16 * r) = __builtin_bit_cast(uint16_t, pb[n][r]);
           }
           uint32_t w[4];
 #pragma unroll
@@ -1533,7 +1542,7 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
     // dG in 64 bits: what cancels between the rows and columns of M has to cancel exactly
     if (mine) {
       double s = 0.;
-      for (int j = so; j < C; j += 4) s += (double)sm[st * LD + j] - (double)sm[j * LD + st];
+      for (int j = so; j < C; j += 4) s += (double)(j < st ? sm[st * LD + j] : 0.f) - (double)(j > st ? sm[j * LD + st] : 0.f);
       s += __shfl_xor(s, 1, 64);
       s += __shfl_xor(s, 2, 64);
       if (so == 0) {
