@@ -18,7 +18,6 @@ import contextlib
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version as _increment_version
 
 from . import _abi
@@ -72,13 +71,30 @@ def _needs_grad(*ts: Optional[torch.Tensor]) -> bool:
     return False
 
 
+class _Twice(torch.autograd.Function):
+    """The first n tensors as they are, depending on all of them, with an error for their gradient."""
+
+    @staticmethod
+    def forward(ctx, n, *ts):
+        return tuple(t if t is None else t.view_as(t) for t in ts[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the gradients of gated_delta_rule and add_rms_norm cannot be differentiated: the operators are differentiable once")
+
+
 def _once(backward):
-    """A backward pass that is differentiable once.  torch's once_differentiable costs 15 us: only
-    where a graph of the backward pass is being built is its error needed."""
-    guarded = once_differentiable(backward)
+    """A backward pass that is differentiable once: where a graph of it is being built, what comes out
+    depends on the gradients that came in and on the inputs, with an error behind it.  (torch's
+    once_differentiable costs 15 us a call, and its outputs do not depend on the inputs: a
+    penalty on the gradients would lose its part in silence.)"""
 
     def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        return _Twice.apply(len(out), *out, *grads, *ctx.saved_tensors)
 
     return staticmethod(run)
 
@@ -86,7 +102,6 @@ def _once(backward):
 class _Rule(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, cu, scale, want_state):
-        q, k, v = _abi._heads(q), _abi._heads(k), _abi._heads(v)
         o, final, saved = _abi.delta_rule(q, k, v, g, beta, state, cu, scale, want_state, True)
         ctx.set_materialize_grads(False)
         ctx.scale, ctx.has_state = scale, state is not None
@@ -123,7 +138,10 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
 
     cu_seqlens (int32 or int64 [N+1], on the device, ascending from 0): B is 1 and N sequences
     are packed in T, each with its own state; empty ones are allowed.  Rows of o and of the
-    gradients outside every sequence are 0.
+    gradients outside every sequence are 0, whatever the inputs hold there.  Within a sequence a
+    NaN or an infinity may reach every token of its chunk of 64 (fp32: 32), those before it too:
+    padding behind the tokens of a batch's row has to be finite (its outputs are to be
+    ignored), or left out by packing.
 
     Differentiable in q, k, v, g, beta and initial_state (once); the gradients are the same
     bits on every run.  A forward that needs gradients keeps 1.5 KiB (bf16; fp32: 2.5 KiB) a
@@ -158,10 +176,11 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
                 initial_state = initial_state.clone()
         _range_push("gsa_hip/delta_rule")
         try:
-            if _needs_grad(q, k, v, g, beta, initial_state):
+            needed = _needs_grad(q, k, v, g, beta, initial_state)
+            q, k, v = _abi._heads(q), _abi._heads(k), _abi._heads(v)
+            if needed:
                 return _Rule.apply(q, k, v, g, beta, initial_state, cu_seqlens, scale, bool(output_final_state))
-            o, final, _ = _abi.delta_rule(_abi._heads(q), _abi._heads(k), _abi._heads(v), g, beta, initial_state, cu_seqlens,
-                                          scale, output_final_state, False)
+            o, final, _ = _abi.delta_rule(q, k, v, g, beta, initial_state, cu_seqlens, scale, output_final_state, False)
             return o, final
         finally:
             _range_pop()

@@ -38,7 +38,6 @@ def _check(x, weight, residual) -> None:
 class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        weight = weight.contiguous()
         y, h, rstd = _abi.rms_norm(x, weight, residual, eps, want_rstd=True)
         ctx.set_materialize_grads(False)
         ctx.added = residual is not None
@@ -72,10 +71,12 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
             return h * weight, h
         _range_push("gsa_hip/rms_norm")
         try:
-            if _needs_grad(x, weight, residual):
+            needed = _needs_grad(x, weight, residual)
+            weight = weight.contiguous()
+            if needed:
                 out = _Norm.apply(x, weight, residual, float(eps))
                 return out if residual is not None else (out, x)
-            y, h, _ = _abi.rms_norm(x, weight.contiguous(), residual, float(eps))
+            y, h, _ = _abi.rms_norm(x, weight, residual, float(eps))
             return y, x if h is None else h
         finally:
             _range_pop()

@@ -621,3 +621,72 @@ def test_step_counts_as_a_change_of_the_state(dev):
         y.backward()
     with torch.inference_mode():
         gated_delta_step(*(x[n] for n in NAMES), torch.zeros(1, 1, D, D, device=dev))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_nan_stays_where_it_is(dev, dtype):
+    """NaN in rows outside the sequences, in another sequence and in another batch row changes nothing here."""
+    offsets = [5, 75, 75, 140, 900, 1000]        # (not a multiple of the chunk anywhere)
+    x = _inputs(1, 1010, 1, 2, dtype, seed=160)
+    do = torch.randn(1, 1010, 2, D, generator=torch.Generator().manual_seed(1)).to(dtype)
+    cu = torch.tensor(offsets, device=dev)
+    want = _train(_leaves(x, dev), do.to(dev), cu)
+    bad = {n: t.clone() for n, t in x.items()}
+    do2 = do.clone()
+    for t in list(bad.values()) + [do2]:
+        t[:, :5] = t[:, 1000:] = t[:, 75:140] = float("nan")
+    got = _train(_leaves(bad, dev), do2.to(dev), cu)
+    for a, b in zip((got[0],) + got[2:], (want[0],) + want[2:]):
+        assert not a[:, :5].any() and not a[:, 1000:].any()
+        assert torch.equal(a[:, 5:75], b[:, 5:75]) and torch.equal(a[:, 140:1000], b[:, 140:1000])
+    assert torch.equal(got[1][[0, 1, 3, 4]], want[1][[0, 1, 3, 4]])
+
+    x = _inputs(3, 70, 1, 2, dtype, seed=161)
+    do = torch.randn(3, 70, 2, D, generator=torch.Generator().manual_seed(2)).to(dtype)
+    want = _train(_leaves(x, dev), do.to(dev))
+    for t in list(x.values()) + [do]:
+        t[1] = float("nan")
+    for a, b in zip(_train(_leaves(x, dev), do.to(dev)), want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+
+
+@pytest.mark.parametrize("T", [100, 1500])
+def test_backward_twice(dev, T):
+    """What the forward kept is not used up (in one piece, by segments)."""
+    leaf = _leaves(_inputs(1, T, 1, 2, torch.bfloat16, seed=170), dev)
+    st = torch.randn(1, 2, D, D, device=dev).requires_grad_(True)
+    o, S = gated_delta_rule(*leaf, initial_state=st, output_final_state=True)
+    gr = [torch.randn_like(o), torch.randn_like(S)]
+    first = torch.autograd.grad([o, S], leaf + [st], gr, retain_graph=True)
+    for a, b in zip(first, torch.autograd.grad([o, S], leaf + [st], gr)):
+        assert torch.equal(a, b)
+
+
+def test_finite_padding(dev):
+    """What lies behind a row's tokens, however large, changes no output and no gradient before it."""
+    x = _inputs(2, 200, 1, 2, torch.bfloat16, seed=180)
+    do = torch.randn(2, 200, 2, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    do[:, 150:] = 0
+    outs = []
+    for fill in (0.0, 1e4):
+        y = {n: t.clone() for n, t in x.items()}
+        for n in ("q", "v"):
+            y[n][:, 150:] = fill
+        leaf = _leaves(y, dev)
+        o, _ = gated_delta_rule(*leaf)
+        outs.append([t[:, :150] for t in (o, *torch.autograd.grad(o, leaf, do.to(dev)))])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_differentiable_once(dev):
+    leaf = _leaves(_inputs(1, 20, 1, 1, torch.float32, seed=190), dev)
+    o, _ = gated_delta_rule(*leaf)
+    d, = torch.autograd.grad(o.sum(), leaf[:1], create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(o.sum() + d.square().sum(), leaf[1:2])
+    far = [t.detach().transpose(2, 3).contiguous().transpose(2, 3).requires_grad_(True) for t in leaf[:3]] + leaf[3:]   # copied
+    o, _ = gated_delta_rule(*far)
+    d, = torch.autograd.grad(o.sum(), far[2], create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(o.sum() + d.square().sum(), far[0])

@@ -222,3 +222,10 @@ def test_two_streams(dev):
     torch.cuda.synchronize()
     for g in got:
         assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+def test_differentiable_once(dev):
+    x, w = torch.randn(4, 64, device=dev, requires_grad=True), torch.ones(64, device=dev, requires_grad=True)
+    d, = torch.autograd.grad(add_rms_norm(x, w)[0].sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad((d * d).sum(), w)
