@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
 //     next chunk's operands are on their way during the whole of this one's products
 // Bound by the issue of instructions, the matrix ones and the splits of fp32 into bf16 parts, which
 // do not overlap within a SIMD; a quarter of the cycles wait (loads of V and the barriers).  A
-// chunk of 64 takes 4.1 us by half heads, 5.9 by whole ones (8 on a full chip), 15 where two blocks
+// chunk of 64 takes 4.1 us by half heads, 5.9 by whole ones (8 on a full chip), 13 where two blocks
 // share a CU.
 // ---------------------------------------------------------------------------
 // Blocks go to the 8 XCDs in turn, each with an L2 of its own: the kBlocks blocks of one head stand 8
@@ -482,6 +482,12 @@ template <typename P> __device__ __forceinline__ const P* uniform(const P* p) {
   const uint64_t x = reinterpret_cast<uint64_t>(p);
   const uint64_t y = (uint64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
   return (const P*)(__attribute__((address_space(1))) const P*)y;      // global memory, said so that accesses are not flat ones
+}
+// x, of which the compiler knows nothing: what it computes from it stays where it is used, instead of being kept
+// over a loop in registers that are then spilled (and what reads those back waits for every load in flight).
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -622,19 +628,20 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_kernel(Delt
           S[t][n][r] = ident && tile_row(t, 4 * g + r) == col0 + 16 * n + (l & 15) ? 1.f : 0.f;
   }
 
+  auto lane = [&]() { return Sh::kDouble || !kOut ? l : here(l); };   // (two blocks a CU: 128 registers)
   auto fetch_k = [&](int64_t t0, int left, int64_t atk) {
-    if constexpr (NP == 1) fetch_rows<C, W>(a.k, sp, t0, left, hk, base + bk, wave, l);
+    if constexpr (NP == 1) fetch_rows<C, W>(a.k, sp, t0, left, hk, base + bk, wave, lane());
     else fetch<W>(a.kr + atk * K::kRows * kUnit, base + bk, K::kRows, wave, l);
   };
   auto fetch_q = [&](int64_t t0, int left, int64_t atk) {
-    if constexpr (NP == 1) fetch_rows<C, W>(a.q, sp, t0, left, hk, base + bq, wave, l);
+    if constexpr (NP == 1) fetch_rows<C, W>(a.q, sp, t0, left, hk, base + bq, wave, lane());
     else fetch<W>(a.qr + atk * K::kRows * kUnit, base + bq, K::kRows, wave, l);
   };
   constexpr int kSome = NP == 1 ? 4 : 2;
   const int rs = row_slot(g, l & 15), place = cols_place(l);
-  const int slice = V::lane(g, l & 15);
+  auto slice = [&]() { return V::lane(lane() >> 4, lane() & 15); };
   auto fetch_v = [&](int64_t t0, int left) {
-    if (!ident) V::fetch(uniform(row_at<T>(a.v, sp, t0, h) + col0), a.v.st, left, base + bv, l);
+    if (!ident) V::fetch(uniform(row_at<T>(a.v, sp, t0, h) + col0), a.v.st, left, base + bv, lane());
   };
   auto fetch_all = [&](int c) {
     const int64_t t0 = (int64_t)c * C, at = (int64_t)(slot0 + c) * a.Hv + h, atk = (int64_t)(slot0 + c) * a.Hk + hk;
@@ -714,7 +721,7 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_kernel(Delt
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float v = ident ? 0.f : to_f32(*reinterpret_cast<const T*>(lds + bv + slice + V::at(mt, r, n)));
+          const float v = ident ? 0.f : to_f32(*reinterpret_cast<const T*>(lds + bv + slice() + V::at(mt, r, n)));
           X[mt][n][r] = b[r] * (v - e[r] * X[mt][n][r]);     // R (behind the sequence beta is 0)
           if (kOut) O[mt][n][r] *= a.scale * e[r];
         }
@@ -760,11 +767,11 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_kernel(Delt
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<T*>(lds + bv + slice + V::at(mt, r, n)) = from_f32<T>(O[mt][n][r]);
+            *reinterpret_cast<T*>(lds + bv + slice() + V::at(mt, r, n)) = from_f32<T>(O[mt][n][r]);
       if (a.u) tiles_store(U, a.u + at * C * kHead, col0, l);
       asm volatile("" ::: "memory");                         // (a wave's LDS accesses keep their order)
       V::store(lds + bv, static_cast<T*>(a.o) + (((int64_t)sp.b * a.s.T + sp.t0 + t0) * a.Hv + h) * kHead + col0, (int64_t)a.Hv * kHead,
-               left, l);
+               left, lane());
     }
     if (more && !Sh::kDouble) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the wave has read its slice
@@ -870,16 +877,18 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_bwd_kernel(
         for (int r = 0; r < 4; ++r)
           d[mt][n][r] = 8 * g + tile_at(mt, r) < left ? (p + tile_at(mt, r) * a.dout.st + 16 * n)[off] : T(0);
   };
+  auto lane = [&]() { return Sh::kDouble || !kOut ? l : here(l); };   // (two blocks a CU: 128 registers)
   auto fetch_k = [&](int64_t t0, int left, int64_t atk) {
-    if constexpr (NP == 1) fetch_rows<C, W>(a.k, sp, t0, left, hk, base + bk, wave, l);
+    if constexpr (NP == 1) fetch_rows<C, W>(a.k, sp, t0, left, hk, base + bk, wave, lane());
     else fetch<W>(a.kr + atk * K::kRows * kUnit, base + bk, K::kRows, wave, l);
   };
   auto fetch_q = [&](int64_t t0, int left, int64_t atk) {
-    if constexpr (NP == 1) fetch_rows<C, W>(a.q, sp, t0, left, hk, base + bq, wave, l);
+    if constexpr (NP == 1) fetch_rows<C, W>(a.q, sp, t0, left, hk, base + bq, wave, lane());
     else fetch<W>(a.qr + atk * K::kRows * kUnit, base + bq, K::kRows, wave, l);
   };
   constexpr int kSome = NP == 1 ? 4 : 2;
-  const int rs = row_slot(g, l & 15), place = cols_place(l), slice = V::lane(g, l & 15);
+  const int rs = row_slot(g, l & 15), place = cols_place(l);
+  auto slice = [&]() { return V::lane(lane() >> 4, lane() & 15); };
   auto fetch_all = [&](int c) {
     const int64_t t0 = (int64_t)c * C, at = (int64_t)(slot0 + c) * a.Hv + h, atk = (int64_t)(slot0 + c) * a.Hk + hk;
     const int left = sp.len - (int)t0;
@@ -1005,14 +1014,14 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_bwd_kernel(
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if (kOut) *reinterpret_cast<T*>(lds + bv + slice + V::at(mt, r, n)) = from_f32<T>(b[r] * R[mt][n][r]);
+          if (kOut) *reinterpret_cast<T*>(lds + bv + slice() + V::at(mt, r, n)) = from_f32<T>(b[r] * R[mt][n][r]);
           R[mt][n][r] *= -b[r] * e[r];
         }
     }
     if constexpr (kOut) {
       asm volatile("" ::: "memory");                         // (a wave's LDS accesses keep their order)
       V::store(lds + bv, static_cast<T*>(a.dv) + (((int64_t)sp.b * a.s.T + sp.t0 + t0) * a.Hv + h) * kHead + col0, (int64_t)a.Hv * kHead,
-               left, l);
+               left, lane());
     }
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
@@ -1220,15 +1229,9 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   const int64_t tok = (int64_t)sp.b * a.s.T + sp.t0 + t0;    // row of [B * T]
   const int64_t at = (int64_t)slot * a.Hv + h, atk = (int64_t)slot * a.Hk + hk;
 
-  // a lane whose offsets the compiler computes where they are used, instead of keeping (and spilling) them
-  auto here = [&]() {
-    int x = l;
-    asm volatile("" : "+v"(x));
-    return x;
-  };
   auto fetch_kq = [&]() {
     if constexpr (NP == 1) {
-      const int l_ = here();
+      const int l_ = here(l);
       fetch_rows<C, 4>(a.k, sp, t0, left, hk, lds_addr(bk), wave, l_);
       fetch_rows<C, 4>(a.q, sp, t0, left, hk, lds_addr(bq), wave, l_);
     } else {
@@ -1243,7 +1246,7 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
   char* bs = bk + wave * 8 * kUnit;
   auto turn = [](int r) { return (r >> 1 & 1) | (r >> 3 & 1) << 1 | (r >> 4 & 1) << 2; };
   auto fetch_states = [&](int ks) {
-    const int l_ = here();
+    const int l_ = here(l);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int r = 8 * u + (l_ >> 3);
