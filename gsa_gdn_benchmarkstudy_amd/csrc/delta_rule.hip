@@ -160,7 +160,7 @@ struct DeltaArgs {
   char* tm;                   // [slots][Hv]: Tm (the backward pass: transposed)
   char* pm;                   // [slots][Hv]: P (transposed)
   float* gates;               // [slots][Hv] units: e^G, e^(G_C - G), beta [C] each
-  float* sums;                // [slots][Hv][2][C]: G (upper and lower part); the backward pass only
+  float* sums;                // [slots][Hv][2][C]: G log2 e (upper and lower part); the backward pass only
   char *kr, *qr;              // [slots][Hk]: K, Q (fp32 inputs; bf16 rows are read from where they are)
   // The scan cut into segments of seg chunks (0: sequences in one piece), [segments][Hv][128][128] each
   int seg, units;             // units: heads of all sequences, or of all segments
@@ -200,10 +200,13 @@ template <typename T> __device__ __forceinline__ Parts<DeltaType<T>::kParts> ope
 
 // ---------------------------------------------------------------------------
 // The operands of every chunk and v head (with kBwd those of the backward scan): 256 threads.
-// 16384 tokens of 16 heads in bf16: 70 us (0.2 GB).  Bound by latency: eight steps that wait for each
-// other (products, the inverse by blocks), four blocks a CU by their 35 KiB of LDS; the VALU, mostly
-// exponentials and splits, is busy for half of the time.
+// 16384 tokens of 16 heads in bf16: 68 us (0.2 GB).  Bound by latency and issue: eight steps that wait
+// for each other (products, the inverse by blocks), four blocks a CU (five, with a smaller A: the same);
+// the VALU, mostly splits, is busy for half of the time.
 // ---------------------------------------------------------------------------
+// e^(G_i - G_j) from the difference of the sums in units of log2: one instruction, right to its last bit
+// but one (under 2^-126 it may be 0), where expf takes 20; the difference rounds as one of G's would.
+__device__ __forceinline__ float decay(float x) { return __builtin_amdgcn_exp2f(x); }
 // 16x16 tile a b of LDS matrices, summed over K (fp32 matrix instruction).
 __device__ __forceinline__ floatx4 tile_f32(const float* a, int lda, const float* b, int ldb, int K) {
   const int l = lane_id(), m = l & 15, kk = l >> 4;
@@ -346,7 +349,8 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
       if (l >= o) G += y;
     }
     const double Ge = __shfl(G, C - 1, 64);
-    const float hi = (float)G, lo = (float)(G - (double)hi);
+    const double G2 = G * 1.4426950408889634074;             // log2 e: the decays between tokens are powers of 2 (decay)
+    const float hi = (float)G2, lo = (float)(G2 - (double)hi);
     if (l < C) {
       gh[l] = hi;
       gl[l] = lo;
@@ -394,7 +398,7 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = tile_row(mt, 4 * g4 + r);
-      const float d = j <= i ? expf((gh[i] - gh[j]) + (gl[i] - gl[j])) : 0.f;
+      const float d = j <= i ? decay((gh[i] - gh[j]) + (gl[i] - gl[j])) : 0.f;
       if (C == 64 || wave >= MT) am[i][j] = a.scale * qk[r] * d;
       kk[nt][r] = j < i ? bt[i] * kk[nt][r] * d : 0.f;
     }
@@ -1481,7 +1485,7 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int ii = 16 * mt + 4 * g + r;
-          const float d = j <= ii ? expf((gates[3 * C + ii] - gates[3 * C + j]) + (gates[4 * C + ii] - gates[4 * C + j])) : 0.f;
+          const float d = j <= ii ? decay((gates[3 * C + ii] - gates[3 * C + j]) + (gates[4 * C + ii] - gates[4 * C + j])) : 0.f;
           const float fd = j < ii ? F[i][r] * d : 0.f;
           ed[r] = a.scale * E[i][r] * d;
           bb[r] = -gates[2 * C + ii] * fd;
@@ -1706,7 +1710,7 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   //   16 heads of 512 tokens 46 / 143 in one piece, 60 / 175 by segments; 768: 62 / 187 and 64 / 185; 1024: 78 / 231 and 69 / 195
   //   64 heads of 1024 tokens 88 / 312 and 100 / 330; 2048: 169 / 627 and 165 / 586; 80 heads of 4096: 377 / 1460 and 406 / 1418
   if (heads <= 64 && length >= std::max<int64_t>(12, heads / 2 - 4)) {
-    // a block a CU, of at least 4 chunks (16384 tokens of 16 heads: 16 segments 358 us, 32 373); joining costs 1.9 us a
+    // a block a CU, of at least 4 chunks (16384 tokens of 16 heads: 16 segments 323 us, 32 356); joining costs 1.9 us a
     // segment and the two passes 16 us a chunk of one: more than sqrt(8 chunks) segments lose
     int64_t pieces = 256 / heads;
     while (pieces > 3 && pieces * pieces > 8 * length) --pieces;
