@@ -690,3 +690,32 @@ def test_differentiable_once(dev):
     d, = torch.autograd.grad(o.sum(), far[2], create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(o.sum() + d.square().sum(), far[0])
+
+
+def test_captured_with_other_sequences(dev):
+    """Offsets are read on the device: a graph of a packed batch serves other lengths, and states by other indices."""
+    x = {n: t.to(dev) for n, t in _inputs(1, 1400, 1, 2, torch.bfloat16, seed=200).items()}
+    one = {n: t[0].to(dev) for n, t in _inputs(1, 4, 1, 2, torch.bfloat16, seed=201).items()}
+    cu = torch.tensor([0, 10, 20, 1400], device=dev)
+    pool, at = torch.zeros(6, 2, D, D, device=dev), torch.tensor([0, 1, 2, -1], device=dev)
+
+    def both():
+        o, S = gated_delta_rule(*(x[n] for n in NAMES), output_final_state=True, cu_seqlens=cu)
+        pool[:3] = S
+        return o, gated_delta_step(*(one[n] for n in NAMES), pool, at)
+
+    with torch.no_grad():
+        both()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = both()
+        for offsets, idx in (([0, 700, 700, 1300], [2, 2, 0, 1]), ([64, 65, 1399, 1400], [1, -1, 7, 1]), ([0, 10, 20, 1400], [0, 1, 2, -1])):
+            cu.copy_(torch.tensor(offsets))
+            at.copy_(torch.tensor(idx))
+            graph.replay()
+            torch.cuda.synchronize()
+            states = pool.clone()
+            for a, b in zip(got, both()):
+                assert torch.equal(a, b)
+            assert torch.equal(states, pool)
