@@ -18,6 +18,7 @@ import contextlib
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.graph import increment_version as _increment_version
 
 from . import _abi
@@ -51,8 +52,19 @@ def _check(n: int, q, k, v, g, beta) -> None:
 _HERE = contextlib.nullcontext()
 
 
+def _refuse_unseen(*ts: Optional[torch.Tensor]) -> None:
+    """Raises where torch follows the call in a way that a kernel's launch escapes, and that would
+    lose it in silence: a tangent of forward-mode differentiation."""
+    if _forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in ts:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the gated delta rule and the RMS norm have no forward-mode derivative (torch.autograd.forward_ad)")
+
+
 def _device(first: torch.Tensor, *others: Optional[torch.Tensor]):
-    """Checks that all tensors are on one GPU and makes it the current one."""
+    """Checks that torch need not see into the call and that all tensors are on one GPU, and makes
+    that the current one."""
+    _refuse_unseen(first, *others)
     at = first.get_device()                      # -1 on the CPU
     for t in others:
         if t is not None and t.get_device() != at:
@@ -90,6 +102,7 @@ def _once(backward):
     penalty on the gradients would lose its part in silence.)"""
 
     def run(ctx, *grads):
+        _refuse_unseen(*grads)
         if not torch.is_grad_enabled():
             return backward(ctx, *grads)
         with torch.no_grad():
@@ -143,8 +156,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     padding behind the tokens of a batch's row has to be finite (its outputs are to be
     ignored), or left out by packing.
 
-    Differentiable in q, k, v, g, beta and initial_state (once); the gradients are the same
-    bits on every run.  A forward that needs gradients keeps 1.5 KiB (bf16; fp32: 2.5 KiB) a
+    Differentiable in q, k, v, g, beta and initial_state, once and backwards (a tangent of
+    torch.autograd.forward_ad raises); the gradients are the same bits on every run.  A forward that needs gradients keeps 1.5 KiB (bf16; fp32: 2.5 KiB) a
     token and v head, and where it works by segments up to 0.25 KiB (0.5 KiB) more.
 
     May be captured into a graph, forward and backward, after one call outside of it; as with any

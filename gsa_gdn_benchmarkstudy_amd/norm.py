@@ -62,8 +62,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     """(y, h) of x [..., D] (bf16 or fp32), weight [D] and residual (x's shape) in x's dtype;
     h is x itself without a residual.  D up to 32768.  Rows of a strided x are read in place
     where its leading dimensions but one collapse (heads of a projection); y and h are
-    contiguous.  Differentiable (once) in all three; the gradients are the same bits on every
-    run, and with a residual x and the residual get the same tensor."""
+    contiguous.  Differentiable in all three, once and backwards; the gradients are the same
+    bits on every run, and with a residual x and the residual get the same tensor."""
     _check(x, weight, residual)
     with _device(x, weight, residual):
         if x.numel() == 0:

@@ -184,3 +184,54 @@ def test_c_rule_sizes(lib):
     assert lib.gsa_delta_rule_saved_bytes(1, 65, 1, 0, 2, 2, 0) == 3 * 2 * (65536 + 32 * 512)
     # packed sequences may each leave a chunk begun: one slot more for every one of them
     assert lib.gsa_delta_rule_saved_bytes(1, 130, 5, 1, 1, 1, 1) == (2 + 5) * (65536 + 64 * 512)
+
+
+# ---------------------------------------------------------------------------
+# What torch would lose in silence
+# ---------------------------------------------------------------------------
+
+def _calls():
+    """(entry point, its floating-point arguments) of every operator."""
+    names = ("q", "k", "v", "g", "beta")
+    rule, step, x = _rule(), _step(), torch.ones(2, 8)
+    return [(lambda *t: gated_delta_rule(*t[:5], initial_state=t[5]), [rule[n] for n in names] + [torch.zeros(1, 2, D, D)]),
+            (lambda *t: gated_delta_step(*t), [step[n] for n in names] + [step["state"]]),
+            (lambda *t: add_rms_norm(t[0], t[1], residual=t[2]), [x, torch.ones(8), x.clone()]),
+            (lambda *t: add_rms_norm_fp8(t[0], t[1], residual=t[2]), [x, torch.ones(8), x.clone()])]
+
+
+@pytest.mark.parametrize("op", range(4))
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_raises(op, grad):
+    """A dual tensor needs no gradient, and its data is there: the result would come without its tangent."""
+    from torch.autograd import forward_ad as fw
+
+    call, args = _calls()[op]
+    for i in range(len(args)):
+        with torch.set_grad_enabled(grad), fw.dual_level():
+            dual = fw.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(*args[:i], dual, *args[i + 1:])
+    with fw.dual_level(), pytest.raises(RuntimeError, match="GPU|CUDA|device"):
+        call(*args)                              # no tangent among them: on to the next check
+
+
+def test_forward_mode_over_the_backward_pass_raises():
+    from torch.autograd import forward_ad as fw
+
+    from gsa_gdn_benchmarkstudy_amd.delta import _once
+
+    class Double(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return 2 * x
+
+        @_once
+        def backward(ctx, dy):
+            return 2 * dy
+
+    x = torch.ones(3, requires_grad=True)
+    with fw.dual_level():
+        dy = fw.make_dual(torch.ones(3), torch.ones(3))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(Double.apply(x), x, dy)
