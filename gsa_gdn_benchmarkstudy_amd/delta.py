@@ -54,11 +54,13 @@ _HERE = contextlib.nullcontext()
 
 def _refuse_unseen(*ts: Optional[torch.Tensor]) -> None:
     """Raises where torch follows the call in a way that a kernel's launch escapes, and that would
-    lose it in silence: a tangent of forward-mode differentiation."""
+    lose it in silence: a tangent of forward-mode differentiation, or torch.jit.trace."""
     if _forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
         for t in ts:
             if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
                 raise RuntimeError("the gated delta rule and the RMS norm have no forward-mode derivative (torch.autograd.forward_ad)")
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError("the gated delta rule and the RMS norm cannot be recorded by torch.jit.trace")
 
 
 def _device(first: torch.Tensor, *others: Optional[torch.Tensor]):

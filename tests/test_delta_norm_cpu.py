@@ -235,3 +235,10 @@ def test_forward_mode_over_the_backward_pass_raises():
         dy = fw.make_dual(torch.ones(3), torch.ones(3))
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(Double.apply(x), x, dy)
+
+
+@pytest.mark.parametrize("op", range(4))
+def test_trace_raises(op):
+    call, args = _calls()[op]
+    with torch.no_grad(), pytest.raises(RuntimeError, match="torch.jit.trace"):
+        torch.jit.trace(call, tuple(args), check_trace=False)
