@@ -1043,7 +1043,7 @@ def delta_rule(q, k, v, g, beta, state_in, cu, scale: float, want_state: bool, w
     a = _delta_args(q, k, v, g, beta, state_in, cu, scale)
     forward, _, keep = _delta_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
     if not forward:
-        raise ValueError(f"{B} x {T} tokens in {a.N} sequences of {Hv} heads: over 2**23 chunks times heads")
+        raise ValueError(f"{B} x {T} tokens in {a.N} sequences of {Hv} heads: over 2**23 chunks times heads, or 2**23 sequences times heads")
     o = torch.empty(B, T, Hv, d, device=v.device, dtype=v.dtype)
     state = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_state else None
     ws = torch.empty(forward, device=v.device, dtype=torch.uint8)

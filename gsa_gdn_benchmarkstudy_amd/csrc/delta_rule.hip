@@ -1693,9 +1693,10 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   DeltaSizes z{};
   z.C = dtype == GSA_DTYPE_BF16 ? gsa::DeltaType<uint16_t>::kChunk : gsa::DeltaType<float>::kChunk;
   if (B < 1 || T < 1 || N < 1 || Hk < 1 || Hv < Hk || Hv % Hk || !dtype_size(dtype)) return z;
-  const int64_t nc = (T + z.C - 1) / z.C;
+  const int64_t nc = ((int64_t)T + z.C - 1) / z.C;
   z.slots = packed ? (int64_t)T / z.C + N : B * nc;
-  if (z.slots * Hv > 1 << 23 || (int64_t)N * Hv > 1 << 23) {    // a grid of 256 threads each
+  // grids of 256 threads a chunk and head and of 512 a sequence and head: a launch has less than 2^32
+  if (z.slots > (1 << 23) / Hv || (int64_t)N * Hv >= 1 << 23) {
     z.slots = 0;
     return z;
   }

@@ -159,8 +159,10 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     ignored), or left out by packing.
 
     Differentiable in q, k, v, g, beta and initial_state, once and backwards (a tangent of
-    torch.autograd.forward_ad raises); the gradients are the same bits on every run.  A forward that needs gradients keeps 1.5 KiB (bf16; fp32: 2.5 KiB) a
-    token and v head, and where it works by segments up to 0.25 KiB (0.5 KiB) more.
+    torch.autograd.forward_ad raises); the gradients are the same bits on every run.  A forward
+    that needs gradients keeps 1.5 KiB (bf16; fp32: 2.5 KiB) a token and v head, and where it
+    works by segments up to 0.25 KiB (0.5 KiB) more.  At most 2**23 chunks times v heads, and
+    fewer than 2**23 sequences times v heads.
 
     May be captured into a graph, forward and backward, after one call outside of it; as with any
     backward pass no eager graph of the same leaves may live then (capture torch.autograd.grad, or

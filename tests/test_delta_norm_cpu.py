@@ -186,6 +186,21 @@ def test_c_rule_sizes(lib):
     assert lib.gsa_delta_rule_saved_bytes(1, 130, 5, 1, 1, 1, 1) == (2 + 5) * (65536 + 64 * 512)
 
 
+def test_c_rule_sizes_at_their_ends(lib):
+    """Sizes that no launch and no index holds are refused: 2**23 chunks or heads of sequences (512 threads
+    each, and a launch has less than 2**32), token counts next to 2**31, products past 64 bits."""
+    last = 2 ** 31 - 1
+    for f in (lib.gsa_delta_rule_saved_bytes, lambda *a: lib.gsa_delta_rule_workspace_bytes(*a, 0),
+              lambda *a: lib.gsa_delta_rule_workspace_bytes(*a, 1)):
+        for dtype in (0, 1):
+            for N in (2 ** 19 - 1, 2 ** 19):     # of 16 heads and one token each: the chunks' launches would do
+                assert (f(N, 1, N, 0, 16, 16, dtype) > 0) == (f(1, 1, N, 1, 16, 16, dtype) > 0) == (N < 2 ** 19)
+            for packed in (0, 1):
+                assert f(1, last, 1, packed, 1, 1, dtype) == f(1, last, 1, packed, last, last, dtype) == 0
+            assert f(last, last, last, 0, last, last, dtype) == f(2 ** 29, 64, 2 ** 29, 0, 32, 32, dtype) == 0
+    assert lib.gsa_delta_rule_saved_bytes(1, 64 * 2 ** 23, 1, 0, 1, 1, 1) > 0 == lib.gsa_delta_rule_saved_bytes(1, 64 * 2 ** 23 + 1, 1, 0, 1, 1, 1)
+
+
 # ---------------------------------------------------------------------------
 # What torch would lose in silence
 # ---------------------------------------------------------------------------
