@@ -148,8 +148,8 @@ template <typename T, int kTpr, int kSlots, bool kVec, bool kFp8>
 __global__ __launch_bounds__(norm_threads(kTpr)) void rms_norm_kernel(NormFwd a) {
   __shared__ float red[2][norm_threads(kTpr) / 64];
   const int li = threadIdx.x % kTpr;
-  const int64_t r = (int64_t)blockIdx.x * (norm_threads(kTpr) / kTpr) + threadIdx.x / kTpr;
-  if (kTpr <= 64 && r >= a.rows) return;         // (a block of one row always has it)
+  const int64_t r = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (norm_threads(kTpr) / kTpr) + threadIdx.x / kTpr;
+  if (r >= a.rows) return;                       // (all of a block of one row together)
   const T* x = norm_row<T>(a.x, r, a.inner);
   float h[kSlots][8];
 #pragma unroll
@@ -422,9 +422,12 @@ template <typename T, bool kFp8>
 int launch_norm(const gsa::NormFwd& a, bool vec, hipStream_t stream) {
   return with_shape(norm_shape(a.D), [&]<int kTpr, int kSlots>() {
     constexpr int kThreads = gsa::norm_threads(kTpr);
-    const unsigned grid = (unsigned)((a.rows + kThreads / kTpr - 1) / (kThreads / kTpr));
-    if (vec) hipLaunchKernelGGL((gsa::rms_norm_kernel<T, kTpr, kSlots, true, kFp8>), dim3(grid), dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((gsa::rms_norm_kernel<T, kTpr, kSlots, false, kFp8>), dim3(grid), dim3(kThreads), 0, stream, a);
+    // one dimension of a launch holds less than 2^32 threads (more are cut off without an error)
+    constexpr int64_t kMost = 1 << 21;
+    const int64_t blocks = (a.rows + kThreads / kTpr - 1) / (kThreads / kTpr);
+    const dim3 grid((unsigned)std::min(blocks, kMost), (unsigned)((blocks + kMost - 1) / kMost));
+    if (vec) hipLaunchKernelGGL((gsa::rms_norm_kernel<T, kTpr, kSlots, true, kFp8>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((gsa::rms_norm_kernel<T, kTpr, kSlots, false, kFp8>), grid, dim3(kThreads), 0, stream, a);
     return launch_status();
   });
 }

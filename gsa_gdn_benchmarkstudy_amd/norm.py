@@ -60,10 +60,10 @@ class _Norm(torch.autograd.Function):
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
                  eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     """(y, h) of x [..., D] (bf16 or fp32), weight [D] and residual (x's shape) in x's dtype;
-    h is x itself without a residual.  D up to 32768.  Rows of a strided x are read in place
-    where its leading dimensions but one collapse (heads of a projection); y and h are
-    contiguous.  Differentiable in all three, once and backwards; the gradients are the same
-    bits on every run, and with a residual x and the residual get the same tensor."""
+    h is x itself without a residual.  D up to 32768, fewer than 2**31 rows.  Rows of a strided
+    x are read in place where its leading dimensions but one collapse (heads of a projection);
+    y and h are contiguous.  Differentiable in all three, once and backwards; the gradients are
+    the same bits on every run, and with a residual x and the residual get the same tensor."""
     _check(x, weight, residual)
     with _device(x, weight, residual):
         if x.numel() == 0:

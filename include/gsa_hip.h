@@ -518,7 +518,7 @@ int gsa_proj_fused(const void* x, int64_t x_st, int B, int T, int D, int H, int 
  *   h = round(x + res) (x itself when res is NULL),  y = h * (mean h^2 + eps)^-1/2 * w
  * Row r of an input lies at base + (r / inner) * s0 + (r % inner) * s1 elements (rows a
  * multiple of inner), so heads of a strided projection are read in place; y, h and dx are
- * contiguous [rows, D], w [D].  1 <= D <= 32768; any alignment of elements (16-byte rows
+ * contiguous [rows, D], w [D].  1 <= D <= 32768, 1 <= rows < 2^31; any alignment of elements (16-byte rows
  * are read and written whole).
  *   gsa_rms_norm:          y, h (with res), and (nullable) rstd fp32 [rows] for the backward
  *   gsa_rms_norm_fp8:      y in e4m3, y = round(y / scale), scale fp32 [rows] = max |y| / 448

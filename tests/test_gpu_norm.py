@@ -229,3 +229,23 @@ def test_differentiable_once(dev):
     d, = torch.autograd.grad(add_rms_norm(x, w)[0].sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad((d * d).sum(), w)
+
+
+@pytest.mark.parametrize("D,rows,fp8", [(8, (1 << 28) + 5, False), (136, (1 << 26) + 3, True), (1032, (1 << 24) + 1, True),
+                                        (8200, (1 << 22) + 1, True)])
+def test_more_rows_than_one_launch_dimension_holds(dev, D, rows, fp8):
+    """2**32 threads in one direction and more: every row is there, and nothing behind the last.  (All rows
+    are one: read with a stride of 0.)"""
+    print(f"rows {rows} of {D}", flush=True)
+    x, _, w = _make((3, D), torch.bfloat16, False, D)
+    x, w = x.to(dev), w.to(dev)
+    many = x[1:2].expand(rows, D)
+    if fp8:
+        y, scale, _ = add_rms_norm_fp8(many, w, eps=EPS)
+        y1, s1, _ = add_rms_norm_fp8(x[1:2], w, eps=EPS)
+        assert bool((scale == s1[0]).all())
+        y, y1 = y.view(torch.uint8), y1.view(torch.uint8)
+    else:
+        y, y1 = add_rms_norm(many, w, eps=EPS)[0], add_rms_norm(x[1:2], w, eps=EPS)[0]
+    for a in range(0, rows, 1 << 22):
+        assert bool((y[a:a + (1 << 22)] == y1).all()), a
