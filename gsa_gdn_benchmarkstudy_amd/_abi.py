@@ -1040,6 +1040,10 @@ def _delta_bytes(*sizes: int):
 def delta_rule(q, k, v, g, beta, state_in, cu, scale: float, want_state: bool, want_saved: bool):
     """gsa_delta_rule: (o, state_out or None, saved or None).  q, k, v as _heads gives them."""
     B, T, Hv, d = v.shape
+    if B * T == 0:                               # nothing to launch: the states as they came
+        n = B if cu is None else cu.numel() - 1
+        state = None if not want_state else v.new_zeros(n, Hv, d, d, dtype=torch.float32) if state_in is None else state_in.clone()
+        return v.new_empty(v.shape), state, v.new_empty(0, dtype=torch.uint8) if want_saved else None
     a = _delta_args(q, k, v, g, beta, state_in, cu, scale)
     forward, _, keep = _delta_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
     if not forward:
@@ -1061,6 +1065,10 @@ def delta_rule(q, k, v, g, beta, state_in, cu, scale: float, want_state: bool, w
 def delta_rule_backward(q, k, v, g, beta, cu, scale: float, saved, dout, dstate, want_dstate: bool):
     """gsa_delta_rule_backward: (dq, dk, dv, dg, dbeta, dstate_in or None)."""
     B, T, Hv, d = v.shape
+    if B * T == 0:
+        n = B if cu is None else cu.numel() - 1
+        ds = None if not want_dstate else v.new_zeros(n, Hv, d, d, dtype=torch.float32) if dstate is None else dstate.clone()
+        return (*(t.new_empty(t.shape) for t in (q, k, v, g, beta)), ds)
     a = _delta_args(q, k, v, g, beta, None, cu, scale)
     dq, dk, dv, dg, db = [torch.empty(t.shape, device=v.device, dtype=t.dtype) for t in (q, k, v, g, beta)]
     ds = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_dstate else None

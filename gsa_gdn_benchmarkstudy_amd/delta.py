@@ -169,7 +169,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     use leaves of the graph's own).
     """
     _check(2, q, k, v, g, beta)
-    B, T, Hv, d = v.shape
+    B, _, Hv, d = v.shape
     if cu_seqlens is not None:
         if B != 1:
             raise ValueError(f"packed sequences come in one row: B is {B}")
@@ -182,11 +182,6 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
             raise ValueError(f"initial_state {tuple(initial_state.shape)} {initial_state.dtype}: expected fp32 {(N, Hv, d, d)}")
     scale = d ** -0.5 if scale is None else float(scale)
     with _device(q, k, v, g, beta, initial_state, cu_seqlens):
-        if B * T == 0:
-            o = v.new_zeros(v.shape)
-            if not output_final_state:
-                return o, None
-            return o, v.new_zeros(N, Hv, d, d, dtype=torch.float32) if initial_state is None else initial_state.clone()
         if initial_state is not None:
             initial_state = initial_state.contiguous()
             if initial_state.data_ptr() % 16:

@@ -719,3 +719,29 @@ def test_captured_with_other_sequences(dev):
             for a, b in zip(got, both()):
                 assert torch.equal(a, b)
             assert torch.equal(states, pool)
+
+
+@pytest.mark.parametrize("B,T", [(2, 0), (0, 5), (0, 0)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_gradients_of_nothing(dev, B, T, packed):
+    """An empty batch in a training step: results in the graph, gradients of their leaves' shapes, a state's handed through."""
+    if packed:
+        B, T = 1, 0
+    x = [torch.zeros(B, T, h, D, device=dev, dtype=torch.bfloat16, requires_grad=True) for h in (1, 1, 2)]
+    x += [torch.zeros(B, T, 2, device=dev, requires_grad=True) for _ in range(2)]
+    N = 3 if packed else B
+    cu = torch.zeros(4, device=dev, dtype=torch.int32) if packed else None
+    st = torch.randn(N, 2, D, D, device=dev, requires_grad=True)
+    dS = torch.randn(N, 2, D, D, device=dev)
+    o, S = gated_delta_rule(*x, initial_state=st, output_final_state=True, cu_seqlens=cu)
+    assert o.requires_grad and o.shape == x[2].shape and torch.equal(S, st) and S.data_ptr() != st.data_ptr() or N == 0
+    d = torch.autograd.grad([o, S], x + [st], [torch.zeros_like(o), dS])
+    assert all(a.shape == b.shape and a.dtype == b.dtype for a, b in zip(d, x + [st])) and torch.equal(d[-1], dS)
+    o, S = gated_delta_rule(*x, output_final_state=True, cu_seqlens=cu)
+    assert S.shape == st.shape and not S.any()
+    (o.sum() + S.sum()).backward()
+    assert all(t.grad is not None and t.grad.shape == t.shape for t in x)
+    o, S = gated_delta_rule(*x, initial_state=st, cu_seqlens=cu)
+    assert S is None
+    d = torch.autograd.grad(o.sum(), x + [st])
+    assert not d[-1].any()
