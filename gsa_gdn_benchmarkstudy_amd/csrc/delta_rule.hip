@@ -1571,9 +1571,10 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaArgs a) {
           if (a.beta_bf16) static_cast<uint16_t*>(a.dbeta)[o] = (uint16_t)f32_to_bf16_bits(x);
           else static_cast<float*>(a.dbeta)[o] = x;
         }
-        // at the end of the chunk: e^G_C <dS1, S0> and every x2
-        dsum[st] = s + x1 - x2 - beta * x3;
-        red[st] = (float)x2;
+        // at the end of the chunk: e^G_C <dS1, S0> and every x2, the same fp32 numbers that their rows lose
+        const float f2 = (float)x2;
+        dsum[st] = s + x1 - (double)f2 - beta * x3;
+        red[st] = f2;
       }
     }
     __syncthreads();

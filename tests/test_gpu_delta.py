@@ -745,3 +745,18 @@ def test_gradients_of_nothing(dev, B, T, packed):
     assert S is None
     d = torch.autograd.grad(o.sum(), x + [st])
     assert not d[-1].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_no_gradient_of_what_has_no_effect(dev, dtype):
+    """The first decay of a sequence without a state, and one that resets all that came before it, change nothing:
+    what the sums of dg from there to the end hold twice has to cancel to the last bits of 64."""
+    x = _inputs(1, 200, 1, 2, dtype, seed=191)
+    x["g"][:, 140] = -float("inf")
+    do = torch.randn(1, 200, 2, D, generator=torch.Generator().manual_seed(4)).to(dtype)
+    leaf = _leaves(x, dev)
+    o, _ = gated_delta_rule(*leaf)
+    (dg,) = torch.autograd.grad(o, leaf[3:4], do.to(dev))
+    most = dg.abs().max()
+    # sums of some 64 x 64 terms in 64 bits: 2^-52 of each, of the size of the largest gradient
+    assert float(dg[:, [0, 140]].abs().max() / most) <= 4096 * 2.0 ** -52
