@@ -48,7 +48,7 @@ EXPORTS = (
     "gsa_rope_qk",
     "gsa_rms_norm", "gsa_rms_norm_fp8", "gsa_rms_norm_backward", "gsa_rms_norm_backward_workspace_bytes",
     "gsa_delta_step", "gsa_delta_rule", "gsa_delta_rule_backward", "gsa_delta_rule_workspace_bytes",
-    "gsa_delta_rule_saved_bytes",
+    "gsa_delta_rule_saved_bytes", "gsa_delta_rule_shape",
 )
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
@@ -133,6 +133,7 @@ _PROTOS = {
                         _vp, _i32, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp], _i32),
     "gsa_delta_rule_workspace_bytes": ([_i32] * 8, ctypes.c_size_t),
     "gsa_delta_rule_saved_bytes": ([_i32] * 7, ctypes.c_size_t),
+    "gsa_delta_rule_shape": ([_i32] * 7, _i32),
     "gsa_delta_rule": ([ctypes.POINTER(DeltaArgs), _vp], _i32),
     "gsa_delta_rule_backward": ([ctypes.POINTER(DeltaArgs), _vp], _i32),
 }

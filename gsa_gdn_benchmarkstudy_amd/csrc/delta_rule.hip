@@ -1672,9 +1672,12 @@ namespace {
 constexpr size_t kAlign = 256;
 inline size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
+// Blocks of the scans that give the outputs: half a head, a head with the CU to itself, or with another one beside it.
+enum { kHalf = 1, kAlone = 2, kTwo = 3 };
+
 // What one call lays out, from its sizes alone (so a backward pass finds what its forward kept).
 struct DeltaSizes {
-  int C, seg, columns;        // tokens of a chunk; chunks of a segment, 0: none; columns of a scan's block
+  int C, seg, shape;          // tokens of a chunk; chunks of a segment, 0: none; of the scans that give the outputs (kHalf, ..)
   int64_t slots, segs;        // 0 slots: out of range
   size_t tm, pm, gates, sums, kr, states, s0, u;
   size_t workspace(bool backward) const {
@@ -1706,7 +1709,7 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   //   1024 tokens of 128 heads 109 / 486 by 64 columns, 134 / 544 by heads; of 160 heads 181 / 750 and 141 / 635
   //   packed (sequences differ in length), 23 of 12289 tokens, 16 heads: 243 and 271; 7 of 6001: - / 632 and 751
   const int64_t heads = (int64_t)N * Hv;
-  z.columns = heads <= (packed ? 384 : 128) ? 64 : 128;
+  z.shape = heads <= (packed ? 384 : 128) ? kHalf : heads <= 256 ? kAlone : kTwo;
   const int64_t length = packed ? nc / N : nc;               // of one sequence
   // Segments cost two passes over them and the join, and pay for few heads and long sequences:
   //   16 heads of 512 tokens 46 / 143 in one piece, 60 / 175 by segments; 768: 62 / 187 and 64 / 185; 1024: 78 / 231 and 69 / 195
@@ -1719,6 +1722,7 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
     const int64_t seg = std::max<int64_t>(4, (length + pieces - 1) / pieces);
     z.seg = (int)seg;
     z.segs = packed ? (int64_t)T / (z.C * seg) + N : B * ((nc + seg - 1) / seg);
+    z.shape = z.segs * Hv <= 256 ? kAlone : kTwo;
   }
   const size_t n = (size_t)z.slots * Hv, nk = (size_t)z.slots * Hk;
   if (dtype == GSA_DTYPE_BF16) backward ? pack_sizes<uint16_t, true>(z, n, nk) : pack_sizes<uint16_t, false>(z, n, nk);
@@ -1785,10 +1789,9 @@ template <typename T> int launch_forward(const gsa::DeltaArgs& a, const DeltaSiz
   if (a.seg) {
     if (const int e = launch_scan<T, false, Heads>(a, 2, s)) return e;
     if (const int e = launch_join<false>(a, z, s)) return e;
-    return a.units <= 256 ? launch_scan<T, true, HeadsAlone>(a, 1, s) : launch_scan<T, true, Heads>(a, 1, s);
   }
-  if (z.columns == 64) return launch_scan<T, true, Columns64>(a, 1, s);
-  return a.units <= 256 ? launch_scan<T, true, HeadsAlone>(a, 1, s) : launch_scan<T, true, Heads>(a, 1, s);
+  return z.shape == kHalf ? launch_scan<T, true, Columns64>(a, 1, s)
+       : z.shape == kAlone ? launch_scan<T, true, HeadsAlone>(a, 1, s) : launch_scan<T, true, Heads>(a, 1, s);
 }
 template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSizes& z, hipStream_t s) {
   if (const int e = launch_outside(a, sizeof(T) == 2 ? GSA_DTYPE_BF16 : GSA_DTYPE_F32, true, s)) return e;
@@ -1797,12 +1800,9 @@ template <typename T> int launch_backward(const gsa::DeltaArgs& a, const DeltaSi
   if (a.seg) {
     if ((e = launch_scan_bwd<T, false, Heads>(a, s))) return e;
     if ((e = launch_join<true>(a, z, s))) return e;
-    e = a.units <= 256 ? launch_scan_bwd<T, true, HeadsAlone>(a, s) : launch_scan_bwd<T, true, Heads>(a, s);
-  } else if (z.columns == 64) {
-    e = launch_scan_bwd<T, true, Columns64>(a, s);
-  } else {
-    e = a.units <= 256 ? launch_scan_bwd<T, true, HeadsAlone>(a, s) : launch_scan_bwd<T, true, Heads>(a, s);
   }
+  e = z.shape == kHalf ? launch_scan_bwd<T, true, Columns64>(a, s)
+    : z.shape == kAlone ? launch_scan_bwd<T, true, HeadsAlone>(a, s) : launch_scan_bwd<T, true, Heads>(a, s);
   if (e) return e;
   constexpr size_t lds = gsa::GradLds<T>::kBytes;
   static_assert(2 * lds <= 160 * 1024, "two blocks a CU");
@@ -1901,6 +1901,10 @@ extern "C" size_t gsa_delta_rule_workspace_bytes(int B, int T, int N, int packed
 extern "C" size_t gsa_delta_rule_saved_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype) {
   const auto z = gsa_host::delta_sizes(B, T, N, packed, Hk, Hv, dtype, false);
   return z.slots ? z.saved() : 0;
+}
+extern "C" int gsa_delta_rule_shape(int B, int T, int N, int packed, int Hk, int Hv, int dtype) {
+  const auto z = gsa_host::delta_sizes(B, T, N, packed, Hk, Hv, dtype, false);
+  return z.slots ? z.shape + (z.seg ? 4 : 0) : 0;
 }
 extern "C" int gsa_delta_rule(const gsa_delta_args* x, void* stream) {
   gsa::DeltaArgs a;

@@ -604,6 +604,9 @@ typedef struct gsa_delta_args {
 } gsa_delta_args;
 size_t gsa_delta_rule_workspace_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype, int backward);
 size_t gsa_delta_rule_saved_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype);
+/* How a call of these sizes goes from chunk to chunk: 0 refused; 1 blocks of half a head, 2 of a head with
+ * a CU each, 3 of a head, two on a CU; 4 more where sequences are cut into segments that are joined again. */
+int gsa_delta_rule_shape(int B, int T, int N, int packed, int Hk, int Hv, int dtype);
 int gsa_delta_rule(const gsa_delta_args* args, void* stream);
 int gsa_delta_rule_backward(const gsa_delta_args* args, void* stream);
 

@@ -201,6 +201,15 @@ def test_c_rule_sizes_at_their_ends(lib):
     assert lib.gsa_delta_rule_saved_bytes(1, 64 * 2 ** 23, 1, 0, 1, 1, 1) > 0 == lib.gsa_delta_rule_saved_bytes(1, 64 * 2 ** 23 + 1, 1, 0, 1, 1, 1)
 
 
+def test_c_rule_shape(lib):
+    """0 with the byte counts; half heads for few of them, whole ones alone and two on a CU for many; segments for long rows."""
+    f = lib.gsa_delta_rule_shape
+    assert f(1, 5, 1, 0, 2, 3, 1) == f(0, 5, 0, 0, 1, 1, 1) == f(1, 5, 1, 0, 1, 1, 7) == f(1, 2 ** 31 - 1, 1, 0, 1, 1, 1) == 0
+    for dtype in (0, 1):
+        assert [f(B, 100, B, 0, 16, 16, dtype) for B in (1, 8, 9, 16, 17, 40)] == [1, 1, 2, 2, 3, 3]
+        assert f(1, 16384, 1, 0, 16, 16, dtype) == 6
+
+
 # ---------------------------------------------------------------------------
 # What torch would lose in silence
 # ---------------------------------------------------------------------------
