@@ -1704,12 +1704,21 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
     z.slots = 0;
     return z;
   }
-  // Blocks of 64 columns while the longest of the pieces decides, whole heads when the chip is full.  Measured for the
-  // whole call, bf16, forward / forward and backward, us:
-  //   1024 tokens of 128 heads 109 / 486 by 64 columns, 134 / 544 by heads; of 160 heads 181 / 750 and 141 / 635
-  //   packed (sequences differ in length), 23 of 12289 tokens, 16 heads: 243 and 271; 7 of 6001: - / 632 and 751
+  // Half heads while the longest chain of chunks decides, whole ones when the chip is full.  Measured for the whole call,
+  // bf16 (fp32: the same order but where said), 12288 tokens, forward / forward and backward, us, by halves, by heads
+  // alone, by two heads on a CU:
+  //   equal rows of a batch: 128 heads 179 / 768, 216 / 885, 270 / 1004; 144: 261 / 995, 204 / 839, 238 / 854;
+  //     256: 177 / 738, 146 / 654, 168 / 657; 272: 227 / 889, 218 / 844, 210 / 795; 768: 191 / 740, 156 / 679, 154 / 661
+  // Packed sequences have lengths that only the device knows:
+  //   one of half of the tokens, the others alike: 144 heads 530 / 1738, 639 / 1971, 785 / 2066; 512: 553 / 1788, 677 / 2098,
+  //     827 / 2163; 1024: 578 / 1828, 700 / 2151, 850 / 2226
+  //   random: 160 heads 350 / 1242, 430 / 1446, 529 / 1489; 224: 281 / 1013, 300 / 1081, 359 / 1118; 368: 221 / 880, 222 / 860,
+  //     239 / 886; 512: 235 / 916, 226 / 874, 214 / 808 (fp32 424 / 1541, 422 / 1523, 396 / 1425); 1024: 246 / 925, 217 / 853, 216 / 825
+  //   all alike: as the rows of a batch
+  // Halves, the best for unequal lengths up to some 250 heads and within 6 % up to 512, cost at most 28 % (all alike);
+  // above, heads alone gain 7 to 20 % but for one long sequence (23 % lost); two on a CU gain nothing on them and lose 50 % there.
   const int64_t heads = (int64_t)N * Hv;
-  z.shape = heads <= (packed ? 384 : 128) ? kHalf : heads <= 256 ? kAlone : kTwo;
+  z.shape = heads <= (packed ? 512 : 128) ? kHalf : packed || heads <= 256 ? kAlone : kTwo;
   const int64_t length = packed ? nc / N : nc;               // of one sequence
   // Segments cost two passes over them and the join, and pay for few heads and long sequences:
   //   16 heads of 512 tokens 46 / 143 in one piece, 60 / 175 by segments; 768: 62 / 187 and 64 / 185; 1024: 78 / 231 and 69 / 195

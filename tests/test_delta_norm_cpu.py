@@ -207,6 +207,7 @@ def test_c_rule_shape(lib):
     assert f(1, 5, 1, 0, 2, 3, 1) == f(0, 5, 0, 0, 1, 1, 1) == f(1, 5, 1, 0, 1, 1, 7) == f(1, 2 ** 31 - 1, 1, 0, 1, 1, 1) == 0
     for dtype in (0, 1):
         assert [f(B, 100, B, 0, 16, 16, dtype) for B in (1, 8, 9, 16, 17, 40)] == [1, 1, 2, 2, 3, 3]
+        assert [f(1, 100 * N, N, 1, 16, 16, dtype) for N in (1, 9, 32, 33, 100)] == [1, 1, 1, 2, 2]
         assert f(1, 16384, 1, 0, 16, 16, dtype) == 6
 
 
