@@ -54,7 +54,8 @@ __global__ __launch_bounds__(256) void delta_step_kernel(StepArgs a) {
   for (int i = 0; i < kRows; ++i) s[i] = *reinterpret_cast<const floatx4*>(S + (group + kGroups * i) * 128);
 
   // Rows of the batch that name one state are one sequence's tokens, in the batch's order: the
-  // block of the first of them takes them all.
+  // block of the first of them takes them all.  Each block looks through all N indices, which grows with N squared
+  // (4 heads, without indices and with: 4096 rows 432 and 509 us, 8192 889 and 1214, 16384 1873 and 3350, 65535 7.7 and 42 ms).
   int more = 0;
   if (a.at) {
     if (tid == 0) found[0] = found[1] = 0;

@@ -207,7 +207,9 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     [slots,Hv,128,128] fp32, each matrix contiguous.  state_indices (int32 or int64 [N], on
     the device): the state of each row; row n has state n without it.  A row whose index is
     outside [0, slots) is padding: its output is 0 and no state changes.  Rows with the same
-    index are consecutive tokens of one sequence, in the batch's order.  At most 65535 rows.
+    index are consecutive tokens of one sequence, in the batch's order.  At most 65535 rows; with
+    state_indices the time grows with their square from some 8000 on (4096 rows: 1.2 times that
+    without, 65535: 5 times).
 
     Forward only: it raises where a gradient would be needed.
     """

@@ -549,7 +549,8 @@ int gsa_rms_norm_backward(const void* h, int64_t h_s0, int64_t h_s1, const void*
  * contiguous); v head h reads q/k head h / (Hv / Hk).  state [slots,Hv,128,128] fp32, each
  * matrix contiguous, strides multiples of 4.  state_idx (nullable: row n has state n; int32 or
  * int64 by idx_bytes): row n's state; one outside [0, slots) is padding: output 0, no state
- * changes.  Rows with the same state are consecutive tokens of it, in the batch's order.
+ * changes.  Rows with the same state are consecutive tokens of it, in the batch's order.  N up to
+ * 65535; every block looks through all indices (65535 rows: 5 times the time without them).
  * o [N,Hv,128] contiguous.
  */
 int gsa_delta_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int64_t k_sn, int64_t k_sh,
