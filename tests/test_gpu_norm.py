@@ -249,3 +249,33 @@ def test_more_rows_than_one_launch_dimension_holds(dev, D, rows, fp8):
         y, y1 = add_rms_norm(many, w, eps=EPS)[0], add_rms_norm(x[1:2], w, eps=EPS)[0]
     for a in range(0, rows, 1 << 22):
         assert bool((y[a:a + (1 << 22)] == y1).all()), a
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [128, 1000, 2048, 4096, 8200])
+def test_fp8_is_the_quotient(dev, D, dtype):
+    """y in 8 bits is the fp32 row divided by its scale and rounded, ties to even: bit for bit, ties among them
+    (quotients of bf16 products often lie between two values of e4m3)."""
+    x, _, w = _make((1000, D), dtype, False, D + 2)
+    x[7], x[8] = x[7] * 2.0 ** -100, 0
+    x, w = x.to(dev), w.to(dev)
+    w[3] = 2.0 ** 100 if D == 1000 else 1.0      # (a row's largest far above the others)
+    y, scale, _ = add_rms_norm_fp8(x, w, eps=EPS)
+    whole, _ = add_rms_norm(x.float(), w.float(), eps=EPS)
+    # on the CPU and by tensors: torch divides by a number as a product with its reciprocal
+    y, scale, whole = y.cpu(), scale.cpu(), whole.cpu()
+    big = whole.abs().amax(-1)
+    assert bool((scale == torch.where(big == 0, 1.0, big / torch.full_like(big, 448.0))).all())
+    want = (whole / scale[:, None].expand_as(whole)).clamp(-448, 448).to(torch.float8_e4m3fn)
+    same = y.view(torch.uint8) == want.view(torch.uint8)
+    assert bool(same.all()), f"{int((~same).sum())} of {same.numel()} differ"
+
+
+def test_fp8_of_an_infinite_row(dev):
+    """A weight that makes one value infinite: scale infinite, that value NaN, the others 0, as a division gives."""
+    x = torch.randn(4, 256, generator=torch.Generator().manual_seed(5)).to(dev)
+    w = torch.ones(256, device=dev)
+    x[:, 9], w[9] = 8.0, 3e38
+    y, scale, _ = add_rms_norm_fp8(x, w, eps=EPS)
+    rest = [i for i in range(256) if i != 9]
+    assert bool(scale.isinf().all()) and bool(y.float()[:, 9].isnan().all()) and not y.float()[:, rest].any()
