@@ -760,3 +760,27 @@ def test_no_gradient_of_what_has_no_effect(dev, dtype):
     most = dg.abs().max()
     # sums of some 64 x 64 terms in 64 bits: 2^-52 of each, of the size of the largest gradient
     assert float(dg[:, [0, 140]].abs().max() / most) <= 4096 * 2.0 ** -52
+
+
+def test_forward_mode(dev):
+    """A tangent raises, on the way forward and on the way back; beside one, calls without any are as ever."""
+    from torch.autograd import forward_ad as fw
+
+    x = _inputs(1, 70, 1, 1, torch.float32, seed=210)
+    leaf = _leaves(x, dev)
+    want = gated_delta_rule(*leaf)[0]
+    w = torch.ones(D, device=dev)
+    with fw.dual_level():
+        v = fw.make_dual(leaf[2].detach(), torch.ones_like(leaf[2]))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                gated_delta_rule(leaf[0], leaf[1], v, *leaf[3:])
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                add_rms_norm(v, w)
+        o = gated_delta_rule(*leaf)[0]
+        assert torch.equal(o, want)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(o, leaf, fw.make_dual(torch.ones_like(o), torch.ones_like(o)), retain_graph=True)
+        d = torch.autograd.grad(o, leaf, torch.ones_like(o))
+    for a, b in zip(d, torch.autograd.grad(want, leaf, torch.ones_like(o))):
+        assert torch.equal(a, b)
