@@ -464,7 +464,9 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
 //   <8, two buffers> and <4, two buffers>: a head and half a head a block, one block a CU; the
 //     next chunk's operands are on their way during the whole of this one's products
 // Bound by the issue of instructions, the matrix ones and the splits of fp32 into bf16 parts, which
-// do not overlap within a SIMD; a quarter of the cycles wait (loads of V and the barriers).  A
+// do not overlap within a SIMD, where four waves share it (the segments' passes: three quarters of its
+// cycles at 4 x 4096 tokens of 16 heads); the outputs' scan has two, and of its cycles 28 % are the matrix
+// instructions', some 30 % the VALU's, the others go with waits for V, LDS and at the barriers.  A
 // chunk of 64 takes 4.1 us by half heads, 5.9 by whole ones (8 on a full chip), 13 where two blocks
 // share a CU.
 // ---------------------------------------------------------------------------
@@ -1054,7 +1056,7 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_bwd_kernel(
 // product of transitions: S <- move S + add (dS <- move^T dS + add), segment after segment.  512
 // threads and 16 columns a block: a wave owns the rows tile_row(wave, .), the state goes round
 // through LDS.  A wave's rows of move and add come by direct loads, two segments ahead, to places of
-// its own (loads to registers that far ahead were waited for at each turn of the loop).  1.9 us a
+// its own (loads to registers that far ahead were waited for at each turn of the loop).  1.9 to 2.4 us a
 // segment, most of it the parts of move's rows, which only 16 columns share.
 constexpr int kJoinWave = 9 * kUnit;                         // 8 of move, 1 of add
 constexpr size_t kJoinLds = 2 * 8 * kJoinWave + 12 * kUnit;
@@ -1724,7 +1726,7 @@ DeltaSizes delta_sizes(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   //   16 heads of 512 tokens 46 / 143 in one piece, 60 / 175 by segments; 768: 62 / 187 and 64 / 185; 1024: 78 / 231 and 69 / 195
   //   64 heads of 1024 tokens 88 / 312 and 100 / 330; 2048: 169 / 627 and 165 / 586; 80 heads of 4096: 377 / 1460 and 406 / 1418
   if (heads <= 64 && length >= std::max<int64_t>(12, heads / 2 - 4)) {
-    // a block a CU, of at least 4 chunks (16384 tokens of 16 heads: 16 segments 323 us, 32 356); joining costs 1.9 us a
+    // a block a CU, of at least 4 chunks (16384 tokens of 16 heads: 16 segments 323 us, 32 356); joining costs some 2 us a
     // segment and the two passes 16 us a chunk of one: more than sqrt(8 chunks) segments lose
     int64_t pieces = 256 / heads;
     while (pieces > 3 && pieces * pieces > 8 * length) --pieces;
