@@ -321,6 +321,7 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
   __shared__ __align__(16) char xbuf[kX];                    // K's rows, then the inverse
   __shared__ __align__(16) float ybuf[C == 32 ? 16 * LD : 1];
   __shared__ float gh[C], gl[C], bt[C];
+  __shared__ int first;                                      // the first row of A that is not finite
   float (*xm)[LD] = reinterpret_cast<float (*)[LD]>(xbuf);
   bf16x8* sk = reinterpret_cast<bf16x8*>(xbuf);
   const int slot = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, share = a.Hv / a.Hk, hk = h / share, tid = threadIdx.x, wave = tid >> 6, l = lane_id();
@@ -333,6 +334,7 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
   const int64_t at = (int64_t)slot * a.Hv + h, atk = (int64_t)slot * a.Hk + hk;
 
   stage_rows<T>(sk, a.k, sp, t0, left, hk, tid);
+  if (tid == 0) first = C;
   if (wave == 0) {
     const bool ok = l < C && l < left;
     float g = 0.f, b = 0.f;
@@ -383,6 +385,7 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
 
   // row tile mt of Q K^T (into am, packed as P) and of K K^T (into am behind it)
   floatx4 kk[MT];
+  float odd = 0.f;
 #pragma unroll
   for (int nt = 0; nt < MT; ++nt) {
     if ((nt >> 1) > (mt >> 1)) continue;                     // (the upper right half is not read)
@@ -399,11 +402,20 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
     for (int r = 0; r < 4; ++r) {
       const int i = tile_row(mt, 4 * g4 + r);
       const float d = j <= i ? decay((gh[i] - gh[j]) + (gl[i] - gl[j])) : 0.f;
-      if (C == 64 || wave >= MT) am[i][j] = a.scale * qk[r] * d;
+      if (C == 64 || wave >= MT) am[i][j] = j <= i ? a.scale * qk[r] * d : 0.f;
       kk[nt][r] = j < i ? bt[i] * kk[nt][r] * d : 0.f;
+      odd = __builtin_fmaf(kk[nt][r], 0.f, odd);
     }
   }
+  if (odd != 0.f)                                            // a NaN or an infinity: the tokens before it do without
+#pragma unroll
+    for (int nt = 0; nt < MT; ++nt)
+      if ((nt >> 1) <= (mt >> 1))
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (kk[nt][r] * 0.f != 0.f) atomicMin(&first, tile_row(mt, 4 * g4 + r));
   __syncthreads();
+  const int cut = first;
   pack_square<C, K::kPParts, kBwd>(a.pm + at * K::kP * kUnit, &am[0][0], LD, tid);
   for (int i = tid; i < C / 32 * 256; i += 256)              // above the diagonal of 32 by 32: 0
     xm[32 * (i >> 8) + (i >> 4 & 15)][32 * (i >> 8) + 16 + (i & 15)] = 0.f;
@@ -413,7 +425,7 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
     for (int nt = 0; nt < MT; ++nt)
       if ((nt >> 1) <= (mt >> 1))
 #pragma unroll
-        for (int r = 0; r < 4; ++r) am[tile_row(mt, 4 * g4 + r)][tile_row(nt, m)] = kk[nt][r];
+        for (int r = 0; r < 4; ++r) am[tile_row(mt, 4 * g4 + r)][tile_row(nt, m)] = tile_row(mt, 4 * g4 + r) < cut ? kk[nt][r] : 0.f;
   __syncthreads();
 
   // (I + A)^-1: blocks of 16 by substitution, a lane a column; then pairs of blocks, and of pairs:
@@ -449,6 +461,11 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(DeltaArgs a) {
     tile_put(ym + i * LD + j, LD, tile_f32(&am[32 + i][0], LD, &xm[0][j], LD, 32), 1.f);
     __syncthreads();
     tile_put(&xm[32 + i][j], LD, tile_f32(&xm[32 + i][32], LD, ym + j, LD, 32), -1.f);
+    __syncthreads();
+  }
+  if (cut < C) {                                             // (the same for all)
+    for (int i = tid; i < C * C; i += 256)
+      if (i / C >= cut && i % C <= i / C) xm[i / C][i % C] = __builtin_nanf("");
     __syncthreads();
   }
   pack_square<C, 3, kBwd>(a.tm + at * K::kT * kUnit, &xm[0][0], LD, tid);
@@ -732,6 +749,50 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_kernel(Delt
           if (kOut) O[mt][n][r] *= a.scale * e[r];
         }
     }
+    // A NaN or an infinity in a column of R: the rows before it are computed without it (a product's zeros above the
+    // diagonal would carry it there), the others become NaN.  The first such row waits in the place of the wave's V.
+    // (The search costs 1 to 2 % of the half heads' scan, nothing by heads.)
+    auto note = [&](int n) { return reinterpret_cast<int*>(lds + bv) + 64 * n + here(l); };
+    auto fill = [&](floatx4 (&x)[MT][NT], float with) {
+      asm volatile("" ::: "memory");
+      const int g8 = here(8 * g);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int bad = *note(n);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[mt][n][r] = g8 + tile_at(mt, r) >= bad ? with : x[mt][n][r];
+      }
+      asm volatile("" ::: "memory");
+    };
+    bool any = false;
+    if constexpr (kOut) {
+      float odd = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) odd = __builtin_fmaf(X[mt][n][r], 0.f, odd);
+      any = __builtin_amdgcn_ballot_w64(odd != 0.f) != 0;
+      if (__builtin_expect(any, 0)) {
+        asm volatile("" ::: "memory");
+        const int g8 = here(8 * g);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          int bad = C;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (X[mt][n][r] * 0.f != 0.f) bad = min(bad, g8 + tile_at(mt, r));
+          bad = min(bad, __shfl_xor(bad, 16, 64));
+          *note(n) = min(bad, __shfl_xor(bad, 32, 64));
+        }
+        fill(X, 0.f);
+      }
+    }
     floatx4 U[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -751,6 +812,7 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_kernel(Delt
     if (!Sh::kDouble) __syncthreads();                       // Tm is free
     if (more && !Sh::kDouble) fetch<W>(a.tm + (at + a.Hv) * K::kT * kUnit, base + bt, K::kT, wave, l);
     if constexpr (kOut) {
+      if (__builtin_expect(any, 0)) fill(U, 0.f);
 #pragma unroll
       for (int js = 0; js < JS; ++js) {
         Parts<K::kPParts> u[NT];
@@ -766,6 +828,10 @@ __global__ __launch_bounds__(64 * Sh::W, Sh::kWaves) void delta_scan_kernel(Delt
                                           staged<K::kPParts>(spm, Square<C>::at(mt + 1, js, false), l)};
           mma_grid(O + mt, x, u);
         }
+      }
+      if (__builtin_expect(any, 0)) {
+        fill(U, __builtin_nanf(""));
+        fill(O, __builtin_nanf(""));
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)

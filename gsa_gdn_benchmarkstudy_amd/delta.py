@@ -153,10 +153,10 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
 
     cu_seqlens (int32 or int64 [N+1], on the device, ascending from 0): B is 1 and N sequences
     are packed in T, each with its own state; empty ones are allowed.  Rows of o and of the
-    gradients outside every sequence are 0, whatever the inputs hold there.  Within a sequence a
-    NaN or an infinity may reach every token of its chunk of 64 (fp32: 32), those before it too:
-    padding behind the tokens of a batch's row has to be finite (its outputs are to be
-    ignored), or left out by packing.
+    gradients outside every sequence are 0, whatever the inputs hold there.  A NaN or an
+    infinity of a token reaches no output before it, so padding behind the tokens of a batch's row
+    may hold anything (its outputs are to be ignored).  Gradients it reaches, as 0 * NaN does in
+    the recurrence's own: where they are wanted, padding has to be finite, or left out by packing.
 
     Differentiable in q, k, v, g, beta and initial_state, once and backwards (a tangent of
     torch.autograd.forward_ad raises); the gradients are the same bits on every run.  A forward

@@ -571,8 +571,8 @@ int gsa_delta_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int
  * state_in, state_out (nullable) fp32 [N,Hv,128,128]; o [B,T,Hv,128] contiguous.
  * At most 2^23 chunks (of 64 tokens, fp32: 32; one more for each packed sequence) times Hv, and N Hv below
  * 2^23: the byte counts below are 0 for what is refused.
- * No output overlaps an input (state_out is not state_in).  A NaN or an infinity of a token may
- * reach all tokens of its chunk of 64 (fp32: 32), those before it too.
+ * No output overlaps an input (state_out is not state_in).  A NaN or an infinity of a token
+ * reaches no output before it; gradients before it it may reach.
  * ws: gsa_delta_rule_workspace_bytes(..., backward).  saved (nullable in the forward):
  * gsa_delta_rule_saved_bytes, the states and deltas that gsa_delta_rule_backward reads.
  *

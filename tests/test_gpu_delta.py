@@ -784,3 +784,69 @@ def test_forward_mode(dev):
         d = torch.autograd.grad(o, leaf, torch.ones_like(o))
     for a, b in zip(d, torch.autograd.grad(want, leaf, torch.ones_like(o))):
         assert torch.equal(a, b)
+
+
+def _not_finite(t):
+    return ~torch.isfinite(t.float())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,T,Hk,Hv,lens", [(1, 150, 2, 2, None), (10, 150, 8, 16, None), (20, 150, 8, 16, None), (1, 1500, 1, 2, None),
+                                            (1, 150, 1, 2, [5, 100, 45])])
+def test_nothing_reaches_tokens_before_it(dev, B, T, Hk, Hv, lens, dtype):
+    """A NaN or an infinity in any input of a token leaves the bits of all outputs before it, of other rows and, in v, of
+    other columns; behind it a NaN shows wherever the recurrence has it."""
+    x = {n: t.to(dev) for n, t in _inputs(B, T, Hk, Hv, dtype, seed=220).items()}
+    cu = None if lens is None else torch.tensor([0] + lens, device=dev).cumsum(0)
+    state = torch.randn(B if lens is None else len(lens), Hv, D, D, generator=torch.Generator().manual_seed(6)).to(dev)
+
+    def run(y):
+        return gated_delta_rule(*(y[n] for n in NAMES), initial_state=state, output_final_state=True, cu_seqlens=cu)
+
+    want, S0 = run(x)
+    b, end = (B - 1, T) if lens is None else (0, 105)             # the row, and the end of the sequence that holds the token
+    seq = b if lens is None else 1
+    for t in ((0, 31, 40, 63, 64, T - 1) if lens is None else (5, 36, 69, 104)):
+        for name in NAMES:
+            for value in (float("nan"), float("inf"), -float("inf")):
+                if name == "g" and value < 0:
+                    continue                                      # (a reset)
+                y = dict(x)
+                y[name] = x[name].clone()
+                where = (b, t, 0, 77) if name in ("q", "k", "v") else (b, t, 0)
+                y[name][where] = value
+                o, S = run(y)
+                hv = slice(0, 1) if name in ("v", "g", "beta") else slice(0, Hv // Hk)    # the v heads that it enters
+                same = torch.ones_like(want, dtype=torch.bool)
+                same[(b, slice(t, t + 1 if name == "q" else end), hv, 77 if name == "v" else slice(None))] = False
+                case = f"{name} {value} at {t}"
+                assert torch.equal(o[same], want[same]), case
+                if name == "q":
+                    assert torch.equal(S, S0), case
+                else:
+                    assert torch.equal(S[:, hv.stop:], S0[:, hv.stop:]), case
+                    keep = [i for i in range(S.shape[0]) if i != seq]
+                    assert torch.equal(S[keep], S0[keep]), case
+                    if name == "v":
+                        cols = [c for c in range(D) if c != 77]
+                        assert torch.equal(S[seq][..., cols], S0[seq][..., cols]), case
+                if value != value:
+                    assert bool(_not_finite(o[~same]).all()), case
+                    if name == "v":
+                        assert bool(S[seq, 0, :, 77].isnan().all()), case
+                    elif name != "q":
+                        assert bool(S[seq, hv].isnan().all()), case
+
+
+def test_padding_of_any_kind(dev):
+    """Rows of a batch padded behind their ends with what was in memory: real tokens as without it."""
+    lens = [150, 64, 1, 97, 130]
+    x = _inputs(5, 150, 2, 4, torch.bfloat16, seed=221)
+    real = torch.arange(150)[None] < torch.tensor(lens)[:, None]
+    outs = []
+    for fill in (0.0, float("nan"), float("inf")):
+        y = {n: t.clone() for n, t in x.items()}
+        for t in y.values():
+            t[~real] = fill
+        outs.append(gated_delta_rule(*(y[n].to(dev) for n in NAMES))[0].cpu()[real])
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
