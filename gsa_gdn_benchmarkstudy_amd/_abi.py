@@ -49,6 +49,8 @@ EXPORTS = (
     "gsa_rms_norm", "gsa_rms_norm_fp8", "gsa_rms_norm_backward", "gsa_rms_norm_backward_workspace_bytes",
     "gsa_delta_step", "gsa_delta_rule", "gsa_delta_rule_backward", "gsa_delta_rule_workspace_bytes",
     "gsa_delta_rule_saved_bytes", "gsa_delta_rule_shape",
+    "gsa_linear_attn", "gsa_linear_attn_backward", "gsa_linear_attn_workspace_bytes", "gsa_linear_attn_saved_bytes",
+    "gsa_linear_step",
 )
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
@@ -66,6 +68,19 @@ class DeltaArgs(ctypes.Structure):
                    ("ws_bytes", ctypes.c_size_t), ("saved", _vp), ("saved_bytes", ctypes.c_size_t), ("dout", _vp)]
                 + [(n, _i64) for n in ("do_sb", "do_st", "do_sh")]
                 + [(n, _vp) for n in ("dstate_out", "dq", "dk", "dv", "dg", "dbeta", "dstate_in")])
+
+
+class LinearArgs(ctypes.Structure):
+    """gsa_linear_args of include/gsa_hip.h."""
+
+    _fields_ = ([(n, _vp) for n in ("q", "k", "v", "g")]
+                + [(f"{n}_{s}", _i64) for n in ("q", "k", "v") for s in ("sb", "st", "sh")]
+                + [("g_sh", _i64), ("cu_seqlens", _vp)]
+                + [(n, _i32) for n in ("cu_bytes", "B", "T", "N", "Hk", "Hv", "d", "dtype")]
+                + [("scale", _f32), ("state_in", _vp), ("o", _vp), ("state_out", _vp), ("ws", _vp),
+                   ("ws_bytes", ctypes.c_size_t), ("saved", _vp), ("saved_bytes", ctypes.c_size_t), ("dout", _vp)]
+                + [(n, _i64) for n in ("do_sb", "do_st", "do_sh")]
+                + [(n, _vp) for n in ("dstate_out", "dq", "dk", "dv", "dg", "dstate_in")])
 
 
 _PROTOS = {
@@ -136,6 +151,12 @@ _PROTOS = {
     "gsa_delta_rule_shape": ([_i32] * 7, _i32),
     "gsa_delta_rule": ([ctypes.POINTER(DeltaArgs), _vp], _i32),
     "gsa_delta_rule_backward": ([ctypes.POINTER(DeltaArgs), _vp], _i32),
+    "gsa_linear_attn_workspace_bytes": ([_i32] * 8, ctypes.c_size_t),
+    "gsa_linear_attn_saved_bytes": ([_i32] * 7, ctypes.c_size_t),
+    "gsa_linear_attn": ([ctypes.POINTER(LinearArgs), _vp], _i32),
+    "gsa_linear_attn_backward": ([ctypes.POINTER(LinearArgs), _vp], _i32),
+    "gsa_linear_step": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _i64, _i32, _i32, _i32,
+                         _i32, _i32, _f32, _i32, _vp, _vp], _i32),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -1083,3 +1104,87 @@ def delta_rule_backward(q, k, v, g, beta, cu, scale: float, saved, dout, dstate,
     if st:
         _check(st, "gsa_delta_rule_backward")
     return dq, dk, dv, dg, db, ds
+
+
+# ---------------------------------------------------------------------------
+# Linear attention with decays
+# ---------------------------------------------------------------------------
+
+def linear_step(q, k, v, g, state, idx, scale: float) -> torch.Tensor:
+    """gsa_linear_step: o [N,Hv,128]; `state` is updated in place."""
+    N, Hv, d = v.shape
+    (qn, qh, qe), (kn, kh, ke), (vn, vh, ve) = q.stride(), k.stride(), v.stride()
+    if qe != 1 or ke != 1 or ve != 1:
+        return linear_step(q.contiguous(), k.contiguous(), v.contiguous(), g, state, idx, scale)
+    o = torch.empty(N, Hv, d, device=v.device, dtype=v.dtype)
+    st = load().gsa_linear_step(q.data_ptr(), qn, qh, k.data_ptr(), kn, kh, v.data_ptr(), vn, vh, g.data_ptr(), g.stride(0),
+                                _ptr(idx), 0 if idx is None else idx.element_size(), state.data_ptr(), *state.stride()[:2], N,
+                                state.shape[0], q.shape[1], Hv, d, scale, dtype_code(q.dtype), o.data_ptr(), _raw_stream(v))
+    if st:
+        _check(st, "gsa_linear_step")
+    return o
+
+
+def _linear_args(q, k, v, g, state_in, cu, scale: float) -> LinearArgs:
+    B, T, Hv, d = v.shape
+    # in the order of the fields
+    return LinearArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                      g.stride(0), _ptr(cu), 0 if cu is None else cu.element_size(), B, T, B if cu is None else cu.numel() - 1,
+                      q.shape[2], Hv, d, dtype_code(q.dtype), scale, _ptr(state_in))
+
+
+@functools.lru_cache(maxsize=256)
+def _linear_bytes(*sizes: int):
+    """Bytes of workspace forward and backward, and of what a forward keeps."""
+    lib = load()
+    forward = lib.gsa_linear_attn_workspace_bytes(*sizes, 0)
+    if forward == ctypes.c_size_t(-1).value:
+        raise ValueError(f"{sizes[0]} x {sizes[1]} tokens in {sizes[2]} sequences of {sizes[5]} heads: over 2**23 chunks times heads, "
+                         "or 2**23 sequences times heads")
+    return forward, lib.gsa_linear_attn_workspace_bytes(*sizes, 1), lib.gsa_linear_attn_saved_bytes(*sizes)
+
+
+def linear_attn(q, k, v, g, state_in, cu, scale: float, want_state: bool, want_saved: bool):
+    """gsa_linear_attn: (o, state_out or None, saved or None).  q, k, v as _heads gives them."""
+    B, T, Hv, d = v.shape
+    if B * T == 0:                               # nothing to launch: the states as they came
+        n = B if cu is None else cu.numel() - 1
+        state = None if not want_state else v.new_zeros(n, Hv, d, d, dtype=torch.float32) if state_in is None else state_in.clone()
+        return v.new_empty(v.shape), state, v.new_empty(0, dtype=torch.uint8) if want_saved else None
+    a = _linear_args(q, k, v, g, state_in, cu, scale)
+    forward, _, keep = _linear_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
+    o = torch.empty(B, T, Hv, d, device=v.device, dtype=v.dtype)
+    state = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_state else None
+    ws = torch.empty(forward, device=v.device, dtype=torch.uint8)
+    a.o, a.state_out, a.ws, a.ws_bytes = o.data_ptr(), _ptr(state), ws.data_ptr(), forward
+    saved = None
+    if want_saved:
+        saved = torch.empty(keep, device=v.device, dtype=torch.uint8)
+        a.saved, a.saved_bytes = saved.data_ptr(), keep
+    st = load().gsa_linear_attn(ctypes.byref(a), _raw_stream(v))
+    if st:
+        _check(st, "gsa_linear_attn")
+    return o, state, saved
+
+
+def linear_attn_backward(q, k, v, g, state_in, cu, scale: float, saved, dout, dstate, want_dg: bool, want_dstate: bool):
+    """gsa_linear_attn_backward: (dq, dk, dv, dg or None, dstate_in or None)."""
+    B, T, Hv, d = v.shape
+    if B * T == 0:
+        n = B if cu is None else cu.numel() - 1
+        ds = None if not want_dstate else v.new_zeros(n, Hv, d, d, dtype=torch.float32) if dstate is None else dstate.clone()
+        return (*(t.new_empty(t.shape) for t in (q, k, v)), torch.zeros_like(g) if want_dg else None, ds)
+    a = _linear_args(q, k, v, g, state_in, cu, scale)
+    dq, dk, dv = [torch.empty(t.shape, device=v.device, dtype=t.dtype) for t in (q, k, v)]
+    dg = torch.empty(Hv, device=v.device, dtype=torch.float32) if want_dg else None
+    ds = torch.empty(a.N, Hv, d, d, device=v.device, dtype=torch.float32) if want_dstate else None
+    _, a.ws_bytes, a.saved_bytes = _linear_bytes(B, T, a.N, int(cu is not None), a.Hk, Hv, a.dtype)
+    ws = torch.empty(a.ws_bytes, device=v.device, dtype=torch.uint8)
+    a.ws, a.saved = ws.data_ptr(), saved.data_ptr()
+    a.dout, (a.do_sb, a.do_st, a.do_sh, _) = dout.data_ptr(), dout.stride()
+    a.dstate_out, a.dstate_in = _ptr(dstate), _ptr(ds)
+    a.dq, a.dk, a.dv, a.dg = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dg)
+    st = load().gsa_linear_attn_backward(ctypes.byref(a), _raw_stream(v))
+    if st:
+        _check(st, "gsa_linear_attn_backward")
+    return dq, dk, dv, dg, ds

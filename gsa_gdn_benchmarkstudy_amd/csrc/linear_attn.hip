@@ -1,0 +1,666 @@
+// Linear attention with a decay for each head over whole sequences, forward and backward, in chunks of C tokens.
+//
+//   S_t = a S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t,   a = e^g          (S [128 x 128], fp32)
+//
+// In a chunk, with X the state before it and D_ij = a^(i-j) (j <= i):
+//   O = scale a^(i+1) Q X + (scale Q K^T * D) V       X' = a^C X + sum_j a^(C-1-j) k_j v_j^T
+// The gradients are the same sum with other operands, two of them from the last token to the first:
+//   dq: rows dO, keys V, values K, X = S^T
+//   dk: rows V, keys dO, values Q, X = D^T, backwards;   dv: rows K, keys Q, values dO, X = D, backwards
+// (D_t = a D_{t+1} + scale q_t do_t^T from the gradient of the final state).  So one kernel (linear_scan_kernel) does all
+// four: a Pass names its operands, its direction and where scale goes.  dg = sum_t <D_t, a S_{t-1}> counts the decays
+// between each query i and key j, i - j of them, by positive terms alone (differences of sums over the sequence would cancel):
+//   inside a chunk          sum_ij (i - j) P_ij (do_i . v_j)
+//   from the key's chunk    its tokens behind the key times the key's part of dk that comes from X
+//   to the query's chunk    its tokens up to the query times the query's part of dq that comes from X
+//   chunks in between       X2, the state with each term times the tokens of the chunks that it has crossed
+//
+// Long sequences of few heads are cut into segments: what each adds to the state from 0 (a pass of the same kernel without
+// outputs), the states between them (linear_join_kernel), all segments' outputs at once.
+//
+// Precision: as the gated delta rule's (mma): fp32 operands enter products as sums of three bf16 parts.  Where only a bf16
+// output depends on them two parts do, 2^-17 of a term under a rounding of 2^-9: X in Q X and P in P V (not where dg is
+// summed from the product).
+#include "chunks.h"
+
+namespace gsa {
+
+constexpr int kWaves = 8;                                    // of a block: 16 columns of the state each
+
+// One sum over the tokens of every sequence.  Heads of q and k (shared) or of v.
+struct Pass {
+  Rows a, b, v, dot;                                         // rows, keys, values; dot: q (dq) or k (dk), for dg
+  int a_shared, b_shared, v_shared;                          // whose rows are those of a q/k head
+  int back, turn;                                            // from the last token to the first; X transposed in memory
+  float in_p, in_x, in_o;                                    // scale of P, of what enters X, of A X
+  const float* first;                                        // [N, Hv, 128, 128]: X before the first token, nullable
+  const float* init;                                         // [segments, Hv, 128, 128]: X before the others' segments
+  const float *far_first, *far;                              // dq: the same of D, for dg
+  void* out;                                                 // [B, T, Hv, 128]; parts: fp32
+  int out_parts;
+  float* last;                                               // [N, Hv, 128, 128]: X behind the last token (back: times a), nullable
+  float* add;                                                // without outputs: X behind a segment from 0
+};
+struct LinearArgs {
+  Seqs s;
+  int Hk, Hv, units, seg;                                    // units: heads of all sequences, or of all segments of seg chunks
+  const float* g; int64_t g_sh;
+  float* dg_parts;                                           // [2][units]
+  Pass pass[3];
+};
+
+// g in units of log2.  e^-128 is 0 in fp32: a lower g (down to -inf, a reset) gives the same without inf * 0.
+__device__ __forceinline__ float log2_decay(const float* g) {
+  const float x = *g;
+  return (x < -128.f ? -128.f : x) * kLog2e;
+}
+__device__ __forceinline__ float power(float g2, int n) { return __builtin_amdgcn_exp2f(g2 * (float)n); }
+
+// P enters a product with bf16 outputs in two parts
+template <typename T, int kDg> struct LinearSizes {
+  static constexpr int C = ChunkType<T>::kChunk, NP = ChunkType<T>::kParts;
+  static constexpr int kPParts = NP == 1 ? 2 : 3, kXParts = NP == 1 && !kDg ? 2 : 3;
+  static constexpr int kRows = (C / 16) * 4 * NP * kUnit, kP = Square<C>::kFrags * kPParts * kUnit, kStage = C * kHead * sizeof(T);
+  static constexpr int kB = 0, kV = kRows, kA = 2 * kRows, kAtP = 3 * kRows, kAtStage = kAtP + kP, kDot = kAtStage + kStage;
+  static constexpr size_t kBytes = kDot + (kDg ? kRows : 0), kState = 2 * kRows;
+};
+
+// A state [128][128] in memory -> the lane's part: rows tile_row(t, 4 g + r), column `col`
+__device__ __forceinline__ void state_load(floatx4 (&S)[8][1], const float* p, int turn, int g, int col) {
+  p = uniform(p);
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const int row = 8 * g + tile_at(t, 0);
+    if (turn) {
+      S[t][0] = *reinterpret_cast<const floatx4*>(p + (uint32_t)(col * kHead + row));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[t][0][r] = p[(uint32_t)((row + r) * kHead + col)];
+    }
+  }
+}
+__device__ __forceinline__ void state_store(const floatx4 (&S)[8][1], float* p, float f, int g, int col) {
+  p = const_cast<float*>(uniform(p));
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[(uint32_t)((8 * g + tile_at(t, r)) * kHead + col)] = S[t][0][r] * f;
+}
+
+// kOut: the outputs; otherwise what a segment adds to X.  kDg: this pass's part of dg: 1 dq's, 2 dk's.
+template <typename T, bool kOut, int kDg>
+__device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, char* lds, float* dg_part) {
+  using Z = LinearSizes<T, kDg>;
+  constexpr int C = Z::C, NP = Z::NP, MT = C / 16, JS = C / 32;
+  const uint32_t base = lds_addr(lds);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id(), g = l >> 4, m = l & 15;
+  const int slot = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, hk = h / (a.Hv / a.Hk);
+  int piece = 0, c0 = 0;
+  Span sp;
+  if (a.seg) {
+    sp = slot_of(a.s, slot, C * a.seg, piece);
+    if (piece < 0) {
+      if (kDg && tid == 0) *dg_part = 0.f;
+      return;
+    }
+    c0 = piece * a.seg;
+  } else {
+    sp = span_of(a.s, slot, C);
+  }
+  const int chunks = (sp.len + C - 1) / C;
+  const bool last = !a.seg || c0 + a.seg >= chunks;
+  const int c1 = last ? chunks : c0 + a.seg;
+  const bool begins = x.back ? last : piece == 0, ends = x.back ? piece == 0 : last;    // the pass's first and last segment
+  if (!kOut && ends) return;                                 // nobody asks for it
+  const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)slot * a.Hv + h) * kHead * kHead;
+  const float g2 = log2_decay(a.g + h * a.g_sh);
+  const int col = tile_row(wave, m);                         // this lane's column of the state and the outputs
+
+  floatx4 X[8][1], X2[kDg == 1 ? 8 : 1];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) X[t][0] = floatx4{0.f, 0.f, 0.f, 0.f};
+  if constexpr (kDg == 1)
+#pragma unroll
+    for (int t = 0; t < 8; ++t) X2[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  if (kOut) {
+    const float* from = begins ? (x.first ? x.first + sn : nullptr) : x.init + gn;
+    if (from) state_load(X, from, x.turn, g, col);
+  }
+
+  // token i of the pass in chunk c is token at(i) of the chunk's rows
+  const int rs = row_slot(g, m), place = cols_place(l);
+  auto fetch = [&](const Rows& r, int shared, int c, int to) {
+    const int left = min(C, sp.len - c * C), hh = shared ? hk : h;
+    if constexpr (NP == 1) {
+      const uint16_t* p = uniform(row_at<uint16_t>(r, sp, (int64_t)c * C, hh));
+      const int mm = (l - 4 * g) & 15;                       // (row_slot)
+#pragma unroll
+      for (int i = 0; i < C / 4 / kWaves; ++i) {
+        const int f = wave + kWaves * i, t = min(tile_row(f >> 2, mm), left - 1);
+        load_lds16(p, (uint32_t)((x.back ? left - 1 - t : t) * (int)r.st + 32 * (f & 3) + 8 * g) * 2u,
+                   __builtin_amdgcn_readfirstlane(base + to + f * kUnit));
+      }
+    } else {
+      bf16x8* dst = reinterpret_cast<bf16x8*>(lds + to);
+      for (int u = tid; u < C * 16; u += 64 * kWaves) {
+        const int d8 = u & 15, i = u >> 4, t = min(i, left - 1);
+        const int tile = 2 * (i >> 5) + ((i >> 2) & 1), mm = 4 * ((i >> 3) & 3) + (i & 3);
+        const Parts<NP> p = operand<T>(row_at<T>(r, sp, (int64_t)c * C + (x.back ? left - 1 - t : t), hh) + 8 * d8, true);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) dst[((tile * 4 + (d8 >> 2)) * NP + n) * 64 + row_slot(d8 & 3, mm)] = p.p[n];
+      }
+    }
+  };
+  const int step = x.back ? -1 : 1;
+  float dg = 0.f;
+  int c = x.back ? c1 - 1 : c0;
+  if (c0 < c1) {
+    fetch(x.b, x.b_shared, c, Z::kB);
+    fetch(x.v, x.v_shared, c, Z::kV);
+    if (kOut) fetch(x.a, x.a_shared, c, Z::kA);
+    if (kDg) fetch(x.dot, 1, c, Z::kDot);
+  }
+  for (int n = c0; n < c1; ++n, c += step) {
+    const bool more = n + 1 < c1;
+    const int left = min(C, sp.len - c * C);
+    // steps of decay from X to the chunk's first token: 1, or (the gradient of the final state) 0
+    const int lead = x.back && c == chunks - 1 ? 0 : 1;
+    const float whole = power(g2, left - 1 + lead);
+    wait_loads();
+    __syncthreads();
+
+    floatx4 O[MT][1];
+    if constexpr (kOut) {
+      // P: row tile mt by MT waves, the others take the columns behind
+      const int mt = wave % MT, part = wave / MT;
+      char* pm = lds + Z::kAtP;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int nt = C == 64 && mt >= 2 ? 2 * part + k : part;
+        if (nt >= MT || (k == 1 && (C == 32 || mt < 2))) continue;
+        floatx4 qk = {0.f, 0.f, 0.f, 0.f}, kv = qk;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          mma(qk, rows_of<NP>(lds + Z::kA, mt, ks, rs), rows_of<NP>(lds + Z::kB, nt, ks, rs));
+          if constexpr (kDg == 1) mma(kv, rows_of<NP>(lds + Z::kDot, mt, ks, rs), rows_of<NP>(lds + Z::kV, nt, ks, rs));
+        }
+        const int j = tile_row(nt, m);
+        const int at = Square<C>::at(mt, nt >> 1, false) * Z::kPParts * kUnit + 16 * (16 * (m >> 2) + 4 * g) + 2 * (4 * (nt & 1) + (m & 3));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = tile_row(mt, 4 * g + r);
+          float p = j <= i ? x.in_p * qk[r] * power(g2, i - j) : 0.f;
+          if constexpr (kDg == 1)
+            if (i < left) dg = __builtin_fmaf(p * (float)(i - j), j < i ? kv[r] : 0.f, dg);
+#pragma unroll
+          for (int e = 0; e < Z::kPParts; ++e) {
+            const __bf16 y = (__bf16)p;
+            *reinterpret_cast<__bf16*>(pm + at + e * kUnit + 16 * r) = y;
+            p -= (float)y;
+          }
+        }
+      }
+      // A X
+#pragma unroll
+      for (int i = 0; i < MT; ++i) O[i][0] = floatx4{0.f, 0.f, 0.f, 0.f};
+      floatx4 O2[MT][1];
+      if constexpr (kDg == 1)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) O2[i][0] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        Parts<NP> r[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) r[i] = rows_of<NP>(lds + Z::kA, i, ks, rs);
+        auto pair = [&](const floatx4& u, const floatx4& v, floatx4 (&to)[MT][1]) {
+          const float y[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+          const Parts<Z::kXParts> p[1] = {parts_of<Z::kXParts>(y)};
+          mma_grid(to, r, p);
+        };
+        pair(X[2 * ks][0], X[2 * ks + 1][0], O);
+        if constexpr (kDg == 1) pair(X2[2 * ks], X2[2 * ks + 1], O2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = tile_row(i, 4 * g + r);
+          const float e = x.in_o * power(g2, t + lead);
+          O[i][0][r] *= e;
+          if constexpr (kDg != 0) {
+            if (t < left) {
+              const int at = ((i * 4 + (col >> 5)) * NP) * kUnit + 16 * row_slot((col >> 3) & 3, 4 * g + r) + 2 * (col & 7);
+              float y = 0.f;
+#pragma unroll
+              for (int e2 = 0; e2 < NP; ++e2) y += (float)*reinterpret_cast<const __bf16*>(lds + Z::kDot + at + e2 * kUnit);
+              if constexpr (kDg == 1) dg = __builtin_fmaf(y, __builtin_fmaf(O[i][0][r], (float)(t + 1), O2[i][0][r] * e), dg);
+              else dg = __builtin_fmaf(y, O[i][0][r] * (float)t, dg);
+            }
+          }
+        }
+      __syncthreads();                                       // P is there; A is free
+      if (more) fetch(x.a, x.a_shared, c + step, Z::kA);
+    }
+
+    // the values: for P V as they are, for X times the decay to the chunk's end
+    Parts<NP> v[JS];
+    Parts<3> vd[JS];
+    float odd = 0.f;
+#pragma unroll
+    for (int js = 0; js < JS; ++js) {
+      v[js] = cols_of<NP>(lds + Z::kV, wave, js, place);
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float s = 0.f;
+#pragma unroll
+        for (int n2 = 0; n2 < NP; ++n2) s += (float)v[js].p[n2][e];
+        odd = __builtin_fmaf(s, 0.f, odd);
+        const int t = 32 * js + 8 * g + e;
+        y[e] = t < left ? s * (x.in_x * power(g2, left - 1 - t)) : 0.f;
+      }
+      vd[js] = split3(y);
+    }
+    if constexpr (kOut) {
+      // A NaN or an infinity in a column of V: the rows before it do without it (the zeros above P's diagonal would carry it
+      // there), the others become NaN.
+      int bad = C;
+      const bool any = __builtin_amdgcn_ballot_w64(odd != 0.f) != 0;
+      if (__builtin_expect(any, 0)) {
+#pragma unroll
+        for (int js = 0; js < JS; ++js)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float s = 0.f;
+#pragma unroll
+            for (int n2 = 0; n2 < NP; ++n2) s += (float)v[js].p[n2][e];
+            if (s * 0.f != 0.f) bad = min(bad, 32 * js + 8 * g + e);
+          }
+        bad = min(bad, __shfl_xor(bad, 16, 64));
+        bad = min(bad, __shfl_xor(bad, 32, 64));
+#pragma unroll
+        for (int js = 0; js < JS; ++js)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (32 * js + 8 * g + e >= bad)
+#pragma unroll
+              for (int n2 = 0; n2 < NP; ++n2) v[js].p[n2][e] = (__bf16)0.f;
+      }
+      const bf16x8* pm = reinterpret_cast<const bf16x8*>(lds + Z::kAtP);
+#pragma unroll
+      for (int js = 0; js < JS; ++js)
+#pragma unroll
+        for (int i = 2 * js; i < MT; i += 2) {
+          const Parts<Z::kPParts> p[2] = {staged<Z::kPParts>(pm, Square<C>::at(i, js, false), l),
+                                          staged<Z::kPParts>(pm, Square<C>::at(i + 1, js, false), l)};
+          const Parts<NP> y[1] = {v[js]};
+          mma_grid(O + i, p, y);
+        }
+      if (__builtin_expect(any, 0))
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (tile_row(i, 4 * g + r) >= bad) O[i][0][r] = __builtin_nanf("");
+      T* stage = reinterpret_cast<T*>(lds + Z::kAtStage);
+      const int64_t row0 = (int64_t)sp.b * a.s.T + sp.t0 + (int64_t)c * C;
+      if (x.out_parts) {
+        float* to = static_cast<float*>(x.out);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int t = tile_row(i, 4 * g + r);
+            if (t < left) to[((row0 + (x.back ? left - 1 - t : t)) * a.Hv + h) * kHead + col] = O[i][0][r];
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) stage[tile_row(i, 4 * g + r) * kHead + col] = from_f32<T>(O[i][0][r]);
+      }
+    }
+
+    // X
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (kDg == 1) X2[t][r] = whole * __builtin_fmaf(X[t][0][r], (float)left, X2[t][r]);
+        X[t][0][r] *= whole;
+      }
+    constexpr int kSome = NP == 1 ? 4 : 2;
+#pragma unroll
+    for (int js = 0; js < JS; ++js)
+#pragma unroll
+      for (int t = 0; t < 8; t += kSome) {
+        Parts<NP> k[kSome];
+#pragma unroll
+        for (int i = 0; i < kSome; ++i) k[i] = cols_of<NP>(lds + Z::kB, t + i, js, place);
+        const Parts<3> y[1] = {vd[js]};
+        mma_grid(X + t, k, y);
+      }
+    __syncthreads();                                         // B, V, dot and P are free; the outputs are staged
+    if (more) {
+      fetch(x.b, x.b_shared, c + step, Z::kB);
+      fetch(x.v, x.v_shared, c + step, Z::kV);
+      if (kDg) fetch(x.dot, 1, c + step, Z::kDot);
+    }
+    if constexpr (kOut) {
+      if (!x.out_parts) {
+        constexpr int kPer = 16 / sizeof(T), kPieces = kHead / kPer;
+        const int64_t row0 = (int64_t)sp.b * a.s.T + sp.t0 + (int64_t)c * C;
+        T* to = const_cast<T*>(uniform(static_cast<T*>(x.out) + (row0 * a.Hv + h) * kHead));
+#pragma unroll
+        for (int i = 0; i < C * kPieces / (64 * kWaves); ++i) {
+          const int u = tid + 64 * kWaves * i, t = u / kPieces;
+          const u32x4 y = *reinterpret_cast<const u32x4*>(lds + Z::kAtStage + 16 * u);
+          if (t < left)
+            *reinterpret_cast<u32x4*>(to + (int64_t)(x.back ? left - 1 - t : t) * a.Hv * kHead + kPer * (u % kPieces)) = y;
+        }
+      }
+    }
+  }
+  if constexpr (!kOut) {
+    state_store(X, x.add + gn, 1.f, g, col);
+  } else {
+    if (ends && x.last) state_store(X, x.last + sn, x.back ? power(g2, chunks ? 1 : 0) : 1.f, g, col);
+    if constexpr (kDg == 1) {
+      const float* far = last ? (x.far_first ? x.far_first + sn : nullptr) : x.far + gn;
+      if (far) {
+        state_load(X, far, x.turn, g, col);
+        const float f = power(g2, last ? 0 : 1);             // D is the next token's, the final state's gradient this one's
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) dg = __builtin_fmaf(X[t][0][r] * f, X2[t][r], dg);
+      }
+    }
+    if constexpr (kDg != 0) {
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) dg += __shfl_xor(dg, o, 64);
+      __syncthreads();
+      float* red = reinterpret_cast<float*>(lds);
+      if (l == 0) red[wave] = dg;
+      __syncthreads();
+      if (tid == 0) {
+        float s = 0.f;
+        for (int w = 0; w < kWaves; ++w) s += red[w];
+        *dg_part = s;
+      }
+    }
+  }
+}
+
+template <typename T, bool kOut, int kDg, int kPerSimd>
+__global__ __launch_bounds__(64 * kWaves, kPerSimd) void linear_scan_kernel(LinearArgs a) {
+  extern __shared__ __align__(16) char lds[];
+  const int which = blockIdx.y;
+  if constexpr (kDg != 0) {
+    if (which == 0) linear_scan<T, kOut, 1>(a, a.pass[0], lds, a.dg_parts + blockIdx.x);
+    else if (which == 1) linear_scan<T, kOut, 2>(a, a.pass[1], lds, a.dg_parts + a.units + blockIdx.x);
+    else linear_scan<T, kOut, 0>(a, a.pass[2], lds, nullptr);
+  } else {
+    linear_scan<T, kOut, 0>(a, a.pass[which], lds, nullptr);
+  }
+}
+
+// X before each segment but the pass's first from what the segments add: 256 threads, 1024 elements of a head's state.
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int C) {
+  const Pass& x = a.pass[0];
+  const int n = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, e = blockIdx.y * 1024 + 4 * threadIdx.x;
+  const int tokens = C * a.seg;
+  const Span sp = span_of(a.s, n, tokens);
+  const int segs = (sp.len + tokens - 1) / tokens;
+  const int64_t sn = ((int64_t)n * a.Hv + h) * kHead * kHead + e;
+  if (segs == 0 && x.last)                                   // an empty sequence: no block has it
+    *reinterpret_cast<floatx4*>(x.last + sn) = x.first ? *reinterpret_cast<const floatx4*>(x.first + sn) : floatx4{0.f, 0.f, 0.f, 0.f};
+  if (segs < 2) return;
+  const float g2 = log2_decay(a.g + h * a.g_sh);
+  floatx4 X = {0.f, 0.f, 0.f, 0.f};
+  if (x.first) X = *reinterpret_cast<const floatx4*>(x.first + sn);
+  auto at = [&](int i) { return ((int64_t)(sp.slot0 + (x.back ? segs - 1 - i : i)) * a.Hv + h) * kHead * kHead + e; };
+  floatx4 add = *reinterpret_cast<const floatx4*>(x.add + at(0));
+  for (int i = 0; i + 1 < segs; ++i) {
+    floatx4 next = {0.f, 0.f, 0.f, 0.f};
+    if (i + 2 < segs) next = *reinterpret_cast<const floatx4*>(x.add + at(i + 1));
+    // the last tokens' segment may be short, and no decay lies before the gradient of the final state
+    const int steps = x.back && i == 0 ? sp.len - (segs - 1) * tokens - 1 : tokens;
+    const float f = power(g2, steps);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) X[r] = __builtin_fmaf(X[r], f, add[r]);
+    *reinterpret_cast<floatx4*>(const_cast<float*>(x.init) + at(i + 1)) = X;
+    add = next;
+  }
+}
+
+// dg of a head: the parts of its blocks, in their order.
+__global__ __launch_bounds__(256) void linear_dg_kernel(const float* parts, int units, int Hv, float* dg) {
+  __shared__ double red[256];
+  const int h = blockIdx.x;
+  double s = 0.;
+  for (int i = threadIdx.x; i < 2 * (units / Hv); i += 256) s += parts[(int64_t)i * Hv + h];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  for (int o = 128; o; o >>= 1) {
+    if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) dg[h] = (float)red[0];
+}
+
+// dq (blockIdx.y 0) and dk of the q/k heads from the parts of the v heads that share them: a thread 8 elements.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_shared_kernel(const float* dq_parts, const float* dk_parts, int64_t rows, int Hk, int share,
+                                                            T* dq, T* dk) {
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x, row = u / 16;          // row: token and q/k head
+  if (row >= rows * Hk) return;
+  const float* p = (blockIdx.y ? dk_parts : dq_parts) + row * share * kHead + 8 * (u & 15);
+  float x[8];
+  load8(p, x);
+  for (int i = 1; i < share; ++i) {
+    float y[8];
+    load8(p + i * kHead, y);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] += y[k];
+  }
+  store8((blockIdx.y ? dk : dq) + row * kHead + 8 * (u & 15), x);
+}
+
+}  // namespace gsa
+
+namespace gsa_host {
+namespace {
+
+// What one call lays out, from its sizes alone (so a backward pass finds what its forward kept).
+struct LinearPlan {
+  int C, seg;                 // tokens of a chunk; chunks of a segment, 0: none
+  int64_t units, segs;        // heads of all sequences or segments (0: out of range); segments
+  size_t states, dg, parts;   // bytes: a state of every segment; dg's parts; dq and dk by v heads
+  size_t workspace(bool backward) const { return 2 * states + (backward ? dg + 2 * parts : 0); }
+};
+LinearPlan linear_plan(int B, int T, int N, int packed, int Hk, int Hv, int dtype) {
+  LinearPlan z{};
+  z.C = dtype == GSA_DTYPE_BF16 ? gsa::ChunkType<uint16_t>::kChunk : gsa::ChunkType<float>::kChunk;
+  if (B < 1 || T < 1 || N < 1 || Hk < 1 || Hv < Hk || Hv % Hk || !dtype_size(dtype)) return z;
+  const int64_t nc = ((int64_t)T + z.C - 1) / z.C, heads = (int64_t)N * Hv;
+  // a grid of 512 threads a unit: a launch has less than 2^32 of them; rows are counted in 32 bits
+  if ((packed ? (int64_t)T / z.C + N : B * nc) > (1 << 23) / Hv || heads >= 1 << 23) return z;
+  const int64_t length = packed ? (nc + N - 1) / N : nc;
+  z.segs = 0;
+  if (heads <= 256 && length >= 4) {
+    const int64_t pieces = std::max<int64_t>(1, 512 / heads), seg = std::max<int64_t>(2, (length + pieces - 1) / pieces);
+    if (seg < length) {
+      z.seg = (int)seg;
+      z.segs = packed ? (int64_t)T / (z.C * seg) + N : B * ((nc + seg - 1) / seg);
+    }
+  }
+  z.units = z.seg ? z.segs * Hv : heads;
+  z.states = (size_t)z.segs * Hv * 128 * 128 * 4;
+  z.dg = up(2 * z.units * 4);
+  z.parts = Hv > Hk ? (size_t)B * T * Hv * 128 * 4 : 0;
+  return z;
+}
+
+template <typename T, bool kOut, int kDg, int kPerSimd> int launch_linear(const gsa::LinearArgs& a, int passes, hipStream_t s) {
+  using Z = gsa::LinearSizes<T, kDg>;
+  constexpr size_t lds = kOut ? Z::kBytes : Z::kState;
+  static_assert(lds * (kPerSimd / 2) <= 160 * 1024);
+  if (const int e = allow_lds<gsa::linear_scan_kernel<T, kOut, kDg, kPerSimd>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::linear_scan_kernel<T, kOut, kDg, kPerSimd>), dim3(a.units, passes), dim3(64 * gsa::kWaves), lds, s, a);
+  return launch_status();
+}
+// X between the segments of a.pass[0]: what each adds, then their join.
+template <typename T> int launch_segments(const gsa::LinearArgs& a, const LinearPlan& z, hipStream_t s) {
+  if (!z.seg) return GSA_OK;
+  if (const int e = launch_linear<T, false, 0, sizeof(T) == 2 ? 4 : 2>(a, 1, s)) return e;
+  hipLaunchKernelGGL(gsa::linear_join_kernel, dim3(a.s.N * a.Hv, 16), dim3(256), 0, s, a, z.C);
+  return launch_status();
+}
+
+int linear_args(const gsa_linear_args* x, bool backward, gsa::LinearArgs& a, LinearPlan& z) {
+  if (!x || !x->q || !x->k || !x->v || !x->g) return GSA_ERR_NULL;
+  if (backward ? !x->dout || !x->dq || !x->dk || !x->dv : !x->o) return GSA_ERR_NULL;
+  if (!dtype_size(x->dtype)) return GSA_ERR_DTYPE;
+  if (x->B < 1 || x->T < 1 || x->N < 1 || x->Hk < 1 || x->Hv < x->Hk || x->Hv % x->Hk || x->Hv > 65535 || x->d != 128)
+    return GSA_ERR_SHAPE;
+  if (x->cu_seqlens ? x->B != 1 || (x->cu_bytes != 4 && x->cu_bytes != 8) : x->N != x->B) return GSA_ERR_SHAPE;
+  z = linear_plan(x->B, x->T, x->N, x->cu_seqlens != nullptr, x->Hk, x->Hv, x->dtype);
+  if (!z.units) return GSA_ERR_SHAPE;
+  if (z.workspace(backward) && !x->ws) return GSA_ERR_NULL;
+  if (backward && z.seg && !x->saved) return GSA_ERR_NULL;
+  if (x->ws_bytes < z.workspace(backward) || (x->saved && x->saved_bytes < z.states)) return GSA_ERR_SHAPE;
+  // a chunk's rows are addressed by 32-bit offsets
+  for (int64_t st : {x->q_st, x->k_st, x->v_st, backward ? x->do_st : (int64_t)0})
+    if (st < 0 || st * 64 * dtype_size(x->dtype) >= (int64_t)1 << 31) return GSA_ERR_SHAPE;
+  auto vec = [&](const void* p, int64_t sb, int64_t st, int64_t sh) {
+    return vec_ok(p, sb, st, x->dtype) && sh % (x->dtype == GSA_DTYPE_BF16 ? 8 : 4) == 0;
+  };
+  if (!vec(x->q, x->q_sb, x->q_st, x->q_sh) || !vec(x->k, x->k_sb, x->k_st, x->k_sh) || !vec(x->v, x->v_sb, x->v_st, x->v_sh) ||
+      (backward && !vec(x->dout, x->do_sb, x->do_st, x->do_sh)))
+    return GSA_ERR_ALIGN;
+  for (const void* p : {(const void*)x->o, (const void*)x->dq, (const void*)x->dk, (const void*)x->dv, (const void*)x->state_in,
+                        (const void*)x->state_out, (const void*)x->dstate_in, (const void*)x->dstate_out, (const void*)x->saved,
+                        (const void*)x->ws})
+    if (p && !aligned(p, 16)) return GSA_ERR_ALIGN;
+  if (!aligned(x->g, 4) || !aligned(x->dg, 4) || (x->cu_seqlens && !aligned(x->cu_seqlens, x->cu_bytes))) return GSA_ERR_ALIGN;
+  a = gsa::LinearArgs{};
+  a.s = {x->cu_seqlens, x->cu_bytes == 8, x->N, x->T};
+  a.Hk = x->Hk;
+  a.Hv = x->Hv;
+  a.units = (int)z.units;
+  a.seg = z.seg;
+  a.g = x->g;
+  a.g_sh = x->g_sh;
+  return GSA_OK;
+}
+// Rows outside every packed sequence: o, or the gradients.
+int launch_outside(const gsa::LinearArgs& a, const gsa_linear_args* x, bool backward, hipStream_t s) {
+  if (!a.s.cu) return GSA_OK;
+  const int64_t row = 128 * (int64_t)dtype_size(x->dtype);
+  const gsa::Outside o = backward ? gsa::Outside{a.s, {(char*)x->dq, (char*)x->dk, (char*)x->dv}, {a.Hk * row, a.Hk * row, a.Hv * row}}
+                                  : gsa::Outside{a.s, {(char*)x->o}, {a.Hv * row}};
+  hipLaunchKernelGGL(gsa::outside_kernel, dim3(256), dim3(256), 0, s, o);
+  return launch_status();
+}
+
+template <typename T> int linear_forward(const gsa_linear_args* x, gsa::LinearArgs& a, const LinearPlan& z, hipStream_t s) {
+  float* add = static_cast<float*>(x->ws);
+  gsa::Pass& p = a.pass[0];
+  p.a = {x->q, x->q_sb, x->q_st, x->q_sh};
+  p.b = {x->k, x->k_sb, x->k_st, x->k_sh};
+  p.v = {x->v, x->v_sb, x->v_st, x->v_sh};
+  p.a_shared = p.b_shared = 1;
+  p.in_p = p.in_o = x->scale;
+  p.in_x = 1.f;
+  p.first = x->state_in;
+  p.init = x->saved && z.seg ? static_cast<float*>(x->saved) : add + z.states / 4;
+  p.add = add;
+  p.out = x->o;
+  p.last = x->state_out;
+  if (const int e = launch_segments<T>(a, z, s)) return e;
+  if (const int e = launch_linear<T, true, 0, sizeof(T) == 2 ? 4 : 2>(a, 1, s)) return e;
+  return launch_outside(a, x, false, s);
+}
+
+template <typename T> int linear_backward(const gsa_linear_args* x, gsa::LinearArgs& a, const LinearPlan& z, hipStream_t s) {
+  char* w = static_cast<char*>(x->ws);
+  float *add = reinterpret_cast<float*>(w), *init = reinterpret_cast<float*>(w + z.states);
+  float *dqp = reinterpret_cast<float*>(w + 2 * z.states + z.dg), *dkp = dqp + z.parts / 4;
+  const bool parts = a.Hv > a.Hk;
+  const gsa::Rows q{x->q, x->q_sb, x->q_st, x->q_sh}, k{x->k, x->k_sb, x->k_st, x->k_sh}, v{x->v, x->v_sb, x->v_st, x->v_sh},
+      dout{x->dout, x->do_sb, x->do_st, x->do_sh};
+  a.dg_parts = reinterpret_cast<float*>(w + 2 * z.states);
+  gsa::Pass dq{}, dk{}, dv{};
+  dq.a = dout; dq.b = v; dq.v = k; dq.dot = q;
+  dq.v_shared = dq.turn = 1;
+  dq.in_p = dq.in_o = x->scale;
+  dq.in_x = 1.f;
+  dq.first = x->state_in;
+  dq.init = static_cast<const float*>(x->saved);
+  dq.far_first = x->dstate_out;
+  dq.far = init;
+  dq.out = parts ? (void*)dqp : x->dq;
+  dq.out_parts = parts;
+  dk.a = v; dk.b = dout; dk.v = q; dk.dot = k;
+  dk.v_shared = dk.turn = dk.back = 1;
+  dk.in_p = dk.in_x = x->scale;
+  dk.in_o = 1.f;
+  dk.first = x->dstate_out;
+  dk.init = init;
+  dk.out = parts ? (void*)dkp : x->dk;
+  dk.out_parts = parts;
+  dv.a = k; dv.b = q; dv.v = dout;
+  dv.a_shared = dv.b_shared = dv.back = 1;
+  dv.in_p = dv.in_x = x->scale;
+  dv.in_o = 1.f;
+  dv.first = x->dstate_out;
+  dv.init = init;
+  dv.out = x->dv;
+  dv.last = x->dstate_in;
+  dv.add = add;
+  a.pass[0] = dv;
+  if (const int e = launch_segments<T>(a, z, s)) return e;
+  a.pass[0] = dq;
+  a.pass[1] = dk;
+  a.pass[2] = dv;
+  int e = x->dg ? launch_linear<T, true, 1, 2>(a, 3, s) : launch_linear<T, true, 0, sizeof(T) == 2 ? 4 : 2>(a, 3, s);
+  if (e) return e;
+  if (x->dg) {
+    hipLaunchKernelGGL(gsa::linear_dg_kernel, dim3(a.Hv), dim3(256), 0, s, a.dg_parts, a.units, a.Hv, x->dg);
+    if ((e = launch_status())) return e;
+  }
+  if (parts) {
+    const int64_t rows = (int64_t)x->B * x->T;
+    hipLaunchKernelGGL(gsa::linear_shared_kernel<T>, dim3((rows * a.Hk * 16 + 255) / 256, 2), dim3(256), 0, s, dqp, dkp, rows, a.Hk,
+                       a.Hv / a.Hk, static_cast<T*>(x->dq), static_cast<T*>(x->dk));
+    if ((e = launch_status())) return e;
+  }
+  return launch_outside(a, x, true, s);
+}
+
+}  // namespace
+}  // namespace gsa_host
+
+extern "C" size_t gsa_linear_attn_workspace_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype, int backward) {
+  const auto z = gsa_host::linear_plan(B, T, N, packed, Hk, Hv, dtype);
+  return z.units ? z.workspace(backward != 0) : (size_t)-1;
+}
+extern "C" size_t gsa_linear_attn_saved_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype) {
+  return gsa_host::linear_plan(B, T, N, packed, Hk, Hv, dtype).states;
+}
+extern "C" int gsa_linear_attn(const gsa_linear_args* x, void* stream) {
+  gsa::LinearArgs a;
+  gsa_host::LinearPlan z;
+  if (const int e = gsa_host::linear_args(x, false, a, z)) return e;
+  const auto s = static_cast<hipStream_t>(stream);
+  return x->dtype == GSA_DTYPE_BF16 ? gsa_host::linear_forward<uint16_t>(x, a, z, s) : gsa_host::linear_forward<float>(x, a, z, s);
+}
+extern "C" int gsa_linear_attn_backward(const gsa_linear_args* x, void* stream) {
+  gsa::LinearArgs a;
+  gsa_host::LinearPlan z;
+  if (const int e = gsa_host::linear_args(x, true, a, z)) return e;
+  const auto s = static_cast<hipStream_t>(stream);
+  return x->dtype == GSA_DTYPE_BF16 ? gsa_host::linear_backward<uint16_t>(x, a, z, s) : gsa_host::linear_backward<float>(x, a, z, s);
+}

@@ -611,6 +611,51 @@ int gsa_delta_rule_shape(int B, int T, int N, int packed, int Hk, int Hv, int dt
 int gsa_delta_rule(const gsa_delta_args* args, void* stream);
 int gsa_delta_rule_backward(const gsa_delta_args* args, void* stream);
 
+/*
+ * Linear attention with a decay for each head, S_t = e^g S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t, over whole
+ * sequences; no counterpart in the reference (its gated delta rule without the correction, with gates by the head).
+ * q, k [B,T,Hk,128], v, o [B,T,Hv,128] in dtype, v head h with q/k head h / (Hv/Hk); g fp32 [Hv], the log of the decay,
+ * at most 0 (below -128: a reset); states fp32 [N,Hv,128,128] (k element, v element).  cu_seqlens as in gsa_delta_args.
+ * The forward fills `saved` (gsa_linear_attn_saved_bytes, which may be 0) where a backward pass follows; the backward
+ * pass reads it and writes dq, dk, dv and, where they are not NULL, dg and dstate_in (both calls with the same sizes).
+ * Rows of o and of the gradients outside every packed sequence become 0.  Head rows contiguous; q, k, v, dout rows
+ * 16-byte aligned, less than 32 MiB apart (fp32: 8 MiB).  *_workspace_bytes: (size_t)-1 for sizes that are refused.
+ */
+typedef struct gsa_linear_args {
+  const void *q, *k, *v;
+  const float* g;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sh;
+  const void* cu_seqlens;
+  int cu_bytes, B, T, N, Hk, Hv, d, dtype;
+  float scale;
+  const float* state_in;
+  void* o;
+  float* state_out;
+  void* ws;
+  size_t ws_bytes;
+  void* saved;
+  size_t saved_bytes;
+  const void* dout;
+  int64_t do_sb, do_st, do_sh;
+  const float* dstate_out;
+  void *dq, *dk, *dv;
+  float *dg, *dstate_in;
+} gsa_linear_args;
+size_t gsa_linear_attn_workspace_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype, int backward);
+size_t gsa_linear_attn_saved_bytes(int B, int T, int N, int packed, int Hk, int Hv, int dtype);
+int gsa_linear_attn(const gsa_linear_args* args, void* stream);
+int gsa_linear_attn_backward(const gsa_linear_args* args, void* stream);
+
+/*
+ * The same for one token of each row of a serving batch, on a pool of states in place: q, k [N,Hk,128], v, o [N,Hv,128],
+ * state fp32 [slots,Hv,128,128].  state_idx (int32 or int64 [N] by idx_bytes, or NULL: row n has state n): a row outside
+ * [0, slots) is padding, its output 0; rows that name one state are consecutive tokens in the batch's order.
+ */
+int gsa_linear_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int64_t k_sn, int64_t k_sh, const void* v,
+                    int64_t v_sn, int64_t v_sh, const float* g, int64_t g_sh, const void* state_idx, int idx_bytes,
+                    float* state, int64_t s_sn, int64_t s_sh, int N, int slots, int Hk, int Hv, int d, float scale,
+                    int dtype, void* o, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,490 @@
+"""Linear attention with decays and its single-token step on the GPU against the recurrence in 64 bits.
+
+Tolerances.  Every result is a sum of products; the oracle run on the inputs' absolute values (scale and
+upstream gradients too) gives the sum A of the terms' sizes.  A result of type t carries one rounding, at
+most eps(t) / 2 of its value.  Under it a term carries at most ROUNDS roundings of 2^-24: two or three
+decays by exp2 (2 roundings each and the one of its exponent, at most 0.4 of a rounding of a decay), the
+parts' products (fp32 operands hold 27 bits in three parts, products under 2^-26 are left out), and the
+sums: 8 steps of 32 summed by the matrix cores, up to 6 products each, twice (96), and one rounding for
+each chunk that the state passes (T / 32) and each segment.  Results in bf16 take two parts of the state
+and of the scores: 2^-18 of each term, 2^-17 allowed.  A gradient of g sums terms that are products
+of results (their errors as above) times counts that are exact.  Heads that share q and k add their
+number of roundings.  Under 2^-126, fp32's smallest normal number, a decay may be flushed.
+"""
+
+import pytest
+import torch
+
+from gsa_gdn_benchmarkstudy_amd import add_rms_norm, linear_attention, linear_attention_step
+from tests import linear_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+NAMES = ("q", "k", "v", "g")
+TYPES = [torch.bfloat16, torch.float32]
+
+
+def _inputs(B, T, Hk, Hv, dtype, seed):
+    gen = torch.Generator().manual_seed(seed)
+
+    def rn(*s):
+        return torch.randn(*s, generator=gen)
+
+    q, k = (torch.nn.functional.silu(rn(B, T, Hk, D)).to(dtype) for _ in range(2))
+    return dict(q=q, k=k, v=rn(B, T, Hv, D).to(dtype), g=-torch.exp2(-8 * (torch.arange(Hv) + torch.rand(Hv, generator=gen)) / Hv))
+
+
+def _state(N, Hv, seed):
+    return torch.randn(N, Hv, D, D, generator=torch.Generator().manual_seed(seed))
+
+
+def _oracle(x, spans, state=None, grads=None, scale=D ** -0.5, want=True):
+    """The recurrence over spans [(row, start, end)]; outputs and gradients laid out as the op's."""
+    leaf = {n: t.double().requires_grad_(grads is not None) for n, t in x.items()}
+    st = None if state is None else state.double().requires_grad_(grads is not None)
+    o = 0 * leaf["v"]
+    finals = []
+    for i, (b, s, e) in enumerate(spans):
+        oi, S = orc.rule(*(leaf[n][b, s:e] for n in "qkv"), leaf["g"], scale, None if st is None else st[i])
+        finals.append(S)
+        if e > s:
+            mask = torch.zeros(o.shape[0], o.shape[1], 1, 1, dtype=torch.float64)
+            mask[b, s:e] = 1
+            o = o + mask * torch.nn.functional.pad(oi, (0, 0, 0, 0, s, o.shape[1] - e))[None]
+    S = torch.stack(finals)
+    if grads is None:
+        return o, S, None
+    ins = [leaf[n] for n in NAMES] + ([st] if st is not None else [])
+    outs, gr = ([o, S], [grads[0].double(), grads[1].double()]) if want else ([o], [grads[0].double()])
+    d = torch.autograd.grad(outs, ins, gr, allow_unused=True)
+    d = [torch.zeros_like(i) if t is None else t for i, t in zip(ins, d)]
+    return o.detach(), S.detach(), dict(zip(NAMES + ("state",), d))
+
+
+def _both(x, spans, state=None, grads=None, scale=D ** -0.5, want=True):
+    """The oracle's results, and the sums of their terms' sizes."""
+    size = {n: t if n == "g" else t.abs() for n, t in x.items()}
+    return (_oracle(x, spans, state, grads, scale, want),
+            _oracle(size, spans, None if state is None else state.abs(), None if grads is None else [t.abs() for t in grads], abs(scale), want))
+
+
+def _run(x, dev, state=None, want=True, cu=None, grads=None, scale=None):
+    leaf = {n: t.to(dev).requires_grad_(grads is not None) for n, t in x.items()}
+    st = None if state is None else state.to(dev).requires_grad_(grads is not None)
+    o, S = linear_attention(*(leaf[n] for n in NAMES), scale=scale, initial_state=st, output_final_state=want, cu_seqlens=cu)
+    if grads is None:
+        return o, S, None
+    ins = [leaf[n] for n in NAMES] + ([st] if st is not None else [])
+    outs, gr = [o], [grads[0].to(dev)]
+    if want:
+        outs.append(S)
+        gr.append(grads[1].to(dev))
+    d = torch.autograd.grad(outs, ins, gr)
+    return o.detach(), None if S is None else S.detach(), dict(zip(NAMES + ("state",), d))
+
+
+def _check(got, ref, size, T, share, name):
+    assert tuple(got.shape) == tuple(ref.shape), name
+    if not got.numel():
+        return
+    half = torch.finfo(got.dtype).eps / 2
+    few = 2.0 ** -17 if got.dtype == torch.bfloat16 else 0.0
+    tol = half * ref.abs() + (few + (128 + T / 16 + share) * 2.0 ** -24) * size + 2.0 ** -126
+    err = (got.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), f"{name}: {(err / tol).max():.2f} of the tolerance (|err| {err.max():.2e})"
+
+
+def _compare(got, both, T, share=1, want=True):
+    ref, size = both
+    _check(got[0], ref[0], size[0], T, share, "o")
+    if want:
+        _check(got[1], ref[1], size[1], T, share, "state")
+    if got[2] is not None:
+        for n, d in got[2].items():
+            _check(d, ref[2][n], size[2][n], T, share, "d" + n)
+
+
+CASES = [(1, 1, 1, 1), (2, 2, 1, 2), (1, 31, 2, 2), (1, 32, 1, 1), (2, 33, 1, 3), (1, 63, 1, 2), (1, 64, 2, 2), (3, 65, 1, 1),
+         (1, 129, 2, 4), (2, 200, 2, 2), (1, 513, 1, 2)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,T,Hk,Hv", CASES)
+def test_forward(dev, B, T, Hk, Hv, dtype):
+    print(f"forward {dtype} B={B} T={T} Hk={Hk} Hv={Hv}", flush=True)
+    x = _inputs(B, T, Hk, Hv, dtype, seed=T)
+    spans = [(b, 0, T) for b in range(B)]
+    _compare(_run(x, dev), _both(x, spans), T)
+    state = _state(B, Hv, 5)
+    _compare(_run(x, dev, state), _both(x, spans, state), T)
+    assert _run(x, dev, want=False)[1] is None
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,T,Hk,Hv", CASES)
+@pytest.mark.parametrize("with_state", [False, True])
+def test_backward(dev, B, T, Hk, Hv, dtype, with_state):
+    print(f"backward {dtype} B={B} T={T} Hk={Hk} Hv={Hv} state={with_state}", flush=True)
+    x = _inputs(B, T, Hk, Hv, dtype, seed=T + 1)
+    gen = torch.Generator().manual_seed(6)
+    state = _state(B, Hv, 7) if with_state else None
+    grads = (torch.randn(B, T, Hv, D, generator=gen).to(dtype), torch.randn(B, Hv, D, D, generator=gen))
+    spans = [(b, 0, T) for b in range(B)]
+    _compare(_run(x, dev, state, with_state, grads=grads), _both(x, spans, state, grads, want=with_state), T, Hv // Hk, with_state)
+
+
+PACKS = [[1], [5, 0, 64, 1, 65, 63], [0, 0, 3], [130, 32, 33], [64, 64, 64], [0], [400, 1, 0, 333]]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens", PACKS)
+@pytest.mark.parametrize("lead,trail,idx", [(0, 0, torch.int32), (3, 37, torch.int64)])
+def test_packed(dev, lens, lead, trail, idx, dtype):
+    """Packed sequences, empty ones among them; rows before the first and behind the last become 0, whatever they hold."""
+    print(f"packed {dtype} {lens} lead={lead} trail={trail}", flush=True)
+    T, N, Hk, Hv = lead + sum(lens) + trail, len(lens), 1, 2
+    if T == 0:
+        return
+    cu = torch.tensor([lead] + lens).cumsum(0).to(idx)
+    x = _inputs(1, T, Hk, Hv, dtype, seed=N)
+    gen = torch.Generator().manual_seed(7)
+    state = _state(N, Hv, 8)
+    grads = (torch.randn(1, T, Hv, D, generator=gen).to(dtype), torch.randn(N, Hv, D, D, generator=gen))
+    spans = [(0, int(cu[i]), int(cu[i + 1])) for i in range(N)]
+    outside = torch.ones(T, dtype=torch.bool)
+    outside[lead:T - trail] = False
+    both = _both(x, spans, state, grads)
+    for t in (x["q"], x["k"], x["v"], grads[0]):
+        t[0, outside] = float("nan")
+    got = _run(x, dev, state, cu=cu.to(dev), grads=grads)
+    _compare(got, both, T, Hv // Hk)
+    for t in (got[0], *(got[2][n] for n in "qkv")):
+        assert not t[0, outside.to(dev)].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,T,Hk,Hv,lens", [(1, 900, 1, 1, None), (2, 1537, 1, 2, None), (1, 2200, 1, 2, [900, 0, 1, 1000, 299])])
+def test_segments(dev, B, T, Hk, Hv, lens, dtype):
+    """Long sequences with few heads: cut into segments that are joined again (packed ones of several lengths)."""
+    print(f"segments {dtype} B={B} T={T} {lens}", flush=True)
+    x = _inputs(B, T, Hk, Hv, dtype, seed=T)
+    N = B if lens is None else len(lens)
+    gen = torch.Generator().manual_seed(14)
+    state = _state(N, Hv, 15)
+    grads = (torch.randn(B, T, Hv, D, generator=gen).to(dtype), torch.randn(N, Hv, D, D, generator=gen))
+    cu = None if lens is None else torch.tensor([0] + lens).cumsum(0)
+    spans = [(b, 0, T) for b in range(B)] if lens is None else [(0, int(cu[i]), int(cu[i + 1])) for i in range(N)]
+    got = _run(x, dev, state, cu=None if cu is None else cu.to(dev), grads=grads)
+    _compare(got, _both(x, spans, state, grads), T, Hv // Hk)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_heads(dev, dtype):
+    """Sequences times heads past the limit for segments: every sequence in one piece."""
+    x = _inputs(70, 70, 2, 4, dtype, seed=3)
+    gen = torch.Generator().manual_seed(4)
+    grads = (torch.randn(70, 70, 4, D, generator=gen).to(dtype), torch.randn(70, 4, D, D, generator=gen))
+    _compare(_run(x, dev, grads=grads), _both(x, [(b, 0, 70) for b in range(70)], grads=grads), 70, 2)
+
+
+def test_offsets_outside_the_tokens_touch_nothing(dev):
+    """Offsets past T or descending: held within the tokens, other sequences are right."""
+    x = _inputs(1, 100, 1, 1, torch.bfloat16, seed=3)
+    o, S, _ = _run(x, dev, cu=torch.tensor([0, 40, 1 << 30], dtype=torch.int64, device=dev))
+    _compare((o, S, None), _both(x, [(0, 0, 40), (0, 40, 100)]), 100)
+    o, S, _ = _run(x, dev, cu=torch.tensor([-5, 40, 20], dtype=torch.int32, device=dev))
+    ref, size = _both(x, [(0, 0, 40)])
+    _check(o[:, :40], ref[0][:, :40], size[0][:, :40], 100, 1, "o")
+    assert not o[:, 40:].any() and not S[1].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("g", [0.0, -1e-4, -0.7, -40.0, -100.0, -1e30, -float("inf"), 0.01])
+def test_decays(dev, g, dtype):
+    """From none to a reset at every token; one that grows."""
+    T = 333
+    x = _inputs(1, T, 1, 2, dtype, seed=11)
+    x["g"][1] = g
+    gen = torch.Generator().manual_seed(8)
+    state = _state(1, 2, 9)
+    grads = (torch.randn(1, T, 2, D, generator=gen).to(dtype), torch.randn(1, 2, D, D, generator=gen))
+    x64 = dict(x, g=x["g"].double().clamp_min(-2000.))       # the oracle's e^g is 0 as well, its gradient 0 and not inf * 0
+    _compare(_run(x, dev, state, grads=grads), _both(x64, [(0, 0, T)], state, grads), T, 2)
+
+
+def test_scale(dev):
+    x = _inputs(1, 150, 1, 1, torch.float32, seed=12)
+    gen = torch.Generator().manual_seed(8)
+    grads = (torch.randn(1, 150, 1, D, generator=gen), torch.randn(1, 1, D, D, generator=gen))
+    _compare(_run(x, dev, grads=grads, scale=-0.31), _both(x, [(0, 0, 150)], grads=grads, scale=-0.31), 150)
+
+
+def test_gradient_against_differences(dev):
+    """The kernels' gradient along random directions against differences of the recurrence in 64 bits."""
+    T = 70
+    x = _inputs(1, T, 1, 2, torch.float32, seed=21)
+    gen = torch.Generator().manual_seed(9)
+    state = _state(1, 2, 10)
+    do, dS = torch.randn(1, T, 2, D, generator=gen), torch.randn(1, 2, D, D, generator=gen)
+    _, _, d = _run(x, dev, state, grads=(do, dS))
+    size = _both(x, [(0, 0, T)], state, (do, dS))[1][2]
+    x64, s64 = {n: t.double() for n, t in x.items()}, state.double()
+
+    def loss(x, s):
+        o, S, _ = _oracle(x, [(0, 0, T)], s)
+        return (o * do.double()).sum() + (S * dS.double()).sum()
+
+    for n in NAMES + ("state",):
+        r = torch.randn((state if n == "state" else x[n]).shape, generator=gen).double()
+        h = 1e-5
+        up, dn = ((loss(x64, s64 + e * r) if n == "state" else loss(x64 | {n: x64[n] + e * r}, s64)) for e in (h, -h))
+        want, got = (up - dn) / (2 * h), (d[n].double().cpu() * r).sum()
+        # differences: h^2 of a third derivative and 2^-52 / h of the loss (1e-6); the gradient's elements as in _check
+        tol = ((136 + T / 16) * 2.0 ** -24 * (size[n] * r.abs())).sum() + 1e-6 * (abs(want) + abs(up))
+        assert abs(want - got) <= tol, (n, want, got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+def test_what_is_not_finite_reaches_no_output_before_it(dev, name, bad, dtype):
+    """One element of one token: every output before it, and of other heads and rows, has the bits it has without."""
+    T, at = 200, 77
+    x = _inputs(2, T, 2, 2, dtype, seed=5)
+    want = _run(x, dev)
+    x[name][1, at, 1, 33] = bad
+    x[name][1, T - 1, 1, 5] = bad
+    o, S, _ = _run(x, dev)
+    assert torch.equal(o[0], want[0][0]) and torch.equal(o[1, :at], want[0][1, :at]) and torch.equal(o[:, :, 0], want[0][:, :, 0])
+    assert torch.equal(S[0], want[1][0])
+    if name == "q":
+        assert torch.equal(o[1, at + 1:T - 1], want[0][1, at + 1:T - 1]) and not o[1, at, 1].isfinite().any()
+    elif name == "v":
+        assert torch.equal(o[1, :, 1, :5], want[0][1, :, 1, :5]) and not o[1, at:, 1, 33].isfinite().any()
+        assert o[1, :T - 1, 1, 5].isfinite().all()
+    else:
+        assert not o[1, at:, 1].isfinite().all()
+
+
+def test_a_packed_neighbour_that_is_not_finite(dev):
+    x = _inputs(1, 150, 1, 2, torch.bfloat16, seed=6)
+    gen = torch.Generator().manual_seed(8)
+    cu = torch.tensor([0, 70, 75, 150], device=dev)
+    grads = (torch.randn(1, 150, 2, D, generator=gen).to(torch.bfloat16), torch.randn(3, 2, D, D, generator=gen))
+    want = _run(x, dev, cu=cu, grads=grads)
+    for t in (x["q"], x["k"], x["v"], grads[0]):
+        t[0, 70:75] = float("nan")
+    got = _run(x, dev, cu=cu, grads=grads)
+    for a, b in ((got[0], want[0]), *((got[2][n], want[2][n]) for n in "qkv")):
+        assert torch.equal(a[:, :70], b[:, :70]) and torch.equal(a[:, 75:], b[:, 75:])
+    assert torch.equal(got[1][0], want[1][0]) and torch.equal(got[1][2], want[1][2])
+
+
+def test_strided_views_and_broadcasts(dev):
+    """Views of one projection output, heads broadcast with stride 0, transposed layouts: the same bits as copies."""
+    gen = torch.Generator().manual_seed(31)
+    B, T, H = 2, 90, 2
+    big = torch.randn(B, T, 3 * H * D + 64, generator=gen).to(torch.bfloat16).to(dev)
+    q, k, v = (big[..., i * H * D:(i + 1) * H * D].view(B, T, H, D) for i in range(3))
+    k = k.transpose(1, 2).contiguous().transpose(1, 2)
+    g = -torch.rand(H, 2, generator=gen).to(dev)[:, 0]
+    a = linear_attention(q, k, v, g, output_final_state=True)
+    b = linear_attention(*(t.contiguous() for t in (q, k, v, g)), output_final_state=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    odd = torch.empty(B * T * H * D + 1, device=dev, dtype=torch.bfloat16)[1:].view(B, T, H, D)
+    odd.copy_(q)                                 # 2-byte aligned: copied
+    assert torch.equal(linear_attention(odd, k, v, g)[0], b[0])
+    one = k[:, :, :1].detach().requires_grad_(True)
+    o, _ = linear_attention(q, one.expand(B, T, H, D), v, g)
+    do = torch.randn(o.shape, generator=gen).to(torch.bfloat16).to(dev)
+    (d1,) = torch.autograd.grad(o, one, do)
+    full = k[:, :, :1].expand(B, T, H, D).contiguous().requires_grad_(True)
+    (d2,) = torch.autograd.grad(linear_attention(q, full, v, g)[0], full, do)
+    assert torch.equal(d1, d2.sum(2, keepdim=True))
+    (d3,) = torch.autograd.grad(linear_attention(q, full, v, g)[0].sum(), full)      # an expanded gradient
+    (d4,) = torch.autograd.grad(linear_attention(q, full, v, g)[0], full, torch.ones_like(o))
+    assert torch.equal(d3, d4)
+    (d5,) = torch.autograd.grad(linear_attention(q, k, v, (g[:1].detach().requires_grad_(True))[:1].expand(H))[0].sum(),
+                                [full], allow_unused=True)
+    assert d5 is None
+    one_g = g[:1].detach().clone().requires_grad_(True)                              # one decay for all heads
+    (d6,) = torch.autograd.grad(linear_attention(q, k, v, one_g.expand(H))[0], one_g, do)
+    every = one_g.detach().expand(H).contiguous().requires_grad_(True)
+    (d7,) = torch.autograd.grad(linear_attention(q, k, v, every)[0], every, do)
+    assert torch.equal(d6, d7.sum(0, keepdim=True))
+
+
+def test_same_bits_and_other_stream(dev):
+    """Two runs, and one on another stream with its own allocations in between: the same bits."""
+    x = _inputs(2, 700, 2, 4, torch.bfloat16, seed=51)
+    gen = torch.Generator().manual_seed(52)
+    grads = (torch.randn(2, 700, 4, D, generator=gen).to(torch.bfloat16), torch.randn(2, 4, D, D, generator=gen))
+    a = _run(x, dev, grads=grads)
+    s = torch.cuda.Stream(device=dev)
+    s.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(s):
+        b = _run(x, dev, grads=grads)
+    torch.cuda.current_stream(dev).wait_stream(s)
+    for y in (b, _run(x, dev, grads=grads)):
+        assert torch.equal(a[0], y[0]) and torch.equal(a[1], y[1])
+        for n in a[2]:
+            assert torch.equal(a[2][n], y[2][n]), n
+
+
+def test_captured_training_and_steps(dev):
+    """Forward, backward and a decoding step in one graph, replayed on new inputs with eager work in between."""
+    x = {n: t.to(dev).requires_grad_(True) for n, t in _inputs(2, 530, 1, 2, torch.bfloat16, seed=61).items()}
+    one = {n: t[:, 0].contiguous().to(dev) if n != "g" else t.to(dev) for n, t in _inputs(2, 1, 1, 2, torch.bfloat16, seed=62).items()}
+    do = torch.randn(2, 530, 2, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(dev)
+
+    def both():
+        o, S = linear_attention(*(x[n] for n in NAMES), output_final_state=True)
+        d = torch.autograd.grad(o, [x[n] for n in NAMES], do)
+        S = S.detach().clone()
+        with torch.no_grad():
+            o1 = linear_attention_step(*(one[n] for n in NAMES), S)
+        return [t.detach() for t in (o, S, o1, *d)]
+
+    s = torch.cuda.Stream(device=dev)
+    s.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(s):
+        both()
+    torch.cuda.current_stream(dev).wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for i in range(4):
+        with torch.no_grad():
+            for n, t in _inputs(2, 530, 1, 2, torch.bfloat16, seed=70 + i).items():
+                x[n].copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        fresh = {n: t.detach().clone().requires_grad_(True) for n, t in x.items()}
+        o, S = linear_attention(*(fresh[n] for n in NAMES), output_final_state=True)
+        d = torch.autograd.grad(o, [fresh[n] for n in NAMES], do)
+        S = S.detach().clone()
+        with torch.no_grad():
+            o1 = linear_attention_step(*(one[n] for n in NAMES), S)
+        for a, b in zip(got, (o, S, o1, *d)):
+            assert torch.equal(a, b)
+
+
+def test_parts_of_the_graph(dev):
+    """No gradient kept where none is needed; outputs and inputs that are left out; once differentiable."""
+    x = {n: t.to(dev) for n, t in _inputs(1, 64, 1, 1, torch.bfloat16, seed=71).items()}
+    assert not linear_attention(*(x[n] for n in NAMES))[0].requires_grad
+    x["v"].requires_grad_(True)
+    with torch.no_grad():
+        assert not linear_attention(*(x[n] for n in NAMES))[0].requires_grad
+    o, S = linear_attention(*(x[n] for n in NAMES), output_final_state=True)
+    (dv,) = torch.autograd.grad(S.sum(), x["v"])                 # o unused
+    assert dv.abs().sum() > 0
+    o, _ = linear_attention(*(x[n] for n in NAMES))
+    (dv,) = torch.autograd.grad(o.float().sum(), x["v"], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dv.sum(), x["v"])                    # once differentiable
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+        q = torch.autograd.forward_ad.make_dual(x["q"], torch.ones_like(x["q"]))
+        linear_attention(q, x["k"], x["v"], x["g"])
+
+
+def test_empty(dev):
+    """No tokens: the state is handed through, and its gradient."""
+    e = torch.zeros(2, 0, 1, D, device=dev, requires_grad=True)
+    g, s = torch.zeros(1, device=dev, requires_grad=True), torch.randn(2, 1, D, D, device=dev).requires_grad_(True)
+    o, S = linear_attention(e, e, e, g, initial_state=s, output_final_state=True)
+    assert o.shape == e.shape and torch.equal(S, s)
+    ds = torch.randn_like(s)
+    for a, b in zip(torch.autograd.grad([o, S], [e, g, s], [torch.zeros_like(o), ds]), (e, torch.zeros_like(g), ds)):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        assert linear_attention_step(e[0], e[0], e[0], g, s.detach()).shape == (0, 1, D)
+
+
+# ---------------------------------------------------------------------------
+# The step
+# ---------------------------------------------------------------------------
+
+def _step_oracle(x, pool, at, scale=D ** -0.5):
+    pool, o = pool.double().clone(), torch.zeros(x["v"].shape, dtype=torch.float64)
+    for i, s in enumerate(at):
+        if 0 <= s < pool.shape[0]:
+            oi, S = orc.rule(*(x[n][i:i + 1].double() for n in "qkv"), x["g"].double(), scale, pool[s])
+            o[i], pool[s] = oi[0], S
+    return o, pool
+
+
+def _step_check(x, pool, at, o, mine):
+    ref, size = _step_oracle(x, pool, at), _step_oracle({n: t if n == "g" else t.abs() for n, t in x.items()}, pool.abs(), at)
+    _check(o, ref[0], size[0], len(at), 1, "o")
+    _check(mine, ref[1], size[1], len(at), 1, "state")
+    for s in set(range(pool.shape[0])) - set(at):
+        assert torch.equal(mine[s].cpu(), pool[s])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,Hk,Hv,slots,at", [
+    (1, 1, 1, 1, None), (3, 2, 4, 5, None), (4, 1, 3, 9, [8, 0, 3, 5]), (5, 2, 2, 4, [3, -1, 0, 4, 1]),
+    (6, 1, 2, 3, [1, 2, 1, -7, 1, 0]), (2, 1, 1, 2, [1 << 20, -1])])
+@pytest.mark.parametrize("idx", [torch.int32, torch.int64])
+def test_step(dev, N, Hk, Hv, slots, at, idx, dtype):
+    """States of rows, padding, an index named more than once (consecutive tokens)."""
+    x = {n: t if n == "g" else t[0] for n, t in _inputs(1, N, Hk, Hv, dtype, seed=N).items()}
+    pool = _state(slots, Hv, 3)
+    mine = pool.to(dev)
+    o = linear_attention_step(*(x[n].to(dev) for n in NAMES), mine, None if at is None else torch.tensor(at, dtype=idx, device=dev))
+    _step_check(x, pool, list(range(N)) if at is None else at, o, mine)
+
+
+def test_step_many_rows(dev):
+    """More rows than a block has threads, every third index twice."""
+    N, slots = 700, 800
+    x = {n: t if n == "g" else t[0] for n, t in _inputs(1, N, 1, 1, torch.bfloat16, seed=5).items()}
+    at = [(i if i % 3 else 2 * i % N) for i in range(N)]
+    pool = _state(slots, 1, 4)
+    mine = pool.to(dev)
+    o = linear_attention_step(*(x[n].to(dev) for n in NAMES), mine, torch.tensor(at, device=dev))
+    _step_check(x, pool, at, o, mine)
+
+
+def test_step_strided_state_and_inputs(dev):
+    x = {n: (t if n == "g" else t[0]).to(dev) for n, t in _inputs(1, 4, 2, 2, torch.bfloat16, seed=6).items()}
+    big = torch.randn(5, 3, 2, D, D, device=dev)
+    keep = big.clone()
+    a = linear_attention_step(*(x[n] for n in NAMES), big[:, 1])
+    st = keep[:, 1].contiguous()
+    wide = torch.zeros(4, 2, 2 * D, device=dev, dtype=torch.bfloat16)
+    wide[..., 1:D + 1] = x["q"]
+    b = linear_attention_step(wide[..., 1:D + 1], *(x[n] for n in NAMES[1:]), st)
+    assert torch.equal(a, b) and torch.equal(big[:, 1], st)
+    assert torch.equal(big[:, 0], keep[:, 0]) and torch.equal(big[:, 2], keep[:, 2])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prefill_then_decode(dev, dtype):
+    """A mixer as it is used: norm, projections, a packed prefill into a pool, steps from it; the same
+    as whole sequences in 64 bits."""
+    torch.manual_seed(0)
+    lens, new, H, width = [75, 1, 130], 3, 2, 256
+    N = len(lens)
+    x = torch.randn(N, max(lens) + new, width).to(dtype)
+    w = (torch.randn(3 * H * D, width) * 0.05).to(dtype).to(dev)
+    wn, g = torch.ones(width, dtype=dtype, device=dev), -torch.tensor([0.3, 0.01], device=dev)
+    with torch.no_grad():
+        q, k, v = torch.nn.functional.linear(add_rms_norm(x.to(dev), wn)[0], w).unflatten(-1, (3, H, D)).unbind(-3)
+        pack = lambda t: torch.cat([t[i, :n] for i, n in enumerate(lens)])[None]  # noqa: E731
+        cu = torch.tensor([0] + lens, device=dev).cumsum(0)
+        o, S = linear_attention(pack(q), pack(k), pack(v), g, cu_seqlens=cu, output_final_state=True)
+        pool, slots = torch.zeros(8, H, D, D, device=dev), torch.tensor([5, 0, 3], device=dev)
+        pool[slots] = S
+        outs = []
+        for t in range(new):
+            at = [n + t for n in lens]
+            outs.append(linear_attention_step(*(torch.stack([a[i, p] for i, p in enumerate(at)]) for a in (q, k, v)), g, pool, slots))
+    for i, n in enumerate(lens):
+        xi = {"q": q[i:i + 1, :n + new].cpu(), "k": k[i:i + 1, :n + new].cpu(), "v": v[i:i + 1, :n + new].cpu(), "g": g.cpu()}
+        ref, size = _both(xi, [(0, 0, n + new)])
+        got = torch.cat([o[0, int(cu[i]):int(cu[i + 1])], *(y[i:i + 1] for y in outs)])
+        _check(got, ref[0][0], size[0][0], n + new, 1, "o")
+        _check(pool[slots[i]], ref[1][0], size[1][0], n + new, 1, "state")
