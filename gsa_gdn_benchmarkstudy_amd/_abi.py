@@ -51,6 +51,8 @@ EXPORTS = (
     "gsa_delta_rule_saved_bytes", "gsa_delta_rule_shape",
     "gsa_linear_attn", "gsa_linear_attn_backward", "gsa_linear_attn_workspace_bytes", "gsa_linear_attn_saved_bytes",
     "gsa_linear_step",
+    "gsa_window_attn", "gsa_window_attn_backward", "gsa_window_attn_workspace_bytes",
+    "gsa_window_cache_write", "gsa_window_step", "gsa_window_step_workspace_bytes",
 )
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
@@ -81,6 +83,18 @@ class LinearArgs(ctypes.Structure):
                    ("ws_bytes", ctypes.c_size_t), ("saved", _vp), ("saved_bytes", ctypes.c_size_t), ("dout", _vp)]
                 + [(n, _i64) for n in ("do_sb", "do_st", "do_sh")]
                 + [(n, _vp) for n in ("dstate_out", "dq", "dk", "dv", "dg", "dstate_in")])
+
+
+class WindowArgs(ctypes.Structure):
+    """gsa_window_args of include/gsa_hip.h."""
+
+    _fields_ = ([(n, _vp) for n in ("q", "k", "v")]
+                + [(f"{n}_{s}", _i64) for n in ("q", "k", "v") for s in ("sb", "st", "sh")]
+                + [("cu_seqlens", _vp)]
+                + [(n, _i32) for n in ("cu_bytes", "B", "T", "N", "H", "Hkv", "d", "dtype", "window", "sinks")]
+                + [("scale", _f32), ("o", _vp), ("lse", _vp), ("dout", _vp)]
+                + [(n, _i64) for n in ("do_sb", "do_st", "do_sh")]
+                + [(n, _vp) for n in ("dq", "dk", "dv", "ws")] + [("ws_bytes", ctypes.c_size_t)])
 
 
 _PROTOS = {
@@ -155,6 +169,14 @@ _PROTOS = {
     "gsa_linear_attn_saved_bytes": ([_i32] * 7, ctypes.c_size_t),
     "gsa_linear_attn": ([ctypes.POINTER(LinearArgs), _vp], _i32),
     "gsa_linear_attn_backward": ([ctypes.POINTER(LinearArgs), _vp], _i32),
+    "gsa_window_attn_workspace_bytes": ([_i32] * 9, ctypes.c_size_t),
+    "gsa_window_attn": ([ctypes.POINTER(WindowArgs), _vp], _i32),
+    "gsa_window_attn_backward": ([ctypes.POINTER(WindowArgs), _vp], _i32),
+    "gsa_window_cache_write": ([_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i32,
+                                _vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp], _i32),
+    "gsa_window_step_workspace_bytes": ([_i32] * 5, ctypes.c_size_t),
+    "gsa_window_step": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
+                         _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp, ctypes.c_size_t, _vp], _i32),
     "gsa_linear_step": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _i64, _i32, _i32, _i32,
                          _i32, _i32, _f32, _i32, _vp, _vp], _i32),
 }
@@ -1188,3 +1210,90 @@ def linear_attn_backward(q, k, v, g, state_in, cu, scale: float, saved, dout, ds
     if st:
         _check(st, "gsa_linear_attn_backward")
     return dq, dk, dv, dg, ds
+
+
+# ---------------------------------------------------------------------------
+# Attention in a sliding window
+# ---------------------------------------------------------------------------
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t [..., heads, 128] with contiguous, 16-byte aligned head rows: itself, or a copy."""
+    size, at = t.element_size(), t.data_ptr()
+    *lead, e = t.stride()
+    for s in lead:
+        at |= s * size
+    return t if e == 1 and at % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _window_args(q, k, v, cu, window: int, sinks: int, scale: float, o, lse) -> WindowArgs:
+    B, T, H, d = q.shape
+    # in the order of the fields
+    return WindowArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(cu),
+                      0 if cu is None else cu.element_size(), B, T, B if cu is None else cu.numel() - 1, H, k.shape[2], d,
+                      dtype_code(q.dtype), window, sinks, scale, o.data_ptr(), _ptr(lse))
+
+
+def window_attn(q, k, v, cu, window: int, sinks: int, scale: float, want_lse: bool):
+    """gsa_window_attn: (o, lse or None).  q, k, v as _heads gives them."""
+    B, T, H, d = q.shape
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = torch.empty(H, B * T, device=q.device, dtype=torch.float32) if want_lse else None
+    if B * T:
+        st = load().gsa_window_attn(ctypes.byref(_window_args(q, k, v, cu, window, sinks, scale, o, lse)), _raw_stream(q))
+        if st:
+            _check(st, "gsa_window_attn")
+    return o, lse
+
+
+def window_attn_backward(q, k, v, cu, window: int, sinks: int, scale: float, o, lse, dout):
+    """gsa_window_attn_backward: (dq, dk, dv)."""
+    dq, dk, dv = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
+    a = _window_args(q, k, v, cu, window, sinks, scale, o, lse)
+    if a.B * a.T == 0:
+        return dq, dk, dv
+    lib = load()
+    n = lib.gsa_window_attn_workspace_bytes(a.B, a.T, a.N, int(cu is not None), a.H, a.Hkv, window, sinks, a.dtype)
+    ws = torch.empty(n, device=q.device, dtype=torch.uint8)
+    a.dout, (a.do_sb, a.do_st, a.do_sh, _) = dout.data_ptr(), dout.stride()
+    a.dq, a.dk, a.dv, a.ws, a.ws_bytes = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n
+    st = lib.gsa_window_attn_backward(ctypes.byref(a), _raw_stream(q))
+    if st:
+        _check(st, "gsa_window_attn_backward")
+    return dq, dk, dv
+
+
+def window_cache_write(k, v, kc, vc, sinks: int, pos, idx, cu) -> None:
+    """gsa_window_cache_write.  k, v as _rows16 gives them."""
+    B, T, Hkv, d = k.shape
+    st = load().gsa_window_cache_write(k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], _ptr(cu),
+                                       0 if cu is None else cu.element_size(), B, T, B if cu is None else cu.numel() - 1, Hkv, d,
+                                       dtype_code(k.dtype), _ptr(pos), 0 if pos is None else pos.element_size(), _ptr(idx),
+                                       0 if idx is None else idx.element_size(), kc.data_ptr(), *kc.stride()[:3], vc.data_ptr(),
+                                       *vc.stride()[:3], kc.shape[0], kc.shape[1], sinks, _raw_stream(k))
+    if st:
+        _check(st, "gsa_window_cache_write")
+
+
+@functools.lru_cache(maxsize=256)
+def _window_step_bytes(*sizes: int) -> int:
+    n = load().gsa_window_step_workspace_bytes(*sizes)
+    if not n:
+        raise ValueError(f"{sizes[0]} rows of {sizes[2]} key heads: at most 65535 of each")
+    return n
+
+
+def window_step(q, k, v, kc, vc, pos, idx, window: int, sinks: int, scale: float) -> torch.Tensor:
+    """gsa_window_step: o [N,H,128]; the caches are updated in place.  q, k, v as _rows16 gives them."""
+    N, H, d = q.shape
+    Hkv = kc.shape[2]
+    n = _window_step_bytes(N, H, Hkv, window, sinks)
+    o = torch.empty(N, H, d, device=q.device, dtype=q.dtype)
+    ws = torch.empty(n, device=q.device, dtype=torch.uint8)
+    kn, kh, vn, vh = (0, 0, 0, 0) if k is None else (*k.stride()[:2], *v.stride()[:2])
+    st = load().gsa_window_step(q.data_ptr(), *q.stride()[:2], _ptr(k), kn, kh, _ptr(v), vn, vh, pos.data_ptr(), pos.element_size(),
+                                _ptr(idx), 0 if idx is None else idx.element_size(), kc.data_ptr(), *kc.stride()[:3], vc.data_ptr(),
+                                *vc.stride()[:3], N, kc.shape[0], kc.shape[1], H, Hkv, d, window, sinks, scale, dtype_code(q.dtype),
+                                o.data_ptr(), ws.data_ptr(), n, _raw_stream(q))
+    if st:
+        _check(st, "gsa_window_step")
+    return o

@@ -26,7 +26,7 @@ ARCH = "gfx950"
 
 HIP_SOURCES = ("indexer.hip", "topk_select.hip", "sparse_attn.hip", "dense_attn.hip", "dense_attn_f32.hip",
                "selected_attn.hip", "proj_fused.hip", "rms_norm.hip", "delta_step.hip", "delta_rule.hip",
-               "linear_step.hip", "linear_attn.hip")
+               "linear_step.hip", "linear_attn.hip", "window_attn.hip", "window_step.hip")
 CXX_SOURCES = ("abi.cpp", "layer.cpp")
 
 # Packed fp32 VALU forms are disabled in device code: the compiler would

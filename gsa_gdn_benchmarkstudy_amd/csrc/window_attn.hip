@@ -1,0 +1,743 @@
+// Attention in a sliding window with a few first tokens that stay visible, forward and backward.
+//
+//   key j is visible to query i:  j <= i  and  (j > i - W  or  j < S)
+//   o_i = sum_j P_ij v_j,  P_ij = 2^(c q_i . k_j - L_i),  c = scale log2 e,  L_i = log2 sum_j 2^(c q_i . k_j)
+// and backwards, with D_i = do_i . o_i:
+//   dS_ij = P_ij (do_i . v_j - D_i)    dq_i = scale sum_j dS_ij k_j    dk_j = scale sum_i dS_ij q_i    dv_j = sum_i P_ij do_i
+//
+// Forward: a block of 4 waves takes 128 queries of a head, walks the tiles of keys that hold a visible one (the first
+// tokens' tiles, then the window's) and keeps the running maximum and sum of each row's softmax.  Both products are taken
+// transposed (v_mfma_f32_32x32x16_bf16): S^T = K Q^T, O^T = V^T P^T, so that lanes l and l ^ 32 hold query l % 32, its
+// softmax state lives in them and P enters the second product from the registers in which it was computed.
+// dq (window_dq_kernel) goes the same way; dk and dv (window_dkv_kernel): a block takes 128 keys of a key head and walks the
+// queries of all heads on it that see them, so that no two blocks write one gradient: no atomics, the same bits on every
+// run.  The first tokens are seen by all later queries; those past the window's are cut into parts of kFar
+// queries, whose sums are added in their order (window_far_kernel).
+//
+// Precision: sums, softmax statistics and D are fp32.  P and dS enter the second products in the inputs' type: bf16 (2^-9 of a
+// term, as the inputs themselves were rounded), or, for fp32, as three bf16 parts each, as all fp32 operands do (chunks.h).
+#include "chunks.h"
+
+namespace gsa {
+
+struct WindowArgs {
+  Seqs s;
+  Rows q, k, v, dout;
+  int B, H, Hkv, W, S;
+  float scale, scale_l2;      // scale log2 e (forward: of |scale|, and above 0)
+  void* o;                    // [B, T, H, 128]
+  float* lse;                 // [H][B * T]: L (forward: nullable)
+  float* D;                   // [H][B * T]
+  void *dq, *dk, *dv;
+  int near, far;              // blocks of window_dkv_kernel: slots of keys, and of far queries times blocks of first tokens
+  int first;                  // blocks of keys with first tokens of a sequence
+  float* near_parts;          // [N][first][Hkv][2][128][128]
+  float* far_parts;           // [slots of far queries][first][Hkv][2][128][128]
+};
+
+constexpr int kRows = 128;    // queries (dk, dv: keys) of a block, 32 a wave
+constexpr int kFar = 1024;    // far queries of a part
+
+template <typename T> struct WindowType;
+template <> struct WindowType<uint16_t> { static constexpr int NP = 1, kTile = 64, kBuffers = 2; };
+template <> struct WindowType<float> { static constexpr int NP = 3, kTile = 32, kBuffers = 1; };
+
+// ---------------------------------------------------------------------------
+// Tiles of kTile rows of 128 elements in LDS: for each bf16 part (plane) rows of 16 units of 16 bytes, unit u of row t in
+// place u ^ swizzle(t), so that neither 16 rows' reads of one unit nor transposed reads of four rows meet in a bank.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int swizzle(int t) { return (t & 7) << 1 | (t >> 3 & 1); }
+// Row m of a 32-row product stands for row perm(m): an accumulator's 8 rows r = 8 s .. + 7 are then 16 s + 8 (l / 32) .. + 7,
+// the 8 that the lane has to hold as an operand of the next product.
+__device__ __forceinline__ int perm(int m) { return (m & ~12) | (m & 4) << 1 | (m & 8) >> 1; }
+
+template <typename T> struct Tile {
+  static constexpr int NP = WindowType<T>::NP, N = WindowType<T>::kTile, kPlane = N * 256, kBytes = NP * kPlane;
+  // Operand with rows t0 + perm(l % 32): elements 16 ks + 8 (l / 32) .. + 7
+  struct RowReader {
+    int at, x;
+    __device__ RowReader(int l) {
+      const int t = perm(l & 31);
+      at = t * 256;
+      x = 16 * (swizzle(t) ^ (l >> 5));
+    }
+    __device__ Parts<NP> read(const char* tile, int t0, int ks) const {
+      Parts<NP> r;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) r.p[i] = *reinterpret_cast<const bf16x8*>(tile + i * kPlane + t0 * 256 + at + ((32 * ks) ^ x));
+      return r;
+    }
+  };
+  // Operand with rows of elements 32 dt + l % 32: rows t0 + 8 (l / 32) .. + 7 of the tile summed over (ds_read_b64_tr_b16: of
+  // 16 lanes, lane i names row i / 4, elements 4 (i % 4) .. + 3 of 16, and gets element i of the four rows)
+  struct ColReader {
+    int at[2];
+    __device__ ColReader(int l) {
+      const int i = l & 15, z = (2 * (l >> 4 & 1) + ((i & 3) >> 1)) ^ (2 * (i >> 2) + (l >> 5));
+      const int row = (8 * (l >> 5) + (i >> 2)) * 256 + 8 * (i & 1);
+      at[0] = row + 16 * z;
+      at[1] = row + 16 * (z ^ 4);
+    }
+    __device__ Parts<NP> read(const char* tile, int t0, int dt) const {
+      Parts<NP> r;
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        s16x4 x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
+              tile + n * kPlane + t0 * 256 + 1024 * e + at[dt & 1] + 16 * ((dt & 2 ? 8 : 0) ^ (8 * e))));
+        r.p[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+      return r;
+    }
+  };
+  // Rows t0 .. of one head (uniform pointer p to row t0, `stride` elements apart) to LDS, `left` of them: rows behind are the
+  // last one again (they are masked).  256 threads; bf16 by direct loads, fp32 by registers (load, then store).
+  struct Loader {
+    static constexpr int kUnits = N * 16 / 256;              // a thread's units
+    floatx4 x[NP == 3 ? 2 * kUnits : 1];
+    __device__ void load(const T* p, int64_t stride, int left, uint32_t lds, int wave, int l) {
+      p = uniform(p);
+      if constexpr (NP == 1) {
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j) {
+          const int t = 16 * j + 4 * wave + (l >> 4), u = (l & 15) ^ swizzle(t);
+          load_lds16(p, (uint32_t)(min(t, left - 1) * (int)stride + 8 * u) * 2u, __builtin_amdgcn_readfirstlane(lds + (4 * j + wave) * 1024));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j) {
+          const int t = 16 * j + 4 * wave + (l >> 4);
+          const T* at = p + (uint32_t)(min(t, left - 1) * (int)stride + 8 * (l & 15));
+          x[2 * j] = *reinterpret_cast<const floatx4*>(at);
+          x[2 * j + 1] = *reinterpret_cast<const floatx4*>(at + 4);
+        }
+      }
+    }
+    __device__ void store(char* tile, int wave, int l) {
+      if constexpr (NP == 3) {
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j) {
+          const int t = 16 * j + 4 * wave + (l >> 4), u = (l & 15) ^ swizzle(t);
+          const Parts<3> p = split_pair(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+          for (int n = 0; n < 3; ++n) *reinterpret_cast<bf16x8*>(tile + n * kPlane + t * 256 + 16 * u) = p.p[n];
+        }
+      }
+    }
+  };
+};
+
+template <int NA, int NB> __device__ __forceinline__ void mma32(floatx16& acc, const Parts<NA>& a, const Parts<NB>& b) {
+#pragma unroll
+  for (int o = 2; o >= 0; --o)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        if (i + j == o) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
+}
+__device__ __forceinline__ void zero(floatx16& x) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = 0.f;
+}
+// Registers 8 s .. + 7 of an accumulator as an operand
+template <int N> __device__ __forceinline__ Parts<N> parts_at(const floatx16& x, int s) {
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = x[8 * s + e];
+  return parts_of<N>(y);
+}
+// Operand with columns of one row of memory each: elements 16 ks + 8 (l / 32) .. + 7
+template <typename T> __device__ __forceinline__ void row_operand(Parts<WindowType<T>::NP> (&x)[8], const T* p, int l) {
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) x[ks] = operand<T>(p + 16 * ks + 8 * (l >> 5), true);
+}
+
+// The transpose of a wave's [128 elements][32 rows] in 4 accumulators to rows of memory: through 32 x 128 elements of LDS of the
+// wave's own.  row: of the wave's rows the i-th, `left` of them are written.
+template <typename T>
+__device__ __forceinline__ void store_rows(const floatx16 (&x)[4], float f, char* lds, T* p, int64_t stride, int left, int l) {
+  const int i = l & 31, h = l >> 5;
+  constexpr int kRowBytes = 128 * sizeof(T);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int at = 32 * dt + 2 * r + 4 * h;               // element of x[dt][r]
+      char* to = lds + i * kRowBytes;
+      if constexpr (sizeof(T) == 2) {
+        const uint2 y = {pack_bf16(x[dt][r] * f, x[dt][r + 1] * f), pack_bf16(x[dt][r + 2] * f, x[dt][r + 3] * f)};
+        *reinterpret_cast<uint2*>(to + (((at >> 3) ^ (i & 15)) << 4) + 2 * (at & 7)) = y;
+      } else {
+        const floatx4 y = {x[dt][r] * f, x[dt][r + 1] * f, x[dt][r + 2] * f, x[dt][r + 3] * f};
+        *reinterpret_cast<floatx4*>(to + (((at >> 2) ^ i) << 4)) = y;
+      }
+    }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // (a wave's LDS accesses keep their order)
+  constexpr int kPieces = kRowBytes / 16, kPer = 64 / kPieces;
+#pragma unroll
+  for (int j = 0; j < 32 / kPer; ++j) {
+    const int t = kPer * j + l / kPieces, u = l % kPieces;
+    const u32x4 y = *reinterpret_cast<const u32x4*>(lds + t * kRowBytes + ((u ^ (sizeof(T) == 2 ? t & 15 : t)) << 4));
+    if (t < left) *reinterpret_cast<u32x4*>(p + t * stride + 16 / sizeof(T) * u) = y;
+  }
+}
+
+// What of a tile of N keys from j0 a wave's queries r0 .. r0 + 31 see: 0 nothing, 1 something, 2 everything.
+template <int N> __device__ __forceinline__ int seen(const WindowArgs& a, int r0, int j0) {
+  if (j0 > r0 + 31 || (j0 + N <= r0 - a.W + 1 && j0 >= a.S)) return 0;
+  return j0 + N - 1 <= r0 && (j0 > r0 + 31 - a.W || j0 + N <= a.S) ? 2 : 1;
+}
+__device__ __forceinline__ bool visible(const WindowArgs& a, int i, int j) { return j <= i && (i - j < a.W || j < a.S); }
+
+// The tiles of keys that queries q0 .. q0 + n - 1 of a sequence of len tokens see
+template <int N> struct KeyTiles {
+  int first, from, count;                                    // tiles of first tokens; the window's first tile; of both
+  __device__ KeyTiles(const WindowArgs& a, int q0, int n, int len) {
+    from = max(0, q0 - a.W + 1) / N;
+    first = min((min(a.S, len) + N - 1) / N, from);
+    count = first + (min(len, q0 + n) + N - 1) / N - from;
+  }
+  __device__ int at(int t) const { return (t < first ? t : from + t - first) * N; }
+};
+
+// One query's output from its visible keys alone, a wave: lane l has elements 2 l, 2 l + 1.
+template <typename T>
+__device__ __forceinline__ void window_row(const WindowArgs& a, const T* q, const T* kbase, const T* vbase, int i, T* o, float* lse, int l) {
+  const float scale = a.scale * kLog2e;
+  const float q0 = to_f32(q[2 * l]), q1 = to_f32(q[2 * l + 1]);
+  float m = -__builtin_inff(), sum = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int j = 0; j <= i; ++j) {
+    if (j >= a.S && j <= i - a.W) j = max(j, i - a.W + 1);
+    const T *k = kbase + j * a.k.st, *v = vbase + j * a.v.st;
+    float s = q0 * to_f32(k[2 * l]) + q1 * to_f32(k[2 * l + 1]);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x, 64);
+    s *= scale;
+    const float top = s > m ? s : m;
+    const float f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top), p = s == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s - top);
+    m = top;
+    sum = sum * f + p;
+    o0 = o0 * f + p * to_f32(v[2 * l]);
+    o1 = o1 * f + p * to_f32(v[2 * l + 1]);
+    if (sum != sum) break;                                   // a score is NaN or +infinity: the whole row is NaN
+  }
+  o[2 * l] = from_f32<T>(sum != sum ? sum : o0 / sum);
+  o[2 * l + 1] = from_f32<T>(sum != sum ? sum : o1 / sum);
+  if (lse && l == 0) *lse = m + __builtin_amdgcn_logf(sum);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
+  using L = Tile<T>;
+  constexpr int NP = L::NP, N = L::N, kBuffers = WindowType<T>::kBuffers, kBuffer = 2 * L::kBytes;
+  extern __shared__ __align__(16) char lds[];
+  const uint32_t base = lds_addr(lds);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+  const int slot = gridDim.x / a.H - 1 - blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hkv);
+  int c;
+  const Span sp = slot_of(a.s, slot, kRows, c);
+  if (c < 0) return;
+  const int q0 = c * kRows, r0 = q0 + 32 * wave, row = r0 + (l & 31), rowc = min(row, sp.len - 1);
+  const T *kbase = uniform(row_at<T>(a.k, sp, 0, hk)), *vbase = uniform(row_at<T>(a.v, sp, 0, hk));
+  const KeyTiles<N> tiles(a, q0, kRows, sp.len);
+  typename L::Loader lk, lv;
+  auto load = [&](int t, int buffer) {
+    const int j0 = tiles.at(t), left = sp.len - j0;
+    lk.load(kbase + j0 * a.k.st, a.k.st, left, base + buffer * kBuffer, wave, l);
+    lv.load(vbase + j0 * a.v.st, a.v.st, left, base + buffer * kBuffer + L::kBytes, wave, l);
+  };
+  load(0, 0);
+  Parts<NP> q[8];
+  row_operand<T>(q, row_at<T>(a.q, sp, rowc, h), l);
+  if (a.scale < 0.f)                                         // (the largest score is then the largest product)
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+      for (int n = 0; n < NP; ++n) q[ks].p[n] = -q[ks].p[n];
+  floatx16 o[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) zero(o[dt]);
+  const typename L::RowReader rows(l);
+  const typename L::ColReader cols(l);
+  // softmax state of the lane's row, log2 domain: the reference m moves only when a tile's maximum exceeds it by more than
+  // kLazy (the sums then stay below 2^8 times what they are, far from fp32's range)
+  constexpr float kLazy = 8.f;
+  float m = -__builtin_inff(), limit = m, minus = 0.f, sum = 0.f;
+  for (int t = 0; t < tiles.count; ++t) {
+    const int buffer = kBuffers == 2 ? t & 1 : 0;
+    char *K = lds + buffer * kBuffer, *V = K + L::kBytes;
+    if constexpr (NP == 3) {
+      if (t) __syncthreads();                                // every wave is through with the last tile
+      lk.store(K, wave, l);
+      lv.store(V, wave, l);
+    }
+    wait_loads();
+    __syncthreads();
+    if (t + 1 < tiles.count) load(t + 1, buffer ^ 1);
+    const int j0 = tiles.at(t), see = r0 < sp.len ? seen<N>(a, r0, j0) : 0;
+    if (!see) continue;
+    floatx16 s[N / 32];
+#pragma unroll
+    for (int n = 0; n < N / 32; ++n) {
+      zero(s[n]);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) mma32(s[n], rows.read(K, 32 * n, ks), q[ks]);
+    }
+    if (see == 1)
+#pragma unroll
+      for (int n = 0; n < N / 32; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = j0 + 32 * n + 16 * (r >> 3) + 8 * (l >> 5) + (r & 7);
+          s[n][r] = visible(a, row, j) ? s[n][r] : -__builtin_inff();
+        }
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int n = 0; n < N / 32; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+    mx = max_halves(mx) * a.scale_l2;
+    if (ballot64(mx > limit)) {                              // some row's reference moves
+      const bool bump = mx > limit;
+      const float f = bump ? __builtin_amdgcn_exp2f(m - mx) : 1.f;           // m = -inf: 0
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+      sum *= f;
+      m = bump ? mx : m;
+      limit = m + kLazy;
+      minus = m == -__builtin_inff() ? 0.f : -m;
+    }
+#pragma unroll
+    for (int n = 0; n < N / 32; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_l2, minus));
+        sum += s[n][r];
+      }
+#pragma unroll
+    for (int n = 0; n < N / 32; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const Parts<NP> p = parts_at<NP>(s[n], k);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) mma32(o[dt], cols.read(V, 32 * n + 16 * k, dt), p);
+      }
+  }
+  sum = sum_halves(sum);
+  __syncthreads();                                           // the tiles are free
+  if (r0 >= sp.len) return;
+  const int left = sp.len - r0;
+  T* out = static_cast<T*>(a.o) + (((int64_t)sp.b * a.s.T + sp.t0 + r0) * a.H + h) * kHead;
+  float odd = sum * 0.f;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(o[dt][r], 0.f, odd);
+  const float f = 1.f / sum;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+  store_rows<T>(o, 1.f, lds + wave * 32 * kHead * sizeof(T), out, (int64_t)a.H * kHead, left, l);
+  float* lse = a.lse ? a.lse + (int64_t)h * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 : nullptr;
+  if (lse && row < sp.len && l < 32) lse[row] = m + __builtin_amdgcn_logf(sum);
+  // A row with something that is not finite in its tiles: what it does not see may have reached it (0 * NaN), so it is
+  // computed once more from its visible keys alone.
+  uint64_t redo = ballot64(!(odd == 0.f));
+  redo = (redo | redo >> 32) & 0xffffffffu;
+  if (__builtin_expect(redo != 0, 0)) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (int i = 0; i < min(32, left); ++i)
+      if (redo >> i & 1)
+        window_row<T>(a, row_at<T>(a.q, sp, r0 + i, h), kbase, vbase, r0 + i, out + (int64_t)i * a.H * kHead, lse ? lse + r0 + i : nullptr, l);
+  }
+}
+
+// dq and D: a block's queries against the tiles of keys, as forwards.
+template <typename T>
+__global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dq_kernel(WindowArgs a) {
+  using L = Tile<T>;
+  constexpr int NP = L::NP, N = L::N, kBuffers = WindowType<T>::kBuffers, kBuffer = 2 * L::kBytes;
+  extern __shared__ __align__(16) char lds[];
+  const uint32_t base = lds_addr(lds);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+  const int slot = gridDim.x / a.H - 1 - blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hkv);
+  int c;
+  const Span sp = slot_of(a.s, slot, kRows, c);
+  if (c < 0) return;
+  const int q0 = c * kRows, r0 = q0 + 32 * wave, row = r0 + (l & 31), rowc = min(row, sp.len - 1);
+  const T *kbase = uniform(row_at<T>(a.k, sp, 0, hk)), *vbase = uniform(row_at<T>(a.v, sp, 0, hk));
+  const KeyTiles<N> tiles(a, q0, kRows, sp.len);
+  typename L::Loader lk, lv;
+  auto load = [&](int t, int buffer) {
+    const int j0 = tiles.at(t), left = sp.len - j0;
+    lk.load(kbase + j0 * a.k.st, a.k.st, left, base + buffer * kBuffer, wave, l);
+    lv.load(vbase + j0 * a.v.st, a.v.st, left, base + buffer * kBuffer + L::kBytes, wave, l);
+  };
+  load(0, 0);
+  Parts<NP> q[8], d[8];
+  row_operand<T>(q, row_at<T>(a.q, sp, rowc, h), l);
+  const T* dout = row_at<T>(a.dout, sp, rowc, h);
+  row_operand<T>(d, dout, l);
+  const int64_t first = (int64_t)sp.b * a.s.T + sp.t0;
+  float D = 0.f;
+  {
+    const T* o = static_cast<const T*>(a.o) + ((first + rowc) * a.H + h) * kHead;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      float x[8], y[8];
+      load8(o + 16 * ks + 8 * (l >> 5), x);
+      load8(dout + 16 * ks + 8 * (l >> 5), y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) D = __builtin_fmaf(x[e], y[e], D);
+    }
+    D = sum_halves(D);
+  }
+  const int64_t at = (int64_t)h * a.B * a.s.T + first + rowc;
+  const float lse = a.lse[at];
+  if (row < sp.len && l < 32) a.D[at] = D;
+  floatx16 acc[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) zero(acc[dt]);
+  const typename L::RowReader rows(l);
+  const typename L::ColReader cols(l);
+  for (int t = 0; t < tiles.count; ++t) {
+    const int buffer = kBuffers == 2 ? t & 1 : 0;
+    char *K = lds + buffer * kBuffer, *V = K + L::kBytes;
+    if constexpr (NP == 3) {
+      if (t) __syncthreads();
+      lk.store(K, wave, l);
+      lv.store(V, wave, l);
+    }
+    wait_loads();
+    __syncthreads();
+    if (t + 1 < tiles.count) load(t + 1, buffer ^ 1);
+    const int j0 = tiles.at(t), see = r0 < sp.len ? seen<N>(a, r0, j0) : 0;
+    if (!see) continue;
+#pragma unroll
+    for (int n = 0; n < N / 32; ++n) {
+      floatx16 s, p;
+      zero(s);
+      zero(p);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) mma32(s, rows.read(K, 32 * n, ks), q[ks]);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) mma32(p, rows.read(V, 32 * n, ks), d[ks]);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, -lse)) * (p[r] - D);
+      if (see == 1)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = j0 + 32 * n + 16 * (r >> 3) + 8 * (l >> 5) + (r & 7);
+          s[r] = visible(a, row, j) ? s[r] : 0.f;
+        }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const Parts<NP> ds = parts_at<NP>(s, k);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) mma32(acc[dt], cols.read(K, 32 * n + 16 * k, dt), ds);
+      }
+    }
+  }
+  __syncthreads();
+  if (r0 >= sp.len) return;
+  store_rows<T>(acc, a.scale, lds + wave * 32 * kHead * sizeof(T), static_cast<T*>(a.dq) + ((first + r0) * a.H + h) * kHead,
+                (int64_t)a.H * kHead, sp.len - r0, l);
+}
+
+// dk and dv of 128 keys of a key head, a wave 32 of them: the queries near them (all that see them, but for far queries of first
+// tokens), or, in the blocks behind, one part of the far queries.
+template <typename T>
+__global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dkv_kernel(WindowArgs a) {
+  using L = Tile<T>;
+  constexpr int NP = L::NP, N = L::N, kBuffers = WindowType<T>::kBuffers, kBuffer = 2 * L::kBytes, kStats = kBuffers * kBuffer;
+  extern __shared__ __align__(16) char lds[];
+  const uint32_t base = lds_addr(lds);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id(), share = a.H / a.Hkv;
+  const int hk = blockIdx.x % a.Hkv;
+  int unit = blockIdx.x / a.Hkv, c, i0, i1, k0;
+  float* parts = nullptr;
+  Span sp;
+  if (unit < a.near) {
+    sp = slot_of(a.s, unit, kRows, c);
+    if (c < 0) return;
+    k0 = c * kRows;
+    i0 = k0;
+    const int64_t end = (int64_t)k0 + kRows - 1 + a.W;
+    i1 = (int)min((int64_t)sp.len, end);
+    if (k0 < a.S && end < sp.len) parts = a.near_parts + (((int64_t)sp.n * a.first + c) * a.Hkv + hk) * 2 * kHead * kHead;
+  } else {
+    unit -= a.near;
+    const int block = unit % a.first;
+    unit /= a.first;
+    sp = slot_of(a.s, unit, kFar, c);
+    k0 = block * kRows;
+    if (c < 0 || k0 >= sp.len) return;
+    const int64_t end = (int64_t)k0 + kRows - 1 + a.W;
+    i0 = (int)max((int64_t)c * kFar, min((int64_t)sp.len, end));
+    i1 = min(sp.len, (c + 1) * kFar);
+    if (i0 >= i1) return;
+    parts = a.far_parts + (((int64_t)unit * a.first + block) * a.Hkv + hk) * 2 * kHead * kHead;
+  }
+  const int j0 = k0 + 32 * wave, key = j0 + (l & 31), keyc = min(key, sp.len - 1);
+  const int tiles = (i1 - i0 + N - 1) / N, count = tiles * share;
+  typename L::Loader lq, ld;
+  float stat[2];                                             // of thread tid < N: L and D of a query
+  auto load = [&](int t, int buffer) {
+    const int h = hk * share + t / tiles, r = i0 + t % tiles * N, left = min(sp.len, i1) - r;
+    lq.load(uniform(row_at<T>(a.q, sp, r, h)), a.q.st, left, base + buffer * kBuffer, wave, l);
+    ld.load(uniform(row_at<T>(a.dout, sp, r, h)), a.dout.st, left, base + buffer * kBuffer + L::kBytes, wave, l);
+    if (tid < N) {
+      const int64_t at = (int64_t)h * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 + r + min(tid, left - 1);
+      stat[0] = a.lse[at];
+      stat[1] = a.D[at];
+    }
+  };
+  load(0, 0);
+  Parts<NP> k[8], v[8];
+  row_operand<T>(k, row_at<T>(a.k, sp, keyc, hk), l);
+  row_operand<T>(v, row_at<T>(a.v, sp, keyc, hk), l);
+  floatx16 dk[4], dv[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) {
+    zero(dk[dt]);
+    zero(dv[dt]);
+  }
+  const typename L::RowReader rows(l);
+  const typename L::ColReader cols(l);
+  for (int t = 0; t < count; ++t) {
+    const int buffer = kBuffers == 2 ? t & 1 : 0;
+    char *Q = lds + buffer * kBuffer, *dO = Q + L::kBytes;
+    float* st = reinterpret_cast<float*>(lds + kStats) + buffer * 2 * N;
+    if constexpr (NP == 3) {
+      if (t) __syncthreads();
+      lq.store(Q, wave, l);
+      ld.store(dO, wave, l);
+    }
+    wait_loads();
+    if (tid < N) {
+      st[tid] = stat[0];
+      st[N + tid] = stat[1];
+    }
+    __syncthreads();
+    if (t + 1 < count) load(t + 1, buffer ^ 1);
+    const int r0 = i0 + t % tiles * N;
+    if (j0 >= sp.len) continue;
+#pragma unroll
+    for (int n = 0; n < N / 32; ++n) {
+      const int i32 = r0 + 32 * n;                           // the 32 queries of this product
+      const int see = i32 < i1 ? seen<32>(a, i32, j0) : 0;
+      if (!see) continue;
+      floatx16 s, p;
+      zero(s);
+      zero(p);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) mma32(s, rows.read(Q, 32 * n, ks), k[ks]);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) mma32(p, rows.read(dO, 32 * n, ks), v[ks]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float lse[8], D[8];
+        load8(st + 32 * n + 16 * x + 8 * (l >> 5), lse);
+        load8(st + N + 32 * n + 16 * x + 8 * (l >> 5), D);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int r = 8 * x + e, i = i32 + 16 * x + 8 * (l >> 5) + e;
+          const bool on = see == 2 && i32 + 31 < i1 ? true : i < i1 && visible(a, i, key);
+          s[r] = on ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, -lse[e])) : 0.f;
+          p[r] = on ? s[r] * (p[r] - D[e]) : 0.f;
+        }
+        const Parts<NP> w = parts_at<NP>(s, x), ds = parts_at<NP>(p, x);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) {
+          mma32(dv[dt], cols.read(dO, 32 * n + 16 * x, dt), w);
+          mma32(dk[dt], cols.read(Q, 32 * n + 16 * x, dt), ds);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (j0 >= sp.len) return;
+  const int left = sp.len - j0;
+  if (parts) {
+    // fp32, through as much LDS as fits: a wave's 32 x 128 at a time
+    char* own = lds + wave * 32 * kHead * 4;
+    static_assert(4 * 32 * kHead * 4 <= kStats + 4096 || NP == 3);
+    store_rows<float>(dk, a.scale, own, parts + 32 * wave * kHead, kHead, 32, l);
+    store_rows<float>(dv, 1.f, own, parts + kHead * kHead + 32 * wave * kHead, kHead, 32, l);
+    return;
+  }
+  char* own = lds + wave * 32 * kHead * sizeof(T);
+  const int64_t o = (((int64_t)sp.b * a.s.T + sp.t0 + j0) * a.Hkv + hk) * kHead;
+  store_rows<T>(dk, a.scale, own, static_cast<T*>(a.dk) + o, (int64_t)a.Hkv * kHead, left, l);
+  store_rows<T>(dv, 1.f, own, static_cast<T*>(a.dv) + o, (int64_t)a.Hkv * kHead, left, l);
+}
+
+// dk and dv of a sequence's first tokens: the near queries' part and those of the far ones, in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void window_far_kernel(WindowArgs a) {
+  const int hk = blockIdx.x % a.Hkv, block = blockIdx.x / a.Hkv % a.first, n = blockIdx.x / a.Hkv / a.first;
+  const Span sp = span_of(a.s, n, kFar);
+  const int k0 = block * kRows;
+  const int64_t end = (int64_t)k0 + kRows - 1 + a.W;
+  if (k0 >= sp.len || end >= sp.len) return;                 // no far queries: written as they were
+  const int64_t one = 2 * kHead * kHead;
+  for (int u = threadIdx.x + 256 * blockIdx.y; u < 2 * kHead * kHead / 8; u += 256 * gridDim.y) {
+    const int t = u / 16 % kHead;
+    if (k0 + t >= sp.len) continue;
+    float x[8];
+    load8(a.near_parts + (((int64_t)n * a.first + block) * a.Hkv + hk) * one + 8 * u, x);
+    for (int c = (int)(end / kFar); c * kFar < sp.len; ++c) {
+      float y[8];
+      load8(a.far_parts + (((int64_t)(sp.slot0 + c) * a.first + block) * a.Hkv + hk) * one + 8 * u, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] += y[e];
+    }
+    T* to = static_cast<T*>(u < kHead * 16 ? a.dk : a.dv);
+    store8(to + (((int64_t)sp.b * a.s.T + sp.t0 + k0 + t) * a.Hkv + hk) * kHead + 8 * (u % 16), x);
+  }
+}
+
+}  // namespace gsa
+
+namespace gsa_host {
+namespace {
+
+struct WindowPlan {
+  int64_t slots, far;         // blocks of queries or keys of all sequences; parts of far queries (0: no far queries)
+  int first, W, S;
+  size_t D, near_parts, far_parts;
+};
+bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, int sinks, int dtype, WindowPlan& z) {
+  z = WindowPlan{};
+  if (B < 1 || T < 1 || N < 1 || Hkv < 1 || H < Hkv || H % Hkv || H > 65535 || window < 1 || sinks < 0 || !dtype_size(dtype)) return false;
+  z.W = std::min(window, T);
+  z.S = std::min(sinks, T);
+  z.slots = packed ? (int64_t)T / gsa::kRows + N : (int64_t)B * ((T + gsa::kRows - 1) / gsa::kRows);
+  // a grid of 256 threads a block: a launch has less than 2^32 of them
+  if (z.slots > (1 << 23) / H || (int64_t)B * T >= (int64_t)1 << 31) return false;
+  if (z.S && z.W < T) {
+    z.first = (z.S + gsa::kRows - 1) / gsa::kRows;
+    z.far = packed ? (int64_t)T / gsa::kFar + N : (int64_t)B * ((T + gsa::kFar - 1) / gsa::kFar);
+    if (z.far * z.first + z.slots > (1 << 23) / H || (int64_t)N * z.first > (1 << 23) / H) return false;
+  }
+  const size_t one = (size_t)Hkv * 2 * 128 * 128 * 4;
+  z.D = up((size_t)H * B * T * 4);
+  z.near_parts = (size_t)N * z.first * one;
+  z.far_parts = (size_t)z.far * z.first * one;
+  return true;
+}
+
+int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, WindowPlan& z) {
+  if (!x || !x->q || !x->k || !x->v || !x->o) return GSA_ERR_NULL;
+  if (backward && (!x->dout || !x->dq || !x->dk || !x->dv || !x->lse || !x->ws)) return GSA_ERR_NULL;
+  if (!dtype_size(x->dtype)) return GSA_ERR_DTYPE;
+  if (x->d != 128 || (x->cu_seqlens ? x->B != 1 || (x->cu_bytes != 4 && x->cu_bytes != 8) : x->N != x->B)) return GSA_ERR_SHAPE;
+  if (!window_plan(x->B, x->T, x->N, x->cu_seqlens != nullptr, x->H, x->Hkv, x->window, x->sinks, x->dtype, z)) return GSA_ERR_SHAPE;
+  if (backward && x->ws_bytes < z.D + z.near_parts + z.far_parts) return GSA_ERR_SHAPE;
+  // a tile's rows are addressed by 32-bit offsets
+  for (int64_t st : {x->q_st, x->k_st, x->v_st, backward ? x->do_st : (int64_t)0})
+    if (st < 0 || st * 64 * dtype_size(x->dtype) >= (int64_t)1 << 31) return GSA_ERR_SHAPE;
+  auto vec = [&](const void* p, int64_t sb, int64_t st, int64_t sh) {
+    return vec_ok(p, sb, st, x->dtype) && sh % (x->dtype == GSA_DTYPE_BF16 ? 8 : 4) == 0;
+  };
+  if (!vec(x->q, x->q_sb, x->q_st, x->q_sh) || !vec(x->k, x->k_sb, x->k_st, x->k_sh) || !vec(x->v, x->v_sb, x->v_st, x->v_sh) ||
+      (backward && !vec(x->dout, x->do_sb, x->do_st, x->do_sh)))
+    return GSA_ERR_ALIGN;
+  for (const void* p : {(const void*)x->o, (const void*)x->dq, (const void*)x->dk, (const void*)x->dv, (const void*)x->ws})
+    if (p && !aligned(p, 16)) return GSA_ERR_ALIGN;
+  if (!aligned(x->lse, 4) || (x->cu_seqlens && !aligned(x->cu_seqlens, x->cu_bytes))) return GSA_ERR_ALIGN;
+  a = gsa::WindowArgs{};
+  a.s = {x->cu_seqlens, x->cu_bytes == 8, x->N, x->T};
+  a.q = {x->q, x->q_sb, x->q_st, x->q_sh};
+  a.k = {x->k, x->k_sb, x->k_st, x->k_sh};
+  a.v = {x->v, x->v_sb, x->v_st, x->v_sh};
+  a.B = x->B;
+  a.H = x->H;
+  a.Hkv = x->Hkv;
+  a.W = z.W;
+  a.S = z.S;
+  a.scale = x->scale;
+  a.scale_l2 = x->scale * gsa::kLog2e;
+  if (!backward) a.scale_l2 = std::max(a.scale_l2 < 0.f ? -a.scale_l2 : a.scale_l2, 1.17549435e-38f);
+  a.o = x->o;
+  a.lse = x->lse;
+  if (backward) {
+    a.dout = {x->dout, x->do_sb, x->do_st, x->do_sh};
+    a.dq = x->dq;
+    a.dk = x->dk;
+    a.dv = x->dv;
+    char* w = static_cast<char*>(x->ws);
+    a.D = reinterpret_cast<float*>(w);
+    a.near = (int)z.slots;
+    a.far = (int)(z.far * z.first);
+    a.first = std::max(z.first, 1);
+    a.near_parts = reinterpret_cast<float*>(w + z.D);
+    a.far_parts = reinterpret_cast<float*>(w + z.D + z.near_parts);
+  }
+  return GSA_OK;
+}
+int window_outside(const gsa::WindowArgs& a, const gsa_window_args* x, bool backward, hipStream_t s) {
+  if (!a.s.cu) return GSA_OK;
+  const int64_t row = 128 * (int64_t)dtype_size(x->dtype);
+  const gsa::Outside o = backward ? gsa::Outside{a.s, {(char*)x->dq, (char*)x->dk, (char*)x->dv}, {a.H * row, a.Hkv * row, a.Hkv * row}}
+                                  : gsa::Outside{a.s, {(char*)x->o}, {a.H * row}};
+  hipLaunchKernelGGL(gsa::outside_kernel, dim3(256), dim3(256), 0, s, o);
+  return launch_status();
+}
+template <typename T> struct WindowLds {
+  using L = gsa::Tile<T>;
+  static constexpr size_t kTiles = (size_t)gsa::WindowType<T>::kBuffers * 2 * L::kBytes;
+  static constexpr size_t kRows = 4 * 32 * 128 * 4;          // a wave's rows on the way out, fp32
+  static constexpr size_t kFwd = kTiles > kRows ? kTiles : kRows, kDkv = kFwd + (size_t)gsa::WindowType<T>::kBuffers * 2 * L::N * 4;
+};
+
+template <typename T> int window_forward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+  constexpr size_t lds = WindowLds<T>::kFwd;
+  if (const int e = allow_lds<gsa::window_fwd_kernel<T>>(lds)) return e;
+  hipLaunchKernelGGL(gsa::window_fwd_kernel<T>, dim3(z.slots * a.H), dim3(256), lds, s, a);
+  return launch_status();
+}
+template <typename T> int window_backward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+  constexpr size_t lds = WindowLds<T>::kFwd, more = WindowLds<T>::kDkv;
+  if (const int e = allow_lds<gsa::window_dq_kernel<T>>(lds)) return e;
+  if (const int e = allow_lds<gsa::window_dkv_kernel<T>>(more)) return e;
+  hipLaunchKernelGGL(gsa::window_dq_kernel<T>, dim3(z.slots * a.H), dim3(256), lds, s, a);
+  if (const int e = launch_status()) return e;
+  hipLaunchKernelGGL(gsa::window_dkv_kernel<T>, dim3((a.near + a.far) * a.Hkv), dim3(256), more, s, a);
+  if (const int e = launch_status()) return e;
+  if (a.far) {
+    hipLaunchKernelGGL(gsa::window_far_kernel<T>, dim3(a.s.N * a.first * a.Hkv, 4), dim3(256), 0, s, a);
+    if (const int e = launch_status()) return e;
+  }
+  return GSA_OK;
+}
+
+}  // namespace
+}  // namespace gsa_host
+
+extern "C" size_t gsa_window_attn_workspace_bytes(int B, int T, int N, int packed, int H, int Hkv, int window, int sinks, int dtype) {
+  gsa_host::WindowPlan z;
+  return gsa_host::window_plan(B, T, N, packed, H, Hkv, window, sinks, dtype, z) ? z.D + z.near_parts + z.far_parts : 0;
+}
+extern "C" int gsa_window_attn(const gsa_window_args* x, void* stream) {
+  gsa::WindowArgs a;
+  gsa_host::WindowPlan z;
+  if (const int e = gsa_host::window_args(x, false, a, z)) return e;
+  const auto s = static_cast<hipStream_t>(stream);
+  const int e = x->dtype == GSA_DTYPE_BF16 ? gsa_host::window_forward<uint16_t>(a, z, s) : gsa_host::window_forward<float>(a, z, s);
+  return e ? e : gsa_host::window_outside(a, x, false, s);
+}
+extern "C" int gsa_window_attn_backward(const gsa_window_args* x, void* stream) {
+  gsa::WindowArgs a;
+  gsa_host::WindowPlan z;
+  if (const int e = gsa_host::window_args(x, true, a, z)) return e;
+  const auto s = static_cast<hipStream_t>(stream);
+  const int e = x->dtype == GSA_DTYPE_BF16 ? gsa_host::window_backward<uint16_t>(a, z, s) : gsa_host::window_backward<float>(a, z, s);
+  return e ? e : gsa_host::window_outside(a, x, true, s);
+}

@@ -619,7 +619,7 @@ int gsa_delta_rule_backward(const gsa_delta_args* args, void* stream);
  * The forward fills `saved` (gsa_linear_attn_saved_bytes, which may be 0) where a backward pass follows; the backward
  * pass reads it and writes dq, dk, dv and, where they are not NULL, dg and dstate_in (both calls with the same sizes).
  * Rows of o and of the gradients outside every packed sequence become 0.  Head rows contiguous; q, k, v, dout rows
- * 16-byte aligned, less than 32 MiB apart (fp32: 8 MiB).  *_workspace_bytes: (size_t)-1 for sizes that are refused.
+ * 16-byte aligned, less than 32 MiB apart.  *_workspace_bytes: (size_t)-1 for sizes that are refused.
  */
 typedef struct gsa_linear_args {
   const void *q, *k, *v;
@@ -655,6 +655,56 @@ int gsa_linear_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, in
                     int64_t v_sn, int64_t v_sh, const float* g, int64_t g_sh, const void* state_idx, int idx_bytes,
                     float* state, int64_t s_sn, int64_t s_sh, int N, int slots, int Hk, int Hv, int d, float scale,
                     int dtype, void* o, void* stream);
+
+/*
+ * Attention in a sliding window with first tokens that stay visible: key j is visible to query i where j <= i and
+ * (j > i - window or j < sinks), positions counted in each sequence.  No counterpart in the reference (its sparse
+ * attention with a fixed selection).  q, o [B,T,H,128], k, v [B,T,Hkv,128] in dtype, head h on key head h / (H/Hkv);
+ * o contiguous.  cu_seqlens as in gsa_delta_args.  The forward writes lse (fp32 [H][B*T], or NULL), which, with o, the
+ * backward pass reads; that takes a workspace and writes dq, dk and dv (contiguous).  Rows of o and of the gradients outside
+ * every packed sequence become 0.  Head rows contiguous; q, k, v, dout rows 16-byte aligned, less than 32 MiB apart.
+ * gsa_window_attn_workspace_bytes: 0 for sizes that are refused.
+ */
+typedef struct gsa_window_args {
+  const void *q, *k, *v;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  const void* cu_seqlens;
+  int cu_bytes, B, T, N, H, Hkv, d, dtype, window, sinks;
+  float scale;
+  void* o;
+  float* lse;
+  const void* dout;
+  int64_t do_sb, do_st, do_sh;
+  void *dq, *dk, *dv;
+  void* ws;
+  size_t ws_bytes;
+} gsa_window_args;
+size_t gsa_window_attn_workspace_bytes(int B, int T, int N, int packed, int H, int Hkv, int window, int sinks, int dtype);
+int gsa_window_attn(const gsa_window_args* args, void* stream);
+int gsa_window_attn_backward(const gsa_window_args* args, void* stream);
+
+/*
+ * The cache of window attention: per sequence `sinks` rows of first tokens and a ring of rows - sinks behind them, the token
+ * at position p in row p (p < sinks) or sinks + (p - sinks) % (rows - sinks).  k_cache, v_cache [slots,rows,Hkv,128] in
+ * dtype, 16-byte aligned rows.  cache_idx (int32 or int64 by idx_bytes, or NULL): the slot of each sequence; one outside
+ * [0, slots) is skipped, as is a negative position.
+ * gsa_window_cache_write: k, v [B,T,Hkv,128] of B sequences (or N packed ones, cu_seqlens); positions (int32 or int64 [N], or
+ * NULL: 0) of each one's first token.
+ * gsa_window_step: row n's token at positions[n], q, o [N,H,128]: k, v [N,Hkv,128] (or both NULL: they are there) go to the
+ * cache, then o is the attention over the window's and the first tokens' keys; 0 for a skipped row.  rows >= window +
+ * sinks.  ws: gsa_window_step_workspace_bytes (0: sizes that are refused), one for each call in flight.
+ */
+int gsa_window_cache_write(const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
+                           int64_t v_sh, const void* cu_seqlens, int cu_bytes, int B, int T, int N, int Hkv, int d, int dtype,
+                           const void* positions, int pos_bytes, const void* cache_idx, int idx_bytes, void* k_cache,
+                           int64_t kc_sn, int64_t kc_st, int64_t kc_sh, void* v_cache, int64_t vc_sn, int64_t vc_st,
+                           int64_t vc_sh, int slots, int rows, int sinks, void* stream);
+size_t gsa_window_step_workspace_bytes(int N, int H, int Hkv, int window, int sinks);
+int gsa_window_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int64_t k_sn, int64_t k_sh, const void* v,
+                    int64_t v_sn, int64_t v_sh, const void* positions, int pos_bytes, const void* cache_idx, int idx_bytes,
+                    void* k_cache, int64_t kc_sn, int64_t kc_st, int64_t kc_sh, void* v_cache, int64_t vc_sn, int64_t vc_st,
+                    int64_t vc_sh, int N, int slots, int rows, int H, int Hkv, int d, int window, int sinks, float scale,
+                    int dtype, void* o, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
