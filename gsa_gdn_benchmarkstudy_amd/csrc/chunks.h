@@ -26,7 +26,8 @@ template <int N> struct Parts { bf16x8 p[N]; };
 
 // Rounded to bf16 by pairs (one v_cvt_pk_bf16_f32); what is left of them.
 __device__ __forceinline__ uint32_t take_part(float& x, float& y) {
-  const uint32_t p = pack_bf16(x, y);
+  uint32_t p = pack_bf16(x, y);
+  asm("" : "+v"(p));                                         // (else the compiler converts x once more by itself)
   x -= bf16lo(p);
   y -= bf16hi(p);
   return p;
@@ -283,26 +284,31 @@ struct Outside {
   char* p[5];
   int64_t bytes[5];
 };
-static __global__ __launch_bounds__(256) void outside_kernel(Outside a) {
+// By the first 256 threads of each of `blocks` blocks.
+__device__ __forceinline__ void clear_outside(const Outside& a, int block, int blocks) {
   __shared__ int most[4];
   int hi = 0;
-  for (int n = threadIdx.x; n <= a.s.N; n += 256) hi = max(hi, (int)a.s.at(n));
+  const bool on = threadIdx.x < 256;
+  for (int n = threadIdx.x; on && n <= a.s.N; n += 256) hi = max(hi, (int)a.s.at(n));
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) hi = max(hi, __shfl_xor(hi, o, 64));
-  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = hi;
+  if (on && (threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = hi;
   __syncthreads();
   hi = max(max(most[0], most[1]), max(most[2], most[3]));
+  if (!on) return;
   const int64_t lo = a.s.at(0);
   for (int i = 0; i < 5; ++i) {
     if (!a.p[i]) continue;
     auto clear = [&](int64_t from, int64_t to) {             // whole elements, 2 bytes at least
       uint16_t* p = reinterpret_cast<uint16_t*>(a.p[i] + from * a.bytes[i]);
-      for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < (to - from) * a.bytes[i] / 2; k += (int64_t)gridDim.x * 256) p[k] = 0;
+      for (int64_t k = (int64_t)block * 256 + threadIdx.x; k < (to - from) * a.bytes[i] / 2; k += (int64_t)blocks * 256) p[k] = 0;
     };
     clear(0, lo);
     clear(hi, a.s.T);
   }
 }
+
+static __global__ __launch_bounds__(256) void outside_kernel(Outside a) { clear_outside(a, blockIdx.x, gridDim.x); }
 
 }  // namespace gsa
 
