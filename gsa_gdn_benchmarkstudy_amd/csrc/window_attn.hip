@@ -29,14 +29,14 @@ struct WindowArgs {
   float* lse;                 // [H][B * T]: L (forward: nullable)
   float* D;                   // [H][B * T]
   void *dq, *dk, *dv;
-  int near, far;              // blocks of window_dkv_kernel: slots of keys, and of far queries times blocks of first tokens
-  int first;                  // blocks of keys with first tokens of a sequence
-  float* near_parts;          // [N][first][Hkv][2][128][128]
-  float* far_parts;           // [slots of far queries][first][Hkv][2][128][128]
+  // dk and dv: blocks of near_keys keys; the far queries of first tokens in parts of kFar queries of a head, far_keys keys a block
+  int near_keys, near_first, far_keys, far_first;            // first: blocks of a sequence's first tokens
+  float* near_parts;          // [N][near_first][Hkv][2][near_keys][128]
+  float* far_parts;           // [slots of far queries][far_first][H][2][far_keys][128]
 };
 
-constexpr int kRows = 128;    // queries (dk, dv: keys) of a block, 32 a wave
-constexpr int kFar = 1024;    // far queries of a part
+constexpr int kRows = 128;    // queries of a block, 32 a wave
+constexpr int kFar = 512;     // far queries of a part
 
 template <typename T> struct WindowType;
 template <> struct WindowType<uint16_t> { static constexpr int NP = 1, kTile = 64, kBuffers = 2; };
@@ -51,8 +51,8 @@ __device__ __forceinline__ int swizzle(int t) { return (t & 7) << 1 | (t >> 3 & 
 // the 8 that the lane has to hold as an operand of the next product.
 __device__ __forceinline__ int perm(int m) { return (m & ~12) | (m & 4) << 1 | (m & 8) >> 1; }
 
-template <typename T> struct Tile {
-  static constexpr int NP = WindowType<T>::NP, N = WindowType<T>::kTile, kPlane = N * 256, kBytes = NP * kPlane;
+template <typename T, int kN = WindowType<T>::kTile> struct Tile {
+  static constexpr int NP = WindowType<T>::NP, N = kN, kPlane = N * 256, kBytes = NP * kPlane;
   // Operand with rows t0 + perm(l % 32): elements 16 ks + 8 (l / 32) .. + 7
   struct RowReader {
     int at, x;
@@ -103,13 +103,13 @@ template <typename T> struct Tile {
 #pragma unroll
         for (int j = 0; j < kUnits; ++j) {
           const int t = 16 * j + 4 * wave + (l >> 4), u = (l & 15) ^ swizzle(t);
-          load_lds16(p, (uint32_t)(min(t, left - 1) * (int)stride + 8 * u) * 2u, __builtin_amdgcn_readfirstlane(lds + (4 * j + wave) * 1024));
+          load_lds16(p, ((uint32_t)min(t, left - 1) * (uint32_t)stride + 8 * u) * 2u, __builtin_amdgcn_readfirstlane(lds + (4 * j + wave) * 1024));
         }
       } else {
 #pragma unroll
         for (int j = 0; j < kUnits; ++j) {
           const int t = 16 * j + 4 * wave + (l >> 4);
-          const T* at = p + (uint32_t)(min(t, left - 1) * (int)stride + 8 * (l & 15));
+          const T* at = p + ((uint32_t)min(t, left - 1) * (uint32_t)stride + 8 * (l & 15));
           x[2 * j] = *reinterpret_cast<const floatx4*>(at);
           x[2 * j + 1] = *reinterpret_cast<const floatx4*>(at + 4);
         }
@@ -450,48 +450,65 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dq
                 (int64_t)a.H * kHead, sp.len - r0, l);
 }
 
-// dk and dv of 128 keys of a key head, a wave 32 of them: the queries near them (all that see them, but for far queries of first
-// tokens), or, in the blocks behind, one part of the far queries.
-template <typename T>
+// Tiles of queries for kGroups groups of 32 keys: at least 32 queries for each wave of a group
+template <typename T, int kGroups> struct WindowGrads {
+  static constexpr int kRows32 = 4 / kGroups, kLeast = WindowType<T>::kTile / 32;
+  using L = Tile<T, 32 * (kRows32 > kLeast ? kRows32 : kLeast)>;
+  static constexpr int kBuffers = WindowType<T>::kBuffers, kTiles = kBuffers * 2 * L::kBytes;
+  static constexpr int kOut = kGroups * 32 * kHead * 4;      // rows on the way out, or the waves' sums
+  static constexpr size_t kBytes = (kTiles > kOut ? kTiles : kOut) + kBuffers * 2 * L::N * 4;
+};
+
+// dk and dv of 32 kGroups keys of a key head.  A wave has 32 of them, and of the tiles' queries each 4 / kGroups-th 32.
+// kFarPart: a part of the far queries of first tokens; otherwise the queries near the keys: all that see them, but for those.
+template <typename T, int kGroups, bool kFarPart>
 __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dkv_kernel(WindowArgs a) {
-  using L = Tile<T>;
-  constexpr int NP = L::NP, N = L::N, kBuffers = WindowType<T>::kBuffers, kBuffer = 2 * L::kBytes, kStats = kBuffers * kBuffer;
+  using W = WindowGrads<T, kGroups>;
+  using L = typename W::L;
+  constexpr int NP = L::NP, N = L::N, kBuffers = W::kBuffers, kBuffer = 2 * L::kBytes, kKeys = 32 * kGroups, kSplit = 4 / kGroups;
   extern __shared__ __align__(16) char lds[];
   const uint32_t base = lds_addr(lds);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id(), share = a.H / a.Hkv;
-  const int hk = blockIdx.x % a.Hkv;
-  int unit = blockIdx.x / a.Hkv, c, i0, i1, k0;
+  int unit, hk, h0, heads, c, i0, i1, k0;
   float* parts = nullptr;
   Span sp;
-  if (unit < a.near) {
-    sp = slot_of(a.s, unit, kRows, c);
+  if constexpr (!kFarPart) {
+    hk = blockIdx.x % a.Hkv;
+    h0 = hk * share;
+    heads = share;
+    unit = blockIdx.x / a.Hkv;
+    sp = slot_of(a.s, unit, kKeys, c);
     if (c < 0) return;
-    k0 = c * kRows;
+    k0 = c * kKeys;
     i0 = k0;
-    const int64_t end = (int64_t)k0 + kRows - 1 + a.W;
+    const int64_t end = (int64_t)k0 + kKeys - 1 + a.W;
     i1 = (int)min((int64_t)sp.len, end);
-    if (k0 < a.S && end < sp.len) parts = a.near_parts + (((int64_t)sp.n * a.first + c) * a.Hkv + hk) * 2 * kHead * kHead;
+    if (k0 < a.S && end < sp.len) parts = a.near_parts + (((int64_t)sp.n * a.near_first + c) * a.Hkv + hk) * 2 * kKeys * kHead;
   } else {
-    unit -= a.near;
-    const int block = unit % a.first;
-    unit /= a.first;
+    h0 = blockIdx.x % a.H;
+    hk = h0 / share;
+    heads = 1;
+    unit = blockIdx.x / a.H;
+    const int block = unit % a.far_first;
+    unit /= a.far_first;
     sp = slot_of(a.s, unit, kFar, c);
-    k0 = block * kRows;
+    k0 = block * kKeys;
     if (c < 0 || k0 >= sp.len) return;
-    const int64_t end = (int64_t)k0 + kRows - 1 + a.W;
+    const int64_t end = (int64_t)k0 / a.near_keys * a.near_keys + a.near_keys - 1 + a.W;
     i0 = (int)max((int64_t)c * kFar, min((int64_t)sp.len, end));
     i1 = min(sp.len, (c + 1) * kFar);
     if (i0 >= i1) return;
-    parts = a.far_parts + (((int64_t)unit * a.first + block) * a.Hkv + hk) * 2 * kHead * kHead;
+    parts = a.far_parts + (((int64_t)unit * a.far_first + block) * a.H + h0) * 2 * kKeys * kHead;
   }
-  const int j0 = k0 + 32 * wave, key = j0 + (l & 31), keyc = min(key, sp.len - 1);
-  const int tiles = (i1 - i0 + N - 1) / N, count = tiles * share;
+  const int group = wave % kGroups, split = wave / kGroups;
+  const int j0 = k0 + 32 * group, key = j0 + (l & 31), keyc = min(key, sp.len - 1);
+  const int tiles = (i1 - i0 + N - 1) / N, count = tiles * heads;
   typename L::Loader lq, ld;
   float stat[2];                                             // of thread tid < N: L and D of a query
   auto load = [&](int t, int buffer) {
-    const int h = hk * share + t / tiles, r = i0 + t % tiles * N, left = min(sp.len, i1) - r;
-    lq.load(uniform(row_at<T>(a.q, sp, r, h)), a.q.st, left, base + buffer * kBuffer, wave, l);
-    ld.load(uniform(row_at<T>(a.dout, sp, r, h)), a.dout.st, left, base + buffer * kBuffer + L::kBytes, wave, l);
+    const int h = h0 + t / tiles, r = i0 + t % tiles * N, left = min(sp.len, i1) - r;
+    lq.load(row_at<T>(a.q, sp, r, h), a.q.st, left, base + buffer * kBuffer, wave, l);
+    ld.load(row_at<T>(a.dout, sp, r, h), a.dout.st, left, base + buffer * kBuffer + L::kBytes, wave, l);
     if (tid < N) {
       const int64_t at = (int64_t)h * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 + r + min(tid, left - 1);
       stat[0] = a.lse[at];
@@ -513,9 +530,9 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
   for (int t = 0; t < count; ++t) {
     const int buffer = kBuffers == 2 ? t & 1 : 0;
     char *Q = lds + buffer * kBuffer, *dO = Q + L::kBytes;
-    float* st = reinterpret_cast<float*>(lds + kStats) + buffer * 2 * N;
-    if constexpr (NP == 3) {
-      if (t) __syncthreads();
+    float* st = reinterpret_cast<float*>(lds + W::kTiles) + buffer * 2 * N;
+    if constexpr (kBuffers == 1) {
+      if (t) __syncthreads();                                // every wave is through with the last tile
       lq.store(Q, wave, l);
       ld.store(dO, wave, l);
     }
@@ -528,8 +545,8 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
     if (t + 1 < count) load(t + 1, buffer ^ 1);
     const int r0 = i0 + t % tiles * N;
     if (j0 >= sp.len) continue;
-#pragma unroll
-    for (int n = 0; n < N / 32; ++n) {
+#pragma unroll 1                                             // (unrolled, two such products at once do not fit the registers)
+    for (int n = split; n < N / 32; n += kSplit) {
       const int i32 = r0 + 32 * n;                           // the 32 queries of this product
       const int see = i32 < i1 ? seen<32>(a, i32, j0) : 0;
       if (!see) continue;
@@ -540,18 +557,30 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
       for (int ks = 0; ks < 8; ++ks) mma32(s, rows.read(Q, 32 * n, ks), k[ks]);
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) mma32(p, rows.read(dO, 32 * n, ks), v[ks]);
+      asm volatile("" : "+v"(s), "+v"(p));
+      const float* stats = st + 32 * n + 8 * (here(l) >> 5);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        float lse[8], D[8];
-        load8(st + 32 * n + 16 * x + 8 * (l >> 5), lse);
-        load8(st + N + 32 * n + 16 * x + 8 * (l >> 5), D);
+        float y[8];
+        load8(stats + 16 * x, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int r = 8 * x + e, i = i32 + 16 * x + 8 * (l >> 5) + e;
-          const bool on = see == 2 && i32 + 31 < i1 ? true : i < i1 && visible(a, i, key);
-          s[r] = on ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, -lse[e])) : 0.f;
-          p[r] = on ? s[r] * (p[r] - D[e]) : 0.f;
+        for (int e = 0; e < 8; ++e) s[8 * x + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * x + e], a.scale_l2, -y[e]));
+        load8(stats + N + 16 * x, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[8 * x + e] = s[8 * x + e] * (p[8 * x + e] - y[e]);
+      }
+      if (see == 1 || i32 + 32 > i1) {
+        const int lh = here(l), i = i32 + 8 * (lh >> 5), j = j0 + (lh & 31);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int ir = i + 16 * (r >> 3) + (r & 7);
+          const bool on = ir < i1 && visible(a, ir, j);
+          s[r] = on ? s[r] : 0.f;
+          p[r] = on ? p[r] : 0.f;
         }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
         const Parts<NP> w = parts_at<NP>(s, x), ds = parts_at<NP>(p, x);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) {
@@ -561,18 +590,35 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
       }
     }
   }
-  __syncthreads();
+  __syncthreads();                                           // the tiles are free
+  if constexpr (kSplit > 1) {
+    // the sums of the waves that share their keys, one after the other: a wave's accumulators of dk, then of dv, through LDS
+    float* swap = reinterpret_cast<float*>(lds) + group * 64 * 64 + l;
+#pragma unroll 1
+    for (int w = 1; w < kSplit; ++w)
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        floatx16 (&x)[4] = which ? dv : dk;
+        if (split == w)
+#pragma unroll
+          for (int r = 0; r < 64; ++r) swap[64 * r] = x[r >> 4][r & 15];
+        __syncthreads();
+        if (split == 0)
+#pragma unroll
+          for (int r = 0; r < 64; ++r) x[r >> 4][r & 15] += swap[64 * r];
+        __syncthreads();
+      }
+    if (split) return;
+  }
   if (j0 >= sp.len) return;
   const int left = sp.len - j0;
   if (parts) {
-    // fp32, through as much LDS as fits: a wave's 32 x 128 at a time
-    char* own = lds + wave * 32 * kHead * 4;
-    static_assert(4 * 32 * kHead * 4 <= kStats + 4096 || NP == 3);
-    store_rows<float>(dk, a.scale, own, parts + 32 * wave * kHead, kHead, 32, l);
-    store_rows<float>(dv, 1.f, own, parts + kHead * kHead + 32 * wave * kHead, kHead, 32, l);
+    char* own = lds + group * 32 * kHead * 4;
+    store_rows<float>(dk, a.scale, own, parts + 32 * group * kHead, kHead, 32, l);
+    store_rows<float>(dv, 1.f, own, parts + (kKeys + 32 * group) * kHead, kHead, 32, l);
     return;
   }
-  char* own = lds + wave * 32 * kHead * sizeof(T);
+  char* own = lds + group * 32 * kHead * sizeof(T);
   const int64_t o = (((int64_t)sp.b * a.s.T + sp.t0 + j0) * a.Hkv + hk) * kHead;
   store_rows<T>(dk, a.scale, own, static_cast<T*>(a.dk) + o, (int64_t)a.Hkv * kHead, left, l);
   store_rows<T>(dv, 1.f, own, static_cast<T*>(a.dv) + o, (int64_t)a.Hkv * kHead, left, l);
@@ -581,25 +627,29 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
 // dk and dv of a sequence's first tokens: the near queries' part and those of the far ones, in their order.
 template <typename T>
 __global__ __launch_bounds__(256) void window_far_kernel(WindowArgs a) {
-  const int hk = blockIdx.x % a.Hkv, block = blockIdx.x / a.Hkv % a.first, n = blockIdx.x / a.Hkv / a.first;
+  const int hk = blockIdx.x % a.Hkv, block = blockIdx.x / a.Hkv % a.near_first, n = blockIdx.x / a.Hkv / a.near_first, share = a.H / a.Hkv;
   const Span sp = span_of(a.s, n, kFar);
-  const int k0 = block * kRows;
-  const int64_t end = (int64_t)k0 + kRows - 1 + a.W;
+  const int k0 = block * a.near_keys;
+  const int64_t end = (int64_t)k0 + a.near_keys - 1 + a.W;
   if (k0 >= sp.len || end >= sp.len) return;                 // no far queries: written as they were
-  const int64_t one = 2 * kHead * kHead;
-  for (int u = threadIdx.x + 256 * blockIdx.y; u < 2 * kHead * kHead / 8; u += 256 * gridDim.y) {
-    const int t = u / 16 % kHead;
-    if (k0 + t >= sp.len) continue;
+  const int near = a.near_keys * kHead, far = a.far_keys * kHead;
+  for (int u = threadIdx.x + 256 * blockIdx.y; u < 2 * near / 8; u += 256 * gridDim.y) {
+    const int which = 8 * u >= near, t = u / 16 - which * a.near_keys, key = k0 + t, e = 8 * (u % 16);
+    if (key >= sp.len) continue;
     float x[8];
-    load8(a.near_parts + (((int64_t)n * a.first + block) * a.Hkv + hk) * one + 8 * u, x);
-    for (int c = (int)(end / kFar); c * kFar < sp.len; ++c) {
-      float y[8];
-      load8(a.far_parts + (((int64_t)(sp.slot0 + c) * a.first + block) * a.Hkv + hk) * one + 8 * u, y);
+    load8(a.near_parts + (((int64_t)n * a.near_first + block) * a.Hkv + hk) * 2 * near + which * near + t * kHead + e, x);
+    if (key < a.S) {                                         // (the others have no far queries)
+      const int fb = key / a.far_keys, at = which * far + key % a.far_keys * kHead + e;
+      for (int c = (int)(end / kFar); c * kFar < sp.len; ++c)
+        for (int h = 0; h < share; ++h) {
+          float y[8];
+          load8(a.far_parts + (((int64_t)(sp.slot0 + c) * a.far_first + fb) * a.H + hk * share + h) * 2 * far + at, y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] += y[e];
+          for (int i = 0; i < 8; ++i) x[i] += y[i];
+        }
     }
-    T* to = static_cast<T*>(u < kHead * 16 ? a.dk : a.dv);
-    store8(to + (((int64_t)sp.b * a.s.T + sp.t0 + k0 + t) * a.Hkv + hk) * kHead + 8 * (u % 16), x);
+    T* to = static_cast<T*>(which ? a.dv : a.dk);
+    store8(to + (((int64_t)sp.b * a.s.T + sp.t0 + key) * a.Hkv + hk) * kHead + e, x);
   }
 }
 
@@ -609,27 +659,35 @@ namespace gsa_host {
 namespace {
 
 struct WindowPlan {
-  int64_t slots, far;         // blocks of queries or keys of all sequences; parts of far queries (0: no far queries)
-  int first, W, S;
+  int64_t slots, near, far;   // blocks of queries of all sequences, of keys, of parts of far queries (0: no far queries)
+  int near_keys, near_first, far_keys, far_first, W, S;
   size_t D, near_parts, far_parts;
+  size_t workspace() const { return D + near_parts + far_parts; }
 };
 bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, int sinks, int dtype, WindowPlan& z) {
   z = WindowPlan{};
   if (B < 1 || T < 1 || N < 1 || Hkv < 1 || H < Hkv || H % Hkv || H > 65535 || window < 1 || sinks < 0 || !dtype_size(dtype)) return false;
   z.W = std::min(window, T);
   z.S = std::min(sinks, T);
-  z.slots = packed ? (int64_t)T / gsa::kRows + N : (int64_t)B * ((T + gsa::kRows - 1) / gsa::kRows);
+  auto slots = [&](int n) { return packed ? (int64_t)T / n + N : (int64_t)B * (((int64_t)T + n - 1) / n); };
+  z.slots = slots(gsa::kRows);
   // a grid of 256 threads a block: a launch has less than 2^32 of them
-  if (z.slots > (1 << 23) / H || (int64_t)B * T >= (int64_t)1 << 31) return false;
+  if (slots(32) > (1 << 23) / H || (int64_t)B * T >= (int64_t)1 << 31) return false;
+  // 64 keys a block (two waves share their keys, each takes half of the queries) while 128 leave CUs idle: us forward and
+  // backward, 16 heads on 4, window 1024, by 128 / 64: T = 4096 365 / 271, B = 4 T = 4096 706 / 720, T = 16384 802 / 823;
+  // on 16 heads T = 2048 170 / 151; window 64, T = 8192 210 / 191.  fp32 always 64 (registers): T = 4096, window 256 471 / 458.
+  z.near_keys = dtype == GSA_DTYPE_BF16 && slots(128) * Hkv >= 512 ? 128 : 64;
+  z.far_keys = dtype == GSA_DTYPE_BF16 ? 32 : 64;
+  z.near = slots(z.near_keys);
   if (z.S && z.W < T) {
-    z.first = (z.S + gsa::kRows - 1) / gsa::kRows;
-    z.far = packed ? (int64_t)T / gsa::kFar + N : (int64_t)B * ((T + gsa::kFar - 1) / gsa::kFar);
-    if (z.far * z.first + z.slots > (1 << 23) / H || (int64_t)N * z.first > (1 << 23) / H) return false;
+    z.near_first = (z.S + z.near_keys - 1) / z.near_keys;
+    z.far_first = (z.S + z.far_keys - 1) / z.far_keys;
+    z.far = slots(gsa::kFar) * z.far_first;
+    if (z.far > (1 << 23) / H || (int64_t)N * z.near_first > (1 << 23) / H) return false;
   }
-  const size_t one = (size_t)Hkv * 2 * 128 * 128 * 4;
   z.D = up((size_t)H * B * T * 4);
-  z.near_parts = (size_t)N * z.first * one;
-  z.far_parts = (size_t)z.far * z.first * one;
+  z.near_parts = (size_t)N * z.near_first * Hkv * 2 * z.near_keys * 128 * 4;
+  z.far_parts = (size_t)z.far * H * 2 * z.far_keys * 128 * 4;
   return true;
 }
 
@@ -639,7 +697,7 @@ int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, Win
   if (!dtype_size(x->dtype)) return GSA_ERR_DTYPE;
   if (x->d != 128 || (x->cu_seqlens ? x->B != 1 || (x->cu_bytes != 4 && x->cu_bytes != 8) : x->N != x->B)) return GSA_ERR_SHAPE;
   if (!window_plan(x->B, x->T, x->N, x->cu_seqlens != nullptr, x->H, x->Hkv, x->window, x->sinks, x->dtype, z)) return GSA_ERR_SHAPE;
-  if (backward && x->ws_bytes < z.D + z.near_parts + z.far_parts) return GSA_ERR_SHAPE;
+  if (backward && x->ws_bytes < z.workspace()) return GSA_ERR_SHAPE;
   // a tile's rows are addressed by 32-bit offsets
   for (int64_t st : {x->q_st, x->k_st, x->v_st, backward ? x->do_st : (int64_t)0})
     if (st < 0 || st * 64 * dtype_size(x->dtype) >= (int64_t)1 << 31) return GSA_ERR_SHAPE;
@@ -674,9 +732,10 @@ int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, Win
     a.dv = x->dv;
     char* w = static_cast<char*>(x->ws);
     a.D = reinterpret_cast<float*>(w);
-    a.near = (int)z.slots;
-    a.far = (int)(z.far * z.first);
-    a.first = std::max(z.first, 1);
+    a.near_keys = z.near_keys;
+    a.near_first = z.near_first;
+    a.far_keys = z.far_keys;
+    a.far_first = z.far_first;
     a.near_parts = reinterpret_cast<float*>(w + z.D);
     a.far_parts = reinterpret_cast<float*>(w + z.D + z.near_parts);
   }
@@ -694,7 +753,7 @@ template <typename T> struct WindowLds {
   using L = gsa::Tile<T>;
   static constexpr size_t kTiles = (size_t)gsa::WindowType<T>::kBuffers * 2 * L::kBytes;
   static constexpr size_t kRows = 4 * 32 * 128 * 4;          // a wave's rows on the way out, fp32
-  static constexpr size_t kFwd = kTiles > kRows ? kTiles : kRows, kDkv = kFwd + (size_t)gsa::WindowType<T>::kBuffers * 2 * L::N * 4;
+  static constexpr size_t kFwd = kTiles > kRows ? kTiles : kRows;
 };
 
 template <typename T> int window_forward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
@@ -703,19 +762,27 @@ template <typename T> int window_forward(const gsa::WindowArgs& a, const WindowP
   hipLaunchKernelGGL(gsa::window_fwd_kernel<T>, dim3(z.slots * a.H), dim3(256), lds, s, a);
   return launch_status();
 }
+template <typename T, int kGroups, bool kFarPart> int launch_dkv(const gsa::WindowArgs& a, int64_t blocks, hipStream_t s) {
+  constexpr size_t lds = gsa::WindowGrads<T, kGroups>::kBytes;
+  static_assert(lds <= 160 * 1024);
+  if (const int e = allow_lds<gsa::window_dkv_kernel<T, kGroups, kFarPart>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::window_dkv_kernel<T, kGroups, kFarPart>), dim3(blocks), dim3(256), lds, s, a);
+  return launch_status();
+}
 template <typename T> int window_backward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
-  constexpr size_t lds = WindowLds<T>::kFwd, more = WindowLds<T>::kDkv;
+  constexpr size_t lds = WindowLds<T>::kFwd;
+  constexpr int kFarGroups = sizeof(T) == 2 ? 1 : 2;
   if (const int e = allow_lds<gsa::window_dq_kernel<T>>(lds)) return e;
-  if (const int e = allow_lds<gsa::window_dkv_kernel<T>>(more)) return e;
   hipLaunchKernelGGL(gsa::window_dq_kernel<T>, dim3(z.slots * a.H), dim3(256), lds, s, a);
   if (const int e = launch_status()) return e;
-  hipLaunchKernelGGL(gsa::window_dkv_kernel<T>, dim3((a.near + a.far) * a.Hkv), dim3(256), more, s, a);
-  if (const int e = launch_status()) return e;
-  if (a.far) {
-    hipLaunchKernelGGL(gsa::window_far_kernel<T>, dim3(a.s.N * a.first * a.Hkv, 4), dim3(256), 0, s, a);
-    if (const int e = launch_status()) return e;
-  }
-  return GSA_OK;
+  const int64_t blocks = z.near * a.Hkv;
+  int e;
+  if constexpr (sizeof(T) == 2) e = z.near_keys == 128 ? launch_dkv<T, 4, false>(a, blocks, s) : launch_dkv<T, 2, false>(a, blocks, s);
+  else e = launch_dkv<T, 2, false>(a, blocks, s);
+  if (e || !z.far) return e;
+  if (const int f = launch_dkv<T, kFarGroups, true>(a, z.far * a.H, s)) return f;
+  hipLaunchKernelGGL(gsa::window_far_kernel<T>, dim3(a.s.N * a.near_first * a.Hkv, 4), dim3(256), 0, s, a);
+  return launch_status();
 }
 
 }  // namespace
@@ -723,7 +790,7 @@ template <typename T> int window_backward(const gsa::WindowArgs& a, const Window
 
 extern "C" size_t gsa_window_attn_workspace_bytes(int B, int T, int N, int packed, int H, int Hkv, int window, int sinks, int dtype) {
   gsa_host::WindowPlan z;
-  return gsa_host::window_plan(B, T, N, packed, H, Hkv, window, sinks, dtype, z) ? z.D + z.near_parts + z.far_parts : 0;
+  return gsa_host::window_plan(B, T, N, packed, H, Hkv, window, sinks, dtype, z) ? z.workspace() : 0;
 }
 extern "C" int gsa_window_attn(const gsa_window_args* x, void* stream) {
   gsa::WindowArgs a;
