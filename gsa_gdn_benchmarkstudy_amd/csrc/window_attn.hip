@@ -18,6 +18,8 @@
 // term, as the inputs themselves were rounded), or, for fp32, as three bf16 parts each, as all fp32 operands do (chunks.h).
 #include "chunks.h"
 
+#include <algorithm>
+
 namespace gsa {
 
 struct WindowArgs {
@@ -30,12 +32,11 @@ struct WindowArgs {
   float* D;                   // [H][B * T]
   void *dq, *dk, *dv;
   // dk and dv: blocks of near_keys keys; the far queries of first tokens in parts of kFar queries of a head, far_keys keys a block
-  int near_keys, near_first, far_keys, far_first;            // first: blocks of a sequence's first tokens
+  int near, near_keys, near_first, far_keys, far_first;      // near: blocks; first: blocks of a sequence's first tokens
   float* near_parts;          // [N][near_first][Hkv][2][near_keys][128]
   float* far_parts;           // [slots of far queries][far_first][H][2][far_keys][128]
 };
 
-constexpr int kRows = 128;    // queries of a block, 32 a wave
 constexpr int kFar = 512;     // far queries of a part
 
 template <typename T> struct WindowType;
@@ -229,20 +230,38 @@ __device__ __forceinline__ void window_row(const WindowArgs& a, const T* q, cons
   if (lse && l == 0) *lse = m + __builtin_amdgcn_logf(sum);
 }
 
-template <typename T>
-__global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
-  using L = Tile<T>;
-  constexpr int NP = L::NP, N = L::N, kBuffers = WindowType<T>::kBuffers, kBuffer = 2 * L::kBytes;
+// Tiles of rows for kGroups groups of 32 rows that a block's 4 waves hold: at least 32 for each wave of a group, and kLeast
+template <typename T, int kGroups, int kLeast> struct WindowTiles {
+  static constexpr int kSplit = 4 / kGroups;
+  using L = Tile<T, 32 * (kSplit > kLeast ? kSplit : kLeast)>;
+  static constexpr int NP_ = L::NP, kBuffers = WindowType<T>::kBuffers, kTiles = kBuffers * 2 * L::kBytes;
+};
+// Queries: 32 kGroups of a block.  LDS also holds the rows on the way out and what the waves of a group hand over.
+template <typename T, int kGroups> struct WindowQueries : WindowTiles<T, kGroups, 1> {
+  using Base = WindowTiles<T, kGroups, 1>;
+  static constexpr int kOut = kGroups * 32 * kHead * (int)sizeof(T), kHand = Base::kSplit > 1 ? kGroups * 66 * 256 : 0;
+  static constexpr size_t kBytes = std::max({Base::kTiles, kOut, kHand});
+  // waves of a SIMD: bf16 three blocks a CU (registers and LDS allow it with tiles of 32 keys), with two waves a group two
+  static constexpr int kWaves = Base::NP_ == 1 ? (kGroups == 4 ? 3 : 2) : kGroups == 4 ? 2 : 1;
+};
+
+// A wave of a group: 32 kGroups queries a block, the wave's every kSplit-th 32 keys.
+template <typename T, int kGroups>
+__global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void window_fwd_kernel(WindowArgs a) {
+  using Z = WindowQueries<T, kGroups>;
+  using L = typename Z::L;
+  constexpr int NP = L::NP, N = L::N, kBuffers = Z::kBuffers, kBuffer = 2 * L::kBytes, kQueries = 32 * kGroups, kSplit = Z::kSplit;
+  constexpr int kMine = N / 32 / kSplit;                     // products of 32 keys a tile and wave
   extern __shared__ __align__(16) char lds[];
   const uint32_t base = lds_addr(lds);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), group = wave % kGroups, split = wave / kGroups;
   const int slot = gridDim.x / a.H - 1 - blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hkv);
   int c;
-  const Span sp = slot_of(a.s, slot, kRows, c);
+  const Span sp = slot_of(a.s, slot, kQueries, c);
   if (c < 0) return;
-  const int q0 = c * kRows, r0 = q0 + 32 * wave, row = r0 + (l & 31), rowc = min(row, sp.len - 1);
+  const int q0 = c * kQueries, r0 = q0 + 32 * group, row = r0 + (l & 31), rowc = min(row, sp.len - 1);
   const T *kbase = uniform(row_at<T>(a.k, sp, 0, hk)), *vbase = uniform(row_at<T>(a.v, sp, 0, hk));
-  const KeyTiles<N> tiles(a, q0, kRows, sp.len);
+  const KeyTiles<N> tiles(a, q0, kQueries, sp.len);
   typename L::Loader lk, lv;
   auto load = [&](int t, int buffer) {
     const int j0 = tiles.at(t), left = sp.len - j0;
@@ -277,59 +296,75 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
     wait_loads();
     __syncthreads();
     if (t + 1 < tiles.count) load(t + 1, buffer ^ 1);
-    const int j0 = tiles.at(t), see = r0 < sp.len ? seen<N>(a, r0, j0) : 0;
-    if (!see) continue;
-    floatx16 s[N / 32];
+    if (r0 >= sp.len) continue;
 #pragma unroll
-    for (int n = 0; n < N / 32; ++n) {
-      zero(s[n]);
+    for (int mine = 0; mine < kMine; ++mine) {
+      const int n = split * kMine + mine, j0 = tiles.at(t) + 32 * n, see = seen<32>(a, r0, j0);
+      if (!see) continue;
+      floatx16 s;
+      zero(s);
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) mma32(s[n], rows.read(K, 32 * n, ks), q[ks]);
-    }
-    if (see == 1)
+      for (int ks = 0; ks < 8; ++ks) mma32(s, rows.read(K, 32 * n, ks), q[ks]);
+      if (see == 1) {
+        const int lh = here(l), j = j0 + 8 * (lh >> 5);
 #pragma unroll
-      for (int n = 0; n < N / 32; ++n)
+        for (int r = 0; r < 16; ++r) s[r] = visible(a, row, j + 16 * (r >> 3) + (r & 7)) ? s[r] : -__builtin_inff();
+      }
+      float mx = -__builtin_inff();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = j0 + 32 * n + 16 * (r >> 3) + 8 * (l >> 5) + (r & 7);
-          s[n][r] = visible(a, row, j) ? s[n][r] : -__builtin_inff();
-        }
-    float mx = -__builtin_inff();
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+      mx = max_halves(mx) * a.scale_l2;
+      if (ballot64(mx > limit)) {                            // some row's reference moves
+        const bool bump = mx > limit;
+        const float f = bump ? __builtin_amdgcn_exp2f(m - mx) : 1.f;         // m = -inf: 0
 #pragma unroll
-    for (int n = 0; n < N / 32; ++n)
+        for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
-    mx = max_halves(mx) * a.scale_l2;
-    if (ballot64(mx > limit)) {                              // some row's reference moves
-      const bool bump = mx > limit;
-      const float f = bump ? __builtin_amdgcn_exp2f(m - mx) : 1.f;           // m = -inf: 0
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= f;
-      sum *= f;
-      m = bump ? mx : m;
-      limit = m + kLazy;
-      minus = m == -__builtin_inff() ? 0.f : -m;
-    }
-#pragma unroll
-    for (int n = 0; n < N / 32; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], a.scale_l2, minus));
-        sum += s[n][r];
+          for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+        sum *= f;
+        m = bump ? mx : m;
+        limit = m + kLazy;
+        minus = m == -__builtin_inff() ? 0.f : -m;
       }
 #pragma unroll
-    for (int n = 0; n < N / 32; ++n)
+      for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, minus));
+        sum += s[r];
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const Parts<NP> p = parts_at<NP>(s[n], k);
+        const Parts<NP> p = parts_at<NP>(s, k);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) mma32(o[dt], cols.read(V, 32 * n + 16 * k, dt), p);
       }
+    }
   }
   sum = sum_halves(sum);
   __syncthreads();                                           // the tiles are free
+  if constexpr (kSplit > 1) {
+    // the waves of a group join one after the other: sums, maximum and sum of the softmax through LDS
+    float* hand = reinterpret_cast<float*>(lds) + group * 66 * 64 + l;
+#pragma unroll 1
+    for (int w = 1; w < kSplit; ++w) {
+      if (split == w) {
+#pragma unroll
+        for (int r = 0; r < 64; ++r) hand[64 * r] = o[r >> 4][r & 15];
+        hand[64 * 64] = m;
+        hand[64 * 65] = sum;
+      }
+      __syncthreads();
+      if (split == 0) {
+        const float mw = hand[64 * 64], top = mw > m ? mw : m;
+        const float f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top), fw = mw == top ? 1.f : __builtin_amdgcn_exp2f(mw - top);
+        m = top;
+        sum = sum * f + hand[64 * 65] * fw;
+#pragma unroll
+        for (int r = 0; r < 64; ++r) o[r >> 4][r & 15] = __builtin_fmaf(o[r >> 4][r & 15], f, hand[64 * r] * fw);
+      }
+      __syncthreads();
+    }
+    if (split) return;
+  }
   if (r0 >= sp.len) return;
   const int left = sp.len - r0;
   T* out = static_cast<T*>(a.o) + (((int64_t)sp.b * a.s.T + sp.t0 + r0) * a.H + h) * kHead;
@@ -338,12 +373,7 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(o[dt][r], 0.f, odd);
-  const float f = 1.f / sum;
-#pragma unroll
-  for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[dt][r] *= f;
-  store_rows<T>(o, 1.f, lds + wave * 32 * kHead * sizeof(T), out, (int64_t)a.H * kHead, left, l);
+  store_rows<T>(o, 1.f / sum, lds + group * 32 * kHead * sizeof(T), out, (int64_t)a.H * kHead, left, l);
   float* lse = a.lse ? a.lse + (int64_t)h * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 : nullptr;
   if (lse && row < sp.len && l < 32) lse[row] = m + __builtin_amdgcn_logf(sum);
   // A row with something that is not finite in its tiles: what it does not see may have reached it (0 * NaN), so it is
@@ -358,21 +388,43 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
   }
 }
 
+// The accumulators of the waves that share their rows, summed in their order into the first wave's through LDS.
+template <int kGroups, int kSplit, int kMany>
+__device__ __forceinline__ void join_waves(floatx16 (*const (&x)[kMany])[4], char* lds, int group, int split, int l) {
+  float* hand = reinterpret_cast<float*>(lds) + group * 64 * 64 + l;
+#pragma unroll 1
+  for (int w = 1; w < kSplit; ++w)
+#pragma unroll
+    for (int n = 0; n < kMany; ++n) {
+      floatx16 (&y)[4] = *x[n];
+      if (split == w)
+#pragma unroll
+        for (int r = 0; r < 64; ++r) hand[64 * r] = y[r >> 4][r & 15];
+      __syncthreads();
+      if (split == 0)
+#pragma unroll
+        for (int r = 0; r < 64; ++r) y[r >> 4][r & 15] += hand[64 * r];
+      __syncthreads();
+    }
+}
+
 // dq and D: a block's queries against the tiles of keys, as forwards.
-template <typename T>
-__global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dq_kernel(WindowArgs a) {
-  using L = Tile<T>;
-  constexpr int NP = L::NP, N = L::N, kBuffers = WindowType<T>::kBuffers, kBuffer = 2 * L::kBytes;
+template <typename T, int kGroups>
+__global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_dq_kernel(WindowArgs a) {
+  using Z = WindowQueries<T, kGroups>;
+  using L = typename Z::L;
+  constexpr int NP = L::NP, N = L::N, kBuffers = Z::kBuffers, kBuffer = 2 * L::kBytes, kQueries = 32 * kGroups, kSplit = Z::kSplit;
+  constexpr int kMine = N / 32 / kSplit;
   extern __shared__ __align__(16) char lds[];
   const uint32_t base = lds_addr(lds);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), group = wave % kGroups, split = wave / kGroups;
   const int slot = gridDim.x / a.H - 1 - blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hkv);
   int c;
-  const Span sp = slot_of(a.s, slot, kRows, c);
+  const Span sp = slot_of(a.s, slot, kQueries, c);
   if (c < 0) return;
-  const int q0 = c * kRows, r0 = q0 + 32 * wave, row = r0 + (l & 31), rowc = min(row, sp.len - 1);
+  const int q0 = c * kQueries, r0 = q0 + 32 * group, row = r0 + (l & 31), rowc = min(row, sp.len - 1);
   const T *kbase = uniform(row_at<T>(a.k, sp, 0, hk)), *vbase = uniform(row_at<T>(a.v, sp, 0, hk));
-  const KeyTiles<N> tiles(a, q0, kRows, sp.len);
+  const KeyTiles<N> tiles(a, q0, kQueries, sp.len);
   typename L::Loader lk, lv;
   auto load = [&](int t, int buffer) {
     const int j0 = tiles.at(t), left = sp.len - j0;
@@ -400,7 +452,7 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dq
   }
   const int64_t at = (int64_t)h * a.B * a.s.T + first + rowc;
   const float lse = a.lse[at];
-  if (row < sp.len && l < 32) a.D[at] = D;
+  if (split == 0 && row < sp.len && l < 32) a.D[at] = D;
   floatx16 acc[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) zero(acc[dt]);
@@ -417,10 +469,11 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dq
     wait_loads();
     __syncthreads();
     if (t + 1 < tiles.count) load(t + 1, buffer ^ 1);
-    const int j0 = tiles.at(t), see = r0 < sp.len ? seen<N>(a, r0, j0) : 0;
-    if (!see) continue;
-#pragma unroll
-    for (int n = 0; n < N / 32; ++n) {
+    if (r0 >= sp.len) continue;
+#pragma unroll 1
+    for (int mine = 0; mine < kMine; ++mine) {
+      const int n = split * kMine + mine, j0 = tiles.at(t) + 32 * n, see = seen<32>(a, r0, j0);
+      if (!see) continue;
       floatx16 s, p;
       zero(s);
       zero(p);
@@ -430,12 +483,11 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dq
       for (int ks = 0; ks < 8; ++ks) mma32(p, rows.read(V, 32 * n, ks), d[ks]);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, -lse)) * (p[r] - D);
-      if (see == 1)
+      if (see == 1) {
+        const int lh = here(l), j = j0 + 8 * (lh >> 5);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = j0 + 32 * n + 16 * (r >> 3) + 8 * (l >> 5) + (r & 7);
-          s[r] = visible(a, row, j) ? s[r] : 0.f;
-        }
+        for (int r = 0; r < 16; ++r) s[r] = visible(a, row, j + 16 * (r >> 3) + (r & 7)) ? s[r] : 0.f;
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const Parts<NP> ds = parts_at<NP>(s, k);
@@ -444,39 +496,41 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dq
       }
     }
   }
-  __syncthreads();
+  __syncthreads();                                           // the tiles are free
+  if constexpr (kSplit > 1) {
+    join_waves<kGroups, kSplit, 1>({&acc}, lds, group, split, l);
+    if (split) return;
+  }
   if (r0 >= sp.len) return;
-  store_rows<T>(acc, a.scale, lds + wave * 32 * kHead * sizeof(T), static_cast<T*>(a.dq) + ((first + r0) * a.H + h) * kHead,
+  store_rows<T>(acc, a.scale, lds + group * 32 * kHead * sizeof(T), static_cast<T*>(a.dq) + ((first + r0) * a.H + h) * kHead,
                 (int64_t)a.H * kHead, sp.len - r0, l);
 }
 
-// Tiles of queries for kGroups groups of 32 keys: at least 32 queries for each wave of a group
-template <typename T, int kGroups> struct WindowGrads {
-  static constexpr int kRows32 = 4 / kGroups, kLeast = WindowType<T>::kTile / 32;
-  using L = Tile<T, 32 * (kRows32 > kLeast ? kRows32 : kLeast)>;
-  static constexpr int kBuffers = WindowType<T>::kBuffers, kTiles = kBuffers * 2 * L::kBytes;
-  static constexpr int kOut = kGroups * 32 * kHead * 4;      // rows on the way out, or the waves' sums
-  static constexpr size_t kBytes = (kTiles > kOut ? kTiles : kOut) + kBuffers * 2 * L::N * 4;
+// Keys: 32 kGroups of a block, tiles of queries (far queries: one buffer, so that two blocks share a CU)
+template <typename T, int kGroups, bool kFarPart> struct WindowKeys : WindowTiles<T, kGroups, WindowType<T>::kTile / 32> {
+  using Base = WindowTiles<T, kGroups, WindowType<T>::kTile / 32>;
+  static constexpr int kBuffers = kFarPart ? 1 : Base::kBuffers, kTiles = kBuffers * 2 * Base::L::kBytes;
+  static constexpr int kStats = std::max(kTiles, kGroups * 64 * 256);        // (rows on the way out: as much as the waves' sums)
+  static constexpr size_t kBytes = kStats + kBuffers * 2 * Base::L::N * 4;
 };
 
 // dk and dv of 32 kGroups keys of a key head.  A wave has 32 of them, and of the tiles' queries each 4 / kGroups-th 32.
 // kFarPart: a part of the far queries of first tokens; otherwise the queries near the keys: all that see them, but for those.
 template <typename T, int kGroups, bool kFarPart>
-__global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dkv_kernel(WindowArgs a) {
-  using W = WindowGrads<T, kGroups>;
-  using L = typename W::L;
-  constexpr int NP = L::NP, N = L::N, kBuffers = W::kBuffers, kBuffer = 2 * L::kBytes, kKeys = 32 * kGroups, kSplit = 4 / kGroups;
-  extern __shared__ __align__(16) char lds[];
+__device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int index) {
+  using Z = WindowKeys<T, kGroups, kFarPart>;
+  using L = typename Z::L;
+  constexpr int NP = L::NP, N = L::N, kBuffers = Z::kBuffers, kBuffer = 2 * L::kBytes, kKeys = 32 * kGroups, kSplit = Z::kSplit;
   const uint32_t base = lds_addr(lds);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id(), share = a.H / a.Hkv;
   int unit, hk, h0, heads, c, i0, i1, k0;
   float* parts = nullptr;
   Span sp;
   if constexpr (!kFarPart) {
-    hk = blockIdx.x % a.Hkv;
+    hk = index % a.Hkv;
     h0 = hk * share;
     heads = share;
-    unit = blockIdx.x / a.Hkv;
+    unit = index / a.Hkv;
     sp = slot_of(a.s, unit, kKeys, c);
     if (c < 0) return;
     k0 = c * kKeys;
@@ -485,10 +539,10 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
     i1 = (int)min((int64_t)sp.len, end);
     if (k0 < a.S && end < sp.len) parts = a.near_parts + (((int64_t)sp.n * a.near_first + c) * a.Hkv + hk) * 2 * kKeys * kHead;
   } else {
-    h0 = blockIdx.x % a.H;
+    h0 = index % a.H;
     hk = h0 / share;
     heads = 1;
-    unit = blockIdx.x / a.H;
+    unit = index / a.H;
     const int block = unit % a.far_first;
     unit /= a.far_first;
     sp = slot_of(a.s, unit, kFar, c);
@@ -515,7 +569,8 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
       stat[1] = a.D[at];
     }
   };
-  load(0, 0);
+  constexpr bool kAhead = kBuffers == 2 || NP == 3;          // the next tile's loads run beside this one's products
+  if (kAhead) load(0, 0);
   Parts<NP> k[8], v[8];
   row_operand<T>(k, row_at<T>(a.k, sp, keyc, hk), l);
   row_operand<T>(v, row_at<T>(a.v, sp, keyc, hk), l);
@@ -530,9 +585,10 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
   for (int t = 0; t < count; ++t) {
     const int buffer = kBuffers == 2 ? t & 1 : 0;
     char *Q = lds + buffer * kBuffer, *dO = Q + L::kBytes;
-    float* st = reinterpret_cast<float*>(lds + W::kTiles) + buffer * 2 * N;
+    float* st = reinterpret_cast<float*>(lds + Z::kStats) + buffer * 2 * N;
     if constexpr (kBuffers == 1) {
       if (t) __syncthreads();                                // every wave is through with the last tile
+      if (!kAhead) load(t, 0);
       lq.store(Q, wave, l);
       ld.store(dO, wave, l);
     }
@@ -542,7 +598,7 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
       st[N + tid] = stat[1];
     }
     __syncthreads();
-    if (t + 1 < count) load(t + 1, buffer ^ 1);
+    if (kAhead && t + 1 < count) load(t + 1, buffer ^ 1);
     const int r0 = i0 + t % tiles * N;
     if (j0 >= sp.len) continue;
 #pragma unroll 1                                             // (unrolled, two such products at once do not fit the registers)
@@ -592,22 +648,7 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
   }
   __syncthreads();                                           // the tiles are free
   if constexpr (kSplit > 1) {
-    // the sums of the waves that share their keys, one after the other: a wave's accumulators of dk, then of dv, through LDS
-    float* swap = reinterpret_cast<float*>(lds) + group * 64 * 64 + l;
-#pragma unroll 1
-    for (int w = 1; w < kSplit; ++w)
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        floatx16 (&x)[4] = which ? dv : dk;
-        if (split == w)
-#pragma unroll
-          for (int r = 0; r < 64; ++r) swap[64 * r] = x[r >> 4][r & 15];
-        __syncthreads();
-        if (split == 0)
-#pragma unroll
-          for (int r = 0; r < 64; ++r) x[r >> 4][r & 15] += swap[64 * r];
-        __syncthreads();
-      }
+    join_waves<kGroups, kSplit, 2>({&dk, &dv}, lds, group, split, l);
     if (split) return;
   }
   if (j0 >= sp.len) return;
@@ -622,6 +663,14 @@ __global__ __launch_bounds__(256, WindowType<T>::NP == 1 ? 2 : 1) void window_dk
   const int64_t o = (((int64_t)sp.b * a.s.T + sp.t0 + j0) * a.Hkv + hk) * kHead;
   store_rows<T>(dk, a.scale, own, static_cast<T*>(a.dk) + o, (int64_t)a.Hkv * kHead, left, l);
   store_rows<T>(dv, 1.f, own, static_cast<T*>(a.dv) + o, (int64_t)a.Hkv * kHead, left, l);
+}
+
+// The blocks of keys, then the parts of the far queries (which fill what those leave idle at the end).
+template <typename T, int kGroups, int kFarGroups>
+__global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_dkv_kernel(WindowArgs a) {
+  extern __shared__ __align__(16) char lds[];
+  if ((int)blockIdx.x < a.near) window_dkv<T, kGroups, false>(a, lds, blockIdx.x);
+  else window_dkv<T, kFarGroups, true>(a, lds, blockIdx.x - a.near);
 }
 
 // dk and dv of a sequence's first tokens: the near queries' part and those of the far ones, in their order.
@@ -660,7 +709,7 @@ namespace {
 
 struct WindowPlan {
   int64_t slots, near, far;   // blocks of queries of all sequences, of keys, of parts of far queries (0: no far queries)
-  int near_keys, near_first, far_keys, far_first, W, S;
+  int queries, near_keys, near_first, far_keys, far_first, W, S;             // queries: of a block
   size_t D, near_parts, far_parts;
   size_t workspace() const { return D + near_parts + far_parts; }
 };
@@ -670,7 +719,12 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   z.W = std::min(window, T);
   z.S = std::min(sinks, T);
   auto slots = [&](int n) { return packed ? (int64_t)T / n + N : (int64_t)B * (((int64_t)T + n - 1) / n); };
-  z.slots = slots(gsa::kRows);
+  // 64 queries a block (two waves share their queries, each takes half of the keys) while 128 leave CUs idle: us forward, 16
+  // heads on 4, by 128 / 64 queries: T = 512 18 / 13, T = 1024, window 256 18 / 13, T = 2048 35 / 26, T = 4096, window 1024
+  // 49 / 53, B = 4 160 / 192; 4 heads T = 2000 52 / 30; fp32 B = 2 T = 1537, 4 heads 52 / 39, T = 4096, 16 heads 76 / 130.
+  // (32 queries, four waves each a quarter of the keys: 15 at T = 512, 27 at T = 2000, worse at all others.)
+  z.queries = slots(128) * H <= 256 ? 64 : 128;
+  z.slots = slots(z.queries);
   // a grid of 256 threads a block: a launch has less than 2^32 of them
   if (slots(32) > (1 << 23) / H || (int64_t)B * T >= (int64_t)1 << 31) return false;
   // 64 keys a block (two waves share their keys, each takes half of the queries) while 128 leave CUs idle: us forward and
@@ -732,6 +786,7 @@ int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, Win
     a.dv = x->dv;
     char* w = static_cast<char*>(x->ws);
     a.D = reinterpret_cast<float*>(w);
+    a.near = (int)(z.near * x->Hkv);
     a.near_keys = z.near_keys;
     a.near_first = z.near_first;
     a.far_keys = z.far_keys;
@@ -749,39 +804,37 @@ int window_outside(const gsa::WindowArgs& a, const gsa_window_args* x, bool back
   hipLaunchKernelGGL(gsa::outside_kernel, dim3(256), dim3(256), 0, s, o);
   return launch_status();
 }
-template <typename T> struct WindowLds {
-  using L = gsa::Tile<T>;
-  static constexpr size_t kTiles = (size_t)gsa::WindowType<T>::kBuffers * 2 * L::kBytes;
-  static constexpr size_t kRows = 4 * 32 * 128 * 4;          // a wave's rows on the way out, fp32
-  static constexpr size_t kFwd = kTiles > kRows ? kTiles : kRows;
-};
-
-template <typename T> int window_forward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
-  constexpr size_t lds = WindowLds<T>::kFwd;
-  if (const int e = allow_lds<gsa::window_fwd_kernel<T>>(lds)) return e;
-  hipLaunchKernelGGL(gsa::window_fwd_kernel<T>, dim3(z.slots * a.H), dim3(256), lds, s, a);
+template <typename T, int kGroups> int launch_fwd(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+  constexpr size_t lds = gsa::WindowQueries<T, kGroups>::kBytes;
+  static_assert(lds <= 160 * 1024);
+  if (const int e = allow_lds<gsa::window_fwd_kernel<T, kGroups>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::window_fwd_kernel<T, kGroups>), dim3(z.slots * a.H), dim3(256), lds, s, a);
   return launch_status();
 }
-template <typename T, int kGroups, bool kFarPart> int launch_dkv(const gsa::WindowArgs& a, int64_t blocks, hipStream_t s) {
-  constexpr size_t lds = gsa::WindowGrads<T, kGroups>::kBytes;
-  static_assert(lds <= 160 * 1024);
-  if (const int e = allow_lds<gsa::window_dkv_kernel<T, kGroups, kFarPart>>(lds)) return e;
-  hipLaunchKernelGGL((gsa::window_dkv_kernel<T, kGroups, kFarPart>), dim3(blocks), dim3(256), lds, s, a);
+template <typename T, int kGroups> int launch_dq(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+  constexpr size_t lds = gsa::WindowQueries<T, kGroups>::kBytes;
+  if (const int e = allow_lds<gsa::window_dq_kernel<T, kGroups>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::window_dq_kernel<T, kGroups>), dim3(z.slots * a.H), dim3(256), lds, s, a);
   return launch_status();
+}
+template <typename T, int kGroups> int launch_dkv(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+  constexpr int kFarGroups = sizeof(T) == 2 ? 1 : 2;
+  constexpr size_t lds = std::max(gsa::WindowKeys<T, kGroups, false>::kBytes, gsa::WindowKeys<T, kFarGroups, true>::kBytes);
+  static_assert(lds <= 160 * 1024);
+  if (const int e = allow_lds<gsa::window_dkv_kernel<T, kGroups, kFarGroups>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::window_dkv_kernel<T, kGroups, kFarGroups>), dim3(a.near + z.far * a.H), dim3(256), lds, s, a);
+  return launch_status();
+}
+template <typename T> int window_forward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+  return z.queries == 64 ? launch_fwd<T, 2>(a, z, s) : launch_fwd<T, 4>(a, z, s);
 }
 template <typename T> int window_backward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
-  constexpr size_t lds = WindowLds<T>::kFwd;
-  constexpr int kFarGroups = sizeof(T) == 2 ? 1 : 2;
-  if (const int e = allow_lds<gsa::window_dq_kernel<T>>(lds)) return e;
-  hipLaunchKernelGGL(gsa::window_dq_kernel<T>, dim3(z.slots * a.H), dim3(256), lds, s, a);
-  if (const int e = launch_status()) return e;
-  const int64_t blocks = z.near * a.Hkv;
-  int e;
-  if constexpr (sizeof(T) == 2) e = z.near_keys == 128 ? launch_dkv<T, 4, false>(a, blocks, s) : launch_dkv<T, 2, false>(a, blocks, s);
-  else e = launch_dkv<T, 2, false>(a, blocks, s);
+  int e = z.queries == 64 ? launch_dq<T, 2>(a, z, s) : launch_dq<T, 4>(a, z, s);
+  if (e) return e;
+  if constexpr (sizeof(T) == 2) e = z.near_keys == 128 ? launch_dkv<T, 4>(a, z, s) : launch_dkv<T, 2>(a, z, s);
+  else e = launch_dkv<T, 2>(a, z, s);
   if (e || !z.far) return e;
-  if (const int f = launch_dkv<T, kFarGroups, true>(a, z.far * a.H, s)) return f;
-  hipLaunchKernelGGL(gsa::window_far_kernel<T>, dim3(a.s.N * a.near_first * a.Hkv, 4), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(gsa::window_far_kernel<T>, dim3(a.s.N * a.near_first * a.Hkv, a.near_keys / 8), dim3(256), 0, s, a);
   return launch_status();
 }
 
