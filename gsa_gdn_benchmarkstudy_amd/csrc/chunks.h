@@ -232,7 +232,12 @@ __device__ __forceinline__ int here(int x) {
   asm volatile("" : "+v"(x));
   return x;
 }
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// All loads have landed, the direct ones to LDS too, and the compiler knows it: waits of its own for registers loaded before a
+// loop would stand inside it, where they wait for the next tile's direct loads, which it does not count.
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+  asm volatile("" ::: "memory");
+}
 
 // `units` KiB from src (16-byte aligned) to LDS, by W waves.
 template <int W> __device__ __forceinline__ void fetch(const void* src, uint32_t lds, int units, int wave, int l) {

@@ -11,7 +11,7 @@
 // softmax state lives in them and P enters the second product from the registers in which it was computed.
 // dq (window_dq_kernel) goes the same way; dk and dv (window_dkv_kernel): a block takes 128 keys of a key head and walks the
 // queries of all heads on it that see them, so that no two blocks write one gradient: no atomics, the same bits on every
-// run.  The first tokens are seen by all later queries; those past the window's are cut into parts of kFar
+// run.  The first tokens are seen by all later queries; those past the window's are cut into parts of
 // queries, whose sums are added in their order (window_far_kernel).
 //
 // Precision: sums, softmax statistics and D are fp32.  P and dS enter the second products in the inputs' type: bf16 (2^-9 of a
@@ -31,13 +31,14 @@ struct WindowArgs {
   float* lse;                 // [H][B * T]: L (forward: nullable)
   float* D;                   // [H][B * T]
   void *dq, *dk, *dv;
-  // dk and dv: blocks of near_keys keys; the far queries of first tokens in parts of kFar queries of a head, far_keys keys a block
-  int near, near_keys, near_first, far_keys, far_first;      // near: blocks; first: blocks of a sequence's first tokens
+  // dk and dv: blocks of near_keys keys; the far queries of first tokens in parts of far_rows queries of a head, far_keys keys a block
+  int near_keys, near_first, far_keys, far_first, far_rows;            // first: blocks of a sequence's first tokens
   float* near_parts;          // [N][near_first][Hkv][2][near_keys][128]
   float* far_parts;           // [slots of far queries][far_first][H][2][far_keys][128]
 };
 
-constexpr int kFar = 512;     // far queries of a part
+
+template <int N> struct Number { static constexpr int value = N; };
 
 template <typename T> struct WindowType;
 template <> struct WindowType<uint16_t> { static constexpr int NP = 1, kTile = 64, kBuffers = 2; };
@@ -98,13 +99,25 @@ template <typename T, int kN = WindowType<T>::kTile> struct Tile {
   struct Loader {
     static constexpr int kUnits = N * 16 / 256;              // a thread's units
     floatx4 x[NP == 3 ? 2 * kUnits : 1];
+    uint32_t lane;                                           // bf16: a lane's place in the first 16 rows, in bytes
+    __device__ Loader(int64_t stride, int wave, int l) {
+      const int t = 4 * wave + (l >> 4);
+      lane = ((uint32_t)t * (uint32_t)stride + 8 * ((l & 15) ^ swizzle(t))) * 2u;
+    }
     __device__ void load(const T* p, int64_t stride, int left, uint32_t lds, int wave, int l) {
       p = uniform(p);
       if constexpr (NP == 1) {
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + wave * 1024);
+        if (left >= N) {
 #pragma unroll
-        for (int j = 0; j < kUnits; ++j) {
-          const int t = 16 * j + 4 * wave + (l >> 4), u = (l & 15) ^ swizzle(t);
-          load_lds16(p, ((uint32_t)min(t, left - 1) * (uint32_t)stride + 8 * u) * 2u, __builtin_amdgcn_readfirstlane(lds + (4 * j + wave) * 1024));
+          for (int j = 0; j < kUnits; ++j) load_lds16(p + 16 * j * stride, lane, to + j * 4096);
+        } else {
+          const int lh = here(l);
+#pragma unroll
+          for (int j = 0; j < kUnits; ++j) {
+            const int t = 16 * j + 4 * wave + (lh >> 4), u = (lh & 15) ^ swizzle(t);
+            load_lds16(p, ((uint32_t)min(t, left - 1) * (uint32_t)stride + 8 * u) * 2u, to + j * 4096);
+          }
         }
       } else {
 #pragma unroll
@@ -262,7 +275,7 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
   const int q0 = c * kQueries, r0 = q0 + 32 * group, row = r0 + (l & 31), rowc = min(row, sp.len - 1);
   const T *kbase = uniform(row_at<T>(a.k, sp, 0, hk)), *vbase = uniform(row_at<T>(a.v, sp, 0, hk));
   const KeyTiles<N> tiles(a, q0, kQueries, sp.len);
-  typename L::Loader lk, lv;
+  typename L::Loader lk(a.k.st, wave, l), lv(a.v.st, wave, l);
   auto load = [&](int t, int buffer) {
     const int j0 = tiles.at(t), left = sp.len - j0;
     lk.load(kbase + j0 * a.k.st, a.k.st, left, base + buffer * kBuffer, wave, l);
@@ -285,8 +298,8 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
   // kLazy (the sums then stay below 2^8 times what they are, far from fp32's range)
   constexpr float kLazy = 8.f;
   float m = -__builtin_inff(), limit = m, minus = 0.f, sum = 0.f;
-  for (int t = 0; t < tiles.count; ++t) {
-    const int buffer = kBuffers == 2 ? t & 1 : 0;
+  auto step = [&](int t, auto which) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
+    constexpr int buffer = kBuffers == 2 ? decltype(which)::value : 0;
     char *K = lds + buffer * kBuffer, *V = K + L::kBytes;
     if constexpr (NP == 3) {
       if (t) __syncthreads();                                // every wave is through with the last tile
@@ -296,7 +309,7 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
     wait_loads();
     __syncthreads();
     if (t + 1 < tiles.count) load(t + 1, buffer ^ 1);
-    if (r0 >= sp.len) continue;
+    if (r0 >= sp.len) return;
 #pragma unroll
     for (int mine = 0; mine < kMine; ++mine) {
       const int n = split * kMine + mine, j0 = tiles.at(t) + 32 * n, see = seen<32>(a, r0, j0);
@@ -338,6 +351,10 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
         for (int dt = 0; dt < 4; ++dt) mma32(o[dt], cols.read(V, 32 * n + 16 * k, dt), p);
       }
     }
+  };
+  for (int t = 0; t < tiles.count; t += 2) {
+    step(t, Number<0>{});
+    if (t + 1 < tiles.count) step(t + 1, Number<1>{});
   }
   sum = sum_halves(sum);
   __syncthreads();                                           // the tiles are free
@@ -425,7 +442,7 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
   const int q0 = c * kQueries, r0 = q0 + 32 * group, row = r0 + (l & 31), rowc = min(row, sp.len - 1);
   const T *kbase = uniform(row_at<T>(a.k, sp, 0, hk)), *vbase = uniform(row_at<T>(a.v, sp, 0, hk));
   const KeyTiles<N> tiles(a, q0, kQueries, sp.len);
-  typename L::Loader lk, lv;
+  typename L::Loader lk(a.k.st, wave, l), lv(a.v.st, wave, l);
   auto load = [&](int t, int buffer) {
     const int j0 = tiles.at(t), left = sp.len - j0;
     lk.load(kbase + j0 * a.k.st, a.k.st, left, base + buffer * kBuffer, wave, l);
@@ -458,8 +475,8 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
   for (int dt = 0; dt < 4; ++dt) zero(acc[dt]);
   const typename L::RowReader rows(l);
   const typename L::ColReader cols(l);
-  for (int t = 0; t < tiles.count; ++t) {
-    const int buffer = kBuffers == 2 ? t & 1 : 0;
+  auto step = [&](int t, auto which) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
+    constexpr int buffer = kBuffers == 2 ? decltype(which)::value : 0;
     char *K = lds + buffer * kBuffer, *V = K + L::kBytes;
     if constexpr (NP == 3) {
       if (t) __syncthreads();
@@ -469,7 +486,7 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
     wait_loads();
     __syncthreads();
     if (t + 1 < tiles.count) load(t + 1, buffer ^ 1);
-    if (r0 >= sp.len) continue;
+    if (r0 >= sp.len) return;
 #pragma unroll 1
     for (int mine = 0; mine < kMine; ++mine) {
       const int n = split * kMine + mine, j0 = tiles.at(t) + 32 * n, see = seen<32>(a, r0, j0);
@@ -495,6 +512,10 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
         for (int dt = 0; dt < 4; ++dt) mma32(acc[dt], cols.read(K, 32 * n + 16 * k, dt), ds);
       }
     }
+  };
+  for (int t = 0; t < tiles.count; t += 2) {
+    step(t, Number<0>{});
+    if (t + 1 < tiles.count) step(t + 1, Number<1>{});
   }
   __syncthreads();                                           // the tiles are free
   if constexpr (kSplit > 1) {
@@ -511,7 +532,7 @@ template <typename T, int kGroups, bool kFarPart> struct WindowKeys : WindowTile
   using Base = WindowTiles<T, kGroups, WindowType<T>::kTile / 32>;
   static constexpr int kBuffers = kFarPart ? 1 : Base::kBuffers, kTiles = kBuffers * 2 * Base::L::kBytes;
   static constexpr int kStats = std::max(kTiles, kGroups * 64 * 256);        // (rows on the way out: as much as the waves' sums)
-  static constexpr size_t kBytes = kStats + kBuffers * 2 * Base::L::N * 4;
+  static constexpr size_t kBytes = kStats + 2 * 2 * std::max(64, Base::L::N) * 4;
 };
 
 // dk and dv of 32 kGroups keys of a key head.  A wave has 32 of them, and of the tiles' queries each 4 / kGroups-th 32.
@@ -522,7 +543,7 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
   using L = typename Z::L;
   constexpr int NP = L::NP, N = L::N, kBuffers = Z::kBuffers, kBuffer = 2 * L::kBytes, kKeys = 32 * kGroups, kSplit = Z::kSplit;
   const uint32_t base = lds_addr(lds);
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id(), share = a.H / a.Hkv;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), share = a.H / a.Hkv;
   int unit, hk, h0, heads, c, i0, i1, k0;
   float* parts = nullptr;
   Span sp;
@@ -545,28 +566,28 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
     unit = index / a.H;
     const int block = unit % a.far_first;
     unit /= a.far_first;
-    sp = slot_of(a.s, unit, kFar, c);
+    sp = slot_of(a.s, unit, a.far_rows, c);
     k0 = block * kKeys;
     if (c < 0 || k0 >= sp.len) return;
     const int64_t end = (int64_t)k0 / a.near_keys * a.near_keys + a.near_keys - 1 + a.W;
-    i0 = (int)max((int64_t)c * kFar, min((int64_t)sp.len, end));
-    i1 = min(sp.len, (c + 1) * kFar);
+    i0 = (int)max((int64_t)c * a.far_rows, min((int64_t)sp.len, end));
+    i1 = min(sp.len, (c + 1) * a.far_rows);
     if (i0 >= i1) return;
     parts = a.far_parts + (((int64_t)unit * a.far_first + block) * a.H + h0) * 2 * kKeys * kHead;
   }
   const int group = wave % kGroups, split = wave / kGroups;
   const int j0 = k0 + 32 * group, key = j0 + (l & 31), keyc = min(key, sp.len - 1);
   const int tiles = (i1 - i0 + N - 1) / N, count = tiles * heads;
-  typename L::Loader lq, ld;
-  float stat[2];                                             // of thread tid < N: L and D of a query
+  typename L::Loader lq(a.q.st, wave, l), ld(a.dout.st, wave, l);
+  constexpr int kStatRow = N < 64 ? 64 : N;                  // L of a tile's queries, then D, each a wave's 64 or two
   auto load = [&](int t, int buffer) {
     const int h = h0 + t / tiles, r = i0 + t % tiles * N, left = min(sp.len, i1) - r;
     lq.load(row_at<T>(a.q, sp, r, h), a.q.st, left, base + buffer * kBuffer, wave, l);
     ld.load(row_at<T>(a.dout, sp, r, h), a.dout.st, left, base + buffer * kBuffer + L::kBytes, wave, l);
-    if (tid < N) {
-      const int64_t at = (int64_t)h * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 + r + min(tid, left - 1);
-      stat[0] = a.lse[at];
-      stat[1] = a.D[at];
+    if (wave < kStatRow / 32) {
+      const int which = wave / (kStatRow / 64), t0 = 64 * (wave % (kStatRow / 64));
+      const float* p = uniform((which ? a.D : a.lse) + (int64_t)h * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 + r);
+      load_lds4(p, 4u * min(t0 + l, left - 1), __builtin_amdgcn_readfirstlane(base + Z::kStats + 4 * (((t & 1) * 2 + which) * kStatRow + t0)));
     }
   };
   constexpr bool kAhead = kBuffers == 2 || NP == 3;          // the next tile's loads run beside this one's products
@@ -585,7 +606,7 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
   for (int t = 0; t < count; ++t) {
     const int buffer = kBuffers == 2 ? t & 1 : 0;
     char *Q = lds + buffer * kBuffer, *dO = Q + L::kBytes;
-    float* st = reinterpret_cast<float*>(lds + Z::kStats) + buffer * 2 * N;
+    const float* st = reinterpret_cast<const float*>(lds + Z::kStats) + (t & 1) * 2 * kStatRow;
     if constexpr (kBuffers == 1) {
       if (t) __syncthreads();                                // every wave is through with the last tile
       if (!kAhead) load(t, 0);
@@ -593,10 +614,6 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
       ld.store(dO, wave, l);
     }
     wait_loads();
-    if (tid < N) {
-      st[tid] = stat[0];
-      st[N + tid] = stat[1];
-    }
     __syncthreads();
     if (kAhead && t + 1 < count) load(t + 1, buffer ^ 1);
     const int r0 = i0 + t % tiles * N;
@@ -621,7 +638,7 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
         load8(stats + 16 * x, y);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[8 * x + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * x + e], a.scale_l2, -y[e]));
-        load8(stats + N + 16 * x, y);
+        load8(stats + kStatRow + 16 * x, y);
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[8 * x + e] = s[8 * x + e] * (p[8 * x + e] - y[e]);
       }
@@ -665,19 +682,18 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
   store_rows<T>(dv, 1.f, own, static_cast<T*>(a.dv) + o, (int64_t)a.Hkv * kHead, left, l);
 }
 
-// The blocks of keys, then the parts of the far queries (which fill what those leave idle at the end).
-template <typename T, int kGroups, int kFarGroups>
+// (One kernel for both kinds of blocks would spill registers, and what reads those back waits for the tiles on their way.)
+template <typename T, int kGroups, bool kFarPart>
 __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_dkv_kernel(WindowArgs a) {
   extern __shared__ __align__(16) char lds[];
-  if ((int)blockIdx.x < a.near) window_dkv<T, kGroups, false>(a, lds, blockIdx.x);
-  else window_dkv<T, kFarGroups, true>(a, lds, blockIdx.x - a.near);
+  window_dkv<T, kGroups, kFarPart>(a, lds, blockIdx.x);
 }
 
 // dk and dv of a sequence's first tokens: the near queries' part and those of the far ones, in their order.
 template <typename T>
 __global__ __launch_bounds__(256) void window_far_kernel(WindowArgs a) {
   const int hk = blockIdx.x % a.Hkv, block = blockIdx.x / a.Hkv % a.near_first, n = blockIdx.x / a.Hkv / a.near_first, share = a.H / a.Hkv;
-  const Span sp = span_of(a.s, n, kFar);
+  const Span sp = span_of(a.s, n, a.far_rows);
   const int k0 = block * a.near_keys;
   const int64_t end = (int64_t)k0 + a.near_keys - 1 + a.W;
   if (k0 >= sp.len || end >= sp.len) return;                 // no far queries: written as they were
@@ -689,7 +705,7 @@ __global__ __launch_bounds__(256) void window_far_kernel(WindowArgs a) {
     load8(a.near_parts + (((int64_t)n * a.near_first + block) * a.Hkv + hk) * 2 * near + which * near + t * kHead + e, x);
     if (key < a.S) {                                         // (the others have no far queries)
       const int fb = key / a.far_keys, at = which * far + key % a.far_keys * kHead + e;
-      for (int c = (int)(end / kFar); c * kFar < sp.len; ++c)
+      for (int c = (int)(end / a.far_rows); c * a.far_rows < sp.len; ++c)
         for (int h = 0; h < share; ++h) {
           float y[8];
           load8(a.far_parts + (((int64_t)(sp.slot0 + c) * a.far_first + fb) * a.H + hk * share + h) * 2 * far + at, y);
@@ -709,7 +725,7 @@ namespace {
 
 struct WindowPlan {
   int64_t slots, near, far;   // blocks of queries of all sequences, of keys, of parts of far queries (0: no far queries)
-  int queries, near_keys, near_first, far_keys, far_first, W, S;             // queries: of a block
+  int queries, near_keys, near_first, far_keys, far_first, far_rows, W, S;   // queries: of a block
   size_t D, near_parts, far_parts;
   size_t workspace() const { return D + near_parts + far_parts; }
 };
@@ -736,7 +752,9 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   if (z.S && z.W < T) {
     z.near_first = (z.S + z.near_keys - 1) / z.near_keys;
     z.far_first = (z.S + z.far_keys - 1) / z.far_keys;
-    z.far = slots(gsa::kFar) * z.far_first;
+    // 512 far queries a part, 128 where that leaves CUs idle
+    z.far_rows = slots(512) * z.far_first * H >= 256 ? 512 : 128;
+    z.far = slots(z.far_rows) * z.far_first;
     if (z.far > (1 << 23) / H || (int64_t)N * z.near_first > (1 << 23) / H) return false;
   }
   z.D = up((size_t)H * B * T * 4);
@@ -786,11 +804,11 @@ int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, Win
     a.dv = x->dv;
     char* w = static_cast<char*>(x->ws);
     a.D = reinterpret_cast<float*>(w);
-    a.near = (int)(z.near * x->Hkv);
     a.near_keys = z.near_keys;
     a.near_first = z.near_first;
     a.far_keys = z.far_keys;
     a.far_first = z.far_first;
+    a.far_rows = z.far_rows;
     a.near_parts = reinterpret_cast<float*>(w + z.D);
     a.far_parts = reinterpret_cast<float*>(w + z.D + z.near_parts);
   }
@@ -817,12 +835,11 @@ template <typename T, int kGroups> int launch_dq(const gsa::WindowArgs& a, const
   hipLaunchKernelGGL((gsa::window_dq_kernel<T, kGroups>), dim3(z.slots * a.H), dim3(256), lds, s, a);
   return launch_status();
 }
-template <typename T, int kGroups> int launch_dkv(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
-  constexpr int kFarGroups = sizeof(T) == 2 ? 1 : 2;
-  constexpr size_t lds = std::max(gsa::WindowKeys<T, kGroups, false>::kBytes, gsa::WindowKeys<T, kFarGroups, true>::kBytes);
+template <typename T, int kGroups, bool kFarPart> int launch_dkv(const gsa::WindowArgs& a, int64_t blocks, hipStream_t s) {
+  constexpr size_t lds = gsa::WindowKeys<T, kGroups, kFarPart>::kBytes;
   static_assert(lds <= 160 * 1024);
-  if (const int e = allow_lds<gsa::window_dkv_kernel<T, kGroups, kFarGroups>>(lds)) return e;
-  hipLaunchKernelGGL((gsa::window_dkv_kernel<T, kGroups, kFarGroups>), dim3(a.near + z.far * a.H), dim3(256), lds, s, a);
+  if (const int e = allow_lds<gsa::window_dkv_kernel<T, kGroups, kFarPart>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::window_dkv_kernel<T, kGroups, kFarPart>), dim3(blocks), dim3(256), lds, s, a);
   return launch_status();
 }
 template <typename T> int window_forward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
@@ -831,9 +848,11 @@ template <typename T> int window_forward(const gsa::WindowArgs& a, const WindowP
 template <typename T> int window_backward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
   int e = z.queries == 64 ? launch_dq<T, 2>(a, z, s) : launch_dq<T, 4>(a, z, s);
   if (e) return e;
-  if constexpr (sizeof(T) == 2) e = z.near_keys == 128 ? launch_dkv<T, 4>(a, z, s) : launch_dkv<T, 2>(a, z, s);
-  else e = launch_dkv<T, 2>(a, z, s);
+  const int64_t blocks = z.near * a.Hkv;
+  if constexpr (sizeof(T) == 2) e = z.near_keys == 128 ? launch_dkv<T, 4, false>(a, blocks, s) : launch_dkv<T, 2, false>(a, blocks, s);
+  else e = launch_dkv<T, 2, false>(a, blocks, s);
   if (e || !z.far) return e;
+  if ((e = launch_dkv<T, sizeof(T) == 2 ? 1 : 2, true>(a, z.far * a.H, s))) return e;
   hipLaunchKernelGGL(gsa::window_far_kernel<T>, dim3(a.s.N * a.near_first * a.Hkv, a.near_keys / 8), dim3(256), 0, s, a);
   return launch_status();
 }
