@@ -287,6 +287,10 @@ __device__ __forceinline__ void load_lds16(const void* base, uint32_t voff, uint
 __device__ __forceinline__ void load_lds4(const void* base, uint32_t voff, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
 }
+// The same of 16 bytes from an address of each lane's own.
+__device__ __forceinline__ void load_lds16_at(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // s_waitcnt immediate (gfx9 encoding): vmcnt(0), expcnt and lgkmcnt not waited

@@ -7,10 +7,9 @@
 // window_write_kernel stores keys and values (those that no later token of the call overwrites).  window_step_kernel:
 // one token of each row of a batch against its visible keys,
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c q . k_j - m)
-// Bound by HBM: each key and value is read once, for all query heads on it; 2 flops a byte and query head.  16 lanes take
-// a key, each 8 elements in fp32 (a wave: 4 keys), and keep their own running maximum, sum and output; these are
-// joined within the wave, then within the block.  Where rows times key heads are few, the keys of a row are split over
-// blocks: each leaves its part in the workspace and counts itself, the last one to arrive joins the parts in their order.
+// Bound by HBM: each key and value is read once, for all query heads on it (16 at most at a time).  Each wave has its own
+// running maximum, sum and output, joined within the block.  Where rows times key heads are few, the keys of a row are split
+// over blocks: each leaves its part in the workspace and counts itself, the last one to arrive joins the parts in their order.
 #include "chunks.h"
 
 namespace gsa {
@@ -76,37 +75,130 @@ struct WindowStepArgs {
 };
 constexpr int kStepPart = kHead + 2;                         // o, m, l
 
-// kHeads query heads of a key head at a time
+// The visible keys of a row's token in order, e = 0 .. count - 1: tokens 0 .. first - 1, then those of the window.
+struct Visible {
+  int first, count, turn, S, ring;                           // turn: the ring's row of the window's first token
+  __device__ Visible(const Places& x, int64_t p, int W) : S(x.S), ring(x.ring) {
+    first = (int)(p + 1 < S ? p + 1 : S);
+    const int64_t from = p - W + 1 > S ? p - W + 1 : S;
+    count = first + (p >= from ? (int)(p - from + 1) : 0);
+    turn = p >= from ? (int)((from - S) % ring) : 0;
+  }
+  __device__ int row(int e) const {
+    const int r = turn + e - first;
+    return e < first ? e : S + (r >= ring ? r - ring : r);
+  }
+};
+
+// No score above -infinity: NaN, as 0 / 0 (cut3 leaves more than 0 above the line).
+__device__ __forceinline__ float quotient(float y, float x) { return x == 0.f ? __builtin_nanf("") : y / x; }
+
+// What a block's four waves hold of `heads` heads (part: o, m, l of each), joined: the outputs where the block has all of the
+// row's keys, else the block's part.
 template <typename T, int kHeads>
-__global__ __launch_bounds__(256) void window_step_kernel(WindowStepArgs a) {
+__device__ __forceinline__ void join_block(float (*part)[kHeads][kStepPart], int heads, bool whole, T* out, float* mine) {
+  for (int u = threadIdx.x; u < heads * kHead; u += 256) {
+    const int h = u / kHead, d = u % kHead;
+    float top = part[0][h][kHead];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, part[w][h][kHead]);
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float mw = part[w][h][kHead], f = mw == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(mw - top);
+      x = __builtin_fmaf(part[w][h][kHead + 1], f, x);
+      y = __builtin_fmaf(part[w][h][d], f, y);
+    }
+    if (whole) {
+      out[u] = from_f32<T>(quotient(y, x));
+    } else {
+      float* to = mine + h * kStepPart;
+      part_store(to + d, y);
+      if (d == 0) {
+        part_store(to + kHead, top);
+        part_store(to + kHead + 1, x);
+      }
+    }
+  }
+}
+// The parts of a row's blocks, by the last one to arrive, in their order.  Several loads are on their way at once.
+template <typename T>
+__device__ __forceinline__ void join_row(const WindowStepArgs& a, int n, int hk, int parts, int share, T* out, float* scratch) {
+  constexpr int kSome = 64;
+  float *tops = scratch, *sums = scratch + kSome;            // (the waves' parts have been read)
+  uint32_t& arrived = *reinterpret_cast<uint32_t*>(scratch + 2 * kSome);
+  const int tid = threadIdx.x, wave = tid >> 6, l = lane_id();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0)
+    arrived = __hip_atomic_fetch_add(a.counters + (int64_t)n * a.Hkv + hk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived != (uint32_t)(parts - 1)) return;
+  const float* const all = a.parts + ((int64_t)n * a.Hkv + hk) * a.splits * share * kStepPart;
+  const int64_t step = (int64_t)share * kStepPart;
+  for (int h0 = 0; h0 < share; h0 += kSome) {
+    const int heads = min(kSome, share - h0);
+    if (h0) __syncthreads();
+    for (int h = wave; h < heads; h += 4) {                  // a wave a head: the maximum and the sum over its parts
+      const float* at = all + (h0 + h) * kStepPart + kHead;
+      float top = -__builtin_inff(), x = 0.f;
+      for (int s = l; s < parts; s += 64) top = fmaxf(top, part_load(at + s * step));
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+      for (int s = l; s < parts; s += 64) {
+        const float ms = part_load(at + s * step), f = ms == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ms - top);
+        x = __builtin_fmaf(part_load(at + s * step + 1), f, x);
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+      if (l == 0) {
+        tops[h] = top;
+        sums[h] = x;
+      }
+    }
+    __syncthreads();
+    for (int u = tid; u < heads * kHead; u += 256) {
+      const int h = u / kHead;
+      const float *at = all + (h0 + h) * kStepPart, top = tops[h];
+      float y = 0.f;
+      for (int s = 0; s < parts; s += 8) {
+        float m[8], v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float* ps = at + min(s + i, parts - 1) * step;
+          m[i] = part_load(ps + kHead);
+          v[i] = part_load(ps + u % kHead);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (s + i < parts) y = __builtin_fmaf(v[i], m[i] == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m[i] - top), y);
+      }
+      out[h0 * kHead + u] = from_f32<T>(quotient(y, sums[h]));
+    }
+  }
+}
+
+// fp32: 16 lanes take a key, each 8 elements (a wave: 4 keys), and keep their own running maximum, sum and output.
+// kHeads query heads of a key head at a time.
+template <int kHeads>
+__global__ __launch_bounds__(256) void window_step_f32_kernel(WindowStepArgs a) {
   constexpr int kKeys = 4;                                   // of 16 lanes on their way at once
   __shared__ float part[4][kHeads][kStepPart];
-  __shared__ uint32_t arrived;
   const int tid = threadIdx.x, wave = tid >> 6, l = lane_id(), li = l & 15, group = tid >> 4;
   const int split = blockIdx.x, hk = blockIdx.y, n = blockIdx.z, share = a.H / a.Hkv;
   const int64_t slot = a.places.slot(n), p = a.places.position(n);
-  T* out = static_cast<T*>(a.o) + ((int64_t)n * a.H + hk * share) * kHead;
+  float* out = static_cast<float*>(a.o) + ((int64_t)n * a.H + hk * share) * kHead;
   if (slot < 0 || p < 0) {                                   // a row of padding
     if (split == 0)
-      for (int i = tid; i < share * kHead; i += 256) out[i] = (T)0;
+      for (int i = tid; i < share * kHead; i += 256) out[i] = 0.f;
     return;
   }
-  // visible keys in order: tokens 0 .. first - 1, then from .. p
-  const int S = a.places.S, ring = a.places.ring;
-  const int first = (int)(p + 1 < S ? p + 1 : S);
-  const int64_t from = p - a.W + 1 > S ? p - a.W + 1 : S;
-  const int count = first + (p >= from ? (int)(p - from + 1) : 0);
-  const int parts = (count + a.chunk - 1) / a.chunk;
+  const Visible see(a.places, p, a.W);
+  const int parts = (see.count + a.chunk - 1) / a.chunk;
   if (split >= parts) return;
-  const int e0 = split * a.chunk, e1 = min(count, e0 + a.chunk);
-  const int turn = p >= from ? (int)((from - S) % ring) : 0; // the ring's row of token `from`
-  const T* kb = reinterpret_cast<const T*>(a.kc.p) + slot * a.kc.sn + hk * a.kc.sh + 8 * li;
-  const T* vb = reinterpret_cast<const T*>(a.vc.p) + slot * a.vc.sn + hk * a.vc.sh + 8 * li;
-  auto row = [&](int e) -> int64_t {
-    if (e < first) return e;
-    const int r = turn + e - first;
-    return S + (r >= ring ? r - ring : r);
-  };
+  const int e0 = split * a.chunk, e1 = min(see.count, e0 + a.chunk);
+  const float* kb = reinterpret_cast<const float*>(a.kc.p) + slot * a.kc.sn + hk * a.kc.sh + 8 * li;
+  const float* vb = reinterpret_cast<const float*>(a.vc.p) + slot * a.vc.sn + hk * a.vc.sh + 8 * li;
   float* const mine = a.parts + (((int64_t)n * a.Hkv + hk) * a.splits + split) * share * kStepPart;
 
   for (int h0 = 0; h0 < share; h0 += kHeads) {
@@ -114,10 +206,10 @@ __global__ __launch_bounds__(256) void window_step_kernel(WindowStepArgs a) {
     float q[kHeads][8], o[kHeads][8], m[kHeads], sum[kHeads];
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
-      const T* qp = static_cast<const T*>(a.q) + n * a.q_sn + (hk * share + h0 + min(h, heads - 1)) * a.q_sh + 8 * li;
+      load8(static_cast<const float*>(a.q) + n * a.q_sn + (hk * share + h0 + min(h, heads - 1)) * a.q_sh + 8 * li, q[h]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        q[h][i] = to_f32(qp[i]) * a.scale_l2;
+        q[h][i] *= a.scale_l2;
         o[h][i] = 0.f;
       }
       m[h] = -__builtin_inff();
@@ -127,7 +219,7 @@ __global__ __launch_bounds__(256) void window_step_kernel(WindowStepArgs a) {
       float k[kKeys][8], v[kKeys][8];
 #pragma unroll
       for (int x = 0; x < kKeys; ++x) {
-        const int64_t r = row(min(e + 16 * x, e1 - 1));
+        const int64_t r = see.row(min(e + 16 * x, e1 - 1));
         load8(kb + r * a.kc.st, k[x]);
         load8(vb + r * a.vc.st, v[x]);
       }
@@ -165,7 +257,7 @@ __global__ __launch_bounds__(256) void window_step_kernel(WindowStepArgs a) {
     for (int h = 0; h < kHeads; ++h) {
       float top = fmaxf(m[h], __shfl_xor(m[h], 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float f = m[h] == -__builtin_inff() ? (sum[h] == 0.f ? 0.f : sum[h]) : __builtin_amdgcn_exp2f(m[h] - top);
+      const float f = m[h] == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m[h] - top);
       float x = sum[h] * f;
       x += __shfl_xor(x, 16, 64);
       x += __shfl_xor(x, 32, 64);
@@ -182,52 +274,155 @@ __global__ __launch_bounds__(256) void window_step_kernel(WindowStepArgs a) {
       }
     }
     __syncthreads();
-    for (int u = tid; u < heads * kHead; u += 256) {
-      const int h = u / kHead, d = u % kHead;
-      float top = part[0][h][kHead];
+    join_block<float, kHeads>(part, heads, parts == 1, out + h0 * kHead, mine + h0 * kStepPart);
+  }
+  if (parts > 1) join_row<float>(a, n, hk, parts, share, out, &part[0][0][0]);
+}
+
+// bf16: a wave takes 32 keys at a time, with 16 query heads of a key head in the columns of both products
+// (v_mfma_f32_16x16x32_bf16; fewer heads leave columns idle, which costs nothing here): S = K Q^T with the keys' rows straight
+// from memory, O^T = V^T P with V through the wave's own LDS (direct loads, transposed reads).  Key row m of tile t stands for
+// key tile_row(t, m), so that a lane's 8 scores are the 8 keys that it has to hold of P.  The next 32 keys' loads run beside
+// the products.  P enters as three bf16 parts (24 bits), cut and not rounded, and at least 2^-126 each: none is negative or 0,
+// so that an infinity of V stays one.
+__device__ __forceinline__ Parts<3> cut3(const float (&x)[8]) {
+  u32x4 w[3];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) top = fmaxf(top, part[w][h][kHead]);
-      float x = 0.f, y = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float mw = part[w][h][kHead], f = mw == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mw - top);
-        x += mw == -__builtin_inff() ? part[w][h][kHead + 1] : part[w][h][kHead + 1] * f;
-        y += mw == -__builtin_inff() ? part[w][h][d] : part[w][h][d] * f;
-      }
-      if (parts == 1) {
-        out[(h0 + h) * kHead + d] = from_f32<T>(y / x);
-      } else {
-        float* to = mine + (h0 + h) * kStepPart;
-        part_store(to + d, y);
-        if (d == 0) {
-          part_store(to + kHead, top);
-          part_store(to + kHead + 1, x);
-        }
-      }
+    for (int n = 0; n < 3; ++n) {
+      const float least = 1.17549435e-38f;
+      const uint32_t ua = __float_as_uint(fmaxf(a, least)), ub = __float_as_uint(fmaxf(b, least));
+      w[n][i] = __builtin_amdgcn_perm(ub, ua, 0x07060302);   // the upper halves
+      a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+      b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
     }
   }
-  if (parts == 1) return;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0)
-    arrived = __hip_atomic_fetch_add(a.counters + (int64_t)n * a.Hkv + hk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (arrived != (uint32_t)(parts - 1)) return;
-  const float* const all = a.parts + ((int64_t)n * a.Hkv + hk) * a.splits * share * kStepPart;
-  for (int u = tid; u < share * kHead; u += 256) {
-    const float* at = all + u / kHead * kStepPart;
-    const int d = u % kHead;
-    float top = -__builtin_inff();
-    for (int s = 0; s < parts; ++s) top = fmaxf(top, part_load(at + (int64_t)s * share * kStepPart + kHead));
-    float x = 0.f, y = 0.f;
-    for (int s = 0; s < parts; ++s) {
-      const float* ps = at + (int64_t)s * share * kStepPart;
-      const float ms = part_load(ps + kHead), f = ms == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ms - top);
-      x = __builtin_fmaf(part_load(ps + kHead + 1), f, x);
-      y = __builtin_fmaf(part_load(ps + d), f, y);
-    }
-    out[u] = from_f32<T>(y / x);
+  Parts<3> r;
+#pragma unroll
+  for (int n = 0; n < 3; ++n) r.p[n] = __builtin_bit_cast(bf16x8, w[n]);
+  return r;
+}
+constexpr int kStepTile = 32 * 256;                          // V of 32 keys in LDS, unit u of key t in place u ^ turn
+__device__ __forceinline__ int step_turn(int t) { return (t & 7) << 1 | (t >> 3 & 1); }
+
+__global__ __launch_bounds__(256, 2) void window_step_bf16_kernel(WindowStepArgs a) {
+  constexpr int kHeads = 16;
+  __shared__ __align__(16) char lds[4 * 2 * kStepTile];      // per wave two buffers; then the waves' parts
+  static_assert(sizeof(lds) >= 4 * kHeads * kStepPart * 4);
+  auto part = reinterpret_cast<float (*)[kHeads][kStepPart]>(lds);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id(), g = l >> 4, m16 = l & 15;
+  const int split = blockIdx.x, hk = blockIdx.y, n = blockIdx.z, share = a.H / a.Hkv;
+  const int64_t slot = a.places.slot(n), p = a.places.position(n);
+  uint16_t* out = static_cast<uint16_t*>(a.o) + ((int64_t)n * a.H + hk * share) * kHead;
+  if (slot < 0 || p < 0) {                                   // a row of padding
+    if (split == 0)
+      for (int i = tid; i < share * kHead; i += 256) out[i] = 0;
+    return;
   }
+  const Visible see(a.places, p, a.W);
+  const int parts = (see.count + a.chunk - 1) / a.chunk;
+  if (split >= parts) return;
+  const int e0 = split * a.chunk, e1 = min(see.count, e0 + a.chunk);
+  const uint16_t* kb = reinterpret_cast<const uint16_t*>(a.kc.p) + slot * a.kc.sn + hk * a.kc.sh;
+  const uint16_t* vb = reinterpret_cast<const uint16_t*>(a.vc.p) + slot * a.vc.sn + hk * a.vc.sh;
+  float* const mine = a.parts + (((int64_t)n * a.Hkv + hk) * a.splits + split) * share * kStepPart;
+  char* const own = lds + wave * 2 * kStepTile;
+  const uint32_t own_at = lds_addr(own);
+  // transposed reads: keys 8 g + 4 e + i / 4 of the tile, elements 16 dt + 4 (i % 4) .. + 3
+  int col[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+    col[d] = (8 * g + (m16 >> 2)) * 256 + 8 * (m16 & 1) + 16 * ((2 * d + ((m16 & 3) >> 1)) ^ (2 * (m16 >> 2) + (g & 1)));
+
+  for (int h0 = 0; h0 < share; h0 += kHeads) {
+    const int heads = min(kHeads, share - h0);
+    bf16x8 q[4];
+    {
+      const uint16_t* qp = static_cast<const uint16_t*>(a.q) + n * a.q_sn + (hk * share + h0 + min(m16, heads - 1)) * a.q_sh + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) q[ks] = *reinterpret_cast<const bf16x8*>(qp + 32 * ks);
+    }
+    floatx4 o[8];
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) o[dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float m = -__builtin_inff(), sum = 0.f;
+    bf16x8 k[2][4];
+    auto load = [&](int e, int buffer) {                     // keys e .. e + 31 (past the last: it again)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint16_t* at = kb + (int64_t)see.row(min(e + 8 * (m16 >> 2) + 4 * t + (m16 & 3), e1 - 1)) * a.kc.st + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) k[t][ks] = *reinterpret_cast<const bf16x8*>(at + 32 * ks);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int t = 4 * j + g;
+        load_lds16_at(vb + (int64_t)see.row(min(e + t, e1 - 1)) * a.vc.st + 8 * (m16 ^ step_turn(t)),
+                      __builtin_amdgcn_readfirstlane(own_at + buffer * kStepTile + j * 1024));
+      }
+    };
+    int e = e0 + 32 * wave, buffer = 0;
+    if (e < e1) load(e, 0);
+    for (; e < e1; e += 128, buffer ^= 1) {
+      wait_loads();
+      floatx4 s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[t][ks], q[ks], s[t], 0, 0, 0);
+      }
+      if (e + 128 < e1) load(e + 128, buffer ^ 1);
+      float x[8], top = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = e + 8 * g + i < e1 ? s[i >> 2][i & 3] * a.scale_l2 : -__builtin_inff();
+        top = fmaxf(top, x[i]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float f = top == m ? 1.f : __builtin_amdgcn_exp2f(m - top), minus = top == -__builtin_inff() ? 0.f : top;
+      m = top;
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(x[i] - minus);
+        sum += x[i];
+      }
+      const Parts<3> w = cut3(x);
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) {
+        s16x4 y[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          y[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
+              own + buffer * kStepTile + col[dt & 3] + 1024 * i + 16 * ((dt & 4 ? 8 : 0) ^ (8 * i))));
+        const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        o[dt] *= f;
+#pragma unroll
+        for (int i = 2; i >= 0; --i) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w.p[i], o[dt], 0, 0, 0);
+      }
+    }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    __syncthreads();                                         // the waves' buffers are free
+    if (m16 < heads) {
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) part[wave][m16][16 * dt + 4 * g + r] = o[dt][r];
+      if (g == 0) {
+        part[wave][m16][kHead] = m;
+        part[wave][m16][kHead + 1] = sum;
+      }
+    }
+    __syncthreads();
+    join_block<uint16_t, kHeads>(part, heads, parts == 1, out + h0 * kHead, mine + h0 * kStepPart);
+    if (h0 + kHeads < share) __syncthreads();
+  }
+  if (parts > 1) join_row<uint16_t>(a, n, hk, parts, share, out, &part[0][0][0]);
 }
 
 }  // namespace gsa
@@ -235,7 +430,7 @@ __global__ __launch_bounds__(256) void window_step_kernel(WindowStepArgs a) {
 namespace gsa_host {
 namespace {
 
-// Keys of a block and blocks of a row and key head: as few keys (64 at least) as give some 1024 blocks.
+// Keys of a block and blocks of a row and key head: as few keys (a multiple of 128: four waves of 32) as give some 1024 blocks.
 struct StepPlan { int chunk, splits; size_t counters, parts; };
 bool step_plan(int N, int H, int Hkv, int window, int sinks, StepPlan& z) {
   if (N < 1 || N > 65535 || Hkv < 1 || Hkv > 65535 || H < Hkv || H % Hkv || window < 1 || sinks < 0 ||
@@ -243,7 +438,7 @@ bool step_plan(int N, int H, int Hkv, int window, int sinks, StepPlan& z) {
     return false;
   const int64_t keys = (int64_t)window + sinks, heads = (int64_t)N * Hkv;
   const int64_t want = std::max<int64_t>(1, 1024 / heads);
-  z.chunk = (int)std::max<int64_t>(64, (keys + want - 1) / want);
+  z.chunk = (int)((std::max<int64_t>(1, (keys + want - 1) / want) + 127) / 128 * 128);
   z.splits = (int)((keys + z.chunk - 1) / z.chunk);
   z.counters = up((size_t)heads * 4);
   z.parts = z.splits > 1 ? (size_t)N * z.splits * H * gsa::kStepPart * 4 : 0;
@@ -264,12 +459,13 @@ int launch_write(const gsa::WindowWriteArgs& a, int64_t blocks, int dtype, hipSt
   else hipLaunchKernelGGL(gsa::window_write_kernel<float>, dim3(blocks), dim3(256), 0, s, a);
   return launch_status();
 }
-template <typename T> int launch_step(const gsa::WindowStepArgs& a, int N, hipStream_t s) {
+int launch_step(const gsa::WindowStepArgs& a, int N, int dtype, hipStream_t s) {
   const dim3 grid(a.splits, a.Hkv, N);
   const int share = a.H / a.Hkv;
-  if (share == 1) hipLaunchKernelGGL((gsa::window_step_kernel<T, 1>), grid, dim3(256), 0, s, a);
-  else if (share == 2) hipLaunchKernelGGL((gsa::window_step_kernel<T, 2>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((gsa::window_step_kernel<T, 4>), grid, dim3(256), 0, s, a);
+  if (dtype == GSA_DTYPE_BF16) hipLaunchKernelGGL(gsa::window_step_bf16_kernel, grid, dim3(256), 0, s, a);
+  else if (share == 1) hipLaunchKernelGGL(gsa::window_step_f32_kernel<1>, grid, dim3(256), 0, s, a);
+  else if (share == 2) hipLaunchKernelGGL(gsa::window_step_f32_kernel<2>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(gsa::window_step_f32_kernel<4>, grid, dim3(256), 0, s, a);
   return launch_status();
 }
 
@@ -334,5 +530,5 @@ extern "C" int gsa_window_step(const void* q, int64_t q_sn, int64_t q_sh, const 
   }
   const gsa::WindowStepArgs a{q, q_sn, q_sh, kc, vc, p, H, Hkv, window, z.splits, z.chunk, scale * gsa::kLog2e, o,
                               reinterpret_cast<float*>(static_cast<char*>(ws) + z.counters), counters};
-  return dtype == GSA_DTYPE_BF16 ? launch_step<uint16_t>(a, N, s) : launch_step<float>(a, N, s);
+  return launch_step(a, N, dtype, s);
 }
