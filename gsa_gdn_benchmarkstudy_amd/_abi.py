@@ -1219,6 +1219,8 @@ def linear_attn_backward(q, k, v, g, state_in, cu, scale: float, saved, dout, ds
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t [..., heads, 128] with contiguous, 16-byte aligned head rows: itself, or a copy."""
     size, at = t.element_size(), t.data_ptr()
+    if at % 16 == 0 and t.is_contiguous():
+        return t
     *lead, e = t.stride()
     for s in lead:
         at |= s * size

@@ -106,13 +106,15 @@ __device__ __forceinline__ void mma_rows_apart(floatx4 (&hi)[M], floatx4 (&lo)[M
 }
 
 // P enters a product with bf16 outputs in two parts
-template <typename T, int kDg> struct LinearSizes {
+template <typename T, int kDg, bool kDouble> struct LinearSizes {
   static constexpr int C = ChunkType<T>::kChunk, NP = ChunkType<T>::kParts;
   static constexpr int kPParts = NP == 1 ? 2 : 3, kXParts = NP == 1 && !kDg ? 2 : 3;
   static constexpr int kRows = (C / 16) * 4 * NP * kUnit, kP = Square<C>::kFrags * kPParts * kUnit, kStage = C * kHead * sizeof(T);
-  static constexpr int kB = 0, kV = kRows, kA = 2 * kRows, kAtP = 3 * kRows, kAtStage = kAtP + kP, kDot = kAtStage + kStage;
+  // keys, values and dot, twice with kDouble; rows, P, the outputs on their way out
+  static constexpr int kB = 0, kV = kRows, kDot = 2 * kRows, kGroup = (kDg ? 3 : 2) * kRows, kA = (kDouble ? 2 : 1) * kGroup;
+  static constexpr int kAtP = kA + kRows, kAtStage = kAtP + kP;
   // powers of the decay: in_x a^(C-1-t), in_o a^(t+1)
-  static constexpr int kToEnd = kDot + (kDg ? kRows : 0), kFromX = kToEnd + 4 * C;
+  static constexpr int kToEnd = kAtStage + kStage, kFromX = kToEnd + 4 * C;
   static constexpr size_t kBytes = kFromX + 4 * C, kState = 2 * kRows + 4 * C;
 };
 
@@ -146,9 +148,9 @@ __device__ __forceinline__ void state_store(const floatx4 (&S)[8][1], float* p, 
 }
 
 // kOut: the outputs; otherwise what a segment adds to X.  kDg: this pass's part of dg: 1 dq's, 2 dk's.
-template <typename T, bool kOut, int kDg>
+template <typename T, bool kOut, int kDg, bool kDouble>
 __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, char* lds, float* dg_part) {
-  using Z = LinearSizes<T, kDg>;
+  using Z = LinearSizes<T, kDg, kDouble>;
   constexpr int C = Z::C, NP = Z::NP, MT = C / 16, JS = C / 32, kToEnd = kOut ? Z::kToEnd : 2 * Z::kRows;
   const uint32_t base = lds_addr(lds);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id(), g = l >> 4, m = l & 15;
@@ -241,11 +243,15 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
   const int step = x.back ? -1 : 1;
   float dg = 0.f;
   int c = x.back ? c1 - 1 : c0;
+  auto fetch_group = [&](int c, int to) {
+    fetch(x.b, x.b_shared, c, to + Z::kB, lane_b);
+    fetch(x.v, x.v_shared, c, to + Z::kV, lane_v);
+    if (kDg) fetch(x.dot, 1, c, to + Z::kDot, lane_dot);
+  };
+  int group = 0;                                             // this chunk's, bytes from lds
   if (c0 < c1) {
-    fetch(x.b, x.b_shared, c, Z::kB, lane_b);
-    fetch(x.v, x.v_shared, c, Z::kV, lane_v);
+    fetch_group(c, 0);
     if (kOut) fetch(x.a, x.a_shared, c, Z::kA, lane_a);
-    if (kDg) fetch(x.dot, 1, c, Z::kDot, lane_dot);
   }
   for (int n = c0; n < c1; ++n, c += step) {
     const bool more = n + 1 < c1;
@@ -255,6 +261,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
     const float whole = power(g2, left - 1 + lead);
     wait_loads();
     __syncthreads();
+    if (kDouble && more) fetch_group(c + step, Z::kGroup - group);
 
     floatx4 O[MT];                                           // O[i][r]: token tile_row(i, m), element col4 + r
     const int col4 = 32 * (wave >> 1) + 4 * (wave & 1);      // (and 8 g)
@@ -273,8 +280,8 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
           }
           return NP == 1 ? hi[0] : hi[0] + lo[0];
         };
-        floatx4 p = product(Z::kA, Z::kB), kv;
-        if constexpr (kDg == 1) kv = product(Z::kDot, Z::kV);
+        floatx4 p = product(Z::kA, group + Z::kB), kv;
+        if constexpr (kDg == 1) kv = product(group + Z::kDot, group + Z::kV);
         const int lh = here(l), i = tile_row(pt, lh & 15), j = 32 * (nt >> 1) + 4 * (nt & 1) + 8 * (lh >> 4);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -317,7 +324,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
         if (!lead) e = x.in_o * power(g2, t);
         float y[4];
         if constexpr (kDg != 0) {                            // q or k of the lane's outputs
-          const char* at = lds + Z::kDot + (i * 4 + (wave >> 1)) * NP * kUnit + 16 * rs + 8 * (wave & 1);
+          const char* at = lds + group + Z::kDot + (i * 4 + (wave >> 1)) * NP * kUnit + 16 * rs + 8 * (wave & 1);
 #pragma unroll
           for (int r = 0; r < 4; ++r) y[r] = 0.f;
 #pragma unroll
@@ -352,7 +359,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
       float odd = 0.f;
 #pragma unroll
       for (int js = 0; js < JS; ++js) {
-        v[js] = cols_of<NP>(lds + Z::kV, wave, js, place);
+        v[js] = cols_of<NP>(lds + group + Z::kV, wave, js, place);
 #pragma unroll
         for (int e = 0; e < 8; ++e) odd = __builtin_fmaf(element(v[js], e), 0.f, odd);
       }
@@ -419,7 +426,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
     Parts<3> vd[JS];
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
-      const Parts<NP> v = cols_of<NP>(lds + Z::kV, wave, js, place);
+      const Parts<NP> v = cols_of<NP>(lds + group + Z::kV, wave, js, place);
       float y[8];
       if (left == C) {
         load8(to_end + 32 * js + 8 * g, y);
@@ -447,7 +454,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
       for (int js = 0; js < JS; ++js) {
         Parts<NP> k[kSome];
 #pragma unroll
-        for (int i = 0; i < kSome; ++i) k[i] = cols_of<NP>(lds + Z::kB, t + i, js, place);
+        for (int i = 0; i < kSome; ++i) k[i] = cols_of<NP>(lds + group + Z::kB, t + i, js, place);
         mma_apart(hi, kApart ? lo : hi, k, vd[js]);
       }
 #pragma unroll
@@ -464,11 +471,8 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
       }
     }
     __syncthreads();                                         // B, V, dot and P are free; the outputs are staged
-    if (more) {
-      fetch(x.b, x.b_shared, c + step, Z::kB, lane_b);
-      fetch(x.v, x.v_shared, c + step, Z::kV, lane_v);
-      if (kDg) fetch(x.dot, 1, c + step, Z::kDot, lane_dot);
-    }
+    if constexpr (kDouble) group = Z::kGroup - group;
+    else if (more) fetch_group(c + step, 0);
     if constexpr (kOut) {
       if (!x.out_parts) {
         constexpr int kPer = 16 / sizeof(T), kPieces = kHead / kPer;
@@ -516,6 +520,9 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
   }
 }
 
+// kPerSimd 4: two blocks share a CU and cover each other's waits; 2: one, the next chunk's operands on their way (bf16)
+template <typename T, int kPerSimd> constexpr bool kTwice = sizeof(T) == 2 && kPerSimd == 2;
+
 template <typename T, bool kOut, int kDg, int kPerSimd>
 __global__ __launch_bounds__(64 * kWaves, kPerSimd) void linear_scan_kernel(LinearArgs a) {
   extern __shared__ __align__(16) char lds[];
@@ -525,11 +532,10 @@ __global__ __launch_bounds__(64 * kWaves, kPerSimd) void linear_scan_kernel(Line
     return;
   }
   if constexpr (kDg != 0) {
-    if (which == 0) linear_scan<T, kOut, 1>(a, a.pass[0], lds, a.dg_parts + blockIdx.x);
-    else if (which == 1) linear_scan<T, kOut, 2>(a, a.pass[1], lds, a.dg_parts + a.units + blockIdx.x);
-    else linear_scan<T, kOut, 0>(a, a.pass[2], lds, nullptr);
+    if (which == 0) linear_scan<T, kOut, 1, kTwice<T, kPerSimd>>(a, a.pass[0], lds, a.dg_parts + blockIdx.x);
+    else linear_scan<T, kOut, 2, kTwice<T, kPerSimd>>(a, a.pass[1], lds, a.dg_parts + a.units + blockIdx.x);
   } else {
-    linear_scan<T, kOut, 0>(a, a.pass[which], lds, nullptr);
+    linear_scan<T, kOut, 0, kTwice<T, kPerSimd>>(a, a.pass[which], lds, nullptr);
   }
 }
 
@@ -631,7 +637,7 @@ LinearPlan linear_plan(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
 }
 
 template <typename T, bool kOut, int kDg, int kPerSimd> int launch_linear(const gsa::LinearArgs& a, int passes, hipStream_t s) {
-  using Z = gsa::LinearSizes<T, kDg>;
+  using Z = gsa::LinearSizes<T, kDg, gsa::kTwice<T, kPerSimd>>;
   constexpr size_t lds = kOut ? Z::kBytes : Z::kState;
   static_assert(lds * (kPerSimd / 2) <= 160 * 1024);
   if (const int e = allow_lds<gsa::linear_scan_kernel<T, kOut, kDg, kPerSimd>>(lds)) return e;
@@ -744,7 +750,15 @@ template <typename T> int linear_backward(const gsa_linear_args* x, gsa::LinearA
   a.pass[2] = dv;
   const int64_t row = 128 * (int64_t)(parts ? 4 * a.Hv : sizeof(T) * a.Hk);
   a.outside = {a.s, {(char*)dq.out, (char*)dk.out, (char*)x->dv}, {row, row, a.Hv * 128 * (int64_t)sizeof(T)}};
-  int e = x->dg ? launch_linear<T, true, 1, 2>(a, 3, s) : launch_linear<T, true, 0, sizeof(T) == 2 ? 4 : 2>(a, 3, s);
+  int e;
+  constexpr int kPerSimd = sizeof(T) == 2 ? 4 : 2;
+  if (x->dg) {                                               // dv goes by itself: without dg two blocks share a CU
+    if ((e = launch_linear<T, true, 1, 2>(a, 2, s))) return e;
+    a.pass[0] = dv;
+    e = launch_linear<T, true, 0, kPerSimd>(a, 1, s);
+  } else {
+    e = launch_linear<T, true, 0, kPerSimd>(a, 3, s);
+  }
   if (e) return e;
   if (x->dg) {
     hipLaunchKernelGGL(gsa::linear_dg_kernel, dim3(a.Hv), dim3(256), 0, s, a.dg_parts, a.units, a.Hv, x->dg);

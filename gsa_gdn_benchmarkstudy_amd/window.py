@@ -64,7 +64,7 @@ def _check_packed(cu, B: int):
 def _index(t: Optional[torch.Tensor], N: int, name: str):
     if t is None:
         return None
-    if tuple(t.shape) != (N,) or t.dtype not in (torch.int32, torch.int64):
+    if t.shape != (N,) or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name}: int32 or int64 [{N}]")
     return t.contiguous()
 
@@ -134,10 +134,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 
 def _check_caches(k_cache, v_cache, Hkv: int, dtype, rows: int) -> None:
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dim() != 4 or tuple(t.shape[2:]) != (Hkv, D_HEAD) or t.dtype != dtype:
+        if t.dim() != 4 or t.shape[2:] != (Hkv, D_HEAD) or t.dtype != dtype:
             raise ValueError(f"{name} {tuple(t.shape)} {t.dtype}: expected {dtype} [slots, rows, {Hkv}, {D_HEAD}]")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("caches are written in place: call it under torch.no_grad()")
+        if t.is_contiguous() and t.data_ptr() % 16 == 0:
+            continue
         s0, s1, s2, s3 = t.stride()
         if s3 != 1 or ((s0 | s1 | s2) * t.element_size() | t.data_ptr()) % 16:
             raise ValueError(f"{name} is updated in place: its rows must be contiguous and 16-byte aligned")
@@ -154,9 +156,8 @@ def _check_caches(k_cache, v_cache, Hkv: int, dtype, rows: int) -> None:
 
 
 def _written(*ts: torch.Tensor) -> None:
-    for t in ts:
-        if not t.is_inference():
-            _increment_version(t)                # a graph that kept the old cache must not use the new one
+    if not ts[0].is_inference() and not ts[1].is_inference():
+        _increment_version(ts)                   # a graph that kept the old caches must not use the new ones
 
 
 def window_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int = 0,
