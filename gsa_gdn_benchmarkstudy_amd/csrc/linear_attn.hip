@@ -360,8 +360,10 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
 #pragma unroll
       for (int js = 0; js < JS; ++js) {
         v[js] = cols_of<NP>(lds + group + Z::kV, wave, js, place);
+        // (times 0, added: v_dot2c_f32_bf16; the first part of an fp32 value is not finite where the value is not)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) odd = __builtin_fmaf(element(v[js], e), 0.f, odd);
+        for (int e = 0; e < 8; e += 2)
+          odd = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[js].p[0][e], v[js].p[0][e + 1]}, bf16x2{(__bf16)0.f, (__bf16)0.f}, odd, false);
       }
       int bad = C;
       const bool any = __builtin_amdgcn_ballot_w64(odd != 0.f) != 0;
@@ -554,17 +556,22 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int C) {
   floatx4 X = {0.f, 0.f, 0.f, 0.f};
   if (x.first) X = *reinterpret_cast<const floatx4*>(x.first + sn);
   auto at = [&](int i) { return ((int64_t)(sp.slot0 + (x.back ? segs - 1 - i : i)) * a.Hv + h) * kHead * kHead + e; };
-  floatx4 add = *reinterpret_cast<const floatx4*>(x.add + at(0));
-  for (int i = 0; i + 1 < segs; ++i) {
-    floatx4 next = {0.f, 0.f, 0.f, 0.f};
-    if (i + 2 < segs) next = *reinterpret_cast<const floatx4*>(x.add + at(i + 1));
-    // the last tokens' segment may be short, and no decay lies before the gradient of the final state
-    const int steps = x.back && i == 0 ? sp.len - (segs - 1) * tokens - 1 : tokens;
-    const float f = power(g2, steps);
+  constexpr int kSome = 8;                                   // loads on their way at once (32 segments of 16 heads: 12 us, one by one 14)
+  for (int i0 = 0; i0 + 1 < segs; i0 += kSome) {
+    floatx4 add[kSome];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) X[r] = __builtin_fmaf(X[r], f, add[r]);
-    *reinterpret_cast<floatx4*>(const_cast<float*>(x.init) + at(i + 1)) = X;
-    add = next;
+    for (int k = 0; k < kSome; ++k) add[k] = *reinterpret_cast<const floatx4*>(x.add + at(min(i0 + k, segs - 2)));
+#pragma unroll
+    for (int k = 0; k < kSome; ++k) {
+      const int i = i0 + k;
+      if (i + 1 >= segs) break;
+      // the last tokens' segment may be short, and no decay lies before the gradient of the final state
+      const int steps = x.back && i == 0 ? sp.len - (segs - 1) * tokens - 1 : tokens;
+      const float f = power(g2, steps);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) X[r] = __builtin_fmaf(X[r], f, add[k][r]);
+      *reinterpret_cast<floatx4*>(const_cast<float*>(x.init) + at(i + 1)) = X;
+    }
   }
 }
 
@@ -622,8 +629,17 @@ LinearPlan linear_plan(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   if ((packed ? (int64_t)T / z.C + N : B * nc) > (1 << 23) / Hv || heads >= 1 << 23) return z;
   const int64_t length = packed ? (nc + N - 1) / N : nc;
   z.segs = 0;
-  if (heads <= 256 && length >= 4) {
-    const int64_t pieces = std::max<int64_t>(1, 512 / heads), seg = std::max<int64_t>(2, (length + pieces - 1) / pieces);
+  // A head is one chain of chunks; cut into segments it is passed over twice, once for the state alone (about half the work). Two
+  // blocks a CU are 512 of them, so a chain is cut into 512 / heads; where the heads fill most of the card the second pass costs
+  // more. Measured in us, segments of n chunks of 64 (0: none), 16 heads a row of the batch, bf16 forward:
+  //   T = 16384, B = 1:  0: 1214  2: 225  4: 156  8: 126 (taken)  16: 150      T = 4096, B = 6:   0: 335  8: 203  16: 202 (taken)
+  //   T = 512,   B = 1:  0: 42    1: 23 (taken)  2: 27  4: 40                  T = 4096, B = 10:  0: 343  16: 343  22: 293 (taken)
+  //   T = 2048,  B = 1:  0: 153   1: 45  2: 39 (taken)  4: 47                  T = 4096, B = 12:  0: 342 (taken)  16: 361  32: 375
+  //   23 sequences, 12289 tokens (368 heads): 0: 116 (taken)  4: 133  8: 127   T = 4096, B = 16:  0: 351 (taken)  16: 460  32: 411
+  // With gradients, B = 4, T = 4096: 0: 1069  4: 582  8: 494 (taken)  16: 520; B = 16: 0: 1562 (taken)  16: 1821.
+  // One chunk a segment pays where the join then has few to go through: T = 1000  1: 30  2: 32.
+  if (heads <= 160 && length >= 4) {
+    const int64_t pieces = 512 / heads, seg = std::max<int64_t>(length <= 16 ? 1 : 2, (length + pieces - 1) / pieces);
     if (seg < length) {
       z.seg = (int)seg;
       z.segs = packed ? (int64_t)T / (z.C * seg) + N : B * ((nc + seg - 1) / seg);
