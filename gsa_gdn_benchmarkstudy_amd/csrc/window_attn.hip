@@ -37,7 +37,6 @@ struct WindowArgs {
   float* far_parts;           // [slots of far queries][far_first][H][2][far_keys][128]
 };
 
-
 template <int N> struct Number { static constexpr int value = N; };
 
 template <typename T> struct WindowType;
@@ -734,6 +733,10 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   if (B < 1 || T < 1 || N < 1 || Hkv < 1 || H < Hkv || H % Hkv || H > 65535 || window < 1 || sinks < 0 || !dtype_size(dtype)) return false;
   z.W = std::min(window, T);
   z.S = std::min(sinks, T);
+  if ((int64_t)z.W + z.S >= T) {                             // every earlier token is visible: the window alone says so
+    z.W = T;
+    z.S = 0;
+  }
   auto slots = [&](int n) { return packed ? (int64_t)T / n + N : (int64_t)B * (((int64_t)T + n - 1) / n); };
   // 64 queries a block (two waves share their queries, each takes half of the keys) while 128 leave CUs idle: us forward, 16
   // heads on 4, by 128 / 64 queries: T = 512 18 / 13, T = 1024, window 256 18 / 13, T = 2048 35 / 26, T = 4096, window 1024
@@ -749,11 +752,13 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   z.near_keys = dtype == GSA_DTYPE_BF16 && slots(128) * Hkv >= 512 ? 128 : 64;
   z.far_keys = dtype == GSA_DTYPE_BF16 ? 32 : 64;
   z.near = slots(z.near_keys);
-  if (z.S && z.W < T) {
+  if (z.S) {
     z.near_first = (z.S + z.near_keys - 1) / z.near_keys;
     z.far_first = (z.S + z.far_keys - 1) / z.far_keys;
-    // 512 far queries a part, 128 where that leaves CUs idle
+    // 512 far queries a part, 128 where that leaves CUs idle; more of them where the parts are many (they fill the card without,
+    // and each leaves 32 KiB, so that the workspace would grow with T times the first tokens)
     z.far_rows = slots(512) * z.far_first * H >= 256 ? 512 : 128;
+    while (z.far_rows < T && slots(z.far_rows) * z.far_first * H > 8192) z.far_rows *= 2;
     z.far = slots(z.far_rows) * z.far_first;
     if (z.far > (1 << 23) / H || (int64_t)N * z.near_first > (1 << 23) / H) return false;
   }

@@ -23,8 +23,9 @@ struct Places {
     const int64_t s = !at ? n : at64 ? static_cast<const int64_t*>(at)[n] : static_cast<const int32_t*>(at)[n];
     return s >= 0 && s < slots ? s : -1;
   }
-  __device__ int64_t position(int n) const {
-    return !pos ? 0 : pos64 ? static_cast<const int64_t*>(pos)[n] : static_cast<const int32_t*>(pos)[n];
+  __device__ int64_t position(int n) const {                 // -1: padding (from 2^62 on sums with it could pass 64 bits)
+    const int64_t p = !pos ? 0 : pos64 ? static_cast<const int64_t*>(pos)[n] : static_cast<const int32_t*>(pos)[n];
+    return p >= 0 && p < (int64_t)1 << 62 ? p : -1;
   }
   __device__ int64_t row(int64_t p) const { return p < S ? p : S + (p - S) % ring; }
 };
@@ -445,7 +446,7 @@ bool step_plan(int N, int H, int Hkv, int window, int sinks, StepPlan& z) {
   return true;
 }
 int places(const void* at, int at_bytes, const void* pos, int pos_bytes, int slots, int rows, int sinks, gsa::Places& p) {
-  if (slots < 1 || sinks < 0 || rows <= sinks) return GSA_ERR_SHAPE;
+  if (slots < 1 || sinks < 0 || rows <= sinks || rows >= 1 << 30) return GSA_ERR_SHAPE;    // (rows are added up in 32 bits)
   if ((at && at_bytes != 4 && at_bytes != 8) || (pos && pos_bytes != 4 && pos_bytes != 8)) return GSA_ERR_SHAPE;
   if ((at && !aligned(at, at_bytes)) || (pos && !aligned(pos, pos_bytes))) return GSA_ERR_ALIGN;
   p = {at, pos, at_bytes == 8, pos_bytes == 8, slots, sinks, rows - sinks};

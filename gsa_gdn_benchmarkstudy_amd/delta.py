@@ -58,9 +58,9 @@ def _refuse_unseen(*ts: Optional[torch.Tensor]) -> None:
     if _forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
         for t in ts:
             if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError("the gated delta rule and the RMS norm have no forward-mode derivative (torch.autograd.forward_ad)")
+                raise RuntimeError("this operator has no forward-mode derivative (torch.autograd.forward_ad)")
     if torch._C._get_tracing_state() is not None:
-        raise RuntimeError("the gated delta rule and the RMS norm cannot be recorded by torch.jit.trace")
+        raise RuntimeError("this operator cannot be recorded by torch.jit.trace")
 
 
 def _device(first: torch.Tensor, *others: Optional[torch.Tensor]):
@@ -94,7 +94,7 @@ class _Twice(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        raise RuntimeError("the gradients of gated_delta_rule and add_rms_norm cannot be differentiated: the operators are differentiable once")
+        raise RuntimeError("the gradients of this operator cannot be differentiated: it is differentiable once")
 
 
 def _once(backward):

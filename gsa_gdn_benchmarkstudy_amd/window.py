@@ -151,8 +151,10 @@ def _check_caches(k_cache, v_cache, Hkv: int, dtype, rows: int) -> None:
                 extent += (n - 1) * stride
     if k_cache.shape != v_cache.shape:
         raise ValueError(f"k_cache {tuple(k_cache.shape)} != v_cache {tuple(v_cache.shape)}")
-    if k_cache.shape[1] < rows:
-        raise ValueError(f"caches of {k_cache.shape[1]} rows: at least {rows}")
+    if not rows <= k_cache.shape[1] <= _MOST:
+        raise ValueError(f"caches of {k_cache.shape[1]} rows: at least {rows}, and at most {_MOST}")
+    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():
+        raise ValueError("k_cache and v_cache are the same memory")
 
 
 def _written(*ts: torch.Tensor) -> None:
@@ -171,8 +173,8 @@ def window_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
     later tokens take the rows of earlier ones.  positions (int32 or int64 [N], on the device): of
     each sequence's first token here; 0 without it (a prompt's beginning).  cache_indices (int32 or int64 [N],
     on the device): each sequence's slot; sequence n has slot n without it.  A slot outside
-    [0, slots) and a negative position are skipped.  Two sequences of one call that write one
-    row leave either's token there.
+    [0, slots) and a position outside [0, 2**62) are skipped.  Two sequences of one call that write one
+    row leave either's key and either's value there.  k and v are not parts of the caches.
     """
     _check_sinks(sinks)
     if k.dim() != 4 or v.shape != k.shape or k.shape[-1] != D_HEAD or k.shape[2] < 1:
@@ -211,7 +213,7 @@ def window_attention_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optiona
     window + sinks rows.  First k and v of all rows go to the caches, then each row's attention is
     taken over the tokens that it sees there, its own among them.  k and v may both be None: they
     are in the caches already.  A row whose index is outside [0, slots) or whose position is
-    negative is padding: its output is 0 and no cache changes.  Rows with the same index are
+    outside [0, 2**62) is padding: its output is 0 and no cache changes.  Rows with the same index are
     tokens of one sequence, each at its own position: up to rows - sinks - window + 1 consecutive ones (more would take
     each other's rows).  Rows of a cache that the token does not see are not read.  At most 65535 rows.
 

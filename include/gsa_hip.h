@@ -687,12 +687,12 @@ int gsa_window_attn_backward(const gsa_window_args* args, void* stream);
  * The cache of window attention: per sequence `sinks` rows of first tokens and a ring of rows - sinks behind them, the token
  * at position p in row p (p < sinks) or sinks + (p - sinks) % (rows - sinks).  k_cache, v_cache [slots,rows,Hkv,128] in
  * dtype, 16-byte aligned rows.  cache_idx (int32 or int64 by idx_bytes, or NULL): the slot of each sequence; one outside
- * [0, slots) is skipped, as is a negative position.
+ * [0, slots) is skipped, as is a position outside [0, 2^62).  The two caches, and k and v, are different memory.
  * gsa_window_cache_write: k, v [B,T,Hkv,128] of B sequences (or N packed ones, cu_seqlens); positions (int32 or int64 [N], or
  * NULL: 0) of each one's first token.
  * gsa_window_step: row n's token at positions[n], q, o [N,H,128]: k, v [N,Hkv,128] (or both NULL: they are there) go to the
- * cache, then o is the attention over the window's and the first tokens' keys; 0 for a skipped row.  rows >= window +
- * sinks.  ws: gsa_window_step_workspace_bytes (0: sizes that are refused), one for each call in flight.
+ * cache, then o is the attention over the window's and the first tokens' keys; 0 for a skipped row.  window + sinks <=
+ * rows < 2^30.  ws: gsa_window_step_workspace_bytes (0: sizes that are refused), one for each call in flight.
  */
 int gsa_window_cache_write(const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
                            int64_t v_sh, const void* cu_seqlens, int cu_bytes, int B, int T, int N, int Hkv, int d, int dtype,

@@ -488,3 +488,31 @@ def test_prefill_then_decode(dev, dtype):
         got = torch.cat([o[0, int(cu[i]):int(cu[i + 1])], *(y[i:i + 1] for y in outs)])
         _check(got, ref[0][0], size[0][0], n + new, 1, "o")
         _check(pool[slots[i]], ref[1][0], size[1][0], n + new, 1, "state")
+
+
+def test_offsets_past_32_bits(dev):
+    """Tokens 512 KiB apart, the last of them past 2^32 bytes and 2^31 elements; a pool of states past 2^32 bytes."""
+    T, Hk, Hv, apart = 8300, 1, 2, 1 << 18
+    big = torch.empty(T * apart, dtype=torch.bfloat16, device=dev)
+    gen = torch.Generator(device=dev).manual_seed(3)
+    near, far = [], []
+    for i, h in enumerate((Hk, Hk, Hv, Hv)):
+        near.append(torch.randn(1, T, h, D, generator=gen, device=dev).to(torch.bfloat16))
+        far.append(big.as_strided((1, T, h, D), (0, apart, D, 1), 4096 * i).copy_(near[-1]))
+    g = torch.tensor([-0.01, -0.3], device=dev)
+    out = []
+    for q, k, v, do in (near, far):
+        leaf = [t.detach().requires_grad_() for t in (q, k, v, g)]
+        o, _ = linear_attention(*leaf)
+        out.append([o.detach(), *torch.autograd.grad(o, leaf, do)])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    slots = 33000                                # x 2 heads x 64 KiB
+    pool = torch.empty(slots, Hv, D, D, device=dev)
+    at = torch.tensor([slots - 1, 0, 16384], device=dev)
+    pool[at] = small = torch.randn(3, Hv, D, D, generator=gen, device=dev)
+    rows = [t[0, :3] for t in near[:3]]
+    with torch.no_grad():
+        a = linear_attention_step(*rows, g, small)
+        b = linear_attention_step(*rows, g, pool, at)
+    assert torch.equal(a, b) and torch.equal(pool[at], small)

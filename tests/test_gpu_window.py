@@ -100,6 +100,15 @@ def test_far_queries_of_first_tokens(dev, B, T, H, Hkv, W, S, dtype):
     _compare(_run(x, dev, W, S, do=do), x, [(b, 0, T) for b in range(B)], W, S, do)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,T,H,Hkv,W,S", [(1, 700, 2, 1, 650, 50), (1, 700, 2, 1, 650, 49), (2, 300, 2, 2, 10, 299), (4, 1100, 24, 2, 50, 1000)])
+def test_many_first_tokens(dev, B, T, H, Hkv, W, S, dtype):
+    """First tokens that are all that the window leaves out, all but one, and so many that their queries' parts grow."""
+    print(f"first tokens {dtype} B={B} T={T} H={H} Hkv={Hkv} W={W} S={S}", flush=True)
+    x, do = _inputs(B, T, H, Hkv, dtype, seed=T + S), _grad(B, T, H, dtype, 7)
+    _compare(_run(x, dev, W, S, do=do), x, [(b, 0, T) for b in range(B)], W, S, do)
+
+
 PACKS = [[1], [5, 0, 64, 1, 65, 63], [0, 0, 3], [130, 32, 33], [128, 64, 256], [0], [1300, 1, 0, 333]]
 
 
@@ -370,6 +379,25 @@ def test_step_many_rows(dev):
     _step_case(dev, torch.bfloat16, N, 2, 1, N + 3, 40, 30, 3, [(7 * i) % 101 for i in range(N)], [(i * 7) % (N + 3) if i % 5 else -1 for i in range(N)])
 
 
+def test_step_positions_past_every_sequence(dev):
+    """Positions whose sums would pass 64 bits are padding, in the step and in the write."""
+    k = torch.randn(3, 2, 1, D, dtype=torch.bfloat16, device=dev)
+    for far in (1 << 62, 2 ** 63 - 1, -2 ** 63):
+        at = torch.tensor([7, far, far - 1 if far > 0 else far], device=dev)
+        kc, vc = (torch.zeros(3, 12, 1, D, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        window_cache_write(k, k, kc, vc, 4, at)
+        assert kc[0].any() and vc[0].any()
+        if far == 1 << 62:                       # 2**62 - 1 is a position
+            assert kc[2].any() and not kc[1].any() and not vc[1].any()
+        else:
+            assert not kc[1:].any() and not vc[1:].any()
+        kc, vc = (torch.zeros(3, 12, 1, D, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        o = window_attention_step(k[:, 0], k[:, 0], k[:, 0], kc, vc, at, 6, 4)
+        assert o[0].any() and not o[1].any() and not kc[1].any() and not vc[1].any()
+        if far != 1 << 62:
+            assert not o[2].any() and not kc[2].any() and not vc[2].any()
+
+
 def test_step_far_position(dev):
     """A position past 2^32."""
     _step_case(dev, torch.bfloat16, 2, 2, 1, 2, 90, 60, 4, [(1 << 40) + 12345, 1 << 33], None, torch.int64)
@@ -501,3 +529,36 @@ def test_prefill_then_decode(dev, dtype):
         xi = {m: t[i:i + 1, :n + new].cpu() for m, t in (("q", q), ("k", k), ("v", v))}
         ref, size, score = _oracle(xi, [(0, 0, n + new)], W, S, D ** -0.5, None)
         _check(torch.cat([o[0, int(cu[i]):int(cu[i + 1])], *(y[i:i + 1] for y in outs)]), ref["o"][0], size["o"][0], score, n + new, "o")
+
+
+def test_offsets_past_32_bits(dev):
+    """Tokens 512 KiB apart, the last of them past 2^32 bytes and 2^31 elements; caches of more."""
+    T, H, Hkv, apart = 8300, 4, 2, 1 << 18
+    big = torch.empty(T * apart, dtype=torch.bfloat16, device=dev)
+    gen = torch.Generator(device=dev).manual_seed(3)
+    near, far = [], []
+    for i, h in enumerate((H, Hkv, Hkv, H)):
+        near.append(torch.randn(1, T, h, D, generator=gen, device=dev).to(torch.bfloat16))
+        far.append(big.as_strided((1, T, h, D), (0, apart, D, 1), 4096 * i).copy_(near[-1]))
+    out = []
+    for q, k, v, do in (near, far):
+        leaf = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = window_attention(*leaf, 300, 3)
+        out.append([o.detach(), *torch.autograd.grad(o, leaf, do)])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    slots = 305
+    wide = [big.as_strided((slots, 64, 1, D), (apart * 27, apart // 64, D, 1), 128 * i) for i in range(2)]
+    assert apart * 27 * (slots - 1) > 1 << 31
+    small = [torch.empty(2, 64, 1, D, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    at, pos = torch.tensor([slots - 1, 0], device=dev), torch.tensor([0, 0], device=dev)
+    tokens = [near[1][:, :80, :1].expand(2, -1, -1, -1), near[2][:, :80, :1].expand(2, -1, -1, -1)]
+    with torch.no_grad():
+        window_cache_write(*tokens, *small, 2, pos, None)
+        window_cache_write(*tokens, *wide, 2, pos, at)
+        for a, b in zip(small, wide):
+            assert torch.equal(a[0], b[slots - 1]) and torch.equal(a[1], b[0])
+        args = [t[0, :2] for t in (near[0], near[1][:, :, :1], near[2][:, :, :1])]
+        x = window_attention_step(*args, *small, pos + 80, 50, 2)
+        y = window_attention_step(*args, *wide, pos + 80, 50, 2, at)
+    assert torch.equal(x, y)
