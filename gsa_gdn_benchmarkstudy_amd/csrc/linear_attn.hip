@@ -9,11 +9,11 @@
 //   dk: rows V, keys dO, values Q, X = D^T, backwards;   dv: rows K, keys Q, values dO, X = D, backwards
 // (D_t = a D_{t+1} + scale q_t do_t^T from the gradient of the final state).  So one kernel (linear_scan_kernel) does all
 // four: a Pass names its operands, its direction and where scale goes.  dg = sum_t <D_t, a S_{t-1}> counts the decays
-// between each query i and key j, i - j of them, by positive terms alone (differences of sums over the sequence would cancel):
+// between each query i and key j, i - j of them, by positive terms alone (differences of sums over the sequence would cancel).
+// dq's pass does it, with X2, the state with each term times the tokens since its key (or since the segment's start):
 //   inside a chunk          sum_ij (i - j) P_ij (do_i . v_j)
-//   from the key's chunk    its tokens behind the key times the key's part of dk that comes from X
-//   to the query's chunk    its tokens up to the query times the query's part of dq that comes from X
-//   chunks in between       X2, the state with each term times the tokens of the chunks that it has crossed
+//   from earlier ones       q_i . ((i + 1) dq_i's part of X + the same of X2)
+//   to later segments       <D, X2> at the segment's end
 //
 // Long sequences of few heads are cut into segments: what each adds to the state from 0 (a pass of the same kernel without
 // outputs), the states between them (linear_join_kernel), all segments' outputs at once.
@@ -45,7 +45,7 @@ struct LinearArgs {
   Seqs s;
   int Hk, Hv, units, seg;                                    // units: heads of all sequences, or of all segments of seg chunks
   const float* g; int64_t g_sh;
-  float* dg_parts;                                           // [2][units]
+  float* dg_parts;                                           // [units]
   Outside outside;                                           // by the kOutside blocks behind the units (packed sequences)
   Pass pass[3];
 };
@@ -106,7 +106,7 @@ __device__ __forceinline__ void mma_rows_apart(floatx4 (&hi)[M], floatx4 (&lo)[M
 }
 
 // P enters a product with bf16 outputs in two parts
-template <typename T, int kDg, bool kDouble> struct LinearSizes {
+template <typename T, bool kDg, bool kDouble> struct LinearSizes {
   static constexpr int C = ChunkType<T>::kChunk, NP = ChunkType<T>::kParts;
   static constexpr int kPParts = NP == 1 ? 2 : 3, kXParts = NP == 1 && !kDg ? 2 : 3;
   static constexpr int kRows = (C / 16) * 4 * NP * kUnit, kP = Square<C>::kFrags * kPParts * kUnit, kStage = C * kHead * sizeof(T);
@@ -147,8 +147,8 @@ __device__ __forceinline__ void state_store(const floatx4 (&S)[8][1], float* p, 
     for (int r = 0; r < 4; ++r) p[(uint32_t)((8 * g + tile_at(t, r)) * kHead + col)] = S[t][0][r] * f;
 }
 
-// kOut: the outputs; otherwise what a segment adds to X.  kDg: this pass's part of dg: 1 dq's, 2 dk's.
-template <typename T, bool kOut, int kDg, bool kDouble>
+// kOut: the outputs; otherwise what a segment adds to X.  kDg: dq's pass, with dg.
+template <typename T, bool kOut, bool kDg, bool kDouble>
 __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, char* lds, float* dg_part) {
   using Z = LinearSizes<T, kDg, kDouble>;
   constexpr int C = Z::C, NP = Z::NP, MT = C / 16, JS = C / 32, kToEnd = kOut ? Z::kToEnd : 2 * Z::kRows;
@@ -176,10 +176,10 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
   const float g2 = log2_decay(a.g + h * a.g_sh);
   const int col = tile_row(wave, m);                         // this lane's column of the state and the outputs
 
-  floatx4 X[8][1], X2[kDg == 1 ? 8 : 1];
+  floatx4 X[8][1], X2[kDg ? 8 : 1];
 #pragma unroll
   for (int t = 0; t < 8; ++t) X[t][0] = floatx4{0.f, 0.f, 0.f, 0.f};
-  if constexpr (kDg == 1)
+  if constexpr (kDg)
 #pragma unroll
     for (int t = 0; t < 8; ++t) X2[t] = floatx4{0.f, 0.f, 0.f, 0.f};
   if (kOut) {
@@ -281,12 +281,12 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
           return NP == 1 ? hi[0] : hi[0] + lo[0];
         };
         floatx4 p = product(Z::kA, group + Z::kB), kv;
-        if constexpr (kDg == 1) kv = product(group + Z::kDot, group + Z::kV);
+        if constexpr (kDg) kv = product(group + Z::kDot, group + Z::kV);
         const int lh = here(l), i = tile_row(pt, lh & 15), j = 32 * (nt >> 1) + 4 * (nt & 1) + 8 * (lh >> 4);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           p[r] = j + r <= i ? p[r] * pd[k][r] : 0.f;
-          if constexpr (kDg == 1)
+          if constexpr (kDg)
             if (i < left) dg = __builtin_fmaf(p[r] * (float)(i - j - r), j + r < i ? kv[r] : 0.f, dg);
         }
         char* to = pm + Square<C>::at(pt, nt >> 1, false) * Z::kPParts * kUnit + 16 * lh + 8 * (nt & 1);
@@ -314,7 +314,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
           else mma_rows(to, p, r);
         };
         pair(X[2 * ks][0], X[2 * ks + 1][0], O, lo);
-        if constexpr (kDg == 1) pair(X2[2 * ks], X2[2 * ks + 1], O2, lo2);
+        if constexpr (kDg) pair(X2[2 * ks], X2[2 * ks + 1], O2, lo2);
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
@@ -323,7 +323,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
         float e = to_end[C + t];
         if (!lead) e = x.in_o * power(g2, t);
         float y[4];
-        if constexpr (kDg != 0) {                            // q or k of the lane's outputs
+        if constexpr (kDg) {                                // q of the lane's outputs
           const char* at = lds + group + Z::kDot + (i * 4 + (wave >> 1)) * NP * kUnit + 16 * rs + 8 * (wave & 1);
 #pragma unroll
           for (int r = 0; r < 4; ++r) y[r] = 0.f;
@@ -339,12 +339,10 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           if constexpr (Z::kXParts == 3) O[i][r] += lo[i][r];
-          if constexpr (kDg == 1) O2[i][r] += lo2[i][r];
+          if constexpr (kDg) O2[i][r] += lo2[i][r];
           O[i][r] *= e;
-          if constexpr (kDg == 1) {
+          if constexpr (kDg) {
             if (t < left) dg = __builtin_fmaf(y[r], __builtin_fmaf(O[i][r], (float)(t + 1), O2[i][r] * e), dg);
-          } else if constexpr (kDg == 2) {
-            if (t < left) dg = __builtin_fmaf(y[r], O[i][r] * (float)t, dg);
           }
         }
       }
@@ -425,7 +423,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
 
     // the values times the decay to the chunk's end
     asm volatile("" ::: "memory");                           // (read again: kept over P V they would cost registers)
-    Parts<3> vd[JS];
+    Parts<3> vd[JS], vd2[kDg ? JS : 1];
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
       const Parts<NP> v = cols_of<NP>(lds + group + Z::kV, wave, js, place);
@@ -442,34 +440,40 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] *= element(v, e);
       vd[js] = split3(y);
+      if constexpr (kDg) {                                   // and that times the tokens to there
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] *= (float)max(0, left - 1 - (32 * js + 8 * g + e));
+        vd2[js] = split3(y);
+      }
     }
 
     // X
     constexpr int kSome = 2;
-    constexpr bool kApart = NP == 3 || kDg != 0;
+    constexpr bool kApart = NP == 3 || kDg;
 #pragma unroll
     for (int t = 0; t < 8; t += kSome) {
-      floatx4 hi[kSome][1], lo[kSome][1];
+      floatx4 hi[kSome][1], lo[kSome][1], hi2[kSome][1], lo2[kSome][1];
 #pragma unroll
-      for (int i = 0; i < kSome; ++i) hi[i][0] = lo[i][0] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < kSome; ++i) hi[i][0] = lo[i][0] = hi2[i][0] = lo2[i][0] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int js = 0; js < JS; ++js) {
         Parts<NP> k[kSome];
 #pragma unroll
         for (int i = 0; i < kSome; ++i) k[i] = cols_of<NP>(lds + group + Z::kB, t + i, js, place);
         mma_apart(hi, kApart ? lo : hi, k, vd[js]);
+        if constexpr (kDg) mma_apart(hi2, lo2, k, vd2[js]);
       }
 #pragma unroll
       for (int i = 0; i < kSome; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if constexpr (kDg == 1) X2[t + i][r] = whole * __builtin_fmaf(X[t + i][0][r], (float)left, X2[t + i][r]);
+          if constexpr (kDg) X2[t + i][r] = __builtin_fmaf(__builtin_fmaf(X[t + i][0][r], (float)left, X2[t + i][r]), whole, hi2[i][0][r] + lo2[i][0][r]);
           X[t + i][0][r] = __builtin_fmaf(X[t + i][0][r], whole, kApart ? hi[i][0][r] + lo[i][0][r] : hi[i][0][r]);
         }
 #pragma unroll
       for (int i = 0; i < kSome; ++i) {                      // here, not where X is used next: the sums would be kept until then
         asm volatile("" : "+v"(X[t + i][0]));
-        if constexpr (kDg == 1) asm volatile("" : "+v"(X2[t + i]));
+        if constexpr (kDg) asm volatile("" : "+v"(X2[t + i]));
       }
     }
     __syncthreads();                                         // B, V, dot and P are free; the outputs are staged
@@ -495,7 +499,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
     state_store(X, x.add + gn, 1.f, g, col);
   } else {
     if (ends && x.last) state_store(X, x.last + sn, x.back ? power(g2, chunks ? 1 : 0) : 1.f, g, col);
-    if constexpr (kDg == 1) {
+    if constexpr (kDg) {
       const float* far = last ? (x.far_first ? x.far_first + sn : nullptr) : x.far + gn;
       if (far) {
         state_load(X, far, x.turn, g, col);
@@ -506,7 +510,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
           for (int r = 0; r < 4; ++r) dg = __builtin_fmaf(X[t][0][r] * f, X2[t][r], dg);
       }
     }
-    if constexpr (kDg != 0) {
+    if constexpr (kDg) {
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) dg += __shfl_xor(dg, o, 64);
       __syncthreads();
@@ -525,7 +529,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
 // kPerSimd 4: two blocks share a CU and cover each other's waits; 2: one, the next chunk's operands on their way (bf16)
 template <typename T, int kPerSimd> constexpr bool kTwice = sizeof(T) == 2 && kPerSimd == 2;
 
-template <typename T, bool kOut, int kDg, int kPerSimd>
+template <typename T, bool kOut, bool kDg, int kPerSimd>
 __global__ __launch_bounds__(64 * kWaves, kPerSimd) void linear_scan_kernel(LinearArgs a) {
   extern __shared__ __align__(16) char lds[];
   const int which = blockIdx.y;
@@ -533,12 +537,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerSimd) void linear_scan_kernel(Line
     if (which == 0) clear_outside(a.outside, blockIdx.x - a.units, kOutside);
     return;
   }
-  if constexpr (kDg != 0) {
-    if (which == 0) linear_scan<T, kOut, 1, kTwice<T, kPerSimd>>(a, a.pass[0], lds, a.dg_parts + blockIdx.x);
-    else linear_scan<T, kOut, 2, kTwice<T, kPerSimd>>(a, a.pass[1], lds, a.dg_parts + a.units + blockIdx.x);
-  } else {
-    linear_scan<T, kOut, 0, kTwice<T, kPerSimd>>(a, a.pass[which], lds, nullptr);
-  }
+  linear_scan<T, kOut, kDg, kTwice<T, kPerSimd>>(a, a.pass[which], lds, kDg ? a.dg_parts + blockIdx.x : nullptr);
 }
 
 // X before each segment but the pass's first from what the segments add: 256 threads, 1024 elements of a head's state.
@@ -580,7 +579,7 @@ __global__ __launch_bounds__(256) void linear_dg_kernel(const float* parts, int 
   __shared__ double red[256];
   const int h = blockIdx.x;
   double s = 0.;
-  for (int i = threadIdx.x; i < 2 * (units / Hv); i += 256) s += parts[(int64_t)i * Hv + h];
+  for (int i = threadIdx.x; i < units / Hv; i += 256) s += parts[(int64_t)i * Hv + h];
   red[threadIdx.x] = s;
   __syncthreads();
   for (int o = 128; o; o >>= 1) {
@@ -647,23 +646,23 @@ LinearPlan linear_plan(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   }
   z.units = z.seg ? z.segs * Hv : heads;
   z.states = (size_t)z.segs * Hv * 128 * 128 * 4;
-  z.dg = up(2 * z.units * 4);
+  z.dg = up(z.units * 4);
   z.parts = Hv > Hk ? (size_t)B * T * Hv * 128 * 4 : 0;
   return z;
 }
 
-template <typename T, bool kOut, int kDg, int kPerSimd> int launch_linear(const gsa::LinearArgs& a, int passes, hipStream_t s) {
+template <typename T, bool kOut, bool kDg, int kPerSimd> int launch_linear(const gsa::LinearArgs& a, int passes, hipStream_t s) {
   using Z = gsa::LinearSizes<T, kDg, gsa::kTwice<T, kPerSimd>>;
   constexpr size_t lds = kOut ? Z::kBytes : Z::kState;
   static_assert(lds * (kPerSimd / 2) <= 160 * 1024);
   if (const int e = allow_lds<gsa::linear_scan_kernel<T, kOut, kDg, kPerSimd>>(lds)) return e;
-  hipLaunchKernelGGL((gsa::linear_scan_kernel<T, kOut, kDg, kPerSimd>), dim3(a.units + (kOut && a.s.cu ? gsa::kOutside : 0), passes), dim3(64 * gsa::kWaves), lds, s, a);
+  hipLaunchKernelGGL((gsa::linear_scan_kernel<T, kOut, kDg, kPerSimd>), dim3(a.units + (kOut && a.outside.s.cu ? gsa::kOutside : 0), passes), dim3(64 * gsa::kWaves), lds, s, a);
   return launch_status();
 }
 // X between the segments of a.pass[0]: what each adds, then their join.
 template <typename T> int launch_segments(const gsa::LinearArgs& a, const LinearPlan& z, hipStream_t s) {
   if (!z.seg) return GSA_OK;
-  if (const int e = launch_linear<T, false, 0, sizeof(T) == 2 ? 4 : 2>(a, 1, s)) return e;
+  if (const int e = launch_linear<T, false, false, sizeof(T) == 2 ? 4 : 2>(a, 1, s)) return e;
   hipLaunchKernelGGL(gsa::linear_join_kernel, dim3(a.s.N * a.Hv, 16), dim3(256), 0, s, a, z.C);
   return launch_status();
 }
@@ -720,7 +719,7 @@ template <typename T> int linear_forward(const gsa_linear_args* x, gsa::LinearAr
   p.last = x->state_out;
   if (const int e = launch_segments<T>(a, z, s)) return e;
   a.outside = {a.s, {(char*)x->o}, {a.Hv * 128 * (int64_t)sizeof(T)}};
-  return launch_linear<T, true, 0, sizeof(T) == 2 ? 4 : 2>(a, 1, s);
+  return launch_linear<T, true, false, sizeof(T) == 2 ? 4 : 2>(a, 1, s);
 }
 
 template <typename T> int linear_backward(const gsa_linear_args* x, gsa::LinearArgs& a, const LinearPlan& z, hipStream_t s) {
@@ -742,7 +741,7 @@ template <typename T> int linear_backward(const gsa_linear_args* x, gsa::LinearA
   dq.far = init;
   dq.out = parts ? (void*)dqp : x->dq;
   dq.out_parts = parts;
-  dk.a = v; dk.b = dout; dk.v = q; dk.dot = k;
+  dk.a = v; dk.b = dout; dk.v = q;
   dk.v_shared = dk.turn = dk.back = 1;
   dk.in_p = dk.in_x = x->scale;
   dk.in_o = 1.f;
@@ -761,19 +760,17 @@ template <typename T> int linear_backward(const gsa_linear_args* x, gsa::LinearA
   dv.add = add;
   a.pass[0] = dv;
   if (const int e = launch_segments<T>(a, z, s)) return e;
-  a.pass[0] = dq;
-  a.pass[1] = dk;
-  a.pass[2] = dv;
+  a.pass[0] = dk;
+  a.pass[1] = dv;
+  a.pass[2] = dq;
   const int64_t row = 128 * (int64_t)(parts ? 4 * a.Hv : sizeof(T) * a.Hk);
   a.outside = {a.s, {(char*)dq.out, (char*)dk.out, (char*)x->dv}, {row, row, a.Hv * 128 * (int64_t)sizeof(T)}};
-  int e;
-  constexpr int kPerSimd = sizeof(T) == 2 ? 4 : 2;
-  if (x->dg) {                                               // dv goes by itself: without dg two blocks share a CU
-    if ((e = launch_linear<T, true, 1, 2>(a, 2, s))) return e;
-    a.pass[0] = dv;
-    e = launch_linear<T, true, 0, kPerSimd>(a, 1, s);
-  } else {
-    e = launch_linear<T, true, 0, kPerSimd>(a, 3, s);
+  int e = launch_linear<T, true, false, sizeof(T) == 2 ? 4 : 2>(a, x->dg ? 2 : 3, s);
+  if (e) return e;
+  if (x->dg) {                                               // dq by itself: more registers, so one block a CU
+    a.pass[0] = dq;
+    a.outside = gsa::Outside{};
+    e = launch_linear<T, true, true, 2>(a, 1, s);
   }
   if (e) return e;
   if (x->dg) {
