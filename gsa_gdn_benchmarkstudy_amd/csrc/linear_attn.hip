@@ -115,7 +115,7 @@ template <typename T, bool kDg, bool kDouble> struct LinearSizes {
   static constexpr int kAtP = kA + kRows, kAtStage = kAtP + kP;
   // powers of the decay: in_x a^(C-1-t), in_o a^(t+1)
   static constexpr int kToEnd = kAtStage + kStage, kFromX = kToEnd + 4 * C;
-  static constexpr size_t kBytes = kFromX + 4 * C, kState = 2 * kRows + 4 * C;
+  static constexpr size_t kBytes = kFromX + 4 * C, kState = kA + 4 * C;
 };
 
 template <int N> __device__ __forceinline__ float element(const Parts<N>& x, int e) {
@@ -151,7 +151,7 @@ __device__ __forceinline__ void state_store(const floatx4 (&S)[8][1], float* p, 
 template <typename T, bool kOut, bool kDg, bool kDouble>
 __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, char* lds, float* dg_part) {
   using Z = LinearSizes<T, kDg, kDouble>;
-  constexpr int C = Z::C, NP = Z::NP, MT = C / 16, JS = C / 32, kToEnd = kOut ? Z::kToEnd : 2 * Z::kRows;
+  constexpr int C = Z::C, NP = Z::NP, MT = C / 16, JS = C / 32, kToEnd = kOut ? Z::kToEnd : Z::kA;
   const uint32_t base = lds_addr(lds);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id(), g = l >> 4, m = l & 15;
   const int slot = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, hk = h / (a.Hv / a.Hk);
@@ -248,18 +248,22 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
     fetch(x.v, x.v_shared, c, to + Z::kV, lane_v);
     if (kDg) fetch(x.dot, 1, c, to + Z::kDot, lane_dot);
   };
+  constexpr bool kLater = kOut && NP == 1 && !kDouble;       // V's loads, the last two, land beside P and A X
   int group = 0;                                             // this chunk's, bytes from lds
   if (c0 < c1) {
-    fetch_group(c, 0);
     if (kOut) fetch(x.a, x.a_shared, c, Z::kA, lane_a);
+    fetch_group(c, 0);
   }
+  if (kLater) wait_loads();
   for (int n = c0; n < c1; ++n, c += step) {
     const bool more = n + 1 < c1;
     const int left = min(C, sp.len - c * C);
     // steps of decay from X to the chunk's first token: 1, or (the gradient of the final state) 0
     const int lead = x.back && c == chunks - 1 ? 0 : 1;
     const float whole = power(g2, left - 1 + lead);
-    wait_loads();
+    if (kLater) __builtin_amdgcn_s_waitcnt(kWaitVmcnt0 + 2);
+    else wait_loads();
+    asm volatile("" ::: "memory");
     __syncthreads();
     if (kDouble && more) fetch_group(c + step, Z::kGroup - group);
 
@@ -346,6 +350,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
           }
         }
       }
+      if (kLater) wait_loads();
       __syncthreads();                                       // P is there; A is free
       if (more) fetch(x.a, x.a_shared, c + step, Z::kA, lane_a);
     }
@@ -476,9 +481,10 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
         if constexpr (kDg) asm volatile("" : "+v"(X2[t + i]));
       }
     }
-    __syncthreads();                                         // B, V, dot and P are free; the outputs are staged
+    if (kOut || !kDouble) __syncthreads();                   // B, V, dot and P are free; the outputs are staged
     if constexpr (kDouble) group = Z::kGroup - group;
-    else if (more) fetch_group(c + step, 0);
+    else if (more && !kLater) fetch_group(c + step, 0);
+    else if (more) fetch(x.b, x.b_shared, c + step, Z::kB, lane_b);
     if constexpr (kOut) {
       if (!x.out_parts) {
         constexpr int kPer = 16 / sizeof(T), kPieces = kHead / kPer;
@@ -494,6 +500,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
         }
       }
     }
+    if (kLater && more) fetch(x.v, x.v_shared, c + step, Z::kV, lane_v);
   }
   if constexpr (!kOut) {
     state_store(X, x.add + gn, 1.f, g, col);
@@ -527,7 +534,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
 }
 
 // kPerSimd 4: two blocks share a CU and cover each other's waits; 2: one, the next chunk's operands on their way (bf16)
-template <typename T, int kPerSimd> constexpr bool kTwice = sizeof(T) == 2 && kPerSimd == 2;
+template <typename T, bool kOut, int kPerSimd> constexpr bool kTwice = sizeof(T) == 2 && (!kOut || kPerSimd == 2);
 
 template <typename T, bool kOut, bool kDg, int kPerSimd>
 __global__ __launch_bounds__(64 * kWaves, kPerSimd) void linear_scan_kernel(LinearArgs a) {
@@ -537,7 +544,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerSimd) void linear_scan_kernel(Line
     if (which == 0) clear_outside(a.outside, blockIdx.x - a.units, kOutside);
     return;
   }
-  linear_scan<T, kOut, kDg, kTwice<T, kPerSimd>>(a, a.pass[which], lds, kDg ? a.dg_parts + blockIdx.x : nullptr);
+  linear_scan<T, kOut, kDg, kTwice<T, kOut, kPerSimd>>(a, a.pass[which], lds, kDg ? a.dg_parts + blockIdx.x : nullptr);
 }
 
 // X before each segment but the pass's first from what the segments add: 256 threads, 1024 elements of a head's state.
@@ -652,7 +659,7 @@ LinearPlan linear_plan(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
 }
 
 template <typename T, bool kOut, bool kDg, int kPerSimd> int launch_linear(const gsa::LinearArgs& a, int passes, hipStream_t s) {
-  using Z = gsa::LinearSizes<T, kDg, gsa::kTwice<T, kPerSimd>>;
+  using Z = gsa::LinearSizes<T, kDg, gsa::kTwice<T, kOut, kPerSimd>>;
   constexpr size_t lds = kOut ? Z::kBytes : Z::kState;
   static_assert(lds * (kPerSimd / 2) <= 160 * 1024);
   if (const int e = allow_lds<gsa::linear_scan_kernel<T, kOut, kDg, kPerSimd>>(lds)) return e;
