@@ -234,8 +234,9 @@ __device__ __forceinline__ int here(int x) {
 }
 // All loads have landed, the direct ones to LDS too, and the compiler knows it: waits of its own for registers loaded before a
 // loop would stand inside it, where they wait for the next tile's direct loads, which it does not count.
-__device__ __forceinline__ void wait_loads() {
-  __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+// kLeft: but for the last so many.
+template <int kLeft = 0> __device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(kWaitVmcnt0 + kLeft);
   asm volatile("" ::: "memory");
 }
 

@@ -105,16 +105,19 @@ __device__ __forceinline__ void mma_rows_apart(floatx4 (&hi)[M], floatx4 (&lo)[M
           }
 }
 
+// What of the next chunk is on its way beside a chunk's products (direct loads: bf16): nothing, its keys, all of it
+enum Ahead { kNothing, kKeys, kAll };
+
 // P enters a product with bf16 outputs in two parts
-template <typename T, bool kDg, bool kDouble> struct LinearSizes {
+template <typename T, bool kDg, Ahead kAhead> struct LinearSizes {
   static constexpr int C = ChunkType<T>::kChunk, NP = ChunkType<T>::kParts;
   static constexpr int kPParts = NP == 1 ? 2 : 3, kXParts = NP == 1 && !kDg ? 2 : 3;
-  static constexpr int kRows = (C / 16) * 4 * NP * kUnit, kP = Square<C>::kFrags * kPParts * kUnit, kStage = C * kHead * sizeof(T);
-  // keys, values and dot, twice with kDouble; rows, P, the outputs on their way out
-  static constexpr int kB = 0, kV = kRows, kDot = 2 * kRows, kGroup = (kDg ? 3 : 2) * kRows, kA = (kDouble ? 2 : 1) * kGroup;
-  static constexpr int kAtP = kA + kRows, kAtStage = kAtP + kP;
+  static constexpr int kRows = (C / 16) * 4 * NP * kUnit, kP = Square<C>::kFrags * kPParts * kUnit;
+  // keys, values and dot (what goes ahead twice, kGroup apart); rows, P
+  static constexpr int kB = 0, kV = (kAhead == kKeys ? 2 : 1) * kRows, kDot = 2 * kRows, kGroup = (kAhead == kKeys ? 1 : kDg ? 3 : 2) * kRows;
+  static constexpr int kA = kAhead == kKeys ? kV + kRows : (kAhead == kAll ? 2 : 1) * kGroup, kAtP = kA + kRows;
   // powers of the decay: in_x a^(C-1-t), in_o a^(t+1)
-  static constexpr int kToEnd = kAtStage + kStage, kFromX = kToEnd + 4 * C;
+  static constexpr int kToEnd = kAtP + kP, kFromX = kToEnd + 4 * C;
   static constexpr size_t kBytes = kFromX + 4 * C, kState = kA + 4 * C;
 };
 
@@ -148,9 +151,9 @@ __device__ __forceinline__ void state_store(const floatx4 (&S)[8][1], float* p, 
 }
 
 // kOut: the outputs; otherwise what a segment adds to X.  kDg: dq's pass, with dg.
-template <typename T, bool kOut, bool kDg, bool kDouble>
+template <typename T, bool kOut, bool kDg, Ahead kAhead>
 __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, char* lds, float* dg_part) {
-  using Z = LinearSizes<T, kDg, kDouble>;
+  using Z = LinearSizes<T, kDg, kAhead>;
   constexpr int C = Z::C, NP = Z::NP, MT = C / 16, JS = C / 32, kToEnd = kOut ? Z::kToEnd : Z::kA;
   const uint32_t base = lds_addr(lds);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id(), g = l >> 4, m = l & 15;
@@ -248,24 +251,24 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
     fetch(x.v, x.v_shared, c, to + Z::kV, lane_v);
     if (kDg) fetch(x.dot, 1, c, to + Z::kDot, lane_dot);
   };
-  constexpr bool kLater = kOut && NP == 1 && !kDouble;       // V's loads, the last two, land beside P and A X
-  int group = 0;                                             // this chunk's, bytes from lds
+  int group = 0;                                             // this chunk's keys (kAll: and values), bytes from lds
   if (c0 < c1) {
     if (kOut) fetch(x.a, x.a_shared, c, Z::kA, lane_a);
-    fetch_group(c, 0);
+    if (kAhead == kKeys) fetch(x.b, x.b_shared, c, Z::kB, lane_b);
+    else fetch_group(c, 0);
   }
-  if (kLater) wait_loads();
   for (int n = c0; n < c1; ++n, c += step) {
     const bool more = n + 1 < c1;
     const int left = min(C, sp.len - c * C);
     // steps of decay from X to the chunk's first token: 1, or (the gradient of the final state) 0
     const int lead = x.back && c == chunks - 1 ? 0 : 1;
     const float whole = power(g2, left - 1 + lead);
-    if (kLater) __builtin_amdgcn_s_waitcnt(kWaitVmcnt0 + 2);
-    else wait_loads();
-    asm volatile("" ::: "memory");
+    wait_loads();
     __syncthreads();
-    if (kDouble && more) fetch_group(c + step, Z::kGroup - group);
+    const int vals = (kAhead == kKeys ? 0 : group) + Z::kV;
+    if (kAhead == kKeys) fetch(x.v, x.v_shared, c, Z::kV, lane_v);         // needed behind P and A X
+    if (kAhead == kKeys && more) fetch(x.b, x.b_shared, c + step, Z::kGroup - group, lane_b);
+    if (kAhead == kAll && more) fetch_group(c + step, Z::kGroup - group);
 
     floatx4 O[MT];                                           // O[i][r]: token tile_row(i, m), element col4 + r
     const int col4 = 32 * (wave >> 1) + 4 * (wave & 1);      // (and 8 g)
@@ -285,7 +288,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
           return NP == 1 ? hi[0] : hi[0] + lo[0];
         };
         floatx4 p = product(Z::kA, group + Z::kB), kv;
-        if constexpr (kDg) kv = product(group + Z::kDot, group + Z::kV);
+        if constexpr (kDg) kv = product(group + Z::kDot, vals);
         const int lh = here(l), i = tile_row(pt, lh & 15), j = 32 * (nt >> 1) + 4 * (nt & 1) + 8 * (lh >> 4);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -350,7 +353,8 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
           }
         }
       }
-      if (kLater) wait_loads();
+      if (kAhead == kKeys && more) wait_loads<2>();          // (the next keys' two)
+      else if (kAhead == kKeys) wait_loads();
       __syncthreads();                                       // P is there; A is free
       if (more) fetch(x.a, x.a_shared, c + step, Z::kA, lane_a);
     }
@@ -362,7 +366,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
       float odd = 0.f;
 #pragma unroll
       for (int js = 0; js < JS; ++js) {
-        v[js] = cols_of<NP>(lds + group + Z::kV, wave, js, place);
+        v[js] = cols_of<NP>(lds + vals, wave, js, place);
         // (times 0, added: v_dot2c_f32_bf16; the first part of an fp32 value is not finite where the value is not)
 #pragma unroll
         for (int e = 0; e < 8; e += 2)
@@ -413,15 +417,22 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
           if (at < left) *reinterpret_cast<floatx4*>(to + (int64_t)(x.back ? left - 1 - at : at) * a.Hv * kHead + e) = O[i];
         }
       } else {
-        // row t of the stage has its 16-byte unit u in place u ^ turn(t), which the lanes of a tile have each their own of
-        char* stage = lds + Z::kAtStage + t * kHead * (int)sizeof(T);
+        const int64_t row0 = (int64_t)sp.b * a.s.T + sp.t0 + (int64_t)c * C, st = (int64_t)a.Hv * kHead;
+        T* to = const_cast<T*>(uniform(static_cast<T*>(x.out) + (row0 * a.Hv + h) * kHead));
+        auto store = [&](T* at, int i) {
+          if constexpr (NP == 1) *reinterpret_cast<uint2*>(at) = uint2{pack_bf16(O[i][0], O[i][1]), pack_bf16(O[i][2], O[i][3])};
+          else *reinterpret_cast<floatx4*>(at) = O[i];
+        };
+        if (left == C) {
+          const uint32_t lane = (uint32_t)(x.back ? 31 - t : t) * (uint32_t)st + e;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          char* to = stage + tile_at(i, 0) * kHead * (int)sizeof(T);
-          if constexpr (NP == 1)
-            *reinterpret_cast<uint2*>(to + 16 * ((e >> 3) ^ (lh & 15)) + 2 * (e & 7)) = uint2{pack_bf16(O[i][0], O[i][1]), pack_bf16(O[i][2], O[i][3])};
-          else
-            *reinterpret_cast<floatx4*>(to + 16 * ((e >> 2) ^ (lh & 15))) = O[i];
+          for (int i = 0; i < MT; ++i) store(to + (x.back ? C - 32 - tile_at(i, 0) : tile_at(i, 0)) * st + lane, i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const int at = t + tile_at(i, 0);
+            if (at < left) store(to + (x.back ? left - 1 - at : at) * st + e, i);
+          }
         }
       }
     }
@@ -431,7 +442,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
     Parts<3> vd[JS], vd2[kDg ? JS : 1];
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
-      const Parts<NP> v = cols_of<NP>(lds + group + Z::kV, wave, js, place);
+      const Parts<NP> v = cols_of<NP>(lds + vals, wave, js, place);
       float y[8];
       if (left == C) {
         load8(to_end + 32 * js + 8 * g, y);
@@ -481,26 +492,12 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
         if constexpr (kDg) asm volatile("" : "+v"(X2[t + i]));
       }
     }
-    if (kOut || !kDouble) __syncthreads();                   // B, V, dot and P are free; the outputs are staged
-    if constexpr (kDouble) group = Z::kGroup - group;
-    else if (more && !kLater) fetch_group(c + step, 0);
-    else if (more) fetch(x.b, x.b_shared, c + step, Z::kB, lane_b);
-    if constexpr (kOut) {
-      if (!x.out_parts) {
-        constexpr int kPer = 16 / sizeof(T), kPieces = kHead / kPer;
-        const int64_t row0 = (int64_t)sp.b * a.s.T + sp.t0 + (int64_t)c * C;
-        T* to = const_cast<T*>(uniform(static_cast<T*>(x.out) + (row0 * a.Hv + h) * kHead));
-#pragma unroll
-        for (int i = 0; i < C * kPieces / (64 * kWaves); ++i) {
-          const int u = here(tid) + 64 * kWaves * i, t = u / kPieces;
-          const int turn = (t & 3) | (t >> 3 & 3) << 2;
-          const u32x4 y = *reinterpret_cast<const u32x4*>(lds + Z::kAtStage + 16 * (u ^ turn));
-          if (t < left)
-            *reinterpret_cast<u32x4*>(to + (int64_t)(x.back ? left - 1 - t : t) * a.Hv * kHead + kPer * (u % kPieces)) = y;
-        }
-      }
+    if constexpr (kAhead != kNothing) {
+      group = Z::kGroup - group;
+    } else {
+      __syncthreads();                                       // B, V, dot and P are free
+      if (more) fetch_group(c + step, 0);
     }
-    if (kLater && more) fetch(x.v, x.v_shared, c + step, Z::kV, lane_v);
   }
   if constexpr (!kOut) {
     state_store(X, x.add + gn, 1.f, g, col);
@@ -533,18 +530,20 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
   }
 }
 
-// kPerSimd 4: two blocks share a CU and cover each other's waits; 2: one, the next chunk's operands on their way (bf16)
-template <typename T, bool kOut, int kPerSimd> constexpr bool kTwice = sizeof(T) == 2 && (!kOut || kPerSimd == 2);
+// bf16: two blocks share a CU (kPerSimd 4) and cover each other's waits; dq with dg one, for its registers.  All of the next
+// chunk where LDS has room for it.
+template <typename T, bool kOut, bool kDg> constexpr int kPerSimd = sizeof(T) == 2 && !kDg ? 4 : 2;
+template <typename T, bool kOut, bool kDg> constexpr Ahead kAheadOf = sizeof(T) == 4 ? kNothing : kOut && !kDg ? kKeys : kAll;
 
-template <typename T, bool kOut, bool kDg, int kPerSimd>
-__global__ __launch_bounds__(64 * kWaves, kPerSimd) void linear_scan_kernel(LinearArgs a) {
+template <typename T, bool kOut, bool kDg>
+__global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, kOut, kDg>)) void linear_scan_kernel(LinearArgs a) {
   extern __shared__ __align__(16) char lds[];
   const int which = blockIdx.y;
   if ((int)blockIdx.x >= a.units) {
     if (which == 0) clear_outside(a.outside, blockIdx.x - a.units, kOutside);
     return;
   }
-  linear_scan<T, kOut, kDg, kTwice<T, kOut, kPerSimd>>(a, a.pass[which], lds, kDg ? a.dg_parts + blockIdx.x : nullptr);
+  linear_scan<T, kOut, kDg, kAheadOf<T, kOut, kDg>>(a, a.pass[which], lds, kDg ? a.dg_parts + blockIdx.x : nullptr);
 }
 
 // X before each segment but the pass's first from what the segments add: 256 threads, 1024 elements of a head's state.
@@ -658,18 +657,18 @@ LinearPlan linear_plan(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   return z;
 }
 
-template <typename T, bool kOut, bool kDg, int kPerSimd> int launch_linear(const gsa::LinearArgs& a, int passes, hipStream_t s) {
-  using Z = gsa::LinearSizes<T, kDg, gsa::kTwice<T, kOut, kPerSimd>>;
+template <typename T, bool kOut, bool kDg> int launch_linear(const gsa::LinearArgs& a, int passes, hipStream_t s) {
+  using Z = gsa::LinearSizes<T, kDg, gsa::kAheadOf<T, kOut, kDg>>;
   constexpr size_t lds = kOut ? Z::kBytes : Z::kState;
-  static_assert(lds * (kPerSimd / 2) <= 160 * 1024);
-  if (const int e = allow_lds<gsa::linear_scan_kernel<T, kOut, kDg, kPerSimd>>(lds)) return e;
-  hipLaunchKernelGGL((gsa::linear_scan_kernel<T, kOut, kDg, kPerSimd>), dim3(a.units + (kOut && a.outside.s.cu ? gsa::kOutside : 0), passes), dim3(64 * gsa::kWaves), lds, s, a);
+  static_assert(lds * (gsa::kPerSimd<T, kOut, kDg> / 2) <= 160 * 1024);
+  if (const int e = allow_lds<gsa::linear_scan_kernel<T, kOut, kDg>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::linear_scan_kernel<T, kOut, kDg>), dim3(a.units + (kOut && a.outside.s.cu ? gsa::kOutside : 0), passes), dim3(64 * gsa::kWaves), lds, s, a);
   return launch_status();
 }
 // X between the segments of a.pass[0]: what each adds, then their join.
 template <typename T> int launch_segments(const gsa::LinearArgs& a, const LinearPlan& z, hipStream_t s) {
   if (!z.seg) return GSA_OK;
-  if (const int e = launch_linear<T, false, false, sizeof(T) == 2 ? 4 : 2>(a, 1, s)) return e;
+  if (const int e = launch_linear<T, false, false>(a, 1, s)) return e;
   hipLaunchKernelGGL(gsa::linear_join_kernel, dim3(a.s.N * a.Hv, 16), dim3(256), 0, s, a, z.C);
   return launch_status();
 }
@@ -726,7 +725,7 @@ template <typename T> int linear_forward(const gsa_linear_args* x, gsa::LinearAr
   p.last = x->state_out;
   if (const int e = launch_segments<T>(a, z, s)) return e;
   a.outside = {a.s, {(char*)x->o}, {a.Hv * 128 * (int64_t)sizeof(T)}};
-  return launch_linear<T, true, false, sizeof(T) == 2 ? 4 : 2>(a, 1, s);
+  return launch_linear<T, true, false>(a, 1, s);
 }
 
 template <typename T> int linear_backward(const gsa_linear_args* x, gsa::LinearArgs& a, const LinearPlan& z, hipStream_t s) {
@@ -772,12 +771,12 @@ template <typename T> int linear_backward(const gsa_linear_args* x, gsa::LinearA
   a.pass[2] = dq;
   const int64_t row = 128 * (int64_t)(parts ? 4 * a.Hv : sizeof(T) * a.Hk);
   a.outside = {a.s, {(char*)dq.out, (char*)dk.out, (char*)x->dv}, {row, row, a.Hv * 128 * (int64_t)sizeof(T)}};
-  int e = launch_linear<T, true, false, sizeof(T) == 2 ? 4 : 2>(a, x->dg ? 2 : 3, s);
+  int e = launch_linear<T, true, false>(a, x->dg ? 2 : 3, s);
   if (e) return e;
   if (x->dg) {                                               // dq by itself: more registers, so one block a CU
     a.pass[0] = dq;
     a.outside = gsa::Outside{};
-    e = launch_linear<T, true, true, 2>(a, 1, s);
+    e = launch_linear<T, true, true>(a, 1, s);
   }
   if (e) return e;
   if (x->dg) {
