@@ -54,32 +54,36 @@ __device__ __forceinline__ int perm(int m) { return (m & ~12) | (m & 4) << 1 | (
 
 template <typename T, int kN = WindowType<T>::kTile> struct Tile {
   static constexpr int NP = WindowType<T>::NP, N = kN, kPlane = N * 256, kBytes = NP * kPlane;
+  // Both readers hold addresses in LDS with the base (a multiple of 256 bytes) in them: what is left is the instruction's
+  // offset.  tile: the tile's place behind the base.
   // Operand with rows t0 + perm(l % 32): elements 16 ks + 8 (l / 32) .. + 7
   struct RowReader {
-    int at, x;
-    __device__ RowReader(int l) {
+    uint32_t at;
+    __device__ RowReader(uint32_t base, int l) {
       const int t = perm(l & 31);
-      at = t * 256;
-      x = 16 * (swizzle(t) ^ (l >> 5));
+      at = base + t * 256 + 16 * (swizzle(t) ^ (l >> 5));
+      asm("" : "+v"(at));                                    // (else the base is taken out again, and added for each read)
     }
-    __device__ Parts<NP> read(const char* tile, int t0, int ks) const {
+    __device__ Parts<NP> read(uint32_t tile, int t0, int ks) const {
       Parts<NP> r;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) r.p[i] = *reinterpret_cast<const bf16x8*>(tile + i * kPlane + t0 * 256 + at + ((32 * ks) ^ x));
+      for (int i = 0; i < NP; ++i)
+        r.p[i] = *(const __attribute__((address_space(3))) bf16x8*)((at ^ 32u * ks) + (tile + i * kPlane + t0 * 256));
       return r;
     }
   };
   // Operand with rows of elements 32 dt + l % 32: rows t0 + 8 (l / 32) .. + 7 of the tile summed over (ds_read_b64_tr_b16: of
   // 16 lanes, lane i names row i / 4, elements 4 (i % 4) .. + 3 of 16, and gets element i of the four rows)
   struct ColReader {
-    int at[2];
-    __device__ ColReader(int l) {
+    uint32_t at[2];
+    __device__ ColReader(uint32_t base, int l) {
       const int i = l & 15, z = (2 * (l >> 4 & 1) + ((i & 3) >> 1)) ^ (2 * (i >> 2) + (l >> 5));
-      const int row = (8 * (l >> 5) + (i >> 2)) * 256 + 8 * (i & 1);
+      const uint32_t row = base + (8 * (l >> 5) + (i >> 2)) * 256 + 8 * (i & 1);
       at[0] = row + 16 * z;
       at[1] = row + 16 * (z ^ 4);
+      asm("" : "+v"(at[0]), "+v"(at[1]));
     }
-    __device__ Parts<NP> read(const char* tile, int t0, int dt) const {
+    __device__ Parts<NP> read(uint32_t tile, int t0, int dt) const {
       Parts<NP> r;
 #pragma unroll
       for (int n = 0; n < NP; ++n) {
@@ -87,7 +91,7 @@ template <typename T, int kN = WindowType<T>::kTile> struct Tile {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-              tile + n * kPlane + t0 * 256 + 1024 * e + at[dt & 1] + 16 * ((dt & 2 ? 8 : 0) ^ (8 * e))));
+              at[dt & 1] + (tile + n * kPlane + t0 * 256 + 1024 * e + 16 * ((dt & 2 ? 8 : 0) ^ (8 * e)))));
         r.p[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
       }
       return r;
@@ -150,6 +154,17 @@ template <int NA, int NB> __device__ __forceinline__ void mma32(floatx16& acc, c
 #pragma unroll
       for (int j = 0; j < NB; ++j)
         if (i + j == o) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
+}
+// The schedule of a product of kMany instructions (bf16), each with an operand from LDS: kAhead reads on their way before each
+// (the compiler's own is one, and waits for it).
+template <int kAhead, int kMany> __device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+  for (int i = kAhead; i < kMany; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
 }
 __device__ __forceinline__ void zero(floatx16& x) {
 #pragma unroll
@@ -264,9 +279,9 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
   using L = typename Z::L;
   constexpr int NP = L::NP, N = L::N, kBuffers = Z::kBuffers, kBuffer = 2 * L::kBytes, kQueries = 32 * kGroups, kSplit = Z::kSplit;
   constexpr int kMine = N / 32 / kSplit;                     // products of 32 keys a tile and wave
-  extern __shared__ __align__(16) char lds[];
+  extern __shared__ __align__(1024) char lds[];
   const uint32_t base = lds_addr(lds);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), group = wave % kGroups, split = wave / kGroups;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), group = wave % kGroups, split = kSplit > 1 ? wave / kGroups : 0;
   const int slot = gridDim.x / a.H - 1 - blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hkv);
   int c;
   const Span sp = slot_of(a.s, slot, kQueries, c);
@@ -291,19 +306,19 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
   floatx16 o[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) zero(o[dt]);
-  const typename L::RowReader rows(l);
-  const typename L::ColReader cols(l);
+  const typename L::RowReader rows(base, l);
+  const typename L::ColReader cols(base, l);
   // softmax state of the lane's row, log2 domain: the reference m moves only when a tile's maximum exceeds it by more than
   // kLazy (the sums then stay below 2^8 times what they are, far from fp32's range)
   constexpr float kLazy = 8.f;
   float m = -__builtin_inff(), limit = m, minus = 0.f, sum = 0.f;
   auto step = [&](int t, auto which) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
     constexpr int buffer = kBuffers == 2 ? decltype(which)::value : 0;
-    char *K = lds + buffer * kBuffer, *V = K + L::kBytes;
+    constexpr uint32_t K = buffer * kBuffer, V = K + L::kBytes;
     if constexpr (NP == 3) {
       if (t) __syncthreads();                                // every wave is through with the last tile
-      lk.store(K, wave, l);
-      lv.store(V, wave, l);
+      lk.store(lds + K, wave, l);
+      lv.store(lds + V, wave, l);
     }
     wait_loads();
     __syncthreads();
@@ -317,6 +332,7 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
       zero(s);
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) mma32(s, rows.read(K, 32 * n, ks), q[ks]);
+      if constexpr (NP == 1) reads_ahead<4, 8>();
       if (see == 1) {
         const int lh = here(l), j = j0 + 8 * (lh >> 5);
 #pragma unroll
@@ -431,9 +447,9 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
   using L = typename Z::L;
   constexpr int NP = L::NP, N = L::N, kBuffers = Z::kBuffers, kBuffer = 2 * L::kBytes, kQueries = 32 * kGroups, kSplit = Z::kSplit;
   constexpr int kMine = N / 32 / kSplit;
-  extern __shared__ __align__(16) char lds[];
+  extern __shared__ __align__(1024) char lds[];
   const uint32_t base = lds_addr(lds);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), group = wave % kGroups, split = wave / kGroups;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), group = wave % kGroups, split = kSplit > 1 ? wave / kGroups : 0;
   const int slot = gridDim.x / a.H - 1 - blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hkv);
   int c;
   const Span sp = slot_of(a.s, slot, kQueries, c);
@@ -472,15 +488,15 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
   floatx16 acc[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) zero(acc[dt]);
-  const typename L::RowReader rows(l);
-  const typename L::ColReader cols(l);
+  const typename L::RowReader rows(base, l);
+  const typename L::ColReader cols(base, l);
   auto step = [&](int t, auto which) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
     constexpr int buffer = kBuffers == 2 ? decltype(which)::value : 0;
-    char *K = lds + buffer * kBuffer, *V = K + L::kBytes;
+    constexpr uint32_t K = buffer * kBuffer, V = K + L::kBytes;
     if constexpr (NP == 3) {
       if (t) __syncthreads();
-      lk.store(K, wave, l);
-      lv.store(V, wave, l);
+      lk.store(lds + K, wave, l);
+      lv.store(lds + V, wave, l);
     }
     wait_loads();
     __syncthreads();
@@ -494,9 +510,11 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
       zero(s);
       zero(p);
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) mma32(s, rows.read(K, 32 * n, ks), q[ks]);
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) mma32(p, rows.read(V, 32 * n, ks), d[ks]);
+      for (int ks = 0; ks < 8; ++ks) {
+        mma32(s, rows.read(K, 32 * n, ks), q[ks]);
+        mma32(p, rows.read(V, 32 * n, ks), d[ks]);
+      }
+      if constexpr (NP == 1) reads_ahead<6, 16>();
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, -lse)) * (p[r] - D);
       if (see == 1) {
@@ -574,7 +592,7 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
     if (i0 >= i1) return;
     parts = a.far_parts + (((int64_t)unit * a.far_first + block) * a.H + h0) * 2 * kKeys * kHead;
   }
-  const int group = wave % kGroups, split = wave / kGroups;
+  const int group = wave % kGroups, split = kSplit > 1 ? wave / kGroups : 0;
   const int j0 = k0 + 32 * group, key = j0 + (l & 31), keyc = min(key, sp.len - 1);
   const int tiles = (i1 - i0 + N - 1) / N, count = tiles * heads;
   typename L::Loader lq(a.q.st, wave, l), ld(a.dout.st, wave, l);
@@ -600,8 +618,8 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
     zero(dk[dt]);
     zero(dv[dt]);
   }
-  const typename L::RowReader rows(l);
-  const typename L::ColReader cols(l);
+  const typename L::RowReader rows(base, l);
+  const typename L::ColReader cols(base, l);
   for (int t = 0; t < count; ++t) {
     const int buffer = kBuffers == 2 ? t & 1 : 0;
     char *Q = lds + buffer * kBuffer, *dO = Q + L::kBytes;
@@ -622,13 +640,22 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
       const int i32 = r0 + 32 * n;                           // the 32 queries of this product
       const int see = i32 < i1 ? seen<32>(a, i32, j0) : 0;
       if (!see) continue;
+      // (for this product alone: kept over the loop, the 8 addresses of rows would cost registers)
+      typename L::RowReader r = rows;
+      typename L::ColReader c = cols;
+      const int shift = buffer * kBuffer + 32 * n * 256;
+      r.at = here(rows.at + shift);
+      c.at[0] = here(cols.at[0] + shift);
+      c.at[1] = here(cols.at[1] + shift);
       floatx16 s, p;
       zero(s);
       zero(p);
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) mma32(s, rows.read(Q, 32 * n, ks), k[ks]);
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) mma32(p, rows.read(dO, 32 * n, ks), v[ks]);
+      for (int ks = 0; ks < 8; ++ks) {
+        mma32(s, r.read(0, 0, ks), k[ks]);
+        mma32(p, r.read(L::kBytes, 0, ks), v[ks]);
+      }
+      if constexpr (NP == 1) reads_ahead<1, 16>();           // (more ahead would not fit the registers)
       asm volatile("" : "+v"(s), "+v"(p));
       const float* stats = st + 32 * n + 8 * (here(l) >> 5);
 #pragma unroll
@@ -644,11 +671,11 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
       if (see == 1 || i32 + 32 > i1) {
         const int lh = here(l), i = i32 + 8 * (lh >> 5), j = j0 + (lh & 31);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int ir = i + 16 * (r >> 3) + (r & 7);
+        for (int y = 0; y < 16; ++y) {
+          const int ir = i + 16 * (y >> 3) + (y & 7);
           const bool on = ir < i1 && visible(a, ir, j);
-          s[r] = on ? s[r] : 0.f;
-          p[r] = on ? p[r] : 0.f;
+          s[y] = on ? s[y] : 0.f;
+          p[y] = on ? p[y] : 0.f;
         }
       }
 #pragma unroll
@@ -656,8 +683,8 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
         const Parts<NP> w = parts_at<NP>(s, x), ds = parts_at<NP>(p, x);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) {
-          mma32(dv[dt], cols.read(dO, 32 * n + 16 * x, dt), w);
-          mma32(dk[dt], cols.read(Q, 32 * n + 16 * x, dt), ds);
+          mma32(dv[dt], c.read(L::kBytes, 16 * x, dt), w);
+          mma32(dk[dt], c.read(0, 16 * x, dt), ds);
         }
       }
     }
@@ -684,7 +711,7 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
 // (One kernel for both kinds of blocks would spill registers, and what reads those back waits for the tiles on their way.)
 template <typename T, int kGroups, bool kFarPart>
 __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_dkv_kernel(WindowArgs a) {
-  extern __shared__ __align__(16) char lds[];
+  extern __shared__ __align__(1024) char lds[];
   window_dkv<T, kGroups, kFarPart>(a, lds, blockIdx.x);
 }
 
