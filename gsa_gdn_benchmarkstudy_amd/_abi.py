@@ -174,7 +174,7 @@ _PROTOS = {
     "gsa_window_attn_backward": ([ctypes.POINTER(WindowArgs), _vp], _i32),
     "gsa_window_cache_write": ([_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i32,
                                 _vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp], _i32),
-    "gsa_window_step_workspace_bytes": ([_i32] * 5, ctypes.c_size_t),
+    "gsa_window_step_workspace_bytes": ([_i32] * 6, ctypes.c_size_t),
     "gsa_window_step": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
                          _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp, ctypes.c_size_t, _vp], _i32),
     "gsa_linear_step": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _i64, _i32, _i32, _i32,
@@ -1288,7 +1288,7 @@ def window_step(q, k, v, kc, vc, pos, idx, window: int, sinks: int, scale: float
     """gsa_window_step: o [N,H,128]; the caches are updated in place.  q, k, v as _rows16 gives them."""
     N, H, d = q.shape
     Hkv = kc.shape[2]
-    n = _window_step_bytes(N, H, Hkv, window, sinks)
+    n = _window_step_bytes(N, H, Hkv, window, sinks, dtype_code(q.dtype))
     o = torch.empty(N, H, d, device=q.device, dtype=q.dtype)
     ws = torch.empty(n, device=q.device, dtype=torch.uint8)
     kn, kh, vn, vh = (0, 0, 0, 0) if k is None else (*k.stride()[:2], *v.stride()[:2])

@@ -18,6 +18,16 @@
 // Long sequences of few heads are cut into segments: what each adds to the state from 0 (a pass of the same kernel without
 // outputs), the states between them (linear_join_kernel), all segments' outputs at once.
 //
+// A block takes a head: 8 waves of 16 columns of the state each, which stays in registers from chunk to chunk (tile_row: a
+// product's result is the next one's operand in the same lanes).  16384 tokens of 16 heads in bf16: state pass 36-39 us (134 MB,
+// 3.5 TB/s; its loads alone 28), join 12, outputs 74-76 (268 MB, 3.5 TB/s).  4 x 4096 tokens with gradients: besides, dk and dv
+// 161-169 us (0.54 GB) and dq with dg 186-203 (0.34 GB).  Of the outputs' cycles a quarter is MFMA and a third VALU
+// (98 MFMA, 460 VALU a wave and chunk: the splits in parts), which do not overlap within a SIMD; the rest waits for loads
+// and at the chunk's two barriers.  dq with dg: 216 MFMA and 1210 VALU, 63 % of its cycles.
+// Measured and not taken (us of the outputs' pass): a block a CU with all of the next chunk ahead 98 (V and the
+// outputs' stage in one buffer, two blocks: 88); outputs through LDS, three barriers a chunk: 85; operands read from LDS several
+// products ahead (schedule groups): the same within 1 %.
+//
 // Precision: as the gated delta rule's (mma): fp32 operands enter products as sums of three bf16 parts.  Where only a bf16
 // output depends on them two parts do, 2^-17 of a term under a rounding of 2^-9: X in Q X and P in P V (not where dg is
 // summed from the product).
@@ -546,7 +556,8 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, kOut, kDg>)) void linear_
   linear_scan<T, kOut, kDg, kAheadOf<T, kOut, kDg>>(a, a.pass[which], lds, kDg ? a.dg_parts + blockIdx.x : nullptr);
 }
 
-// X before each segment but the pass's first from what the segments add: 256 threads, 1024 elements of a head's state.
+// X before each segment but the pass's first from what the segments add: 256 threads, 1024 elements of a head's state.  Bound by
+// latency: 67 MB in 12 us where 16 heads have 32 segments, 11 us for 64 heads of 8.
 __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int C) {
   const Pass& x = a.pass[0];
   const int n = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, e = blockIdx.y * 1024 + 4 * threadIdx.x;
@@ -580,7 +591,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int C) {
   }
 }
 
-// dg of a head: the parts of its blocks, in their order.
+// dg of a head: the parts of its blocks, in their order (4-5 us: a launch).
 __global__ __launch_bounds__(256) void linear_dg_kernel(const float* parts, int units, int Hv, float* dg) {
   __shared__ double red[256];
   const int h = blockIdx.x;
@@ -595,7 +606,8 @@ __global__ __launch_bounds__(256) void linear_dg_kernel(const float* parts, int 
   if (threadIdx.x == 0) dg[h] = (float)red[0];
 }
 
-// dq (blockIdx.y 0) and dk of the q/k heads from the parts of the v heads that share them: a thread 8 elements.
+// dq (blockIdx.y 0) and dk of the q/k heads from the parts of the v heads that share them: a thread 8 elements.  Bound by HBM: 4
+// bytes an element and v head read, sizeof(T) an element and q/k head written.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_shared_kernel(const float* dq_parts, const float* dk_parts, int64_t rows, int Hk, int share,
                                                             T* dq, T* dk) {

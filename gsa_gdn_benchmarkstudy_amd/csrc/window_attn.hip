@@ -14,6 +14,15 @@
 // run.  The first tokens are seen by all later queries; those past the window's are cut into parts of
 // queries, whose sums are added in their order (window_far_kernel).
 //
+// Bound by issue: a wave's 32 queries and 32 keys take 16 MFMA (512 cycles), 16 exponentials and some 90 further VALU (about as
+// many cycles), which do not overlap within a SIMD; three waves a SIMD hide most of what else there is.  Forward, 16384
+// tokens, window 4096, 16 heads on 4, bf16: 486-500 us, 0.98 PFLOP/s in the pairs that are seen (a large library product: 1.33).
+// 4 x 4096 tokens, window 1024, with gradients: forward 164-168 us, dq 235-240, dk and dv 300-330, far queries 34-36 (134 MB of
+// q and do read once more: 28), their join 10.
+// Measured and not taken: a swizzle under which transposed reads meet in no bank (conflicts a third of LDS's cycles now,
+// 0 then): 505 us for 494 forward, 687 for 668 with gradients, for what the addresses cost; tiles of 64 keys forward and two
+// blocks a CU: slower throughout; dk and dv by one wave a SIMD: 857 for 707.
+//
 // Precision: sums, softmax statistics and D are fp32.  P and dS enter the second products in the inputs' type: bf16 (2^-9 of a
 // term, as the inputs themselves were rounded), or, for fp32, as three bf16 parts each, as all fp32 operands do (chunks.h).
 #include "chunks.h"
@@ -45,7 +54,7 @@ template <> struct WindowType<float> { static constexpr int NP = 3, kTile = 32, 
 
 // ---------------------------------------------------------------------------
 // Tiles of kTile rows of 128 elements in LDS: for each bf16 part (plane) rows of 16 units of 16 bytes, unit u of row t in
-// place u ^ swizzle(t), so that neither 16 rows' reads of one unit nor transposed reads of four rows meet in a bank.
+// place u ^ swizzle(t), so that 16 rows' reads of one unit meet in no bank (transposed reads of 32 lanes do, two by two).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int swizzle(int t) { return (t & 7) << 1 | (t >> 3 & 1); }
 // Row m of a 32-row product stands for row perm(m): an accumulator's 8 rows r = 8 s .. + 7 are then 16 s + 8 (l / 32) .. + 7,

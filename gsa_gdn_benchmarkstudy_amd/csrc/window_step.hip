@@ -10,6 +10,10 @@
 // Bound by HBM: each key and value is read once, for all query heads on it (16 at most at a time).  Each wave has its own
 // running maximum, sum and output, joined within the block.  Where rows times key heads are few, the keys of a row are split
 // over blocks: each leaves its part in the workspace and counts itself, the last one to arrive joins the parts in their order.
+// 61 rows of 2052 keys, 16 heads on 4, bf16: 40 us for 199 MB (5.0 TB/s) behind a write of
+// 4-5; one row of 1028 keys: 10.6 behind 2.5 (nine blocks a head; one waits for the others' parts).
+// (The write in the same launch would save 5 us; it would need every block to look for other rows of its own
+// sequence, and the counters of split rows to be clear before.)
 #include "chunks.h"
 
 namespace gsa {
@@ -431,14 +435,21 @@ __global__ __launch_bounds__(256, 2) void window_step_bf16_kernel(WindowStepArgs
 namespace gsa_host {
 namespace {
 
-// Keys of a block and blocks of a row and key head: as few keys (a multiple of 128: four waves of 32) as give some 1024 blocks.
+// Keys of a block (a multiple of 128: four waves of 32) and blocks of a row and key head: a row's keys are split where the key
+// heads of all rows are fewer than half of the blocks that the card wants, one a CU in bf16, two in fp32.  us in a graph, 16 heads on
+// 4, by blocks in all (the write, 4-5, included); the join is what more of them cost:
+//   1 row, window 1024: 12.3 (9 blocks a head: 36)        16 rows, 4096:  64 blocks 36   256: 30.5 (taken)   512: 31.5  1024: 35
+//   1 row, 8192:   256: 18.3 (taken)  512: 23.8  1024: 24.6    24 rows, 2048:  96: 32.9   192: 26.9 (taken)   288: 31.0
+//   4 rows, 4096:  128: 19.3  256: 17.7 (taken)  512: 20.3     33 rows, 2048: 132: 33.6 (taken)  264: 39.8   396: 33.0
+//   1 row, 65536:  256: 38.7 (taken)  512: 46.7  4096: 119     61 rows, 2048: 244: 45.0 (taken)  488: 49.4   976: 53.5
+//   fp32, 16 rows, 4096:  256: 57.7  512: 54.1 (taken)  1024: 57.3    33 rows, 2048:  132: 89.8  396: 56.7 (taken)  528: 70.2
 struct StepPlan { int chunk, splits; size_t counters, parts; };
-bool step_plan(int N, int H, int Hkv, int window, int sinks, StepPlan& z) {
-  if (N < 1 || N > 65535 || Hkv < 1 || Hkv > 65535 || H < Hkv || H % Hkv || window < 1 || sinks < 0 ||
+bool step_plan(int N, int H, int Hkv, int window, int sinks, int dtype, StepPlan& z) {
+  if (!dtype_size(dtype) || N < 1 || N > 65535 || Hkv < 1 || Hkv > 65535 || H < Hkv || H % Hkv || window < 1 || sinks < 0 ||
       (int64_t)window + sinks >= 1 << 30)
     return false;
   const int64_t keys = (int64_t)window + sinks, heads = (int64_t)N * Hkv;
-  const int64_t want = std::max<int64_t>(1, 1024 / heads);
+  const int64_t want = std::max<int64_t>(1, (dtype == GSA_DTYPE_BF16 ? 256 : 512) / heads);
   z.chunk = (int)((std::max<int64_t>(1, (keys + want - 1) / want) + 127) / 128 * 128);
   z.splits = (int)((keys + z.chunk - 1) / z.chunk);
   z.counters = up((size_t)heads * 4);
@@ -463,6 +474,7 @@ int launch_write(const gsa::WindowWriteArgs& a, int64_t blocks, int dtype, hipSt
 int launch_step(const gsa::WindowStepArgs& a, int N, int dtype, hipStream_t s) {
   const dim3 grid(a.splits, a.Hkv, N);
   const int share = a.H / a.Hkv;
+  // fp32, 16 rows of 2048 keys, query heads of a key head at a time: 16 heads on 4: 1 93, 2 54, 4 38 us; 64 on 8: 343, 178, 99
   if (dtype == GSA_DTYPE_BF16) hipLaunchKernelGGL(gsa::window_step_bf16_kernel, grid, dim3(256), 0, s, a);
   else if (share == 1) hipLaunchKernelGGL(gsa::window_step_f32_kernel<1>, grid, dim3(256), 0, s, a);
   else if (share == 2) hipLaunchKernelGGL(gsa::window_step_f32_kernel<2>, grid, dim3(256), 0, s, a);
@@ -499,9 +511,9 @@ extern "C" int gsa_window_cache_write(const void* k, int64_t k_sb, int64_t k_st,
   return launch_write(a, blocks, dtype, static_cast<hipStream_t>(stream));
 }
 
-extern "C" size_t gsa_window_step_workspace_bytes(int N, int H, int Hkv, int window, int sinks) {
+extern "C" size_t gsa_window_step_workspace_bytes(int N, int H, int Hkv, int window, int sinks, int dtype) {
   gsa_host::StepPlan z;
-  return gsa_host::step_plan(N, H, Hkv, window, sinks, z) ? z.counters + z.parts : 0;
+  return gsa_host::step_plan(N, H, Hkv, window, sinks, dtype, z) ? z.counters + z.parts : 0;
 }
 extern "C" int gsa_window_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int64_t k_sn, int64_t k_sh, const void* v,
                                int64_t v_sn, int64_t v_sh, const void* positions, int pos_bytes, const void* cache_idx, int idx_bytes,
@@ -512,7 +524,7 @@ extern "C" int gsa_window_step(const void* q, int64_t q_sn, int64_t q_sh, const 
   if (!q || !positions || !k_cache || !v_cache || !o || !ws || !k != !v) return GSA_ERR_NULL;
   if (!dtype_size(dtype)) return GSA_ERR_DTYPE;
   StepPlan z;
-  if (d != 128 || !step_plan(N, H, Hkv, window, sinks, z) || rows < (int64_t)window + sinks || (!cache_idx && N > slots)) return GSA_ERR_SHAPE;
+  if (d != 128 || !step_plan(N, H, Hkv, window, sinks, dtype, z) || rows < (int64_t)window + sinks || (!cache_idx && N > slots)) return GSA_ERR_SHAPE;
   if (ws_bytes < z.counters + z.parts) return GSA_ERR_SHAPE;
   gsa::Places p;
   if (const int e = places(cache_idx, idx_bytes, positions, pos_bytes, slots, rows, sinks, p)) return e;

@@ -699,7 +699,7 @@ int gsa_window_cache_write(const void* k, int64_t k_sb, int64_t k_st, int64_t k_
                            const void* positions, int pos_bytes, const void* cache_idx, int idx_bytes, void* k_cache,
                            int64_t kc_sn, int64_t kc_st, int64_t kc_sh, void* v_cache, int64_t vc_sn, int64_t vc_st,
                            int64_t vc_sh, int slots, int rows, int sinks, void* stream);
-size_t gsa_window_step_workspace_bytes(int N, int H, int Hkv, int window, int sinks);
+size_t gsa_window_step_workspace_bytes(int N, int H, int Hkv, int window, int sinks, int dtype);
 int gsa_window_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int64_t k_sn, int64_t k_sh, const void* v,
                     int64_t v_sn, int64_t v_sh, const void* positions, int pos_bytes, const void* cache_idx, int idx_bytes,
                     void* k_cache, int64_t kc_sn, int64_t kc_st, int64_t kc_sh, void* v_cache, int64_t vc_sn, int64_t vc_st,

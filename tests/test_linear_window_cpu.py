@@ -304,12 +304,18 @@ def test_c_window_step_refusals(lib):
 
 def test_c_window_step_sizes(lib):
     f = lib.gsa_window_step_workspace_bytes
-    for bad in ((0, 1, 1, 1, 0), (65536, 1, 1, 1, 0), (1, 0, 0, 1, 0), (1, 3, 2, 1, 0), (1, 1, 1, 0, 0), (1, 1, 1, 1, -1), (1, 1, 1, 1 << 30, 0)):
+    for bad in ((0, 1, 1, 1, 0, 1), (65536, 1, 1, 1, 0, 1), (1, 0, 0, 1, 0, 1), (1, 3, 2, 1, 0, 1), (1, 1, 1, 0, 0, 1), (1, 1, 1, 1, -1, 1),
+                (1, 1, 1, 1 << 30, 0, 1), (1, 1, 1, 1, 0, 2)):
         assert f(*bad) == 0, bad
-    few, many = f(1, 16, 4, 1024, 4), f(61, 16, 4, 1024, 4)
-    assert f(1, 16, 4, 128, 0) == f(1, 16, 4, 1, 0) < few            # one block of 128 keys: no parts
-    assert few == f(1, 16, 4, 128, 0) + 9 * 16 * 130 * 4              # 1028 keys in blocks of 128
-    assert many == f(61, 16, 4, 1, 0) + 61 * 3 * 16 * 130 * 4         # 244 rows and key heads: 4 blocks each, of 384 keys
+
+    def splits(N, H, Hkv, keys, dtype):          # from the parts: 130 floats a head and block
+        one, n = f(N, H, Hkv, 1, 0, dtype), f(N, H, Hkv, keys, 0, dtype)
+        assert (n - one) % (N * H * 130 * 4) == 0
+        return max(1, (n - one) // (N * H * 130 * 4))
+
+    assert splits(1, 16, 4, 128, 1) == 1 and splits(1, 16, 4, 129, 1) == 2 and splits(1, 16, 4, 1028, 1) == 9
+    assert splits(1, 16, 4, 65536, 1) == 64 and splits(24, 16, 4, 2052, 1) == 2
+    assert splits(33, 16, 4, 2052, 1) == splits(61, 16, 4, 2052, 1) == 1 and splits(33, 16, 4, 2052, 0) == 3
 
 
 # ---------------------------------------------------------------------------
