@@ -12,7 +12,7 @@
 // dq (window_dq_kernel) goes the same way; dk and dv (window_dkv_kernel): a block takes 128 keys of a key head and walks the
 // queries of all heads on it that see them, so that no two blocks write one gradient: no atomics, the same bits on every
 // run.  The first tokens are seen by all later queries; those past the window's are cut into parts of
-// queries, whose sums are added in their order (window_far_kernel).
+// queries, whose sums are added in their order (window_join_kernel).
 //
 // Bound by issue: a wave's 32 queries and 32 keys take 16 MFMA (512 cycles), 16 exponentials and some 90 further VALU (about as
 // many cycles), which do not overlap within a SIMD; three waves a SIMD hide most of what else there is.  Forward, 16384
@@ -42,7 +42,8 @@ struct WindowArgs {
   void *dq, *dk, *dv;
   // dk and dv: blocks of near_keys keys; the far queries of first tokens in parts of far_rows queries of a head, far_keys keys a block
   int near_keys, near_first, far_keys, far_first, far_rows;            // first: blocks of a sequence's first tokens
-  float* near_parts;          // [N][near_first][Hkv][2][near_keys][128]
+  int near_split;             // parts that a block's queries are cut into
+  float* near_parts;          // [N][near_first][Hkv][2][near_keys][128]; near_split > 1: [slots of keys][Hkv][near_split][2][..
   float* far_parts;           // [slots of far queries][far_first][H][2][far_keys][128]
 };
 
@@ -570,21 +571,24 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
   constexpr int NP = L::NP, N = L::N, kBuffers = Z::kBuffers, kBuffer = 2 * L::kBytes, kKeys = 32 * kGroups, kSplit = Z::kSplit;
   const uint32_t base = lds_addr(lds);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), share = a.H / a.Hkv;
-  int unit, hk, h0, heads, c, i0, i1, k0;
+  int unit, hk, h0, heads, c, i0, i1, k0, part = 0;
   float* parts = nullptr;
   Span sp;
   if constexpr (!kFarPart) {
-    hk = index % a.Hkv;
+    part = index % a.near_split;
+    unit = index / a.near_split;
+    hk = unit % a.Hkv;
     h0 = hk * share;
     heads = share;
-    unit = index / a.Hkv;
+    unit /= a.Hkv;
     sp = slot_of(a.s, unit, kKeys, c);
     if (c < 0) return;
     k0 = c * kKeys;
     i0 = k0;
     const int64_t end = (int64_t)k0 + kKeys - 1 + a.W;
     i1 = (int)min((int64_t)sp.len, end);
-    if (k0 < a.S && end < sp.len) parts = a.near_parts + (((int64_t)sp.n * a.near_first + c) * a.Hkv + hk) * 2 * kKeys * kHead;
+    if (a.near_split > 1) parts = a.near_parts + (int64_t)index * 2 * kKeys * kHead;
+    else if (k0 < a.S && end < sp.len) parts = a.near_parts + (((int64_t)sp.n * a.near_first + c) * a.Hkv + hk) * 2 * kKeys * kHead;
   } else {
     h0 = index % a.H;
     hk = h0 / share;
@@ -603,7 +607,8 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
   }
   const int group = wave % kGroups, split = kSplit > 1 ? wave / kGroups : 0;
   const int j0 = k0 + 32 * group, key = j0 + (l & 31), keyc = min(key, sp.len - 1);
-  const int tiles = (i1 - i0 + N - 1) / N, count = tiles * heads;
+  const int tiles = (i1 - i0 + N - 1) / N, all = tiles * heads;
+  const int first = kFarPart ? 0 : (int)((int64_t)all * part / a.near_split), count = kFarPart ? all : (int)((int64_t)all * (part + 1) / a.near_split);
   typename L::Loader lq(a.q.st, wave, l), ld(a.dout.st, wave, l);
   constexpr int kStatRow = N < 64 ? 64 : N;                  // L of a tile's queries, then D, each a wave's 64 or two
   auto load = [&](int t, int buffer) {
@@ -617,7 +622,7 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
     }
   };
   constexpr bool kAhead = kBuffers == 2 || NP == 3;          // the next tile's loads run beside this one's products
-  if (kAhead) load(0, 0);
+  if (kAhead && first < count) load(first, kBuffers == 2 ? first & 1 : 0);
   Parts<NP> k[8], v[8];
   row_operand<T>(k, row_at<T>(a.k, sp, keyc, hk), l);
   row_operand<T>(v, row_at<T>(a.v, sp, keyc, hk), l);
@@ -629,12 +634,12 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
   }
   const typename L::RowReader rows(base, l);
   const typename L::ColReader cols(base, l);
-  for (int t = 0; t < count; ++t) {
+  for (int t = first; t < count; ++t) {
     const int buffer = kBuffers == 2 ? t & 1 : 0;
     char *Q = lds + buffer * kBuffer, *dO = Q + L::kBytes;
     const float* st = reinterpret_cast<const float*>(lds + Z::kStats) + (t & 1) * 2 * kStatRow;
     if constexpr (kBuffers == 1) {
-      if (t) __syncthreads();                                // every wave is through with the last tile
+      if (t > first) __syncthreads();                        // every wave is through with the last tile
       if (!kAhead) load(t, 0);
       lq.store(Q, wave, l);
       ld.store(dO, wave, l);
@@ -724,26 +729,44 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
   window_dkv<T, kGroups, kFarPart>(a, lds, blockIdx.x);
 }
 
-// dk and dv of a sequence's first tokens: the near queries' part and those of the far ones, in their order.
+// dk and dv of what came in parts: of all keys (near_split > 1) or a sequence's first tokens; the near queries' parts and
+// those of the far ones, in their order.
 template <typename T>
-__global__ __launch_bounds__(256) void window_far_kernel(WindowArgs a) {
-  const int hk = blockIdx.x % a.Hkv, block = blockIdx.x / a.Hkv % a.near_first, n = blockIdx.x / a.Hkv / a.near_first, share = a.H / a.Hkv;
-  const Span sp = span_of(a.s, n, a.far_rows);
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
+  const int hk = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv, share = a.H / a.Hkv;
+  Span sp;
+  int block, far_slot;
+  if (a.near_split > 1) {
+    sp = slot_of(a.s, unit, a.near_keys, block);
+    if (block < 0) return;
+  } else {
+    block = unit % a.near_first;
+    sp = span_of(a.s, unit / a.near_first, a.near_keys);
+  }
   const int k0 = block * a.near_keys;
   const int64_t end = (int64_t)k0 + a.near_keys - 1 + a.W;
-  if (k0 >= sp.len || end >= sp.len) return;                 // no far queries: written as they were
+  const bool far_too = k0 < a.S && end < sp.len;
+  if (k0 >= sp.len || (a.near_split == 1 && !far_too)) return;         // (written as they were)
+  far_slot = far_too ? span_of(a.s, sp.n, a.far_rows).slot0 : 0;
   const int near = a.near_keys * kHead, far = a.far_keys * kHead;
+  const float* parts = a.near_parts + (int64_t)blockIdx.x * a.near_split * 2 * near;
   for (int u = threadIdx.x + 256 * blockIdx.y; u < 2 * near / 8; u += 256 * gridDim.y) {
     const int which = 8 * u >= near, t = u / 16 - which * a.near_keys, key = k0 + t, e = 8 * (u % 16);
     if (key >= sp.len) continue;
     float x[8];
-    load8(a.near_parts + (((int64_t)n * a.near_first + block) * a.Hkv + hk) * 2 * near + which * near + t * kHead + e, x);
-    if (key < a.S) {                                         // (the others have no far queries)
+    load8(parts + which * near + t * kHead + e, x);
+    for (int i = 1; i < a.near_split; ++i) {
+      float y[8];
+      load8(parts + (2 * i + which) * near + t * kHead + e, y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] += y[k];
+    }
+    if (far_too && key < a.S) {                              // (the others have no far queries)
       const int fb = key / a.far_keys, at = which * far + key % a.far_keys * kHead + e;
       for (int c = (int)(end / a.far_rows); c * a.far_rows < sp.len; ++c)
         for (int h = 0; h < share; ++h) {
           float y[8];
-          load8(a.far_parts + (((int64_t)(sp.slot0 + c) * a.far_first + fb) * a.H + hk * share + h) * 2 * far + at, y);
+          load8(a.far_parts + (((int64_t)(far_slot + c) * a.far_first + fb) * a.H + hk * share + h) * 2 * far + at, y);
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] += y[i];
         }
@@ -760,7 +783,7 @@ namespace {
 
 struct WindowPlan {
   int64_t slots, near, far;   // blocks of queries of all sequences, of keys, of parts of far queries (0: no far queries)
-  int queries, near_keys, near_first, far_keys, far_first, far_rows, W, S;   // queries: of a block
+  int queries, near_keys, near_split, near_first, far_keys, far_first, far_rows, W, S;   // queries: of a block
   size_t D, near_parts, far_parts;
   size_t workspace() const { return D + near_parts + far_parts; }
 };
@@ -788,6 +811,13 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   z.near_keys = dtype == GSA_DTYPE_BF16 && slots(128) * Hkv >= 512 ? 128 : 64;
   z.far_keys = dtype == GSA_DTYPE_BF16 ? 32 : 64;
   z.near = slots(z.near_keys);
+  // A block's queries in parts (summed by window_join_kernel) where the blocks are fewer than the card takes at once, two a CU, fp32
+  // one; at least 4 tiles a part.  us backward, by parts: bf16, 16 heads on 4, T = 512 1: 69  4: 41  8: 38 (taken: 8); T = 2048, window
+  // 1024 1: 167  2: 120  4: 103 (taken)  8: 113; T = 4096 1: 214  2: 189 (taken)  4: 197; 8 heads on 1, T = 4096 1: 808  4: 271
+  // 8: 189 (taken); T = 300, 4 heads 1: 27 (taken)  2: 28; 512 blocks (16 heads, T = 2048) 1: 92 (taken)  2: 110; fp32 B = 2
+  // T = 1537, 4 heads on 2, window 256 1: 154  2: 127 (taken)  4: 145; 256 blocks 1: 493 (taken)  2: 512.
+  const int64_t room = (dtype == GSA_DTYPE_BF16 ? 512 : 256) / (z.near * Hkv);
+  z.near_split = (int)std::clamp<int64_t>(H / Hkv * ((z.W + (int64_t)z.near_keys) / 64) / 4, 1, std::max<int64_t>(1, room));
   if (z.S) {
     z.near_first = (z.S + z.near_keys - 1) / z.near_keys;
     z.far_first = (z.S + z.far_keys - 1) / z.far_keys;
@@ -799,7 +829,7 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
     if (z.far > (1 << 23) / H || (int64_t)N * z.near_first > (1 << 23) / H) return false;
   }
   z.D = up((size_t)H * B * T * 4);
-  z.near_parts = (size_t)N * z.near_first * Hkv * 2 * z.near_keys * 128 * 4;
+  z.near_parts = (z.near_split > 1 ? (size_t)z.near * z.near_split : (size_t)N * z.near_first) * Hkv * 2 * z.near_keys * 128 * 4;
   z.far_parts = (size_t)z.far * H * 2 * z.far_keys * 128 * 4;
   return true;
 }
@@ -846,6 +876,7 @@ int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, Win
     char* w = static_cast<char*>(x->ws);
     a.D = reinterpret_cast<float*>(w);
     a.near_keys = z.near_keys;
+    a.near_split = z.near_split;
     a.near_first = z.near_first;
     a.far_keys = z.far_keys;
     a.far_first = z.far_first;
@@ -889,12 +920,14 @@ template <typename T> int window_forward(const gsa::WindowArgs& a, const WindowP
 template <typename T> int window_backward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
   int e = z.queries == 64 ? launch_dq<T, 2>(a, z, s) : launch_dq<T, 4>(a, z, s);
   if (e) return e;
-  const int64_t blocks = z.near * a.Hkv;
+  const int64_t blocks = z.near * z.near_split * a.Hkv;
   if constexpr (sizeof(T) == 2) e = z.near_keys == 128 ? launch_dkv<T, 4, false>(a, blocks, s) : launch_dkv<T, 2, false>(a, blocks, s);
   else e = launch_dkv<T, 2, false>(a, blocks, s);
-  if (e || !z.far) return e;
-  if ((e = launch_dkv<T, sizeof(T) == 2 ? 1 : 2, true>(a, z.far * a.H, s))) return e;
-  hipLaunchKernelGGL(gsa::window_far_kernel<T>, dim3(a.s.N * a.near_first * a.Hkv, a.near_keys / 8), dim3(256), 0, s, a);
+  if (e) return e;
+  if (z.far && (e = launch_dkv<T, sizeof(T) == 2 ? 1 : 2, true>(a, z.far * a.H, s))) return e;
+  if (!z.far && z.near_split == 1) return GSA_OK;
+  const int64_t units = z.near_split > 1 ? z.near : (int64_t)a.s.N * a.near_first;
+  hipLaunchKernelGGL(gsa::window_join_kernel<T>, dim3(units * a.Hkv, a.near_keys / 8), dim3(256), 0, s, a);
   return launch_status();
 }
 

@@ -109,6 +109,24 @@ def test_many_first_tokens(dev, B, T, H, Hkv, W, S, dtype):
     _compare(_run(x, dev, W, S, do=do), x, [(b, 0, T) for b in range(B)], W, S, do)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,T,H,Hkv,W,S", [(8, 600, 16, 8, 50, 5), (8, 1100, 8, 8, 200, 35), (9, 897, 8, 8, 897, 0), (5, 1000, 32, 16, 128, 200)])
+def test_many_blocks(dev, B, T, H, Hkv, W, S, dtype):
+    """Enough blocks of keys and queries for the larger ones, none of them in parts; first tokens with and without far queries."""
+    print(f"many {dtype} B={B} T={T} H={H} Hkv={Hkv} W={W} S={S}", flush=True)
+    x, do = _inputs(B, T, H, Hkv, dtype, seed=T + S), _grad(B, T, H, dtype, 7)
+    _compare(_run(x, dev, W, S, do=do), x, [(b, 0, T) for b in range(B)], W, S, do)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_blocks_packed(dev, dtype):
+    lens = [700, 0, 1500, 65, 2300, 1, 1283]
+    T, H = sum(lens), 12
+    x, do = _inputs(1, T, H, H, dtype, seed=T), _grad(1, T, H, dtype, 7)
+    cu = torch.tensor([0] + lens).cumsum(0)
+    _compare(_run(x, dev, 150, 4, cu=cu.to(dev), do=do), x, [(0, int(cu[i]), int(cu[i + 1])) for i in range(len(lens))], 150, 4, do)
+
+
 PACKS = [[1], [5, 0, 64, 1, 65, 63], [0, 0, 3], [130, 32, 33], [128, 64, 256], [0], [1300, 1, 0, 333]]
 
 

@@ -257,9 +257,11 @@ def test_c_window_sizes(lib):
                 (last, last, last, 0, 1, 1, 1, 0, 1), (1, 2 ** 26, 1, 0, 8, 8, last, last, 1)):
         assert f(*bad) == 0, bad
     # D alone where there are no far queries: a window of everything, first tokens that are all of it, none
-    assert f(1, 640, 1, 0, 2, 1, last, last, 1) == f(1, 640, 1, 0, 2, 1, 600, 40, 1) == f(1, 640, 1, 0, 2, 1, 9, 0, 1) == 640 * 2 * 4
-    # near sums of 64 keys (dk and dv, fp32) and far sums of 32 keys for 5 parts of 128 queries and each head
-    assert f(1, 640, 1, 0, 2, 1, 9, 4, 1) == 640 * 2 * 4 + 2 * 64 * 512 + 5 * 2 * 2 * 32 * 512
+    assert f(1, 320, 1, 0, 2, 2, last, last, 1) == f(1, 320, 1, 0, 2, 2, 280, 40, 1) == f(1, 320, 1, 0, 2, 2, 9, 0, 1) == 320 * 2 * 4
+    # near sums of 64 keys (dk and dv, fp32) and far sums of 32 keys for 3 parts of 128 queries and each head
+    assert f(1, 320, 1, 0, 2, 2, 9, 4, 1) == 320 * 2 * 4 + 2 * 2 * 64 * 512 + 3 * 2 * 2 * 32 * 512
+    # few blocks of keys (5 and one key head) for many tiles of queries (8 heads, 6 tiles): 12 parts for each block
+    assert f(1, 320, 1, 0, 8, 1, last, 0, 1) == 320 * 8 * 4 + 5 * 12 * 2 * 64 * 512
     # many first tokens: the parts hold more queries, not the workspace more parts
     assert f(1, 65536, 1, 0, 16, 4, 100, 30000, 1) < 2 << 30
 
