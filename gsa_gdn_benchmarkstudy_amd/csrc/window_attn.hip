@@ -17,7 +17,7 @@
 // Bound by issue: a wave's 32 queries and 32 keys take 16 MFMA (512 cycles), 16 exponentials and some 90 further VALU (about as
 // many cycles), which do not overlap within a SIMD; three waves a SIMD hide most of what else there is.  Forward, 16384
 // tokens, window 4096, 16 heads on 4, bf16: 486-500 us, 0.98 PFLOP/s in the pairs that are seen (a large library product: 1.33).
-// 4 x 4096 tokens, window 1024, with gradients: forward 164-168 us, dq 235-240, dk and dv 300-330, far queries 34-36 (134 MB of
+// 4 x 4096 tokens, window 1024, with gradients: forward 152-167 us, dq 217-240, dk and dv 278-310, far queries 31-34 (134 MB of
 // q and do read once more: 28), their join 10.
 // Measured and not taken: a swizzle under which transposed reads meet in no bank (conflicts a third of LDS's cycles now,
 // 0 then): 505 us for 494 forward, 687 for 668 with gradients, for what the addresses cost; tiles of 64 keys forward and two
@@ -669,7 +669,7 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
         mma32(s, r.read(0, 0, ks), k[ks]);
         mma32(p, r.read(L::kBytes, 0, ks), v[ks]);
       }
-      if constexpr (NP == 1) reads_ahead<1, 16>();           // (more ahead would not fit the registers)
+      if constexpr (NP == 1) reads_ahead<3, 16>();           // (1: 293 us, 2 280, 3 278, 4 281; 4 x 4096 tokens, window 1024)
       asm volatile("" : "+v"(s), "+v"(p));
       const float* stats = st + 32 * n + 8 * (here(l) >> 5);
 #pragma unroll
