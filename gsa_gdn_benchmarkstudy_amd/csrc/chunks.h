@@ -314,7 +314,7 @@ __device__ __forceinline__ void clear_outside(const Outside& a, int block, int b
   }
 }
 
-static __global__ __launch_bounds__(256) void outside_kernel(Outside a) { clear_outside(a, blockIdx.x, gridDim.x); }
+[[maybe_unused]] static __global__ __launch_bounds__(256) void outside_kernel(Outside a) { clear_outside(a, blockIdx.x, gridDim.x); }
 
 }  // namespace gsa
 

@@ -78,7 +78,7 @@ template <typename T, int kN = WindowType<T>::kTile> struct Tile {
       Parts<NP> r;
 #pragma unroll
       for (int i = 0; i < NP; ++i)
-        r.p[i] = *(const __attribute__((address_space(3))) bf16x8*)((at ^ 32u * ks) + (tile + i * kPlane + t0 * 256));
+        r.p[i] = *(const __attribute__((address_space(3))) bf16x8*)(uintptr_t)((at ^ 32u * ks) + (tile + i * kPlane + t0 * 256));
       return r;
     }
   };
@@ -100,7 +100,7 @@ template <typename T, int kN = WindowType<T>::kTile> struct Tile {
         s16x4 x[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
+          x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(
               at[dt & 1] + (tile + n * kPlane + t0 * 256 + 1024 * e + 16 * ((dt & 2 ? 8 : 0) ^ (8 * e)))));
         r.p[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
       }

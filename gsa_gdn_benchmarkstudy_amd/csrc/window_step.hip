@@ -10,10 +10,8 @@
 // Bound by HBM: each key and value is read once, for all query heads on it (16 at most at a time).  Each wave has its own
 // running maximum, sum and output, joined within the block.  Where rows times key heads are few, the keys of a row are split
 // over blocks: each leaves its part in the workspace and counts itself, the last one to arrive joins the parts in their order.
-// 61 rows of 2052 keys, 16 heads on 4, bf16: 40 us for 199 MB (5.0 TB/s) behind a write of
-// 4-5; one row of 1028 keys: 10.6 behind 2.5 (nine blocks a head; one waits for the others' parts).
-// (The write in the same launch would save 5 us; it would need every block to look for other rows of its own
-// sequence, and the counters of split rows to be clear before.)
+// 61 rows of 2052 keys, 16 heads on 4, bf16: 42 us for 199 MB (4.7 TB/s), the write with it; one row of 1028 keys: 10.6
+// behind a write of 2.5 (nine blocks a head; one waits for the others' parts; their counters have to be clear before).
 #include "chunks.h"
 
 namespace gsa {
@@ -74,11 +72,39 @@ struct WindowStepArgs {
   Places places;
   int H, Hkv, W, splits, chunk;                              // chunk: keys of a block
   float scale_l2;
+  Rows k, v;                                                 // [N, Hkv, 128]: keys and values that the blocks write themselves (null: written)
+  int N;
   void* o;                                                   // [N, H, 128]
   float* parts;                                              // [N][Hkv][splits][H / Hkv][kStepPart]
   uint32_t* counters;                                        // [N][Hkv]
 };
 constexpr int kStepPart = kHead + 2;                         // o, m, l
+
+// The new keys and values of row n's sequence, its own and those of other rows on the same slot, to the cache: one key head, by
+// each block that reads them (several blocks may write the same).  Written from the CU that reads, so nothing but the wait
+// orders the two.
+template <typename T> __device__ __forceinline__ void write_new(const WindowStepArgs& a, int n, int hk, int64_t slot) {
+  if (!a.k.p) return;
+  constexpr int kPieces = kHead * sizeof(T) / 16;
+  const int wave = threadIdx.x >> 6, l = lane_id(), piece = l % kPieces;
+  auto put = [&](int j) {
+    const int64_t p = a.places.position(j);
+    if (p < 0 || l >= 2 * kPieces) return;
+    const Rows& x = l < kPieces ? a.k : a.v;
+    const Cache& y = l < kPieces ? a.kc : a.vc;
+    const u32x4 z = *reinterpret_cast<const u32x4*>(static_cast<const char*>(x.p) + (j * x.sb + hk * x.sh) * (int64_t)sizeof(T) + 16 * piece);
+    *reinterpret_cast<u32x4*>(y.p + (slot * y.sn + a.places.row(p) * y.st + hk * y.sh) * (int64_t)sizeof(T) + 16 * piece) = z;
+  };
+  if (!a.places.at) {
+    if (wave == 0) put(n);
+  } else {
+    for (int j0 = 64 * wave; j0 < a.N; j0 += 256)
+      for (uint64_t same = ballot64(j0 + l < a.N && a.places.slot(min(j0 + l, a.N - 1)) == slot); same; same &= same - 1)
+        put(j0 + __builtin_ctzll(same));
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
 
 // The visible keys of a row's token in order, e = 0 .. count - 1: tokens 0 .. first - 1, then those of the window.
 struct Visible {
@@ -201,6 +227,7 @@ __global__ __launch_bounds__(256) void window_step_f32_kernel(WindowStepArgs a) 
   const Visible see(a.places, p, a.W);
   const int parts = (see.count + a.chunk - 1) / a.chunk;
   if (split >= parts) return;
+  write_new<float>(a, n, hk, slot);
   const int e0 = split * a.chunk, e1 = min(see.count, e0 + a.chunk);
   const float* kb = reinterpret_cast<const float*>(a.kc.p) + slot * a.kc.sn + hk * a.kc.sh + 8 * li;
   const float* vb = reinterpret_cast<const float*>(a.vc.p) + slot * a.vc.sn + hk * a.vc.sh + 8 * li;
@@ -329,6 +356,7 @@ __global__ __launch_bounds__(256, 2) void window_step_bf16_kernel(WindowStepArgs
   const Visible see(a.places, p, a.W);
   const int parts = (see.count + a.chunk - 1) / a.chunk;
   if (split >= parts) return;
+  write_new<uint16_t>(a, n, hk, slot);
   const int e0 = split * a.chunk, e1 = min(see.count, e0 + a.chunk);
   const uint16_t* kb = reinterpret_cast<const uint16_t*>(a.kc.p) + slot * a.kc.sn + hk * a.kc.sh;
   const uint16_t* vb = reinterpret_cast<const uint16_t*>(a.vc.p) + slot * a.vc.sn + hk * a.vc.sh;
@@ -456,6 +484,7 @@ bool step_plan(int N, int H, int Hkv, int window, int sinks, int dtype, StepPlan
   z.parts = z.splits > 1 ? (size_t)N * z.splits * H * gsa::kStepPart * 4 : 0;
   return true;
 }
+constexpr int kLooked = 512;                                 // indices that a block looks through
 int places(const void* at, int at_bytes, const void* pos, int pos_bytes, int slots, int rows, int sinks, gsa::Places& p) {
   if (slots < 1 || sinks < 0 || rows <= sinks || rows >= 1 << 30) return GSA_ERR_SHAPE;    // (rows are added up in 32 bits)
   if ((at && at_bytes != 4 && at_bytes != 8) || (pos && pos_bytes != 4 && pos_bytes != 8)) return GSA_ERR_SHAPE;
@@ -534,14 +563,19 @@ extern "C" int gsa_window_step(const void* q, int64_t q_sn, int64_t q_sh, const 
   const auto s = static_cast<hipStream_t>(stream);
   auto* counters = static_cast<uint32_t*>(ws);
   const gsa::Cache kc{static_cast<char*>(k_cache), kc_sn, kc_st, kc_sh}, vc{static_cast<char*>(v_cache), vc_sn, vc_st, vc_sh};
-  if (k) {
+  // Whole rows: each block writes what it reads, a launch less.  It looks through all indices for that, so where they are many
+  // the write has a launch of its own.  us with it / without: 61 rows of 2052 keys 45.0 / 42.2, 33 of 516 15.5 / 13.5, 300 of 132
+  // 26.7 / 26.0, 300 of 1028 124 / 121, 1000 of 260 116 / 131, 4000 of 132 75 / 107 (without indices 75 / 75).
+  const bool writes = k && z.splits == 1 && (!cache_idx || N <= kLooked);
+  if (k && !writes) {
     // each row a sequence of one token; its block clears the row's counters too
     const gsa::WindowWriteArgs w{{nullptr, 0, N, 1}, {k, k_sn, 0, k_sh}, {v, v_sn, 0, v_sh}, kc, vc, p, Hkv, z.splits > 1 ? counters : nullptr};
     if (const int e = launch_write(w, N, dtype, s)) return e;
-  } else if (z.splits > 1) {
+  } else if (!k && z.splits > 1) {
     if (const int e = launch_clear(counters, N * Hkv, s)) return e;
   }
-  const gsa::WindowStepArgs a{q, q_sn, q_sh, kc, vc, p, H, Hkv, window, z.splits, z.chunk, scale * gsa::kLog2e, o,
+  const gsa::WindowStepArgs a{q, q_sn, q_sh, kc, vc, p, H, Hkv, window, z.splits, z.chunk, scale * gsa::kLog2e,
+                              {writes ? k : nullptr, k_sn, 0, k_sh}, {writes ? v : nullptr, v_sn, 0, v_sh}, N, o,
                               reinterpret_cast<float*>(static_cast<char*>(ws) + z.counters), counters};
   return launch_step(a, N, dtype, s);
 }

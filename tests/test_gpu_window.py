@@ -397,6 +397,21 @@ def test_step_many_rows(dev):
     _step_case(dev, torch.bfloat16, N, 2, 1, N + 3, 40, 30, 3, [(7 * i) % 101 for i in range(N)], [(i * 7) % (N + 3) if i % 5 else -1 for i in range(N)])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [70, 512, 513])
+def test_step_rows_of_the_same_sequences(dev, N, dtype):
+    """Tokens of some sequences scattered over the batch, among padding: written by the blocks that read them, or before."""
+    W, S, slots = 40, 3, N // 2
+    gen = torch.Generator().manual_seed(N)
+    at = torch.randint(-1, slots, (N,), generator=gen).tolist()
+    seen, pos = {}, []
+    for s in at:                                 # consecutive tokens of each sequence, in the batch's order
+        seen[s] = seen.get(s, 20 + 7 * s) + 1
+        pos.append(seen[s] if s % 11 else -5)
+    most = max(seen[s] - (20 + 7 * s) for s in seen if s >= 0)
+    _step_case(dev, dtype, N, 4, 2, slots, S + W + most - 1, W, S, pos, at)
+
+
 def test_step_positions_past_every_sequence(dev):
     """Positions whose sums would pass 64 bits are padding, in the step and in the write."""
     k = torch.randn(3, 2, 1, D, dtype=torch.bfloat16, device=dev)
