@@ -540,9 +540,9 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
   }
 }
 
-// bf16: two blocks share a CU (kPerSimd 4) and cover each other's waits; dq with dg one, for its registers.  All of the next
-// chunk where LDS has room for it.
-template <typename T, bool kOut, bool kDg> constexpr int kPerSimd = sizeof(T) == 2 && !kDg ? 4 : 2;
+// Two blocks share a CU (kPerSimd 4) and cover each other's waits (fp32, 16384 tokens of 16 heads forward: 323 -> 287 us); dq with dg
+// is alone, for its registers.  bf16: all of the next chunk ahead where LDS has room for it.
+template <typename T, bool kOut, bool kDg> constexpr int kPerSimd = !kDg ? 4 : 2;
 template <typename T, bool kOut, bool kDg> constexpr Ahead kAheadOf = sizeof(T) == 4 ? kNothing : kOut && !kDg ? kKeys : kAll;
 
 template <typename T, bool kOut, bool kDg>
