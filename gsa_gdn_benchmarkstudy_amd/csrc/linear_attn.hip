@@ -646,17 +646,21 @@ LinearPlan linear_plan(int B, int T, int N, int packed, int Hk, int Hv, int dtyp
   if ((packed ? (int64_t)T / z.C + N : B * nc) > (1 << 23) / Hv || heads >= 1 << 23) return z;
   const int64_t length = packed ? (nc + N - 1) / N : nc;
   z.segs = 0;
-  // A head is one chain of chunks; cut into segments it is passed over twice, once for the state alone (about half the work). Two
-  // blocks a CU are 512 of them, so a chain is cut into 512 / heads; where the heads fill most of the card the second pass costs
-  // more. Measured in us, segments of n chunks of 64 (0: none), 16 heads a row of the batch, bf16 forward:
-  //   T = 16384, B = 1:  0: 1214  2: 225  4: 156  8: 126 (taken)  16: 150      T = 4096, B = 6:   0: 335  8: 203  16: 202 (taken)
-  //   T = 512,   B = 1:  0: 42    1: 23 (taken)  2: 27  4: 40                  T = 4096, B = 10:  0: 343  16: 343  22: 293 (taken)
-  //   T = 2048,  B = 1:  0: 153   1: 45  2: 39 (taken)  4: 47                  T = 4096, B = 12:  0: 342 (taken)  16: 361  32: 375
-  //   23 sequences, 12289 tokens (368 heads): 0: 116 (taken)  4: 133  8: 127   T = 4096, B = 16:  0: 351 (taken)  16: 460  32: 411
-  // With gradients, B = 4, T = 4096: 0: 1069  4: 582  8: 494 (taken)  16: 520; B = 16: 0: 1562 (taken)  16: 1821.
-  // One chunk a segment pays where the join then has few to go through: T = 1000  1: 30  2: 32.
+  // A head is one chain of chunks; cut into segments it is passed over twice, once for the state alone (about half the work), so
+  // where the heads fill most of the card that costs more.  Few heads: a block a CU, 256 / heads segments (fewer states to join, and
+  // dq's pass has a CU's block at a time anyhow); more of them, packed ones, whose lengths differ, and fp32: two a CU, 512 / heads.
+  // Measured in us, segments of n chunks of 64 (0: none), 16 heads a row of the batch, bf16 forward:
+  //   T = 512:   0: 37    1: 22 (taken)  2: 25  4: 35        B = 6, T = 4096:   0: 270   8: 191  13: 169 (taken)  16: 184
+  //   T = 2048:  0: 134   1: 43  2: 36 (taken)  4: 41        B = 10, T = 4096:  0: 273   16: 296  22: 268 (taken)
+  //   T = 4096:  2: 54  4: 48 (taken)  8: 64                 B = 12, T = 4096:  0: 276 (taken)  16: 327  22: 346
+  //   T = 16384: 0: 1020  4: 149  8: 121  16: 121 (taken)    B = 16, T = 4096:  0: 312 (taken)  16: 416  32: 378
+  //   packed, 23 sequences, 12289 tokens: 0: 101 (taken)  4: 125  8: 118;  4 sequences, 16384: 8: 140 (taken)  16: 170
+  // With gradients, T = 16384  4: 564  8: 482  16: 439 (taken)  32: 669; B = 4, T = 4096  0: 1024  8: 455  16: 431 (taken);
+  // B = 16, T = 4096  0: 1401 (taken)  16: 1694.  fp32 (chunks of 32), T = 16384  8: 291  16: 266 (taken)  32: 333.
+  // One chunk a segment pays where the join then has few to go through: T = 1000  1: 29  2: 30.
   if (heads <= 160 && length >= 4) {
-    const int64_t pieces = 512 / heads, seg = std::max<int64_t>(length <= 16 ? 1 : 2, (length + pieces - 1) / pieces);
+    const int64_t pieces = (dtype == GSA_DTYPE_BF16 && !packed && heads <= 64 ? 256 : 512) / heads;
+    const int64_t seg = std::max<int64_t>(length <= 16 ? 1 : 2, (length + pieces - 1) / pieces);
     if (seg < length) {
       z.seg = (int)seg;
       z.segs = packed ? (int64_t)T / (z.C * seg) + N : B * ((nc + seg - 1) / seg);

@@ -200,8 +200,10 @@ def test_c_linear_sizes(lib):
             assert (f(N, 1, N, 0, 16, 16, 1) != refused) == (f(1, 1, N, 1, 16, 16, 1) != refused) == (N < 2 ** 19)
     saved = lib.gsa_linear_attn_saved_bytes
     assert lib.gsa_linear_attn_workspace_bytes(1, 64, 1, 0, 2, 2, 1, 0) == saved(1, 64, 1, 0, 2, 2, 1) == 0     # one chunk
-    # a state of 64 KiB for each segment and v head: of 8 chunks of 64 where 16 heads have 16384 tokens; none for many heads
-    assert saved(1, 16384, 1, 0, 16, 16, 1) == 32 * 16 * 65536
+    # a state of 64 KiB for each segment and v head: of 16 chunks of 64 where 16 heads have 16384 tokens (packed: of 8, and one
+    # more begun; fp32: of 16 of 32); none for many heads
+    assert saved(1, 16384, 1, 0, 16, 16, 1) == 16 * 16 * 65536
+    assert saved(1, 16384, 1, 1, 16, 16, 1) == 33 * 16 * 65536 and saved(1, 16384, 1, 0, 16, 16, 0) == 32 * 16 * 65536
     assert saved(11, 16384, 11, 0, 16, 16, 1) == 0
 
 
