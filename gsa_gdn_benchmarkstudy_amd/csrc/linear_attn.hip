@@ -19,14 +19,14 @@
 // outputs), the states between them (linear_join_kernel), all segments' outputs at once.
 //
 // A block takes a head: 8 waves of 16 columns of the state each, which stays in registers from chunk to chunk (tile_row: a
-// product's result is the next one's operand in the same lanes).  16384 tokens of 16 heads in bf16: state pass 36-39 us (134 MB,
-// 3.5 TB/s; its loads alone 28), join 12, outputs 74-76 (268 MB, 3.5 TB/s).  4 x 4096 tokens with gradients: besides, dk and dv
-// 161-169 us (0.54 GB) and dq with dg 186-203 (0.34 GB).  Of the outputs' cycles a quarter is MFMA and a third VALU
-// (98 MFMA, 460 VALU a wave and chunk: the splits in parts), which do not overlap within a SIMD; the rest waits for loads
-// and at the chunk's two barriers.  dq with dg: 216 MFMA and 1210 VALU, 63 % of its cycles.
-// Measured and not taken (us of the outputs' pass): a block a CU with all of the next chunk ahead 98 (V and the
-// outputs' stage in one buffer, two blocks: 88); outputs through LDS, three barriers a chunk: 85; operands read from LDS several
-// products ahead (schedule groups): the same within 1 %.
+// product's result is the next one's operand in the same lanes).  4 x 4096 tokens of 16 heads in bf16: state pass 39-42 us (0.1
+// GB, 2.5 TB/s; its loads alone, two blocks a CU, 28), join 6, outputs 86-91 (0.27 GB, 3.1 TB/s); with gradients besides dk and dv
+// 136-143 (0.54 GB, 3.9 TB/s) and dq with dg 157-169 (0.34 GB).  Of the outputs' cycles a quarter is MFMA and a quarter VALU
+// (98 MFMA, 400 VALU a wave and chunk: the splits in parts), a third each for dk and dv, which do not overlap within a SIMD; the rest
+// waits for loads and at the chunk's two barriers.  dq with dg: 216 MFMA and 1160 VALU, three quarters of its cycles.
+// Measured and not taken (us of the outputs' pass, two blocks a CU, now 76): one block a CU with all of the next chunk ahead 98
+// where V and the outputs' stage in one buffer gave 88; outputs through LDS, three barriers a chunk 85; operands read from LDS
+// several products ahead (schedule groups) the same within 1 %, as two parts of the values in X for three.
 //
 // Precision: as the gated delta rule's (mma): fp32 operands enter products as sums of three bf16 parts.  Where only a bf16
 // output depends on them two parts do, 2^-17 of a term under a rounding of 2^-9: X in Q X and P in P V (not where dg is
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<T, kOut, kDg>)) void linear_
 }
 
 // X before each segment but the pass's first from what the segments add: 256 threads, 1024 elements of a head's state.  Bound by
-// latency: 67 MB in 12 us where 16 heads have 32 segments, 11 us for 64 heads of 8.
+// latency: 33 MB in 6-8 us where 16 heads have 16 segments or 64 heads 4.
 __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int C) {
   const Pass& x = a.pass[0];
   const int n = blockIdx.x / a.Hv, h = blockIdx.x % a.Hv, e = blockIdx.y * 1024 + 4 * threadIdx.x;
