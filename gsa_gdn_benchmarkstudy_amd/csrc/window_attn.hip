@@ -798,16 +798,16 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   }
   auto slots = [&](int n) { return packed ? (int64_t)T / n + N : (int64_t)B * (((int64_t)T + n - 1) / n); };
   // 64 queries a block (two waves share their queries, each takes half of the keys) while 128 leave CUs idle: us forward, 16
-  // heads on 4, by 128 / 64 queries: T = 512 18 / 13, T = 1024, window 256 18 / 13, T = 2048 35 / 26, T = 4096, window 1024
-  // 49 / 53, B = 4 160 / 192; 4 heads T = 2000 52 / 30; fp32 B = 2 T = 1537, 4 heads 52 / 39, T = 4096, 16 heads 76 / 130.
+  // heads on 4, window 1024, by 128 / 64 queries: T = 512 18 / 13, T = 1024, window 256 18 / 14, T = 2048 35 / 28, T = 4096 48 / 54,
+  // B = 4 145 / 182; 4 heads T = 2000 33 / 21; fp32 B = 2 T = 1537, 4 heads 112 / 77, T = 4096, 16 heads 188 / 292.
   // (32 queries, four waves each a quarter of the keys: 15 at T = 512, 27 at T = 2000, worse at all others.)
   z.queries = slots(128) * H <= 256 ? 64 : 128;
   z.slots = slots(z.queries);
   // a grid of 256 threads a block: a launch has less than 2^32 of them
   if (slots(32) > (1 << 23) / H || (int64_t)B * T >= (int64_t)1 << 31) return false;
   // 64 keys a block (two waves share their keys, each takes half of the queries) while 128 leave CUs idle: us forward and
-  // backward, 16 heads on 4, window 1024, by 128 / 64: T = 4096 365 / 271, B = 4 T = 4096 706 / 720, T = 16384 802 / 823;
-  // on 16 heads T = 2048 170 / 151; window 64, T = 8192 210 / 191.  fp32 always 64 (registers): T = 4096, window 256 471 / 458.
+  // backward, 16 heads on 4, window 1024, by 128 / 64: T = 4096 252 / 245, B = 4 T = 4096 644 / 655, T = 16384 718 / 735;
+  // on 16 heads T = 2048 146 / 144, T = 4096 212 / 215; window 64, T = 8192 170 / 156.  fp32 always 64, for its registers.
   z.near_keys = dtype == GSA_DTYPE_BF16 && slots(128) * Hkv >= 512 ? 128 : 64;
   z.far_keys = dtype == GSA_DTYPE_BF16 ? 32 : 64;
   z.near = slots(z.near_keys);
