@@ -92,7 +92,7 @@ class WindowArgs(ctypes.Structure):
                 + [(f"{n}_{s}", _i64) for n in ("q", "k", "v") for s in ("sb", "st", "sh")]
                 + [("cu_seqlens", _vp)]
                 + [(n, _i32) for n in ("cu_bytes", "B", "T", "N", "H", "Hkv", "d", "dtype", "window", "sinks")]
-                + [("scale", _f32), ("o", _vp), ("lse", _vp), ("dout", _vp)]
+                + [("scale", _f32), ("o", _vp), ("lse", _vp), ("o_low", _vp), ("dout", _vp)]
                 + [(n, _i64) for n in ("do_sb", "do_st", "do_sh")]
                 + [(n, _vp) for n in ("dq", "dk", "dv", "ws")] + [("ws_bytes", ctypes.c_size_t)])
 
@@ -1227,30 +1227,31 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     return t if e == 1 and at % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _window_args(q, k, v, cu, window: int, sinks: int, scale: float, o, lse) -> WindowArgs:
+def _window_args(q, k, v, cu, window: int, sinks: int, scale: float, o, lse, low) -> WindowArgs:
     B, T, H, d = q.shape
     # in the order of the fields
     return WindowArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(cu),
                       0 if cu is None else cu.element_size(), B, T, B if cu is None else cu.numel() - 1, H, k.shape[2], d,
-                      dtype_code(q.dtype), window, sinks, scale, o.data_ptr(), _ptr(lse))
+                      dtype_code(q.dtype), window, sinks, scale, o.data_ptr(), _ptr(lse), _ptr(low))
 
 
-def window_attn(q, k, v, cu, window: int, sinks: int, scale: float, want_lse: bool):
-    """gsa_window_attn: (o, lse or None).  q, k, v as _heads gives them."""
+def window_attn(q, k, v, cu, window: int, sinks: int, scale: float, want_saved: bool):
+    """gsa_window_attn: (o, and what a backward pass needs besides or None: lse, bf16: the rest of o).  q, k, v as _heads gives them."""
     B, T, H, d = q.shape
     o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty(H, B * T, device=q.device, dtype=torch.float32) if want_lse else None
+    lse = torch.empty(H, B * T, device=q.device, dtype=torch.float32) if want_saved else None
+    low = torch.empty(q.shape, device=q.device, dtype=q.dtype) if want_saved and q.dtype == torch.bfloat16 else None
     if B * T:
-        st = load().gsa_window_attn(ctypes.byref(_window_args(q, k, v, cu, window, sinks, scale, o, lse)), _raw_stream(q))
+        st = load().gsa_window_attn(ctypes.byref(_window_args(q, k, v, cu, window, sinks, scale, o, lse, low)), _raw_stream(q))
         if st:
             _check(st, "gsa_window_attn")
-    return o, lse
+    return o, lse, low
 
 
-def window_attn_backward(q, k, v, cu, window: int, sinks: int, scale: float, o, lse, dout):
+def window_attn_backward(q, k, v, cu, window: int, sinks: int, scale: float, o, lse, low, dout):
     """gsa_window_attn_backward: (dq, dk, dv)."""
     dq, dk, dv = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
-    a = _window_args(q, k, v, cu, window, sinks, scale, o, lse)
+    a = _window_args(q, k, v, cu, window, sinks, scale, o, lse, low)
     if a.B * a.T == 0:
         return dq, dk, dv
     lib = load()

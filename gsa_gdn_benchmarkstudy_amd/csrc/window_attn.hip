@@ -23,7 +23,8 @@
 // 0 then): 505 us for 494 forward, 687 for 668 with gradients, for what the addresses cost; tiles of 64 keys forward and two
 // blocks a CU: slower throughout; dk and dv by one wave a SIMD: 857 for 707.
 //
-// Precision: sums, softmax statistics and D are fp32.  P and dS enter the second products in the inputs' type: bf16 (2^-9 of a
+// Precision: sums, softmax statistics and D are fp32, D from o with what its rounding to bf16 left (with the rounded o alone the
+// gradients' error is 1.7 times a rounding of theirs where 4 keys are visible, for 1.4).  P and dS enter the second products in the inputs' type: bf16 (2^-9 of a
 // term, as the inputs themselves were rounded), or, for fp32, as three bf16 parts each, as all fp32 operands do (chunks.h).
 #include "chunks.h"
 
@@ -36,7 +37,7 @@ struct WindowArgs {
   Rows q, k, v, dout;
   int B, H, Hkv, W, S;
   float scale, scale_l2;      // scale log2 e (forward: of |scale|, and above 0)
-  void* o;                    // [B, T, H, 128]
+  void *o, *low;              // [B, T, H, 128]; bf16: what o's rounding left, in bf16 (nullable)
   float* lse;                 // [H][B * T]: L (forward: nullable)
   float* D;                   // [H][B * T]
   void *dq, *dk, *dv;
@@ -243,7 +244,7 @@ template <int N> struct KeyTiles {
 
 // One query's output from its visible keys alone, a wave: lane l has elements 2 l, 2 l + 1.
 template <typename T>
-__device__ __forceinline__ void window_row(const WindowArgs& a, const T* q, const T* kbase, const T* vbase, int i, T* o, float* lse, int l) {
+__device__ __forceinline__ void window_row(const WindowArgs& a, const T* q, const T* kbase, const T* vbase, int i, T* o, T* low, float* lse, int l) {
   const float scale = a.scale * kLog2e;
   const float q0 = to_f32(q[2 * l]), q1 = to_f32(q[2 * l + 1]);
   float m = -__builtin_inff(), sum = 0.f, o0 = 0.f, o1 = 0.f;
@@ -262,8 +263,14 @@ __device__ __forceinline__ void window_row(const WindowArgs& a, const T* q, cons
     o1 = o1 * f + p * to_f32(v[2 * l + 1]);
     if (sum != sum) break;                                   // a score is NaN or +infinity: the whole row is NaN
   }
-  o[2 * l] = from_f32<T>(sum != sum ? sum : o0 / sum);
-  o[2 * l + 1] = from_f32<T>(sum != sum ? sum : o1 / sum);
+  o0 = sum != sum ? sum : o0 / sum;
+  o1 = sum != sum ? sum : o1 / sum;
+  o[2 * l] = from_f32<T>(o0);
+  o[2 * l + 1] = from_f32<T>(o1);
+  if (low) {
+    low[2 * l] = from_f32<T>(o0 - to_f32(from_f32<T>(o0)));
+    low[2 * l + 1] = from_f32<T>(o1 - to_f32(from_f32<T>(o1)));
+  }
   if (lse && l == 0) *lse = m + __builtin_amdgcn_logf(sum);
 }
 
@@ -283,7 +290,8 @@ template <typename T, int kGroups> struct WindowQueries : WindowTiles<T, kGroups
 };
 
 // A wave of a group: 32 kGroups queries a block, the wave's every kSplit-th 32 keys.
-template <typename T, int kGroups>
+// kP: parts of P (and dS) in the second products
+template <typename T, int kGroups, int kP>
 __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void window_fwd_kernel(WindowArgs a) {
   using Z = WindowQueries<T, kGroups>;
   using L = typename Z::L;
@@ -369,11 +377,13 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
         s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, minus));
         sum += s[r];
       }
+      {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const Parts<NP> p = parts_at<NP>(s, k);
+        for (int k = 0; k < 2; ++k) {
+          const Parts<kP> p = parts_at<kP>(s, k);
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) mma32(o[dt], cols.read(V, 32 * n + 16 * k, dt), p);
+          for (int dt = 0; dt < 4; ++dt) mma32(o[dt], cols.read(V, 32 * n + 16 * k, dt), p);
+        }
       }
     }
   };
@@ -409,13 +419,33 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
   }
   if (r0 >= sp.len) return;
   const int left = sp.len - r0;
-  T* out = static_cast<T*>(a.o) + (((int64_t)sp.b * a.s.T + sp.t0 + r0) * a.H + h) * kHead;
+  const int64_t to = (((int64_t)sp.b * a.s.T + sp.t0 + r0) * a.H + h) * kHead;
+  T *out = static_cast<T*>(a.o) + to, *low = a.low ? static_cast<T*>(a.low) + to : nullptr;
   float odd = sum * 0.f;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(o[dt][r], 0.f, odd);
   store_rows<T>(o, 1.f / sum, lds + group * 32 * kHead * sizeof(T), out, (int64_t)a.H * kHead, left, l);
+  if constexpr (NP == 1)
+    if (low) {
+      const float f = 1.f / sum;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        asm volatile("" : "+v"(o[dt]));                      // (else the rounded rows above are kept in registers for this)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          o[dt][r] *= f;
+          o[dt][r + 1] *= f;
+          float x = o[dt][r], y = o[dt][r + 1];
+          take_part(x, y);
+          o[dt][r] = x;
+          o[dt][r + 1] = y;
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the rows have been read back
+      store_rows<T>(o, 1.f, lds + group * 32 * kHead * sizeof(T), low, (int64_t)a.H * kHead, left, l);
+    }
   float* lse = a.lse ? a.lse + (int64_t)h * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 : nullptr;
   if (lse && row < sp.len && l < 32) lse[row] = m + __builtin_amdgcn_logf(sum);
   // A row with something that is not finite in its tiles: what it does not see may have reached it (0 * NaN), so it is
@@ -426,7 +456,7 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     for (int i = 0; i < min(32, left); ++i)
       if (redo >> i & 1)
-        window_row<T>(a, row_at<T>(a.q, sp, r0 + i, h), kbase, vbase, r0 + i, out + (int64_t)i * a.H * kHead, lse ? lse + r0 + i : nullptr, l);
+        window_row<T>(a, row_at<T>(a.q, sp, r0 + i, h), kbase, vbase, r0 + i, out + (int64_t)i * a.H * kHead, low ? low + (int64_t)i * a.H * kHead : nullptr, lse ? lse + r0 + i : nullptr, l);
   }
 }
 
@@ -451,7 +481,7 @@ __device__ __forceinline__ void join_waves(floatx16 (*const (&x)[kMany])[4], cha
 }
 
 // dq and D: a block's queries against the tiles of keys, as forwards.
-template <typename T, int kGroups>
+template <typename T, int kGroups, int kP>
 __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_dq_kernel(WindowArgs a) {
   using Z = WindowQueries<T, kGroups>;
   using L = typename Z::L;
@@ -487,6 +517,12 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
       float x[8], y[8];
       load8(o + 16 * ks + 8 * (l >> 5), x);
       load8(dout + 16 * ks + 8 * (l >> 5), y);
+      if (a.low) {
+        float z[8];
+        load8(static_cast<const T*>(a.low) + ((first + rowc) * a.H + h) * kHead + 16 * ks + 8 * (l >> 5), z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] += z[e];
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) D = __builtin_fmaf(x[e], y[e], D);
     }
@@ -532,11 +568,13 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = visible(a, row, j + 16 * (r >> 3) + (r & 7)) ? s[r] : 0.f;
       }
+      {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const Parts<NP> ds = parts_at<NP>(s, k);
+        for (int k = 0; k < 2; ++k) {
+          const Parts<kP> ds = parts_at<kP>(s, k);
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) mma32(acc[dt], cols.read(K, 32 * n + 16 * k, dt), ds);
+          for (int dt = 0; dt < 4; ++dt) mma32(acc[dt], cols.read(K, 32 * n + 16 * k, dt), ds);
+        }
       }
     }
   };
@@ -564,7 +602,7 @@ template <typename T, int kGroups, bool kFarPart> struct WindowKeys : WindowTile
 
 // dk and dv of 32 kGroups keys of a key head.  A wave has 32 of them, and of the tiles' queries each 4 / kGroups-th 32.
 // kFarPart: a part of the far queries of first tokens; otherwise the queries near the keys: all that see them, but for those.
-template <typename T, int kGroups, bool kFarPart>
+template <typename T, int kGroups, bool kFarPart, int kP>
 __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int index) {
   using Z = WindowKeys<T, kGroups, kFarPart>;
   using L = typename Z::L;
@@ -692,13 +730,15 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
           p[y] = on ? p[y] : 0.f;
         }
       }
+      {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const Parts<NP> w = parts_at<NP>(s, x), ds = parts_at<NP>(p, x);
+        for (int x = 0; x < 2; ++x) {
+          const Parts<kP> w = parts_at<kP>(s, x), ds = parts_at<kP>(p, x);
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
-          mma32(dv[dt], c.read(L::kBytes, 16 * x, dt), w);
-          mma32(dk[dt], c.read(0, 16 * x, dt), ds);
+          for (int dt = 0; dt < 4; ++dt) {
+            mma32(dv[dt], c.read(L::kBytes, 16 * x, dt), w);
+            mma32(dk[dt], c.read(0, 16 * x, dt), ds);
+          }
         }
       }
     }
@@ -723,10 +763,10 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
 }
 
 // (One kernel for both kinds of blocks would spill registers, and what reads those back waits for the tiles on their way.)
-template <typename T, int kGroups, bool kFarPart>
+template <typename T, int kGroups, bool kFarPart, int kP>
 __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_dkv_kernel(WindowArgs a) {
   extern __shared__ __align__(1024) char lds[];
-  window_dkv<T, kGroups, kFarPart>(a, lds, blockIdx.x);
+  window_dkv<T, kGroups, kFarPart, kP>(a, lds, blockIdx.x);
 }
 
 // dk and dv of what came in parts: of all keys (near_split > 1) or a sequence's first tokens; the near queries' parts and
@@ -834,6 +874,9 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   return true;
 }
 
+// Visible keys up to which P and dS take two parts: the rounding of few terms does not average (two visible keys' are one and the
+// same error over a whole row), and one tile's products more cost little there.
+constexpr int kFine = 128;
 int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, WindowPlan& z) {
   if (!x || !x->q || !x->k || !x->v || !x->o) return GSA_ERR_NULL;
   if (backward && (!x->dout || !x->dq || !x->dk || !x->dv || !x->lse || !x->ws)) return GSA_ERR_NULL;
@@ -850,7 +893,7 @@ int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, Win
   if (!vec(x->q, x->q_sb, x->q_st, x->q_sh) || !vec(x->k, x->k_sb, x->k_st, x->k_sh) || !vec(x->v, x->v_sb, x->v_st, x->v_sh) ||
       (backward && !vec(x->dout, x->do_sb, x->do_st, x->do_sh)))
     return GSA_ERR_ALIGN;
-  for (const void* p : {(const void*)x->o, (const void*)x->dq, (const void*)x->dk, (const void*)x->dv, (const void*)x->ws})
+  for (const void* p : {(const void*)x->o, (const void*)x->o_low, (const void*)x->dq, (const void*)x->dk, (const void*)x->dv, (const void*)x->ws})
     if (p && !aligned(p, 16)) return GSA_ERR_ALIGN;
   if (!aligned(x->lse, 4) || (x->cu_seqlens && !aligned(x->cu_seqlens, x->cu_bytes))) return GSA_ERR_ALIGN;
   a = gsa::WindowArgs{};
@@ -867,6 +910,7 @@ int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, Win
   a.scale_l2 = x->scale * gsa::kLog2e;
   if (!backward) a.scale_l2 = std::max(a.scale_l2 < 0.f ? -a.scale_l2 : a.scale_l2, 1.17549435e-38f);
   a.o = x->o;
+  a.low = x->dtype == GSA_DTYPE_BF16 ? x->o_low : nullptr;
   a.lse = x->lse;
   if (backward) {
     a.dout = {x->dout, x->do_sb, x->do_st, x->do_sh};
@@ -894,37 +938,37 @@ int window_outside(const gsa::WindowArgs& a, const gsa_window_args* x, bool back
   hipLaunchKernelGGL(gsa::outside_kernel, dim3(256), dim3(256), 0, s, o);
   return launch_status();
 }
-template <typename T, int kGroups> int launch_fwd(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+template <typename T, int kGroups, int kP> int launch_fwd(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
   constexpr size_t lds = gsa::WindowQueries<T, kGroups>::kBytes;
   static_assert(lds <= 160 * 1024);
-  if (const int e = allow_lds<gsa::window_fwd_kernel<T, kGroups>>(lds)) return e;
-  hipLaunchKernelGGL((gsa::window_fwd_kernel<T, kGroups>), dim3(z.slots * a.H), dim3(256), lds, s, a);
+  if (const int e = allow_lds<gsa::window_fwd_kernel<T, kGroups, kP>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::window_fwd_kernel<T, kGroups, kP>), dim3(z.slots * a.H), dim3(256), lds, s, a);
   return launch_status();
 }
-template <typename T, int kGroups> int launch_dq(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+template <typename T, int kGroups, int kP> int launch_dq(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
   constexpr size_t lds = gsa::WindowQueries<T, kGroups>::kBytes;
-  if (const int e = allow_lds<gsa::window_dq_kernel<T, kGroups>>(lds)) return e;
-  hipLaunchKernelGGL((gsa::window_dq_kernel<T, kGroups>), dim3(z.slots * a.H), dim3(256), lds, s, a);
+  if (const int e = allow_lds<gsa::window_dq_kernel<T, kGroups, kP>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::window_dq_kernel<T, kGroups, kP>), dim3(z.slots * a.H), dim3(256), lds, s, a);
   return launch_status();
 }
-template <typename T, int kGroups, bool kFarPart> int launch_dkv(const gsa::WindowArgs& a, int64_t blocks, hipStream_t s) {
+template <typename T, int kGroups, bool kFarPart, int kP> int launch_dkv(const gsa::WindowArgs& a, int64_t blocks, hipStream_t s) {
   constexpr size_t lds = gsa::WindowKeys<T, kGroups, kFarPart>::kBytes;
   static_assert(lds <= 160 * 1024);
-  if (const int e = allow_lds<gsa::window_dkv_kernel<T, kGroups, kFarPart>>(lds)) return e;
-  hipLaunchKernelGGL((gsa::window_dkv_kernel<T, kGroups, kFarPart>), dim3(blocks), dim3(256), lds, s, a);
+  if (const int e = allow_lds<gsa::window_dkv_kernel<T, kGroups, kFarPart, kP>>(lds)) return e;
+  hipLaunchKernelGGL((gsa::window_dkv_kernel<T, kGroups, kFarPart, kP>), dim3(blocks), dim3(256), lds, s, a);
   return launch_status();
 }
-template <typename T> int window_forward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
-  return z.queries == 64 ? launch_fwd<T, 2>(a, z, s) : launch_fwd<T, 4>(a, z, s);
+template <typename T, int kP> int window_forward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+  return z.queries == 64 ? launch_fwd<T, 2, kP>(a, z, s) : launch_fwd<T, 4, kP>(a, z, s);
 }
-template <typename T> int window_backward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
-  int e = z.queries == 64 ? launch_dq<T, 2>(a, z, s) : launch_dq<T, 4>(a, z, s);
+template <typename T, int kP> int window_backward(const gsa::WindowArgs& a, const WindowPlan& z, hipStream_t s) {
+  int e = z.queries == 64 ? launch_dq<T, 2, kP>(a, z, s) : launch_dq<T, 4, kP>(a, z, s);
   if (e) return e;
   const int64_t blocks = z.near * z.near_split * a.Hkv;
-  if constexpr (sizeof(T) == 2) e = z.near_keys == 128 ? launch_dkv<T, 4, false>(a, blocks, s) : launch_dkv<T, 2, false>(a, blocks, s);
-  else e = launch_dkv<T, 2, false>(a, blocks, s);
+  if constexpr (sizeof(T) == 2) e = z.near_keys == 128 ? launch_dkv<T, 4, false, kP>(a, blocks, s) : launch_dkv<T, 2, false, kP>(a, blocks, s);
+  else e = launch_dkv<T, 2, false, kP>(a, blocks, s);
   if (e) return e;
-  if (z.far && (e = launch_dkv<T, sizeof(T) == 2 ? 1 : 2, true>(a, z.far * a.H, s))) return e;
+  if (z.far && (e = launch_dkv<T, sizeof(T) == 2 ? 1 : 2, true, kP>(a, z.far * a.H, s))) return e;
   if (!z.far && z.near_split == 1) return GSA_OK;
   const int64_t units = z.near_split > 1 ? z.near : (int64_t)a.s.N * a.near_first;
   hipLaunchKernelGGL(gsa::window_join_kernel<T>, dim3(units * a.Hkv, a.near_keys / 8), dim3(256), 0, s, a);
@@ -943,7 +987,8 @@ extern "C" int gsa_window_attn(const gsa_window_args* x, void* stream) {
   gsa_host::WindowPlan z;
   if (const int e = gsa_host::window_args(x, false, a, z)) return e;
   const auto s = static_cast<hipStream_t>(stream);
-  const int e = x->dtype == GSA_DTYPE_BF16 ? gsa_host::window_forward<uint16_t>(a, z, s) : gsa_host::window_forward<float>(a, z, s);
+  const int e = x->dtype == GSA_DTYPE_F32 ? gsa_host::window_forward<float, 3>(a, z, s)
+                : a.W + a.S <= gsa_host::kFine ? gsa_host::window_forward<uint16_t, 2>(a, z, s) : gsa_host::window_forward<uint16_t, 1>(a, z, s);
   return e ? e : gsa_host::window_outside(a, x, false, s);
 }
 extern "C" int gsa_window_attn_backward(const gsa_window_args* x, void* stream) {
@@ -951,6 +996,7 @@ extern "C" int gsa_window_attn_backward(const gsa_window_args* x, void* stream) 
   gsa_host::WindowPlan z;
   if (const int e = gsa_host::window_args(x, true, a, z)) return e;
   const auto s = static_cast<hipStream_t>(stream);
-  const int e = x->dtype == GSA_DTYPE_BF16 ? gsa_host::window_backward<uint16_t>(a, z, s) : gsa_host::window_backward<float>(a, z, s);
+  const int e = x->dtype == GSA_DTYPE_F32 ? gsa_host::window_backward<float, 3>(a, z, s)
+                : a.W + a.S <= gsa_host::kFine ? gsa_host::window_backward<uint16_t, 2>(a, z, s) : gsa_host::window_backward<uint16_t, 1>(a, z, s);
   return e ? e : gsa_host::window_outside(a, x, true, s);
 }

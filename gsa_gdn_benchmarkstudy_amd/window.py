@@ -72,20 +72,20 @@ def _index(t: Optional[torch.Tensor], N: int, name: str):
 class _Window(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, window, sinks, scale):
-        o, lse = _abi.window_attn(q, k, v, cu, window, sinks, scale, True)
+        o, lse, low = _abi.window_attn(q, k, v, cu, window, sinks, scale, True)
         ctx.set_materialize_grads(False)
         ctx.window, ctx.sinks, ctx.scale = window, sinks, scale
-        ctx.save_for_backward(q, k, v, cu, o, lse)
+        ctx.save_for_backward(q, k, v, cu, o, lse, low)
         return o
 
     @_once
     def backward(ctx, do):
-        q, k, v, cu, o, lse = ctx.saved_tensors
+        q, k, v, cu, o, lse, low = ctx.saved_tensors
         if do is None:
             return (None,) * 7
         _range_push("gsa_hip/window_attention_backward")
         try:
-            grads = _abi.window_attn_backward(q, k, v, cu, ctx.window, ctx.sinks, ctx.scale, o, lse, _abi._heads(do))
+            grads = _abi.window_attn_backward(q, k, v, cu, ctx.window, ctx.sinks, ctx.scale, o, lse, low, _abi._heads(do))
         finally:
             _range_pop()
         return (*grads, None, None, None, None)

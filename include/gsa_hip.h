@@ -660,8 +660,9 @@ int gsa_linear_step(const void* q, int64_t q_sn, int64_t q_sh, const void* k, in
  * Attention in a sliding window with first tokens that stay visible: key j is visible to query i where j <= i and
  * (j > i - window or j < sinks), positions counted in each sequence.  No counterpart in the reference (its sparse
  * attention with a fixed selection).  q, o [B,T,H,128], k, v [B,T,Hkv,128] in dtype, head h on key head h / (H/Hkv);
- * o contiguous.  cu_seqlens as in gsa_delta_args.  The forward writes lse (fp32 [H][B*T], or NULL), which, with o, the
- * backward pass reads; that takes a workspace and writes dq, dk and dv (contiguous).  Rows of o and of the gradients outside
+ * o contiguous.  cu_seqlens as in gsa_delta_args.  The forward writes lse (fp32 [H][B*T], or NULL) and, in bf16, o_low (as o,
+ * or NULL: what o's rounding left, rounded), which, with o, the backward pass reads (without o_low its sums do . o carry o's
+ * rounding, which shows where few keys are visible); that takes a workspace and writes dq, dk and dv (contiguous).  Rows of o and of the gradients outside
  * every packed sequence become 0.  Head rows contiguous; q, k, v, dout rows 16-byte aligned, less than 32 MiB apart.
  * gsa_window_attn_workspace_bytes: 0 for sizes that are refused.
  */
@@ -673,6 +674,7 @@ typedef struct gsa_window_args {
   float scale;
   void* o;
   float* lse;
+  void* o_low;
   const void* dout;
   int64_t do_sb, do_st, do_sh;
   void *dq, *dk, *dv;

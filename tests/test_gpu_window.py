@@ -127,6 +127,20 @@ def test_many_blocks_packed(dev, dtype):
     _compare(_run(x, dev, 150, 4, cu=cu.to(dev), do=do), x, [(0, int(cu[i]), int(cu[i + 1])) for i in range(len(lens))], 150, 4, do)
 
 
+@pytest.mark.parametrize("W,S,few", [(1, 0, True), (2, 0, True), (4, 0, True), (16, 3, True), (100, 28, True), (129, 0, False), (1000, 0, False)])
+def test_bf16_errors_in_the_norm(dev, W, S, few):
+    """Where few keys are visible P and dS take two parts: results are off by their own rounding, the rest is 2^-17 of terms, under
+    a tenth of it in the norm.  Elsewhere by P's or dS's as well, which does not depend on theirs: the square root of 2 of one
+    rounding's error (1.41; sums over more than 128 terms and 1400 rows: within 1.47)."""
+    x, do = _inputs(2, 700, 4, 2, torch.bfloat16, seed=W), _grad(2, 700, 4, torch.bfloat16, 7)
+    got = _run(x, dev, W, S, do=do)
+    ref, size, _ = _oracle(x, [(0, 0, 700), (1, 0, 700)], W, S, D ** -0.5, do)
+    for n in got:
+        one = (ref[n].to(torch.bfloat16).double() - ref[n]).norm()
+        least = 2.0 ** -20 * size[n].norm()      # (one visible key: dq and dk are 0)
+        assert (got[n].double().cpu() - ref[n]).norm() <= (1.1 if few else 1.47) * one + least, n
+
+
 PACKS = [[1], [5, 0, 64, 1, 65, 63], [0, 0, 3], [130, 32, 33], [128, 64, 256], [0], [1300, 1, 0, 333]]
 
 

@@ -225,7 +225,7 @@ def test_c_linear_step_refusals(lib):
 
 def _window_c(lib, backward=False, **kw):
     a = _abi.WindowArgs(B=2, T=1000, N=2, H=2, Hkv=1, d=128, dtype=1, window=300, sinks=4, scale=0.1)
-    for n in ("q", "k", "v", "o", "lse", "ws", "dout", "dq", "dk", "dv"):
+    for n in ("q", "k", "v", "o", "lse", "o_low", "ws", "dout", "dq", "dk", "dv"):
         setattr(a, n, P)
     for n in ("q", "k", "v", "do"):
         setattr(a, n + "_sb", 256000), setattr(a, n + "_st", 256), setattr(a, n + "_sh", 128)
@@ -245,7 +245,7 @@ def test_c_window_refusals(lib):
                    dict(T=2 ** 31 - 1), dict(cu_seqlens=P, cu_bytes=4), dict(cu_seqlens=P, cu_bytes=2, B=1), dict(q_st=-256),
                    dict(k_st=1 << 24)):
             assert _window_c(lib, back, **kw) == 2, kw
-        for kw in (dict(q=P + 8), dict(k_st=257), dict(v_sb=4), dict(k_sh=132), dict(lse=MIS), dict(o=P + 8),
+        for kw in (dict(q=P + 8), dict(k_st=257), dict(v_sb=4), dict(k_sh=132), dict(lse=MIS), dict(o=P + 8), dict(o_low=P + 8),
                    dict(cu_seqlens=P + 2, cu_bytes=4, B=1, N=2)):
             assert _window_c(lib, back, **kw) == 4, kw
     assert _window_c(lib, True, ws_bytes=1024) == 2
