@@ -17,15 +17,16 @@
 // Bound by issue: a wave's 32 queries and 32 keys take 16 MFMA (512 cycles), 16 exponentials and some 90 further VALU (about as
 // many cycles), which do not overlap within a SIMD; three waves a SIMD hide most of what else there is.  Forward, 16384
 // tokens, window 4096, 16 heads on 4, bf16: 482-500 us, 0.98 PFLOP/s in the pairs that are seen (a large library product: 1.33).
-// 4 x 4096 tokens, window 1024, with gradients: forward 149-167 us, dq 214-240, dk and dv 278-310, far queries 31-34 (134 MB of
+// 4 x 4096 tokens, window 1024, with gradients: forward 155-167 us, dq 214-240, dk and dv 278-310, far queries 31-34 (134 MB of
 // q and do read once more: 28), their join 10.
 // Measured and not taken: a swizzle under which transposed reads meet in no bank (conflicts a third of LDS's cycles now,
 // 0 then): 505 us for 494 forward, 687 for 668 with gradients, for what the addresses cost; tiles of 64 keys forward and two
 // blocks a CU: slower throughout; dk and dv by one wave a SIMD: 857 for 707.
 //
 // Precision: sums, softmax statistics and D are fp32, D from o with what its rounding to bf16 left (with the rounded o alone the
-// gradients' error is 1.7 times a rounding of theirs where 4 keys are visible, for 1.4).  P and dS enter the second products in the inputs' type: bf16 (2^-9 of a
-// term, as the inputs themselves were rounded), or, for fp32, as three bf16 parts each, as all fp32 operands do (chunks.h).
+// gradients' error is 1.7 times a rounding of theirs where 4 keys are visible, for 1.4).  P and dS enter the second products in
+// bf16 (2^-9 of a term, as the inputs themselves were rounded; in two parts where few keys are visible: kFine), or, for fp32, as
+// three bf16 parts each, as all fp32 operands do (chunks.h).
 #include "chunks.h"
 
 #include <algorithm>
@@ -875,7 +876,9 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
 }
 
 // Visible keys up to which P and dS take two parts: the rounding of few terms does not average (two visible keys' are one and the
-// same error over a whole row), and one tile's products more cost little there.
+// same error over a whole row), and the further products cost little there.  us by one part / two: B = 4, T = 4096 with gradients, 68
+// keys 277 / 298, 128 310 / 338, 256 361 / 411, 512 467 / 563, 1028 670 / 861; T = 16384 forward, 128 66 / 65, 256 82 / 82, 512
+// 110 / 122, 4100 476 / 628.  Errors in the norm, in roundings of the result: one part 1.41 (few keys: up to 1.5), two 1.00.
 constexpr int kFine = 128;
 int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, WindowPlan& z) {
   if (!x || !x->q || !x->k || !x->v || !x->o) return GSA_ERR_NULL;
