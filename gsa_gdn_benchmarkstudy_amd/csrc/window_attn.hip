@@ -378,13 +378,11 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
         s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, minus));
         sum += s[r];
       }
-      {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const Parts<kP> p = parts_at<kP>(s, k);
+      for (int k = 0; k < 2; ++k) {
+        const Parts<kP> p = parts_at<kP>(s, k);
 #pragma unroll
-          for (int dt = 0; dt < 4; ++dt) mma32(o[dt], cols.read(V, 32 * n + 16 * k, dt), p);
-        }
+        for (int dt = 0; dt < 4; ++dt) mma32(o[dt], cols.read(V, 32 * n + 16 * k, dt), p);
       }
     }
   };
@@ -569,13 +567,11 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = visible(a, row, j + 16 * (r >> 3) + (r & 7)) ? s[r] : 0.f;
       }
-      {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const Parts<kP> ds = parts_at<kP>(s, k);
+      for (int k = 0; k < 2; ++k) {
+        const Parts<kP> ds = parts_at<kP>(s, k);
 #pragma unroll
-          for (int dt = 0; dt < 4; ++dt) mma32(acc[dt], cols.read(K, 32 * n + 16 * k, dt), ds);
-        }
+        for (int dt = 0; dt < 4; ++dt) mma32(acc[dt], cols.read(K, 32 * n + 16 * k, dt), ds);
       }
     }
   };
@@ -731,15 +727,13 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
           p[y] = on ? p[y] : 0.f;
         }
       }
-      {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const Parts<kP> w = parts_at<kP>(s, x), ds = parts_at<kP>(p, x);
+      for (int x = 0; x < 2; ++x) {
+        const Parts<kP> w = parts_at<kP>(s, x), ds = parts_at<kP>(p, x);
 #pragma unroll
-          for (int dt = 0; dt < 4; ++dt) {
-            mma32(dv[dt], c.read(L::kBytes, 16 * x, dt), w);
-            mma32(dk[dt], c.read(0, 16 * x, dt), ds);
-          }
+        for (int dt = 0; dt < 4; ++dt) {
+          mma32(dv[dt], c.read(L::kBytes, 16 * x, dt), w);
+          mma32(dk[dt], c.read(0, 16 * x, dt), ds);
         }
       }
     }
