@@ -25,7 +25,7 @@
 //
 // Precision: sums, softmax statistics and D are fp32, D from o with what its rounding to bf16 left (with the rounded o alone the
 // gradients' error is 1.7 times a rounding of theirs where 4 keys are visible, for 1.4).  P and dS enter the second products in
-// bf16 (2^-9 of a term, as the inputs themselves were rounded; in two parts where few keys are visible: kFine), or, for fp32, as
+// bf16 (2^-9 of a term, as the inputs themselves were rounded; in two parts where a query sees few keys: kFine), or, for fp32, as
 // three bf16 parts each, as all fp32 operands do (chunks.h).
 #include "chunks.h"
 
@@ -167,6 +167,15 @@ template <int NA, int NB> __device__ __forceinline__ void mma32(floatx16& acc, c
       for (int j = 0; j < NB; ++j)
         if (i + j == o) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
 }
+// Visible keys up to which P and dS of bf16 take two parts: the rounding of few terms does not average (two visible keys' are one and
+// the same error over a whole row).  Windows with first tokens of at most so many have kernels of their own (kP = 2): the further products
+// cost little there.  us by one part / two: B = 4, T = 4096 with gradients, 68 keys 277 / 298, 128 310 / 338, 256 361 / 411, 512 467 / 563,
+// 1028 670 / 861; T = 16384 forward, 128 66 / 65, 256 82 / 82, 512 110 / 122, 4100 476 / 628.  Under longer windows the queries that see
+// few keys are the first ones of a sequence: their products take the lower part beforehand (few_visible, add_low).  Errors in the
+// norm, in roundings of the result: one part 1.41 (few keys: up to 1.5), two 1.00.
+constexpr int kFine = 128;
+// All queries before i of a sequence do
+__device__ __forceinline__ bool few_visible(int i, const Span& sp) { return min(i, sp.len) <= kFine; }
 // The schedule of a product of kMany instructions (bf16), each with an operand from LDS: kAhead reads on their way before each
 // (the compiler's own is one, and waits for it).
 template <int kAhead, int kMany> __device__ __forceinline__ void reads_ahead() {
@@ -291,7 +300,7 @@ template <typename T, int kGroups> struct WindowQueries : WindowTiles<T, kGroups
 };
 
 // A wave of a group: 32 kGroups queries a block, the wave's every kSplit-th 32 keys.
-// kP: parts of P (and dS) in the second products
+// kP: parts of P (and dS) in the second products; 1: but for queries that see few keys
 template <typename T, int kGroups, int kP>
 __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void window_fwd_kernel(WindowArgs a) {
   using Z = WindowQueries<T, kGroups>;
@@ -331,7 +340,7 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
   // kLazy (the sums then stay below 2^8 times what they are, far from fp32's range)
   constexpr float kLazy = 8.f;
   float m = -__builtin_inff(), limit = m, minus = 0.f, sum = 0.f;
-  auto step = [&](int t, auto which) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
+  auto step = [&](int t, auto which, auto parts) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
     constexpr int buffer = kBuffers == 2 ? decltype(which)::value : 0;
     constexpr uint32_t K = buffer * kBuffer, V = K + L::kBytes;
     if constexpr (NP == 3) {
@@ -380,16 +389,20 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const Parts<kP> p = parts_at<kP>(s, k);
+        const auto p = parts_at<decltype(parts)::value>(s, k);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) mma32(o[dt], cols.read(V, 32 * n + 16 * k, dt), p);
       }
     }
   };
-  for (int t = 0; t < tiles.count; t += 2) {
-    step(t, Number<0>{});
-    if (t + 1 < tiles.count) step(t + 1, Number<1>{});
-  }
+  auto walk = [&](auto parts) __attribute__((always_inline)) {
+    for (int t = 0; t < tiles.count; t += 2) {
+      step(t, Number<0>{}, parts);
+      if (t + 1 < tiles.count) step(t + 1, Number<1>{}, parts);
+    }
+  };
+  if (kP == 1 && few_visible(q0 + kQueries, sp)) walk(Number<2>{});
+  else walk(Number<kP>{});
   sum = sum_halves(sum);
   __syncthreads();                                           // the tiles are free
   if constexpr (kSplit > 1) {
@@ -535,7 +548,7 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
   for (int dt = 0; dt < 4; ++dt) zero(acc[dt]);
   const typename L::RowReader rows(base, l);
   const typename L::ColReader cols(base, l);
-  auto step = [&](int t, auto which) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
+  auto step = [&](int t, auto which, auto parts) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
     constexpr int buffer = kBuffers == 2 ? decltype(which)::value : 0;
     constexpr uint32_t K = buffer * kBuffer, V = K + L::kBytes;
     if constexpr (NP == 3) {
@@ -569,16 +582,20 @@ __global__ __launch_bounds__(256, (WindowType<T>::NP == 1 ? 2 : 1)) void window_
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const Parts<kP> ds = parts_at<kP>(s, k);
+        const auto ds = parts_at<decltype(parts)::value>(s, k);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) mma32(acc[dt], cols.read(K, 32 * n + 16 * k, dt), ds);
       }
     }
   };
-  for (int t = 0; t < tiles.count; t += 2) {
-    step(t, Number<0>{});
-    if (t + 1 < tiles.count) step(t + 1, Number<1>{});
-  }
+  auto walk = [&](auto parts) __attribute__((always_inline)) {
+    for (int t = 0; t < tiles.count; t += 2) {
+      step(t, Number<0>{}, parts);
+      if (t + 1 < tiles.count) step(t + 1, Number<1>{}, parts);
+    }
+  };
+  if (kP == 1 && few_visible(q0 + kQueries, sp)) walk(Number<2>{});
+  else walk(Number<kP>{});
   __syncthreads();                                           // the tiles are free
   if constexpr (kSplit > 1) {
     join_waves<kGroups, kSplit, 1>({&acc}, lds, group, split, l);
@@ -644,15 +661,17 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
   const int j0 = k0 + 32 * group, key = j0 + (l & 31), keyc = min(key, sp.len - 1);
   const int tiles = (i1 - i0 + N - 1) / N, all = tiles * heads;
   const int first = kFarPart ? 0 : (int)((int64_t)all * part / a.near_split), count = kFarPart ? all : (int)((int64_t)all * (part + 1) / a.near_split);
+  const T *q0 = uniform(row_at<T>(a.q, sp, i0, h0)), *d0 = uniform(row_at<T>(a.dout, sp, i0, h0));
+  const int64_t stat0 = (int64_t)h0 * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 + i0;
   typename L::Loader lq(a.q.st, wave, l), ld(a.dout.st, wave, l);
   constexpr int kStatRow = N < 64 ? 64 : N;                  // L of a tile's queries, then D, each a wave's 64 or two
   auto load = [&](int t, int buffer) {
-    const int h = h0 + t / tiles, r = i0 + t % tiles * N, left = min(sp.len, i1) - r;
-    lq.load(row_at<T>(a.q, sp, r, h), a.q.st, left, base + buffer * kBuffer, wave, l);
-    ld.load(row_at<T>(a.dout, sp, r, h), a.dout.st, left, base + buffer * kBuffer + L::kBytes, wave, l);
+    const int h = t / tiles, r = t % tiles * N, left = i1 - i0 - r;
+    lq.load(q0 + r * a.q.st + h * a.q.sh, a.q.st, left, base + buffer * kBuffer, wave, l);
+    ld.load(d0 + r * a.dout.st + h * a.dout.sh, a.dout.st, left, base + buffer * kBuffer + L::kBytes, wave, l);
     if (wave < kStatRow / 32) {
       const int which = wave / (kStatRow / 64), t0 = 64 * (wave % (kStatRow / 64));
-      const float* p = uniform((which ? a.D : a.lse) + (int64_t)h * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 + r);
+      const float* p = uniform((which ? a.D : a.lse) + stat0 + (int64_t)h * a.B * a.s.T + r);
       load_lds4(p, 4u * min(t0 + l, left - 1), __builtin_amdgcn_readfirstlane(base + Z::kStats + 4 * (((t & 1) * 2 + which) * kStatRow + t0)));
     }
   };
@@ -669,74 +688,89 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
   }
   const typename L::RowReader rows(base, l);
   const typename L::ColReader cols(base, l);
-  for (int t = first; t < count; ++t) {
-    const int buffer = kBuffers == 2 ? t & 1 : 0;
-    char *Q = lds + buffer * kBuffer, *dO = Q + L::kBytes;
-    const float* st = reinterpret_cast<const float*>(lds + Z::kStats) + (t & 1) * 2 * kStatRow;
-    if constexpr (kBuffers == 1) {
-      if (t > first) __syncthreads();                        // every wave is through with the last tile
-      if (!kAhead) load(t, 0);
-      lq.store(Q, wave, l);
-      ld.store(dO, wave, l);
-    }
-    wait_loads();
-    __syncthreads();
-    if (kAhead && t + 1 < count) load(t + 1, buffer ^ 1);
-    const int r0 = i0 + t % tiles * N;
-    if (j0 >= sp.len) continue;
+  auto walk = [&](int from, int to, auto parts) __attribute__((always_inline)) {
+    constexpr int kParts = decltype(parts)::value;
+    for (int t = from; t < to; ++t) {
+      const int buffer = kBuffers == 2 ? t & 1 : 0;
+      char *Q = lds + buffer * kBuffer, *dO = Q + L::kBytes;
+      const float* st = reinterpret_cast<const float*>(lds + Z::kStats) + (t & 1) * 2 * kStatRow;
+      if constexpr (kBuffers == 1) {
+        if (t > first) __syncthreads();                        // every wave is through with the last tile
+        if (!kAhead) load(t, 0);
+        lq.store(Q, wave, l);
+        ld.store(dO, wave, l);
+      }
+      wait_loads();
+      __syncthreads();
+      if (kAhead && t + 1 < count) load(t + 1, buffer ^ 1);
+      const int r0 = i0 + t % tiles * N;
+      if (j0 >= sp.len) continue;
 #pragma unroll 1                                             // (unrolled, two such products at once do not fit the registers)
-    for (int n = split; n < N / 32; n += kSplit) {
-      const int i32 = r0 + 32 * n;                           // the 32 queries of this product
-      const int see = i32 < i1 ? seen<32>(a, i32, j0) : 0;
-      if (!see) continue;
-      // (for this product alone: kept over the loop, the 8 addresses of rows would cost registers)
-      typename L::RowReader r = rows;
-      typename L::ColReader c = cols;
-      const int shift = buffer * kBuffer + 32 * n * 256;
-      r.at = here(rows.at + shift);
-      c.at[0] = here(cols.at[0] + shift);
-      c.at[1] = here(cols.at[1] + shift);
-      floatx16 s, p;
-      zero(s);
-      zero(p);
+      for (int n = split; n < N / 32; n += kSplit) {
+        const int i32 = r0 + 32 * n;                           // the 32 queries of this product
+        const int see = i32 < i1 ? seen<32>(a, i32, j0) : 0;
+        if (!see) continue;
+        // (for this product alone: kept over the loop, the 8 addresses of rows would cost registers)
+        typename L::RowReader r = rows;
+        typename L::ColReader c = cols;
+        const int shift = buffer * kBuffer + 32 * n * 256;
+        r.at = here(rows.at + shift);
+        c.at[0] = here(cols.at[0] + shift);
+        c.at[1] = here(cols.at[1] + shift);
+        floatx16 s, p;
+        zero(s);
+        zero(p);
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        mma32(s, r.read(0, 0, ks), k[ks]);
-        mma32(p, r.read(L::kBytes, 0, ks), v[ks]);
-      }
-      if constexpr (NP == 1) reads_ahead<3, 16>();           // (1: 293 us, 2 280, 3 278, 4 281; 4 x 4096 tokens, window 1024)
-      asm volatile("" : "+v"(s), "+v"(p));
-      const float* stats = st + 32 * n + 8 * (here(l) >> 5);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float y[8];
-        load8(stats + 16 * x, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[8 * x + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * x + e], a.scale_l2, -y[e]));
-        load8(stats + kStatRow + 16 * x, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p[8 * x + e] = s[8 * x + e] * (p[8 * x + e] - y[e]);
-      }
-      if (see == 1 || i32 + 32 > i1) {
-        const int lh = here(l), i = i32 + 8 * (lh >> 5), j = j0 + (lh & 31);
-#pragma unroll
-        for (int y = 0; y < 16; ++y) {
-          const int ir = i + 16 * (y >> 3) + (y & 7);
-          const bool on = ir < i1 && visible(a, ir, j);
-          s[y] = on ? s[y] : 0.f;
-          p[y] = on ? p[y] : 0.f;
+        for (int ks = 0; ks < 8; ++ks) {
+          mma32(s, r.read(0, 0, ks), k[ks]);
+          mma32(p, r.read(L::kBytes, 0, ks), v[ks]);
         }
-      }
+        if constexpr (NP == 1) reads_ahead<3, 16>();           // (1: 293 us, 2 280, 3 278, 4 281; 4 x 4096 tokens, window 1024)
+        asm volatile("" : "+v"(s), "+v"(p));
+        const float* stats = st + 32 * n + 8 * (here(l) >> 5);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const Parts<kP> w = parts_at<kP>(s, x), ds = parts_at<kP>(p, x);
+        for (int x = 0; x < 2; ++x) {
+          float y[8];
+          load8(stats + 16 * x, y);
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
-          mma32(dv[dt], c.read(L::kBytes, 16 * x, dt), w);
-          mma32(dk[dt], c.read(0, 16 * x, dt), ds);
+          for (int e = 0; e < 8; ++e) s[8 * x + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * x + e], a.scale_l2, -y[e]));
+          load8(stats + kStatRow + 16 * x, y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[8 * x + e] = s[8 * x + e] * (p[8 * x + e] - y[e]);
+        }
+        if (see == 1 || i32 + 32 > i1) {
+          const int lh = here(l), i = i32 + 8 * (lh >> 5), j = j0 + (lh & 31);
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            const int ir = i + 16 * (y >> 3) + (y & 7);
+            const bool on = ir < i1 && visible(a, ir, j);
+            s[y] = on ? s[y] : 0.f;
+            p[y] = on ? p[y] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const auto w = parts_at<kParts>(s, x), ds = parts_at<kParts>(p, x);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) {
+            mma32(dv[dt], c.read(L::kBytes, 16 * x, dt), w);
+            mma32(dk[dt], c.read(0, 16 * x, dt), ds);
+          }
         }
       }
     }
+  };
+  // Queries that see few keys, then the others of a head (a loop each: both kinds in one would spill registers)
+  if constexpr (kP == 1) {
+    const int few = std::clamp((kFine - i0 + N - 1) / N, 0, tiles);
+    for (int t = first; t < count;) {
+      const int head = t / tiles * tiles, end = min(head + tiles, count), mid = std::clamp(head + few, t, end);
+      walk(t, mid, Number<2>{});
+      walk(mid, end, Number<1>{});
+      t = end;
+    }
+  } else {
+    walk(first, count, Number<kP>{});
   }
   __syncthreads();                                           // the tiles are free
   if constexpr (kSplit > 1) {
@@ -869,11 +903,6 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   return true;
 }
 
-// Visible keys up to which P and dS take two parts: the rounding of few terms does not average (two visible keys' are one and the
-// same error over a whole row), and the further products cost little there.  us by one part / two: B = 4, T = 4096 with gradients, 68
-// keys 277 / 298, 128 310 / 338, 256 361 / 411, 512 467 / 563, 1028 670 / 861; T = 16384 forward, 128 66 / 65, 256 82 / 82, 512
-// 110 / 122, 4100 476 / 628.  Errors in the norm, in roundings of the result: one part 1.41 (few keys: up to 1.5), two 1.00.
-constexpr int kFine = 128;
 int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, WindowPlan& z) {
   if (!x || !x->q || !x->k || !x->v || !x->o) return GSA_ERR_NULL;
   if (backward && (!x->dout || !x->dq || !x->dk || !x->dv || !x->lse || !x->ws)) return GSA_ERR_NULL;
@@ -985,7 +1014,7 @@ extern "C" int gsa_window_attn(const gsa_window_args* x, void* stream) {
   if (const int e = gsa_host::window_args(x, false, a, z)) return e;
   const auto s = static_cast<hipStream_t>(stream);
   const int e = x->dtype == GSA_DTYPE_F32 ? gsa_host::window_forward<float, 3>(a, z, s)
-                : a.W + a.S <= gsa_host::kFine ? gsa_host::window_forward<uint16_t, 2>(a, z, s) : gsa_host::window_forward<uint16_t, 1>(a, z, s);
+                : a.W + a.S <= gsa::kFine ? gsa_host::window_forward<uint16_t, 2>(a, z, s) : gsa_host::window_forward<uint16_t, 1>(a, z, s);
   return e ? e : gsa_host::window_outside(a, x, false, s);
 }
 extern "C" int gsa_window_attn_backward(const gsa_window_args* x, void* stream) {
@@ -994,6 +1023,6 @@ extern "C" int gsa_window_attn_backward(const gsa_window_args* x, void* stream) 
   if (const int e = gsa_host::window_args(x, true, a, z)) return e;
   const auto s = static_cast<hipStream_t>(stream);
   const int e = x->dtype == GSA_DTYPE_F32 ? gsa_host::window_backward<float, 3>(a, z, s)
-                : a.W + a.S <= gsa_host::kFine ? gsa_host::window_backward<uint16_t, 2>(a, z, s) : gsa_host::window_backward<uint16_t, 1>(a, z, s);
+                : a.W + a.S <= gsa::kFine ? gsa_host::window_backward<uint16_t, 2>(a, z, s) : gsa_host::window_backward<uint16_t, 1>(a, z, s);
   return e ? e : gsa_host::window_outside(a, x, true, s);
 }
