@@ -61,12 +61,32 @@ struct LinearArgs {
 };
 constexpr int kOutside = 64;
 
-// g in units of log2.  e^-128 is 0 in fp32: a lower g (down to -inf, a reset) gives the same without inf * 0.
-__device__ __forceinline__ float log2_decay(const float* g) {
-  const float x = *g;
-  return (x < -128.f ? -128.f : x) * kLog2e;
+// e^-128 is 0 in fp32: a lower g (down to -inf, a reset) gives the same without inf * 0.
+struct Decay { float g, hi, lo; };                           // hi + lo: g in units of log2
+__device__ __forceinline__ Decay decay_of(const float* p) {
+  const float x = *p, g = x < -128.f ? -128.f : x, hi = g * kLog2e;
+  return {g, hi, __builtin_fmaf(g, 1.9259629911e-8f, __builtin_fmaf(g, kLog2e, -hi))};       // (log2 e less its fp32 value)
 }
-__device__ __forceinline__ float power(float g2, int n) { return __builtin_amdgcn_exp2f(g2 * (float)n); }
+// e^(g n), one exp2's error whatever n: what the exponent's rounding left comes in by its first term.
+__device__ __forceinline__ float power(const Decay& d, int n) {
+  const float t = d.hi * (float)n, rest = __builtin_fmaf(d.hi, (float)n, -t) + d.lo * (float)n, y = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(y, rest * 0.69314718f, y);
+}
+// e^(g n) in two floats, a factor that a state is multiplied with again and again: its rounding would come in once for each chunk
+// that a term passes (fp32, 2050 chunks in one piece, g = -2e-5: 2.9e-5 of the state; so 5e-7).  So what rounding a factor leaves
+// goes into the next one, and the product of any number of them in a row is off by one rounding.
+struct Whole { float hi, lo; };
+__device__ __forceinline__ Whole whole_power(const Decay& d, int n) {
+  const double y = exp((double)d.g * n);
+  const float hi = (float)y;
+  return {hi, hi < __builtin_inff() ? (float)(y - hi) : 0.f};
+}
+struct Factors { Whole w; float left[kWaves]; };             // a^C of whole chunks; in LDS, as registers are short
+__device__ __forceinline__ float next_factor(const Whole& w, float& left) {
+  const float t = w.lo + left, y = w.hi + t;
+  left = t - (y - w.hi);
+  return y;
+}
 
 // The matrix cores cut what they add to an accumulator below its last bit, always downwards.  So the products of smaller
 // parts are summed apart, where that is less, and sums over many chunks (X) take each chunk's sum by an fma.
@@ -126,9 +146,9 @@ template <typename T, bool kDg, Ahead kAhead> struct LinearSizes {
   // keys, values and dot (what goes ahead twice, kGroup apart); rows, P
   static constexpr int kB = 0, kV = (kAhead == kKeys ? 2 : 1) * kRows, kDot = 2 * kRows, kGroup = (kAhead == kKeys ? 1 : kDg ? 3 : 2) * kRows;
   static constexpr int kA = kAhead == kKeys ? kV + kRows : (kAhead == kAll ? 2 : 1) * kGroup, kAtP = kA + kRows;
-  // powers of the decay: in_x a^(C-1-t), in_o a^(t+1)
+  // powers of the decay: in_x a^(C-1-t), in_o a^(t+1); the chunks' factors
   static constexpr int kToEnd = kAtP + kP, kFromX = kToEnd + 4 * C;
-  static constexpr size_t kBytes = kFromX + 4 * C, kState = kA + 4 * C;
+  static constexpr size_t kBytes = kFromX + 4 * C + sizeof(Factors), kState = kA + 4 * C + sizeof(Factors);
 };
 
 template <int N> __device__ __forceinline__ float element(const Parts<N>& x, int e) {
@@ -186,7 +206,7 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
   const bool begins = x.back ? last : piece == 0, ends = x.back ? piece == 0 : last;    // the pass's first and last segment
   if (!kOut && ends) return;                                 // nobody asks for it
   const int64_t sn = ((int64_t)sp.n * a.Hv + h) * kHead * kHead, gn = ((int64_t)slot * a.Hv + h) * kHead * kHead;
-  const float g2 = log2_decay(a.g + h * a.g_sh);
+  const Decay g2 = decay_of(a.g + h * a.g_sh);
   const int col = tile_row(wave, m);                         // this lane's column of the state and the outputs
 
   floatx4 X[8][1], X2[kDg ? 8 : 1];
@@ -243,6 +263,9 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
     to_end[tid] = x.in_x * power(g2, C - 1 - tid);
     if (kOut) to_end[C + tid] = x.in_o * power(g2, tid + 1);
   }
+  Factors* const a_whole = reinterpret_cast<Factors*>(to_end + (kOut ? 2 * C : C));
+  if (tid == 0) a_whole->w = whole_power(g2, C);
+  a_whole->left[wave] = 0.f;
   // P: row tile pt of it by the waves pt, pt + MT, ..; this wave's columns are tile part or tiles 2 part, 2 part + 1
   const int pt = wave % MT, part = wave / MT;
   constexpr int kTiles = C == 64 ? 2 : 1;
@@ -272,7 +295,6 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
     const int left = min(C, sp.len - c * C);
     // steps of decay from X to the chunk's first token: 1, or (the gradient of the final state) 0
     const int lead = x.back && c == chunks - 1 ? 0 : 1;
-    const float whole = power(g2, left - 1 + lead);
     wait_loads();
     __syncthreads();
     const int vals = (kAhead == kKeys ? 0 : group) + Z::kV;
@@ -449,6 +471,14 @@ __device__ __forceinline__ void linear_scan(const LinearArgs& a, const Pass& x, 
 
     // the values times the decay to the chunk's end
     asm volatile("" ::: "memory");                           // (read again: kept over P V they would cost registers)
+    float whole;
+    if (c == chunks - 1) {
+      whole = power(g2, left - 1 + lead);
+    } else {
+      float rest = a_whole->left[wave];
+      whole = next_factor(a_whole->w, rest);
+      a_whole->left[wave] = rest;
+    }
     Parts<3> vd[JS], vd2[kDg ? JS : 1];
 #pragma unroll
     for (int js = 0; js < JS; ++js) {
@@ -568,9 +598,12 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int C) {
   if (segs == 0 && x.last)                                   // an empty sequence: no block has it
     *reinterpret_cast<floatx4*>(x.last + sn) = x.first ? *reinterpret_cast<const floatx4*>(x.first + sn) : floatx4{0.f, 0.f, 0.f, 0.f};
   if (segs < 2) return;
-  const float g2 = log2_decay(a.g + h * a.g_sh);
+  const Decay g2 = decay_of(a.g + h * a.g_sh);
   floatx4 X = {0.f, 0.f, 0.f, 0.f};
   if (x.first) X = *reinterpret_cast<const floatx4*>(x.first + sn);
+  // the last tokens' segment may be short, and no decay lies before the gradient of the final state
+  const Whole whole = whole_power(g2, tokens);
+  float left = 0.f;
   auto at = [&](int i) { return ((int64_t)(sp.slot0 + (x.back ? segs - 1 - i : i)) * a.Hv + h) * kHead * kHead + e; };
   constexpr int kSome = 8;                                   // loads on their way at once (32 segments of 16 heads: 12 us, one by one 14)
   for (int i0 = 0; i0 + 1 < segs; i0 += kSome) {
@@ -581,9 +614,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int C) {
     for (int k = 0; k < kSome; ++k) {
       const int i = i0 + k;
       if (i + 1 >= segs) break;
-      // the last tokens' segment may be short, and no decay lies before the gradient of the final state
-      const int steps = x.back && i == 0 ? sp.len - (segs - 1) * tokens - 1 : tokens;
-      const float f = power(g2, steps);
+      const float f = x.back && i == 0 ? power(g2, sp.len - (segs - 1) * tokens - 1) : next_factor(whole, left);
 #pragma unroll
       for (int r = 0; r < 4; ++r) X[r] = __builtin_fmaf(X[r], f, add[k][r]);
       *reinterpret_cast<floatx4*>(const_cast<float*>(x.init) + at(i + 1)) = X;
