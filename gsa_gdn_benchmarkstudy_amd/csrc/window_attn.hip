@@ -30,8 +30,19 @@
 #include "chunks.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace gsa {
+
+// Where something is kept of blocks of sequences' first tokens.  Only sequences longer than the window have such blocks, so the
+// places are bounded by the tokens and not by the sequences: of a sequence from token t on, block b is in place t / div * mult + b,
+// with div the least tokens of such a sequence and mult the blocks of one, or, where that is fewer, div the keys of a
+// block (each block holds that many tokens of its own) and mult 1; div 0: sequence n's blocks from n * mult on.  The parts of far queries
+// behind a sequence's first part go by the same rule, as blocks of as many tokens as they have queries.
+struct FirstPlaces {
+  int div, mult;
+  __device__ int at(int n, int start, int b) const { return (div ? start / div : n) * mult + b; }
+};
 
 struct WindowArgs {
   Seqs s;
@@ -46,7 +57,10 @@ struct WindowArgs {
   int near_keys, near_first, far_keys, far_first, far_rows;            // first: blocks of a sequence's first tokens
   int near_split;             // parts that a block's queries are cut into
   float* near_parts;          // [N][near_first][Hkv][2][near_keys][128]; near_split > 1: [slots of keys][Hkv][near_split][2][..
-  float* far_parts;           // [slots of far queries][far_first][H][2][far_keys][128]
+  // the first far_rows far queries of a block are in far_at's places, the further ones behind those: more_at's places, far_first each
+  FirstPlaces far_at, more_at;
+  int far_places, more;       // more: further parts of a sequence, at most
+  float* far_parts;           // [places][H][2][far_keys][128]
 };
 
 template <int N> struct Number { static constexpr int value = N; };
@@ -614,6 +628,35 @@ template <typename T, int kGroups, bool kFarPart> struct WindowKeys : WindowTile
   static constexpr size_t kBytes = kStats + 2 * 2 * std::max(64, Base::L::N) * 4;
 };
 
+// A sequence's first token, counted over all rows of a batch; the sequence that holds a token (len 0: none does).
+__device__ __forceinline__ int start_of(const Seqs& s, const Span& sp) { return s.cu ? sp.t0 : sp.n * s.T; }
+__device__ __forceinline__ Span holder(const Seqs& s, int token) {
+  int lo = 0;
+  if (!s.cu) {
+    lo = token / s.T;
+  } else {
+    for (int hi = s.N - 1; lo < hi;) {                       // the last sequence that does not begin behind it
+      const int m = (lo + hi + 1) / 2;
+      if (__builtin_amdgcn_readfirstlane((int)s.at(m)) <= token) lo = m; else hi = m - 1;
+    }
+  }
+  Span sp = span_of(s, lo, 1);
+  const int t = token - start_of(s, sp);
+  if (t < 0 || t >= sp.len) sp.len = 0;
+  return sp;
+}
+// The sequence and block of a place; len 0: none.
+__device__ __forceinline__ Span holder(const Seqs& s, const FirstPlaces& p, int place, int blocks, int& b) {
+  if (!p.div) {
+    b = place % p.mult;
+    return span_of(s, place / p.mult, 1);
+  }
+  Span sp = holder(s, (int)min((int64_t)INT_MAX, (int64_t)(place / p.mult + 1) * p.div - 1));
+  b = place - start_of(s, sp) / p.div * p.mult;
+  if (b < 0 || b >= blocks) sp.len = 0;
+  return sp;
+}
+
 // dk and dv of 32 kGroups keys of a key head.  A wave has 32 of them, and of the tiles' queries each 4 / kGroups-th 32.
 // kFarPart: a part of the far queries of first tokens; otherwise the queries near the keys: all that see them, but for those.
 template <typename T, int kGroups, bool kFarPart, int kP>
@@ -646,16 +689,21 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
     hk = h0 / share;
     heads = 1;
     unit = index / a.H;
-    const int block = unit % a.far_first;
-    unit /= a.far_first;
-    sp = slot_of(a.s, unit, a.far_rows, c);
+    int block;
+    if (unit < a.far_places) {
+      sp = holder(a.s, a.far_at, unit, a.far_first, block);
+      c = 0;
+    } else {
+      block = (unit - a.far_places) % a.far_first;
+      sp = holder(a.s, a.more_at, (unit - a.far_places) / a.far_first, a.more, c);
+      ++c;
+    }
     k0 = block * kKeys;
-    if (c < 0 || k0 >= sp.len) return;
-    const int64_t end = (int64_t)k0 / a.near_keys * a.near_keys + a.near_keys - 1 + a.W;
-    i0 = (int)max((int64_t)c * a.far_rows, min((int64_t)sp.len, end));
-    i1 = min(sp.len, (c + 1) * a.far_rows);
-    if (i0 >= i1) return;
-    parts = a.far_parts + (((int64_t)unit * a.far_first + block) * a.H + h0) * 2 * kKeys * kHead;
+    const int64_t from = (int64_t)k0 / a.near_keys * a.near_keys + a.near_keys - 1 + a.W + (int64_t)c * a.far_rows;
+    if (k0 >= a.S || from >= sp.len) return;
+    i0 = (int)from;
+    i1 = (int)min((int64_t)sp.len, from + a.far_rows);
+    parts = a.far_parts + ((int64_t)unit * a.H + h0) * 2 * kKeys * kHead;
   }
   const int group = wave % kGroups, split = kSplit > 1 ? wave / kGroups : 0;
   const int j0 = k0 + 32 * group, key = j0 + (l & 31), keyc = min(key, sp.len - 1);
@@ -804,7 +852,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
   const int hk = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv, share = a.H / a.Hkv;
   Span sp;
-  int block, far_slot;
+  int block;
   if (a.near_split > 1) {
     sp = slot_of(a.s, unit, a.near_keys, block);
     if (block < 0) return;
@@ -816,7 +864,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
   const int64_t end = (int64_t)k0 + a.near_keys - 1 + a.W;
   const bool far_too = k0 < a.S && end < sp.len;
   if (k0 >= sp.len || (a.near_split == 1 && !far_too)) return;         // (written as they were)
-  far_slot = far_too ? span_of(a.s, sp.n, a.far_rows).slot0 : 0;
+  const int start = start_of(a.s, sp);
   const int near = a.near_keys * kHead, far = a.far_keys * kHead;
   const float* parts = a.near_parts + (int64_t)blockIdx.x * a.near_split * 2 * near;
   for (int u = threadIdx.x + 256 * blockIdx.y; u < 2 * near / 8; u += 256 * gridDim.y) {
@@ -832,13 +880,15 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
     }
     if (far_too && key < a.S) {                              // (the others have no far queries)
       const int fb = key / a.far_keys, at = which * far + key % a.far_keys * kHead + e;
-      for (int c = (int)(end / a.far_rows); c * a.far_rows < sp.len; ++c)
+      for (int c = 0; end + (int64_t)c * a.far_rows < sp.len; ++c) {
+        const int place = c ? a.far_places + a.more_at.at(sp.n, start, c - 1) * a.far_first + fb : a.far_at.at(sp.n, start, fb);
         for (int h = 0; h < share; ++h) {
           float y[8];
-          load8(a.far_parts + (((int64_t)(far_slot + c) * a.far_first + fb) * a.H + hk * share + h) * 2 * far + at, y);
+          load8(a.far_parts + ((int64_t)place * a.H + hk * share + h) * 2 * far + at, y);
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] += y[i];
         }
+      }
     }
     T* to = static_cast<T*>(which ? a.dv : a.dk);
     store8(to + (((int64_t)sp.b * a.s.T + sp.t0 + key) * a.Hkv + hk) * kHead + e, x);
@@ -853,9 +903,18 @@ namespace {
 struct WindowPlan {
   int64_t slots, near, far;   // blocks of queries of all sequences, of keys, of parts of far queries (0: no far queries)
   int queries, near_keys, near_split, near_first, far_keys, far_first, far_rows, W, S;   // queries: of a block
+  gsa::FirstPlaces far_at, more_at;
+  int far_places, more;
   size_t D, near_parts, far_parts;
   size_t workspace() const { return D + near_parts + far_parts; }
 };
+// Places for `blocks` blocks of `keys` first tokens of each sequence of at least `least` tokens: how many.
+int64_t first_places(int64_t tokens, int64_t N, int64_t least, int blocks, int keys, gsa::FirstPlaces& p) {
+  const int64_t by_start = tokens / least * blocks, by_token = tokens / keys;
+  if (N * blocks <= std::min(by_start, by_token)) return p = {0, blocks}, N * blocks;
+  if (by_start <= by_token) return p = {(int)least, blocks}, by_start;
+  return p = {keys, 1}, by_token;
+}
 bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, int sinks, int dtype, WindowPlan& z) {
   z = WindowPlan{};
   if (B < 1 || T < 1 || N < 1 || Hkv < 1 || H < Hkv || H % Hkv || H > 65535 || window < 1 || sinks < 0 || !dtype_size(dtype)) return false;
@@ -887,19 +946,31 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   // T = 1537, 4 heads on 2, window 256 1: 154  2: 127 (taken)  4: 145; 256 blocks 1: 493 (taken)  2: 512.
   const int64_t room = (dtype == GSA_DTYPE_BF16 ? 512 : 256) / (z.near * Hkv);
   z.near_split = (int)std::clamp<int64_t>(H / Hkv * ((z.W + (int64_t)z.near_keys) / 64) / 4, 1, std::max<int64_t>(1, room));
-  if (z.S) {
+  int64_t parts = 0;                                         // places for sums of far queries
+  const int64_t least = (int64_t)z.W + z.near_keys;                  // tokens of a sequence that has far queries, at least
+  if (z.S && least <= T) {
     z.near_first = (z.S + z.near_keys - 1) / z.near_keys;
-    z.far_first = (z.S + z.far_keys - 1) / z.far_keys;
+    z.far_first = std::min((z.S + z.far_keys - 1) / z.far_keys, (T - z.W) / z.near_keys * (z.near_keys / z.far_keys));
+    const int64_t tokens = (int64_t)B * T;
+    z.far_places = (int)first_places(tokens, N, least, z.far_first, z.far_keys, z.far_at);
     // 512 far queries a part, 128 where that leaves CUs idle; more of them where the parts are many (they fill the card without,
-    // and each leaves 32 KiB, so that the workspace would grow with T times the first tokens)
-    z.far_rows = slots(512) * z.far_first * H >= 256 ? 512 : 128;
-    while (z.far_rows < T && slots(z.far_rows) * z.far_first * H > 8192) z.far_rows *= 2;
-    z.far = slots(z.far_rows) * z.far_first;
-    if (z.far > (1 << 23) / H || (int64_t)N * z.near_first > (1 << 23) / H) return false;
+    // and each leaves 32 KiB, so that the workspace would grow with T times the first tokens).  By the tokens alone: sequences add a
+    // first part each, however many queries a part has.  us backward, 60000 tokens and 600 sequences of 17 beside them, 16 heads on
+    // 4, window 64, 4 first: with all far queries of a head in one block, which is what 600 parts would ask for, 2628, so 1202.
+    int64_t rows = tokens / 512 * z.far_first * H >= 256 ? 512 : 128;
+    while (tokens / rows * z.far_first * H > 8192) rows *= 2;
+    z.far_rows = (int)std::min<int64_t>(rows, INT_MAX);
+    z.more = (int)((T - least) / rows);
+    // (only packed sequences, whose lengths the host does not know, have blocks without work: 64 of 576 cost 9 us of 36)
+    const int64_t more = packed ? tokens / rows : (int64_t)B * z.more;
+    if (packed) z.more_at = {z.far_rows, 1}; else z.more_at = {0, z.more};
+    z.far = z.far_places + more * z.far_first;
+    parts = z.far_places + tokens / rows * z.far_first;
+    if ((int64_t)N * z.near_first > (1 << 23) / H) return false;
   }
   z.D = up((size_t)H * B * T * 4);
   z.near_parts = (z.near_split > 1 ? (size_t)z.near * z.near_split : (size_t)N * z.near_first) * Hkv * 2 * z.near_keys * 128 * 4;
-  z.far_parts = (size_t)z.far * H * 2 * z.far_keys * 128 * 4;
+  z.far_parts = (size_t)parts * H * 2 * z.far_keys * 128 * 4;
   return true;
 }
 
@@ -951,6 +1022,10 @@ int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, Win
     a.far_keys = z.far_keys;
     a.far_first = z.far_first;
     a.far_rows = z.far_rows;
+    a.far_at = z.far_at;
+    a.far_places = z.far_places;
+    a.more_at = z.more_at;
+    a.more = z.more;
     a.near_parts = reinterpret_cast<float*>(w + z.D);
     a.far_parts = reinterpret_cast<float*>(w + z.D + z.near_parts);
   }
