@@ -56,7 +56,8 @@ struct WindowArgs {
   // dk and dv: blocks of near_keys keys; the far queries of first tokens in parts of far_rows queries of a head, far_keys keys a block
   int near_keys, near_first, far_keys, far_first, far_rows;            // first: blocks of a sequence's first tokens
   int near_split;             // parts that a block's queries are cut into
-  float* near_parts;          // [N][near_first][Hkv][2][near_keys][128]; near_split > 1: [slots of keys][Hkv][near_split][2][..
+  FirstPlaces near_at;
+  float* near_parts;          // [near_at's places][Hkv][2][near_keys][128]; near_split > 1: [slots of keys][Hkv][near_split][2][..
   // the first far_rows far queries of a block are in far_at's places, the further ones behind those: more_at's places, far_first each
   FirstPlaces far_at, more_at;
   int far_places, more;       // more: further parts of a sequence, at most
@@ -683,7 +684,7 @@ __device__ __forceinline__ void window_dkv(const WindowArgs& a, char* lds, int i
     const int64_t end = (int64_t)k0 + kKeys - 1 + a.W;
     i1 = (int)min((int64_t)sp.len, end);
     if (a.near_split > 1) parts = a.near_parts + (int64_t)index * 2 * kKeys * kHead;
-    else if (k0 < a.S && end < sp.len) parts = a.near_parts + (((int64_t)sp.n * a.near_first + c) * a.Hkv + hk) * 2 * kKeys * kHead;
+    else if (k0 < a.S && end < sp.len) parts = a.near_parts + ((int64_t)a.near_at.at(sp.n, start_of(a.s, sp), c) * a.Hkv + hk) * 2 * kKeys * kHead;
   } else {
     h0 = index % a.H;
     hk = h0 / share;
@@ -857,8 +858,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
     sp = slot_of(a.s, unit, a.near_keys, block);
     if (block < 0) return;
   } else {
-    block = unit % a.near_first;
-    sp = span_of(a.s, unit / a.near_first, a.near_keys);
+    sp = holder(a.s, a.near_at, unit, a.near_first, block);
   }
   const int k0 = block * a.near_keys;
   const int64_t end = (int64_t)k0 + a.near_keys - 1 + a.W;
@@ -903,8 +903,8 @@ namespace {
 struct WindowPlan {
   int64_t slots, near, far;   // blocks of queries of all sequences, of keys, of parts of far queries (0: no far queries)
   int queries, near_keys, near_split, near_first, far_keys, far_first, far_rows, W, S;   // queries: of a block
-  gsa::FirstPlaces far_at, more_at;
-  int far_places, more;
+  gsa::FirstPlaces near_at, far_at, more_at;
+  int near_places, far_places, more;
   size_t D, near_parts, far_parts;
   size_t workspace() const { return D + near_parts + far_parts; }
 };
@@ -949,9 +949,10 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
   int64_t parts = 0;                                         // places for sums of far queries
   const int64_t least = (int64_t)z.W + z.near_keys;                  // tokens of a sequence that has far queries, at least
   if (z.S && least <= T) {
-    z.near_first = (z.S + z.near_keys - 1) / z.near_keys;
+    z.near_first = std::min((z.S + z.near_keys - 1) / z.near_keys, (T - z.W) / z.near_keys);
     z.far_first = std::min((z.S + z.far_keys - 1) / z.far_keys, (T - z.W) / z.near_keys * (z.near_keys / z.far_keys));
     const int64_t tokens = (int64_t)B * T;
+    z.near_places = (int)first_places(tokens, N, least, z.near_first, z.near_keys, z.near_at);
     z.far_places = (int)first_places(tokens, N, least, z.far_first, z.far_keys, z.far_at);
     // 512 far queries a part, 128 where that leaves CUs idle; more of them where the parts are many (they fill the card without,
     // and each leaves 32 KiB, so that the workspace would grow with T times the first tokens).  By the tokens alone: sequences add a
@@ -966,10 +967,9 @@ bool window_plan(int B, int T, int N, int packed, int H, int Hkv, int window, in
     if (packed) z.more_at = {z.far_rows, 1}; else z.more_at = {0, z.more};
     z.far = z.far_places + more * z.far_first;
     parts = z.far_places + tokens / rows * z.far_first;
-    if ((int64_t)N * z.near_first > (1 << 23) / H) return false;
   }
   z.D = up((size_t)H * B * T * 4);
-  z.near_parts = (z.near_split > 1 ? (size_t)z.near * z.near_split : (size_t)N * z.near_first) * Hkv * 2 * z.near_keys * 128 * 4;
+  z.near_parts = (z.near_split > 1 ? (size_t)z.near * z.near_split : (size_t)z.near_places) * Hkv * 2 * z.near_keys * 128 * 4;
   z.far_parts = (size_t)parts * H * 2 * z.far_keys * 128 * 4;
   return true;
 }
@@ -1019,6 +1019,7 @@ int window_args(const gsa_window_args* x, bool backward, gsa::WindowArgs& a, Win
     a.near_keys = z.near_keys;
     a.near_split = z.near_split;
     a.near_first = z.near_first;
+    a.near_at = z.near_at;
     a.far_keys = z.far_keys;
     a.far_first = z.far_first;
     a.far_rows = z.far_rows;
@@ -1071,7 +1072,7 @@ template <typename T, int kP> int window_backward(const gsa::WindowArgs& a, cons
   if (e) return e;
   if (z.far && (e = launch_dkv<T, sizeof(T) == 2 ? 1 : 2, true, kP>(a, z.far * a.H, s))) return e;
   if (!z.far && z.near_split == 1) return GSA_OK;
-  const int64_t units = z.near_split > 1 ? z.near : (int64_t)a.s.N * a.near_first;
+  const int64_t units = z.near_split > 1 ? z.near : z.near_places;
   hipLaunchKernelGGL(gsa::window_join_kernel<T>, dim3(units * a.Hkv, a.near_keys / 8), dim3(256), 0, s, a);
   return launch_status();
 }
