@@ -66,6 +66,19 @@ struct WindowArgs {
 
 template <int N> struct Number { static constexpr int value = N; };
 
+// Three parts of any finite value: those that round to an infinity of bf16 have its largest value as their first part.
+__device__ __forceinline__ Parts<3> split_wide(const float (&x)[8]) {
+  constexpr float kMost = 0x1.fep127f;
+  float c[8], rest[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = __builtin_fabsf(x[e]) < __builtin_inff() ? fminf(fmaxf(x[e], -kMost), kMost) : x[e];
+  const bf16x8 first = parts_of<1>(c).p[0];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) rest[e] = x[e] - (float)first[e];
+  const Parts<2> more = parts_of<2>(rest);
+  return {first, more.p[0], more.p[1]};
+}
+
 template <typename T> struct WindowType;
 template <> struct WindowType<uint16_t> { static constexpr int NP = 1, kTile = 64, kBuffers = 2; };
 template <> struct WindowType<float> { static constexpr int NP = 3, kTile = 32, kBuffers = 1; };
@@ -159,12 +172,14 @@ template <typename T, int kN = WindowType<T>::kTile> struct Tile {
         }
       }
     }
-    __device__ void store(char* tile, int wave, int l) {
+    template <bool kWide = false> __device__ void store(char* tile, int wave, int l) {
       if constexpr (NP == 3) {
 #pragma unroll
         for (int j = 0; j < kUnits; ++j) {
           const int t = 16 * j + 4 * wave + (l >> 4), u = (l & 15) ^ swizzle(t);
-          const Parts<3> p = split_pair(x[2 * j], x[2 * j + 1]);
+          const floatx4 &y = x[2 * j], &z = x[2 * j + 1];
+          const float all[8] = {y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]};
+          const Parts<3> p = kWide ? split_wide(all) : split3(all);
 #pragma unroll
           for (int n = 0; n < 3; ++n) *reinterpret_cast<bf16x8*>(tile + n * kPlane + t * 256 + 16 * u) = p.p[n];
         }
@@ -267,36 +282,63 @@ template <int N> struct KeyTiles {
   __device__ int at(int t) const { return (t < first ? t : from + t - first) * N; }
 };
 
-// One query's output from its visible keys alone, a wave: lane l has elements 2 l, 2 l + 1.
-template <typename T>
-__device__ __forceinline__ void window_row(const WindowArgs& a, const T* q, const T* kbase, const T* vbase, int i, T* o, T* low, float* lse, int l) {
-  const float scale = a.scale * kLog2e;
-  const float q0 = to_f32(q[2 * l]), q1 = to_f32(q[2 * l + 1]);
-  float m = -__builtin_inff(), sum = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int j = 0; j <= i; ++j) {
-    if (j >= a.S && j <= i - a.W) j = max(j, i - a.W + 1);
-    const T *k = kbase + j * a.k.st, *v = vbase + j * a.v.st;
-    float s = q0 * to_f32(k[2 * l]) + q1 * to_f32(k[2 * l + 1]);
+// 0 for what is not finite, or (kNot) for what is
+template <bool kNot> __device__ __forceinline__ bf16x8 finite(const bf16x8& x) {
+  u32x4 y = __builtin_bit_cast(u32x4, x);
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x, 64);
-    s *= scale;
-    const float top = s > m ? s : m;
-    const float f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top), p = s == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s - top);
-    m = top;
-    sum = sum * f + p;
-    o0 = o0 * f + p * to_f32(v[2 * l]);
-    o1 = o1 * f + p * to_f32(v[2 * l + 1]);
-    if (sum != sum) break;                                   // a score is NaN or +infinity: the whole row is NaN
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t odd = ((y[i] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((y[i] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+    y[i] &= kNot ? odd : ~odd;
   }
-  o0 = sum != sum ? sum : o0 / sum;
-  o1 = sum != sum ? sum : o1 / sum;
-  o[2 * l] = from_f32<T>(o0);
-  o[2 * l + 1] = from_f32<T>(o1);
-  if (low) {
-    low[2 * l] = from_f32<T>(o0 - to_f32(from_f32<T>(o0)));
-    low[2 * l + 1] = from_f32<T>(o1 - to_f32(from_f32<T>(o1)));
+  return __builtin_bit_cast(bf16x8, y);
+}
+template <int N> __device__ __forceinline__ Parts<N> finite(Parts<N> x) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) x.p[n] = finite<false>(x.p[n]);
+  return x;
+}
+// What the values that are not finite do to the outputs (made without them) of the 32 queries from r0 on that see them: NaN, or where
+// all that a query sees in a column are infinities of one sign that one.  A wave: lane l looks at elements 2 l, 2 l + 1 of each key
+// and keeps the queries that see such a one, a bit each; the masks go through 384 words of LDS to the lanes that hold the outputs.
+template <typename T>
+__device__ __forceinline__ void spoil(const WindowArgs& a, const T* vbase, int r0, int len, floatx16 (&o)[4], uint32_t* lds, int l) {
+  const int from = max(0, r0 - a.W + 1), first = min(a.S, from), count = first + min(r0 + 31, len - 1) - from + 1;
+  uint32_t nan[2] = {0u, 0u}, inf[2][2] = {{0u, 0u}, {0u, 0u}};
+#pragma unroll 8
+  for (int e = 0; e < count; ++e) {
+    const int j = e < first ? e : from + e - first;
+    const T* v = vbase + j * a.v.st + 2 * l;
+    const int hi = j < a.S ? 31 : (int)min((int64_t)31, (int64_t)j - r0 + a.W - 1);
+    const uint32_t rows = ~0u << max(0, j - r0) & ~0u >> (31 - hi);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float x = to_f32(v[c]);
+      nan[c] |= x != x ? rows : 0u;
+      inf[c][0] |= x == __builtin_inff() ? rows : 0u;
+      inf[c][1] |= x == -__builtin_inff() ? rows : 0u;
+    }
   }
-  if (lse && l == 0) *lse = m + __builtin_amdgcn_logf(sum);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    lds[2 * l + c] = nan[c] | (inf[c][0] & inf[c][1]);
+    lds[kHead + 2 * l + c] = inf[c][0];
+    lds[2 * kHead + 2 * l + c] = inf[c][1];
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  const uint32_t row = 1u << (l & 31);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const uint32_t* at = lds + 32 * dt + 2 * r + 4 * (l >> 5);         // element of o[dt][r]
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float y = o[dt][r + i];
+        y = at[2 * kHead + i] & row ? -__builtin_inff() : y;
+        y = at[kHead + i] & row ? __builtin_inff() : y;
+        o[dt][r + i] = at[i] & row ? __builtin_nanf("") : y;
+      }
+    }
 }
 
 // Tiles of rows for kGroups groups of 32 rows that a block's 4 waves hold: at least 32 for each wave of a group, and kLeast
@@ -340,28 +382,41 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
   };
   load(0, 0);
   Parts<NP> q[8];
-  row_operand<T>(q, row_at<T>(a.q, sp, rowc, h), l);
-  if (a.scale < 0.f)                                         // (the largest score is then the largest product)
+  auto query = [&](bool wide) __attribute__((always_inline)) {
+    const T* p = row_at<T>(a.q, sp, rowc, h);
+    row_operand<T>(q, p, l);
+    if constexpr (NP == 3) {
+      if (wide) {
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks)
+        for (int ks = 0; ks < 8; ++ks) {
+          float x[8];
+          load8(p + 16 * ks + 8 * (l >> 5), x);
+          q[ks] = split_wide(x);
+        }
+      }
+    }
+    if (a.scale < 0.f)                                       // (the largest score is then the largest product)
 #pragma unroll
-      for (int n = 0; n < NP; ++n) q[ks].p[n] = -q[ks].p[n];
+      for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+        for (int n = 0; n < NP; ++n) q[ks].p[n] = -q[ks].p[n];
+  };
+  query(false);
   floatx16 o[4];
-#pragma unroll
-  for (int dt = 0; dt < 4; ++dt) zero(o[dt]);
   const typename L::RowReader rows(base, l);
   const typename L::ColReader cols(base, l);
   // softmax state of the lane's row, log2 domain: the reference m moves only when a tile's maximum exceeds it by more than
   // kLazy (the sums then stay below 2^8 times what they are, far from fp32's range)
   constexpr float kLazy = 8.f;
-  float m = -__builtin_inff(), limit = m, minus = 0.f, sum = 0.f;
-  auto step = [&](int t, auto which, auto parts) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
+  float m, limit, minus, sum;
+  // clean: without the values that are not finite (of keys those give the score that they have: -infinity, or one that makes a row NaN)
+  auto step = [&](int t, auto which, auto parts, auto clean) __attribute__((always_inline)) {   // the buffer's place in LDS is a constant
     constexpr int buffer = kBuffers == 2 ? decltype(which)::value : 0;
     constexpr uint32_t K = buffer * kBuffer, V = K + L::kBytes;
     if constexpr (NP == 3) {
       if (t) __syncthreads();                                // every wave is through with the last tile
-      lk.store(lds + K, wave, l);
-      lv.store(lds + V, wave, l);
+      lk.template store<decltype(clean)::value != 0>(lds + K, wave, l);
+      lv.template store<decltype(clean)::value != 0>(lds + V, wave, l);
     }
     wait_loads();
     __syncthreads();
@@ -374,7 +429,15 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
       floatx16 s;
       zero(s);
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) mma32(s, rows.read(K, 32 * n, ks), q[ks]);
+      for (int ks = 0; ks < 8; ++ks) {
+        const Parts<NP> k = rows.read(K, 32 * n, ks);
+        if constexpr (NP == 3 && decltype(clean)::value) {   // an infinity's other parts are NaN: it goes by itself, times q's first part
+          mma32(s, finite(k), q[ks]);
+          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(finite<true>(k.p[0]), q[ks].p[0], s, 0, 0, 0);
+        } else {
+          mma32(s, k, q[ks]);
+        }
+      }
       if constexpr (NP == 1) reads_ahead<4, 8>();
       if (see == 1) {
         const int lh = here(l), j = j0 + 8 * (lh >> 5);
@@ -406,21 +469,28 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
       for (int k = 0; k < 2; ++k) {
         const auto p = parts_at<decltype(parts)::value>(s, k);
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) mma32(o[dt], cols.read(V, 32 * n + 16 * k, dt), p);
+        for (int dt = 0; dt < 4; ++dt) {
+          const Parts<NP> v = cols.read(V, 32 * n + 16 * k, dt);
+          mma32(o[dt], decltype(clean)::value ? finite(v) : v, p);
+        }
       }
     }
   };
-  auto walk = [&](auto parts) __attribute__((always_inline)) {
+  auto walk = [&](auto parts, auto clean) __attribute__((always_inline)) {
     for (int t = 0; t < tiles.count; t += 2) {
-      step(t, Number<0>{}, parts);
-      if (t + 1 < tiles.count) step(t + 1, Number<1>{}, parts);
+      step(t, Number<0>{}, parts, clean);
+      if (t + 1 < tiles.count) step(t + 1, Number<1>{}, parts, clean);
     }
   };
-  if (kP == 1 && few_visible(q0 + kQueries, sp)) walk(Number<2>{});
-  else walk(Number<kP>{});
-  sum = sum_halves(sum);
-  __syncthreads();                                           // the tiles are free
-  if constexpr (kSplit > 1) {
+  auto attend = [&](auto clean) __attribute__((always_inline)) {
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) zero(o[dt]);
+    m = limit = -__builtin_inff();
+    minus = sum = 0.f;
+    if (kP == 1 && few_visible(q0 + kQueries, sp)) walk(Number<2>{}, clean);
+    else walk(Number<kP>{}, clean);
+    sum = sum_halves(sum);
+    __syncthreads();                                         // the tiles are free
     // the waves of a group join one after the other: sums, maximum and sum of the softmax through LDS
     float* hand = reinterpret_cast<float*>(lds) + group * 66 * 64 + l;
 #pragma unroll 1
@@ -442,17 +512,29 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
       }
       __syncthreads();
     }
-    if (split) return;
-  }
-  if (r0 >= sp.len) return;
-  const int left = sp.len - r0;
-  const int64_t to = (((int64_t)sp.b * a.s.T + sp.t0 + r0) * a.H + h) * kHead;
-  T *out = static_cast<T*>(a.o) + to, *low = a.low ? static_cast<T*>(a.low) + to : nullptr;
+  };
+  attend(Number<0>{});
+  // Something that is not finite in a row's tiles may have reached it without being seen (0 * NaN).  Then the block goes through them
+  // once more without such values, and what they do to the queries that see them is put in by itself: the others' outputs are
+  // the same bits as if finite values stood there.  2 x 6000 tokens, window 4096, 8 heads on 2, bf16: 170 us, with NaN behind one row's
+  // tokens 750, where all queries see one 975 (each such query by itself, key by key: 2200 and 61000).
+  const bool mine = split == 0 && r0 < sp.len;
   float odd = sum * 0.f;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(o[dt][r], 0.f, odd);
+  const bool again = __syncthreads_or(mine && !(odd == 0.f));
+  if (__builtin_expect(again, 0)) {
+    load(0, 0);
+    if constexpr (NP == 3) query(true);
+    attend(Number<1>{});
+  }
+  if (!mine) return;
+  if (__builtin_expect(again, 0)) spoil<T>(a, vbase, r0, sp.len, o, reinterpret_cast<uint32_t*>(lds + group * 32 * kHead * sizeof(T)), l);
+  const int left = sp.len - r0;
+  const int64_t to = (((int64_t)sp.b * a.s.T + sp.t0 + r0) * a.H + h) * kHead;
+  T *out = static_cast<T*>(a.o) + to, *low = a.low ? static_cast<T*>(a.low) + to : nullptr;
   store_rows<T>(o, 1.f / sum, lds + group * 32 * kHead * sizeof(T), out, (int64_t)a.H * kHead, left, l);
   if constexpr (NP == 1)
     if (low) {
@@ -475,16 +557,6 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
     }
   float* lse = a.lse ? a.lse + (int64_t)h * a.B * a.s.T + (int64_t)sp.b * a.s.T + sp.t0 : nullptr;
   if (lse && row < sp.len && l < 32) lse[row] = m + __builtin_amdgcn_logf(sum);
-  // A row with something that is not finite in its tiles: what it does not see may have reached it (0 * NaN), so it is
-  // computed once more from its visible keys alone.
-  uint64_t redo = ballot64(!(odd == 0.f));
-  redo = (redo | redo >> 32) & 0xffffffffu;
-  if (__builtin_expect(redo != 0, 0)) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    for (int i = 0; i < min(32, left); ++i)
-      if (redo >> i & 1)
-        window_row<T>(a, row_at<T>(a.q, sp, r0 + i, h), kbase, vbase, r0 + i, out + (int64_t)i * a.H * kHead, low ? low + (int64_t)i * a.H * kHead : nullptr, lse ? lse + r0 + i : nullptr, l);
-  }
 }
 
 // The accumulators of the waves that share their rows, summed in their order into the first wave's through LDS.

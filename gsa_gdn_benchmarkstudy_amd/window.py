@@ -102,8 +102,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     cu_seqlens (int32 or int64 [N+1], on the device, ascending from 0): B is 1 and N sequences are
     packed in T, each with its own window and first tokens; empty ones are allowed.  Rows of o and
     of the gradients outside every sequence are 0, whatever the inputs hold there.  What a query
-    does not see may hold a NaN or an infinity without reaching its output, so padding behind the tokens of
-    a batch's row may hold anything (its outputs are to be ignored; rows beside it take longer).
+    does not see may hold a NaN or an infinity without changing a bit of its output, so padding behind the tokens of
+    a batch's row may hold anything (its outputs are to be ignored; queries that stand with it in a block of 64 or 128 take
+    up to some six times as long).
     Gradients it reaches, as 0 * NaN does: where they are wanted, padding has to be finite, or
     left out by packing.
 
