@@ -217,6 +217,11 @@ template <int kAhead, int kMany> __device__ __forceinline__ void reads_ahead() {
   }
   __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
 }
+// By halves, so that a long row's sum is rounded once a tile: one after the other, 8192 keys' fp32 dq was off by 1.7 times what plain
+// fp32 sums give where v and dO have a mean (the error of a row's sum is common to all of its outputs, and so adds up in do . o).
+__device__ __forceinline__ float sum16(const floatx16& x) {
+  return (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) + (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
+}
 __device__ __forceinline__ void zero(floatx16& x) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) x[r] = 0.f;
@@ -461,10 +466,8 @@ __global__ __launch_bounds__(256, (WindowQueries<T, kGroups>::kWaves)) void wind
         minus = m == -__builtin_inff() ? 0.f : -m;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, minus));
-        sum += s[r];
-      }
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_l2, minus));
+      sum += sum16(s);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const auto p = parts_at<decltype(parts)::value>(s, k);

@@ -13,6 +13,7 @@ bf16, each element, where at most 128 keys are visible: half a step of the resul
 import pytest
 import torch
 
+from gsa_gdn_benchmarkstudy_amd import window_attention
 from tests import test_gpu_window as tw
 
 pytestmark = pytest.mark.gpu
@@ -82,3 +83,33 @@ def test_short_windows(dev, B, T, H, Hkv, lens, W, S):
     for n in got:
         _in_the_norm(got[n], ref[n], size[n], 1.1, n)
         _elements(got[n], ref[n], size[n], score, T, n)
+
+
+def _in_full(q, k, v, do, W):
+    """The definition's results in the inputs' type by whole matrices: [1, T, H, 128], keys of one head."""
+    T = q.shape[1]
+    q, do, k, v = (t[0].transpose(0, 1) for t in (q, do, k, v))
+    at = torch.arange(T, device=q.device)
+    seen = (at[:, None] >= at) & (at[:, None] - at < W)
+    p = torch.softmax((q @ k.transpose(1, 2) * 128 ** -0.5).masked_fill(~seen, -float("inf")), -1)
+    o = p @ v
+    ds = p * (do @ v.transpose(1, 2) - (do * o).sum(-1, keepdim=True)) * 128 ** -0.5
+    dk, dv = ((a.transpose(1, 2) @ b).sum(0, keepdim=True) for a, b in ((ds, q), (p, do)))
+    return {n: t.transpose(0, 1)[None] for n, t in (("o", o), ("dq", ds @ k), ("dk", dk), ("dv", dv))}
+
+
+@pytest.mark.parametrize("T,W", [(8192, 8192), (4096, 4096), (4096, 300)])
+def test_fp32_errors_of_long_sums(dev, T, W):
+    """Four query heads on a key head and values and gradients with a mean: sums that grow over thousands of keys and queries.  Their errors
+    are those of plain fp32 sums in torch or less: either side rounds a score and a do . v over 128 products, and the sums over
+    keys once a tile here; 1.25 for what such errors scatter by."""
+    gen = torch.Generator(device=dev).manual_seed(T)
+    q, k, v, do = (torch.randn(1, T, h, 128, generator=gen, device=dev) + mean for h, mean in ((4, 0), (1, 0), (1, 1), (4, 1)))
+    ref, plain = _in_full(*(t.double() for t in (q, k, v, do)), W), _in_full(q, k, v, do, W)
+    leaf = [t.requires_grad_() for t in (q, k, v)]
+    o = window_attention(*leaf, W)
+    got = {"o": o.detach(), **dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaf, do)))}
+    for n in got:
+        own, other = ((t[n].double() - ref[n]).norm() / ref[n].norm() for t in (got, plain))
+        print(f"{n}: {own:.2e}, plain {other:.2e}", flush=True)
+        assert own <= 1.25 * other, n
