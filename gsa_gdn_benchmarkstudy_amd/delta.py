@@ -52,21 +52,21 @@ def _check(n: int, q, k, v, g, beta) -> None:
 _HERE = contextlib.nullcontext()
 
 
-def _refuse_unseen(*ts: Optional[torch.Tensor]) -> None:
+def _refuse_unseen(name: str, *ts: Optional[torch.Tensor]) -> None:
     """Raises where torch follows the call in a way that a kernel's launch escapes, and that would
     lose it in silence: a tangent of forward-mode differentiation, or torch.jit.trace."""
     if _forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
         for t in ts:
             if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError("this operator has no forward-mode derivative (torch.autograd.forward_ad)")
+                raise RuntimeError(f"{name} has no forward-mode derivative (torch.autograd.forward_ad)")
     if torch._C._get_tracing_state() is not None:
-        raise RuntimeError("this operator cannot be recorded by torch.jit.trace")
+        raise RuntimeError(f"{name} cannot be recorded by torch.jit.trace")
 
 
-def _device(first: torch.Tensor, *others: Optional[torch.Tensor]):
+def _device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]):
     """Checks that torch need not see into the call and that all tensors are on one GPU, and makes
     that the current one."""
-    _refuse_unseen(first, *others)
+    _refuse_unseen(name, first, *others)
     at = first.get_device()                      # -1 on the CPU
     for t in others:
         if t is not None and t.get_device() != at:
@@ -89,32 +89,36 @@ class _Twice(torch.autograd.Function):
     """The first n tensors as they are, depending on all of them, with an error for their gradient."""
 
     @staticmethod
-    def forward(ctx, n, *ts):
+    def forward(ctx, name, n, *ts):
+        ctx.name = name
         return tuple(t if t is None else t.view_as(t) for t in ts[:n])
 
     @staticmethod
     def backward(ctx, *grads):
-        raise RuntimeError("the gradients of this operator cannot be differentiated: it is differentiable once")
+        raise RuntimeError(f"the gradients of {ctx.name} cannot be differentiated: it is differentiable once")
 
 
 def _once(backward):
     """A backward pass that is differentiable once: where a graph of it is being built, what comes out
     depends on the gradients that came in and on the inputs, with an error behind it.  (torch's
     once_differentiable costs 15 us a call, and its outputs do not depend on the inputs: a
-    penalty on the gradients would lose its part in silence.)"""
+    penalty on the gradients would lose its part in silence.)  Errors name the Function's `operator`."""
 
     def run(ctx, *grads):
-        _refuse_unseen(*grads)
+        name = getattr(getattr(ctx, "_forward_cls", None), "operator", "this operator")
+        _refuse_unseen(name, *grads)
         if not torch.is_grad_enabled():
             return backward(ctx, *grads)
         with torch.no_grad():
             out = backward(ctx, *grads)
-        return _Twice.apply(len(out), *out, *grads, *ctx.saved_tensors)
+        return _Twice.apply(name, len(out), *out, *grads, *ctx.saved_tensors)
 
     return staticmethod(run)
 
 
 class _Rule(torch.autograd.Function):
+    operator = "gated_delta_rule"
+
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, cu, scale, want_state):
         o, final, saved = _abi.delta_rule(q, k, v, g, beta, state, cu, scale, want_state, True)
@@ -181,7 +185,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         if tuple(initial_state.shape) != (N, Hv, d, d) or initial_state.dtype != torch.float32:
             raise ValueError(f"initial_state {tuple(initial_state.shape)} {initial_state.dtype}: expected fp32 {(N, Hv, d, d)}")
     scale = d ** -0.5 if scale is None else float(scale)
-    with _device(q, k, v, g, beta, initial_state, cu_seqlens):
+    with _device("gated_delta_rule", q, k, v, g, beta, initial_state, cu_seqlens):
         if initial_state is not None:
             initial_state = initial_state.contiguous()
             if initial_state.data_ptr() % 16:
@@ -234,7 +238,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         raise ValueError(f"{N} rows, {state.shape[0]} states")
     if _needs_grad(q, k, v, g, beta, state):
         raise RuntimeError("gated_delta_step is forward only: call it under torch.no_grad()")
-    with _device(q, k, v, g, beta, state, state_indices):
+    with _device("gated_delta_step", q, k, v, g, beta, state, state_indices):
         if N == 0 or state.shape[0] == 0:
             return v.new_zeros(v.shape)
         _range_push("gsa_hip/delta_step")

@@ -52,6 +52,8 @@ def _state_in(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 
 class _Linear(torch.autograd.Function):
+    operator = "linear_attention"
+
     @staticmethod
     def forward(ctx, q, k, v, g, state, cu, scale, want_state):
         o, final, saved = _abi.linear_attn(q, k, v, g, state, cu, scale, want_state, True)
@@ -113,7 +115,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         if tuple(initial_state.shape) != (N, Hv, d, d) or initial_state.dtype != torch.float32:
             raise ValueError(f"initial_state {tuple(initial_state.shape)} {initial_state.dtype}: expected fp32 {(N, Hv, d, d)}")
     scale = d ** -0.5 if scale is None else float(scale)
-    with _device(q, k, v, g, initial_state, cu_seqlens):
+    with _device("linear_attention", q, k, v, g, initial_state, cu_seqlens):
         initial_state = _state_in(initial_state)
         _range_push("gsa_hip/linear_attention")
         try:
@@ -161,7 +163,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: 
         raise ValueError(f"{N} rows, {state.shape[0]} states")
     if _needs_grad(q, k, v, g, state):
         raise RuntimeError("linear_attention_step is forward only: call it under torch.no_grad()")
-    with _device(q, k, v, g, state, state_indices):
+    with _device("linear_attention_step", q, k, v, g, state, state_indices):
         if N == 0 or state.shape[0] == 0:
             return v.new_zeros(v.shape)
         _range_push("gsa_hip/linear_step")

@@ -36,6 +36,8 @@ def _check(x, weight, residual) -> None:
 
 
 class _Norm(torch.autograd.Function):
+    operator = "add_rms_norm"
+
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         y, h, rstd = _abi.rms_norm(x, weight, residual, eps, want_rstd=True)
@@ -65,7 +67,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     y and h are contiguous.  Differentiable in all three, once and backwards; the gradients are
     the same bits on every run, and with a residual x and the residual get the same tensor."""
     _check(x, weight, residual)
-    with _device(x, weight, residual):
+    with _device("add_rms_norm", x, weight, residual):
         if x.numel() == 0:
             h = x if residual is None else x + residual
             return h * weight, h
@@ -90,7 +92,7 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
     _check(x, weight, residual)
     if _needs_grad(x, weight, residual):
         raise RuntimeError("add_rms_norm_fp8 is forward only: call it under torch.no_grad()")
-    with _device(x, weight, residual):
+    with _device("add_rms_norm_fp8", x, weight, residual):
         if x.numel() == 0:
             return (torch.empty_like(x, dtype=torch.float8_e4m3fn), x.new_ones(x.shape[:-1], dtype=torch.float32),
                     x if residual is None else x + residual)

@@ -70,6 +70,8 @@ def _index(t: Optional[torch.Tensor], N: int, name: str):
 
 
 class _Window(torch.autograd.Function):
+    operator = "window_attention"
+
     @staticmethod
     def forward(ctx, q, k, v, cu, window, sinks, scale):
         o, lse, low = _abi.window_attn(q, k, v, cu, window, sinks, scale, True)
@@ -121,7 +123,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     if cu_seqlens is not None:
         cu_seqlens = _check_packed(cu_seqlens, q.shape[0])
     scale = D_HEAD ** -0.5 if scale is None else float(scale)
-    with _device(q, k, v, cu_seqlens):
+    with _device("window_attention", q, k, v, cu_seqlens):
         _range_push("gsa_hip/window_attention")
         try:
             needed = _needs_grad(q, k, v)
@@ -193,7 +195,7 @@ def window_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
         raise ValueError(f"{N} sequences, {k_cache.shape[0]} caches")
     if _needs_grad(k, v):
         raise RuntimeError("window_cache_write is forward only: call it under torch.no_grad()")
-    with _device(k, v, k_cache, v_cache, positions, cache_indices, cu_seqlens):
+    with _device("window_cache_write", k, v, k_cache, v_cache, positions, cache_indices, cu_seqlens):
         if B * T == 0 or k_cache.shape[0] == 0:
             return
         _range_push("gsa_hip/window_cache_write")
@@ -237,7 +239,7 @@ def window_attention_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optiona
         raise ValueError(f"{N} rows, {k_cache.shape[0]} caches")
     if _needs_grad(q, k, v):
         raise RuntimeError("window_attention_step is forward only: call it under torch.no_grad()")
-    with _device(q, k, v, k_cache, v_cache, positions, cache_indices):
+    with _device("window_attention_step", q, k, v, k_cache, v_cache, positions, cache_indices):
         if N == 0 or k_cache.shape[0] == 0:
             return q.new_zeros(q.shape)
         _range_push("gsa_hip/window_step")
