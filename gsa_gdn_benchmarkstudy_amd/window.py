@@ -161,7 +161,8 @@ def _check_caches(k_cache, v_cache, Hkv: int, dtype, rows: int) -> None:
 
 
 def _written(*ts: torch.Tensor) -> None:
-    if not ts[0].is_inference() and not ts[1].is_inference():
+    ts = tuple(t for t in ts if not t.is_inference())
+    if ts:
         _increment_version(ts)                   # a graph that kept the old caches must not use the new ones
 
 
