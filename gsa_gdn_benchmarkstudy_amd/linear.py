@@ -109,6 +109,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
             raise ValueError(f"packed sequences come in one row: B is {B}")
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype not in (torch.int32, torch.int64):
             raise ValueError("cu_seqlens: int32 or int64 [N + 1]")
+        if cu_seqlens.numel() >= 1 << 31:        # (the C interface counts in 32 bits)
+            raise ValueError(f"{cu_seqlens.numel() - 1} sequences: fewer than 2**31 - 1")
         cu_seqlens = cu_seqlens.contiguous()
     N = B if cu_seqlens is None else cu_seqlens.numel() - 1
     if initial_state is not None:

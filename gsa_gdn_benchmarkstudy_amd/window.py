@@ -58,6 +58,8 @@ def _check_packed(cu, B: int):
         raise ValueError(f"packed sequences come in one row: B is {B}")
     if cu.dim() != 1 or cu.numel() < 2 or cu.dtype not in (torch.int32, torch.int64):
         raise ValueError("cu_seqlens: int32 or int64 [N + 1]")
+    if cu.numel() >= 1 << 31:                    # (the C interface counts in 32 bits)
+        raise ValueError(f"{cu.numel() - 1} sequences: fewer than 2**31 - 1")
     return cu.contiguous()
 
 
@@ -112,7 +114,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 
     Differentiable in q, k and v, once and backwards (a tangent of torch.autograd.forward_ad raises);
     the gradients are the same bits on every run.  Fewer than 2**31 tokens and at most 2**23 blocks of
-    128 tokens times heads.
+    32 tokens (a sequence's last one may be shorter) times heads.
 
     May be captured into a graph, forward and backward, after one call outside of it; as with any
     backward pass no eager graph of the same leaves may live then (capture torch.autograd.grad, or
@@ -178,7 +180,8 @@ def window_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
     each sequence's first token here; 0 without it (a prompt's beginning).  cache_indices (int32 or int64 [N],
     on the device): each sequence's slot; sequence n has slot n without it.  A slot outside
     [0, slots) and a position outside [0, 2**62) are skipped.  Two sequences of one call that write one
-    row leave either's key and either's value there.  k and v are not parts of the caches.
+    row leave either's key and either's value there.  k and v are not parts of the caches.  Fewer than 2**29 tokens, in
+    fewer than 2**23 blocks of 64.
     """
     _check_sinks(sinks)
     if k.dim() != 4 or v.shape != k.shape or k.shape[-1] != D_HEAD or k.shape[2] < 1:
@@ -187,6 +190,8 @@ def window_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
         raise ValueError(f"k and v must share a dtype: got {k.dtype}, {v.dtype}")
     _abi.dtype_code(k.dtype)
     B, T, Hkv, _ = k.shape
+    if B * T >= 1 << 29:
+        raise ValueError(f"{B} x {T} tokens: fewer than 2**29")
     _check_caches(k_cache, v_cache, Hkv, k.dtype, sinks + 1)
     if cu_seqlens is not None:
         cu_seqlens = _check_packed(cu_seqlens, B)

@@ -1,8 +1,9 @@
-"""What a write does to the caches' versions."""
+"""Window attention and its caches at the ends of what they count, and what a write does to the caches' versions."""
 
 import pytest
 import torch
 
+from gsa_gdn_benchmarkstudy_amd import _abi, linear_attention, window_attention, window_cache_write
 from gsa_gdn_benchmarkstudy_amd.window import _written
 
 
@@ -15,3 +16,35 @@ def test_versions_of_written_caches(inference):
             caches[i] = torch.zeros(2)
     _written(*caches)
     assert [t._version for t in caches if not t.is_inference()] == [1] * (2 - len(inference))
+
+
+def _one(*s):
+    """Of any size without memory."""
+    return torch.zeros(1).expand(*s)
+
+
+def test_more_tokens_than_the_c_interface_counts():
+    """Broadcast keys of 2**32 + 5 tokens would be written as 5."""
+    caches = [torch.zeros(1, 8, 1, 128) for _ in range(2)]
+    for B, T in ((1, 2 ** 32 + 5), (2 ** 16, 2 ** 16), (2, 2 ** 28)):
+        with pytest.raises(ValueError, match="tokens"):
+            window_cache_write(_one(B, T, 1, 128), _one(B, T, 1, 128), *caches)
+
+
+def test_more_sequences_than_the_c_interface_counts():
+    x, cu = torch.zeros(1, 3, 1, 128), torch.zeros(1, dtype=torch.int32).expand(2 ** 32 + 3)
+    for call in (lambda: linear_attention(x, x, x, torch.zeros(1), cu_seqlens=cu), lambda: window_attention(x, x, x, 2, cu_seqlens=cu),
+                 lambda: window_cache_write(x, x, torch.zeros(1, 8, 1, 128), torch.zeros(1, 8, 1, 128), cu_seqlens=cu)):
+        with pytest.raises(ValueError, match="sequences"):
+            call()
+
+
+@pytest.mark.parametrize("H", [1, 16])
+def test_the_documented_limit_of_window_attention(H):
+    """At most 2**23 blocks of 32 tokens times heads, whatever the first tokens."""
+    f = _abi.load().gsa_window_attn_workspace_bytes
+    for S in (0, 4, 1000):
+        T = 2 ** 23 // H * 32
+        assert f(1, T, 1, 0, H, H, 1, S, 1) > 0 and f(1, T + 1, 1, 0, H, H, 1, S, 1) == 0
+        # packed: a block begun for each sequence besides
+        assert f(1, T - 32 * 100, 100, 1, H, H, 1, S, 1) > 0 and f(1, T - 32 * 100, 101, 1, H, H, 1, S, 1) == 0
