@@ -19,9 +19,9 @@
 // outputs), the states between them (linear_join_kernel), all segments' outputs at once.
 //
 // A block takes a head: 8 waves of 16 columns of the state each, which stays in registers from chunk to chunk (tile_row: a
-// product's result is the next one's operand in the same lanes).  4 x 4096 tokens of 16 heads in bf16: state pass 39-42 us (0.1
-// GB, 2.5 TB/s; its loads alone, two blocks a CU, 28), join 6, outputs 86-91 (0.27 GB, 3.1 TB/s); with gradients besides dk and dv
-// 136-143 (0.54 GB, 3.9 TB/s) and dq with dg 157-169 (0.34 GB).  Of the outputs' cycles a quarter is MFMA and a quarter VALU
+// product's result is the next one's operand in the same lanes).  4 x 4096 tokens of 16 heads in bf16: state pass 39-45 us (0.1
+// GB, 2.5 TB/s; its loads alone, two blocks a CU, 28), join 7, outputs 86-91 (0.27 GB, 3.1 TB/s); with gradients besides dk and dv
+// 136-143 (0.54 GB, 3.9 TB/s) and dq with dg 156-169 (0.34 GB).  Of the outputs' cycles a quarter is MFMA and a quarter VALU
 // (98 MFMA, 400 VALU a wave and chunk: the splits in parts), a third each for dk and dv, which do not overlap within a SIMD; the rest
 // waits for loads and at the chunk's two barriers.  dq with dg: 216 MFMA and 1160 VALU, three quarters of its cycles.
 // Measured and not taken (us of the outputs' pass, two blocks a CU, now 76): one block a CU with all of the next chunk ahead 98

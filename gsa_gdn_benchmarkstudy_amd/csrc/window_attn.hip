@@ -16,8 +16,8 @@
 //
 // Bound by issue: a wave's 32 queries and 32 keys take 16 MFMA (512 cycles), 16 exponentials and some 90 further VALU (about as
 // many cycles), which do not overlap within a SIMD; three waves a SIMD hide most of what else there is.  Forward, 16384
-// tokens, window 4096, 16 heads on 4, bf16: 482-500 us, 0.98 PFLOP/s in the pairs that are seen (a large library product: 1.33).
-// 4 x 4096 tokens, window 1024, with gradients: forward 155-167 us, dq 214-240, dk and dv 278-310, far queries 31-34 (134 MB of
+// tokens, window 4096, 16 heads on 4, bf16: 480-500 us, 0.98 PFLOP/s in the pairs that are seen (a large library product: 1.33).
+// 4 x 4096 tokens, window 1024, with gradients: forward 153-163 us, dq 227-236, dk and dv 265-285, far queries 29-31 (134 MB of
 // q and do read once more: 28), their join 10.
 // Measured and not taken: a swizzle under which transposed reads meet in no bank (conflicts a third of LDS's cycles now,
 // 0 then): 505 us for 494 forward, 687 for 668 with gradients, for what the addresses cost; tiles of 64 keys forward and two
