@@ -1,8 +1,9 @@
 """Attention in a sliding window, its cache and its single-token step on the GPU against the definition in 64 bits.
 
 Tolerances.  The oracle gives with each result the sum A of its terms' sizes.  A result of type t carries one rounding, at
-most eps(t) / 2 of its value.  In bf16 P enters the second product rounded (2^-8 of a term), the gradients' dS too, and D = do . o
-takes the rounded o (2^-8 of its terms): 2^-8 A for o and dv, 2^-7 A for dq and dk.  Scores are sums of 128 products in
+most eps(t) / 2 of its value.  In bf16 P enters the second product rounded (2^-8 of a term) and the gradients' dS too: 2^-8 A for o
+and dv, and 2^-7 A for dq and dk, which is enough for D = do . o from o rounded to bf16 as well (the kernels use o in two parts, and
+two parts of P and dS where few keys are visible: tests/test_gpu_window_precision.py holds them to that).  Scores are sums of 128 products in
 fp32: at most 32 + 6 roundings of 2^-24 of the sum of their terms' sizes (8 steps of 16 summed by the matrix cores, up to 6
 products each), which moves P by as much, numerator and denominator; so do the exponent's rounding, exp2 and the
 running sums: (2 * 40 * score + 128 + T / 8) roundings of A in all.
