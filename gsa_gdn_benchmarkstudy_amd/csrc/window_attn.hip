@@ -201,10 +201,10 @@ template <int NA, int NB> __device__ __forceinline__ void mma32(floatx16& acc, c
 // the same error over a whole row).  Windows with first tokens of at most so many have kernels of their own (kP = 2): the further products
 // cost little there.  us by one part / two: B = 4, T = 4096 with gradients, 68 keys 277 / 298, 128 310 / 338, 256 361 / 411, 512 467 / 563,
 // 1028 670 / 861; T = 16384 forward, 128 66 / 65, 256 82 / 82, 512 110 / 122, 4100 476 / 628.  Under longer windows the queries that see
-// few keys are the first ones of a sequence: their products take the lower part beforehand (few_visible, add_low).  Errors in the
-// norm, in roundings of the result: one part 1.41 (few keys: up to 1.5), two 1.00.
+// few keys are the first ones of a sequence: blocks of them, and tiles of them in dk and dv, go through a loop of two parts.  Errors in
+// the norm, in roundings of the result: one part 1.41 (few keys: up to 1.5), two 1.00.
 constexpr int kFine = 128;
-// All queries before i of a sequence do
+// All queries before i of a sequence see few keys, whatever the window
 __device__ __forceinline__ bool few_visible(int i, const Span& sp) { return min(i, sp.len) <= kFine; }
 // The schedule of a product of kMany instructions (bf16), each with an operand from LDS: kAhead reads on their way before each
 // (the compiler's own is one, and waits for it).
